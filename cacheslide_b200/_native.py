@@ -140,7 +140,27 @@ class QKVParams(ctypes.Structure):
     ]
 
 
+class RotaryParams(ctypes.Structure):
+    """cs_rotary_params: head norms and position rotation of queries and keys."""
+    _fields_ = [
+        ("cos", _p), ("sin", _p), ("table_rows", _i64), ("table_stride", _i64),
+        ("positions", _p), ("tokens", _i64),
+        ("head_dim", _i32), ("rot", _i32), ("interleaved", _i32), ("dtype", _i32),
+        ("weight_dtype", _i32), ("eps", _f64),
+        ("q", _p), ("q_stride_tok", _i64), ("q_stride_head", _i64), ("q_heads", _i32),
+        ("q_weight", _p), ("q_out", _p), ("qo_stride_tok", _i64), ("qo_stride_head", _i64),
+        ("k", _p), ("k_stride_tok", _i64), ("k_stride_head", _i64), ("k_heads", _i32),
+        ("k_weight", _p), ("k_out", _p), ("ko_stride_tok", _i64), ("ko_stride_head", _i64),
+        ("status", _p),
+    ]
+
+
 _SIGNATURES = {
+    "cs_qk_norm_rope": [ctypes.POINTER(RotaryParams), _p],
+    "cs_qk_norm_rope_grad_workspace": [ctypes.POINTER(RotaryParams)],
+    "cs_qk_norm_rope_grad": [ctypes.POINTER(RotaryParams), _p, _p, _p, _p, _p, _p],
+    "cs_kv_append_rotated": [ctypes.POINTER(RotaryParams), ctypes.POINTER(PagedKV), _p, _p, _i64,
+                             _i64, _p],
     "cs_slide_gather": [ctypes.POINTER(PagedKV), _p, _i64, _p, _p, _i64, _i64, _p, _p],
     "cs_slide_scatter": [ctypes.POINTER(PagedKV), _p, _p, _i64, _p, _p, _i64, _i64, _p, _p],
     "cs_slide_relocate": [ctypes.POINTER(PagedKV), _p, _p, _i64, _p, _p],
@@ -191,6 +211,7 @@ _SIGNATURES = {
 }
 _RESTYPES = {"cs_build_info": ctypes.c_char_p, "cs_abi_version": _i32,
              "cs_cope_attn_decode_workspace": _i64,
+             "cs_qk_norm_rope_grad_workspace": _i64,
              "cs_cope_attn_decode_batch_workspace": _i64}
 
 EXPORTED = tuple(_SIGNATURES)

@@ -1,0 +1,230 @@
+"""Rotary queries and keys over the paged pool.
+
+A rotary model (or the rotary layers of a mixed one) serves from the same
+paged pool as the contextual-position layers, with its keys rotated before
+they are stored:
+
+* ``rotary_tables``  -- float32 cosines and sines of every position;
+* ``qk_norm_rope``   -- RMS norm of each query / key head and the rotation in
+  one pass, differentiable in the queries, keys and both norm weights;
+* ``append_rotated`` -- the serving form: the new tokens' keys (normed and
+  rotated) and values go straight to their slots of the pool, and their
+  queries come back normed and rotated, in one launch.
+
+The reference has no rotary form (its layers count contextual positions,
+position.py:295-307); slots, records and the sidecar are those of
+``NativePagedKV`` (paged.py:205-240).  ``prefix.SharedPrefixAttention`` reads
+what ``append_rotated`` writes.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+from torch import Tensor
+
+from . import _native as N
+from .paged import NativePagedKV
+
+MAX_HEAD_DIM = 512
+_TYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def rotary_tables(positions: int, rotary_dim: int, *, base: float = 10000.0,
+                  device: torch.device | str = "cuda") -> tuple[Tensor, Tensor]:
+    """cos and sin, float32 ``[positions, rotary_dim / 2]``, of the angles
+    ``position * base^(-2 i / rotary_dim)`` (computed in float64)."""
+    if type(positions) is not int or positions < 1:
+        raise ValueError("positions must be a positive integer")
+    if type(rotary_dim) is not int or rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError("rotary_dim must be a positive even integer")
+    i = torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device)
+    angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] \
+        * float(base) ** (-i / rotary_dim)
+    return angle.cos().float(), angle.sin().float()
+
+
+def _rows(name: str, x: Tensor) -> Tensor:
+    if not isinstance(x, Tensor) or x.ndim != 3 or x.dtype not in _TYPES:
+        raise ValueError(f"{name} must be float32/float16/bfloat16 [token, head, dim]")
+    return x if x.stride(2) == 1 else x.contiguous()
+
+
+def _params(query: Tensor | None, key: Tensor, positions: Tensor, cos: Tensor, sin: Tensor,
+            q_weight: Tensor | None, k_weight: Tensor | None, eps: float,
+            interleaved: bool) -> N.RotaryParams:
+    """The checks every entry point shares; fills everything but the outputs."""
+    tokens, _, dim = key.shape
+    dtype, device = key.dtype, key.device
+    if query is not None and (query.shape[0] != tokens or query.shape[2] != dim
+                              or query.dtype != dtype):
+        raise ValueError("query and key must share tokens, head dim and dtype")
+    if dim % 2 or not 2 <= dim <= MAX_HEAD_DIM:
+        raise ValueError(f"head dim must be even and at most {MAX_HEAD_DIM}")
+    if (positions.ndim != 1 or positions.dtype != torch.int64 or positions.shape[0] != tokens
+            or positions.stride(0) != 1 and tokens > 1):
+        raise ValueError("positions must be a contiguous int64 [token] vector")
+    if (cos.ndim != 2 or cos.dtype != torch.float32 or sin.dtype != torch.float32
+            or cos.shape != sin.shape or cos.stride() != sin.stride() or cos.stride(1) != 1
+            and cos.shape[1] > 1):
+        raise ValueError("cos and sin must be float32 [position, rotary_dim / 2]")
+    rot = 2 * cos.shape[1]
+    if rot > dim:
+        raise ValueError("the rotated part is larger than the head")
+    if not eps >= 0.0:
+        raise ValueError("eps must be nonnegative")
+    weights = [w for w in (q_weight, k_weight) if w is not None]
+    for w in weights:
+        if w.shape != (dim,) or w.dtype not in _TYPES or w.dtype != weights[0].dtype \
+                or w.stride(0) != 1:
+            raise ValueError("norm weights must be contiguous floating [head dim] of one dtype")
+    for t in (query, positions, cos, sin, *weights):
+        if t is not None and t.device != device:
+            raise ValueError("all tensors must be on the same CUDA device")
+    if device.type != "cuda":
+        N.require_cuda(key)
+    p = N.RotaryParams()
+    p.cos, p.sin = cos.data_ptr(), sin.data_ptr()
+    p.table_rows, p.table_stride = cos.shape[0], cos.stride(0)
+    p.positions, p.tokens = positions.data_ptr(), tokens
+    p.head_dim, p.rot, p.interleaved = dim, rot, 1 if interleaved else 0
+    p.dtype = N.DTYPES[dtype]
+    p.eps = eps
+    if weights:
+        p.weight_dtype = N.DTYPES[weights[0].dtype]
+        p.q_weight, p.k_weight = N.ptr(q_weight), N.ptr(k_weight)
+    if query is not None:
+        p.q, p.q_heads = query.data_ptr(), query.shape[1]
+        p.q_stride_tok, p.q_stride_head = query.stride(0), query.stride(1)
+    p.k, p.k_heads = key.data_ptr(), key.shape[1]
+    p.k_stride_tok, p.k_stride_head = key.stride(0), key.stride(1)
+    return p
+
+
+def _outputs(p: N.RotaryParams, q_out: Tensor | None, k_out: Tensor | None) -> None:
+    if q_out is not None:
+        p.q_out, p.qo_stride_tok, p.qo_stride_head = (q_out.data_ptr(), q_out.stride(0),
+                                                      q_out.stride(1))
+    if k_out is not None:
+        p.k_out, p.ko_stride_tok, p.ko_stride_head = (k_out.data_ptr(), k_out.stride(0),
+                                                      k_out.stride(1))
+
+
+def _forward(query, key, positions, cos, sin, q_weight, k_weight, eps, interleaved, status):
+    p = _params(query, key, positions, cos, sin, q_weight, k_weight, eps, interleaved)
+    q_out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    k_out = torch.empty(key.shape, dtype=key.dtype, device=key.device)
+    _outputs(p, q_out, k_out)
+    p.status = None if status is None else status.ptr
+    N.check(N.load().cs_qk_norm_rope(ctypes.byref(p), N.stream_of(key.device)),
+            "cs_qk_norm_rope")
+    return q_out, k_out
+
+
+class _NormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, query, key, positions, cos, sin, q_weight, k_weight, eps, interleaved,
+                status):
+        ctx.save_for_backward(query, key, positions, cos, sin, q_weight, k_weight)
+        ctx.how = eps, interleaved, status
+        return _forward(query, key, positions, cos, sin, q_weight, k_weight, eps, interleaved,
+                        status)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, q_dy, k_dy):
+        query, key, positions, cos, sin, q_weight, k_weight = ctx.saved_tensors
+        eps, interleaved, status = ctx.how
+        p = _params(query, key, positions, cos, sin, q_weight, k_weight, eps, interleaved)
+        q_dy, k_dy = q_dy.contiguous(), k_dy.contiguous()
+        dq, dk = torch.empty_like(q_dy), torch.empty_like(k_dy)
+        _outputs(p, dq, dk)
+        p.status = None if status is None else status.ptr
+        dqw = None if q_weight is None else torch.empty_like(q_weight)
+        dkw = None if k_weight is None else torch.empty_like(k_weight)
+        lib = N.load()
+        size = lib.cs_qk_norm_rope_grad_workspace(ctypes.byref(p))
+        workspace = torch.empty(size, dtype=torch.uint8, device=key.device)
+        N.check(lib.cs_qk_norm_rope_grad(
+            ctypes.byref(p), q_dy.data_ptr(), k_dy.data_ptr(), N.ptr(dqw), N.ptr(dkw),
+            workspace.data_ptr(), N.stream_of(key.device)), "cs_qk_norm_rope_grad")
+        return dq, dk, None, None, None, dqw, dkw, None, None, None
+
+
+def qk_norm_rope(query: Tensor, key: Tensor, positions: Tensor, cos: Tensor, sin: Tensor,
+                 q_weight: Tensor | None = None, k_weight: Tensor | None = None, *,
+                 eps: float = 1e-6, interleaved: bool = False,
+                 status: N.Status | None = None) -> tuple[Tensor, Tensor]:
+    """RMS norm of each head (where its weight is given) and the position
+    rotation of queries ``[token, q_head, dim]`` and keys ``[token, kv_head,
+    dim]``, in float32 with one rounding to the input dtype.
+
+    ``cos`` / ``sin`` come from ``rotary_tables``; twice their width is the
+    rotated part of the head, the rest passes through.  ``interleaved`` pairs
+    elements (2i, 2i + 1) instead of (i, i + rotary_dim / 2).  Gradients flow
+    to query, key and the weights.  A position outside the tables makes its
+    rows NaN and sets ``ST_POS_RANGE`` in ``status`` (read it after the
+    stream has drained)."""
+    query, key = _rows("query", query), _rows("key", key)
+    if torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (query, key, q_weight, k_weight)):
+        return _NormRope.apply(query, key, positions, cos, sin, q_weight, k_weight, eps,
+                               interleaved, status)
+    return _forward(query, key, positions, cos, sin, q_weight, k_weight, eps, interleaved, status)
+
+
+def pool_view(kv: Tensor | NativePagedKV | N.PagedKV) -> N.PagedKV:
+    """The C-ABI view of a pool ``[blocks, kv_heads, block_size, 2 * dim]``, of
+    an arena (with its sidecar), or a view made before."""
+    if isinstance(kv, N.PagedKV):
+        return kv
+    if isinstance(kv, NativePagedKV):
+        return kv.device_view()
+    if not isinstance(kv, Tensor) or kv.device.type != "cuda":
+        raise ValueError("kv must be a CUDA pool tensor or a NativePagedKV")
+    return N.paged_view(kv)
+
+
+def append_rotated(kv: Tensor | NativePagedKV | N.PagedKV, slots: Tensor, key: Tensor,
+                   value: Tensor, positions: Tensor, cos: Tensor, sin: Tensor, *,
+                   query: Tensor | None = None, q_weight: Tensor | None = None,
+                   k_weight: Tensor | None = None, eps: float = 1e-6, interleaved: bool = False,
+                   out: Tensor | None = None, status: N.Status | None = None) -> Tensor | None:
+    """Write new tokens to the paged pool: the record of ``slots[t]`` (int64)
+    becomes the normed, rotated ``key[t]`` and ``value[t]``; with ``query``,
+    its normed, rotated rows are returned (into ``out`` when given, which may
+    be ``query`` itself).
+
+    Norms, rotation and tables as in ``qk_norm_rope``.  Slot -1 marks padding
+    and is not written; any other slot outside the pool (and sidecar), or a
+    position outside the tables, is skipped and sets ``ST_SLOT_RANGE`` /
+    ``ST_POS_RANGE`` in ``status``.  Distinct tokens need distinct slots.  The
+    slot map's guards are the caller's: this writes where it is told, as a
+    model runner's cache write does."""
+    key, value = _rows("key", key), _rows("value", value)
+    if value.shape != key.shape or value.dtype != key.dtype or value.device != key.device:
+        raise ValueError("key and value must share shape, dtype and device")
+    if query is not None:
+        query = _rows("query", query)
+    view = pool_view(kv)
+    p = _params(query, key, positions, cos, sin, q_weight, k_weight, eps, interleaved)
+    if view.dtype != p.dtype or view.kv_heads != p.k_heads or view.head_dim != p.head_dim:
+        raise ValueError("K/V must match the pool's dtype, KV heads and head dim")
+    if (slots.ndim != 1 or slots.dtype != torch.int64 or slots.shape[0] != key.shape[0]
+            or slots.device != key.device or slots.stride(0) != 1 and slots.shape[0] > 1):
+        raise ValueError("slots must be a contiguous int64 [token] vector")
+    if query is not None:
+        if out is None:
+            out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+        elif (out.shape != query.shape or out.dtype != query.dtype or out.device != query.device
+              or out.stride(2) != 1):
+            raise ValueError("out must match query, with a contiguous last dimension")
+        _outputs(p, out, None)
+    elif out is not None or q_weight is not None:
+        raise ValueError("out and q_weight need a query")
+    p.status = None if status is None else status.ptr
+    N.check(N.load().cs_kv_append_rotated(
+        ctypes.byref(p), ctypes.byref(view), slots.data_ptr(), value.data_ptr(), value.stride(0),
+        value.stride(1), N.stream_of(key.device)), "cs_kv_append_rotated")
+    return out

@@ -633,6 +633,71 @@ CS_API int cs_cope_validate_path(const void* positions, int64_t ps_h,
                                  int64_t nq, int64_t nk, double atol,
                                  int32_t dtype, int32_t* status, void* stream);
 
+/* --------------------------------------------- rotary keys and queries */
+/*
+ * RMS norm of each query / key head and the position rotation, one pass:
+ *   n = x * r,  r = (mean_i x_i^2 + eps)^-1/2        (only with a weight)
+ *   y = R(pos) (n * w)
+ * R(pos) turns pair p < rot/2 of the head by the angle whose cosine and sine
+ * are row `pos` of the float32 tables cos / sin [table_rows, rot/2]; the
+ * elements past rot pass through.  Pair p is (p, p + rot/2), or (2p, 2p + 1)
+ * when `interleaved`.  A position outside the table makes the row's rotated
+ * elements NaN and sets CS_ST_POS_RANGE.
+ */
+typedef struct {
+  const float* cos;
+  const float* sin;
+  int64_t table_rows, table_stride; /* stride in elements, both tables    */
+  const int64_t* positions;         /* [tokens]                           */
+  int64_t tokens;
+  int32_t head_dim, rot, interleaved;
+  int32_t dtype;        /* cs_dtype of q, k, their outputs and gradients  */
+  int32_t weight_dtype; /* cs_dtype of the weights                        */
+  double eps;
+  const void* q;        /* [tokens, q_heads, head_dim] (q_heads may be 0) */
+  int64_t q_stride_tok, q_stride_head;
+  int32_t q_heads;
+  const void* q_weight; /* [head_dim] or NULL: no norm                    */
+  void* q_out;
+  int64_t qo_stride_tok, qo_stride_head;
+  const void* k;
+  int64_t k_stride_tok, k_stride_head;
+  int32_t k_heads;
+  const void* k_weight;
+  void* k_out;
+  int64_t ko_stride_tok, ko_stride_head;
+  int32_t* status;
+} cs_rotary_params;
+
+CS_API int cs_qk_norm_rope(const cs_rotary_params* p, void* stream);
+
+/*
+ * Its gradient.  p->q / k are the forward's inputs, q_dy / k_dy the outputs'
+ * gradients (same strides as q_out / k_out in p), and p->q_out / k_out give
+ * the buffers of dx (their strides apply to dy and dx alike):
+ *   g = R(pos)^T dy,  dx = r (w g - n mean_i(w_i g_i n_i)),  dw = sum g n.
+ * dw (weight_dtype, [head_dim], NULL without a weight) is summed over a
+ * fixed partition of the rows in a fixed order: equal calls give equal bits.
+ * The workspace holds the partial sums; its size does not depend on tokens.
+ */
+CS_API int64_t cs_qk_norm_rope_grad_workspace(const cs_rotary_params* p);
+CS_API int cs_qk_norm_rope_grad(const cs_rotary_params* p, const void* q_dy,
+                                const void* k_dy, void* q_dw, void* k_dw,
+                                void* workspace, void* stream);
+
+/*
+ * Append to the paged pool: record of slots[t] = (R(pos) norm(k[t]), v[t]),
+ * with the queries of the same tokens normed and rotated into p->q_out in the
+ * same launch (q_heads = 0: none).  p->k_out is not used.  Slot -1 is padding
+ * (not written); any other slot outside the arena, or a position outside the
+ * table, is skipped and sets its status bit.  Of equal slots in one call any
+ * one row is kept.
+ */
+CS_API int cs_kv_append_rotated(const cs_rotary_params* p, const cs_paged_kv* kv,
+                                const int64_t* slots, const void* v,
+                                int64_t v_stride_tok, int64_t v_stride_head,
+                                void* stream);
+
 /* library identification: compile-time arch string and ABI version */
 CS_API const char* cs_build_info(void);
 CS_API int32_t cs_abi_version(void);

@@ -9,7 +9,10 @@ the CUDA library implements:
 * ``oracle.wca``   -- WCA deviation, adaptation weight, mean-head cosine and
   the stable top-budget selection (reference ``src/cacheslide_vllm/wca.py``);
 * ``oracle.slide`` -- paged KV slot addressing, gather and scatter
-  (reference ``src/cacheslide_vllm/paged.py``).
+  (reference ``src/cacheslide_vllm/paged.py``);
+* ``oracle.rotary`` -- head norms and position rotation with their gradient,
+  from the formulas (the reference has no rotary form; checked against
+  differences in ``tests/test_rotary.py``).
 
 Only ``tests/``, ``__graft_entry__.smoke()`` and the ``cpu_baseline`` /
 ``--impl reference`` legs of ``bench.py`` may import it, and only as the checker
