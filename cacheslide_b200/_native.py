@@ -155,7 +155,37 @@ class RotaryParams(ctypes.Structure):
     ]
 
 
+class PrefixShape(ctypes.Structure):
+    """cs_prefix_shape: the lengths of a batch behind shared prefixes."""
+    _fields_ = [
+        ("q_heads", _i32), ("kv_heads", _i32), ("head_dim", _i32), ("dtype", _i32),
+        ("groups", _i32), ("requests", _i32),
+        ("prefix_lens", _p), ("group_sizes", _p), ("query_lens", _p), ("suffix_lens", _p),
+    ]
+
+
+class PrefixPlanInfo(ctypes.Structure):
+    """cs_prefix_plan_info: where a plan's parts lie and what a call needs."""
+    _fields_ = [
+        ("words", _i64), ("workspace", _i64), ("tokens", _i64), ("n_prefix", _i64),
+        ("n_suffix", _i64), ("item_off", _i64), ("n_items", _i64), ("join_off", _i64),
+        ("n_join", _i64), ("list_off", _i64), ("part_tokens", _i64), ("variant", _i32),
+    ]
+
+
+class PrefixParams(ctypes.Structure):
+    """cs_prefix_params: one call of the attention behind shared prefixes."""
+    _fields_ = [
+        ("q", _p), ("q_stride_tok", _i64), ("q_stride_head", _i64), ("paged", PagedKV),
+        ("prefix_slots", _p), ("suffix_slots", _p), ("q_heads", _i32), ("scale", _f64),
+        ("out", _p), ("o_stride_tok", _i64), ("o_stride_head", _i64), ("lse", _p),
+        ("status", _p),
+    ]
+
+
 _SIGNATURES = {
+    "cs_prefix_plan": [ctypes.POINTER(PrefixShape), ctypes.POINTER(PrefixPlanInfo), _p, _i64],
+    "cs_prefix_attn": [ctypes.POINTER(PrefixParams), ctypes.POINTER(PrefixPlanInfo), _p, _p, _p],
     "cs_qk_norm_rope": [ctypes.POINTER(RotaryParams), _p],
     "cs_qk_norm_rope_grad_workspace": [ctypes.POINTER(RotaryParams)],
     "cs_qk_norm_rope_grad": [ctypes.POINTER(RotaryParams), _p, _p, _p, _p, _p, _p],

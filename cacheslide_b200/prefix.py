@@ -1,0 +1,139 @@
+"""Attention of a batch whose requests share a long prefix in the paged pool.
+
+Retrieval batches, chat tenants and several samples of one document keep the
+common part of their prompts in the pool once (shared blocks in their block
+tables).  Decoding, verifying drafted tokens or prefilling the questions then
+reads that part once for the whole batch, and each request's own keys once
+for that request: ``SharedPrefixAttention`` is the rotary layers' counterpart
+of the per-request attention of runtime.py:490-508 (causal softmax attention
+over ``NativePagedKV``'s records, paged.py:205-240).
+
+The batch's lengths become a plan once (``cs_prefix_plan``), reused by every
+layer of the step; each call is a launch or two on the current stream,
+without host synchronisation.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from collections.abc import Sequence
+
+import torch
+from torch import Tensor
+
+from . import _native as N
+from .paged import NativePagedKV
+from .rotary import pool_view
+
+_TYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _lens(name: str, values: Sequence[int]) -> tuple[ctypes.Array, int]:
+    values = list(values)
+    if any(type(v) is not int or not 0 <= v < 1 << 31 for v in values):
+        raise ValueError(f"{name} must be nonnegative integers below 2^31")
+    return (ctypes.c_int64 * max(1, len(values)))(*values), sum(values)
+
+
+class SharedPrefixAttention:
+    """The attention of one batch layout; call it once per layer.
+
+    ``query_lens[b]`` query tokens of request ``b`` are the newest of its
+    ``suffix_lens[b]`` own keys: query ``i`` of ``n`` sees its group's whole
+    prefix and own keys up to ``suffix_len - n + i`` (its own position).  A
+    request may have fewer own keys than queries (the first queries then see
+    only the prefix).  The requests form consecutive groups of
+    ``group_sizes``, group ``g`` sharing ``prefix_lens[g]`` keys; by default
+    one group holds them all."""
+
+    def __init__(self, q_heads: int, kv_heads: int, head_dim: int, dtype: torch.dtype,
+                 device: torch.device | str, *, query_lens: Sequence[int],
+                 suffix_lens: Sequence[int], prefix_lens: Sequence[int],
+                 group_sizes: Sequence[int] | None = None):
+        if dtype not in _TYPES:
+            raise ValueError("dtype must be float32, float16 or bfloat16")
+        if min(q_heads, kv_heads, head_dim) < 1 or q_heads % kv_heads:
+            raise ValueError("query heads must be a multiple of KV heads")
+        if group_sizes is None:
+            group_sizes = [len(query_lens)]
+        if len(query_lens) != len(suffix_lens) or len(prefix_lens) != len(group_sizes):
+            raise ValueError("one query and suffix length a request, one prefix length a group")
+        queries, self.tokens = _lens("query_lens", query_lens)
+        suffixes, self.suffix_keys = _lens("suffix_lens", suffix_lens)
+        prefixes, self.prefix_keys = _lens("prefix_lens", prefix_lens)
+        sizes, members = _lens("group_sizes", group_sizes)
+        if members != len(query_lens):
+            raise ValueError("group_sizes must add up to the requests")
+        self.q_heads, self.kv_heads, self.head_dim = q_heads, kv_heads, head_dim
+        self.dtype, self.device = dtype, torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        shape = N.PrefixShape(
+            q_heads, kv_heads, head_dim, N.DTYPES[dtype], len(prefix_lens), len(query_lens),
+            ctypes.addressof(prefixes), ctypes.addressof(sizes), ctypes.addressof(queries),
+            ctypes.addressof(suffixes))
+        self.info = N.PrefixPlanInfo()
+        lib = N.load()
+        capacity = 16 * self.tokens + 4096
+        while True:
+            words = torch.empty(capacity, dtype=torch.int32)
+            rc = lib.cs_prefix_plan(ctypes.byref(shape), ctypes.byref(self.info),
+                                    words.data_ptr(), capacity)
+            if rc != N.CS_ERR_TOO_LARGE or self.info.words <= capacity:
+                break
+            capacity = self.info.words
+        N.check(rc, "cs_prefix_plan")
+        self.words = words[:self.info.words].to(self.device)
+
+    def __call__(self, query: Tensor, kv: Tensor | NativePagedKV | N.PagedKV,
+                 prefix_slots: Tensor, suffix_slots: Tensor, *, scale: float | None = None,
+                 out: Tensor | None = None, return_lse: bool = False,
+                 status: N.Status | None = None) -> Tensor | tuple[Tensor, Tensor]:
+        """``query`` [token, q_head, dim] of all requests in order;
+        ``prefix_slots`` / ``suffix_slots`` (int64) the pool slots of the
+        groups' prefixes and the requests' own keys, concatenated.  ``scale``
+        defaults to ``dim ** -0.5``.  Returns [token, q_head, dim] (and, with
+        ``return_lse``, the float32 log of each row's softmax denominator,
+        -inf for a row that sees no key, whose output is zero).
+
+        A slot outside the pool reads as a zero key and value and sets
+        ``ST_SLOT_RANGE`` in ``status``."""
+        shape = (self.tokens, self.q_heads, self.head_dim)
+        if query.shape != shape or query.dtype != self.dtype or query.device != self.device:
+            raise ValueError(f"query must be {self.dtype} {shape} on {self.device}")
+        for name, slots, count in (("prefix_slots", prefix_slots, self.prefix_keys),
+                                   ("suffix_slots", suffix_slots, self.suffix_keys)):
+            if slots.shape != (count,) or slots.dtype != torch.int64 or \
+                    slots.device != self.device or slots.stride(0) != 1 and count > 1:
+                raise ValueError(f"{name} must be a contiguous int64 vector of {count} slots")
+        if query.stride(2) != 1:
+            query = query.contiguous()
+        view = pool_view(kv)
+        if view.dtype != N.DTYPES[self.dtype] or view.kv_heads != self.kv_heads \
+                or view.head_dim != self.head_dim:
+            raise ValueError("the pool's dtype, KV heads and head dim must be the plan's")
+        if scale is None:
+            scale = self.head_dim ** -0.5
+        elif not math.isfinite(scale):
+            raise ValueError("scale must be finite")
+        if out is None:
+            out = torch.empty(shape, dtype=self.dtype, device=self.device)
+        elif out.shape != shape or out.dtype != self.dtype or out.device != self.device \
+                or out.stride(2) != 1:
+            raise ValueError("out must match query, with a contiguous last dimension")
+        if self.device.type != "cuda":
+            N.require_cuda(query)
+        lse = torch.empty(shape[:2], dtype=torch.float32, device=self.device) \
+            if return_lse else None
+        p = N.PrefixParams(
+            query.data_ptr(), query.stride(0), query.stride(1), view, prefix_slots.data_ptr(),
+            suffix_slots.data_ptr(), self.q_heads, scale, out.data_ptr(), out.stride(0),
+            out.stride(1), N.ptr(lse), None if status is None else status.ptr)
+        workspace = None
+        if self.info.workspace:
+            workspace = torch.empty(self.info.workspace, dtype=torch.uint8, device=self.device)
+        N.check(N.load().cs_prefix_attn(
+            ctypes.byref(p), ctypes.byref(self.info), self.words.data_ptr(), N.ptr(workspace),
+            N.stream_of(self.device)), "cs_prefix_attn")
+        return (out, lse) if return_lse else out

@@ -698,6 +698,69 @@ CS_API int cs_kv_append_rotated(const cs_rotary_params* p, const cs_paged_kv* kv
                                 int64_t v_stride_tok, int64_t v_stride_head,
                                 void* stream);
 
+/* ----------------------------------- attention behind a shared prefix */
+/*
+ * A batch of requests in `groups` consecutive groups.  Group g's requests all
+ * see its prefix, prefix_lens[g] keys resident once in the paged pool; request
+ * b also sees its own keys, suffix_lens[b] of them, the newest query_lens[b]
+ * positions of which are its query tokens: query i of n sees the whole
+ * prefix and own keys 0 .. suffix_len - n + i.  Tokens, own keys and prefix
+ * keys are concatenated in request (group) order.
+ *
+ *   o = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q.k_j - max),
+ *   lse = max + log(sum_j p_j);  o = 0 and lse = -inf where nothing is seen.
+ *
+ * cs_prefix_plan lays the batch out as work for the kernels, once for all
+ * layers of a step.  It writes `info` and, when `capacity` holds it, the plan
+ * (int32 words, to be copied to the device); otherwise it returns
+ * CS_ERR_TOO_LARGE with info->words set.  Runs on the host only.
+ */
+typedef struct {
+  int32_t q_heads, kv_heads, head_dim, dtype;
+  int32_t groups, requests;
+  const int64_t* prefix_lens; /* [groups]                       */
+  const int64_t* group_sizes; /* [groups], summing to requests  */
+  const int64_t* query_lens;  /* [requests]                     */
+  const int64_t* suffix_lens; /* [requests]                     */
+} cs_prefix_shape;
+
+typedef struct {
+  int64_t words;          /* size of the plan                             */
+  int64_t workspace;      /* bytes of device workspace a call needs       */
+  int64_t tokens, n_prefix, n_suffix;
+  int64_t item_off, n_items;           /* work items, in plan words       */
+  int64_t join_off, n_join, list_off;  /* tokens joined from partials     */
+  int64_t part_tokens;
+  int32_t variant;        /* 0: CUDA cores; 1, 2: tensor cores, 128 or 256
+                             query rows a block                           */
+} cs_prefix_plan_info;
+
+CS_API int cs_prefix_plan(const cs_prefix_shape* shape, cs_prefix_plan_info* info,
+                          int32_t* words, int64_t capacity);
+
+typedef struct {
+  const void* q;  /* [tokens, q_heads, head_dim]                          */
+  int64_t q_stride_tok, q_stride_head;
+  cs_paged_kv paged;
+  const int64_t* prefix_slots; /* [n_prefix] of all groups                */
+  const int64_t* suffix_slots; /* [n_suffix] of all requests              */
+  int32_t q_heads;
+  double scale;
+  void* out;      /* [tokens, q_heads, head_dim], dtype of the pool       */
+  int64_t o_stride_tok, o_stride_head;
+  float* lse;     /* [tokens, q_heads] natural logarithm, or NULL         */
+  int32_t* status;
+} cs_prefix_params;
+
+/*
+ * The attention itself.  `plan` is the device copy of the plan's words and
+ * `workspace` holds info->workspace bytes that nothing else uses meanwhile
+ * (its content does not matter).  A slot outside the pool sets
+ * CS_ST_SLOT_RANGE and its key is read as zeros.
+ */
+CS_API int cs_prefix_attn(const cs_prefix_params* p, const cs_prefix_plan_info* info,
+                          const int32_t* plan, void* workspace, void* stream);
+
 /* library identification: compile-time arch string and ABI version */
 CS_API const char* cs_build_info(void);
 CS_API int32_t cs_abi_version(void);

@@ -12,7 +12,9 @@ the CUDA library implements:
   (reference ``src/cacheslide_vllm/paged.py``);
 * ``oracle.rotary`` -- head norms and position rotation with their gradient,
   from the formulas (the reference has no rotary form; checked against
-  differences in ``tests/test_rotary.py``).
+  differences in ``tests/test_rotary.py``);
+* ``oracle.prefix`` -- attention behind shared prefixes, request by request
+  in float64 torch.
 
 Only ``tests/``, ``__graft_entry__.smoke()`` and the ``cpu_baseline`` /
 ``--impl reference`` legs of ``bench.py`` may import it, and only as the checker
