@@ -41,6 +41,7 @@
 
 #include "common.cuh"
 #include "sm100.cuh"
+#include "tma_rows.cuh"
 
 namespace cs {
 
@@ -114,16 +115,6 @@ constexpr uint32_t kSmemBytes = kMeta + kMetaBytes;  // 230,768 B (limit 232,448
 // each tile; T = Q E lands in the first NP S columns of its tile at start
 constexpr uint32_t kColS = 0, kColO = 256;  // + 128 * tile
 // named barrier 1: the 128 producer threads
-// tile::gather4: rows r0..r3 of a 2-D tensor map, 64 elements from column x,
-// into 4 consecutive 128-byte rows at dst (the map's 128-byte swizzle applies)
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, int x, int r0,
-                                            int r1, int r2, int r3, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar)
-      : "memory");
-}
 // barrier that also ANDs a flag over its participants: every participant
 // leaves with the same answer, so exits from loops stay collective and no
 // partner is left waiting at a later barrier
@@ -147,19 +138,6 @@ __device__ __forceinline__ float floor_pos(float x, int& i) {
   return t - 12582912.0f;
 }
 
-template <typename T> struct Pack2;
-template <> struct Pack2<__nv_bfloat16> {
-  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
-    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<uint32_t*>(&v);
-  }
-};
-template <> struct Pack2<__half> {
-  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
-    __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<uint32_t*>(&v);
-  }
-};
 // packed pair -> (lo, hi)
 __device__ __forceinline__ float2 unpack2(uint32_t w, __nv_bfloat16) {
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
@@ -1552,43 +1530,6 @@ bool prefill_supported(const cs_attn_params* p) {
       return false;
   }
   return true;
-}
-
-// cuTensorMapEncodeTiled from the driver, resolved at first use through the
-// runtime (the library does not link libcuda, so it loads on hosts without a GPU)
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiledFn encode_tiled() {
-  static const EncodeTiledFn fn = [] {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) !=
-            cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      return static_cast<EncodeTiledFn>(nullptr);
-    return reinterpret_cast<EncodeTiledFn>(f);
-  }();
-  return fn;
-}
-
-// 2-D row map over `rows` rows of `inner` 16-bit elements, `unit` bytes apart,
-// read in 64 x box_rows boxes with the 128-byte swizzle of the UMMA operand tiles
-bool encode_rows(CUtensorMap* m, const void* base, bool bf16, int64_t inner, int64_t rows,
-                 int64_t unit, uint32_t box_rows) {
-  if (base == nullptr || reinterpret_cast<uintptr_t>(base) % 16 || unit % 16 ||
-      unit < inner * 2 || rows < 1 || rows > INT32_MAX || inner < 128)
-    return false;
-  const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)unit};
-  const cuuint32_t box[2] = {64, box_rows}, es[2] = {1, 1};
-  const EncodeTiledFn encode = encode_tiled();
-  if (encode == nullptr) return false;
-  return encode(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-                const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // Row structure of the K/V storage for the TMA path: every row the kernel

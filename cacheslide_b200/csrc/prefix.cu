@@ -1,13 +1,13 @@
 // Attention of a batch behind shared prefixes (cs_prefix_plan,
 // cs_prefix_attn): the host's plan of the batch and the CUDA-core kernel.
-//
-// Plan, int32 words:
-//   tokens   [tokens][4]  prefix keys [p0, p1) and own keys [lo, hi) that the
-//                         token sees, as places in the two slot arrays
+#include <algorithm>
+#include <cmath>
 #include <cstring>
+#include <new>
 #include <type_traits>
+#include <vector>
 
-#include "common.cuh"
+#include "prefix.cuh"
 
 namespace cs {
 namespace {
@@ -115,16 +115,152 @@ __global__ void __launch_bounds__(kRowWarps * 32) prefix_rows_kernel(RowArgs a) 
 }  // namespace
 }  // namespace cs
 
-extern "C" int cs_prefix_plan(const cs_prefix_shape* s, cs_prefix_plan_info* info, int32_t* words,
-                              int64_t capacity) {
-  using namespace cs;
-  CS_HOST_CHECK(s != nullptr && info != nullptr && capacity >= 0);
-  CS_HOST_CHECK(s->q_heads > 0 && s->kv_heads > 0 && s->q_heads % s->kv_heads == 0);
-  CS_HOST_CHECK(s->head_dim > 0 && s->groups >= 0 && s->requests >= 0);
-  CS_HOST_CHECK(s->groups == 0 || (s->prefix_lens && s->group_sizes));
-  CS_HOST_CHECK(s->requests == 0 || (s->query_lens && s->suffix_lens));
-  if (s->dtype != CS_F32 && s->dtype != CS_F16 && s->dtype != CS_BF16) return CS_ERR_UNSUPPORTED;
-  if (s->head_dim > kMaxDim) return CS_ERR_UNSUPPORTED;
+namespace cs {
+namespace {
+
+// A unit of work before it is cut: tokens x prefix keys, then own keys.
+struct Unit {
+  int64_t tok0, ntok, a0, a1, b0, b1;
+  int64_t steps() const { return tiles(a1 - a0) + tiles(b1 - b0); }
+  static int64_t tiles(int64_t n) { return (n + kPrefixTile - 1) / kPrefixTile; }
+};
+
+struct Layout {
+  const int32_t* tok;  // the plan's token rows
+  int64_t tokens;
+  int group;           // query heads a KV head
+  int kv_heads, q_heads, head_dim;
+  std::vector<int64_t> group_tok;   // first token of each group, and the end
+  std::vector<int64_t> req_tok;     // first token of each request, and the end
+  int64_t lo(int64_t t) const { return tok[4 * t + 2]; }
+  int64_t hi(int64_t t) const { return tok[4 * t + 3]; }
+};
+
+// Row tiles of `rows` query rows with all their keys: the prefix, then every
+// own key that one of the tile's tokens sees.
+std::vector<Unit> whole_units(const Layout& l, int rows) {
+  std::vector<Unit> out;
+  const int64_t per = (int64_t)(kPrefixTile / l.group) * (rows / kPrefixTile);
+  for (size_t g = 0; g + 1 < l.group_tok.size(); ++g)
+    for (int64_t t = l.group_tok[g]; t < l.group_tok[g + 1]; t += per) {
+      const int64_t n = std::min(per, l.group_tok[g + 1] - t);
+      out.push_back({t, n, l.tok[4 * t], l.tok[4 * t + 1], l.lo(t), l.hi(t + n - 1)});
+    }
+  return out;
+}
+
+// The prefix apart from the own keys: row tiles over the prefix alone, and
+// runs of whole requests (at most a row tile of tokens, about `keys` keys)
+// over their own keys, so that few rows meet keys that they do not see.
+std::vector<Unit> split_units(const Layout& l, int64_t keys) {
+  std::vector<Unit> out;
+  const int64_t per = kPrefixTile / l.group;
+  for (size_t g = 0; g + 1 < l.group_tok.size(); ++g)
+    for (int64_t t = l.group_tok[g]; t < l.group_tok[g + 1]; t += per)
+      out.push_back({t, std::min(per, l.group_tok[g + 1] - t), l.tok[4 * t], l.tok[4 * t + 1], 0,
+                     0});
+  int64_t first = 0, count = 0, b0 = 0, b1 = 0;
+  auto flush = [&] {
+    if (count > 0) out.push_back({first, count, 0, 0, b0, b1});
+    count = 0;
+  };
+  for (size_t r = 0; r + 1 < l.req_tok.size(); ++r) {
+    const int64_t t0 = l.req_tok[r], n = l.req_tok[r + 1] - t0;
+    if (n == 0 || l.hi(t0 + n - 1) == l.lo(t0)) continue;  // no query, or no own key seen
+    if (n > per) {
+      flush();
+      for (int64_t t = t0; t < t0 + n; t += per) {
+        const int64_t m = std::min(per, t0 + n - t);
+        out.push_back({t, m, 0, 0, l.lo(t), l.hi(t + m - 1)});
+      }
+      continue;
+    }
+    const int64_t k0 = l.lo(t0), k1 = l.hi(t0 + n - 1);
+    if (count > 0 && (t0 + n - first > per || k1 - b0 > keys)) flush();
+    if (count == 0) {
+      first = t0;
+      b0 = k0;
+    }
+    count = t0 + n - first;
+    b1 = k1;
+  }
+  flush();
+  return out;
+}
+
+// Every unit cut into equal runs of at most `most` key tiles, of a part's
+// tokens only those that see its keys.
+std::vector<PrefixItem> cut(const Layout& l, const std::vector<Unit>& units, int64_t most) {
+  std::vector<PrefixItem> out;
+  for (const Unit& u : units) {
+    const int64_t steps = u.steps(), na = Unit::tiles(u.a1 - u.a0);
+    if (steps == 0) continue;
+    const int64_t parts = (steps + most - 1) / most;
+    for (int64_t p = 0; p < parts; ++p) {
+      const int64_t s0 = steps * p / parts, s1 = steps * (p + 1) / parts;
+      Unit v = u;
+      v.a0 = std::min(u.a1, u.a0 + std::min(s0, na) * kPrefixTile);
+      v.a1 = std::min(u.a1, u.a0 + std::min(s1, na) * kPrefixTile);
+      v.b0 = std::min(u.b1, u.b0 + std::max<int64_t>(s0 - na, 0) * kPrefixTile);
+      v.b1 = std::min(u.b1, u.b0 + std::max<int64_t>(s1 - na, 0) * kPrefixTile);
+      if (v.a0 == v.a1) {
+        while (v.ntok > 0 && l.hi(v.tok0) <= v.b0) ++v.tok0, --v.ntok;
+        while (v.ntok > 0 && l.lo(v.tok0 + v.ntok - 1) >= v.b1) --v.ntok;
+        if (v.ntok == 0) continue;
+      }
+      out.push_back({(int32_t)v.tok0, (int32_t)v.ntok, (int32_t)v.a0, (int32_t)v.a1,
+                     (int32_t)v.b0, (int32_t)v.b1, -1, 0});
+    }
+  }
+  return out;
+}
+
+int64_t item_steps(const PrefixItem& i) {
+  return Unit::tiles(i.a1 - i.a0) + Unit::tiles(i.b1 - i.b0);
+}
+
+// Estimated time of a launch, in key tiles of one 128-row block: blocks are
+// dealt out in order over `slots`, each costs its tiles and `fixed` more, and
+// a partial result costs its way to memory and back.
+double estimate(const Layout& l, const std::vector<PrefixItem>& items, int slots, double step,
+                double fixed) {
+  double sum = 0, longest = 0, parts = 0;
+  for (const PrefixItem& i : items) {
+    const double c = item_steps(i) * step + fixed;
+    sum += c;
+    longest = std::max(longest, c);
+    parts += i.ntok;
+  }
+  const double blocks = (double)items.size() * l.kv_heads;
+  // full waves of equal blocks, or the dealt sum plus half a block's tail
+  const double mean = items.empty() ? 0 : sum / items.size();
+  const double waves = std::max(longest, std::min(std::ceil(blocks / slots) * mean,
+                                                  sum * l.kv_heads / slots + 0.5 * longest));
+  return waves + parts * l.q_heads * l.head_dim * 8.0 / 6.0e6;
+}
+
+// The cut of least estimated time: candidates are numbers of key tiles a part.
+template <typename Make>
+double best_cut(const Layout& l, int slots, double step, double fixed, Make units_for,
+                std::vector<PrefixItem>& best) {
+  double least = -1;
+  int64_t longest = 1;
+  for (int64_t most = 1; most <= 2 * longest; most += most < 16 ? 1 : most / 8) {
+    const std::vector<Unit> units = units_for(most);
+    for (const Unit& u : units) longest = std::max(longest, u.steps());
+    std::vector<PrefixItem> items = cut(l, units, most);
+    if ((int64_t)items.size() * l.kv_heads > (int64_t)slots * 16 && most < longest) continue;
+    const double e = estimate(l, items, slots, step, fixed);
+    if (least < 0 || e < least) {
+      least = e;
+      best = std::move(items);
+    }
+  }
+  return least;
+}
+
+int make_plan(const cs_prefix_shape* s, cs_prefix_plan_info* info, int32_t* words,
+              int64_t capacity) {
   int64_t tokens = 0, n_suffix = 0, n_prefix = 0, members = 0;
   for (int b = 0; b < s->requests; ++b) {
     CS_HOST_CHECK(s->query_lens[b] >= 0 && s->suffix_lens[b] >= 0);
@@ -136,18 +272,20 @@ extern "C" int cs_prefix_plan(const cs_prefix_shape* s, cs_prefix_plan_info* inf
     CS_HOST_CHECK(s->group_sizes[g] >= 0 && s->prefix_lens[g] >= 0);
     members += s->group_sizes[g];
     n_prefix += s->prefix_lens[g];
-    if (n_prefix > INT32_MAX / 2 || members > s->requests) break;
+    if (n_prefix > INT32_MAX / 2) return CS_ERR_UNSUPPORTED;
+    CS_HOST_CHECK(members <= s->requests);
   }
-  if (n_prefix > INT32_MAX / 2) return CS_ERR_UNSUPPORTED;
   CS_HOST_CHECK(members == s->requests);
   std::memset(info, 0, sizeof(*info));
   info->tokens = tokens;
   info->n_prefix = n_prefix;
   info->n_suffix = n_suffix;
-  info->words = tokens * 4;
-  if (words == nullptr || capacity < info->words) return CS_ERR_TOO_LARGE;
-  int32_t* w = words;
-  int64_t b = 0, p0 = 0, k0 = 0;
+
+  std::vector<int32_t> rows(tokens * 4);
+  Layout l{rows.data(), tokens, s->q_heads / s->kv_heads, s->kv_heads, s->q_heads, s->head_dim,
+           {0}, {0}};
+  int32_t* w = rows.data();
+  int64_t b = 0, p0 = 0, k0 = 0, t = 0;
   for (int g = 0; g < s->groups; ++g) {
     for (int64_t m = 0; m < s->group_sizes[g]; ++m, ++b) {
       const int64_t n = s->query_lens[b], keys = s->suffix_lens[b];
@@ -159,10 +297,98 @@ extern "C" int cs_prefix_plan(const cs_prefix_shape* s, cs_prefix_plan_info* inf
         w[3] = (int32_t)(k0 + (seen > 0 ? seen : 0));
       }
       k0 += keys;
+      t += n;
+      l.req_tok.push_back(t);
     }
     p0 += s->prefix_lens[g];
+    l.group_tok.push_back(t);
   }
+
+  std::vector<PrefixItem> items;
+  std::vector<int32_t> join, list;
+  const bool tc = (s->dtype == CS_F16 || s->dtype == CS_BF16) &&
+                  (s->head_dim == 64 || s->head_dim == 128) && l.group <= kPrefixTile;
+  if (tc && tokens > 0) {
+    info->variant = 1;
+    const int sms = num_sms();
+    // two 128-row blocks an SM, or one 256-row block whose step takes as long
+    // as two of theirs but reads its keys once for all its rows
+    const double e1 = best_cut(l, 2 * sms, 1.0, 2.5,
+                               [&](int64_t most) { return split_units(l, most * kPrefixTile); },
+                               items);
+    std::vector<PrefixItem> wide;
+    const double e2 = best_cut(l, sms, 0.9, 4.0,
+                               [&](int64_t) { return whole_units(l, 2 * kPrefixTile); }, wide);
+    if (e2 >= 0 && (e1 < 0 || e2 < e1)) {
+      info->variant = 2;
+      items = std::move(wide);
+    }
+    std::stable_sort(items.begin(), items.end(), [](const PrefixItem& x, const PrefixItem& y) {
+      return item_steps(x) > item_steps(y);
+    });
+    // a token in one item alone gets its output from it, if that holds for
+    // all of the item's tokens; the others are joined from partials
+    std::vector<int32_t> in(tokens + 1, 0);
+    for (const PrefixItem& i : items)
+      for (int32_t k = 0; k < i.ntok; ++k) ++in[i.tok0 + k];
+    std::vector<char> alone(items.size(), 1);
+    std::vector<int32_t> parts(tokens + 1, 0);
+    for (size_t x = 0; x < items.size(); ++x) {
+      PrefixItem& i = items[x];
+      for (int32_t k = 0; k < i.ntok; ++k)
+        if (in[i.tok0 + k] != 1) alone[x] = 0;
+      if (alone[x]) continue;
+      if (info->part_tokens > INT32_MAX / 2) return CS_ERR_UNSUPPORTED;
+      i.part = (int32_t)info->part_tokens;
+      info->part_tokens += i.ntok;
+      for (int32_t k = 0; k < i.ntok; ++k) ++parts[i.tok0 + k];
+    }
+    std::vector<int32_t> at(tokens + 1, 0);
+    int32_t entries = 0;
+    for (int64_t x = 0; x < tokens; ++x) {
+      at[x] = entries;
+      if (parts[x] == 0 && in[x] != 0) continue;  // written by its item
+      join.insert(join.end(), {(int32_t)x, entries, parts[x], 0});
+      entries += parts[x];
+    }
+    list.resize(entries);
+    for (const PrefixItem& i : items)
+      for (int32_t k = 0; i.part >= 0 && k < i.ntok; ++k) list[at[i.tok0 + k]++] = i.part + k;
+  }
+  const int64_t iw = (int64_t)items.size() * (sizeof(PrefixItem) / 4);
+  info->n_items = (int64_t)items.size();
+  info->n_join = (int64_t)join.size() / 4;
+  info->item_off = tokens * 4;
+  info->join_off = info->item_off + iw;
+  info->list_off = info->join_off + (int64_t)join.size();
+  info->words = info->list_off + (int64_t)list.size();
+  info->workspace = info->part_tokens * s->q_heads * (s->head_dim + 1) * (int64_t)sizeof(float);
+  if (words == nullptr || capacity < info->words) return CS_ERR_TOO_LARGE;
+  std::copy(rows.begin(), rows.end(), words);
+  if (iw) std::memcpy(words + info->item_off, items.data(), iw * 4);
+  std::copy(join.begin(), join.end(), words + info->join_off);
+  std::copy(list.begin(), list.end(), words + info->list_off);
   return CS_OK;
+}
+
+}  // namespace
+}  // namespace cs
+
+extern "C" int cs_prefix_plan(const cs_prefix_shape* s, cs_prefix_plan_info* info, int32_t* words,
+                              int64_t capacity) {
+  using namespace cs;
+  CS_HOST_CHECK(s != nullptr && info != nullptr && capacity >= 0);
+  CS_HOST_CHECK(s->q_heads > 0 && s->kv_heads > 0 && s->q_heads % s->kv_heads == 0);
+  CS_HOST_CHECK(s->head_dim > 0 && s->groups >= 0 && s->requests >= 0);
+  CS_HOST_CHECK(s->groups == 0 || (s->prefix_lens && s->group_sizes));
+  CS_HOST_CHECK(s->requests == 0 || (s->query_lens && s->suffix_lens));
+  if (s->dtype != CS_F32 && s->dtype != CS_F16 && s->dtype != CS_BF16) return CS_ERR_UNSUPPORTED;
+  if (s->head_dim > kMaxDim) return CS_ERR_UNSUPPORTED;
+  try {
+    return make_plan(s, info, words, capacity);
+  } catch (const std::bad_alloc&) {
+    return CS_ERR_UNSUPPORTED;
+  }
 }
 
 extern "C" int cs_prefix_attn(const cs_prefix_params* p, const cs_prefix_plan_info* info,
@@ -178,14 +404,18 @@ extern "C" int cs_prefix_attn(const cs_prefix_params* p, const cs_prefix_plan_in
   CS_HOST_CHECK(p->q && p->out && plan && (info->workspace == 0 || workspace));
   CS_HOST_CHECK((info->n_prefix == 0 || p->prefix_slots) &&
                 (info->n_suffix == 0 || p->suffix_slots));
+  if (info->variant > 0) {
+    const int rc = prefix_attn_sm100(*p, *info, plan, workspace, as_stream(stream));
+    if (rc != CS_ERR_UNSUPPORTED) return rc;
+  }
   const int64_t es = dtype_size(kv.dtype);
   RowArgs a{static_cast<const char*>(p->q), p->q_stride_tok * es, p->q_stride_head * es,
             PagedView::make(kv), p->prefix_slots, p->suffix_slots,
             reinterpret_cast<const int4*>(plan), p->q_heads, (int)(p->q_heads / kv.kv_heads),
             (int)kv.head_dim, (float)p->scale, static_cast<char*>(p->out), p->o_stride_tok * es,
             p->o_stride_head * es, p->lse, p->status};
-  const unsigned blocks = (unsigned)(info->tokens * p->q_heads);
   if (info->tokens * p->q_heads > INT32_MAX) return CS_ERR_UNSUPPORTED;
+  const unsigned blocks = (unsigned)(info->tokens * p->q_heads);
   if (kv.dtype == CS_F32)
     prefix_rows_kernel<float><<<blocks, kRowWarps * 32, 0, as_stream(stream)>>>(a);
   else if (kv.dtype == CS_F16)

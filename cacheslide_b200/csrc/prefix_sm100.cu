@@ -1,0 +1,735 @@
+// Tensor-core attention behind shared prefixes for sm_100a (tcgen05, TMEM,
+// TMA), and the join of its partial results.
+//
+// One block takes one work item of the plan for one KV head: up to NT tiles
+// of 128 query rows (128 / G tokens x the G query heads of the KV head) and
+// the item's keys, first its range of the prefix, then its range of the own
+// keys, in tiles of 128.  Per tile
+//   S = Q K^T (tcgen05, TMEM),  P = 2^(S c - m),  O += P V (P from TMEM)
+// with the running maximum m and sum of each row in registers.  Every row
+// sees the whole prefix range; of the own keys it sees [lo, hi) of its token,
+// which covers the causal limit, requests of other lengths in the same tile
+// and padding alike.
+//
+// Warps: 4 NT softmax (one thread a row), a K and a V producer, NT MMA
+// issuers.  Keys come through the slot arrays: TMA boxes of 64 x 16 for runs
+// of 16 keys in consecutive rows of the pool, tile::gather4 for 4 keys of one
+// map, 16-byte cp.async for the rest (range ends, which are filled with
+// zeros, and pools no tensor map describes).
+//
+// Bound: HBM for decodes (each record once a row tile), the tensor and
+// exponential units for question prefills.
+#include <cuda.h>
+#include <math.h>
+
+#include <numeric>
+#include <type_traits>
+
+#include "prefix.cuh"
+#include "sm100.cuh"
+#include "tma_rows.cuh"
+
+namespace cs {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct PArgs {
+  // [0] pool with 64 x 1 boxes (gather4), [1] with 64 x 16; [2], [3] sidecar
+  // K and [4], [5] sidecar V alike
+  CUtensorMap tm[6];
+  PagedView pv;
+  const char* q;
+  int64_t qt, qh;  // byte strides
+  char* out;
+  int64_t ot, oh;
+  float* lse;
+  const int64_t* prefix_slots;
+  const int64_t* suffix_slots;
+  const int4* tokens;
+  const PrefixItem* items;
+  float* part_o;    // [part token][query head][dim], normalised
+  float* part_lse;  // [part token][query head], log2 of the softmax denominator
+  int32_t* status;
+  int64_t nrb, nrh, nro, srr, srh;  // slot -> map row
+  int hq, hkv, G, R;  // R: tokens a row tile
+  int bs_shift;       // log2(block size), -1 when it is no power of two
+  int tma;            // 1: tensor maps describe the pool
+  int vec_q, vec_out; // 16-byte loads / stores fit
+  int neg;            // the scale is negative: the queries are negated
+  float scale2;       // |scale| * log2 e
+  float scale_signed2;
+};
+
+template <typename T> constexpr int umma_format() { return std::is_same<T, __half>::value ? 0 : 1; }
+// P is stored as 2^(x - m + kUp): fp16's normal numbers then reach 2^-21 of the
+// row's largest weight, and 2^(kUp + kLazy) stays below its maximum
+template <typename T> constexpr float p_up() { return std::is_same<T, __half>::value ? 7.f : 0.f; }
+constexpr float kLazy = 8.f;  // O is rescaled when the maximum grew by more than 2^8
+
+template <int D, int NT>
+struct Shape {
+  // key tiles in flight: two where they fit beside the queries
+  static constexpr int KS = (D == 64 || NT == 2) ? 2 : 1;
+  static constexpr int VS = KS;
+  static constexpr int kSoft = 4 * NT;
+  static constexpr int kThreads = 32 * (kSoft + 2 + NT);
+  static constexpr uint32_t TB = kPrefixTile * D * 2;
+  static constexpr uint32_t oQ = 0, oK = NT * TB, oV = oK + KS * TB, oMeta = oV + VS * TB;
+  // barriers, 8 bytes each
+  static constexpr uint32_t bQ = 0, bK = 8, bV = bK + 8 * KS, bS = bV + 8 * VS,
+                            bP = bS + 8 * NT * KS, bPV = bP + 8 * NT, bEnd = bPV + 8 * NT * VS,
+                            oTmem = bEnd + 8, oAbort = oTmem + 4, oBad = oAbort + 4,
+                            kMeta = oBad + 2 * NT * 16;
+  static constexpr uint32_t kSmem = oMeta + kMeta + 1024;  // the base is rounded up to 1024
+  static constexpr uint32_t kCols = 256 * NT;
+  static constexpr uint32_t cS = 0, cO = 128 * NT;  // S of tile i at 128 i, O at cO + D i
+};
+
+struct Step {
+  int base, n, own;  // first key, keys, 1: own keys
+};
+__device__ __forceinline__ Step step_of(const PrefixItem& it, int na, int t) {
+  Step s;
+  s.own = t >= na;
+  s.base = s.own ? it.b0 + (t - na) * kPrefixTile : it.a0 + t * kPrefixTile;
+  const int end = s.own ? it.b1 : it.a1;
+  s.n = end - s.base < kPrefixTile ? end - s.base : kPrefixTile;
+  return s;
+}
+
+// bits lo .. hi - 1 of the 32 columns from col0 on
+__device__ __forceinline__ uint32_t col_bits(int lo, int hi, int col0) {
+  lo = lo - col0 < 0 ? 0 : lo - col0;
+  hi = hi - col0 > 32 ? 32 : hi - col0;
+  if (hi <= lo) return 0u;
+  const uint32_t up = hi == 32 ? ~0u : (1u << hi) - 1u;
+  return up & ~((1u << lo) - 1u);
+}
+
+__device__ __forceinline__ void mbar_arrive_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void st_shared16(uint32_t dst, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z),
+               "r"(v.w)
+               : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t src) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(src)
+               : "memory");
+  return v;
+}
+
+// where the keys of one lane (4 consecutive keys of a tile) come from
+struct Src {
+  int row[4];     // row of the tensor map
+  int kind[4];    // 0: none (beyond the range, or no valid slot), 1: pool, 2: sidecar
+  int64_t slot[4];
+};
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
+    prefix_sm100_kernel(const __grid_constant__ PArgs a) {
+  using Sh = Shape<D, NT>;
+  extern __shared__ char smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t sbase = (raw + 1023u) & ~1023u;
+  char* smem = smem_raw + (sbase - raw);
+  const uint32_t mb = sbase + Sh::oMeta;
+  volatile int* abort = reinterpret_cast<volatile int*>(smem + Sh::oMeta + Sh::oAbort);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = blockIdx.x % a.hkv;
+  const PrefixItem it = a.items[blockIdx.x / a.hkv];
+  const int na = (it.a1 - it.a0 + kPrefixTile - 1) / kPrefixTile;
+  const int steps = na + (it.b1 - it.b0 + kPrefixTile - 1) / kPrefixTile;
+  const int tiles = NT == 2 && it.ntok > a.R ? 2 : 1;
+
+  if (tid == 0) {
+    mbar_init(mb + Sh::bQ, 128 * tiles);
+    for (int s = 0; s < Sh::KS; ++s) mbar_init(mb + Sh::bK + 8 * s, 32);
+    for (int s = 0; s < Sh::VS; ++s) mbar_init(mb + Sh::bV + 8 * s, 32);
+    for (int s = 0; s < NT * Sh::KS; ++s) mbar_init(mb + Sh::bS + 8 * s, 1);
+    for (int s = 0; s < NT; ++s) mbar_init(mb + Sh::bP + 8 * s, 128);
+    for (int s = 0; s < NT * Sh::VS; ++s) mbar_init(mb + Sh::bPV + 8 * s, 1);
+    *abort = 0;
+    mbar_init_fence();
+  }
+  if (warp == Sh::kSoft + 2) tmem_alloc(mb + Sh::oTmem, Sh::kCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + Sh::oMeta + Sh::oTmem);
+  auto barS = [&](int qt, int t) { return mb + Sh::bS + 8 * (qt * Sh::KS + t % Sh::KS); };
+  auto barPV = [&](int qt, int t) { return mb + Sh::bPV + 8 * (qt * Sh::VS + t % Sh::VS); };
+
+  if (warp == Sh::kSoft || warp == Sh::kSoft + 1) {
+    // ============================================== producers: K, then V warp
+    const bool isv = warp != Sh::kSoft;
+    const int ST = isv ? Sh::VS : Sh::KS;
+    bool slot_bad = false;
+    auto load_src = [&](int t, Src& s) {
+      const Step st = step_of(it, na, t);
+      const int64_t* slots = (st.own ? a.suffix_slots : a.prefix_slots) + st.base;
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        const int j = 4 * lane + m;
+        s.slot[m] = j < st.n ? slots[j] : -1;
+        s.kind[m] = 0;
+        s.row[m] = 0;
+        if (j < st.n) {
+          if (!a.pv.valid(s.slot[m])) {
+            slot_bad = true;
+            s.slot[m] = -1;
+          } else if (s.slot[m] < a.pv.native_total) {
+            int64_t b, o;
+            if (a.bs_shift >= 0) {
+              b = s.slot[m] >> a.bs_shift;
+              o = s.slot[m] - (b << a.bs_shift);
+            } else {
+              b = s.slot[m] / a.pv.bs;
+              o = s.slot[m] - b * a.pv.bs;
+            }
+            s.kind[m] = 1;
+            s.row[m] = (int)(b * a.nrb + g * a.nrh + o * a.nro);
+          } else {
+            s.kind[m] = 2;
+            s.row[m] = (int)((s.slot[m] - a.pv.native_total) * a.srr + g * a.srh);
+          }
+        }
+      }
+    };
+    Src cur, nxt;
+    if (steps > 0) load_src(0, cur);
+    int issued = 0;
+    for (int t = 0; t < steps; ++t) {
+      // the stage is free once every tile's product of its last use is done
+      if (t >= ST) {
+        bool ok = true;
+        for (int qt = 0; qt < tiles; ++qt)
+          ok = ok && mbar_wait(isv ? barPV(qt, t) : barS(qt, t), (t / ST - 1) & 1, abort);
+        if (!__all_sync(~0u, ok)) break;
+      }
+      const uint32_t bar = mb + (isv ? Sh::bV : Sh::bK) + 8 * (t % ST);
+      const uint32_t dst = sbase + (isv ? Sh::oV : Sh::oK) + (t % ST) * Sh::TB;
+      // 16 keys (4 lanes) in consecutive rows of one map; else 4 keys of one map
+      const int k0 = cur.kind[0];
+      const bool four = a.tma && k0 != 0 && cur.kind[1] == k0 && cur.kind[2] == k0 &&
+                        cur.kind[3] == k0;
+      const int r16 = __shfl_sync(~0u, cur.row[0], lane & ~3);
+      const int k16 = __shfl_sync(~0u, k0, lane & ~3);
+      const bool seq = four && k0 == k16 && cur.row[0] == r16 + 4 * (lane & 3) &&
+                       cur.row[1] == cur.row[0] + 1 && cur.row[2] == cur.row[0] + 2 &&
+                       cur.row[3] == cur.row[0] + 3;
+      const uint32_t sq = __ballot_sync(~0u, seq);
+      const bool run = ((sq >> (lane & ~3)) & 0xFu) == 0xFu;
+      const int x0 = isv && k0 == 1 ? D : 0;
+      const int map0 = k0 == 2 ? (isv ? 4 : 2) : 0;
+      if (run || four) {
+        const bool lead = run && (lane & 3) == 0;
+        mbar_arrive_tx(bar, run ? (lead ? 16 * D * 2 : 0) : 4 * D * 2);
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          const uint32_t to = dst + c * 16384 + 4 * lane * 128;
+          if (lead) tma_tile2d(to, &a.tm[map0 + 1], x0 + 64 * c, cur.row[0], bar);
+          else if (!run)
+            tma_gather4(to, &a.tm[map0], x0 + 64 * c, cur.row[0], cur.row[1], cur.row[2],
+                        cur.row[3], bar);
+        }
+      } else {
+        // rows one by one; a place without a key is zeroed (its value must be
+        // finite: its weight is zero)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const int j = 4 * lane + m;
+          const bool ok = cur.slot[m] >= 0;
+          const char* src =
+              ok ? a.pv.addr(cur.slot[m], g, isv ? D : 0) : a.pv.cache;
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c)
+            cp_async16(dst + sw128(j, c, kPrefixTile), ok ? src + 16 * c : src, ok);
+        }
+        cp_async_wait_all();
+        fence_async_smem();
+        mbar_arrive(bar);
+      }
+      issued = t + 1;
+      if (t + 1 < steps) {
+        load_src(t + 1, nxt);
+        cur = nxt;
+      }
+    }
+    // nothing of this block's copies is in flight when it ends
+    for (int t = issued - ST < 0 ? 0 : issued - ST; t < issued; ++t) {
+      const uint32_t bar = mb + (isv ? Sh::bV : Sh::bK) + 8 * (t % ST);
+      const long long t0 = clock64();
+      while (!mbar_try(bar, (t / ST) & 1) && clock64() - t0 < kWaitCycles) {
+      }
+    }
+    if (slot_bad) report(a.status, CS_ST_SLOT_RANGE);
+
+  } else if (warp >= Sh::kSoft + 2) {
+    // ==================================================== MMA, one warp a tile
+    const int qt = warp - (Sh::kSoft + 2);
+    if (lane == 0 && qt < tiles) {
+      const uint32_t id_s = umma_idesc(128, 128, umma_format<T>(), 0, 0);
+      const uint32_t id_o = umma_idesc(128, D, umma_format<T>(), 0, 1);  // V is MN-major
+      const uint32_t qa = sbase + Sh::oQ + qt * Sh::TB;
+      const uint32_t sc = tmem + Sh::cS + 128 * qt, oc = tmem + Sh::cO + D * qt;
+      bool ok = mbar_wait(mb + Sh::bQ, 0, abort);
+      uint32_t last = 0, lastph = 0;  // the newest group issued
+      for (int t = 0; ok && t < steps; ++t) {
+        const uint32_t kb = sbase + Sh::oK + (t % Sh::KS) * Sh::TB;
+        const uint32_t vb = sbase + Sh::oV + (t % Sh::VS) * Sh::TB;
+        if (!(ok = mbar_wait(mb + Sh::bK + 8 * (t % Sh::KS), (t / Sh::KS) & 1, abort))) break;
+        // S takes the columns that P of the last step lies in
+        if (t > 0 && !(ok = mbar_wait(barPV(qt, t - 1), ((t - 1) / Sh::VS) & 1, abort))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
+          tc_mma(sc, umma_desc(qa + off, 16, 1024), umma_desc(kb + off, 16, 1024), id_s,
+                 kk ? 1u : 0u);
+        }
+        last = barS(qt, t);
+        lastph = (t / Sh::KS) & 1;
+        tc_commit(last);
+        if (!(ok = mbar_wait(mb + Sh::bP + 8 * qt, t & 1, abort))) break;
+        if (!(ok = mbar_wait(mb + Sh::bV + 8 * (t % Sh::VS), (t / Sh::VS) & 1, abort))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < kPrefixTile / 16; ++kk)
+          tc_mma_ts(oc, sc + kk * 8, umma_desc(vb + kk * 2048, 16384, 1024), id_o,
+                    (t | kk) ? 1u : 0u);
+        last = barPV(qt, t);
+        lastph = (t / Sh::VS) & 1;
+        tc_commit(last);
+      }
+      if (last) {
+        const long long t0 = clock64();
+        while (!mbar_try(last, lastph) && clock64() - t0 < kWaitCycles) {
+        }
+      }
+    }
+    __syncwarp();
+
+  } else if ((warp >> 2) < tiles) {
+    // ================================================== softmax, a thread a row
+    const int qt = warp >> 2;
+    const int r = (warp & 3) * 32 + lane;  // TMEM lane
+    const int tok = qt * a.R + r / a.G, h = g * a.G + r % a.G;
+    const bool row_ok = r < a.R * a.G && tok < it.ntok;
+    {
+      // queries into the swizzled operand layout, 16 bytes a step
+      constexpr int C = D / 8;
+      for (int i = tid & 127; i < kPrefixTile * C; i += 128) {
+        const int row = i / C, c = i % C;
+        const int tk = qt * a.R + row / a.G;
+        if (row < a.R * a.G && tk < it.ntok) {
+          const char* src = a.q + (int64_t)(it.tok0 + tk) * a.qt +
+                            (int64_t)(g * a.G + row % a.G) * a.qh + 16 * c;
+          uint4 v;
+          if (a.vec_q) {
+            v = *reinterpret_cast<const uint4*>(src);
+          } else {
+            const uint16_t* s = reinterpret_cast<const uint16_t*>(src);
+            v.x = s[0] | (uint32_t)s[1] << 16;
+            v.y = s[2] | (uint32_t)s[3] << 16;
+            v.z = s[4] | (uint32_t)s[5] << 16;
+            v.w = s[6] | (uint32_t)s[7] << 16;
+          }
+          if (a.neg) v = make_uint4(v.x ^ 0x80008000u, v.y ^ 0x80008000u, v.z ^ 0x80008000u,
+                                    v.w ^ 0x80008000u);
+          st_shared16(sbase + Sh::oQ + qt * Sh::TB + sw128(row, c, kPrefixTile), v);
+        }
+      }
+      fence_async_smem();
+      mbar_arrive(mb + Sh::bQ);
+    }
+    const int4 tk = row_ok ? a.tokens[it.tok0 + tok] : make_int4(0, 0, 0, 0);
+    const int first_hi = a.tokens[it.tok0].w, last_lo = a.tokens[it.tok0 + it.ntok - 1].z;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t sc = tmem + lane_base + Sh::cS + 128 * qt;
+    const uint32_t oc = tmem + lane_base + Sh::cO + D * qt;
+    float mref = -INFINITY, lsum = 0.f;  // log2 domain; P = 2^(x - mref + up)
+    bool ok = true;
+    int checked = 0;
+    auto wait_pv = [&](int t) {
+      ok = __all_sync(~0u, mbar_wait(barPV(qt, t), (t / Sh::VS) & 1, abort));
+      tc_fence_after();
+      return ok;
+    };
+
+    for (int t = 0; t < steps; ++t) {
+      const Step st = step_of(it, na, t);
+      int vlo = 0, vhi = 0;
+      if (row_ok) {
+        vlo = st.own ? (tk.z > st.base ? tk.z - st.base : 0) : 0;
+        vhi = st.own ? (tk.w - st.base < st.n ? tk.w - st.base : st.n) : st.n;
+      }
+      // Some row of the block may not see some key: a value that is not
+      // finite there would reach it as 0 x inf.  Such keys (bits of bad) leave
+      // the product and are added to the rows that see them below.
+      uint32_t bad[4] = {0u, 0u, 0u, 0u};
+      if (st.own && (last_lo > st.base || first_hi < st.base + st.n)) {
+        ok = ok && __all_sync(~0u, mbar_wait(mb + Sh::bV + 8 * (t % Sh::VS), (t / Sh::VS) & 1,
+                                             abort));
+        constexpr int C = D / 8;
+        const int c0 = tiles == 2 ? qt * (C / 2) : 0, c1 = tiles == 2 ? c0 + C / 2 : C;
+        const uint32_t vrow = sbase + Sh::oV + (t % Sh::VS) * Sh::TB;
+        bool nf = false;
+        if (ok) {
+          for (int c = c0; c < c1; ++c) {
+            const uint4 v = ld_shared16(vrow + sw128(r, c, kPrefixTile));
+            const uint32_t e = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+            auto all_ones = [&](uint32_t w) {
+              const uint32_t x = w & e;
+              return (x & 0xffffu) == (e & 0xffffu) || (x >> 16) == (e >> 16);
+            };
+            nf |= all_ones(v.x) || all_ones(v.y) || all_ones(v.z) || all_ones(v.w);
+          }
+        }
+        const uint32_t word = __ballot_sync(~0u, nf);
+        volatile uint32_t* slot = reinterpret_cast<volatile uint32_t*>(
+            smem + Sh::oMeta + Sh::oBad + (checked & 1) * (16 * NT));
+        ++checked;
+        if (lane == 0) slot[warp] = word;
+        asm volatile("bar.sync 1, %0;" ::"r"(128 * tiles) : "memory");
+#pragma unroll
+        for (int w = 0; w < 4; ++w) bad[w] = slot[w] | (tiles == 2 ? slot[(w + 4) % (4 * NT)] : 0u);
+        if (ok && (bad[0] | bad[1] | bad[2] | bad[3])) {
+          if ((bad[r >> 5] >> (r & 31)) & 1u) {
+            for (int c = c0; c < c1; ++c)
+              st_shared16(vrow + sw128(r, c, kPrefixTile), make_uint4(0u, 0u, 0u, 0u));
+          }
+          fence_async_smem();
+        }
+        // the other tile's product must not start on half a cleared row
+        if (tiles == 2 && (bad[0] | bad[1] | bad[2] | bad[3]))
+          asm volatile("bar.sync 1, 256;" ::: "memory");
+      }
+      if (!ok) continue;  // a wait expired: only the barriers above are kept
+      ok = __all_sync(~0u, mbar_wait(barS(qt, t), (t / Sh::KS) & 1, abort));
+      if (!ok) continue;
+      tc_fence_after();
+      uint32_t v[32];
+      if (__all_sync(~0u, vhi <= vlo)) {  // nothing to see for these 32 rows
+#pragma unroll
+        for (int c = 0; c < 16; ++c) v[c] = 0u;
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc) CS_TMEM_ST16(sc + 16 * cc, v);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(mb + Sh::bP + 8 * qt);
+        continue;
+      }
+      float top = -INFINITY;
+#pragma unroll 1
+      for (int cc = 0; cc < 4; ++cc) {
+        const uint32_t bits = col_bits(vlo, vhi, 32 * cc);
+        if (__all_sync(~0u, bits == 0u)) continue;
+        CS_TMEM_LD32(sc + 32 * cc, v);
+        tmem_wait_ld();
+        if (__all_sync(~0u, bits == ~0u)) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) top = fmaxf(top, __uint_as_float(v[c]));
+        } else {
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            top = fmaxf(top, (bits >> c) & 1u ? __uint_as_float(v[c]) : -INFINITY);
+        }
+      }
+      const float top2 = top == -INFINITY ? -INFINITY : top * a.scale2;
+      const bool grow = top2 > mref + kLazy || mref == -INFINITY;
+      const bool rescale = grow && mref > -INFINITY && top2 > mref;
+      if (__any_sync(~0u, rescale)) {  // t > 0: a row has a finite maximum
+        if (!wait_pv(t - 1)) continue;
+        const float f = rescale ? ex2(mref - top2) : 1.f;
+        lsum *= f;
+#pragma unroll 1
+        for (int cc = 0; cc < D / 32; ++cc) {
+          CS_TMEM_LD32(oc + 32 * cc, v);
+          tmem_wait_ld();
+#pragma unroll
+          for (int c = 0; c < 32; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * f);
+          CS_TMEM_ST32(oc + 32 * cc, v);
+        }
+        tmem_wait_st();
+      }
+      if (grow) mref = top2;
+      // the largest weight so far is 2^up, or up to 2^kLazy more
+      const float sub = (mref > -INFINITY ? mref : 0.f) - p_up<T>();
+      float s0 = 0.f, s1 = 0.f;
+#pragma unroll 1
+      for (int cc = 0; cc < 4; ++cc) {
+        const uint32_t bits = col_bits(vlo, vhi, 32 * cc);
+        if (__all_sync(~0u, bits == 0u)) {
+#pragma unroll
+          for (int c = 0; c < 16; ++c) v[c] = 0u;
+        } else {
+          CS_TMEM_LD32(sc + 32 * cc, v);
+          tmem_wait_ld();
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            v[c] = __float_as_uint(ex2(fmaf(__uint_as_float(v[c]), a.scale2, -sub)));
+          if (!__all_sync(~0u, bits == ~0u)) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) v[c] = (bits >> c) & 1u ? v[c] : 0u;
+          }
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            const float e0 = __uint_as_float(v[2 * c]), e1 = __uint_as_float(v[2 * c + 1]);
+            s0 += e0;
+            s1 += e1;
+            v[c] = Pack2<T>::pack(e0, e1);
+          }
+        }
+        CS_TMEM_ST16(sc + 16 * cc, v);
+      }
+      lsum += s0 + s1;
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(mb + Sh::bP + 8 * qt);
+
+      if (bad[0] | bad[1] | bad[2] | bad[3]) {
+        if (!wait_pv(t)) continue;
+        const int64_t* slots = a.suffix_slots + st.base;
+        for (int j = 0; j < st.n; ++j) {
+          if (!((bad[j >> 5] >> (j & 31)) & 1u)) continue;
+          const bool see = j >= vlo && j < vhi;
+          const T* rec = reinterpret_cast<const T*>(a.pv.addr(slots[j], g, 0));
+          const T* val = reinterpret_cast<const T*>(a.pv.addr(slots[j], g, D));
+          float dot = 0.f;
+          if (see) {
+            const T* q = reinterpret_cast<const T*>(a.q + (int64_t)(it.tok0 + tok) * a.qt +
+                                                    (int64_t)h * a.qh);
+            for (int e = 0; e < D; ++e) dot += Elem<T>::to_f(q[e]) * Elem<T>::to_f(rec[e]);
+          }
+          const float p = ex2(fmaf(dot, a.scale_signed2, -sub));
+#pragma unroll 1
+          for (int cc = 0; cc < D / 32; ++cc) {
+            CS_TMEM_LD32(oc + 32 * cc, v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (see)
+                v[c] = __float_as_uint(fmaf(p, Elem<T>::to_f(val[32 * cc + c]),
+                                            __uint_as_float(v[c])));
+            CS_TMEM_ST32(oc + 32 * cc, v);
+            tmem_wait_st();
+          }
+        }
+        tc_fence_before();
+      }
+    }
+
+    // ---------------------------------------------------------------- output
+    if (ok && steps > 0) wait_pv(steps - 1);
+    const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+    const float lse2 = lsum == 0.f ? -INFINITY
+                                   : (mref > -INFINITY ? mref : 0.f) - p_up<T>() + log2f(lsum);
+    const int64_t token = it.tok0 + tok;
+    const int64_t prow = ((int64_t)it.part + tok) * a.hq + h;
+    char* orow = a.out + token * a.ot + (int64_t)h * a.oh;
+#pragma unroll 1
+    for (int cc = 0; cc < D / 32; ++cc) {
+      uint32_t v[32];
+      if (ok && steps > 0) {
+        CS_TMEM_LD32(oc + 32 * cc, v);
+        tmem_wait_ld();
+      }
+#pragma unroll
+      for (int c = 0; c < 32; ++c)
+        v[c] = ok && steps > 0 && lsum != 0.f ? __float_as_uint(__uint_as_float(v[c]) * inv) : 0u;
+      if (!row_ok || !ok) continue;
+      if (it.part >= 0) {
+        float4* dst = reinterpret_cast<float4*>(a.part_o + prow * D + 32 * cc);
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          dst[c] = make_float4(__uint_as_float(v[4 * c]), __uint_as_float(v[4 * c + 1]),
+                               __uint_as_float(v[4 * c + 2]), __uint_as_float(v[4 * c + 3]));
+      } else if (a.vec_out) {
+        uint4* dst = reinterpret_cast<uint4*>(orow + 64 * cc);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t w[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            w[u] = Pack2<T>::pack(__uint_as_float(v[8 * c + 2 * u]),
+                                  __uint_as_float(v[8 * c + 2 * u + 1]));
+          dst[c] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 32; ++c)
+          reinterpret_cast<T*>(orow)[32 * cc + c] = Elem<T>::from_f(__uint_as_float(v[c]));
+      }
+    }
+    if (row_ok && ok) {
+      if (it.part >= 0) a.part_lse[prow] = lse2;
+      else if (a.lse) a.lse[token * a.hq + h] = lse2 * kLn2;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && *abort) report(a.status, CS_ST_TIMEOUT);
+  if (warp == Sh::kSoft + 2) {
+    tc_fence_after();
+    tmem_dealloc(tmem, Sh::kCols);
+  }
+}
+
+// One warp per (join token, head): o = sum_c w_c o_c / sum_c w_c with
+// w_c = 2^(lse_c - max), the partials in the plan's order.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) prefix_join_kernel(const PArgs a, const int4* join,
+                                                          const int32_t* list, int n) {
+  constexpr int E = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int64_t w = blockIdx.x * 4ll + (threadIdx.x >> 5);
+  if (w >= (int64_t)n * a.hq) return;
+  const int4 j = join[w / a.hq];
+  const int h = (int)(w % a.hq);
+  float top = -INFINITY;
+  for (int c = lane; c < j.z; c += 32)
+    top = fmaxf(top, a.part_lse[(int64_t)list[j.y + c] * a.hq + h]);
+  top = warp_max(top);
+  float o[E], sum = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+  for (int c = 0; c < j.z; ++c) {
+    const int64_t row = (int64_t)list[j.y + c] * a.hq + h;
+    const float l = a.part_lse[row];
+    if (l == -INFINITY) continue;
+    const float f = ex2(l - top);  // NaN stays NaN
+    sum += f;
+    const float* src = a.part_o + row * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = fmaf(f, src[e], o[e]);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  T* out = reinterpret_cast<T*>(a.out + (int64_t)j.x * a.ot + (int64_t)h * a.oh) + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; ++e) out[e] = Elem<T>::from_f(o[e] * inv);
+  if (a.lse && lane == 0)
+    a.lse[(int64_t)j.x * a.hq + h] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+}
+
+bool setup_maps(PArgs& a, const cs_paged_kv& kv) {
+  const PagedView& pv = a.pv;
+  const bool bf16 = kv.dtype == CS_BF16;
+  const int64_t D = pv.head_dim;
+  if (pv.sb < 0 || pv.sh < 0 || pv.so < 0) return false;
+  const int64_t unit = std::gcd(std::gcd(pv.sb, pv.sh), pv.so);
+  if (unit <= 0) return false;
+  const int64_t rows = ((kv.num_blocks - 1) * pv.sb + (pv.kv_heads - 1) * pv.sh +
+                        (pv.bs - 1) * pv.so) / unit + 1;
+  if (!encode_rows(&a.tm[0], pv.cache, bf16, 2 * D, rows, unit, 1) ||
+      !encode_rows(&a.tm[1], pv.cache, bf16, 2 * D, rows, unit, 16))
+    return false;
+  a.nrb = pv.sb / unit;
+  a.nrh = pv.sh / unit;
+  a.nro = pv.so / unit;
+  if (pv.side_capacity > 0) {
+    if (pv.ssr < 0 || pv.ssh < 0) return false;
+    const int64_t su = std::gcd(pv.ssr, pv.ssh);
+    if (su <= 0) return false;
+    const int64_t sr = ((pv.side_capacity - 1) * pv.ssr + (pv.kv_heads - 1) * pv.ssh) / su + 1;
+    if (!encode_rows(&a.tm[2], pv.side_k, bf16, D, sr, su, 1) ||
+        !encode_rows(&a.tm[3], pv.side_k, bf16, D, sr, su, 16) ||
+        !encode_rows(&a.tm[4], pv.side_v, bf16, D, sr, su, 1) ||
+        !encode_rows(&a.tm[5], pv.side_v, bf16, D, sr, su, 16))
+      return false;
+    a.srr = pv.ssr / su;
+    a.srh = pv.ssh / su;
+  } else {  // never addressed: no slot reaches the sidecar
+    a.tm[2] = a.tm[4] = a.tm[0];
+    a.tm[3] = a.tm[5] = a.tm[1];
+  }
+  return true;
+}
+
+template <typename T, int D, int NT>
+int launch_main(const PArgs& a, int64_t blocks, cudaStream_t stream) {
+  auto kernel = prefix_sm100_kernel<T, D, NT>;
+  static const cudaError_t set = cudaFuncSetAttribute(
+      kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D, NT>::kSmem);
+  if (set != cudaSuccess) return CS_ERR_CUDA;
+  kernel<<<(unsigned)blocks, Shape<D, NT>::kThreads, Shape<D, NT>::kSmem, stream>>>(a);
+  CS_LAUNCH_CHECK();
+  return CS_OK;
+}
+
+template <typename T, int D>
+int launch_all(const PArgs& a, const cs_prefix_plan_info& info, const int32_t* plan,
+               cudaStream_t stream) {
+  if (info.n_items > 0) {
+    const int64_t blocks = info.n_items * a.hkv;
+    const int rc = info.variant == 2 ? launch_main<T, D, 2>(a, blocks, stream)
+                                     : launch_main<T, D, 1>(a, blocks, stream);
+    if (rc != CS_OK) return rc;
+  }
+  if (info.n_join > 0) {
+    const unsigned blocks = (unsigned)((info.n_join * a.hq + 3) / 4);
+    prefix_join_kernel<T, D><<<blocks, 128, 0, stream>>>(
+        a, reinterpret_cast<const int4*>(plan + info.join_off), plan + info.list_off,
+        (int)info.n_join);
+    CS_LAUNCH_CHECK();
+  }
+  return CS_OK;
+}
+
+}  // namespace
+
+int prefix_attn_sm100(const cs_prefix_params& p, const cs_prefix_plan_info& info,
+                      const int32_t* plan, void* workspace, cudaStream_t stream) {
+  const cs_paged_kv& kv = p.paged;
+  PArgs a;
+  a.pv = PagedView::make(kv);
+  if (!a.pv.vec16()) return CS_ERR_UNSUPPORTED;
+  a.q = static_cast<const char*>(p.q);
+  a.qt = p.q_stride_tok * 2;
+  a.qh = p.q_stride_head * 2;
+  a.out = static_cast<char*>(p.out);
+  a.ot = p.o_stride_tok * 2;
+  a.oh = p.o_stride_head * 2;
+  auto al = [](const void* x, int64_t t, int64_t h) {
+    return reinterpret_cast<uintptr_t>(x) % 16 == 0 && t % 16 == 0 && h % 16 == 0;
+  };
+  a.vec_q = al(p.q, a.qt, a.qh);
+  a.vec_out = al(p.out, a.ot, a.oh);
+  a.lse = p.lse;
+  a.prefix_slots = p.prefix_slots;
+  a.suffix_slots = p.suffix_slots;
+  a.tokens = reinterpret_cast<const int4*>(plan);
+  a.items = reinterpret_cast<const PrefixItem*>(plan + info.item_off);
+  a.part_o = static_cast<float*>(workspace);
+  a.part_lse = a.part_o + info.part_tokens * p.q_heads * kv.head_dim;
+  a.status = p.status;
+  a.hq = p.q_heads;
+  a.hkv = (int)kv.kv_heads;
+  a.G = a.hq / a.hkv;
+  a.R = kPrefixTile / a.G;
+  a.bs_shift = -1;
+  for (int s = 0; s < 31; ++s)
+    if ((int64_t)1 << s == kv.block_size) a.bs_shift = s;
+  a.neg = p.scale < 0.0;
+  a.scale2 = fabsf((float)p.scale) * kLog2e;
+  a.scale_signed2 = (float)p.scale * kLog2e;
+  a.nrb = a.nrh = a.nro = a.srr = a.srh = 0;
+  a.tma = setup_maps(a, kv) ? 1 : 0;
+  const bool half = kv.dtype == CS_F16;
+  if (kv.head_dim == 128)
+    return half ? launch_all<__half, 128>(a, info, plan, stream)
+                : launch_all<__nv_bfloat16, 128>(a, info, plan, stream);
+  return half ? launch_all<__half, 64>(a, info, plan, stream)
+              : launch_all<__nv_bfloat16, 64>(a, info, plan, stream);
+}
+
+}  // namespace cs
