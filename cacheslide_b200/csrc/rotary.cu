@@ -124,7 +124,8 @@ __device__ __forceinline__ void norm_turn_row(const RotArgs& a, const T* x, At a
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kRowWarps * 32) norm_rope_rows_kernel(RotArgs a) {
+__global__ void __launch_bounds__(kRowWarps * 32)
+    norm_rope_rows_kernel(const __grid_constant__ RotArgs a) {
   const int lane = threadIdx.x & 31;
   const int heads = a.q.heads + a.k.heads;
   const int64_t total = a.tokens * heads;
@@ -275,78 +276,70 @@ __global__ void __launch_bounds__(kRowWarps * 32)
 }
 
 // ------------------------------------------------------------ vector kernels
-// LPR lanes own a row, each two 16-byte vectors of it (P pairs of elements):
+// LPR lanes own a row, each 4 pairs of it as two vectors of 4 elements:
 // half-split pairs take one vector of either half, interleaved pairs lie
-// inside the vectors.  A warp takes 32 / LPR rows at once and U such groups
-// back to back, all loads before the first arithmetic, so that a thread has
-// 2 U vectors in flight; rows are flattened over (token, head).
-template <typename T> constexpr int kVecPairs = 16 / (int)sizeof(T);
+// inside the vectors.  A warp takes a task: up to kGroups groups of 32 / LPR
+// heads of one token and one kind (q, k or v), whose angles and weights it
+// loads once, all rows' loads before the first arithmetic.  Vectors of 4
+// keep a lane's share small (8 elements of a row): with 8 pairs a lane the
+// kernels held 98 (forward) and 118 (gradient) registers, a quarter of the
+// SM's warps, and 2.9 TB/s.
+constexpr int kP = 4;        // pairs a lane
+constexpr int kGroups = 4;   // row groups a task
+constexpr int kVecWarps = 4;
+
+template <typename T> struct Vec4 { using type = uint2; };
+template <> struct Vec4<float> { using type = uint4; };
 
 template <typename T>
-__device__ __forceinline__ void unpack(const uint4& v, float* f) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (std::is_same<T, float>::value) {
-      f[i] = __uint_as_float(w[i]);
-    } else if constexpr (std::is_same<T, __half>::value) {
-      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      f[2 * i] = x.x;
-      f[2 * i + 1] = x.y;
-    } else {
-      f[2 * i] = __uint_as_float(w[i] << 16);
-      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
+__device__ __forceinline__ void unpack(const typename Vec4<T>::type& v, float* f) {
+  if constexpr (std::is_same<T, float>::value) {
+    f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y);
+    f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
+  } else if constexpr (std::is_same<T, __half>::value) {
+    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&v.x));
+    const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+    f[0] = x.x, f[1] = x.y, f[2] = y.x, f[3] = y.y;
+  } else {
+    f[0] = __uint_as_float(v.x << 16), f[1] = __uint_as_float(v.x & 0xffff0000u);
+    f[2] = __uint_as_float(v.y << 16), f[3] = __uint_as_float(v.y & 0xffff0000u);
   }
 }
 template <typename T>
-__device__ __forceinline__ uint4 pack(const float* f) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (std::is_same<T, float>::value) w[i] = __float_as_uint(f[i]);
-    else w[i] = Pack2<T>::pack(f[2 * i], f[2 * i + 1]);
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+__device__ __forceinline__ typename Vec4<T>::type pack(const float* f) {
+  if constexpr (std::is_same<T, float>::value)
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                      __float_as_uint(f[3]));
+  else
+    return make_uint2(Pack2<T>::pack(f[0], f[1]), Pack2<T>::pack(f[2], f[3]));
 }
 
-// the P weights at element e of a head (16-byte aligned), as float32
-template <typename T, int P>
+// 4 weights from element e of a head on, as float32
 __device__ __forceinline__ void weights_at(const void* w, int dtype, int e, float* f) {
   if (dtype == CS_F32) {
-#pragma unroll
-    for (int i = 0; i < P / 4; ++i)
-      unpack<float>(__ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(w) + e) + i),
-                    f + 4 * i);
-  } else if constexpr (P == 8) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(w) + e));
-    if (dtype == CS_F16) unpack<__half>(v, f);
-    else unpack<__nv_bfloat16>(v, f);
+    unpack<float>(__ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(w) + e)), f);
   } else {
     const uint2 v = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(w) + e));
-    float g[8];
-    if (dtype == CS_F16) unpack<__half>(make_uint4(v.x, v.y, 0u, 0u), g);
-    else unpack<__nv_bfloat16>(make_uint4(v.x, v.y, 0u, 0u), g);
-#pragma unroll
-    for (int i = 0; i < P; ++i) f[i] = g[i];
+    if (dtype == CS_F16) unpack<__half>(v, f);
+    else unpack<__nv_bfloat16>(v, f);
   }
 }
 
-// which elements a lane owns: vectors at e0 and e1; pairs p0 .. p0 + P - 1
-// when they turn
+// which elements a lane owns: vectors at e0 and e1; pairs p0 .. p0 + 3 when
+// they turn
 struct Lane {
   int p0, e0, e1;
   bool turns;
 };
-template <int P>
+template <bool INTER>
 __device__ __forceinline__ Lane lane_of(const RotArgs& a, int l) {
   Lane n;
-  n.p0 = l * P;
+  n.p0 = l * kP;
   const int half = a.rot >> 1;
   n.turns = n.p0 < half;
   if (n.turns) {
-    n.e0 = a.interleaved ? 2 * n.p0 : n.p0;
-    n.e1 = a.interleaved ? n.e0 + P : n.p0 + half;
+    n.e0 = INTER ? 2 * n.p0 : n.p0;
+    n.e1 = INTER ? n.e0 + kP : n.p0 + half;
   } else {
     n.e0 = a.rot + (n.p0 - half);
     n.e1 = n.e0 + ((a.dim - a.rot) >> 1);
@@ -354,44 +347,28 @@ __device__ __forceinline__ Lane lane_of(const RotArgs& a, int l) {
   return n;
 }
 
-template <int P>
 __device__ __forceinline__ void angles(const RotArgs& a, int64_t pos, int p0, float* c, float* s) {
   if (pos >= 0 && pos < a.table_rows) {
-    const float4* cr = reinterpret_cast<const float4*>(a.cos + pos * a.table_stride + p0);
-    const float4* sr = reinterpret_cast<const float4*>(a.sin + pos * a.table_stride + p0);
-#pragma unroll
-    for (int i = 0; i < P / 4; ++i) {
-      const float4 x = __ldg(cr + i), y = __ldg(sr + i);
-      c[4 * i] = x.x, c[4 * i + 1] = x.y, c[4 * i + 2] = x.z, c[4 * i + 3] = x.w;
-      s[4 * i] = y.x, s[4 * i + 1] = y.y, s[4 * i + 2] = y.z, s[4 * i + 3] = y.w;
-    }
+    const float4 x = __ldg(reinterpret_cast<const float4*>(a.cos + pos * a.table_stride + p0));
+    const float4 y = __ldg(reinterpret_cast<const float4*>(a.sin + pos * a.table_stride + p0));
+    c[0] = x.x, c[1] = x.y, c[2] = x.z, c[3] = x.w;
+    s[0] = y.x, s[1] = y.y, s[2] = y.z, s[3] = y.w;
   } else {
 #pragma unroll
-    for (int i = 0; i < P; ++i) c[i] = s[i] = __int_as_float(0x7fc00000);
+    for (int i = 0; i < kP; ++i) c[i] = s[i] = __int_as_float(0x7fc00000);
   }
 }
 
-// (x0, x1): a lane's two vectors, turned by +angle (sign 1) or -angle (-1)
-template <int P>
-__device__ __forceinline__ void turn(float* x0, float* x1, const float* c, const float* s,
-                                     bool interleaved, float sign) {
-  if (interleaved) {
+// (x0, x1): a lane's two vectors, turned by the angle of (c, s)
+template <bool INTER>
+__device__ __forceinline__ void turn(float* x0, float* x1, const float* c, const float* s) {
 #pragma unroll
-    for (int i = 0; i < P / 2; ++i) {
-      float a = x0[2 * i], b = x0[2 * i + 1], t = sign * s[i];
-      x0[2 * i] = turned0(a, b, c[i], t);
-      x0[2 * i + 1] = turned1(a, b, c[i], t);
-      a = x1[2 * i], b = x1[2 * i + 1], t = sign * s[P / 2 + i];
-      x1[2 * i] = turned0(a, b, c[P / 2 + i], t);
-      x1[2 * i + 1] = turned1(a, b, c[P / 2 + i], t);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-      const float a = x0[i], b = x1[i], t = sign * s[i];
-      x0[i] = turned0(a, b, c[i], t);
-      x1[i] = turned1(a, b, c[i], t);
-    }
+  for (int i = 0; i < kP; ++i) {
+    float& u = INTER ? (i < 2 ? x0[2 * i] : x1[2 * i - 4]) : x0[i];
+    float& v = INTER ? (i < 2 ? x0[2 * i + 1] : x1[2 * i - 3]) : x1[i];
+    const float a = u, b = v;
+    u = turned0(a, b, c[i], s[i]);
+    v = turned1(a, b, c[i], s[i]);
   }
 }
 
@@ -409,194 +386,202 @@ struct AppendArgs {
   int bs_shift;
 };
 
-// Forward and append: rows of q, then k, then (append) v of each token.
-template <typename T, int LPR, int U>
-__global__ void __launch_bounds__(256)
-    norm_rope_vec_kernel(const RotArgs a, const AppendArgs ap) {
-  constexpr int P = kVecPairs<T>, S = 32 / LPR;
+// tasks that cover `heads` rows of a token
+__host__ __device__ inline int tasks_of(int heads, int lanes) {
+  const int per = 32 / lanes * kGroups;
+  return (heads + per - 1) / per;
+}
+
+// Forward and append: tasks of q, then k, then (append) v of each token.
+template <typename T, int LPR, bool INTER, bool APPEND>
+__global__ void __launch_bounds__(kVecWarps * 32)
+    norm_rope_vec_kernel(const __grid_constant__ RotArgs a, const __grid_constant__ AppendArgs ap,
+                         unsigned tasks) {
+  using V = typename Vec4<T>::type;
+  constexpr int S = 32 / LPR;
   const int lane = threadIdx.x & 31;
-  const int heads = a.q.heads + a.k.heads + (ap.slots ? a.k.heads : 0);
-  const int64_t total = a.tokens * heads;
-  const int64_t base = (blockIdx.x * 8ll + (threadIdx.x >> 5)) * (S * U) + lane / LPR;
-  if (base - lane / LPR >= total) return;
-  const Lane ln = lane_of<P>(a, lane % LPR);
-  int64_t t = base / heads;
-  int h = (int)(base - t * heads);
-  uint4 x0[U], x1[U];
-  char* dst[U];
-  int kind[U];  // 0: no row, 1: norm and turn, 2: copy
-  int64_t pos[U];
-  const void* wp[U];
+  const unsigned task = blockIdx.x * kVecWarps + (threadIdx.x >> 5);
+  if (task >= tasks) return;
+  const int nq = tasks_of(a.q.heads, LPR), nk = tasks_of(a.k.heads, LPR);
+  const unsigned per = nq + (APPEND ? 2 : 1) * nk;
+  const unsigned t = task / per;
+  int part = task - t * per;
+  int kind = 0;  // 0: q, 1: k, 2: v
+  if (part >= nq) part -= nq, kind = 1;
+  if (APPEND && kind == 1 && part >= nk) part -= nk, kind = 2;
+  const Rows& rw = kind == 0 ? a.q : (kind == 1 ? a.k : ap.v);
+  const int heads = rw.heads;
+  const int h0 = part * (S * kGroups) + lane / LPR;
+  const Lane ln = lane_of<INTER>(a, lane % LPR);
+  const char* x = rw.x + t * rw.xt + h0 * rw.xh;
+  V x0[kGroups], x1[kGroups];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    kind[u] = 0;
-    wp[u] = nullptr;
-    if (base + u * S < total) {
-      int hh = h;
-      const Rows* rw = &a.q;
-      kind[u] = 1;
-      if (hh >= a.q.heads) {
-        hh -= a.q.heads;
-        rw = &a.k;
-        if (hh >= a.k.heads) {
-          hh -= a.k.heads;
-          rw = &ap.v;
-          kind[u] = 2;
-        }
-      }
-      const T* x = reinterpret_cast<const T*>(rw->x + t * rw->xt + hh * rw->xh);
-      x0[u] = *reinterpret_cast<const uint4*>(x + ln.e0);
-      x1[u] = *reinterpret_cast<const uint4*>(x + ln.e1);
-      wp[u] = rw->w;
-      pos[u] = a.positions[t];
-      dst[u] = rw->y + t * rw->yt + hh * rw->yh;
-      const bool pos_ok = pos[u] >= 0 && pos[u] < a.table_rows;
-      if (!pos_ok && lane % LPR == 0) report(a.status, CS_ST_POS_RANGE);
-      if (ap.slots && h >= a.q.heads) {
-        const int64_t slot = ap.slots[t];
-        if (!ap.pv.valid(slot) || !pos_ok) {
-          if (slot != -1 && !ap.pv.valid(slot) && lane % LPR == 0)
-            report(a.status, CS_ST_SLOT_RANGE);
-          dst[u] = nullptr;
-        } else if (slot < ap.pv.native_total && ap.bs_shift >= 0) {
-          const int64_t b = slot >> ap.bs_shift, o = slot - (b << ap.bs_shift);
-          dst[u] = ap.pv.cache + b * ap.pv.sb + hh * ap.pv.sh + o * ap.pv.so +
-                   (kind[u] == 2 ? a.dim * (int)sizeof(T) : 0);
-        } else {
-          dst[u] = ap.pv.addr(slot, hh, kind[u] == 2 ? a.dim : 0);
-        }
-      }
-    }
-    h += S;
-    while (h >= heads) {
-      h -= heads;
-      ++t;
+  for (int u = 0; u < kGroups; ++u) {
+    if (h0 + u * S < heads) {
+      const T* row = reinterpret_cast<const T*>(x + u * S * rw.xh);
+      x0[u] = *reinterpret_cast<const V*>(row + ln.e0);
+      x1[u] = *reinterpret_cast<const V*>(row + ln.e1);
+    } else {
+      x0[u] = x1[u] = V{};
     }
   }
+  const int64_t pos = a.positions[t];
+  const bool pos_ok = pos >= 0 && pos < a.table_rows;
+  if (!pos_ok && lane == 0) report(a.status, CS_ST_POS_RANGE);
+  char* y = rw.y + t * rw.yt + h0 * rw.yh;
+  int64_t yh = rw.yh;
+  if (APPEND && kind > 0) {
+    const int64_t slot = ap.slots[t];
+    if (!ap.pv.valid(slot)) {
+      if (slot != -1 && lane == 0) report(a.status, CS_ST_SLOT_RANGE);
+      return;
+    }
+    if (!pos_ok) return;
+    if (slot < ap.pv.native_total) {
+      const int64_t b = ap.bs_shift >= 0 ? slot >> ap.bs_shift : slot / ap.pv.bs;
+      const int64_t o = slot - (ap.bs_shift >= 0 ? b << ap.bs_shift : b * ap.pv.bs);
+      yh = ap.pv.sh;
+      y = ap.pv.cache + b * ap.pv.sb + o * ap.pv.so + h0 * yh +
+          (kind == 2 ? a.dim * (int)sizeof(T) : 0);
+    } else {
+      yh = ap.pv.ssh;
+      y = (kind == 2 ? ap.pv.side_v : ap.pv.side_k) + (slot - ap.pv.native_total) * ap.pv.ssr +
+          h0 * yh;
+    }
+  }
+  if (!APPEND || kind < 2) {
+    float c[kP], s[kP], w0[kP], w1[kP];
+    if (ln.turns) angles(a, pos, ln.p0, c, s);
+    if (rw.w) {
+      weights_at(rw.w, a.wdtype, ln.e0, w0);
+      weights_at(rw.w, a.wdtype, ln.e1, w1);
+    }
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    // every lane takes part in the row sums
-    float f0[P], f1[P];
-    float ss = 0.f;
-    if (kind[u] == 1) {
+    for (int u = 0; u < kGroups; ++u) {
+      float f0[kP], f1[kP];
       unpack<T>(x0[u], f0);
       unpack<T>(x1[u], f1);
+      if (rw.w) {
+        float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < P; ++i) ss += f0[i] * f0[i] + f1[i] * f1[i];
-    }
-    ss = row_sum<LPR>(ss);
-    if (kind[u] == 0) continue;
-    if (kind[u] == 1) {
-      if (wp[u]) {
-        const float r = rsqrtf(ss * a.inv_dim + a.eps);
-        float w[P];
-        weights_at<T, P>(wp[u], a.wdtype, ln.e0, w);
+        for (int i = 0; i < kP; ++i) ss += f0[i] * f0[i] + f1[i] * f1[i];
+        const float r = rsqrtf(row_sum<LPR>(ss) * a.inv_dim + a.eps);
 #pragma unroll
-        for (int i = 0; i < P; ++i) f0[i] *= r * w[i];
-        weights_at<T, P>(wp[u], a.wdtype, ln.e1, w);
-#pragma unroll
-        for (int i = 0; i < P; ++i) f1[i] *= r * w[i];
+        for (int i = 0; i < kP; ++i) {
+          f0[i] *= r * w0[i];
+          f1[i] *= r * w1[i];
+        }
       }
-      if (ln.turns) {
-        float c[P], s[P];
-        angles<P>(a, pos[u], ln.p0, c, s);
-        turn<P>(f0, f1, c, s, a.interleaved, 1.f);
-      }
+      if (ln.turns) turn<INTER>(f0, f1, c, s);
       x0[u] = pack<T>(f0);
       x1[u] = pack<T>(f1);
     }
-    if (dst[u] == nullptr) continue;
-    T* y = reinterpret_cast<T*>(dst[u]);
-    *reinterpret_cast<uint4*>(y + ln.e0) = x0[u];
-    *reinterpret_cast<uint4*>(y + ln.e1) = x1[u];
+  }
+#pragma unroll
+  for (int u = 0; u < kGroups; ++u) {
+    if (h0 + u * S < heads) {
+      T* row = reinterpret_cast<T*>(y + u * S * yh);
+      *reinterpret_cast<V*>(row + ln.e0) = x0[u];
+      *reinterpret_cast<V*>(row + ln.e1) = x1[u];
+    }
   }
 }
 
-// Gradient: blocks below nq take rows of q, the rest rows of k, each a fixed
+// Gradient: blocks below nq take tasks of q, the rest tasks of k, each a fixed
 // share whatever the count; dw of a lane's elements stays in its registers,
 // then lanes, warps and (in grad_weight_kernel) blocks are added in order.
-template <typename T, int LPR>
-__global__ void __launch_bounds__(256)
-    norm_rope_grad_vec_kernel(const RotArgs a, int nq, float* __restrict__ part) {
-  constexpr int P = kVecPairs<T>, S = 32 / LPR;
-  __shared__ float acc[8][kMaxDim];
+constexpr int kGradGroups = 2;
+template <typename T, int LPR, bool INTER>
+__global__ void __launch_bounds__(256, 3)
+    norm_rope_grad_vec_kernel(const __grid_constant__ RotArgs a, int nq,
+                              float* __restrict__ part) {
+  using V = typename Vec4<T>::type;
+  constexpr int S = 32 / LPR, U = kGradGroups;
+  __shared__ float acc[8][LPR * 2 * kP];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bool isk = (int)blockIdx.x >= nq;
   const Rows& rw = isk ? a.k : a.q;
   const int b = isk ? blockIdx.x - nq : blockIdx.x;
-  const int blocks = isk ? gridDim.x - nq : nq;
-  const Lane ln = lane_of<P>(a, lane % LPR);
-  float w0[P], w1[P], d0[P], d1[P];
+  const unsigned blocks = isk ? gridDim.x - nq : nq;
+  const Lane ln = lane_of<INTER>(a, lane % LPR);
+  float w0[kP], w1[kP], d0[kP], d1[kP];
 #pragma unroll
-  for (int i = 0; i < P; ++i) w0[i] = w1[i] = d0[i] = d1[i] = 0.f;
-  if (rw.w) {
-    weights_at<T, P>(rw.w, a.wdtype, ln.e0, w0);
-    weights_at<T, P>(rw.w, a.wdtype, ln.e1, w1);
+  for (int i = 0; i < kP; ++i) w0[i] = w1[i] = d0[i] = d1[i] = 0.f;
+  const bool norm = rw.w != nullptr;
+  if (norm) {
+    weights_at(rw.w, a.wdtype, ln.e0, w0);
+    weights_at(rw.w, a.wdtype, ln.e1, w1);
   }
-  const int64_t total = a.tokens * rw.heads;
-  const int64_t step = (int64_t)blocks * 8 * S;
-  for (int64_t first = ((int64_t)b * 8 + warp) * S; first < total; first += step) {
-    const int64_t row = first + lane / LPR;
-    const bool live = row < total;
-    float g0[P], g1[P], n0[P], n1[P];
-    float ss = 0.f, dot = 0.f;
-    T* dx = nullptr;
-    if (live) {
-      const int64_t t = row / rw.heads;
-      const int h = (int)(row - t * rw.heads);
-      const int64_t pos = a.positions[t];
-      const T* dy = reinterpret_cast<const T*>(rw.dy + t * rw.yt + h * rw.yh);
-      dx = reinterpret_cast<T*>(rw.y + t * rw.yt + h * rw.yh);
-      const uint4 y0 = *reinterpret_cast<const uint4*>(dy + ln.e0);
-      const uint4 y1 = *reinterpret_cast<const uint4*>(dy + ln.e1);
-      uint4 x0, x1;
-      if (rw.w) {
-        const T* x = reinterpret_cast<const T*>(rw.x + t * rw.xt + h * rw.xh);
-        x0 = *reinterpret_cast<const uint4*>(x + ln.e0);
-        x1 = *reinterpret_cast<const uint4*>(x + ln.e1);
-      }
-      if (lane % LPR == 0 && (pos < 0 || pos >= a.table_rows)) report(a.status, CS_ST_POS_RANGE);
-      unpack<T>(y0, g0);
-      unpack<T>(y1, g1);
-      if (ln.turns) {
-        float c[P], s[P];
-        angles<P>(a, pos, ln.p0, c, s);
-        turn<P>(g0, g1, c, s, a.interleaved, -1.f);
-      }
-      if (rw.w) {
-        unpack<T>(x0, n0);
-        unpack<T>(x1, n1);
+  const unsigned per = (rw.heads + S * U - 1) / (S * U);
+  const unsigned total = (unsigned)a.tokens * per;
+  for (unsigned task = b * 8u + warp; task < total; task += blocks * 8u) {
+    const unsigned t = task / per;
+    const int h0 = (task - t * per) * (S * U) + lane / LPR;
+    const char* x = rw.x + t * rw.xt + h0 * rw.xh;
+    const char* dy = rw.dy + t * rw.yt + h0 * rw.yh;
+    char* dx = rw.y + t * rw.yt + h0 * rw.yh;
+    V x0[U], x1[U], y0[U], y1[U];
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
+    for (int u = 0; u < U; ++u) {
+      x0[u] = x1[u] = y0[u] = y1[u] = V{};
+      if (h0 + u * S < rw.heads) {
+        const T* yr = reinterpret_cast<const T*>(dy + u * S * rw.yh);
+        y0[u] = *reinterpret_cast<const V*>(yr + ln.e0);
+        y1[u] = *reinterpret_cast<const V*>(yr + ln.e1);
+        if (norm) {
+          const T* xr = reinterpret_cast<const T*>(x + u * S * rw.xh);
+          x0[u] = *reinterpret_cast<const V*>(xr + ln.e0);
+          x1[u] = *reinterpret_cast<const V*>(xr + ln.e1);
+        }
+      }
+    }
+    const int64_t pos = a.positions[t];
+    if (lane == 0 && (pos < 0 || pos >= a.table_rows)) report(a.status, CS_ST_POS_RANGE);
+    float c[kP], s[kP];
+    if (ln.turns) {
+      angles(a, pos, ln.p0, c, s);
+#pragma unroll
+      for (int i = 0; i < kP; ++i) s[i] = -s[i];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float g0[kP], g1[kP];
+      unpack<T>(y0[u], g0);
+      unpack<T>(y1[u], g1);
+      if (ln.turns) turn<INTER>(g0, g1, c, s);
+      if (norm) {
+        float n0[kP], n1[kP], ss = 0.f, dot = 0.f;
+        unpack<T>(x0[u], n0);
+        unpack<T>(x1[u], n1);
+#pragma unroll
+        for (int i = 0; i < kP; ++i) {
           ss += n0[i] * n0[i] + n1[i] * n1[i];
           dot += w0[i] * g0[i] * n0[i] + w1[i] * g1[i] * n1[i];
         }
-      }
-    }
-    if (rw.w) {
-      ss = row_sum<LPR>(ss);
-      dot = row_sum<LPR>(dot);
-      if (live) {
-        const float r = rsqrtf(ss * a.inv_dim + a.eps);
-        const float mean = dot * r * a.inv_dim;  // mean(w g n)
+        const float r = rsqrtf(row_sum<LPR>(ss) * a.inv_dim + a.eps);
+        const float mean = row_sum<LPR>(dot) * r * a.inv_dim;  // mean(w g n)
+        // rows past the end hold zeros and add zeros
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-          const float u = n0[i] * r, v = n1[i] * r;
-          d0[i] += g0[i] * u;
-          d1[i] += g1[i] * v;
-          g0[i] = r * (w0[i] * g0[i] - u * mean);
-          g1[i] = r * (w1[i] * g1[i] - v * mean);
+        for (int i = 0; i < kP; ++i) {
+          const float p = n0[i] * r, q = n1[i] * r;
+          if (h0 + u * S < rw.heads) {
+            d0[i] += g0[i] * p;
+            d1[i] += g1[i] * q;
+          }
+          g0[i] = r * (w0[i] * g0[i] - p * mean);
+          g1[i] = r * (w1[i] * g1[i] - q * mean);
         }
       }
-    }
-    if (live) {
-      *reinterpret_cast<uint4*>(dx + ln.e0) = pack<T>(g0);
-      *reinterpret_cast<uint4*>(dx + ln.e1) = pack<T>(g1);
+      if (h0 + u * S < rw.heads) {
+        T* row = reinterpret_cast<T*>(dx + u * S * rw.yh);
+        *reinterpret_cast<V*>(row + ln.e0) = pack<T>(g0);
+        *reinterpret_cast<V*>(row + ln.e1) = pack<T>(g1);
+      }
     }
   }
-  if (!rw.w) return;
+  if (!norm) return;
 #pragma unroll
-  for (int i = 0; i < P; ++i) {
+  for (int i = 0; i < kP; ++i) {
 #pragma unroll
     for (int o = LPR; o < 32; o <<= 1) {
       d0[i] += __shfl_xor_sync(0xffffffffu, d0[i], o);
@@ -690,20 +675,24 @@ unsigned row_blocks(int64_t rows) {
 }
 
 // Lanes a row of the vector kernels, 0 where they do not fit: whole vectors
-// in every part of a head, and 16-byte aligned rows, tables and weights.
+// of 4 elements in every part of a head, rows, tables and weights aligned to
+// them, and fewer than 2^31 tasks.
 int vec_lanes(const RotArgs& a, int dtype, bool grad) {
-  const int P = 16 / dtype_size(dtype), half = a.dim / 2;
-  const int lanes = half / P;
-  if (half % P || (a.rot / 2) % P || lanes > 32 || (lanes & (lanes - 1))) return 0;
-  auto al = [](const void* x, int64_t t, int64_t h) {
-    return reinterpret_cast<uintptr_t>(x) % 16 == 0 && t % 16 == 0 && h % 16 == 0;
+  const int half = a.dim / 2, lanes = half / kP;
+  if (half % kP || (a.rot / 2) % kP || lanes > 32 || (lanes & (lanes - 1))) return 0;
+  const int64_t unit = 4 * dtype_size(dtype);
+  auto al = [](const void* x, int64_t t, int64_t h, int64_t unit) {
+    return reinterpret_cast<uintptr_t>(x) % unit == 0 && t % unit == 0 && h % unit == 0;
   };
   for (const Rows* r : {&a.q, &a.k}) {
     if (r->heads == 0) continue;
-    if (!al(r->x, r->xt, r->xh) || !al(r->y, r->yt, r->yh) || !al(r->w, 0, 0)) return 0;
-    if (grad && !al(r->dy, r->yt, r->yh)) return 0;
+    if (!al(r->x, r->xt, r->xh, unit) || !al(r->y, r->yt, r->yh, unit) || !al(r->w, 0, 0, 16))
+      return 0;
+    if (grad && !al(r->dy, r->yt, r->yh, unit)) return 0;
   }
-  if (a.rot > 0 && (!al(a.cos, a.table_stride * 4, 0) || !al(a.sin, 0, 0))) return 0;
+  if (a.rot > 0 && (!al(a.cos, a.table_stride * 4, 0, 16) || !al(a.sin, 0, 0, 16))) return 0;
+  const int64_t most = 2ll * (a.q.heads + a.k.heads) + 3;
+  if (a.tokens > INT32_MAX / most) return 0;
   return lanes;
 }
 
@@ -728,20 +717,22 @@ void by_lanes(int lanes, F f) {
   }
 }
 
-int launch_vec(const RotArgs& a, const AppendArgs& ap, int64_t rows, int dtype, int lanes,
-               cudaStream_t stream) {
+int launch_vec(const RotArgs& a, const AppendArgs* ap, int dtype, int lanes, cudaStream_t stream) {
+  const int64_t tasks = a.tokens * (tasks_of(a.q.heads, lanes) +
+                                    (ap ? 2 : 1) * tasks_of(a.k.heads, lanes));
+  const unsigned blocks = (unsigned)((tasks + kVecWarps - 1) / kVecWarps);
   return by_type(dtype, [&](auto* ty) {
     using T = std::remove_pointer_t<decltype(ty)>;
     by_lanes(lanes, [&](auto l) {
-      constexpr int LPR = decltype(l)::value;
-      // one group of rows a warp while that leaves SMs idle, four when not
-      const int64_t per = 8 * (32 / LPR);
-      const int64_t one = (rows + per - 1) / per;
-      if (one <= 4ll * num_sms())
-        norm_rope_vec_kernel<T, LPR, 1><<<(unsigned)one, 256, 0, stream>>>(a, ap);
-      else
-        norm_rope_vec_kernel<T, LPR, 4>
-            <<<(unsigned)((rows + 4 * per - 1) / (4 * per)), 256, 0, stream>>>(a, ap);
+      constexpr int L = decltype(l)::value;
+      auto go = [&](auto inter, auto append) {
+        norm_rope_vec_kernel<T, L, decltype(inter)::value, decltype(append)::value>
+            <<<blocks, kVecWarps * 32, 0, stream>>>(a, ap ? *ap : AppendArgs{}, (unsigned)tasks);
+      };
+      if (a.interleaved && ap) go(std::true_type(), std::true_type());
+      else if (a.interleaved) go(std::true_type(), std::false_type());
+      else if (ap) go(std::false_type(), std::true_type());
+      else go(std::false_type(), std::false_type());
     });
   });
 }
@@ -756,7 +747,7 @@ extern "C" int cs_qk_norm_rope(const cs_rotary_params* p, void* stream) {
   const int64_t rows = p->tokens * (p->q_heads + p->k_heads);
   if (rows == 0) return CS_OK;
   if (const int lanes = vec_lanes(a, p->dtype, false))
-    return launch_vec(a, AppendArgs{}, rows, p->dtype, lanes, as_stream(stream));
+    return launch_vec(a, nullptr, p->dtype, lanes, as_stream(stream));
   return by_type(p->dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     norm_rope_rows_kernel<T><<<row_blocks(rows), kRowWarps * 32, 0, as_stream(stream)>>>(a);
@@ -781,10 +772,10 @@ extern "C" int cs_qk_norm_rope_grad(const cs_rotary_params* p, const void* q_dy,
   // blocks in proportion to the heads, no more than the rows fill
   const int heads = p->q_heads + p->k_heads;
   const int lanes = vec_lanes(a, p->dtype, true);
-  const int64_t per = lanes ? 8 * (32 / lanes) : kRowWarps;
+  const int per = lanes ? 32 / lanes * kGradGroups : 1;  // rows a warp takes at once
   auto share = [&](int h) {
     const int64_t most = heads ? ((int64_t)kGradBlocks * h + heads - 1) / heads : 0;
-    const int64_t want = (p->tokens * h + per - 1) / per;
+    const int64_t want = (p->tokens * ((h + per - 1) / per) + 7) / 8;
     return (int)std::max<int64_t>(1, std::min(most, want));
   };
   const int nq = share(p->q_heads), n = nq + share(p->k_heads);
@@ -793,8 +784,11 @@ extern "C" int cs_qk_norm_rope_grad(const cs_rotary_params* p, const void* q_dy,
     float* part = static_cast<float*>(workspace);
     if (lanes)
       by_lanes(lanes, [&](auto l) {
-        norm_rope_grad_vec_kernel<T, decltype(l)::value>
-            <<<n, 256, 0, as_stream(stream)>>>(a, nq, part);
+        constexpr int L = decltype(l)::value;
+        if (a.interleaved)
+          norm_rope_grad_vec_kernel<T, L, true><<<n, 256, 0, as_stream(stream)>>>(a, nq, part);
+        else
+          norm_rope_grad_vec_kernel<T, L, false><<<n, 256, 0, as_stream(stream)>>>(a, nq, part);
       });
     else
       norm_rope_grad_rows_kernel<T><<<n, kRowWarps * 32, 0, as_stream(stream)>>>(a, nq, part);
@@ -822,8 +816,8 @@ extern "C" int cs_kv_append_rotated(const cs_rotary_params* p, const cs_paged_kv
   const Rows vr{static_cast<const char*>(v), nullptr, nullptr, nullptr, v_stride_tok * es,
                 v_stride_head * es, 0, 0, p->k_heads};
   const PagedView pv = PagedView::make(*kv);
-  if (pv.vec16() && reinterpret_cast<uintptr_t>(v) % 16 == 0 && vr.xt % 16 == 0 &&
-      vr.xh % 16 == 0) {
+  if (pv.vec16() && reinterpret_cast<uintptr_t>(v) % (4 * es) == 0 && vr.xt % (4 * es) == 0 &&
+      vr.xh % (4 * es) == 0) {
     RotArgs d = a;  // k has no dense output
     d.k.y = nullptr;
     d.k.yt = d.k.yh = 0;
@@ -831,8 +825,8 @@ extern "C" int cs_kv_append_rotated(const cs_rotary_params* p, const cs_paged_kv
       int shift = -1;
       for (int s = 0; s < 31; ++s)
         if ((int64_t)1 << s == kv->block_size) shift = s;
-      return launch_vec(d, AppendArgs{pv, slots, vr, shift}, rows, p->dtype, lanes,
-                        as_stream(stream));
+      const AppendArgs ap{pv, slots, vr, shift};
+      return launch_vec(d, &ap, p->dtype, lanes, as_stream(stream));
     }
   }
   return by_type(p->dtype, [&](auto* t) {
