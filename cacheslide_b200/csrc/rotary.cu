@@ -22,7 +22,7 @@ namespace {
 
 constexpr int kMaxDim = 512;
 constexpr int kMaxPairs = kMaxDim / 2 / 32;  // pairs a lane of a warp-per-row kernel
-constexpr int kGradBlocks = 740;             // 148 SMs x 5: the fixed partition of dw
+constexpr int kGradBlocks = 296;             // 148 SMs x 2: the fixed partition of dw
 constexpr int kRowWarps = 8;
 
 struct Rows {
@@ -487,116 +487,281 @@ __global__ void __launch_bounds__(kVecWarps * 32)
   }
 }
 
-// Gradient: blocks below nq take tasks of q, the rest tasks of k, each a fixed
-// share whatever the count; dw of a lane's elements stays in its registers,
-// then lanes, warps and (in grad_weight_kernel) blocks are added in order.
-constexpr int kGradGroups = 2;
+// ----------------------------------------------------------- streamed kernel
+// For many rows: 16-byte vectors (P = 8 pairs a lane, 4 in float32), each warp
+// streaming its rows through a ring of row groups in shared memory by
+// cp.async, every lane its own vectors (so no barrier): bytes in flight cost
+// no registers, and a lane's longer share halves the instructions a row.
+template <typename T> constexpr int kPairs = 16 / (int)sizeof(T);
+
+// A lane's P pairs, two at a time for the packed float32 instructions: a[i]
+// holds the first elements of pairs 2i and 2i + 1, b[i] the second.
+template <int P>
+struct Pairs {
+  float2 a[P / 2], b[P / 2];
+};
+
+template <typename T, int P>
+__device__ __forceinline__ void unpack16(const uint4& v, float* f) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (P == 4) {
+      f[i] = __uint_as_float(w[i]);
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[2 * i] = x.x, f[2 * i + 1] = x.y;
+    } else {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+}
+template <typename T, int P>
+__device__ __forceinline__ uint4 pack16(const float* f) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (P == 4) w[i] = __float_as_uint(f[i]);
+    else w[i] = Pack2<T>::pack(f[2 * i], f[2 * i + 1]);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// two vectors' elements <-> pairs
+template <int P, bool INTER>
+__device__ __forceinline__ void to_pairs(const float* u, const float* v, Pairs<P>& p) {
+#pragma unroll
+  for (int i = 0; i < P / 2; ++i) {
+    if constexpr (INTER) {
+      const float* x = i < P / 4 ? u + 4 * i : v + 4 * i - P;
+      p.a[i] = make_float2(x[0], x[2]);
+      p.b[i] = make_float2(x[1], x[3]);
+    } else {
+      p.a[i] = make_float2(u[2 * i], u[2 * i + 1]);
+      p.b[i] = make_float2(v[2 * i], v[2 * i + 1]);
+    }
+  }
+}
+template <int P, bool INTER>
+__device__ __forceinline__ void from_pairs(const Pairs<P>& p, float* u, float* v) {
+#pragma unroll
+  for (int i = 0; i < P / 2; ++i) {
+    if constexpr (INTER) {
+      float* x = i < P / 4 ? u + 4 * i : v + 4 * i - P;
+      x[0] = p.a[i].x, x[2] = p.a[i].y;
+      x[1] = p.b[i].x, x[3] = p.b[i].y;
+    } else {
+      u[2 * i] = p.a[i].x, u[2 * i + 1] = p.a[i].y;
+      v[2 * i] = p.b[i].x, v[2 * i + 1] = p.b[i].y;
+    }
+  }
+}
+template <typename T, int P, bool INTER>
+__device__ __forceinline__ void load_pairs(const uint4& x, const uint4& y, Pairs<P>& p) {
+  float u[P], v[P];
+  unpack16<T, P>(x, u);
+  unpack16<T, P>(y, v);
+  to_pairs<P, INTER>(u, v, p);
+}
+template <typename T, int P, bool INTER>
+__device__ __forceinline__ void store_pairs(const Pairs<P>& p, uint4& x, uint4& y) {
+  float u[P], v[P];
+  from_pairs<P, INTER>(p, u, v);
+  x = pack16<T, P>(u);
+  y = pack16<T, P>(v);
+}
+template <int P, bool INTER>
+__device__ __forceinline__ Lane lane_of16(const RotArgs& a, int l) {
+  Lane n;
+  n.p0 = l * P;
+  const int half = a.rot >> 1;
+  n.turns = n.p0 < half;
+  if (n.turns) {
+    n.e0 = INTER ? 2 * n.p0 : n.p0;
+    n.e1 = INTER ? n.e0 + P : n.p0 + half;
+  } else {
+    n.e0 = a.rot + (n.p0 - half);
+    n.e1 = n.e0 + ((a.dim - a.rot) >> 1);
+  }
+  return n;
+}
+template <int P, bool INTER>
+__device__ __forceinline__ void load_weights(const void* w, int dtype, const Lane& ln,
+                                             Pairs<P>& p) {
+  float u[P], v[P];
+#pragma unroll
+  for (int i = 0; i < P / 4; ++i) {
+    weights_at(w, dtype, ln.e0 + 4 * i, u + 4 * i);
+    weights_at(w, dtype, ln.e1 + 4 * i, v + 4 * i);
+  }
+  to_pairs<P, INTER>(u, v, p);
+}
+template <int P>
+__device__ __forceinline__ void load_angles(const RotArgs& a, int64_t pos, int p0, float2* c,
+                                            float2* s) {
+#pragma unroll
+  for (int i = 0; i < P / 4; ++i)
+    angles(a, pos, p0 + 4 * i, reinterpret_cast<float*>(c + 2 * i),
+           reinterpret_cast<float*>(s + 2 * i));
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 neg(float2 x) { return make_float2(-x.x, -x.y); }
+
+// a warp's place in its share: row group u of a part of token t
+struct Place {
+  unsigned task, t;
+  int u, end;
+  __device__ __forceinline__ void start(unsigned total, unsigned parts, int groups) {
+    if (task >= total) return;
+    t = task / parts;
+    const int q = (int)(task - t * parts);
+    u = groups * q / (int)parts;
+    end = groups * (q + 1) / (int)parts;
+  }
+};
+
+// Gradient: blocks below nq take tokens of q, the rest tokens of k, each warp
+// every W-th (token, part of its heads), a fixed share; dw of a lane's
+// elements stays in its registers, then lanes, warps and (in
+// grad_weight_kernel) blocks are added in order.
+constexpr int kGradWarps = 8;
+constexpr int kGradRing = 3;  // row groups in flight a warp, 2 KB each
+
 template <typename T, int LPR, bool INTER>
-__global__ void __launch_bounds__(256, 3)
-    norm_rope_grad_vec_kernel(const __grid_constant__ RotArgs a, int nq,
-                              float* __restrict__ part) {
-  using V = typename Vec4<T>::type;
-  constexpr int S = 32 / LPR, U = kGradGroups;
-  __shared__ float acc[8][LPR * 2 * kP];
+__global__ void __launch_bounds__(kGradWarps * 32, 2)
+    norm_rope_grad_kernel(const __grid_constant__ RotArgs a, int nq, int most_parts,
+                          float* __restrict__ part) {
+  constexpr int P = kPairs<T>, S = 32 / LPR, R = kGradRing;
+  extern __shared__ uint4 smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // [ring slot][x0, x1, dy0, dy1][lane]
+  uint4* ring = smem + warp * (R * 4 * 32) + lane;
+  const uint32_t ring_at = smem_u32(ring);
   const bool isk = (int)blockIdx.x >= nq;
   const Rows& rw = isk ? a.k : a.q;
   const int b = isk ? blockIdx.x - nq : blockIdx.x;
-  const unsigned blocks = isk ? gridDim.x - nq : nq;
-  const Lane ln = lane_of<INTER>(a, lane % LPR);
-  float w0[kP], w1[kP], d0[kP], d1[kP];
-#pragma unroll
-  for (int i = 0; i < kP; ++i) w0[i] = w1[i] = d0[i] = d1[i] = 0.f;
+  const unsigned step = (isk ? gridDim.x - nq : nq) * kGradWarps;
+  const Lane ln = lane_of16<P, INTER>(a, lane % LPR);
   const bool norm = rw.w != nullptr;
-  if (norm) {
-    weights_at(rw.w, a.wdtype, ln.e0, w0);
-    weights_at(rw.w, a.wdtype, ln.e1, w1);
-  }
-  const unsigned per = (rw.heads + S * U - 1) / (S * U);
-  const unsigned total = (unsigned)a.tokens * per;
-  for (unsigned task = b * 8u + warp; task < total; task += blocks * 8u) {
-    const unsigned t = task / per;
-    const int h0 = (task - t * per) * (S * U) + lane / LPR;
-    const char* x = rw.x + t * rw.xt + h0 * rw.xh;
-    const char* dy = rw.dy + t * rw.yt + h0 * rw.yh;
-    char* dx = rw.y + t * rw.yt + h0 * rw.yh;
-    V x0[U], x1[U], y0[U], y1[U];
+  Pairs<P> w, d;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      x0[u] = x1[u] = y0[u] = y1[u] = V{};
-      if (h0 + u * S < rw.heads) {
-        const T* yr = reinterpret_cast<const T*>(dy + u * S * rw.yh);
-        y0[u] = *reinterpret_cast<const V*>(yr + ln.e0);
-        y1[u] = *reinterpret_cast<const V*>(yr + ln.e1);
+  for (int i = 0; i < P / 2; ++i) w.a[i] = w.b[i] = d.a[i] = d.b[i] = both(0.f);
+  if (norm) load_weights<P, INTER>(rw.w, a.wdtype, ln, w);
+  const int groups = (rw.heads + S - 1) / S;
+  // no part is empty: q and k have different numbers of groups
+  const unsigned parts = most_parts < groups ? most_parts : groups;
+  const unsigned total = (unsigned)a.tokens * parts;
+  Place in{(unsigned)b * kGradWarps + warp, 0, 0, 0};
+  in.start(total, parts, groups);
+  Place at = in;
+  auto issue = [&](int slot) {
+    if (in.task < total) {
+      const int h = in.u * S + lane / LPR;
+      if (h < rw.heads) {
+        const uint32_t to = ring_at + slot * (4 * 32 * 16);
+        const T* dy = reinterpret_cast<const T*>(rw.dy + in.t * rw.yt + h * rw.yh);
+        cp_async16(to + 2 * 512, dy + ln.e0, true);
+        cp_async16(to + 3 * 512, dy + ln.e1, true);
         if (norm) {
-          const T* xr = reinterpret_cast<const T*>(x + u * S * rw.xh);
-          x0[u] = *reinterpret_cast<const V*>(xr + ln.e0);
-          x1[u] = *reinterpret_cast<const V*>(xr + ln.e1);
+          const T* x = reinterpret_cast<const T*>(rw.x + in.t * rw.xt + h * rw.xh);
+          cp_async16(to, x + ln.e0, true);
+          cp_async16(to + 512, x + ln.e1, true);
         }
       }
+      if (++in.u == in.end) {
+        in.task += step;
+        in.start(total, parts, groups);
+      }
     }
-    const int64_t pos = a.positions[t];
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int r = 0; r < R - 1; ++r) issue(r);
+  int slot = 0;
+  while (at.task < total) {
+    const int64_t pos = a.positions[at.t];
     if (lane == 0 && (pos < 0 || pos >= a.table_rows)) report(a.status, CS_ST_POS_RANGE);
-    float c[kP], s[kP];
-    if (ln.turns) {
-      angles(a, pos, ln.p0, c, s);
+    float2 c[P / 2], s[P / 2];
+    if (ln.turns) load_angles<P>(a, pos, ln.p0, c, s);
+    for (; at.u < at.end; ++at.u) {
+      cp_async_wait<R - 2>();
+      const uint4* mine = ring + slot * (4 * 32);
+      Pairs<P> g, n;
+      load_pairs<T, P, INTER>(mine[64], mine[96], g);
+      if (norm) load_pairs<T, P, INTER>(mine[0], mine[32], n);
+      // the slot read in the last round is free
+      issue(slot == 0 ? R - 1 : slot - 1);
+      slot = slot == R - 1 ? 0 : slot + 1;
+      const int h = at.u * S + lane / LPR;
+      const bool live = h < rw.heads;
+      if (ln.turns) {
 #pragma unroll
-      for (int i = 0; i < kP; ++i) s[i] = -s[i];
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float g0[kP], g1[kP];
-      unpack<T>(y0[u], g0);
-      unpack<T>(y1[u], g1);
-      if (ln.turns) turn<INTER>(g0, g1, c, s);
+        for (int i = 0; i < P / 2; ++i) {
+          const float2 t = __ffma2_rn(g.a[i], c[i], __fmul2_rn(g.b[i], s[i]));
+          g.b[i] = __ffma2_rn(g.b[i], c[i], __fmul2_rn(g.a[i], neg(s[i])));
+          g.a[i] = t;
+        }
+      }
       if (norm) {
-        float n0[kP], n1[kP], ss = 0.f, dot = 0.f;
-        unpack<T>(x0[u], n0);
-        unpack<T>(x1[u], n1);
+        Pairs<P> wg;
+        float2 ss = both(0.f), dot = both(0.f);
 #pragma unroll
-        for (int i = 0; i < kP; ++i) {
-          ss += n0[i] * n0[i] + n1[i] * n1[i];
-          dot += w0[i] * g0[i] * n0[i] + w1[i] * g1[i] * n1[i];
+        for (int i = 0; i < P / 2; ++i) {
+          ss = __ffma2_rn(n.a[i], n.a[i], ss);
+          ss = __ffma2_rn(n.b[i], n.b[i], ss);
+          wg.a[i] = __fmul2_rn(w.a[i], g.a[i]);
+          wg.b[i] = __fmul2_rn(w.b[i], g.b[i]);
+          dot = __ffma2_rn(wg.a[i], n.a[i], dot);
+          dot = __ffma2_rn(wg.b[i], n.b[i], dot);
         }
-        const float r = rsqrtf(row_sum<LPR>(ss) * a.inv_dim + a.eps);
-        const float mean = row_sum<LPR>(dot) * r * a.inv_dim;  // mean(w g n)
-        // rows past the end hold zeros and add zeros
+        const float r = rsqrtf(row_sum<LPR>(ss.x + ss.y) * a.inv_dim + a.eps);
+        // n is x r: dx = r (w g) - n (r mean(w g n))
+        const float m = row_sum<LPR>(dot.x + dot.y) * r * a.inv_dim * r;
+        const float2 rr = both(r), mm = both(-m), keep = both(live ? r : 0.f);
 #pragma unroll
-        for (int i = 0; i < kP; ++i) {
-          const float p = n0[i] * r, q = n1[i] * r;
-          if (h0 + u * S < rw.heads) {
-            d0[i] += g0[i] * p;
-            d1[i] += g1[i] * q;
+        for (int i = 0; i < P / 2; ++i) {
+          if (live) {
+            d.a[i] = __ffma2_rn(g.a[i], __fmul2_rn(n.a[i], keep), d.a[i]);
+            d.b[i] = __ffma2_rn(g.b[i], __fmul2_rn(n.b[i], keep), d.b[i]);
           }
-          g0[i] = r * (w0[i] * g0[i] - p * mean);
-          g1[i] = r * (w1[i] * g1[i] - q * mean);
+          g.a[i] = __ffma2_rn(__fmul2_rn(n.a[i], rr), mm, __fmul2_rn(wg.a[i], rr));
+          g.b[i] = __ffma2_rn(__fmul2_rn(n.b[i], rr), mm, __fmul2_rn(wg.b[i], rr));
         }
       }
-      if (h0 + u * S < rw.heads) {
-        T* row = reinterpret_cast<T*>(dx + u * S * rw.yh);
-        *reinterpret_cast<V*>(row + ln.e0) = pack<T>(g0);
-        *reinterpret_cast<V*>(row + ln.e1) = pack<T>(g1);
+      if (live) {
+        uint4 y0, y1;
+        store_pairs<T, P, INTER>(g, y0, y1);
+        T* row = reinterpret_cast<T*>(rw.y + at.t * rw.yt + h * rw.yh);
+        *reinterpret_cast<uint4*>(row + ln.e0) = y0;
+        *reinterpret_cast<uint4*>(row + ln.e1) = y1;
       }
     }
+    at.task += step;
+    at.start(total, parts, groups);
   }
+  cp_async_wait<0>();
   if (!norm) return;
+  __syncthreads();  // the ring becomes the place of the block's sums
+  float* acc = reinterpret_cast<float*>(smem);
+  float d0[P], d1[P];
+  from_pairs<P, INTER>(d, d0, d1);
 #pragma unroll
-  for (int i = 0; i < kP; ++i) {
+  for (int i = 0; i < P; ++i) {
 #pragma unroll
     for (int o = LPR; o < 32; o <<= 1) {
       d0[i] += __shfl_xor_sync(0xffffffffu, d0[i], o);
       d1[i] += __shfl_xor_sync(0xffffffffu, d1[i], o);
     }
     if (lane < LPR) {
-      acc[warp][ln.e0 + i] = d0[i];
-      acc[warp][ln.e1 + i] = d1[i];
+      acc[warp * a.dim + ln.e0 + i] = d0[i];
+      acc[warp * a.dim + ln.e1 + i] = d1[i];
     }
   }
   __syncthreads();
   for (int e = threadIdx.x; e < a.dim; e += blockDim.x) {
     float s = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) s += acc[w][e];
+    for (int w = 0; w < kGradWarps; ++w) s += acc[w * a.dim + e];
     part[(int64_t)blockIdx.x * a.dim + e] = s;
   }
 }
@@ -674,13 +839,13 @@ unsigned row_blocks(int64_t rows) {
   return (unsigned)(want < cap ? want : cap);
 }
 
-// Lanes a row of the vector kernels, 0 where they do not fit: whole vectors
-// of 4 elements in every part of a head, rows, tables and weights aligned to
-// them, and fewer than 2^31 tasks.
-int vec_lanes(const RotArgs& a, int dtype, bool grad) {
-  const int half = a.dim / 2, lanes = half / kP;
-  if (half % kP || (a.rot / 2) % kP || lanes > 32 || (lanes & (lanes - 1))) return 0;
-  const int64_t unit = 4 * dtype_size(dtype);
+// Lanes a row for `pairs` pairs a lane, 0 where that does not fit: whole
+// vectors of `pairs` elements in every part of a head, rows, tables and
+// weights aligned to them, and fewer than 2^31 tasks.
+int vec_lanes(const RotArgs& a, int dtype, int pairs, bool grad) {
+  const int half = a.dim / 2, lanes = half / pairs;
+  if (half % pairs || (a.rot / 2) % pairs || lanes > 32 || (lanes & (lanes - 1))) return 0;
+  const int64_t unit = pairs * dtype_size(dtype);
   auto al = [](const void* x, int64_t t, int64_t h, int64_t unit) {
     return reinterpret_cast<uintptr_t>(x) % unit == 0 && t % unit == 0 && h % unit == 0;
   };
@@ -746,7 +911,7 @@ extern "C" int cs_qk_norm_rope(const cs_rotary_params* p, void* stream) {
   if (int rc = make_args(p, a, true)) return rc;
   const int64_t rows = p->tokens * (p->q_heads + p->k_heads);
   if (rows == 0) return CS_OK;
-  if (const int lanes = vec_lanes(a, p->dtype, false))
+  if (const int lanes = vec_lanes(a, p->dtype, kP, false))
     return launch_vec(a, nullptr, p->dtype, lanes, as_stream(stream));
   return by_type(p->dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
@@ -756,7 +921,7 @@ extern "C" int cs_qk_norm_rope(const cs_rotary_params* p, void* stream) {
 
 extern "C" int64_t cs_qk_norm_rope_grad_workspace(const cs_rotary_params* p) {
   if (p == nullptr || p->head_dim <= 0 || p->head_dim > cs::kMaxDim) return 0;
-  return (cs::kGradBlocks + 1ll) * p->head_dim * (int64_t)sizeof(float);
+  return (int64_t)cs::kGradBlocks * p->head_dim * (int64_t)sizeof(float);
 }
 
 extern "C" int cs_qk_norm_rope_grad(const cs_rotary_params* p, const void* q_dy, const void* k_dy,
@@ -769,26 +934,34 @@ extern "C" int cs_qk_norm_rope_grad(const cs_rotary_params* p, const void* q_dy,
   CS_HOST_CHECK(p->tokens == 0 || ((p->q_heads == 0 || q_dy) && (p->k_heads == 0 || k_dy)));
   a.q.dy = static_cast<const char*>(q_dy);
   a.k.dy = static_cast<const char*>(k_dy);
-  // blocks in proportion to the heads, no more than the rows fill
+  // blocks in proportion to the heads, no more than the rows fill; where the
+  // tokens alone do not fill them, a token's row groups go to several warps
   const int heads = p->q_heads + p->k_heads;
-  const int lanes = vec_lanes(a, p->dtype, true);
-  const int per = lanes ? 32 / lanes * kGradGroups : 1;  // rows a warp takes at once
-  auto share = [&](int h) {
-    const int64_t most = heads ? ((int64_t)kGradBlocks * h + heads - 1) / heads : 0;
-    const int64_t want = (p->tokens * ((h + per - 1) / per) + 7) / 8;
-    return (int)std::max<int64_t>(1, std::min(most, want));
+  const int lanes = vec_lanes(a, p->dtype, 16 / (int)dtype_size(p->dtype), true);
+  const int groups = lanes ? (std::max(p->q_heads, p->k_heads) * lanes + 31) / 32 : 1;
+  const int64_t fill = (int64_t)kGradBlocks * kGradWarps;
+  const int parts = (int)std::max<int64_t>(
+      1, std::min<int64_t>(groups, p->tokens ? fill / p->tokens : 1));
+  const int most_q = heads && p->k_heads ? (int)((int64_t)kGradBlocks * p->q_heads / heads)
+                                         : kGradBlocks - 1;
+  auto share = [&](int h, int most) {
+    const int64_t want = ((lanes ? p->tokens * parts : p->tokens * h) + 7) / 8;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(most, want));
   };
-  const int nq = share(p->q_heads), n = nq + share(p->k_heads);
+  const int nq = share(p->q_heads, most_q);
+  const int n = nq + share(p->k_heads, kGradBlocks - std::max(most_q, 1));
   const int rc = by_type(p->dtype, [&](auto* ty) {
     using T = std::remove_pointer_t<decltype(ty)>;
     float* part = static_cast<float*>(workspace);
     if (lanes)
       by_lanes(lanes, [&](auto l) {
-        constexpr int L = decltype(l)::value;
-        if (a.interleaved)
-          norm_rope_grad_vec_kernel<T, L, true><<<n, 256, 0, as_stream(stream)>>>(a, nq, part);
-        else
-          norm_rope_grad_vec_kernel<T, L, false><<<n, 256, 0, as_stream(stream)>>>(a, nq, part);
+        auto go = [&](auto inter) {
+          auto kernel = norm_rope_grad_kernel<T, decltype(l)::value, decltype(inter)::value>;
+          constexpr int kBytes = kGradWarps * kGradRing * 4 * 32 * 16;
+          kernel<<<n, kGradWarps * 32, kBytes, as_stream(stream)>>>(a, nq, parts, part);
+        };
+        if (a.interleaved) go(std::true_type());
+        else go(std::false_type());
       });
     else
       norm_rope_grad_rows_kernel<T><<<n, kRowWarps * 32, 0, as_stream(stream)>>>(a, nq, part);
@@ -821,7 +994,7 @@ extern "C" int cs_kv_append_rotated(const cs_rotary_params* p, const cs_paged_kv
     RotArgs d = a;  // k has no dense output
     d.k.y = nullptr;
     d.k.yt = d.k.yh = 0;
-    if (const int lanes = vec_lanes(d, p->dtype, false)) {
+    if (const int lanes = vec_lanes(d, p->dtype, kP, false)) {
       int shift = -1;
       for (int s = 0; s < 31; ++s)
         if ((int64_t)1 << s == kv->block_size) shift = s;
