@@ -11,6 +11,8 @@
 // Bound: HBM.  Each element is read once and written once (16-bit: 4 bytes
 // an element and direction); the arithmetic is about ten operations an
 // element.
+#include <math.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -22,7 +24,7 @@ namespace {
 
 constexpr int kMaxDim = 512;
 constexpr int kMaxPairs = kMaxDim / 2 / 32;  // pairs a lane of a warp-per-row kernel
-constexpr int kGradBlocks = 296;             // 148 SMs x 2: the fixed partition of dw
+constexpr int kStreamBlocks = 296;           // 148 SMs x 2: the fixed partition of the gradient
 constexpr int kRowWarps = 8;
 
 struct Rows {
@@ -585,27 +587,25 @@ __device__ __forceinline__ Lane lane_of16(const RotArgs& a, int l) {
   }
   return n;
 }
-template <int P, bool INTER>
-__device__ __forceinline__ void load_weights(const void* w, int dtype, const Lane& ln,
-                                             Pairs<P>& p) {
-  float u[P], v[P];
-#pragma unroll
-  for (int i = 0; i < P / 4; ++i) {
-    weights_at(w, dtype, ln.e0 + 4 * i, u + 4 * i);
-    weights_at(w, dtype, ln.e1 + 4 * i, v + 4 * i);
-  }
-  to_pairs<P, INTER>(u, v, p);
-}
-template <int P>
-__device__ __forceinline__ void load_angles(const RotArgs& a, int64_t pos, int p0, float2* c,
-                                            float2* s) {
-#pragma unroll
-  for (int i = 0; i < P / 4; ++i)
-    angles(a, pos, p0 + 4 * i, reinterpret_cast<float*>(c + 2 * i),
-           reinterpret_cast<float*>(s + 2 * i));
-}
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 __device__ __forceinline__ float2 neg(float2 x) { return make_float2(-x.x, -x.y); }
+
+// P floats of shared memory, 16-byte aligned
+template <int P>
+__device__ __forceinline__ void load_floats(const float* src, float* f) {
+#pragma unroll
+  for (int i = 0; i < P / 4; ++i) {
+    const float4 v = reinterpret_cast<const float4*>(src)[i];
+    f[4 * i] = v.x, f[4 * i + 1] = v.y, f[4 * i + 2] = v.z, f[4 * i + 3] = v.w;
+  }
+}
+template <int P, bool INTER>
+__device__ __forceinline__ void shared_weights(const float* w, const Lane& ln, Pairs<P>& p) {
+  float u[P], v[P];
+  load_floats<P>(w + ln.e0, u);
+  load_floats<P>(w + ln.e1, v);
+  to_pairs<P, INTER>(u, v, p);
+}
 
 // a warp's place in its share: row group u of a part of token t
 struct Place {
@@ -623,109 +623,172 @@ struct Place {
 // Gradient: blocks below nq take tokens of q, the rest tokens of k, each warp
 // every W-th (token, part of its heads), a fixed share; dw of a lane's
 // elements stays in its registers, then lanes, warps and (in
-// grad_weight_kernel) blocks are added in order.
-constexpr int kGradWarps = 8;
-constexpr int kGradRing = 3;  // row groups in flight a warp, 2 KB each
+// grad_weight_kernel) blocks are added in order.  Angles come with the rows
+// of a token's first group, weights lie in shared memory.
+//
+// 32768 tokens of 32/8 heads of 128, bf16: 187 us, 5.4 TB/s.  Tried: plain loads of 4
+// pairs a lane, two row groups in flight, three blocks an SM (286 us); this
+// ring with 80 registers and three blocks (325 us: spills); the same ring for
+// the forward (119 us against 123 us with plain loads, but 167 us where pairs
+// are interleaved), so the forward stays with plain loads.
+constexpr int kStreamWarps = 8;
+constexpr int kRing = 4;  // row groups a warp has in flight, one being read
+
+template <typename T, int LPR>
+struct Stream {
+  static constexpr int P = kPairs<T>, kDim = 2 * P * LPR;
+  static constexpr int kVecs = 4;  // x0, x1, dy0, dy1
+  // 16-byte units: rows [ring][vector][lane], angles [ring][cos, sin][dim / 2],
+  // a warp each; then the weights, a block
+  static constexpr int kRows = kRing * kVecs * 32, kAngles = kRing * (kDim / 4);
+  static constexpr int kWarp = kRows + kAngles;
+  static constexpr int kUnits = kStreamWarps * kWarp + kDim / 4;
+  static_assert(kStreamWarps * kDim <= kStreamWarps * kWarp * 4, "dw sums alias the ring");
+};
 
 template <typename T, int LPR, bool INTER>
-__global__ void __launch_bounds__(kGradWarps * 32, 2)
+__global__ void __launch_bounds__(kStreamWarps * 32, 2)
     norm_rope_grad_kernel(const __grid_constant__ RotArgs a, int nq, int most_parts,
                           float* __restrict__ part) {
-  constexpr int P = kPairs<T>, S = 32 / LPR, R = kGradRing;
+  using St = Stream<T, LPR>;
+  constexpr int P = St::P, S = 32 / LPR, D = St::kDim;
   extern __shared__ uint4 smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  // [ring slot][x0, x1, dy0, dy1][lane]
-  uint4* ring = smem + warp * (R * 4 * 32) + lane;
+  uint4* ring = smem + warp * St::kWarp + lane;
   const uint32_t ring_at = smem_u32(ring);
+  float* ang = reinterpret_cast<float*>(smem + warp * St::kWarp + St::kRows);
+  const uint32_t ang_at = smem_u32(ang);
+  float* wsm = reinterpret_cast<float*>(smem + kStreamWarps * St::kWarp);
   const bool isk = (int)blockIdx.x >= nq;
   const Rows& rw = isk ? a.k : a.q;
-  const int b = isk ? blockIdx.x - nq : blockIdx.x;
-  const unsigned step = (isk ? gridDim.x - nq : nq) * kGradWarps;
+  const int first = isk ? nq : 0;
+  const unsigned step = (isk ? gridDim.x - nq : nq) * kStreamWarps;
   const Lane ln = lane_of16<P, INTER>(a, lane % LPR);
   const bool norm = rw.w != nullptr;
-  Pairs<P> w, d;
+  const int half = a.rot >> 1;
+  for (int e = threadIdx.x; e < D; e += blockDim.x)
+    wsm[e] = norm ? load_weight(rw.w, a.wdtype, e) : 1.f;
+  __syncthreads();
+
+  Pairs<P> d;
 #pragma unroll
-  for (int i = 0; i < P / 2; ++i) w.a[i] = w.b[i] = d.a[i] = d.b[i] = both(0.f);
-  if (norm) load_weights<P, INTER>(rw.w, a.wdtype, ln, w);
+  for (int i = 0; i < P / 2; ++i) d.a[i] = d.b[i] = both(0.f);
   const int groups = (rw.heads + S - 1) / S;
   // no part is empty: q and k have different numbers of groups
   const unsigned parts = most_parts < groups ? most_parts : groups;
   const unsigned total = (unsigned)a.tokens * parts;
-  Place in{(unsigned)b * kGradWarps + warp, 0, 0, 0};
+  Place in{(unsigned)(blockIdx.x - first) * kStreamWarps + warp, 0, 0, 0};
   in.start(total, parts, groups);
   Place at = in;
-  auto issue = [&](int slot) {
+  // the position of the token that `in` comes to next, read a task ahead
+  int64_t pos = in.task < total ? a.positions[in.t] : 0;
+  bool fresh = true;  // `in` is at a task's first group
+  int in_slot = 0, in_ang = 0;
+  // interleaved pairs: a lane's two vectors are neighbours, so each copy takes
+  // half of every 32-byte sector and the other half should hit L1
+  auto copy = [&](uint32_t dst, const T* src) {
+    if constexpr (INTER)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else
+      cp_async16(dst, src, true);
+  };
+  auto issue = [&]() {
     if (in.task < total) {
+      if (fresh) {
+        const bool ok = pos >= 0 && pos < a.table_rows;
+        if (!ok && lane == 0 && in.u == 0) report(a.status, CS_ST_POS_RANGE);
+        for (int i = lane; i < half / 2; i += 32) {
+          // units of 4 angles: half / 4 of cos, as many of sin
+          const bool sn = i >= half / 4;
+          const int e = 4 * (sn ? i - half / 4 : i), to = in_ang * D + (sn ? D / 2 : 0) + e;
+          if (ok)
+            cp_async16(ang_at + to * 4, (sn ? a.sin : a.cos) + pos * a.table_stride + e, true);
+          else
+            *reinterpret_cast<float4*>(ang + to) = make_float4(NAN, NAN, NAN, NAN);
+        }
+        const unsigned ahead = in.task + step;
+        if (ahead < total) pos = a.positions[ahead / parts];
+        in_ang = in_ang == kRing - 1 ? 0 : in_ang + 1;
+        fresh = false;
+      }
       const int h = in.u * S + lane / LPR;
       if (h < rw.heads) {
-        const uint32_t to = ring_at + slot * (4 * 32 * 16);
-        const T* dy = reinterpret_cast<const T*>(rw.dy + in.t * rw.yt + h * rw.yh);
-        cp_async16(to + 2 * 512, dy + ln.e0, true);
-        cp_async16(to + 3 * 512, dy + ln.e1, true);
+        const uint32_t to = ring_at + in_slot * (St::kVecs * 512);
         if (norm) {
           const T* x = reinterpret_cast<const T*>(rw.x + in.t * rw.xt + h * rw.xh);
-          cp_async16(to, x + ln.e0, true);
-          cp_async16(to + 512, x + ln.e1, true);
+          copy(to, x + ln.e0);
+          copy(to + 512, x + ln.e1);
         }
+        const T* dy = reinterpret_cast<const T*>(rw.dy + in.t * rw.yt + h * rw.yh);
+        copy(to + 1024, dy + ln.e0);
+        copy(to + 1536, dy + ln.e1);
       }
       if (++in.u == in.end) {
         in.task += step;
         in.start(total, parts, groups);
+        fresh = true;
       }
     }
     cp_async_commit();
+    in_slot = in_slot == kRing - 1 ? 0 : in_slot + 1;
   };
 #pragma unroll
-  for (int r = 0; r < R - 1; ++r) issue(r);
-  int slot = 0;
+  for (int r = 0; r < kRing - 1; ++r) issue();
+
+  int slot = 0, aslot = 0;
   while (at.task < total) {
-    const int64_t pos = a.positions[at.t];
-    if (lane == 0 && (pos < 0 || pos >= a.table_rows)) report(a.status, CS_ST_POS_RANGE);
-    float2 c[P / 2], s[P / 2];
-    if (ln.turns) load_angles<P>(a, pos, ln.p0, c, s);
+    const float* cs = ang + aslot * D + ln.p0;
+    aslot = aslot == kRing - 1 ? 0 : aslot + 1;
     for (; at.u < at.end; ++at.u) {
-      cp_async_wait<R - 2>();
-      const uint4* mine = ring + slot * (4 * 32);
-      Pairs<P> g, n;
-      load_pairs<T, P, INTER>(mine[64], mine[96], g);
-      if (norm) load_pairs<T, P, INTER>(mine[0], mine[32], n);
-      // the slot read in the last round is free
-      issue(slot == 0 ? R - 1 : slot - 1);
-      slot = slot == R - 1 ? 0 : slot + 1;
+      cp_async_wait<kRing - 2>();
+      __syncwarp();  // the angles are the warp's
+      const uint4* mine = ring + slot * (St::kVecs * 32);
+      slot = slot == kRing - 1 ? 0 : slot + 1;
       const int h = at.u * S + lane / LPR;
       const bool live = h < rw.heads;
+      Pairs<P> g, n, w;
+      load_pairs<T, P, INTER>(mine[64], mine[96], g);
+      if (norm) load_pairs<T, P, INTER>(mine[0], mine[32], n);
       if (ln.turns) {
+        float cv[P], sv[P];
+        load_floats<P>(cs, cv);
+        load_floats<P>(cs + D / 2, sv);
 #pragma unroll
         for (int i = 0; i < P / 2; ++i) {
-          const float2 t = __ffma2_rn(g.a[i], c[i], __fmul2_rn(g.b[i], s[i]));
-          g.b[i] = __ffma2_rn(g.b[i], c[i], __fmul2_rn(g.a[i], neg(s[i])));
+          const float2 c = make_float2(cv[2 * i], cv[2 * i + 1]);
+          const float2 s = make_float2(sv[2 * i], sv[2 * i + 1]);
+          const float2 t = __ffma2_rn(g.a[i], c, __fmul2_rn(g.b[i], s));
+          g.b[i] = __ffma2_rn(g.b[i], c, neg(__fmul2_rn(g.a[i], s)));
           g.a[i] = t;
         }
       }
+      issue();  // into the slot read in the last round
       if (norm) {
-        Pairs<P> wg;
         float2 ss = both(0.f), dot = both(0.f);
+        shared_weights<P, INTER>(wsm, ln, w);
 #pragma unroll
         for (int i = 0; i < P / 2; ++i) {
+          w.a[i] = __fmul2_rn(w.a[i], g.a[i]);
+          w.b[i] = __fmul2_rn(w.b[i], g.b[i]);
           ss = __ffma2_rn(n.a[i], n.a[i], ss);
           ss = __ffma2_rn(n.b[i], n.b[i], ss);
-          wg.a[i] = __fmul2_rn(w.a[i], g.a[i]);
-          wg.b[i] = __fmul2_rn(w.b[i], g.b[i]);
-          dot = __ffma2_rn(wg.a[i], n.a[i], dot);
-          dot = __ffma2_rn(wg.b[i], n.b[i], dot);
+          dot = __ffma2_rn(w.a[i], n.a[i], dot);
+          dot = __ffma2_rn(w.b[i], n.b[i], dot);
         }
         const float r = rsqrtf(row_sum<LPR>(ss.x + ss.y) * a.inv_dim + a.eps);
         // n is x r: dx = r (w g) - n (r mean(w g n))
         const float m = row_sum<LPR>(dot.x + dot.y) * r * a.inv_dim * r;
-        const float2 rr = both(r), mm = both(-m), keep = both(live ? r : 0.f);
+        const float2 rr = both(r), mm = both(-m);
 #pragma unroll
         for (int i = 0; i < P / 2; ++i) {
+          n.a[i] = __fmul2_rn(n.a[i], rr);
+          n.b[i] = __fmul2_rn(n.b[i], rr);
           if (live) {
-            d.a[i] = __ffma2_rn(g.a[i], __fmul2_rn(n.a[i], keep), d.a[i]);
-            d.b[i] = __ffma2_rn(g.b[i], __fmul2_rn(n.b[i], keep), d.b[i]);
+            d.a[i] = __ffma2_rn(g.a[i], n.a[i], d.a[i]);
+            d.b[i] = __ffma2_rn(g.b[i], n.b[i], d.b[i]);
           }
-          g.a[i] = __ffma2_rn(__fmul2_rn(n.a[i], rr), mm, __fmul2_rn(wg.a[i], rr));
-          g.b[i] = __ffma2_rn(__fmul2_rn(n.b[i], rr), mm, __fmul2_rn(wg.b[i], rr));
+          g.a[i] = __ffma2_rn(n.a[i], mm, __fmul2_rn(w.a[i], rr));
+          g.b[i] = __ffma2_rn(n.b[i], mm, __fmul2_rn(w.b[i], rr));
         }
       }
       if (live) {
@@ -753,16 +816,16 @@ __global__ void __launch_bounds__(kGradWarps * 32, 2)
       d1[i] += __shfl_xor_sync(0xffffffffu, d1[i], o);
     }
     if (lane < LPR) {
-      acc[warp * a.dim + ln.e0 + i] = d0[i];
-      acc[warp * a.dim + ln.e1 + i] = d1[i];
+      acc[warp * D + ln.e0 + i] = d0[i];
+      acc[warp * D + ln.e1 + i] = d1[i];
     }
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < a.dim; e += blockDim.x) {
+  for (int e = threadIdx.x; e < D; e += blockDim.x) {
     float s = 0.f;
 #pragma unroll
-    for (int w = 0; w < kGradWarps; ++w) s += acc[w * a.dim + e];
-    part[(int64_t)blockIdx.x * a.dim + e] = s;
+    for (int w = 0; w < kStreamWarps; ++w) s += acc[w * D + e];
+    part[(int64_t)blockIdx.x * D + e] = s;
   }
 }
 
@@ -882,6 +945,29 @@ void by_lanes(int lanes, F f) {
   }
 }
 
+// The streamed kernel's blocks: in proportion to the kinds' heads, no more
+// than the rows fill; where the tokens alone do not fill them, a token's row
+// groups go to several warps.
+struct Shares {
+  int nq, n, parts;
+};
+Shares shares(const RotArgs& a, int lanes) {
+  const int hq = a.q.heads, hk = a.k.heads, heads = hq + hk;
+  const int groups = std::max(1, (std::max(hq, hk) * lanes + 31) / 32);
+  const int64_t fill = (int64_t)kStreamBlocks * kStreamWarps;
+  Shares s;
+  s.parts = (int)std::max<int64_t>(1, std::min<int64_t>(groups, fill / a.tokens));
+  const int64_t want = (a.tokens * s.parts + kStreamWarps - 1) / kStreamWarps;
+  auto blocks = [&](int h) {
+    if (h == 0) return 0;
+    const int64_t most = std::max<int64_t>(1, (int64_t)kStreamBlocks * h / heads);
+    return (int)std::min(most, want);
+  };
+  s.nq = blocks(hq);
+  s.n = s.nq + blocks(hk);
+  return s;
+}
+
 int launch_vec(const RotArgs& a, const AppendArgs* ap, int dtype, int lanes, cudaStream_t stream) {
   const int64_t tasks = a.tokens * (tasks_of(a.q.heads, lanes) +
                                     (ap ? 2 : 1) * tasks_of(a.k.heads, lanes));
@@ -921,7 +1007,7 @@ extern "C" int cs_qk_norm_rope(const cs_rotary_params* p, void* stream) {
 
 extern "C" int64_t cs_qk_norm_rope_grad_workspace(const cs_rotary_params* p) {
   if (p == nullptr || p->head_dim <= 0 || p->head_dim > cs::kMaxDim) return 0;
-  return (int64_t)cs::kGradBlocks * p->head_dim * (int64_t)sizeof(float);
+  return (int64_t)cs::kStreamBlocks * p->head_dim * (int64_t)sizeof(float);
 }
 
 extern "C" int cs_qk_norm_rope_grad(const cs_rotary_params* p, const void* q_dy, const void* k_dy,
@@ -934,38 +1020,49 @@ extern "C" int cs_qk_norm_rope_grad(const cs_rotary_params* p, const void* q_dy,
   CS_HOST_CHECK(p->tokens == 0 || ((p->q_heads == 0 || q_dy) && (p->k_heads == 0 || k_dy)));
   a.q.dy = static_cast<const char*>(q_dy);
   a.k.dy = static_cast<const char*>(k_dy);
-  // blocks in proportion to the heads, no more than the rows fill; where the
-  // tokens alone do not fill them, a token's row groups go to several warps
-  const int heads = p->q_heads + p->k_heads;
-  const int lanes = vec_lanes(a, p->dtype, 16 / (int)dtype_size(p->dtype), true);
-  const int groups = lanes ? (std::max(p->q_heads, p->k_heads) * lanes + 31) / 32 : 1;
-  const int64_t fill = (int64_t)kGradBlocks * kGradWarps;
-  const int parts = (int)std::max<int64_t>(
-      1, std::min<int64_t>(groups, p->tokens ? fill / p->tokens : 1));
-  const int most_q = heads && p->k_heads ? (int)((int64_t)kGradBlocks * p->q_heads / heads)
-                                         : kGradBlocks - 1;
-  auto share = [&](int h, int most) {
-    const int64_t want = ((lanes ? p->tokens * parts : p->tokens * h) + 7) / 8;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(most, want));
-  };
-  const int nq = share(p->q_heads, most_q);
-  const int n = nq + share(p->k_heads, kGradBlocks - std::max(most_q, 1));
-  const int rc = by_type(p->dtype, [&](auto* ty) {
-    using T = std::remove_pointer_t<decltype(ty)>;
-    float* part = static_cast<float*>(workspace);
-    if (lanes)
+  if (p->tokens == 0) {  // no rows: the sums are empty
+    if (qw || kw)
+      grad_weight_kernel<<<dim3((p->head_dim + 31) / 32, 2), dim3(32, 32), 0, as_stream(stream)>>>(
+          static_cast<const float*>(workspace), 0, 0, p->head_dim, p->weight_dtype,
+          qw ? q_dw : nullptr, kw ? k_dw : nullptr);
+    CS_LAUNCH_CHECK();
+    return CS_OK;
+  }
+  float* part = static_cast<float*>(workspace);
+  const int lanes = vec_lanes(a, p->dtype, 16 / dtype_size(p->dtype), true);
+  int nq, n, rc;
+  if (lanes) {
+    const Shares s = shares(a, lanes);
+    nq = s.nq, n = s.n;
+    rc = n == 0 ? CS_OK : by_type(p->dtype, [&](auto* ty) {
+      using T = std::remove_pointer_t<decltype(ty)>;
       by_lanes(lanes, [&](auto l) {
         auto go = [&](auto inter) {
-          auto kernel = norm_rope_grad_kernel<T, decltype(l)::value, decltype(inter)::value>;
-          constexpr int kBytes = kGradWarps * kGradRing * 4 * 32 * 16;
-          kernel<<<n, kGradWarps * 32, kBytes, as_stream(stream)>>>(a, nq, parts, part);
+          constexpr int L = decltype(l)::value;
+          auto kernel = norm_rope_grad_kernel<T, L, decltype(inter)::value>;
+          constexpr int kBytes = Stream<T, L>::kUnits * 16;
+          static const cudaError_t set =
+              cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+          (void)set;  // a failure shows at the launch
+          kernel<<<s.n, kStreamWarps * 32, kBytes, as_stream(stream)>>>(a, s.nq, s.parts, part);
         };
         if (a.interleaved) go(std::true_type());
         else go(std::false_type());
       });
-    else
+    });
+  } else {
+    const int hq = p->q_heads, heads = hq + p->k_heads;
+    auto share = [&](int h) {
+      return h == 0 ? 0
+                    : (int)std::min<int64_t>(std::max(1, (int)((int64_t)kStreamBlocks * h / heads)),
+                                             (p->tokens * h + kRowWarps - 1) / kRowWarps);
+    };
+    nq = share(hq), n = nq + share(p->k_heads);
+    rc = n == 0 ? CS_OK : by_type(p->dtype, [&](auto* ty) {
+      using T = std::remove_pointer_t<decltype(ty)>;
       norm_rope_grad_rows_kernel<T><<<n, kRowWarps * 32, 0, as_stream(stream)>>>(a, nq, part);
-  });
+    });
+  }
   if (rc != CS_OK || (!qw && !kw)) return rc;
   grad_weight_kernel<<<dim3((p->head_dim + 31) / 32, 2), dim3(32, 32), 0, as_stream(stream)>>>(
       static_cast<const float*>(workspace), nq, n, p->head_dim, p->weight_dtype,
