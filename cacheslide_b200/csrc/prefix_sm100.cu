@@ -74,7 +74,15 @@ struct Shape {
   static constexpr int KS = (D == 64 || NT == 2) ? 2 : 1;
   static constexpr int VS = KS;
   static constexpr int kSoft = 4 * NT;
-  static constexpr int kThreads = 32 * (kSoft + 2 + NT);
+  // one more warpgroup: K, V, NT MMA warps (and an idle one beside one tile)
+  static constexpr int kThreads = 128 * (NT + 1);
+  // registers a thread: at launch, then the softmax warpgroups' (a row's 128
+  // scores live in them) and the other warpgroup's
+  static constexpr int kLaunch = NT == 1 ? 128 : 168;
+  static constexpr int kSoftRegs = NT == 1 ? 184 : 200;
+  static constexpr int kOtherRegs = NT == 1 ? 72 : 96;
+  static_assert(128 * NT * kSoftRegs + 128 * kOtherRegs <= kThreads * kLaunch,
+                "register split exceeds the block's launch allocation");
   static constexpr uint32_t TB = kPrefixTile * D * 2;
   static constexpr uint32_t oQ = 0, oK = NT * TB, oV = oK + KS * TB, oMeta = oV + VS * TB;
   // barriers, 8 bytes each
@@ -86,6 +94,34 @@ struct Shape {
   static constexpr uint32_t kCols = 256 * NT;
   static constexpr uint32_t cS = 0, cO = 128 * NT;  // S of tile i at 128 i, O at cO + D i
 };
+
+// the larger of the two, NaN if either is
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+// 2^x of two finite numbers below 128 on the FMA units: x = i + f with i the
+// nearest integer (left in the low bits by adding 1.5 * 2^23), 2^f by the
+// polynomial of degree 5 of least relative error on [-1/2, 1/2] (a Remez
+// exchange in float64, coefficients rounded: 1.5e-7), i added to the
+// exponent.  Below -126 the result stays 2^-126.
+__device__ __forceinline__ float2 pow2_pair(float2 x) {
+  auto two = [](float c) { return make_float2(c, c); };
+  x = make_float2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+  const float2 t = __fadd2_rn(x, two(12582912.f));
+  const float2 r = __fadd2_rn(t, two(-12582912.f));
+  const float2 f = __ffma2_rn(r, two(-1.f), x);
+  float2 p = two(0x1.5c08e6p-10f);
+  p = __ffma2_rn(p, f, two(0x1.3d0c52p-7f));
+  p = __ffma2_rn(p, f, two(0x1.c6b6e4p-5f));
+  p = __ffma2_rn(p, f, two(0x1.ebf918p-3f));
+  p = __ffma2_rn(p, f, two(0x1.62e428p-1f));
+  p = __ffma2_rn(p, f, two(0x1.000002p+0f));
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+}
 
 struct Step {
   int base, n, own;  // first key, keys, 1: own keys
@@ -169,6 +205,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
   auto barPV = [&](int qt, int t) { return mb + Sh::bPV + 8 * (qt * Sh::VS + t % Sh::VS); };
 
   if (warp == Sh::kSoft || warp == Sh::kSoft + 1) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Sh::kOtherRegs));
     // ============================================== producers: K, then V warp
     const bool isv = warp != Sh::kSoft;
     const int ST = isv ? Sh::VS : Sh::KS;
@@ -274,6 +311,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     if (slot_bad) report(a.status, CS_ST_SLOT_RANGE);
 
   } else if (warp >= Sh::kSoft + 2) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Sh::kOtherRegs));
     // ==================================================== MMA, one warp a tile
     const int qt = warp - (Sh::kSoft + 2);
     if (lane == 0 && qt < tiles) {
@@ -318,7 +356,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     }
     __syncwarp();
 
-  } else if ((warp >> 2) < tiles) {
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Sh::kSoftRegs));
+    if ((warp >> 2) < tiles) {
     // ================================================== softmax, a thread a row
     const int qt = warp >> 2;
     const int r = (warp & 3) * 32 + lane;  // TMEM lane
@@ -417,7 +457,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       ok = __all_sync(~0u, mbar_wait(barS(qt, t), (t / Sh::KS) & 1, abort));
       if (!ok) continue;
       tc_fence_after();
-      uint32_t v[32];
+      uint32_t v[128];
       if (__all_sync(~0u, vhi <= vlo)) {  // nothing to see for these 32 rows
 #pragma unroll
         for (int c = 0; c < 16; ++c) v[c] = 0u;
@@ -428,21 +468,38 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
         mbar_arrive(mb + Sh::bP + 8 * qt);
         continue;
       }
-      float top = -INFINITY;
-#pragma unroll 1
-      for (int cc = 0; cc < 4; ++cc) {
-        const uint32_t bits = col_bits(vlo, vhi, 32 * cc);
-        if (__all_sync(~0u, bits == 0u)) continue;
-        CS_TMEM_LD32(sc + 32 * cc, v);
-        tmem_wait_ld();
-        if (__all_sync(~0u, bits == ~0u)) {
+      CS_TMEM_LD32(sc, v);
+      CS_TMEM_LD32(sc + 32, (v + 32));
+      CS_TMEM_LD32(sc + 64, (v + 64));
+      CS_TMEM_LD32(sc + 96, (v + 96));
+      tmem_wait_ld();
+      const bool whole = __all_sync(~0u, vlo <= 0 && vhi >= kPrefixTile);
+      if (!whole) {
 #pragma unroll
-          for (int c = 0; c < 32; ++c) top = fmaxf(top, __uint_as_float(v[c]));
-        } else {
+        for (int cc = 0; cc < 4; ++cc) {
+          const uint32_t bits = col_bits(vlo, vhi, 32 * cc);
 #pragma unroll
           for (int c = 0; c < 32; ++c)
-            top = fmaxf(top, (bits >> c) & 1u ? __uint_as_float(v[c]) : -INFINITY);
+            v[32 * cc + c] = (bits >> c) & 1u ? v[32 * cc + c] : 0xff800000u;  // -inf
         }
+      }
+      float top;
+      {
+        float m[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          m[k] = max_nan(__uint_as_float(v[k]), __uint_as_float(v[k + 4]));
+#pragma unroll
+        for (int c = 8; c < kPrefixTile; c += 8) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            m[k] = max_nan(m[k], max_nan(__uint_as_float(v[c + k]), __uint_as_float(v[c + k + 4])));
+        }
+        top = max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3]));
+      }
+      if (!(top < INFINITY)) {  // a NaN or +inf score makes the row NaN
+        lsum = __int_as_float(0x7fffffff);
+        top = -INFINITY;
       }
       const float top2 = top == -INFINITY ? -INFINITY : top * a.scale2;
       const bool grow = top2 > mref + kLazy || mref == -INFINITY;
@@ -451,47 +508,48 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
         if (!wait_pv(t - 1)) continue;
         const float f = rescale ? ex2(mref - top2) : 1.f;
         lsum *= f;
+        uint32_t o[16];
 #pragma unroll 1
-        for (int cc = 0; cc < D / 32; ++cc) {
-          CS_TMEM_LD32(oc + 32 * cc, v);
+        for (int cc = 0; cc < D / 16; ++cc) {
+          CS_TMEM_LD16(oc + 16 * cc, o);
           tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < 32; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * f);
-          CS_TMEM_ST32(oc + 32 * cc, v);
+          for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
+          CS_TMEM_ST16(oc + 16 * cc, o);
         }
         tmem_wait_st();
       }
       if (grow) mref = top2;
       // the largest weight so far is 2^up, or up to 2^kLazy more
       const float sub = (mref > -INFINITY ? mref : 0.f) - p_up<T>();
-      float s0 = 0.f, s1 = 0.f;
-#pragma unroll 1
+      const float2 scale = make_float2(a.scale2, a.scale2), off = make_float2(-sub, -sub);
+      // whole tiles of rows with a maximum may take part of their exponentials
+      // from the FMA units (pow2_pair does not reach 0 for masked scores)
+      const bool poly = whole && __all_sync(~0u, mref > -INFINITY);
+      float2 s0 = make_float2(0.f, 0.f), s1 = s0;
+#pragma unroll
       for (int cc = 0; cc < 4; ++cc) {
-        const uint32_t bits = col_bits(vlo, vhi, 32 * cc);
-        if (__all_sync(~0u, bits == 0u)) {
+        uint32_t* w = v + 32 * cc;
+        auto weight = [&](int c, bool fma_units) {
+          float2 x = __ffma2_rn(make_float2(__uint_as_float(w[2 * c]), __uint_as_float(w[2 * c + 1])),
+                                scale, off);
+          if (fma_units) x = pow2_pair(x);
+          else x = make_float2(ex2(x.x), ex2(x.y));
+          if (c & 1) s1 = __fadd2_rn(s1, x);
+          else s0 = __fadd2_rn(s0, x);
+          return Pack2<T>::pack(x.x, x.y);
+        };
+        uint32_t o[16];
+        if (poly) {
 #pragma unroll
-          for (int c = 0; c < 16; ++c) v[c] = 0u;
+          for (int c = 0; c < 16; ++c) o[c] = weight(c, c % 4 == 3);
         } else {
-          CS_TMEM_LD32(sc + 32 * cc, v);
-          tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < 32; ++c)
-            v[c] = __float_as_uint(ex2(fmaf(__uint_as_float(v[c]), a.scale2, -sub)));
-          if (!__all_sync(~0u, bits == ~0u)) {
-#pragma unroll
-            for (int c = 0; c < 32; ++c) v[c] = (bits >> c) & 1u ? v[c] : 0u;
-          }
-#pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            const float e0 = __uint_as_float(v[2 * c]), e1 = __uint_as_float(v[2 * c + 1]);
-            s0 += e0;
-            s1 += e1;
-            v[c] = Pack2<T>::pack(e0, e1);
-          }
+          for (int c = 0; c < 16; ++c) o[c] = weight(c, false);
         }
-        CS_TMEM_ST16(sc + 16 * cc, v);
+        CS_TMEM_ST16(sc + 16 * cc, o);
       }
-      lsum += s0 + s1;
+      lsum += (s0.x + s0.y) + (s1.x + s1.y);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(mb + Sh::bP + 8 * qt);
@@ -573,6 +631,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     if (row_ok && ok) {
       if (it.part >= 0) a.part_lse[prow] = lse2;
       else if (a.lse) a.lse[token * a.hq + h] = lse2 * kLn2;
+    }
     }
   }
 
@@ -658,9 +717,16 @@ bool setup_maps(PArgs& a, const cs_paged_kv& kv) {
 template <typename T, int D, int NT>
 int launch_main(const PArgs& a, int64_t blocks, cudaStream_t stream) {
   auto kernel = prefix_sm100_kernel<T, D, NT>;
-  static const cudaError_t set = cudaFuncSetAttribute(
-      kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D, NT>::kSmem);
-  if (set != cudaSuccess) return CS_ERR_CUDA;
+  // once per kernel: the register split inside it (setmaxnreg) is only sound
+  // when the block was launched with the registers it assumes
+  static const bool ready = [&] {
+    cudaFuncAttributes at;
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                Shape<D, NT>::kSmem) == cudaSuccess &&
+           cudaFuncGetAttributes(&at, kernel) == cudaSuccess &&
+           at.numRegs == Shape<D, NT>::kLaunch;
+  }();
+  if (!ready) return CS_ERR_CUDA;
   kernel<<<(unsigned)blocks, Shape<D, NT>::kThreads, Shape<D, NT>::kSmem, stream>>>(a);
   CS_LAUNCH_CHECK();
   return CS_OK;
@@ -720,8 +786,9 @@ int prefix_attn_sm100(const cs_prefix_params& p, const cs_prefix_plan_info& info
   for (int s = 0; s < 31; ++s)
     if ((int64_t)1 << s == kv.block_size) a.bs_shift = s;
   a.neg = p.scale < 0.0;
-  a.scale2 = fabsf((float)p.scale) * kLog2e;
-  a.scale_signed2 = (float)p.scale * kLog2e;
+  // masked scores are -inf before they are scaled, so the factor is never 0
+  a.scale2 = fmaxf(fabsf((float)p.scale) * kLog2e, 1e-30f);
+  a.scale_signed2 = a.neg ? -a.scale2 : a.scale2;
   a.nrb = a.nrh = a.nro = a.srr = a.srh = 0;
   a.tma = setup_maps(a, kv) ? 1 : 0;
   const bool half = kv.dtype == CS_F16;
