@@ -87,8 +87,8 @@ struct Shape {
   static constexpr uint32_t oQ = 0, oK = NT * TB, oV = oK + KS * TB, oMeta = oV + VS * TB;
   // barriers, 8 bytes each
   static constexpr uint32_t bQ = 0, bK = 8, bV = bK + 8 * KS, bS = bV + 8 * VS,
-                            bP = bS + 8 * NT * KS, bPV = bP + 8 * NT, bEnd = bPV + 8 * NT * VS,
-                            oTmem = bEnd + 8, oAbort = oTmem + 4, oBad = oAbort + 4,
+                            bP = bS + 8 * NT * KS, bPV = bP + 8 * NT, bTurn = bPV + 8 * NT * VS,
+                            oTmem = bTurn + 16, oAbort = oTmem + 4, oBad = oAbort + 4,
                             kMeta = oBad + 2 * NT * 16;
   static constexpr uint32_t kSmem = oMeta + kMeta + 1024;  // the base is rounded up to 1024
   static constexpr uint32_t kCols = 256 * NT;
@@ -99,6 +99,12 @@ struct Shape {
 __device__ __forceinline__ float max_nan(float a, float b) {
   float y;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
 
@@ -193,6 +199,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     for (int s = 0; s < NT * Sh::KS; ++s) mbar_init(mb + Sh::bS + 8 * s, 1);
     for (int s = 0; s < NT; ++s) mbar_init(mb + Sh::bP + 8 * s, 128);
     for (int s = 0; s < NT * Sh::VS; ++s) mbar_init(mb + Sh::bPV + 8 * s, 1);
+    mbar_init(mb + Sh::bTurn, 128);
+    mbar_init(mb + Sh::bTurn + 8, 128);
     *abort = 0;
     mbar_init_fence();
   }
@@ -399,6 +407,12 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     float mref = -INFINITY, lsum = 0.f;  // log2 domain; P = 2^(x - mref + up)
     bool ok = true;
     int checked = 0;
+    // The tiles' softmaxes take turns, so that one tile's products run beside
+    // the other's softmax: in step, both share the issue slots, then both wait
+    // for the tensor unit (5850 clocks a key tile of 2 x 128 rows).
+    auto pass_turn = [&] {
+      if (tiles == 2) mbar_arrive(mb + Sh::bTurn + 8 * (1 - qt));
+    };
     auto wait_pv = [&](int t) {
       ok = __all_sync(~0u, mbar_wait(barPV(qt, t), (t / Sh::VS) & 1, abort));
       tc_fence_after();
@@ -457,6 +471,12 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       ok = __all_sync(~0u, mbar_wait(barS(qt, t), (t / Sh::KS) & 1, abort));
       if (!ok) continue;
       tc_fence_after();
+      if (tiles == 2) {
+        if (qt == 1 || t > 0) {
+          ok = __all_sync(~0u, mbar_wait(mb + Sh::bTurn + 8 * qt, (qt ? t : t - 1) & 1, abort));
+          if (!ok) continue;
+        }
+      }
       uint32_t v[128];
       if (__all_sync(~0u, vhi <= vlo)) {  // nothing to see for these 32 rows
 #pragma unroll
@@ -466,6 +486,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(mb + Sh::bP + 8 * qt);
+        pass_turn();
         continue;
       }
       CS_TMEM_LD32(sc, v);
@@ -493,9 +514,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
         for (int c = 8; c < kPrefixTile; c += 8) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            m[k] = max_nan(m[k], max_nan(__uint_as_float(v[c + k]), __uint_as_float(v[c + k + 4])));
+            m[k] = max3_nan(m[k], __uint_as_float(v[c + k]), __uint_as_float(v[c + k + 4]));
         }
-        top = max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3]));
+        top = max_nan(max3_nan(m[0], m[1], m[2]), m[3]);
       }
       if (!(top < INFINITY)) {  // a NaN or +inf score makes the row NaN
         lsum = __int_as_float(0x7fffffff);
@@ -553,6 +574,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(mb + Sh::bP + 8 * qt);
+      pass_turn();
 
       if (bad[0] | bad[1] | bad[2] | bad[3]) {
         if (!wait_pv(t)) continue;
