@@ -154,6 +154,23 @@ __device__ __forceinline__ void mbar_arrive_tx(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
                : "memory");
 }
+// the same lane of a whole warp every time
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+// mbar_wait for a whole warp that must see the phase at once: it polls instead
+// of being suspended
+__device__ __forceinline__ bool mbar_spin(uint32_t bar, uint32_t parity, volatile int* abort) {
+  for (int i = 0; i < 64; ++i)
+    if (__all_sync(~0u, mbar_test(bar, parity))) return true;
+  return __all_sync(~0u, mbar_wait(bar, parity, abort));
+}
 __device__ __forceinline__ void st_shared16(uint32_t dst, uint4 v) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z),
                "r"(v.w)
@@ -321,40 +338,52 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
   } else if (warp >= Sh::kSoft + 2) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Sh::kOtherRegs));
     // ==================================================== MMA, one warp a tile
-    const int qt = warp - (Sh::kSoft + 2);
-    if (lane == 0 && qt < tiles) {
+    // The whole warp walks the steps, so that descriptors stay in uniform
+    // registers; one elected lane issues.  (One lane alone, with descriptors
+    // built for each product, took 90 clocks a product of 64.)
+    const int qt = __shfl_sync(~0u, warp, 0) - (Sh::kSoft + 2);
+    if (qt < tiles) {
+      const bool leader = elect_one();
       const uint32_t id_s = umma_idesc(128, 128, umma_format<T>(), 0, 0);
       const uint32_t id_o = umma_idesc(128, D, umma_format<T>(), 0, 1);  // V is MN-major
-      const uint32_t qa = sbase + Sh::oQ + qt * Sh::TB;
-      const uint32_t sc = tmem + Sh::cS + 128 * qt, oc = tmem + Sh::cO + D * qt;
-      bool ok = mbar_wait(mb + Sh::bQ, 0, abort);
+      const uint64_t dq = umma_desc(sbase + Sh::oQ + qt * Sh::TB, 16, 1024);
+      const uint64_t dk0 = umma_desc(sbase + Sh::oK, 16, 1024);
+      const uint64_t dv0 = umma_desc(sbase + Sh::oV, 16384, 1024);
+      const uint32_t tm = __shfl_sync(~0u, tmem, 0);
+      const uint32_t sc = tm + Sh::cS + 128 * qt, oc = tm + Sh::cO + D * qt;
+      bool ok = mbar_spin(mb + Sh::bQ, 0, abort);
       uint32_t last = 0, lastph = 0;  // the newest group issued
       for (int t = 0; ok && t < steps; ++t) {
-        const uint32_t kb = sbase + Sh::oK + (t % Sh::KS) * Sh::TB;
-        const uint32_t vb = sbase + Sh::oV + (t % Sh::VS) * Sh::TB;
-        if (!(ok = mbar_wait(mb + Sh::bK + 8 * (t % Sh::KS), (t / Sh::KS) & 1, abort))) break;
+        const int ks = t % Sh::KS, vs = t % Sh::VS;
+        const uint64_t dk = dk0 + (uint64_t)(ks * (Sh::TB >> 4));
+        const uint64_t dv = dv0 + (uint64_t)(vs * (Sh::TB >> 4));
+        if (!(ok = mbar_spin(mb + Sh::bK + 8 * ks, (t / Sh::KS) & 1, abort))) break;
         // S takes the columns that P of the last step lies in
-        if (t > 0 && !(ok = mbar_wait(barPV(qt, t - 1), ((t - 1) / Sh::VS) & 1, abort))) break;
+        if (t > 0 && !(ok = mbar_spin(barPV(qt, t - 1), ((t - 1) / Sh::VS) & 1, abort))) break;
         tc_fence_after();
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
-          tc_mma(sc, umma_desc(qa + off, 16, 1024), umma_desc(kb + off, 16, 1024), id_s,
-                 kk ? 1u : 0u);
-        }
         last = barS(qt, t);
         lastph = (t / Sh::KS) & 1;
-        tc_commit(last);
-        if (!(ok = mbar_wait(mb + Sh::bP + 8 * qt, t & 1, abort))) break;
-        if (!(ok = mbar_wait(mb + Sh::bV + 8 * (t % Sh::VS), (t / Sh::VS) & 1, abort))) break;
-        tc_fence_after();
+        if (leader) {
 #pragma unroll
-        for (int kk = 0; kk < kPrefixTile / 16; ++kk)
-          tc_mma_ts(oc, sc + kk * 8, umma_desc(vb + kk * 2048, 16384, 1024), id_o,
-                    (t | kk) ? 1u : 0u);
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint64_t off = (kk >> 2) * 1024 + (kk & 3) * 2;  // 16-byte units
+            tc_mma(sc, dq + off, dk + off, id_s, kk ? 1u : 0u);
+          }
+          tc_commit(last);
+        }
+        __syncwarp();
+        if (!(ok = mbar_spin(mb + Sh::bP + 8 * qt, t & 1, abort))) break;
+        if (!(ok = mbar_spin(mb + Sh::bV + 8 * vs, (t / Sh::VS) & 1, abort))) break;
+        tc_fence_after();
         last = barPV(qt, t);
         lastph = (t / Sh::VS) & 1;
-        tc_commit(last);
+        if (leader) {
+#pragma unroll
+          for (int kk = 0; kk < kPrefixTile / 16; ++kk)
+            tc_mma_ts(oc, sc + kk * 8, dv + kk * 128, id_o, (t | kk) ? 1u : 0u);
+          tc_commit(last);
+        }
+        __syncwarp();
       }
       if (last) {
         const long long t0 = clock64();
