@@ -84,7 +84,9 @@ struct Shape {
   static_assert(128 * NT * kSoftRegs + 128 * kOtherRegs <= kThreads * kLaunch,
                 "register split exceeds the block's launch allocation");
   static constexpr uint32_t TB = kPrefixTile * D * 2;
-  static constexpr uint32_t oQ = 0, oK = NT * TB, oV = oK + KS * TB, oMeta = oV + VS * TB;
+  // a query tile's place also takes its output rows, 2 D bytes each and 16 more
+  static constexpr uint32_t QB = TB + 128 * 16;
+  static constexpr uint32_t oQ = 0, oK = NT * QB, oV = oK + KS * TB, oMeta = oV + VS * TB;
   // barriers, 8 bytes each
   static constexpr uint32_t bQ = 0, bK = 8, bV = bK + 8 * KS, bS = bV + 8 * VS,
                             bP = bS + 8 * NT * KS, bPV = bP + 8 * NT, bTurn = bPV + 8 * NT * VS,
@@ -209,6 +211,42 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
   const int steps = na + (it.b1 - it.b0 + kPrefixTile - 1) / kPrefixTile;
   const int tiles = NT == 2 && it.ntok > a.R ? 2 : 1;
 
+  // (producers) the sources of a key tile; the first tile's are under way
+  // before the block's first barrier
+  bool slot_bad = false;
+  auto load_src = [&](int t, Src& s) {
+    const Step st = step_of(it, na, t);
+    const int64_t* slots = (st.own ? a.suffix_slots : a.prefix_slots) + st.base;
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      const int j = 4 * lane + m;
+      s.slot[m] = j < st.n ? slots[j] : -1;
+      s.kind[m] = 0;
+      s.row[m] = 0;
+      if (j < st.n) {
+        if (!a.pv.valid(s.slot[m])) {
+          slot_bad = true;
+          s.slot[m] = -1;
+        } else if (s.slot[m] < a.pv.native_total) {
+          int64_t b, o;
+          if (a.bs_shift >= 0) {
+            b = s.slot[m] >> a.bs_shift;
+            o = s.slot[m] - (b << a.bs_shift);
+          } else {
+            b = s.slot[m] / a.pv.bs;
+            o = s.slot[m] - b * a.pv.bs;
+          }
+          s.kind[m] = 1;
+          s.row[m] = (int)(b * a.nrb + g * a.nrh + o * a.nro);
+        } else {
+          s.kind[m] = 2;
+          s.row[m] = (int)((s.slot[m] - a.pv.native_total) * a.srr + g * a.srh);
+        }
+      }
+    }
+  };
+  Src cur;
+  if ((warp == Sh::kSoft || warp == Sh::kSoft + 1) && steps > 0) load_src(0, cur);
   if (tid == 0) {
     mbar_init(mb + Sh::bQ, 128 * tiles);
     for (int s = 0; s < Sh::KS; ++s) mbar_init(mb + Sh::bK + 8 * s, 32);
@@ -234,40 +272,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     // ============================================== producers: K, then V warp
     const bool isv = warp != Sh::kSoft;
     const int ST = isv ? Sh::VS : Sh::KS;
-    bool slot_bad = false;
-    auto load_src = [&](int t, Src& s) {
-      const Step st = step_of(it, na, t);
-      const int64_t* slots = (st.own ? a.suffix_slots : a.prefix_slots) + st.base;
-#pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        const int j = 4 * lane + m;
-        s.slot[m] = j < st.n ? slots[j] : -1;
-        s.kind[m] = 0;
-        s.row[m] = 0;
-        if (j < st.n) {
-          if (!a.pv.valid(s.slot[m])) {
-            slot_bad = true;
-            s.slot[m] = -1;
-          } else if (s.slot[m] < a.pv.native_total) {
-            int64_t b, o;
-            if (a.bs_shift >= 0) {
-              b = s.slot[m] >> a.bs_shift;
-              o = s.slot[m] - (b << a.bs_shift);
-            } else {
-              b = s.slot[m] / a.pv.bs;
-              o = s.slot[m] - b * a.pv.bs;
-            }
-            s.kind[m] = 1;
-            s.row[m] = (int)(b * a.nrb + g * a.nrh + o * a.nro);
-          } else {
-            s.kind[m] = 2;
-            s.row[m] = (int)((s.slot[m] - a.pv.native_total) * a.srr + g * a.srh);
-          }
-        }
-      }
-    };
-    Src cur, nxt;
-    if (steps > 0) load_src(0, cur);
+    Src nxt;
     int issued = 0;
     for (int t = 0; t < steps; ++t) {
       // the stage is free once every tile's product of its last use is done
@@ -346,7 +351,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       const bool leader = elect_one();
       const uint32_t id_s = umma_idesc(128, 128, umma_format<T>(), 0, 0);
       const uint32_t id_o = umma_idesc(128, D, umma_format<T>(), 0, 1);  // V is MN-major
-      const uint64_t dq = umma_desc(sbase + Sh::oQ + qt * Sh::TB, 16, 1024);
+      const uint64_t dq = umma_desc(sbase + Sh::oQ + qt * Sh::QB, 16, 1024);
       const uint64_t dk0 = umma_desc(sbase + Sh::oK, 16, 1024);
       const uint64_t dv0 = umma_desc(sbase + Sh::oV, 16384, 1024);
       const uint32_t tm = __shfl_sync(~0u, tmem, 0);
@@ -404,25 +409,29 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     {
       // queries into the swizzled operand layout, 16 bytes a step
       constexpr int C = D / 8;
-      for (int i = tid & 127; i < kPrefixTile * C; i += 128) {
-        const int row = i / C, c = i % C;
-        const int tk = qt * a.R + row / a.G;
-        if (row < a.R * a.G && tk < it.ntok) {
-          const char* src = a.q + (int64_t)(it.tok0 + tk) * a.qt +
-                            (int64_t)(g * a.G + row % a.G) * a.qh + 16 * c;
-          uint4 v;
-          if (a.vec_q) {
-            v = *reinterpret_cast<const uint4*>(src);
-          } else {
-            const uint16_t* s = reinterpret_cast<const uint16_t*>(src);
-            v.x = s[0] | (uint32_t)s[1] << 16;
-            v.y = s[2] | (uint32_t)s[3] << 16;
-            v.z = s[4] | (uint32_t)s[5] << 16;
-            v.w = s[6] | (uint32_t)s[7] << 16;
-          }
-          if (a.neg) v = make_uint4(v.x ^ 0x80008000u, v.y ^ 0x80008000u, v.z ^ 0x80008000u,
-                                    v.w ^ 0x80008000u);
-          st_shared16(sbase + Sh::oQ + qt * Sh::TB + sw128(row, c, kPrefixTile), v);
+      const int left = it.ntok - qt * a.R;
+      const int rows = (left < a.R ? left : a.R) * a.G;
+      const uint32_t qs = sbase + Sh::oQ + qt * Sh::QB;
+      const char* base = a.q + (int64_t)(it.tok0 + qt * a.R) * a.qt + (int64_t)(g * a.G) * a.qh;
+      const int c = tid % C;
+      auto from = [&](int row) {
+        const int tk = row / a.G;
+        return base + tk * a.qt + (row - tk * a.G) * a.qh + 16 * c;
+      };
+      if (a.vec_q && !a.neg) {
+#pragma unroll 4
+        for (int row = (tid & 127) / C; row < rows; row += 128 / C)
+          cp_async16(qs + sw128(row, c, kPrefixTile), from(row), true);
+        cp_async_wait_all();
+      } else {
+        for (int row = (tid & 127) / C; row < rows; row += 128 / C) {
+          uint16_t e[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            e[k] = reinterpret_cast<const uint16_t*>(from(row))[k] ^ (a.neg ? 0x8000 : 0);
+          st_shared16(qs + sw128(row, c, kPrefixTile),
+                      make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16,
+                                 e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16));
         }
       }
       fence_async_smem();
@@ -645,44 +654,74 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     const int64_t token = it.tok0 + tok;
     const int64_t prow = ((int64_t)it.part + tok) * a.hq + h;
     char* orow = a.out + token * a.ot + (int64_t)h * a.oh;
+    const bool part = it.part >= 0;
+    if (part) orow = reinterpret_cast<char*>(a.part_o + prow * D);
+    const bool have = ok && steps > 0 && lsum != 0.f;
+    if (part || a.vec_out) {
+      // each thread stages its row (32-bit partials in two halves) where the
+      // queries were and sends it off as one bulk copy: stores from the
+      // registers touch 32 rows an instruction, 5300 clocks for a tile
+      const uint32_t buf = sbase + Sh::oQ + qt * Sh::QB + r * (2 * D + 16);
 #pragma unroll 1
-    for (int cc = 0; cc < D / 32; ++cc) {
-      uint32_t v[32];
-      if (ok && steps > 0) {
+      for (int half = 0; half < (part ? 2 : 1); ++half) {
+        if (half) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        uint32_t v[32];
+        if (part) {
+#pragma unroll
+          for (int cc = 0; cc < D / 64; ++cc) {
+            CS_TMEM_LD32(oc + half * (D / 2) + 32 * cc, v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 32; ++c) v[c] = have ? __float_as_uint(__uint_as_float(v[c]) * inv) : 0u;
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              st_shared16(buf + 128 * cc + 16 * c,
+                          make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]));
+          }
+        } else {
+#pragma unroll
+          for (int cc = 0; cc < D / 32; ++cc) {
+            CS_TMEM_LD32(oc + 32 * cc, v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+              const float x = have ? __uint_as_float(v[2 * c]) * inv : 0.f;
+              const float y = have ? __uint_as_float(v[2 * c + 1]) * inv : 0.f;
+              v[c] = Pack2<T>::pack(x, y);
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              st_shared16(buf + 64 * cc + 16 * c,
+                          make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]));
+          }
+        }
+        if (row_ok && ok) {
+          fence_async_smem();
+          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(
+                           orow + half * 2 * D),
+                       "r"(buf), "n"(2 * D)
+                       : "memory");
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+      }
+    } else {
+#pragma unroll 1
+      for (int cc = 0; cc < D / 32; ++cc) {
+        uint32_t v[32];
         CS_TMEM_LD32(oc + 32 * cc, v);
         tmem_wait_ld();
-      }
-#pragma unroll
-      for (int c = 0; c < 32; ++c)
-        v[c] = ok && steps > 0 && lsum != 0.f ? __float_as_uint(__uint_as_float(v[c]) * inv) : 0u;
-      if (!row_ok || !ok) continue;
-      if (it.part >= 0) {
-        float4* dst = reinterpret_cast<float4*>(a.part_o + prow * D + 32 * cc);
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-          dst[c] = make_float4(__uint_as_float(v[4 * c]), __uint_as_float(v[4 * c + 1]),
-                               __uint_as_float(v[4 * c + 2]), __uint_as_float(v[4 * c + 3]));
-      } else if (a.vec_out) {
-        uint4* dst = reinterpret_cast<uint4*>(orow + 64 * cc);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t w[4];
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            w[u] = Pack2<T>::pack(__uint_as_float(v[8 * c + 2 * u]),
-                                  __uint_as_float(v[8 * c + 2 * u + 1]));
-          dst[c] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-      } else {
+        if (!row_ok || !ok) continue;
 #pragma unroll
         for (int c = 0; c < 32; ++c)
-          reinterpret_cast<T*>(orow)[32 * cc + c] = Elem<T>::from_f(__uint_as_float(v[c]));
+          reinterpret_cast<T*>(orow)[32 * cc + c] =
+              Elem<T>::from_f(have ? __uint_as_float(v[c]) * inv : 0.f);
       }
     }
     if (row_ok && ok) {
       if (it.part >= 0) a.part_lse[prow] = lse2;
       else if (a.lse) a.lse[token * a.hq + h] = lse2 * kLn2;
     }
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
   }
 
@@ -713,15 +752,37 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const PArgs a, const i
   float o[E], sum = 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int c = 0; c < j.z; ++c) {
-    const int64_t row = (int64_t)list[j.y + c] * a.hq + h;
-    const float l = a.part_lse[row];
-    if (l == -INFINITY) continue;
-    const float f = ex2(l - top);  // NaN stays NaN
-    sum += f;
-    const float* src = a.part_o + row * D + lane * E;
+  for (int c0 = 0; c0 < j.z; c0 += 32) {
+    // a lane's partial of these 32: its place and weight (NaN stays NaN)
+    int64_t row = 0;
+    float f = 0.f;
+    if (c0 + lane < j.z) {
+      row = (int64_t)list[j.y + c0 + lane] * a.hq + h;
+      const float l = a.part_lse[row];
+      f = l == -INFINITY ? 0.f : ex2(l - top);
+    }
+    sum += warp_sum(f);
+    const int n = j.z - c0 < 32 ? j.z - c0 : 32;
+#pragma unroll 1
+    for (int c = 0; c < n; c += 8) {
+      float x[8][E], w[8];
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = fmaf(f, src[e], o[e]);
+      for (int k = 0; k < 8; ++k) {
+        const int64_t rk = __shfl_sync(~0u, row, c + k);
+        w[k] = __shfl_sync(~0u, f, c + k);
+        if (c + k >= n || w[k] == 0.f) w[k] = 0.f;
+        else {
+#pragma unroll
+          for (int e = 0; e < E; ++e) x[k][e] = a.part_o[rk * D + lane * E + e];
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (w[k] != 0.f) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[e] = fmaf(w[k], x[k][e], o[e]);
+        }
+    }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   T* out = reinterpret_cast<T*>(a.out + (int64_t)j.x * a.ot + (int64_t)h * a.oh) + lane * E;
