@@ -13,8 +13,8 @@
 //
 // Warps: 4 NT softmax (one thread a row), a K and a V producer, NT MMA
 // issuers.  Keys come through the slot arrays: TMA boxes of 64 x 16 for runs
-// of 16 keys in consecutive rows of the pool, tile::gather4 for 4 keys of one
-// map, 16-byte cp.async for the rest (range ends, which are filled with
+// of 16 keys in consecutive rows of the pool, 16-byte cp.async row by row for
+// the rest (scattered slots, the sidecar, range ends, which are filled with
 // zeros, and pools no tensor map describes).
 //
 // Bound: HBM for decodes (each record once a row tile), the tensor and
@@ -36,9 +36,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct PArgs {
-  // [0] pool with 64 x 1 boxes (gather4), [1] with 64 x 16; [2], [3] sidecar
-  // K and [4], [5] sidecar V alike
-  CUtensorMap tm[6];
+  CUtensorMap tm;  // the pool's rows in boxes of 64 x 16
   PagedView pv;
   const char* q;
   int64_t qt, qh;  // byte strides
@@ -52,7 +50,7 @@ struct PArgs {
   float* part_o;    // [part token][query head][dim], normalised
   float* part_lse;  // [part token][query head], log2 of the softmax denominator
   int32_t* status;
-  int64_t nrb, nrh, nro, srr, srh;  // slot -> map row
+  int64_t nrb, nrh, nro;  // block, head, offset -> map row
   int hq, hkv, G, R;  // R: tokens a row tile
   int bs_shift;       // log2(block size), -1 when it is no power of two
   int tma;            // 1: tensor maps describe the pool
@@ -91,7 +89,10 @@ struct Shape {
   static constexpr uint32_t bQ = 0, bK = 8, bV = bK + 8 * KS, bS = bV + 8 * VS,
                             bP = bS + 8 * NT * KS, bPV = bP + 8 * NT, bTurn = bPV + 8 * NT * VS,
                             oTmem = bTurn + 16, oAbort = oTmem + 4, oBad = oAbort + 4,
-                            kMeta = oBad + 2 * NT * 16;
+                            oRows = (oBad + 2 * NT * 16 + 15) / 16 * 16,
+                            kMeta = oRows + 2 * 128 * 8;
+  static_assert(oMeta % 1024 == 0 && oRows % 16 == 0 && oBad % 4 == 0 && oTmem % 4 == 0,
+                "alignment of the shared-memory places");
   static constexpr uint32_t kSmem = oMeta + kMeta + 1024;  // the base is rounded up to 1024
   static constexpr uint32_t kCols = 256 * NT;
   static constexpr uint32_t cS = 0, cO = 128 * NT;  // S of tile i at 128 i, O at cO + D i
@@ -189,9 +190,9 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t src) {
 
 // where the keys of one lane (4 consecutive keys of a tile) come from
 struct Src {
-  int row[4];     // row of the tensor map
-  int kind[4];    // 0: none (beyond the range, or no valid slot), 1: pool, 2: sidecar
-  int64_t slot[4];
+  uint64_t at[4];  // the K or V half of the record; 0: none (beyond the range, or no valid slot)
+  int row;         // row of the tensor map of the first key
+  bool run;        // the four lie in consecutive rows of the pool's map
 };
 
 template <typename T, int D, int NT>
@@ -211,42 +212,44 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
   const int steps = na + (it.b1 - it.b0 + kPrefixTile - 1) / kPrefixTile;
   const int tiles = NT == 2 && it.ntok > a.R ? 2 : 1;
 
-  // (producers) the sources of a key tile; the first tile's are under way
-  // before the block's first barrier
+  // (producers) the sources of a key tile
   bool slot_bad = false;
+  const bool isv = warp != Sh::kSoft;
   auto load_src = [&](int t, Src& s) {
     const Step st = step_of(it, na, t);
     const int64_t* slots = (st.own ? a.suffix_slots : a.prefix_slots) + st.base;
+    int64_t sl[4];
+#pragma unroll
+    for (int m = 0; m < 4; ++m) sl[m] = 4 * lane + m < st.n ? slots[4 * lane + m] : -1;
+    s.run = a.tma != 0 && sl[0] >= 0 && sl[3] < a.pv.native_total;
+    s.row = 0;
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
-      const int j = 4 * lane + m;
-      s.slot[m] = j < st.n ? slots[j] : -1;
-      s.kind[m] = 0;
-      s.row[m] = 0;
-      if (j < st.n) {
-        if (!a.pv.valid(s.slot[m])) {
-          slot_bad = true;
-          s.slot[m] = -1;
-        } else if (s.slot[m] < a.pv.native_total) {
-          int64_t b, o;
+      s.at[m] = 0;
+      int64_t b = 0, o = 0;
+      if (a.pv.valid(sl[m])) {
+        if (sl[m] < a.pv.native_total) {
           if (a.bs_shift >= 0) {
-            b = s.slot[m] >> a.bs_shift;
-            o = s.slot[m] - (b << a.bs_shift);
+            b = sl[m] >> a.bs_shift;
+            o = sl[m] - (b << a.bs_shift);
           } else {
-            b = s.slot[m] / a.pv.bs;
-            o = s.slot[m] - b * a.pv.bs;
+            b = sl[m] / a.pv.bs;
+            o = sl[m] - b * a.pv.bs;
           }
-          s.kind[m] = 1;
-          s.row[m] = (int)(b * a.nrb + g * a.nrh + o * a.nro);
+          s.at[m] = reinterpret_cast<uint64_t>(a.pv.cache) + b * a.pv.sb + g * a.pv.sh +
+                    o * a.pv.so + (isv ? 2 * D : 0);
         } else {
-          s.kind[m] = 2;
-          s.row[m] = (int)((s.slot[m] - a.pv.native_total) * a.srr + g * a.srh);
+          s.at[m] = reinterpret_cast<uint64_t>(isv ? a.pv.side_v : a.pv.side_k) +
+                    (sl[m] - a.pv.native_total) * a.pv.ssr + g * a.pv.ssh;
         }
+      } else if (4 * lane + m < st.n) {
+        slot_bad = true;
       }
+      if (m == 0) s.row = (int)(b * a.nrb + g * a.nrh + o * a.nro);
+      // consecutive slots of one block, and blocks whose offsets are rows
+      s.run = s.run && sl[m] == sl[0] + m && (m == 0 || o > 0) && a.nro == 1;
     }
   };
-  Src cur;
-  if ((warp == Sh::kSoft || warp == Sh::kSoft + 1) && steps > 0) load_src(0, cur);
   if (tid == 0) {
     mbar_init(mb + Sh::bQ, 128 * tiles);
     for (int s = 0; s < Sh::KS; ++s) mbar_init(mb + Sh::bK + 8 * s, 32);
@@ -258,8 +261,16 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     mbar_init(mb + Sh::bTurn + 8, 128);
     *abort = 0;
     mbar_init_fence();
+    if (a.tma)
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&a.tm)) : "memory");
   }
   if (warp == Sh::kSoft + 2) tmem_alloc(mb + Sh::oTmem, Sh::kCols);
+  // everything above touches only this block and the plan, which no kernel
+  // writes; from here on the preceding grids' results are read
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  Src cur;
+  if ((warp == Sh::kSoft || warp == Sh::kSoft + 1) && steps > 0) load_src(0, cur);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -270,7 +281,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
   if (warp == Sh::kSoft || warp == Sh::kSoft + 1) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Sh::kOtherRegs));
     // ============================================== producers: K, then V warp
-    const bool isv = warp != Sh::kSoft;
     const int ST = isv ? Sh::VS : Sh::KS;
     Src nxt;
     int issued = 0;
@@ -284,47 +294,50 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       }
       const uint32_t bar = mb + (isv ? Sh::bV : Sh::bK) + 8 * (t % ST);
       const uint32_t dst = sbase + (isv ? Sh::oV : Sh::oK) + (t % ST) * Sh::TB;
-      // 16 keys (4 lanes) in consecutive rows of one map; else 4 keys of one map
-      const int k0 = cur.kind[0];
-      const bool four = a.tma && k0 != 0 && cur.kind[1] == k0 && cur.kind[2] == k0 &&
-                        cur.kind[3] == k0;
-      const int r16 = __shfl_sync(~0u, cur.row[0], lane & ~3);
-      const int k16 = __shfl_sync(~0u, k0, lane & ~3);
-      const bool seq = four && k0 == k16 && cur.row[0] == r16 + 4 * (lane & 3) &&
-                       cur.row[1] == cur.row[0] + 1 && cur.row[2] == cur.row[0] + 2 &&
-                       cur.row[3] == cur.row[0] + 3;
-      const uint32_t sq = __ballot_sync(~0u, seq);
-      const bool run = ((sq >> (lane & ~3)) & 0xFu) == 0xFu;
-      const int x0 = isv && k0 == 1 ? D : 0;
-      const int map0 = k0 == 2 ? (isv ? 4 : 2) : 0;
-      if (run || four) {
-        const bool lead = run && (lane & 3) == 0;
-        mbar_arrive_tx(bar, run ? (lead ? 16 * D * 2 : 0) : 4 * D * 2);
+      // 16 keys (4 lanes) in consecutive rows: one TMA box an operand half;
+      // the others row by row with cp.async, whole rows an instruction, the
+      // addresses through shared memory.  (tile::gather4 is issued lane by
+      // lane, about 100 clocks each: 6400 for a tile of scattered rows.)
+      const int r16 = __shfl_sync(~0u, cur.row, lane & ~3);
+      const uint32_t sq = __ballot_sync(~0u, cur.run && cur.row == r16 + 4 * (lane & 3));
+      const bool lead = (lane & 3) == 0 && ((sq >> lane) & 0xFu) == 0xFu;
+      const uint32_t leads = __ballot_sync(~0u, lead);
+      if (leads != 0x11111111u) {
+        const uint32_t tab = mb + Sh::oRows + (isv ? 1024 : 0);
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          const uint32_t to = dst + c * 16384 + 4 * lane * 128;
-          if (lead) tma_tile2d(to, &a.tm[map0 + 1], x0 + 64 * c, cur.row[0], bar);
-          else if (!run)
-            tma_gather4(to, &a.tm[map0], x0 + 64 * c, cur.row[0], cur.row[1], cur.row[2],
-                        cur.row[3], bar);
-        }
-      } else {
-        // rows one by one; a place without a key is zeroed (its value must be
-        // finite: its weight is zero)
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          const int j = 4 * lane + m;
-          const bool ok = cur.slot[m] >= 0;
-          const char* src =
-              ok ? a.pv.addr(cur.slot[m], g, isv ? D : 0) : a.pv.cache;
-#pragma unroll
-          for (int c = 0; c < D / 8; ++c)
-            cp_async16(dst + sw128(j, c, kPrefixTile), ok ? src + 16 * c : src, ok);
-        }
-        cp_async_wait_all();
-        fence_async_smem();
-        mbar_arrive(bar);
+        for (int m = 0; m < 4; m += 2)
+          st_shared16(tab + 32 * lane + 8 * m,
+                      make_uint4((uint32_t)cur.at[m], (uint32_t)(cur.at[m] >> 32),
+                                 (uint32_t)cur.at[m + 1], (uint32_t)(cur.at[m + 1] >> 32)));
       }
+      if (lane == 0) mbar_expect_tx(bar, __popc(leads) * 16 * D * 2);
+      __syncwarp();
+      if (lead) {
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+          tma_tile2d(dst + c * 16384 + 4 * lane * 128, &a.tm, (isv ? D : 0) + 64 * c, cur.row, bar);
+      }
+      if (leads != 0x11111111u) {
+        constexpr int C = D / 8, RI = 32 / C;  // 16-byte pieces a row, rows an instruction
+        const uint64_t* tab = reinterpret_cast<const uint64_t*>(smem + Sh::oMeta + Sh::oRows +
+                                                                (isv ? 1024 : 0));
+        for (int q = 0; q < 8; ++q) {
+          if ((leads >> (4 * q)) & 1u) continue;
+          uint64_t at[16 / RI];
+#pragma unroll
+          for (int i = 0; i < 16 / RI; ++i) at[i] = tab[16 * q + i * RI + lane / C];
+#pragma unroll
+          for (int i = 0; i < 16 / RI; ++i) {
+            const int j = 16 * q + i * RI + lane / C;
+            const uint64_t src =
+                at[i] ? at[i] + 16 * (lane % C) : reinterpret_cast<uint64_t>(a.pv.cache);
+            cp_async16(dst + sw128(j, lane % C, kPrefixTile), reinterpret_cast<const void*>(src),
+                       at[i] != 0);
+          }
+        }
+        __syncwarp();
+      }
+      cp_async_arrive_noinc(bar);
       issued = t + 1;
       if (t + 1 < steps) {
         load_src(t + 1, nxt);
@@ -365,6 +378,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
         if (!(ok = mbar_spin(mb + Sh::bK + 8 * ks, (t / Sh::KS) & 1, abort))) break;
         // S takes the columns that P of the last step lies in
         if (t > 0 && !(ok = mbar_spin(barPV(qt, t - 1), ((t - 1) / Sh::VS) & 1, abort))) break;
+        fence_async_smem();  // rows copied by cp.async
         tc_fence_after();
         last = barS(qt, t);
         lastph = (t / Sh::KS) & 1;
@@ -379,6 +393,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
         __syncwarp();
         if (!(ok = mbar_spin(mb + Sh::bP + 8 * qt, t & 1, abort))) break;
         if (!(ok = mbar_spin(mb + Sh::bV + 8 * vs, (t / Sh::VS) & 1, abort))) break;
+        fence_async_smem();
         tc_fence_after();
         last = barPV(qt, t);
         lastph = (t / Sh::VS) & 1;
@@ -659,12 +674,15 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     const bool have = ok && steps > 0 && lsum != 0.f;
     if (part || a.vec_out) {
       // each thread stages its row (32-bit partials in two halves) where the
-      // queries were and sends it off as one bulk copy: stores from the
-      // registers touch 32 rows an instruction, 5300 clocks for a tile
-      const uint32_t buf = sbase + Sh::oQ + qt * Sh::QB + r * (2 * D + 16);
+      // queries were, and the warp writes whole rows: stores straight from the
+      // registers touch 32 rows an instruction, and a bulk copy a row is
+      // issued lane by lane (5300 clocks a tile, either way)
+      constexpr int L = 2 * D / 16;  // lanes a row
+      const uint32_t stage = sbase + Sh::oQ + qt * Sh::QB + (r - lane) * (2 * D + 16);
+      const uint32_t buf = stage + lane * (2 * D + 16);
+      const uint64_t to = row_ok && ok ? reinterpret_cast<uint64_t>(orow) : 0;
 #pragma unroll 1
       for (int half = 0; half < (part ? 2 : 1); ++half) {
-        if (half) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         uint32_t v[32];
         if (part) {
 #pragma unroll
@@ -672,7 +690,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
             CS_TMEM_LD32(oc + half * (D / 2) + 32 * cc, v);
             tmem_wait_ld();
 #pragma unroll
-            for (int c = 0; c < 32; ++c) v[c] = have ? __float_as_uint(__uint_as_float(v[c]) * inv) : 0u;
+            for (int c = 0; c < 32; ++c)
+              v[c] = have ? __float_as_uint(__uint_as_float(v[c]) * inv) : 0u;
 #pragma unroll
             for (int c = 0; c < 8; ++c)
               st_shared16(buf + 128 * cc + 16 * c,
@@ -695,14 +714,22 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
                           make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]));
           }
         }
-        if (row_ok && ok) {
-          fence_async_smem();
-          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(
-                           orow + half * 2 * D),
-                       "r"(buf), "n"(2 * D)
-                       : "memory");
-          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        __syncwarp();
+#pragma unroll
+        for (int n0 = 0; n0 < L; n0 += 8) {
+          uint4 x[8];
+          uint64_t dst[8];
+#pragma unroll
+          for (int n = 0; n < 8; ++n) {
+            const int row = (n0 + n) * (32 / L) + lane / L;
+            dst[n] = __shfl_sync(~0u, to, row);
+            x[n] = ld_shared16(stage + row * (2 * D + 16) + 16 * (lane % L));
+          }
+#pragma unroll
+          for (int n = 0; n < 8; ++n)
+            if (dst[n]) *reinterpret_cast<uint4*>(dst[n] + half * 2 * D + 16 * (lane % L)) = x[n];
         }
+        __syncwarp();
       }
     } else {
 #pragma unroll 1
@@ -721,7 +748,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       if (it.part >= 0) a.part_lse[prow] = lse2;
       else if (a.lse) a.lse[token * a.hq + h] = lse2 * kLn2;
     }
-    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
   }
 
@@ -740,6 +766,8 @@ template <typename T, int D>
 __global__ void __launch_bounds__(128) prefix_join_kernel(const PArgs a, const int4* join,
                                                           const int32_t* list, int n) {
   constexpr int E = D / 32;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31;
   const int64_t w = blockIdx.x * 4ll + (threadIdx.x >> 5);
   if (w >= (int64_t)n * a.hq) return;
@@ -801,29 +829,34 @@ bool setup_maps(PArgs& a, const cs_paged_kv& kv) {
   if (unit <= 0) return false;
   const int64_t rows = ((kv.num_blocks - 1) * pv.sb + (pv.kv_heads - 1) * pv.sh +
                         (pv.bs - 1) * pv.so) / unit + 1;
-  if (!encode_rows(&a.tm[0], pv.cache, bf16, 2 * D, rows, unit, 1) ||
-      !encode_rows(&a.tm[1], pv.cache, bf16, 2 * D, rows, unit, 16))
-    return false;
+  if (!encode_rows(&a.tm, pv.cache, bf16, 2 * D, rows, unit, 16)) return false;
   a.nrb = pv.sb / unit;
   a.nrh = pv.sh / unit;
   a.nro = pv.so / unit;
-  if (pv.side_capacity > 0) {
-    if (pv.ssr < 0 || pv.ssh < 0) return false;
-    const int64_t su = std::gcd(pv.ssr, pv.ssh);
-    if (su <= 0) return false;
-    const int64_t sr = ((pv.side_capacity - 1) * pv.ssr + (pv.kv_heads - 1) * pv.ssh) / su + 1;
-    if (!encode_rows(&a.tm[2], pv.side_k, bf16, D, sr, su, 1) ||
-        !encode_rows(&a.tm[3], pv.side_k, bf16, D, sr, su, 16) ||
-        !encode_rows(&a.tm[4], pv.side_v, bf16, D, sr, su, 1) ||
-        !encode_rows(&a.tm[5], pv.side_v, bf16, D, sr, su, 16))
-      return false;
-    a.srr = pv.ssr / su;
-    a.srh = pv.ssh / su;
-  } else {  // never addressed: no slot reaches the sidecar
-    a.tm[2] = a.tm[4] = a.tm[0];
-    a.tm[3] = a.tm[5] = a.tm[1];
-  }
   return true;
+}
+
+// A launch that may start beside the end of the grid before it on the stream;
+// the kernel waits for that grid (griddepcontrol.wait) before it reads or
+// writes global memory.
+template <typename K, typename... A>
+int launch_dependent(K kernel, unsigned blocks, int threads, uint32_t smem, cudaStream_t stream,
+                     A... args) {
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3(blocks);
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = stream;
+  c.attrs = at;
+  c.numAttrs = 1;
+  if (cudaLaunchKernelEx(&c, kernel, args...) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return CS_ERR_CUDA;
+  }
+  return CS_OK;
 }
 
 template <typename T, int D, int NT>
@@ -839,9 +872,8 @@ int launch_main(const PArgs& a, int64_t blocks, cudaStream_t stream) {
            at.numRegs == Shape<D, NT>::kLaunch;
   }();
   if (!ready) return CS_ERR_CUDA;
-  kernel<<<(unsigned)blocks, Shape<D, NT>::kThreads, Shape<D, NT>::kSmem, stream>>>(a);
-  CS_LAUNCH_CHECK();
-  return CS_OK;
+  return launch_dependent(kernel, (unsigned)blocks, Shape<D, NT>::kThreads, Shape<D, NT>::kSmem,
+                          stream, a);
 }
 
 template <typename T, int D>
@@ -855,10 +887,9 @@ int launch_all(const PArgs& a, const cs_prefix_plan_info& info, const int32_t* p
   }
   if (info.n_join > 0) {
     const unsigned blocks = (unsigned)((info.n_join * a.hq + 3) / 4);
-    prefix_join_kernel<T, D><<<blocks, 128, 0, stream>>>(
-        a, reinterpret_cast<const int4*>(plan + info.join_off), plan + info.list_off,
-        (int)info.n_join);
-    CS_LAUNCH_CHECK();
+    return launch_dependent(prefix_join_kernel<T, D>, blocks, 128, 0, stream, a,
+                            reinterpret_cast<const int4*>(plan + info.join_off),
+                            plan + info.list_off, (int)info.n_join);
   }
   return CS_OK;
 }
@@ -901,7 +932,7 @@ int prefix_attn_sm100(const cs_prefix_params& p, const cs_prefix_plan_info& info
   // masked scores are -inf before they are scaled, so the factor is never 0
   a.scale2 = fmaxf(fabsf((float)p.scale) * kLog2e, 1e-30f);
   a.scale_signed2 = a.neg ? -a.scale2 : a.scale2;
-  a.nrb = a.nrh = a.nro = a.srr = a.srh = 0;
+  a.nrb = a.nrh = a.nro = 0;
   a.tma = setup_maps(a, kv) ? 1 : 0;
   const bool half = kv.dtype == CS_F16;
   if (kv.head_dim == 128)
