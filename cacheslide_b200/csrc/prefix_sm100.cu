@@ -57,7 +57,7 @@ struct PArgs {
   int vec_q, vec_out; // 16-byte loads / stores fit
   int neg;            // the scale is negative: the queries are negated
   float scale2;       // |scale| * log2 e
-  float scale_signed2;
+  float scale;
 };
 
 template <typename T> constexpr int umma_format() { return std::is_same<T, __half>::value ? 0 : 1; }
@@ -88,10 +88,10 @@ struct Shape {
   // barriers, 8 bytes each
   static constexpr uint32_t bQ = 0, bK = 8, bV = bK + 8 * KS, bS = bV + 8 * VS,
                             bP = bS + 8 * NT * KS, bPV = bP + 8 * NT, bTurn = bPV + 8 * NT * VS,
-                            oTmem = bTurn + 16, oAbort = oTmem + 4, oBad = oAbort + 4,
-                            oRows = (oBad + 2 * NT * 16 + 15) / 16 * 16,
+                            oTmem = bTurn + 16, oAbort = oTmem + 4, 
+                            oRows = (oAbort + 4 + 15) / 16 * 16,
                             kMeta = oRows + 2 * 128 * 8;
-  static_assert(oMeta % 1024 == 0 && oRows % 16 == 0 && oBad % 4 == 0 && oTmem % 4 == 0,
+  static_assert(oMeta % 1024 == 0 && oRows % 16 == 0 && oTmem % 4 == 0,
                 "alignment of the shared-memory places");
   static constexpr uint32_t kSmem = oMeta + kMeta + 1024;  // the base is rounded up to 1024
   static constexpr uint32_t kCols = 256 * NT;
@@ -194,6 +194,51 @@ struct Src {
   int row;         // row of the tensor map of the first key
   bool run;        // the four lie in consecutive rows of the pool's map
 };
+
+// One row of an item by one warp, over the keys that it sees (the CUDA-core
+// form of prefix.cu): the way out for rows whose sums are not finite.
+template <typename T, int D>
+__device__ __noinline__ void row_again(const PArgs& a, const PrefixItem& it, int g, int tok, int h,
+                                       int lane, void* out, bool part) {
+  constexpr int E = D / 32;
+  const int4 tk = a.tokens[it.tok0 + tok];
+  const T* q = reinterpret_cast<const T*>(a.q + (int64_t)(it.tok0 + tok) * a.qt + (int64_t)h * a.qh);
+  float qr[E], acc[E], mx = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    qr[e] = Elem<T>::to_f(q[lane * E + e]) * a.scale;
+    acc[e] = 0.f;
+  }
+  const int lo = tk.z > it.b0 ? tk.z : it.b0, hi = tk.w < it.b1 ? tk.w : it.b1;
+  const int np = it.a1 - it.a0, n = np + (hi > lo ? hi - lo : 0);
+  for (int j = 0; j < n; ++j) {
+    const int64_t s = j < np ? a.prefix_slots[it.a0 + j] : a.suffix_slots[lo + (j - np)];
+    const bool have = a.pv.valid(s);
+    float dot = 0.f, v[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      v[e] = 0.f;
+      if (have) {
+        dot += qr[e] * Elem<T>::to_f(*reinterpret_cast<const T*>(a.pv.addr(s, g, lane * E + e)));
+        v[e] = Elem<T>::to_f(*reinterpret_cast<const T*>(a.pv.addr(s, g, D + lane * E + e)));
+      }
+    }
+    dot = warp_sum(dot);
+    if (dot == -INFINITY) continue;
+    const float top = fmaxf(mx, dot);
+    const float keep = mx == -INFINITY ? 0.f : expf(mx - top), p = expf(dot - top);
+    mx = top;
+    sum = sum * keep + p;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = acc[e] * keep + p * v[e];
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float x = sum == 0.f ? 0.f : acc[e] / sum;
+    if (part) static_cast<float*>(out)[lane * E + e] = x;
+    else static_cast<T*>(out)[lane * E + e] = Elem<T>::from_f(x);
+  }
+}
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
@@ -453,13 +498,11 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       mbar_arrive(mb + Sh::bQ);
     }
     const int4 tk = row_ok ? a.tokens[it.tok0 + tok] : make_int4(0, 0, 0, 0);
-    const int first_hi = a.tokens[it.tok0].w, last_lo = a.tokens[it.tok0 + it.ntok - 1].z;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t sc = tmem + lane_base + Sh::cS + 128 * qt;
     const uint32_t oc = tmem + lane_base + Sh::cO + D * qt;
     float mref = -INFINITY, lsum = 0.f;  // log2 domain; P = 2^(x - mref + up)
     bool ok = true;
-    int checked = 0;
     // The tiles' softmaxes take turns, so that one tile's products run beside
     // the other's softmax: in step, both share the issue slots, then both wait
     // for the tensor unit (5850 clocks a key tile of 2 x 128 rows).
@@ -479,56 +522,13 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
         vlo = st.own ? (tk.z > st.base ? tk.z - st.base : 0) : 0;
         vhi = st.own ? (tk.w - st.base < st.n ? tk.w - st.base : st.n) : st.n;
       }
-      // Some row of the block may not see some key: a value that is not
-      // finite there would reach it as 0 x inf.  Such keys (bits of bad) leave
-      // the product and are added to the rows that see them below.
-      uint32_t bad[4] = {0u, 0u, 0u, 0u};
-      if (st.own && (last_lo > st.base || first_hi < st.base + st.n)) {
-        ok = ok && __all_sync(~0u, mbar_wait(mb + Sh::bV + 8 * (t % Sh::VS), (t / Sh::VS) & 1,
-                                             abort));
-        constexpr int C = D / 8;
-        const int c0 = tiles == 2 ? qt * (C / 2) : 0, c1 = tiles == 2 ? c0 + C / 2 : C;
-        const uint32_t vrow = sbase + Sh::oV + (t % Sh::VS) * Sh::TB;
-        bool nf = false;
-        if (ok) {
-          for (int c = c0; c < c1; ++c) {
-            const uint4 v = ld_shared16(vrow + sw128(r, c, kPrefixTile));
-            const uint32_t e = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
-            auto all_ones = [&](uint32_t w) {
-              const uint32_t x = w & e;
-              return (x & 0xffffu) == (e & 0xffffu) || (x >> 16) == (e >> 16);
-            };
-            nf |= all_ones(v.x) || all_ones(v.y) || all_ones(v.z) || all_ones(v.w);
-          }
-        }
-        const uint32_t word = __ballot_sync(~0u, nf);
-        volatile uint32_t* slot = reinterpret_cast<volatile uint32_t*>(
-            smem + Sh::oMeta + Sh::oBad + (checked & 1) * (16 * NT));
-        ++checked;
-        if (lane == 0) slot[warp] = word;
-        asm volatile("bar.sync 1, %0;" ::"r"(128 * tiles) : "memory");
-#pragma unroll
-        for (int w = 0; w < 4; ++w) bad[w] = slot[w] | (tiles == 2 ? slot[(w + 4) % (4 * NT)] : 0u);
-        if (ok && (bad[0] | bad[1] | bad[2] | bad[3])) {
-          if ((bad[r >> 5] >> (r & 31)) & 1u) {
-            for (int c = c0; c < c1; ++c)
-              st_shared16(vrow + sw128(r, c, kPrefixTile), make_uint4(0u, 0u, 0u, 0u));
-          }
-          fence_async_smem();
-        }
-        // the other tile's product must not start on half a cleared row
-        if (tiles == 2 && (bad[0] | bad[1] | bad[2] | bad[3]))
-          asm volatile("bar.sync 1, 256;" ::: "memory");
-      }
-      if (!ok) continue;  // a wait expired: only the barriers above are kept
+      if (!ok) break;  // a wait expired
       ok = __all_sync(~0u, mbar_wait(barS(qt, t), (t / Sh::KS) & 1, abort));
-      if (!ok) continue;
+      if (!ok) break;
       tc_fence_after();
-      if (tiles == 2) {
-        if (qt == 1 || t > 0) {
-          ok = __all_sync(~0u, mbar_wait(mb + Sh::bTurn + 8 * qt, (qt ? t : t - 1) & 1, abort));
-          if (!ok) continue;
-        }
+      if (tiles == 2 && (qt == 1 || t > 0)) {
+        ok = __all_sync(~0u, mbar_wait(mb + Sh::bTurn + 8 * qt, (qt ? t : t - 1) & 1, abort));
+        if (!ok) break;
       }
       uint32_t v[128];
       if (__all_sync(~0u, vhi <= vlo)) {  // nothing to see for these 32 rows
@@ -579,7 +579,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       const bool grow = top2 > mref + kLazy || mref == -INFINITY;
       const bool rescale = grow && mref > -INFINITY && top2 > mref;
       if (__any_sync(~0u, rescale)) {  // t > 0: a row has a finite maximum
-        if (!wait_pv(t - 1)) continue;
+        if (!wait_pv(t - 1)) break;
         const float f = rescale ? ex2(mref - top2) : 1.f;
         lsum *= f;
         uint32_t o[16];
@@ -628,37 +628,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       tc_fence_before();
       mbar_arrive(mb + Sh::bP + 8 * qt);
       pass_turn();
-
-      if (bad[0] | bad[1] | bad[2] | bad[3]) {
-        if (!wait_pv(t)) continue;
-        const int64_t* slots = a.suffix_slots + st.base;
-        for (int j = 0; j < st.n; ++j) {
-          if (!((bad[j >> 5] >> (j & 31)) & 1u)) continue;
-          const bool see = j >= vlo && j < vhi;
-          const T* rec = reinterpret_cast<const T*>(a.pv.addr(slots[j], g, 0));
-          const T* val = reinterpret_cast<const T*>(a.pv.addr(slots[j], g, D));
-          float dot = 0.f;
-          if (see) {
-            const T* q = reinterpret_cast<const T*>(a.q + (int64_t)(it.tok0 + tok) * a.qt +
-                                                    (int64_t)h * a.qh);
-            for (int e = 0; e < D; ++e) dot += Elem<T>::to_f(q[e]) * Elem<T>::to_f(rec[e]);
-          }
-          const float p = ex2(fmaf(dot, a.scale_signed2, -sub));
-#pragma unroll 1
-          for (int cc = 0; cc < D / 32; ++cc) {
-            CS_TMEM_LD32(oc + 32 * cc, v);
-            tmem_wait_ld();
-#pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (see)
-                v[c] = __float_as_uint(fmaf(p, Elem<T>::to_f(val[32 * cc + c]),
-                                            __uint_as_float(v[c])));
-            CS_TMEM_ST32(oc + 32 * cc, v);
-            tmem_wait_st();
-          }
-        }
-        tc_fence_before();
-      }
     }
 
     // ---------------------------------------------------------------- output
@@ -672,6 +641,11 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     const bool part = it.part >= 0;
     if (part) orow = reinterpret_cast<char*>(a.part_o + prow * D);
     const bool have = ok && steps > 0 && lsum != 0.f;
+    // An infinite or NaN value of a key that this row does not see reaches its
+    // sums as 0 x inf = NaN, so a row that is not finite is computed again
+    // below, from the keys it sees alone.
+    float worst = 0.f;
+    auto finite = [&](uint32_t x) { worst = max_nan(worst, fabsf(__uint_as_float(x))); };
     if (part || a.vec_out) {
       // each thread stages its row (32-bit partials in two halves) where the
       // queries were, and the warp writes whole rows: stores straight from the
@@ -690,8 +664,10 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
             CS_TMEM_LD32(oc + half * (D / 2) + 32 * cc, v);
             tmem_wait_ld();
 #pragma unroll
-            for (int c = 0; c < 32; ++c)
+            for (int c = 0; c < 32; ++c) {
               v[c] = have ? __float_as_uint(__uint_as_float(v[c]) * inv) : 0u;
+              finite(v[c]);
+            }
 #pragma unroll
             for (int c = 0; c < 8; ++c)
               st_shared16(buf + 128 * cc + 16 * c,
@@ -706,6 +682,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
             for (int c = 0; c < 16; ++c) {
               const float x = have ? __uint_as_float(v[2 * c]) * inv : 0.f;
               const float y = have ? __uint_as_float(v[2 * c + 1]) * inv : 0.f;
+              finite(__float_as_uint(x));
+              finite(__float_as_uint(y));
               v[c] = Pack2<T>::pack(x, y);
             }
 #pragma unroll
@@ -739,10 +717,22 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
         tmem_wait_ld();
         if (!row_ok || !ok) continue;
 #pragma unroll
-        for (int c = 0; c < 32; ++c)
-          reinterpret_cast<T*>(orow)[32 * cc + c] =
-              Elem<T>::from_f(have ? __uint_as_float(v[c]) * inv : 0.f);
+        for (int c = 0; c < 32; ++c) {
+          const float x = have ? __uint_as_float(v[c]) * inv : 0.f;
+          finite(__float_as_uint(x));
+          reinterpret_cast<T*>(orow)[32 * cc + c] = Elem<T>::from_f(x);
+        }
       }
+    }
+    __syncwarp();
+    for (uint32_t again = __ballot_sync(~0u, row_ok && have && !(worst < INFINITY)); again;
+         again &= again - 1) {
+      const int src = __ffs(again) - 1;
+      const int rr = r - lane + src;
+      const int tt = qt * a.R + rr / a.G, hh = g * a.G + rr % a.G;
+      row_again<T, D>(a, it, g, tt, hh, lane,
+                      reinterpret_cast<void*>(__shfl_sync(~0u, reinterpret_cast<uint64_t>(orow), src)),
+                      part);
     }
     if (row_ok && ok) {
       if (it.part >= 0) a.part_lse[prow] = lse2;
@@ -931,7 +921,7 @@ int prefix_attn_sm100(const cs_prefix_params& p, const cs_prefix_plan_info& info
   a.neg = p.scale < 0.0;
   // masked scores are -inf before they are scaled, so the factor is never 0
   a.scale2 = fmaxf(fabsf((float)p.scale) * kLog2e, 1e-30f);
-  a.scale_signed2 = a.neg ? -a.scale2 : a.scale2;
+  a.scale = (float)p.scale;
   a.nrb = a.nrh = a.nro = 0;
   a.tma = setup_maps(a, kv) ? 1 : 0;
   const bool half = kv.dtype == CS_F16;
