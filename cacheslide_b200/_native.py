@@ -284,7 +284,14 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+# the current stream's handle without a Stream object around it, where this
+# torch has that (a decode step calls this a few hundred times)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_of(device: torch.device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -330,12 +337,9 @@ def paged_view(
         raise ValueError("cache must be [blocks, kv_heads, block_size, 2*D]")
     if cache.dtype not in DTYPES:
         raise ValueError("cache dtype must be float16/bfloat16/float32/float64")
-    kv = PagedKV()
-    kv.cache = cache.data_ptr()
-    kv.num_blocks, kv.kv_heads, kv.block_size = cache.shape[0], cache.shape[1], cache.shape[2]
-    kv.head_dim = cache.shape[3] // 2
-    kv.stride_block, kv.stride_head, kv.stride_offset, kv.stride_elem = cache.stride()
-    kv.dtype = DTYPES[cache.dtype]
+    blocks, heads, block_size, width = cache.shape
+    kv = PagedKV(cache.data_ptr(), blocks, heads, block_size, width // 2, *cache.stride(),
+                 None, None, 0, 0, 0, 0, DTYPES[cache.dtype])
     if side_k is not None and side_v is not None:
         if side_k.stride() != side_v.stride() or side_k.shape != side_v.shape:
             raise ValueError("sidecar K and V must share shape and strides")

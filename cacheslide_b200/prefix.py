@@ -66,6 +66,7 @@ class SharedPrefixAttention:
         if members != len(query_lens):
             raise ValueError("group_sizes must add up to the requests")
         self.q_heads, self.kv_heads, self.head_dim = q_heads, kv_heads, head_dim
+        self.shape = torch.Size((self.tokens, q_heads, head_dim))
         self.dtype, self.device = dtype, torch.device(device)
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
@@ -99,16 +100,19 @@ class SharedPrefixAttention:
 
         A slot outside the pool reads as a zero key and value and sets
         ``ST_SLOT_RANGE`` in ``status``."""
-        shape = (self.tokens, self.q_heads, self.head_dim)
-        if query.shape != shape or query.dtype != self.dtype or query.device != self.device:
-            raise ValueError(f"query must be {self.dtype} {shape} on {self.device}")
+        shape, device = self.shape, self.device
+        index = device.index
+        if query.shape != shape or query.dtype is not self.dtype or query.get_device() != index:
+            raise ValueError(f"query must be {self.dtype} {tuple(shape)} on {device}")
         for name, slots, count in (("prefix_slots", prefix_slots, self.prefix_keys),
                                    ("suffix_slots", suffix_slots, self.suffix_keys)):
-            if slots.shape != (count,) or slots.dtype != torch.int64 or \
-                    slots.device != self.device or slots.stride(0) != 1 and count > 1:
+            if slots.shape != (count,) or slots.dtype is not torch.int64 or \
+                    slots.get_device() != index or count > 1 and slots.stride(0) != 1:
                 raise ValueError(f"{name} must be a contiguous int64 vector of {count} slots")
-        if query.stride(2) != 1:
+        qs = query.stride()
+        if qs[2] != 1:
             query = query.contiguous()
+            qs = query.stride()
         view = pool_view(kv)
         if view.dtype != N.DTYPES[self.dtype] or view.kv_heads != self.kv_heads \
                 or view.head_dim != self.head_dim:
@@ -118,22 +122,19 @@ class SharedPrefixAttention:
         elif not math.isfinite(scale):
             raise ValueError("scale must be finite")
         if out is None:
-            out = torch.empty(shape, dtype=self.dtype, device=self.device)
-        elif out.shape != shape or out.dtype != self.dtype or out.device != self.device \
+            out = torch.empty(shape, dtype=self.dtype, device=device)
+        elif out.shape != shape or out.dtype is not self.dtype or out.get_device() != index \
                 or out.stride(2) != 1:
             raise ValueError("out must match query, with a contiguous last dimension")
-        if self.device.type != "cuda":
-            N.require_cuda(query)
-        lse = torch.empty(shape[:2], dtype=torch.float32, device=self.device) \
-            if return_lse else None
+        os = out.stride()
+        lse = torch.empty(shape[:2], dtype=torch.float32, device=device) if return_lse else None
         p = N.PrefixParams(
-            query.data_ptr(), query.stride(0), query.stride(1), view, prefix_slots.data_ptr(),
-            suffix_slots.data_ptr(), self.q_heads, scale, out.data_ptr(), out.stride(0),
-            out.stride(1), N.ptr(lse), None if status is None else status.ptr)
+            query.data_ptr(), qs[0], qs[1], view, prefix_slots.data_ptr(),
+            suffix_slots.data_ptr(), self.q_heads, scale, out.data_ptr(), os[0], os[1],
+            N.ptr(lse), None if status is None else status.ptr)
         workspace = None
         if self.info.workspace:
-            workspace = torch.empty(self.info.workspace, dtype=torch.uint8, device=self.device)
-        N.check(N.load().cs_prefix_attn(
-            ctypes.byref(p), ctypes.byref(self.info), self.words.data_ptr(), N.ptr(workspace),
-            N.stream_of(self.device)), "cs_prefix_attn")
+            workspace = torch.empty(self.info.workspace, dtype=torch.uint8, device=device)
+        N.check(N.load().cs_prefix_attn(p, self.info, self.words.data_ptr(), N.ptr(workspace),
+                                        N.stream_of(device)), "cs_prefix_attn")
         return (out, lse) if return_lse else out

@@ -19,8 +19,6 @@ what ``append_rotated`` writes.
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 from torch import Tensor
 
@@ -46,79 +44,85 @@ def rotary_tables(positions: int, rotary_dim: int, *, base: float = 10000.0,
 
 
 def _rows(name: str, x: Tensor) -> Tensor:
-    if not isinstance(x, Tensor) or x.ndim != 3 or x.dtype not in _TYPES:
+    if not isinstance(x, Tensor) or x.dim() != 3 or x.dtype not in _TYPES:
         raise ValueError(f"{name} must be float32/float16/bfloat16 [token, head, dim]")
     return x if x.stride(2) == 1 else x.contiguous()
 
 
+def _weight(w: Tensor, dim: int, device: int) -> int:
+    if w.shape != (dim,) or w.dtype not in _TYPES or w.stride(0) != 1 and dim > 1:
+        raise ValueError("norm weights must be contiguous floating [head dim]")
+    if w.get_device() != device:
+        raise ValueError("all tensors must be on the same CUDA device")
+    return w.data_ptr()
+
+
 def _params(query: Tensor | None, key: Tensor, positions: Tensor, cos: Tensor, sin: Tensor,
-            q_weight: Tensor | None, k_weight: Tensor | None, eps: float,
-            interleaved: bool) -> N.RotaryParams:
-    """The checks every entry point shares; fills everything but the outputs."""
-    tokens, _, dim = key.shape
-    dtype, device = key.dtype, key.device
-    if query is not None and (query.shape[0] != tokens or query.shape[2] != dim
-                              or query.dtype != dtype):
-        raise ValueError("query and key must share tokens, head dim and dtype")
+            q_weight: Tensor | None, k_weight: Tensor | None, eps: float, interleaved: bool,
+            q_out: Tensor | None, k_out: Tensor | None,
+            status: N.Status | None) -> N.RotaryParams:
+    """The checks every entry point shares, and the C struct of the call."""
+    tokens, k_heads, dim = key.shape
+    dtype, device = key.dtype, key.get_device()
     if dim % 2 or not 2 <= dim <= MAX_HEAD_DIM:
         raise ValueError(f"head dim must be even and at most {MAX_HEAD_DIM}")
-    if (positions.ndim != 1 or positions.dtype != torch.int64 or positions.shape[0] != tokens
-            or positions.stride(0) != 1 and tokens > 1):
+    if (positions.shape != (tokens,) or positions.dtype is not torch.int64
+            or tokens > 1 and positions.stride(0) != 1):
         raise ValueError("positions must be a contiguous int64 [token] vector")
-    if (cos.ndim != 2 or cos.dtype != torch.float32 or sin.dtype != torch.float32
-            or cos.shape != sin.shape or cos.stride() != sin.stride() or cos.stride(1) != 1
-            and cos.shape[1] > 1):
+    strides = cos.stride()
+    if (len(strides) != 2 or cos.dtype is not torch.float32 or sin.dtype is not torch.float32
+            or cos.shape != sin.shape or strides != sin.stride()
+            or strides[1] != 1 and cos.shape[1] > 1):
         raise ValueError("cos and sin must be float32 [position, rotary_dim / 2]")
-    rot = 2 * cos.shape[1]
-    if rot > dim:
+    rows, half = cos.shape
+    if 2 * half > dim:
         raise ValueError("the rotated part is larger than the head")
     if not eps >= 0.0:
         raise ValueError("eps must be nonnegative")
-    weights = [w for w in (q_weight, k_weight) if w is not None]
-    for w in weights:
-        if w.shape != (dim,) or w.dtype not in _TYPES or w.dtype != weights[0].dtype \
-                or w.stride(0) != 1:
-            raise ValueError("norm weights must be contiguous floating [head dim] of one dtype")
-    for t in (query, positions, cos, sin, *weights):
-        if t is not None and t.device != device:
-            raise ValueError("all tensors must be on the same CUDA device")
-    if device.type != "cuda":
-        N.require_cuda(key)
-    p = N.RotaryParams()
-    p.cos, p.sin = cos.data_ptr(), sin.data_ptr()
-    p.table_rows, p.table_stride = cos.shape[0], cos.stride(0)
-    p.positions, p.tokens = positions.data_ptr(), tokens
-    p.head_dim, p.rot, p.interleaved = dim, rot, 1 if interleaved else 0
-    p.dtype = N.DTYPES[dtype]
-    p.eps = eps
-    if weights:
-        p.weight_dtype = N.DTYPES[weights[0].dtype]
-        p.q_weight, p.k_weight = N.ptr(q_weight), N.ptr(k_weight)
+    if (positions.get_device() != device or cos.get_device() != device
+            or sin.get_device() != device):
+        raise ValueError("all tensors must be on the same CUDA device")
+    qw = kw = None
+    weight_dtype = 0
+    if q_weight is not None:
+        qw = _weight(q_weight, dim, device)
+        weight_dtype = N.DTYPES[q_weight.dtype]
+    if k_weight is not None:
+        kw = _weight(k_weight, dim, device)
+        if q_weight is not None and k_weight.dtype is not q_weight.dtype:
+            raise ValueError("norm weights must share a dtype")
+        weight_dtype = N.DTYPES[k_weight.dtype]
+    q = (None, 0, 0, 0)
     if query is not None:
-        p.q, p.q_heads = query.data_ptr(), query.shape[1]
-        p.q_stride_tok, p.q_stride_head = query.stride(0), query.stride(1)
-    p.k, p.k_heads = key.data_ptr(), key.shape[1]
-    p.k_stride_tok, p.k_stride_head = key.stride(0), key.stride(1)
-    return p
-
-
-def _outputs(p: N.RotaryParams, q_out: Tensor | None, k_out: Tensor | None) -> None:
+        q_tokens, q_heads, q_dim = query.shape
+        if q_tokens != tokens or q_dim != dim or query.dtype is not dtype:
+            raise ValueError("query and key must share tokens, head dim and dtype")
+        if query.get_device() != device:
+            raise ValueError("all tensors must be on the same CUDA device")
+        st = query.stride()
+        q = (query.data_ptr(), st[0], st[1], q_heads)
+    if device < 0:
+        N.require_cuda(key)
+    qo = ko = (None, 0, 0)
     if q_out is not None:
-        p.q_out, p.qo_stride_tok, p.qo_stride_head = (q_out.data_ptr(), q_out.stride(0),
-                                                      q_out.stride(1))
+        st = q_out.stride()
+        qo = (q_out.data_ptr(), st[0], st[1])
     if k_out is not None:
-        p.k_out, p.ko_stride_tok, p.ko_stride_head = (k_out.data_ptr(), k_out.stride(0),
-                                                      k_out.stride(1))
+        st = k_out.stride()
+        ko = (k_out.data_ptr(), st[0], st[1])
+    st = key.stride()
+    return N.RotaryParams(
+        cos.data_ptr(), sin.data_ptr(), rows, strides[0], positions.data_ptr(), tokens, dim,
+        2 * half, 1 if interleaved else 0, N.DTYPES[dtype], weight_dtype, eps, *q, qw, *qo,
+        key.data_ptr(), st[0], st[1], k_heads, kw, *ko, None if status is None else status.ptr)
 
 
 def _forward(query, key, positions, cos, sin, q_weight, k_weight, eps, interleaved, status):
-    p = _params(query, key, positions, cos, sin, q_weight, k_weight, eps, interleaved)
     q_out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
     k_out = torch.empty(key.shape, dtype=key.dtype, device=key.device)
-    _outputs(p, q_out, k_out)
-    p.status = None if status is None else status.ptr
-    N.check(N.load().cs_qk_norm_rope(ctypes.byref(p), N.stream_of(key.device)),
-            "cs_qk_norm_rope")
+    p = _params(query, key, positions, cos, sin, q_weight, k_weight, eps, interleaved, q_out,
+                k_out, status)
+    N.check(N.load().cs_qk_norm_rope(p, N.stream_of(key.device)), "cs_qk_norm_rope")
     return q_out, k_out
 
 
@@ -136,19 +140,18 @@ class _NormRope(torch.autograd.Function):
     def backward(ctx, q_dy, k_dy):
         query, key, positions, cos, sin, q_weight, k_weight = ctx.saved_tensors
         eps, interleaved, status = ctx.how
-        p = _params(query, key, positions, cos, sin, q_weight, k_weight, eps, interleaved)
         q_dy, k_dy = q_dy.contiguous(), k_dy.contiguous()
         dq, dk = torch.empty_like(q_dy), torch.empty_like(k_dy)
-        _outputs(p, dq, dk)
-        p.status = None if status is None else status.ptr
+        p = _params(query, key, positions, cos, sin, q_weight, k_weight, eps, interleaved, dq, dk,
+                    status)
         dqw = None if q_weight is None else torch.empty_like(q_weight)
         dkw = None if k_weight is None else torch.empty_like(k_weight)
         lib = N.load()
-        size = lib.cs_qk_norm_rope_grad_workspace(ctypes.byref(p))
-        workspace = torch.empty(size, dtype=torch.uint8, device=key.device)
+        workspace = torch.empty(lib.cs_qk_norm_rope_grad_workspace(p), dtype=torch.uint8,
+                                device=key.device)
         N.check(lib.cs_qk_norm_rope_grad(
-            ctypes.byref(p), q_dy.data_ptr(), k_dy.data_ptr(), N.ptr(dqw), N.ptr(dkw),
-            workspace.data_ptr(), N.stream_of(key.device)), "cs_qk_norm_rope_grad")
+            p, q_dy.data_ptr(), k_dy.data_ptr(), N.ptr(dqw), N.ptr(dkw), workspace.data_ptr(),
+            N.stream_of(key.device)), "cs_qk_norm_rope_grad")
         return dq, dk, None, None, None, dqw, dkw, None, None, None
 
 
@@ -203,28 +206,29 @@ def append_rotated(kv: Tensor | NativePagedKV | N.PagedKV, slots: Tensor, key: T
     slot map's guards are the caller's: this writes where it is told, as a
     model runner's cache write does."""
     key, value = _rows("key", key), _rows("value", value)
-    if value.shape != key.shape or value.dtype != key.dtype or value.device != key.device:
+    device = key.get_device()
+    if value.shape != key.shape or value.dtype is not key.dtype or value.get_device() != device:
         raise ValueError("key and value must share shape, dtype and device")
+    tokens = key.shape[0]
+    if (slots.shape != (tokens,) or slots.dtype is not torch.int64
+            or slots.get_device() != device or tokens > 1 and slots.stride(0) != 1):
+        raise ValueError("slots must be a contiguous int64 [token] vector")
+    view = pool_view(kv)
     if query is not None:
         query = _rows("query", query)
-    view = pool_view(kv)
-    p = _params(query, key, positions, cos, sin, q_weight, k_weight, eps, interleaved)
-    if view.dtype != p.dtype or view.kv_heads != p.k_heads or view.head_dim != p.head_dim:
-        raise ValueError("K/V must match the pool's dtype, KV heads and head dim")
-    if (slots.ndim != 1 or slots.dtype != torch.int64 or slots.shape[0] != key.shape[0]
-            or slots.device != key.device or slots.stride(0) != 1 and slots.shape[0] > 1):
-        raise ValueError("slots must be a contiguous int64 [token] vector")
-    if query is not None:
         if out is None:
             out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-        elif (out.shape != query.shape or out.dtype != query.dtype or out.device != query.device
-              or out.stride(2) != 1):
+        elif (out.shape != query.shape or out.dtype is not query.dtype
+              or out.get_device() != device or out.stride(2) != 1):
             raise ValueError("out must match query, with a contiguous last dimension")
-        _outputs(p, out, None)
     elif out is not None or q_weight is not None:
         raise ValueError("out and q_weight need a query")
-    p.status = None if status is None else status.ptr
-    N.check(N.load().cs_kv_append_rotated(
-        ctypes.byref(p), ctypes.byref(view), slots.data_ptr(), value.data_ptr(), value.stride(0),
-        value.stride(1), N.stream_of(key.device)), "cs_kv_append_rotated")
+    p = _params(query, key, positions, cos, sin, q_weight, k_weight, eps, interleaved, out, None,
+                status)
+    if view.dtype != p.dtype or view.kv_heads != p.k_heads or view.head_dim != p.head_dim:
+        raise ValueError("K/V must match the pool's dtype, KV heads and head dim")
+    st = value.stride()
+    N.check(N.load().cs_kv_append_rotated(p, view, slots.data_ptr(), value.data_ptr(), st[0],
+                                          st[1], N.stream_of(key.device)),
+            "cs_kv_append_rotated")
     return out
