@@ -32,6 +32,7 @@
 namespace cs {
 namespace {
 
+constexpr int kHalf = kPrefixTile / 2;  // keys of a sub-step: scores, softmax, P V
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -74,28 +75,23 @@ struct Shape {
   static constexpr int kSoft = 4 * NT;
   // one more warpgroup: K, V, NT MMA warps (and an idle one beside one tile)
   static constexpr int kThreads = 128 * (NT + 1);
-  // registers a thread: at launch, then the softmax warpgroups' (a row's 128
-  // scores live in them) and the other warpgroup's
-  static constexpr int kLaunch = NT == 1 ? 128 : 168;
-  static constexpr int kSoftRegs = NT == 1 ? 184 : 200;
-  static constexpr int kOtherRegs = NT == 1 ? 72 : 96;
-  static_assert(128 * NT * kSoftRegs + 128 * kOtherRegs <= kThreads * kLaunch,
-                "register split exceeds the block's launch allocation");
   static constexpr uint32_t TB = kPrefixTile * D * 2;
   // a query tile's place also takes its output rows, 2 D bytes each and 16 more
   static constexpr uint32_t QB = TB + 128 * 16;
   static constexpr uint32_t oQ = 0, oK = NT * QB, oV = oK + KS * TB, oMeta = oV + VS * TB;
-  // barriers, 8 bytes each
-  static constexpr uint32_t bQ = 0, bK = 8, bV = bK + 8 * KS, bS = bV + 8 * VS,
-                            bP = bS + 8 * NT * KS, bPV = bP + 8 * NT, bTurn = bPV + 8 * NT * VS,
-                            oTmem = bTurn + 16, oAbort = oTmem + 4, 
+  // barriers, 8 bytes each; S, P and PV a score buffer of a row tile, K / V and
+  // their "read" barriers a stage
+  static constexpr uint32_t bQ = 0, bK = 8, bV = bK + 8 * KS, bKr = bV + 8 * VS,
+                            bVr = bKr + 8 * KS, bS = bVr + 8 * VS, bP = bS + 16 * NT,
+                            bPV = bP + 16 * NT, oTmem = bPV + 16 * NT, oAbort = oTmem + 4,
                             oRows = (oAbort + 4 + 15) / 16 * 16,
                             kMeta = oRows + 2 * 128 * 8;
   static_assert(oMeta % 1024 == 0 && oRows % 16 == 0 && oTmem % 4 == 0,
                 "alignment of the shared-memory places");
   static constexpr uint32_t kSmem = oMeta + kMeta + 1024;  // the base is rounded up to 1024
   static constexpr uint32_t kCols = 256 * NT;
-  static constexpr uint32_t cS = 0, cO = 128 * NT;  // S of tile i at 128 i, O at cO + D i
+  // two score buffers of 64 columns at 128 i for row tile i, O at cO + D i
+  static constexpr uint32_t cS = 0, cO = 128 * NT;
 };
 
 // the larger of the two, NaN if either is
@@ -299,11 +295,13 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     mbar_init(mb + Sh::bQ, 128 * tiles);
     for (int s = 0; s < Sh::KS; ++s) mbar_init(mb + Sh::bK + 8 * s, 32);
     for (int s = 0; s < Sh::VS; ++s) mbar_init(mb + Sh::bV + 8 * s, 32);
-    for (int s = 0; s < NT * Sh::KS; ++s) mbar_init(mb + Sh::bS + 8 * s, 1);
-    for (int s = 0; s < NT; ++s) mbar_init(mb + Sh::bP + 8 * s, 128);
-    for (int s = 0; s < NT * Sh::VS; ++s) mbar_init(mb + Sh::bPV + 8 * s, 1);
-    mbar_init(mb + Sh::bTurn, 128);
-    mbar_init(mb + Sh::bTurn + 8, 128);
+    for (int s = 0; s < Sh::KS; ++s) mbar_init(mb + Sh::bKr + 8 * s, tiles);
+    for (int s = 0; s < Sh::VS; ++s) mbar_init(mb + Sh::bVr + 8 * s, tiles);
+    for (int s = 0; s < 2 * NT; ++s) {
+      mbar_init(mb + Sh::bS + 8 * s, 1);
+      mbar_init(mb + Sh::bP + 8 * s, 128);
+      mbar_init(mb + Sh::bPV + 8 * s, 1);
+    }
     *abort = 0;
     mbar_init_fence();
     if (a.tma)
@@ -320,23 +318,20 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + Sh::oMeta + Sh::oTmem);
-  auto barS = [&](int qt, int t) { return mb + Sh::bS + 8 * (qt * Sh::KS + t % Sh::KS); };
-  auto barPV = [&](int qt, int t) { return mb + Sh::bPV + 8 * (qt * Sh::VS + t % Sh::VS); };
+  // sub-step u (64 keys) uses score buffer u & 1 of its row tile
+  auto at = [&](uint32_t bar, int qt, int u) { return mb + bar + 8 * (2 * qt + (u & 1)); };
+  auto halves = [&](int t) { return step_of(it, na, t).n > kHalf ? 2 : 1; };
 
   if (warp == Sh::kSoft || warp == Sh::kSoft + 1) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Sh::kOtherRegs));
     // ============================================== producers: K, then V warp
     const int ST = isv ? Sh::VS : Sh::KS;
     Src nxt;
     int issued = 0;
     for (int t = 0; t < steps; ++t) {
-      // the stage is free once every tile's product of its last use is done
-      if (t >= ST) {
-        bool ok = true;
-        for (int qt = 0; qt < tiles; ++qt)
-          ok = ok && mbar_wait(isv ? barPV(qt, t) : barS(qt, t), (t / ST - 1) & 1, abort);
-        if (!__all_sync(~0u, ok)) break;
-      }
+      // the stage is free once every row tile is done with its last use
+      if (t >= ST && !__all_sync(~0u, mbar_wait(mb + (isv ? Sh::bVr : Sh::bKr) + 8 * (t % ST),
+                                                (t / ST - 1) & 1, abort)))
+        break;
       const uint32_t bar = mb + (isv ? Sh::bV : Sh::bK) + 8 * (t % ST);
       const uint32_t dst = sbase + (isv ? Sh::oV : Sh::oK) + (t % ST) * Sh::TB;
       // 16 keys (4 lanes) in consecutive rows: one TMA box an operand half;
@@ -399,7 +394,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     if (slot_bad) report(a.status, CS_ST_SLOT_RANGE);
 
   } else if (warp >= Sh::kSoft + 2) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Sh::kOtherRegs));
     // ==================================================== MMA, one warp a tile
     // The whole warp walks the steps, so that descriptors stay in uniform
     // registers; one elected lane issues.  (One lane alone, with descriptors
@@ -407,7 +401,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     const int qt = __shfl_sync(~0u, warp, 0) - (Sh::kSoft + 2);
     if (qt < tiles) {
       const bool leader = elect_one();
-      const uint32_t id_s = umma_idesc(128, 128, umma_format<T>(), 0, 0);
+      const uint32_t id_s = umma_idesc(128, kHalf, umma_format<T>(), 0, 0);
       const uint32_t id_o = umma_idesc(128, D, umma_format<T>(), 0, 1);  // V is MN-major
       const uint64_t dq = umma_desc(sbase + Sh::oQ + qt * Sh::QB, 16, 1024);
       const uint64_t dk0 = umma_desc(sbase + Sh::oK, 16, 1024);
@@ -416,39 +410,66 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       const uint32_t sc = tm + Sh::cS + 128 * qt, oc = tm + Sh::cO + D * qt;
       bool ok = mbar_spin(mb + Sh::bQ, 0, abort);
       uint32_t last = 0, lastph = 0;  // the newest group issued
-      for (int t = 0; ok && t < steps; ++t) {
-        const int ks = t % Sh::KS, vs = t % Sh::VS;
-        const uint64_t dk = dk0 + (uint64_t)(ks * (Sh::TB >> 4));
-        const uint64_t dv = dv0 + (uint64_t)(vs * (Sh::TB >> 4));
-        if (!(ok = mbar_spin(mb + Sh::bK + 8 * ks, (t / Sh::KS) & 1, abort))) break;
-        // S takes the columns that P of the last step lies in
-        if (t > 0 && !(ok = mbar_spin(barPV(qt, t - 1), ((t - 1) / Sh::VS) & 1, abort))) break;
-        fence_async_smem();  // rows copied by cp.async
+      int qk_t = 0, qk_h = 0, qk_u = 0;  // the next scores to compute
+      auto scores = [&]() {
+        if (qk_h == 0) {
+          ok = mbar_spin(mb + Sh::bK + 8 * (qk_t % Sh::KS), (qk_t / Sh::KS) & 1, abort);
+          if (!ok) return;
+          fence_async_smem();  // rows copied by cp.async
+        }
         tc_fence_after();
-        last = barS(qt, t);
-        lastph = (t / Sh::KS) & 1;
+        const uint64_t dk = dk0 + (uint64_t)((qk_t % Sh::KS) * (Sh::TB >> 4) + qk_h * 512);
+        const uint32_t s = sc + kHalf * (qk_u & 1);
+        last = at(Sh::bS, qt, qk_u);
+        lastph = (qk_u >> 1) & 1;
         if (leader) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint64_t off = (kk >> 2) * 1024 + (kk & 3) * 2;  // 16-byte units
-            tc_mma(sc, dq + off, dk + off, id_s, kk ? 1u : 0u);
+            tc_mma(s, dq + off, dk + off, id_s, kk ? 1u : 0u);
           }
           tc_commit(last);
         }
         __syncwarp();
-        if (!(ok = mbar_spin(mb + Sh::bP + 8 * qt, t & 1, abort))) break;
-        if (!(ok = mbar_spin(mb + Sh::bV + 8 * vs, (t / Sh::VS) & 1, abort))) break;
-        fence_async_smem();
-        tc_fence_after();
-        last = barPV(qt, t);
-        lastph = (t / Sh::VS) & 1;
-        if (leader) {
-#pragma unroll
-          for (int kk = 0; kk < kPrefixTile / 16; ++kk)
-            tc_mma_ts(oc, sc + kk * 8, dv + kk * 128, id_o, (t | kk) ? 1u : 0u);
-          tc_commit(last);
+        ++qk_u;
+        if (++qk_h == halves(qk_t)) {
+          qk_h = 0;
+          ++qk_t;
         }
-        __syncwarp();
+      };
+      if (ok && steps > 0) scores();
+      if (ok && qk_t < steps) scores();
+      int u = 0;
+      for (int t = 0; ok && t < steps; ++t) {
+        const int nh = halves(t);
+        for (int h = 0; ok && h < nh; ++h, ++u) {
+          const uint32_t ph = (u >> 1) & 1;
+          if (!(ok = mbar_spin(at(Sh::bP, qt, u), ph, abort))) break;
+          if (h == 0) {
+            if (!(ok = mbar_spin(mb + Sh::bV + 8 * (t % Sh::VS), (t / Sh::VS) & 1, abort))) break;
+            fence_async_smem();
+          }
+          tc_fence_after();
+          const uint64_t dv = dv0 + (uint64_t)((t % Sh::VS) * (Sh::TB >> 4) + h * 512);
+          const uint32_t p = sc + kHalf * (u & 1);
+          last = at(Sh::bPV, qt, u);
+          lastph = ph;
+          if (leader) {
+#pragma unroll
+            for (int kk = 0; kk < kHalf / 16; ++kk)
+              tc_mma_ts(oc, p + kk * 8, dv + kk * 128, id_o, (u | kk) ? 1u : 0u);
+            tc_commit(last);
+          }
+          __syncwarp();
+          // the next scores but one take the buffer that P lies in, and the
+          // next V tile but VS - 1 the stage just read
+          const bool refill = h == nh - 1 && t + Sh::VS < steps;
+          if (qk_t < steps || refill) {
+            if (!(ok = mbar_spin(last, ph, abort))) break;
+            if (refill && leader) mbar_arrive(mb + Sh::bVr + 8 * (t % Sh::VS));
+            if (qk_t < steps) scores();
+          }
+        }
       }
       if (last) {
         const long long t0 = clock64();
@@ -459,7 +480,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     __syncwarp();
 
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Sh::kSoftRegs));
     if ((warp >> 2) < tiles) {
     // ================================================== softmax, a thread a row
     const int qt = warp >> 2;
@@ -499,58 +519,53 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     }
     const int4 tk = row_ok ? a.tokens[it.tok0 + tok] : make_int4(0, 0, 0, 0);
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t sc = tmem + lane_base + Sh::cS + 128 * qt;
+    const uint32_t sc0 = tmem + lane_base + Sh::cS + 128 * qt;
     const uint32_t oc = tmem + lane_base + Sh::cO + D * qt;
     float mref = -INFINITY, lsum = 0.f;  // log2 domain; P = 2^(x - mref + up)
     bool ok = true;
-    // The tiles' softmaxes take turns, so that one tile's products run beside
-    // the other's softmax: in step, both share the issue slots, then both wait
-    // for the tensor unit (5850 clocks a key tile of 2 x 128 rows).
-    auto pass_turn = [&] {
-      if (tiles == 2) mbar_arrive(mb + Sh::bTurn + 8 * (1 - qt));
-    };
-    auto wait_pv = [&](int t) {
-      ok = __all_sync(~0u, mbar_wait(barPV(qt, t), (t / Sh::VS) & 1, abort));
+    auto wait_pv = [&](int u) {
+      ok = __all_sync(~0u, mbar_wait(at(Sh::bPV, qt, u), (u >> 1) & 1, abort));
       tc_fence_after();
       return ok;
     };
 
-    for (int t = 0; t < steps; ++t) {
-      const Step st = step_of(it, na, t);
+    int u = 0;
+    for (int t = 0, h2 = 0; t < steps; ++u) {
+      Step st = step_of(it, na, t);
+      const bool last_half = h2 == 1 || st.n <= kHalf;
+      st.base += kHalf * h2;
+      st.n = st.n - kHalf * h2 < kHalf ? st.n - kHalf * h2 : kHalf;
+      const int stage = t % Sh::KS;
+      if (last_half) ++t, h2 = 0;
+      else h2 = 1;
       int vlo = 0, vhi = 0;
       if (row_ok) {
         vlo = st.own ? (tk.z > st.base ? tk.z - st.base : 0) : 0;
         vhi = st.own ? (tk.w - st.base < st.n ? tk.w - st.base : st.n) : st.n;
       }
+      const uint32_t sc = sc0 + kHalf * (u & 1);
+      ok = __all_sync(~0u, mbar_wait(at(Sh::bS, qt, u), (u >> 1) & 1, abort));
       if (!ok) break;  // a wait expired
-      ok = __all_sync(~0u, mbar_wait(barS(qt, t), (t / Sh::KS) & 1, abort));
-      if (!ok) break;
+      if (last_half && (tid & 127) == 0) mbar_arrive(mb + Sh::bKr + 8 * stage);
       tc_fence_after();
-      if (tiles == 2 && (qt == 1 || t > 0)) {
-        ok = __all_sync(~0u, mbar_wait(mb + Sh::bTurn + 8 * qt, (qt ? t : t - 1) & 1, abort));
-        if (!ok) break;
-      }
-      uint32_t v[128];
+      uint32_t v[kHalf];
       if (__all_sync(~0u, vhi <= vlo)) {  // nothing to see for these 32 rows
 #pragma unroll
         for (int c = 0; c < 16; ++c) v[c] = 0u;
-#pragma unroll
-        for (int cc = 0; cc < 4; ++cc) CS_TMEM_ST16(sc + 16 * cc, v);
+        CS_TMEM_ST16(sc, v);
+        CS_TMEM_ST16(sc + 16, v);
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(mb + Sh::bP + 8 * qt);
-        pass_turn();
+        mbar_arrive(at(Sh::bP, qt, u));
         continue;
       }
       CS_TMEM_LD32(sc, v);
       CS_TMEM_LD32(sc + 32, (v + 32));
-      CS_TMEM_LD32(sc + 64, (v + 64));
-      CS_TMEM_LD32(sc + 96, (v + 96));
       tmem_wait_ld();
-      const bool whole = __all_sync(~0u, vlo <= 0 && vhi >= kPrefixTile);
+      const bool whole = __all_sync(~0u, vlo <= 0 && vhi >= kHalf);
       if (!whole) {
 #pragma unroll
-        for (int cc = 0; cc < 4; ++cc) {
+        for (int cc = 0; cc < 2; ++cc) {
           const uint32_t bits = col_bits(vlo, vhi, 32 * cc);
 #pragma unroll
           for (int c = 0; c < 32; ++c)
@@ -564,7 +579,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
         for (int k = 0; k < 4; ++k)
           m[k] = max_nan(__uint_as_float(v[k]), __uint_as_float(v[k + 4]));
 #pragma unroll
-        for (int c = 8; c < kPrefixTile; c += 8) {
+        for (int c = 8; c < kHalf; c += 8) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             m[k] = max3_nan(m[k], __uint_as_float(v[c + k]), __uint_as_float(v[c + k + 4]));
@@ -578,8 +593,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       const float top2 = top == -INFINITY ? -INFINITY : top * a.scale2;
       const bool grow = top2 > mref + kLazy || mref == -INFINITY;
       const bool rescale = grow && mref > -INFINITY && top2 > mref;
-      if (__any_sync(~0u, rescale)) {  // t > 0: a row has a finite maximum
-        if (!wait_pv(t - 1)) break;
+      if (__any_sync(~0u, rescale)) {  // u > 0: a row has a finite maximum
+        if (!wait_pv(u - 1)) break;
         const float f = rescale ? ex2(mref - top2) : 1.f;
         lsum *= f;
         uint32_t o[16];
@@ -602,7 +617,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       const bool poly = whole && __all_sync(~0u, mref > -INFINITY);
       float2 s0 = make_float2(0.f, 0.f), s1 = s0;
 #pragma unroll
-      for (int cc = 0; cc < 4; ++cc) {
+      for (int cc = 0; cc < 2; ++cc) {
         uint32_t* w = v + 32 * cc;
         auto weight = [&](int c, bool fma_units) {
           float2 x = __ffma2_rn(make_float2(__uint_as_float(w[2 * c]), __uint_as_float(w[2 * c + 1])),
@@ -626,12 +641,11 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       lsum += (s0.x + s0.y) + (s1.x + s1.y);
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(mb + Sh::bP + 8 * qt);
-      pass_turn();
+      mbar_arrive(at(Sh::bP, qt, u));
     }
 
     // ---------------------------------------------------------------- output
-    if (ok && steps > 0) wait_pv(steps - 1);
+    if (ok && u > 0) wait_pv(u - 1);
     const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
     const float lse2 = lsum == 0.f ? -INFINITY
                                    : (mref > -INFINITY ? mref : 0.f) - p_up<T>() + log2f(lsum);
@@ -852,15 +866,9 @@ int launch_dependent(K kernel, unsigned blocks, int threads, uint32_t smem, cuda
 template <typename T, int D, int NT>
 int launch_main(const PArgs& a, int64_t blocks, cudaStream_t stream) {
   auto kernel = prefix_sm100_kernel<T, D, NT>;
-  // once per kernel: the register split inside it (setmaxnreg) is only sound
-  // when the block was launched with the registers it assumes
-  static const bool ready = [&] {
-    cudaFuncAttributes at;
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                Shape<D, NT>::kSmem) == cudaSuccess &&
-           cudaFuncGetAttributes(&at, kernel) == cudaSuccess &&
-           at.numRegs == Shape<D, NT>::kLaunch;
-  }();
+  static const bool ready =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           Shape<D, NT>::kSmem) == cudaSuccess;
   if (!ready) return CS_ERR_CUDA;
   return launch_dependent(kernel, (unsigned)blocks, Shape<D, NT>::kThreads, Shape<D, NT>::kSmem,
                           stream, a);
