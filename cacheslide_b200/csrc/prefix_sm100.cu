@@ -32,7 +32,7 @@
 namespace cs {
 namespace {
 
-constexpr int kHalf = kPrefixTile / 2;  // keys of a sub-step: scores, softmax, P V
+constexpr int kKeys = 64;  // keys of a step: one K and V tile, scores, softmax, P V
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -69,15 +69,18 @@ constexpr float kLazy = 8.f;  // O is rescaled when the maximum grew by more tha
 
 template <int D, int NT>
 struct Shape {
-  // key tiles in flight: two where they fit beside the queries
-  static constexpr int KS = (D == 64 || NT == 2) ? 2 : 1;
-  static constexpr int VS = KS;
+  // key tiles in flight; two blocks of one row tile share an SM
+  static constexpr int KS = NT == 2 ? 4 : 2, VS = KS;
+  // A stage of two is free with the product before last, whose barrier cannot
+  // move on before the stage is filled again; deeper rings have barriers of
+  // their own for "read".
+  static constexpr bool kDirect = KS == 2;
   static constexpr int kSoft = 4 * NT;
   // one more warpgroup: K, V, NT MMA warps (and an idle one beside one tile)
   static constexpr int kThreads = 128 * (NT + 1);
-  static constexpr uint32_t TB = kPrefixTile * D * 2;
+  static constexpr uint32_t TB = kKeys * D * 2;  // a K or V tile
   // a query tile's place also takes its output rows, 2 D bytes each and 16 more
-  static constexpr uint32_t QB = TB + 128 * 16;
+  static constexpr uint32_t QB = kPrefixTile * D * 2 + 128 * 16;
   static constexpr uint32_t oQ = 0, oK = NT * QB, oV = oK + KS * TB, oMeta = oV + VS * TB;
   // barriers, 8 bytes each; S, P and PV a score buffer of a row tile, K / V and
   // their "read" barriers a stage
@@ -85,7 +88,7 @@ struct Shape {
                             bVr = bKr + 8 * KS, bS = bVr + 8 * VS, bP = bS + 16 * NT,
                             bPV = bP + 16 * NT, oTmem = bPV + 16 * NT, oAbort = oTmem + 4,
                             oRows = (oAbort + 4 + 15) / 16 * 16,
-                            kMeta = oRows + 2 * 128 * 8;
+                            kMeta = oRows + 2 * kKeys * 8;
   static_assert(oMeta % 1024 == 0 && oRows % 16 == 0 && oTmem % 4 == 0,
                 "alignment of the shared-memory places");
   static constexpr uint32_t kSmem = oMeta + kMeta + 1024;  // the base is rounded up to 1024
@@ -134,9 +137,9 @@ struct Step {
 __device__ __forceinline__ Step step_of(const PrefixItem& it, int na, int t) {
   Step s;
   s.own = t >= na;
-  s.base = s.own ? it.b0 + (t - na) * kPrefixTile : it.a0 + t * kPrefixTile;
+  s.base = s.own ? it.b0 + (t - na) * kKeys : it.a0 + t * kKeys;
   const int end = s.own ? it.b1 : it.a1;
-  s.n = end - s.base < kPrefixTile ? end - s.base : kPrefixTile;
+  s.n = end - s.base < kKeys ? end - s.base : kKeys;
   return s;
 }
 
@@ -184,11 +187,11 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t src) {
   return v;
 }
 
-// where the keys of one lane (4 consecutive keys of a tile) come from
+// where the keys of one lane (2 consecutive keys of a tile) come from
 struct Src {
-  uint64_t at[4];  // the K or V half of the record; 0: none (beyond the range, or no valid slot)
+  uint64_t at[2];  // the K or V half of the record; 0: none (beyond the range, or no valid slot)
   int row;         // row of the tensor map of the first key
-  bool run;        // the four lie in consecutive rows of the pool's map
+  bool run;        // the two lie in consecutive rows of the pool's map
 };
 
 // One row of an item by one warp, over the keys that it sees (the CUDA-core
@@ -249,8 +252,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = blockIdx.x % a.hkv;
   const PrefixItem it = a.items[blockIdx.x / a.hkv];
-  const int na = (it.a1 - it.a0 + kPrefixTile - 1) / kPrefixTile;
-  const int steps = na + (it.b1 - it.b0 + kPrefixTile - 1) / kPrefixTile;
+  const int na = (it.a1 - it.a0 + kKeys - 1) / kKeys;
+  const int steps = na + (it.b1 - it.b0 + kKeys - 1) / kKeys;
   const int tiles = NT == 2 && it.ntok > a.R ? 2 : 1;
 
   // (producers) the sources of a key tile
@@ -259,13 +262,13 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
   auto load_src = [&](int t, Src& s) {
     const Step st = step_of(it, na, t);
     const int64_t* slots = (st.own ? a.suffix_slots : a.prefix_slots) + st.base;
-    int64_t sl[4];
+    int64_t sl[2];
 #pragma unroll
-    for (int m = 0; m < 4; ++m) sl[m] = 4 * lane + m < st.n ? slots[4 * lane + m] : -1;
-    s.run = a.tma != 0 && sl[0] >= 0 && sl[3] < a.pv.native_total;
+    for (int m = 0; m < 2; ++m) sl[m] = 2 * lane + m < st.n ? slots[2 * lane + m] : -1;
+    s.run = a.tma != 0 && sl[0] >= 0 && sl[1] < a.pv.native_total;
     s.row = 0;
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
+    for (int m = 0; m < 2; ++m) {
       s.at[m] = 0;
       int64_t b = 0, o = 0;
       if (a.pv.valid(sl[m])) {
@@ -283,7 +286,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
           s.at[m] = reinterpret_cast<uint64_t>(isv ? a.pv.side_v : a.pv.side_k) +
                     (sl[m] - a.pv.native_total) * a.pv.ssr + g * a.pv.ssh;
         }
-      } else if (4 * lane + m < st.n) {
+      } else if (2 * lane + m < st.n) {
         slot_bad = true;
       }
       if (m == 0) s.row = (int)(b * a.nrb + g * a.nrh + o * a.nro);
@@ -318,9 +321,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + Sh::oMeta + Sh::oTmem);
-  // sub-step u (64 keys) uses score buffer u & 1 of its row tile
-  auto at = [&](uint32_t bar, int qt, int u) { return mb + bar + 8 * (2 * qt + (u & 1)); };
-  auto halves = [&](int t) { return step_of(it, na, t).n > kHalf ? 2 : 1; };
+  // step t uses score buffer t & 1 of its row tile
+  auto at = [&](uint32_t bar, int qt, int t) { return mb + bar + 8 * (2 * qt + (t & 1)); };
 
   if (warp == Sh::kSoft || warp == Sh::kSoft + 1) {
     // ============================================== producers: K, then V warp
@@ -329,50 +331,54 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     int issued = 0;
     for (int t = 0; t < steps; ++t) {
       // the stage is free once every row tile is done with its last use
-      if (t >= ST && !__all_sync(~0u, mbar_wait(mb + (isv ? Sh::bVr : Sh::bKr) + 8 * (t % ST),
-                                                (t / ST - 1) & 1, abort)))
-        break;
+      if (t >= ST) {
+        bool ok = true;
+        if constexpr (Sh::kDirect) {
+          for (int qt = 0; qt < tiles; ++qt)
+            ok = ok && mbar_wait(at(isv ? Sh::bPV : Sh::bS, qt, t), (t / 2 - 1) & 1, abort);
+        } else {
+          ok = mbar_wait(mb + (isv ? Sh::bVr : Sh::bKr) + 8 * (t % ST), (t / ST - 1) & 1, abort);
+        }
+        if (!__all_sync(~0u, ok)) break;
+      }
       const uint32_t bar = mb + (isv ? Sh::bV : Sh::bK) + 8 * (t % ST);
       const uint32_t dst = sbase + (isv ? Sh::oV : Sh::oK) + (t % ST) * Sh::TB;
       // 16 keys (4 lanes) in consecutive rows: one TMA box an operand half;
       // the others row by row with cp.async, whole rows an instruction, the
       // addresses through shared memory.  (tile::gather4 is issued lane by
       // lane, about 100 clocks each: 6400 for a tile of scattered rows.)
-      const int r16 = __shfl_sync(~0u, cur.row, lane & ~3);
-      const uint32_t sq = __ballot_sync(~0u, cur.run && cur.row == r16 + 4 * (lane & 3));
-      const bool lead = (lane & 3) == 0 && ((sq >> lane) & 0xFu) == 0xFu;
+      const int r16 = __shfl_sync(~0u, cur.row, lane & ~7);
+      const uint32_t sq = __ballot_sync(~0u, cur.run && cur.row == r16 + 2 * (lane & 7));
+      const bool lead = (lane & 7) == 0 && ((sq >> lane) & 0xFFu) == 0xFFu;
       const uint32_t leads = __ballot_sync(~0u, lead);
-      if (leads != 0x11111111u) {
-        const uint32_t tab = mb + Sh::oRows + (isv ? 1024 : 0);
-#pragma unroll
-        for (int m = 0; m < 4; m += 2)
-          st_shared16(tab + 32 * lane + 8 * m,
-                      make_uint4((uint32_t)cur.at[m], (uint32_t)(cur.at[m] >> 32),
-                                 (uint32_t)cur.at[m + 1], (uint32_t)(cur.at[m + 1] >> 32)));
-      }
+      const uint32_t tab_at = Sh::oRows + (isv ? kKeys * 8 : 0);
+      if (leads != 0x01010101u)
+        st_shared16(mb + tab_at + 16 * lane,
+                    make_uint4((uint32_t)cur.at[0], (uint32_t)(cur.at[0] >> 32),
+                               (uint32_t)cur.at[1], (uint32_t)(cur.at[1] >> 32)));
       if (lane == 0) mbar_expect_tx(bar, __popc(leads) * 16 * D * 2);
       __syncwarp();
       if (lead) {
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
-          tma_tile2d(dst + c * 16384 + 4 * lane * 128, &a.tm, (isv ? D : 0) + 64 * c, cur.row, bar);
+          tma_tile2d(dst + c * (kKeys * 128) + 2 * lane * 128, &a.tm, (isv ? D : 0) + 64 * c,
+                     cur.row, bar);
       }
-      if (leads != 0x11111111u) {
+      if (leads != 0x01010101u) {
         constexpr int C = D / 8, RI = 32 / C;  // 16-byte pieces a row, rows an instruction
-        const uint64_t* tab = reinterpret_cast<const uint64_t*>(smem + Sh::oMeta + Sh::oRows +
-                                                                (isv ? 1024 : 0));
-        for (int q = 0; q < 8; ++q) {
-          if ((leads >> (4 * q)) & 1u) continue;
-          uint64_t at[16 / RI];
+        const uint64_t* tab = reinterpret_cast<const uint64_t*>(smem + Sh::oMeta + tab_at);
+        for (int q = 0; q < kKeys / 16; ++q) {
+          if ((leads >> (8 * q)) & 1u) continue;
+          uint64_t src[16 / RI];
 #pragma unroll
-          for (int i = 0; i < 16 / RI; ++i) at[i] = tab[16 * q + i * RI + lane / C];
+          for (int i = 0; i < 16 / RI; ++i) src[i] = tab[16 * q + i * RI + lane / C];
 #pragma unroll
           for (int i = 0; i < 16 / RI; ++i) {
             const int j = 16 * q + i * RI + lane / C;
-            const uint64_t src =
-                at[i] ? at[i] + 16 * (lane % C) : reinterpret_cast<uint64_t>(a.pv.cache);
-            cp_async16(dst + sw128(j, lane % C, kPrefixTile), reinterpret_cast<const void*>(src),
-                       at[i] != 0);
+            const uint64_t p =
+                src[i] ? src[i] + 16 * (lane % C) : reinterpret_cast<uint64_t>(a.pv.cache);
+            cp_async16(dst + sw128(j, lane % C, kKeys), reinterpret_cast<const void*>(p),
+                       src[i] != 0);
           }
         }
         __syncwarp();
@@ -401,74 +407,59 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     const int qt = __shfl_sync(~0u, warp, 0) - (Sh::kSoft + 2);
     if (qt < tiles) {
       const bool leader = elect_one();
-      const uint32_t id_s = umma_idesc(128, kHalf, umma_format<T>(), 0, 0);
+      const uint32_t id_s = umma_idesc(128, kKeys, umma_format<T>(), 0, 0);
       const uint32_t id_o = umma_idesc(128, D, umma_format<T>(), 0, 1);  // V is MN-major
       const uint64_t dq = umma_desc(sbase + Sh::oQ + qt * Sh::QB, 16, 1024);
       const uint64_t dk0 = umma_desc(sbase + Sh::oK, 16, 1024);
-      const uint64_t dv0 = umma_desc(sbase + Sh::oV, 16384, 1024);
+      const uint64_t dv0 = umma_desc(sbase + Sh::oV, kKeys * 128, 1024);
       const uint32_t tm = __shfl_sync(~0u, tmem, 0);
       const uint32_t sc = tm + Sh::cS + 128 * qt, oc = tm + Sh::cO + D * qt;
       bool ok = mbar_spin(mb + Sh::bQ, 0, abort);
       uint32_t last = 0, lastph = 0;  // the newest group issued
-      int qk_t = 0, qk_h = 0, qk_u = 0;  // the next scores to compute
-      auto scores = [&]() {
-        if (qk_h == 0) {
-          ok = mbar_spin(mb + Sh::bK + 8 * (qk_t % Sh::KS), (qk_t / Sh::KS) & 1, abort);
-          if (!ok) return;
-          fence_async_smem();  // rows copied by cp.async
-        }
+      auto scores = [&](int t) {
+        ok = mbar_spin(mb + Sh::bK + 8 * (t % Sh::KS), (t / Sh::KS) & 1, abort);
+        if (!ok) return;
+        fence_async_smem();  // rows copied by cp.async
         tc_fence_after();
-        const uint64_t dk = dk0 + (uint64_t)((qk_t % Sh::KS) * (Sh::TB >> 4) + qk_h * 512);
-        const uint32_t s = sc + kHalf * (qk_u & 1);
-        last = at(Sh::bS, qt, qk_u);
-        lastph = (qk_u >> 1) & 1;
+        const uint64_t dk = dk0 + (uint64_t)((t % Sh::KS) * (Sh::TB >> 4));
+        const uint32_t s = sc + kKeys * (t & 1);
+        last = at(Sh::bS, qt, t);
+        lastph = (t >> 1) & 1;
         if (leader) {
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint64_t off = (kk >> 2) * 1024 + (kk & 3) * 2;  // 16-byte units
-            tc_mma(s, dq + off, dk + off, id_s, kk ? 1u : 0u);
-          }
+          for (int kk = 0; kk < D / 16; ++kk)  // offsets in 16-byte units
+            tc_mma(s, dq + (kk >> 2) * 1024 + (kk & 3) * 2,
+                   dk + (kk >> 2) * (kKeys * 8) + (kk & 3) * 2, id_s, kk ? 1u : 0u);
           tc_commit(last);
         }
         __syncwarp();
-        ++qk_u;
-        if (++qk_h == halves(qk_t)) {
-          qk_h = 0;
-          ++qk_t;
-        }
       };
-      if (ok && steps > 0) scores();
-      if (ok && qk_t < steps) scores();
-      int u = 0;
+      if (ok && steps > 0) scores(0);
+      if (ok && steps > 1) scores(1);
       for (int t = 0; ok && t < steps; ++t) {
-        const int nh = halves(t);
-        for (int h = 0; ok && h < nh; ++h, ++u) {
-          const uint32_t ph = (u >> 1) & 1;
-          if (!(ok = mbar_spin(at(Sh::bP, qt, u), ph, abort))) break;
-          if (h == 0) {
-            if (!(ok = mbar_spin(mb + Sh::bV + 8 * (t % Sh::VS), (t / Sh::VS) & 1, abort))) break;
-            fence_async_smem();
-          }
-          tc_fence_after();
-          const uint64_t dv = dv0 + (uint64_t)((t % Sh::VS) * (Sh::TB >> 4) + h * 512);
-          const uint32_t p = sc + kHalf * (u & 1);
-          last = at(Sh::bPV, qt, u);
-          lastph = ph;
-          if (leader) {
+        const uint32_t ph = (t >> 1) & 1;
+        if (!(ok = mbar_spin(at(Sh::bP, qt, t), ph, abort))) break;
+        if (!(ok = mbar_spin(mb + Sh::bV + 8 * (t % Sh::VS), (t / Sh::VS) & 1, abort))) break;
+        fence_async_smem();
+        tc_fence_after();
+        const uint64_t dv = dv0 + (uint64_t)((t % Sh::VS) * (Sh::TB >> 4));
+        const uint32_t p = sc + kKeys * (t & 1);
+        last = at(Sh::bPV, qt, t);
+        lastph = ph;
+        if (leader) {
 #pragma unroll
-            for (int kk = 0; kk < kHalf / 16; ++kk)
-              tc_mma_ts(oc, p + kk * 8, dv + kk * 128, id_o, (u | kk) ? 1u : 0u);
-            tc_commit(last);
-          }
-          __syncwarp();
-          // the next scores but one take the buffer that P lies in, and the
-          // next V tile but VS - 1 the stage just read
-          const bool refill = h == nh - 1 && t + Sh::VS < steps;
-          if (qk_t < steps || refill) {
-            if (!(ok = mbar_spin(last, ph, abort))) break;
-            if (refill && leader) mbar_arrive(mb + Sh::bVr + 8 * (t % Sh::VS));
-            if (qk_t < steps) scores();
-          }
+          for (int kk = 0; kk < kKeys / 16; ++kk)
+            tc_mma_ts(oc, p + kk * 8, dv + kk * 128, id_o, (t | kk) ? 1u : 0u);
+          tc_commit(last);
+        }
+        __syncwarp();
+        // the next scores but one take the buffer that P lies in, and a later
+        // V tile the stage just read
+        const bool refill = !Sh::kDirect && t + Sh::VS < steps;
+        if (t + 2 < steps || refill) {
+          if (!(ok = mbar_spin(last, ph, abort))) break;
+          if (refill && leader) mbar_arrive(mb + Sh::bVr + 8 * (t % Sh::VS));
+          if (t + 2 < steps) scores(t + 2);
         }
       }
       if (last) {
@@ -523,32 +514,25 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     const uint32_t oc = tmem + lane_base + Sh::cO + D * qt;
     float mref = -INFINITY, lsum = 0.f;  // log2 domain; P = 2^(x - mref + up)
     bool ok = true;
-    auto wait_pv = [&](int u) {
-      ok = __all_sync(~0u, mbar_wait(at(Sh::bPV, qt, u), (u >> 1) & 1, abort));
+    auto wait_pv = [&](int t) {
+      ok = __all_sync(~0u, mbar_wait(at(Sh::bPV, qt, t), (t >> 1) & 1, abort));
       tc_fence_after();
       return ok;
     };
 
-    int u = 0;
-    for (int t = 0, h2 = 0; t < steps; ++u) {
-      Step st = step_of(it, na, t);
-      const bool last_half = h2 == 1 || st.n <= kHalf;
-      st.base += kHalf * h2;
-      st.n = st.n - kHalf * h2 < kHalf ? st.n - kHalf * h2 : kHalf;
-      const int stage = t % Sh::KS;
-      if (last_half) ++t, h2 = 0;
-      else h2 = 1;
+    for (int t = 0; t < steps; ++t) {
+      const Step st = step_of(it, na, t);
       int vlo = 0, vhi = 0;
       if (row_ok) {
         vlo = st.own ? (tk.z > st.base ? tk.z - st.base : 0) : 0;
         vhi = st.own ? (tk.w - st.base < st.n ? tk.w - st.base : st.n) : st.n;
       }
-      const uint32_t sc = sc0 + kHalf * (u & 1);
-      ok = __all_sync(~0u, mbar_wait(at(Sh::bS, qt, u), (u >> 1) & 1, abort));
+      const uint32_t sc = sc0 + kKeys * (t & 1);
+      ok = __all_sync(~0u, mbar_wait(at(Sh::bS, qt, t), (t >> 1) & 1, abort));
       if (!ok) break;  // a wait expired
-      if (last_half && (tid & 127) == 0) mbar_arrive(mb + Sh::bKr + 8 * stage);
+      if (!Sh::kDirect && (tid & 127) == 0) mbar_arrive(mb + Sh::bKr + 8 * (t % Sh::KS));
       tc_fence_after();
-      uint32_t v[kHalf];
+      uint32_t v[kKeys];
       if (__all_sync(~0u, vhi <= vlo)) {  // nothing to see for these 32 rows
 #pragma unroll
         for (int c = 0; c < 16; ++c) v[c] = 0u;
@@ -556,13 +540,13 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
         CS_TMEM_ST16(sc + 16, v);
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(at(Sh::bP, qt, u));
+        mbar_arrive(at(Sh::bP, qt, t));
         continue;
       }
       CS_TMEM_LD32(sc, v);
       CS_TMEM_LD32(sc + 32, (v + 32));
       tmem_wait_ld();
-      const bool whole = __all_sync(~0u, vlo <= 0 && vhi >= kHalf);
+      const bool whole = __all_sync(~0u, vlo <= 0 && vhi >= kKeys);
       if (!whole) {
 #pragma unroll
         for (int cc = 0; cc < 2; ++cc) {
@@ -579,7 +563,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
         for (int k = 0; k < 4; ++k)
           m[k] = max_nan(__uint_as_float(v[k]), __uint_as_float(v[k + 4]));
 #pragma unroll
-        for (int c = 8; c < kHalf; c += 8) {
+        for (int c = 8; c < kKeys; c += 8) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             m[k] = max3_nan(m[k], __uint_as_float(v[c + k]), __uint_as_float(v[c + k + 4]));
@@ -593,8 +577,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       const float top2 = top == -INFINITY ? -INFINITY : top * a.scale2;
       const bool grow = top2 > mref + kLazy || mref == -INFINITY;
       const bool rescale = grow && mref > -INFINITY && top2 > mref;
-      if (__any_sync(~0u, rescale)) {  // u > 0: a row has a finite maximum
-        if (!wait_pv(u - 1)) break;
+      if (__any_sync(~0u, rescale)) {  // t > 0: a row has a finite maximum
+        if (!wait_pv(t - 1)) break;
         const float f = rescale ? ex2(mref - top2) : 1.f;
         lsum *= f;
         uint32_t o[16];
@@ -641,11 +625,11 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       lsum += (s0.x + s0.y) + (s1.x + s1.y);
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(at(Sh::bP, qt, u));
+      mbar_arrive(at(Sh::bP, qt, t));
     }
 
     // ---------------------------------------------------------------- output
-    if (ok && u > 0) wait_pv(u - 1);
+    if (ok && steps > 0) wait_pv(steps - 1);
     const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
     const float lse2 = lsum == 0.f ? -INFINITY
                                    : (mref > -INFINITY ? mref : 0.f) - p_up<T>() + log2f(lsum);
