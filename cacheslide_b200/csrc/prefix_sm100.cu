@@ -152,10 +152,6 @@ __device__ __forceinline__ uint32_t col_bits(int lo, int hi, int col0) {
   return up & ~((1u << lo) - 1u);
 }
 
-__device__ __forceinline__ void mbar_arrive_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
-               : "memory");
-}
 // the same lane of a whole warp every time
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
@@ -166,11 +162,10 @@ __device__ __forceinline__ bool elect_one() {
       : "=r"(p));
   return p != 0;
 }
-// mbar_wait for a whole warp that must see the phase at once: it polls instead
-// of being suspended
-__device__ __forceinline__ bool mbar_spin(uint32_t bar, uint32_t parity, volatile int* abort) {
-  for (int i = 0; i < 64; ++i)
-    if (__all_sync(~0u, mbar_test(bar, parity))) return true;
+// bounded wait of a whole warp; a phase that is over already costs one test
+// (the clock and the abort flag are read only when it is not)
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+  if (__all_sync(~0u, mbar_try(bar, parity))) return true;
   return __all_sync(~0u, mbar_wait(bar, parity, abort));
 }
 __device__ __forceinline__ void st_shared16(uint32_t dst, uint4 v) {
@@ -256,15 +251,27 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
   const int steps = na + (it.b1 - it.b0 + kKeys - 1) / kKeys;
   const int tiles = NT == 2 && it.ntok > a.R ? 2 : 1;
 
-  // (producers) the sources of a key tile
+  // (producers) the slots of a key tile are read three tiles ahead: beside the
+  // streams of K and V such a read takes 2500 clocks
   bool slot_bad = false;
   const bool isv = warp != Sh::kSoft;
-  auto load_src = [&](int t, Src& s) {
-    const Step st = step_of(it, na, t);
-    const int64_t* slots = (st.own ? a.suffix_slots : a.prefix_slots) + st.base;
-    int64_t sl[2];
+  struct Slots {
+    int64_t s[2];
+  };
+  auto load_slots = [&](int t) {
+    Slots r{{-1, -1}};
+    if (t < steps) {
+      const Step st = step_of(it, na, t);
+      const int64_t* slots = (st.own ? a.suffix_slots : a.prefix_slots) + st.base;
 #pragma unroll
-    for (int m = 0; m < 2; ++m) sl[m] = 2 * lane + m < st.n ? slots[2 * lane + m] : -1;
+      for (int m = 0; m < 2; ++m)
+        if (2 * lane + m < st.n) r.s[m] = slots[2 * lane + m];
+    }
+    return r;
+  };
+  auto resolve = [&](int t, const Slots& in, Src& s) {
+    const Step st = step_of(it, na, t);
+    const int64_t* sl = in.s;
     s.run = a.tma != 0 && sl[0] >= 0 && sl[1] < a.pv.native_total;
     s.row = 0;
 #pragma unroll
@@ -315,8 +322,11 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
   // writes; from here on the preceding grids' results are read
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  Src cur;
-  if ((warp == Sh::kSoft || warp == Sh::kSoft + 1) && steps > 0) load_src(0, cur);
+  Slots ahead[3];
+  if (warp == Sh::kSoft || warp == Sh::kSoft + 1) {
+#pragma unroll
+    for (int k = 0; k < 3; ++k) ahead[k] = load_slots(k);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -327,19 +337,23 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
   if (warp == Sh::kSoft || warp == Sh::kSoft + 1) {
     // ============================================== producers: K, then V warp
     const int ST = isv ? Sh::VS : Sh::KS;
-    Src nxt;
     int issued = 0;
     for (int t = 0; t < steps; ++t) {
+      Src cur;
+      resolve(t, ahead[0], cur);
+      ahead[0] = ahead[1];
+      ahead[1] = ahead[2];
+      ahead[2] = load_slots(t + 3);
       // the stage is free once every row tile is done with its last use
       if (t >= ST) {
         bool ok = true;
         if constexpr (Sh::kDirect) {
           for (int qt = 0; qt < tiles; ++qt)
-            ok = ok && mbar_wait(at(isv ? Sh::bPV : Sh::bS, qt, t), (t / 2 - 1) & 1, abort);
+            ok = ok && warp_wait(at(isv ? Sh::bPV : Sh::bS, qt, t), (t / 2 - 1) & 1, abort);
         } else {
-          ok = mbar_wait(mb + (isv ? Sh::bVr : Sh::bKr) + 8 * (t % ST), (t / ST - 1) & 1, abort);
+          ok = warp_wait(mb + (isv ? Sh::bVr : Sh::bKr) + 8 * (t % ST), (t / ST - 1) & 1, abort);
         }
-        if (!__all_sync(~0u, ok)) break;
+        if (!ok) break;
       }
       const uint32_t bar = mb + (isv ? Sh::bV : Sh::bK) + 8 * (t % ST);
       const uint32_t dst = sbase + (isv ? Sh::oV : Sh::oK) + (t % ST) * Sh::TB;
@@ -385,10 +399,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       }
       cp_async_arrive_noinc(bar);
       issued = t + 1;
-      if (t + 1 < steps) {
-        load_src(t + 1, nxt);
-        cur = nxt;
-      }
     }
     // nothing of this block's copies is in flight when it ends
     for (int t = issued - ST < 0 ? 0 : issued - ST; t < issued; ++t) {
@@ -414,10 +424,10 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       const uint64_t dv0 = umma_desc(sbase + Sh::oV, kKeys * 128, 1024);
       const uint32_t tm = __shfl_sync(~0u, tmem, 0);
       const uint32_t sc = tm + Sh::cS + 128 * qt, oc = tm + Sh::cO + D * qt;
-      bool ok = mbar_spin(mb + Sh::bQ, 0, abort);
+      bool ok = warp_wait(mb + Sh::bQ, 0, abort);
       uint32_t last = 0, lastph = 0;  // the newest group issued
       auto scores = [&](int t) {
-        ok = mbar_spin(mb + Sh::bK + 8 * (t % Sh::KS), (t / Sh::KS) & 1, abort);
+        ok = warp_wait(mb + Sh::bK + 8 * (t % Sh::KS), (t / Sh::KS) & 1, abort);
         if (!ok) return;
         fence_async_smem();  // rows copied by cp.async
         tc_fence_after();
@@ -438,8 +448,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       if (ok && steps > 1) scores(1);
       for (int t = 0; ok && t < steps; ++t) {
         const uint32_t ph = (t >> 1) & 1;
-        if (!(ok = mbar_spin(at(Sh::bP, qt, t), ph, abort))) break;
-        if (!(ok = mbar_spin(mb + Sh::bV + 8 * (t % Sh::VS), (t / Sh::VS) & 1, abort))) break;
+        if (!(ok = warp_wait(at(Sh::bP, qt, t), ph, abort))) break;
+        if (!(ok = warp_wait(mb + Sh::bV + 8 * (t % Sh::VS), (t / Sh::VS) & 1, abort))) break;
         fence_async_smem();
         tc_fence_after();
         const uint64_t dv = dv0 + (uint64_t)((t % Sh::VS) * (Sh::TB >> 4));
@@ -457,7 +467,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
         // V tile the stage just read
         const bool refill = !Sh::kDirect && t + Sh::VS < steps;
         if (t + 2 < steps || refill) {
-          if (!(ok = mbar_spin(last, ph, abort))) break;
+          if (!(ok = warp_wait(last, ph, abort))) break;
           if (refill && leader) mbar_arrive(mb + Sh::bVr + 8 * (t % Sh::VS));
           if (t + 2 < steps) scores(t + 2);
         }
@@ -515,7 +525,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     float mref = -INFINITY, lsum = 0.f;  // log2 domain; P = 2^(x - mref + up)
     bool ok = true;
     auto wait_pv = [&](int t) {
-      ok = __all_sync(~0u, mbar_wait(at(Sh::bPV, qt, t), (t >> 1) & 1, abort));
+      ok = warp_wait(at(Sh::bPV, qt, t), (t >> 1) & 1, abort);
       tc_fence_after();
       return ok;
     };
@@ -528,7 +538,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
         vhi = st.own ? (tk.w - st.base < st.n ? tk.w - st.base : st.n) : st.n;
       }
       const uint32_t sc = sc0 + kKeys * (t & 1);
-      ok = __all_sync(~0u, mbar_wait(at(Sh::bS, qt, t), (t >> 1) & 1, abort));
+      ok = warp_wait(at(Sh::bS, qt, t), (t >> 1) & 1, abort);
       if (!ok) break;  // a wait expired
       if (!Sh::kDirect && (tid & 127) == 0) mbar_arrive(mb + Sh::bKr + 8 * (t % Sh::KS));
       tc_fence_after();
