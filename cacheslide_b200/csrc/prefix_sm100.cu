@@ -338,12 +338,10 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     // ============================================== producers: K, then V warp
     const int ST = isv ? Sh::VS : Sh::KS;
     int issued = 0;
-    for (int t = 0; t < steps; ++t) {
+    auto produce = [&](int t, Slots& mine) {
       Src cur;
-      resolve(t, ahead[0], cur);
-      ahead[0] = ahead[1];
-      ahead[1] = ahead[2];
-      ahead[2] = load_slots(t + 3);
+      resolve(t, mine, cur);
+      mine = load_slots(t + 3);
       // the stage is free once every row tile is done with its last use
       if (t >= ST) {
         bool ok = true;
@@ -353,11 +351,11 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
         } else {
           ok = warp_wait(mb + (isv ? Sh::bVr : Sh::bKr) + 8 * (t % ST), (t / ST - 1) & 1, abort);
         }
-        if (!ok) break;
+        if (!ok) return false;
       }
       const uint32_t bar = mb + (isv ? Sh::bV : Sh::bK) + 8 * (t % ST);
       const uint32_t dst = sbase + (isv ? Sh::oV : Sh::oK) + (t % ST) * Sh::TB;
-      // 16 keys (4 lanes) in consecutive rows: one TMA box an operand half;
+      // 16 keys (8 lanes) in consecutive rows: one TMA box an operand half;
       // the others row by row with cp.async, whole rows an instruction, the
       // addresses through shared memory.  (tile::gather4 is issued lane by
       // lane, about 100 clocks each: 6400 for a tile of scattered rows.)
@@ -399,6 +397,13 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       }
       cp_async_arrive_noinc(bar);
       issued = t + 1;
+      return true;
+    };
+    // three at a time: a slot moved between registers would have to arrive first
+    for (int t = 0; t < steps; t += 3) {
+      if (!produce(t, ahead[0])) break;
+      if (t + 1 < steps && !produce(t + 1, ahead[1])) break;
+      if (t + 2 < steps && !produce(t + 2, ahead[2])) break;
     }
     // nothing of this block's copies is in flight when it ends
     for (int t = issued - ST < 0 ? 0 : issued - ST; t < issued; ++t) {
