@@ -75,9 +75,16 @@ struct Shape {
   // move on before the stage is filled again; deeper rings have barriers of
   // their own for "read".
   static constexpr bool kDirect = KS == 2;
-  static constexpr int kSoft = 4 * NT;
-  // one more warpgroup: K, V, NT MMA warps (and an idle one beside one tile)
-  static constexpr int kThreads = 128 * (NT + 1);
+  // threads a row in the softmax: two where one block has the SM (64 questions
+  // of 64 tokens behind 5120 keys: 357 us against 367 with one), one where two
+  // blocks share it (32 sessions of 4 drafts: 208 us against 224 with two).
+  // Making the row tiles' exponentials take turns, or start half a step apart,
+  // cost more than it gave (364 and 366 us).
+  static constexpr int TPR = NT;
+  static constexpr int kTile = 128 * TPR;  // softmax threads of a row tile
+  // the softmax warps, then K, V and NT MMA warps, to a whole warpgroup
+  static constexpr int kSoft = 4 * NT * TPR;
+  static constexpr int kThreads = kTile * NT + 128;
   static constexpr uint32_t TB = kKeys * D * 2;  // a K or V tile
   // a query tile's place also takes its output rows, 2 D bytes each and 16 more
   static constexpr uint32_t QB = kPrefixTile * D * 2 + 128 * 16;
@@ -86,9 +93,11 @@ struct Shape {
   // their "read" barriers a stage
   static constexpr uint32_t bQ = 0, bK = 8, bV = bK + 8 * KS, bKr = bV + 8 * VS,
                             bVr = bKr + 8 * KS, bS = bVr + 8 * VS, bP = bS + 16 * NT,
-                            bPV = bP + 16 * NT, oTmem = bPV + 16 * NT, oAbort = oTmem + 4,
+                            bPV = bP + 16 * NT, bMax = bPV + 16 * NT, oTmem = bMax + 32 * NT,
+                            oAbort = oTmem + 4,
                             oRows = (oAbort + 4 + 15) / 16 * 16,
-                            kMeta = oRows + 2 * kKeys * 8;
+                            oMax = oRows + 2 * kKeys * 8,
+                            kMeta = oMax + NT * 2 * 2 * 128 * 4;
   static_assert(oMeta % 1024 == 0 && oRows % 16 == 0 && oTmem % 4 == 0,
                 "alignment of the shared-memory places");
   static constexpr uint32_t kSmem = oMeta + kMeta + 1024;  // the base is rounded up to 1024
@@ -108,27 +117,6 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float y;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
-}
-
-// 2^x of two finite numbers below 128 on the FMA units: x = i + f with i the
-// nearest integer (left in the low bits by adding 1.5 * 2^23), 2^f by the
-// polynomial of degree 5 of least relative error on [-1/2, 1/2] (a Remez
-// exchange in float64, coefficients rounded: 1.5e-7), i added to the
-// exponent.  Below -126 the result stays 2^-126.
-__device__ __forceinline__ float2 pow2_pair(float2 x) {
-  auto two = [](float c) { return make_float2(c, c); };
-  x = make_float2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
-  const float2 t = __fadd2_rn(x, two(12582912.f));
-  const float2 r = __fadd2_rn(t, two(-12582912.f));
-  const float2 f = __ffma2_rn(r, two(-1.f), x);
-  float2 p = two(0x1.5c08e6p-10f);
-  p = __ffma2_rn(p, f, two(0x1.3d0c52p-7f));
-  p = __ffma2_rn(p, f, two(0x1.c6b6e4p-5f));
-  p = __ffma2_rn(p, f, two(0x1.ebf918p-3f));
-  p = __ffma2_rn(p, f, two(0x1.62e428p-1f));
-  p = __ffma2_rn(p, f, two(0x1.000002p+0f));
-  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 
 struct Step {
@@ -302,16 +290,17 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     }
   };
   if (tid == 0) {
-    mbar_init(mb + Sh::bQ, 128 * tiles);
+    mbar_init(mb + Sh::bQ, Sh::kTile * tiles);
     for (int s = 0; s < Sh::KS; ++s) mbar_init(mb + Sh::bK + 8 * s, 32);
     for (int s = 0; s < Sh::VS; ++s) mbar_init(mb + Sh::bV + 8 * s, 32);
     for (int s = 0; s < Sh::KS; ++s) mbar_init(mb + Sh::bKr + 8 * s, tiles);
     for (int s = 0; s < Sh::VS; ++s) mbar_init(mb + Sh::bVr + 8 * s, tiles);
     for (int s = 0; s < 2 * NT; ++s) {
       mbar_init(mb + Sh::bS + 8 * s, 1);
-      mbar_init(mb + Sh::bP + 8 * s, 128);
+      mbar_init(mb + Sh::bP + 8 * s, Sh::kTile);
       mbar_init(mb + Sh::bPV + 8 * s, 1);
     }
+    for (int s = 0; s < 4 * NT; ++s) mbar_init(mb + Sh::bMax + 8 * s, 2);
     *abort = 0;
     mbar_init_fence();
     if (a.tma)
@@ -486,9 +475,10 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     __syncwarp();
 
   } else {
-    if ((warp >> 2) < tiles) {
-    // ================================================== softmax, a thread a row
-    const int qt = warp >> 2;
+    constexpr int TPR = Sh::TPR, VC = kKeys / TPR;  // scores of a step a thread holds
+    if (warp / (4 * TPR) < tiles) {
+    // ================================================================= softmax
+    const int qt = warp / (4 * TPR), part2 = (warp >> 2) % TPR;
     const int r = (warp & 3) * 32 + lane;  // TMEM lane
     const int tok = qt * a.R + r / a.G, h = g * a.G + r % a.G;
     const bool row_ok = r < a.R * a.G && tok < it.ntok;
@@ -506,11 +496,11 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       };
       if (a.vec_q && !a.neg) {
 #pragma unroll 4
-        for (int row = (tid & 127) / C; row < rows; row += 128 / C)
+        for (int row = (tid % Sh::kTile) / C; row < rows; row += Sh::kTile / C)
           cp_async16(qs + sw128(row, c, kPrefixTile), from(row), true);
         cp_async_wait_all();
       } else {
-        for (int row = (tid & 127) / C; row < rows; row += 128 / C) {
+        for (int row = (tid % Sh::kTile) / C; row < rows; row += Sh::kTile / C) {
           uint16_t e[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k)
@@ -529,6 +519,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     const uint32_t oc = tmem + lane_base + Sh::cO + D * qt;
     float mref = -INFINITY, lsum = 0.f;  // log2 domain; P = 2^(x - mref + up)
     bool ok = true;
+    int exchanges = 0;  // of maxima with the row's other thread
+    const uint32_t pair = mb + Sh::bMax + 8 * (4 * qt + (warp & 3));
+    float* row_max = reinterpret_cast<float*>(smem + Sh::oMeta + Sh::oMax) + qt * 512;
     auto wait_pv = [&](int t) {
       ok = warp_wait(at(Sh::bPV, qt, t), (t >> 1) & 1, abort);
       tc_fence_after();
@@ -545,27 +538,27 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       const uint32_t sc = sc0 + kKeys * (t & 1);
       ok = warp_wait(at(Sh::bS, qt, t), (t >> 1) & 1, abort);
       if (!ok) break;  // a wait expired
-      if (!Sh::kDirect && (tid & 127) == 0) mbar_arrive(mb + Sh::bKr + 8 * (t % Sh::KS));
+      if (!Sh::kDirect && tid % Sh::kTile == 0) mbar_arrive(mb + Sh::bKr + 8 * (t % Sh::KS));
       tc_fence_after();
-      uint32_t v[kKeys];
+      uint32_t v[VC];
+      // both threads of a row leave this way together
       if (__all_sync(~0u, vhi <= vlo)) {  // nothing to see for these 32 rows
 #pragma unroll
         for (int c = 0; c < 16; ++c) v[c] = 0u;
-        CS_TMEM_ST16(sc, v);
-        CS_TMEM_ST16(sc + 16, v);
+#pragma unroll
+        for (int cc = 0; cc < VC / 32; ++cc) CS_TMEM_ST16(sc + 16 * (part2 + cc), v);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(at(Sh::bP, qt, t));
         continue;
       }
-      CS_TMEM_LD32(sc, v);
-      CS_TMEM_LD32(sc + 32, (v + 32));
+      CS_TMEM_LD32(sc + 32 * part2, v);
+      if constexpr (TPR == 1) CS_TMEM_LD32(sc + 32, (v + 32));
       tmem_wait_ld();
-      const bool whole = __all_sync(~0u, vlo <= 0 && vhi >= kKeys);
-      if (!whole) {
+      if (!__all_sync(~0u, vlo <= 0 && vhi >= kKeys)) {
 #pragma unroll
-        for (int cc = 0; cc < 2; ++cc) {
-          const uint32_t bits = col_bits(vlo, vhi, 32 * cc);
+        for (int cc = 0; cc < VC / 32; ++cc) {
+          const uint32_t bits = col_bits(vlo, vhi, 32 * (part2 + cc));
 #pragma unroll
           for (int c = 0; c < 32; ++c)
             v[32 * cc + c] = (bits >> c) & 1u ? v[32 * cc + c] : 0xff800000u;  // -inf
@@ -578,12 +571,24 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
         for (int k = 0; k < 4; ++k)
           m[k] = max_nan(__uint_as_float(v[k]), __uint_as_float(v[k + 4]));
 #pragma unroll
-        for (int c = 8; c < kKeys; c += 8) {
+        for (int c = 8; c < VC; c += 8) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             m[k] = max3_nan(m[k], __uint_as_float(v[c + k]), __uint_as_float(v[c + k + 4]));
         }
         top = max_nan(max3_nan(m[0], m[1], m[2]), m[3]);
+      }
+      // the row's maximum from both its threads; past this barrier both have
+      // read their scores, so P may take their columns
+      if constexpr (TPR == 2) {
+        float* mx = row_max + (exchanges & 1) * 256;
+        mx[part2 * 128 + r] = top;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(pair);
+        ok = warp_wait(pair, exchanges & 1, abort);
+        if (!ok) break;
+        ++exchanges;
+        top = max_nan(top, mx[(1 - part2) * 128 + r]);
       }
       if (!(top < INFINITY)) {  // a NaN or +inf score makes the row NaN
         lsum = __int_as_float(0x7fffffff);
@@ -598,12 +603,13 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
         lsum *= f;
         uint32_t o[16];
 #pragma unroll 1
-        for (int cc = 0; cc < D / 16; ++cc) {
-          CS_TMEM_LD16(oc + 16 * cc, o);
+        for (int cc = 0; cc < D / 16 / TPR; ++cc) {
+          const uint32_t col = oc + part2 * (D / 2) + 16 * cc;
+          CS_TMEM_LD16(col, o);
           tmem_wait_ld();
 #pragma unroll
           for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
-          CS_TMEM_ST16(oc + 16 * cc, o);
+          CS_TMEM_ST16(col, o);
         }
         tmem_wait_st();
       }
@@ -611,32 +617,28 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       // the largest weight so far is 2^up, or up to 2^kLazy more
       const float sub = (mref > -INFINITY ? mref : 0.f) - p_up<T>();
       const float2 scale = make_float2(a.scale2, a.scale2), off = make_float2(-sub, -sub);
-      // whole tiles of rows with a maximum may take part of their exponentials
-      // from the FMA units (pow2_pair does not reach 0 for masked scores)
-      const bool poly = whole && __all_sync(~0u, mref > -INFINITY);
       float2 s0 = make_float2(0.f, 0.f), s1 = s0;
+      // in passes over the scores, so that no instruction waits for the one
+      // before it
 #pragma unroll
-      for (int cc = 0; cc < 2; ++cc) {
-        uint32_t* w = v + 32 * cc;
-        auto weight = [&](int c, bool fma_units) {
-          float2 x = __ffma2_rn(make_float2(__uint_as_float(w[2 * c]), __uint_as_float(w[2 * c + 1])),
-                                scale, off);
-          if (fma_units) x = pow2_pair(x);
-          else x = make_float2(ex2(x.x), ex2(x.y));
-          if (c & 1) s1 = __fadd2_rn(s1, x);
-          else s0 = __fadd2_rn(s0, x);
-          return Pack2<T>::pack(x.x, x.y);
-        };
-        uint32_t o[16];
-        if (poly) {
-#pragma unroll
-          for (int c = 0; c < 16; ++c) o[c] = weight(c, c % 4 == 3);
-        } else {
-#pragma unroll
-          for (int c = 0; c < 16; ++c) o[c] = weight(c, false);
-        }
-        CS_TMEM_ST16(sc + 16 * cc, o);
+      for (int c = 0; c < VC; c += 2) {
+        const float2 x = __ffma2_rn(make_float2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])),
+                                    scale, off);
+        v[c] = __float_as_uint(x.x);
+        v[c + 1] = __float_as_uint(x.y);
       }
+#pragma unroll
+      for (int c = 0; c < VC; ++c) v[c] = __float_as_uint(ex2(__uint_as_float(v[c])));
+#pragma unroll
+      for (int c = 0; c < VC; c += 4) {
+        s0 = __fadd2_rn(s0, make_float2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])));
+        s1 = __fadd2_rn(s1, make_float2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])));
+      }
+#pragma unroll
+      for (int c = 0; c < VC / 2; ++c)
+        v[c] = Pack2<T>::pack(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1]));
+#pragma unroll
+      for (int cc = 0; cc < VC / 32; ++cc) CS_TMEM_ST16(sc + 16 * (part2 + cc), (v + 16 * cc));
       lsum += (s0.x + s0.y) + (s1.x + s1.y);
       tmem_wait_st();
       tc_fence_before();
@@ -645,6 +647,14 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
 
     // ---------------------------------------------------------------- output
     if (ok && steps > 0) wait_pv(steps - 1);
+    if constexpr (TPR == 2) {  // the row's sum from both its threads
+      float* sum = row_max + (exchanges & 1) * 256;
+      sum[part2 * 128 + r] = lsum;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(pair);
+      ok = ok && warp_wait(pair, exchanges & 1, abort);
+      lsum += sum[(1 - part2) * 128 + r];
+    }
     const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
     const float lse2 = lsum == 0.f ? -INFINITY
                                    : (mref > -INFINITY ? mref : 0.f) - p_up<T>() + log2f(lsum);
@@ -664,32 +674,35 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       // queries were, and the warp writes whole rows: stores straight from the
       // registers touch 32 rows an instruction, and a bulk copy a row is
       // issued lane by lane (5300 clocks a tile, either way)
-      constexpr int L = 2 * D / 16;  // lanes a row
-      const uint32_t stage = sbase + Sh::oQ + qt * Sh::QB + (r - lane) * (2 * D + 16);
-      const uint32_t buf = stage + lane * (2 * D + 16);
+      constexpr int B = 2 * D / TPR;  // bytes of a row a thread stages at once
+      constexpr int L = B / 16;       // lanes that write them
+      constexpr int W = 2 * D + 16;
+      const uint32_t stage = sbase + Sh::oQ + qt * Sh::QB + (r - lane) * W + part2 * B;
+      const uint32_t buf = stage + lane * W;
       const uint64_t to = row_ok && ok ? reinterpret_cast<uint64_t>(orow) : 0;
 #pragma unroll 1
-      for (int half = 0; half < (part ? 2 : 1); ++half) {
+      for (int round = 0; round < (part ? 2 : 1); ++round) {
         uint32_t v[32];
+        const uint32_t col = oc + part2 * (D / 2);
         if (part) {
 #pragma unroll
-          for (int cc = 0; cc < D / 64; ++cc) {
-            CS_TMEM_LD32(oc + half * (D / 2) + 32 * cc, v);
+          for (int cc = 0; cc < B / 64; ++cc) {
+            CS_TMEM_LD16(col + round * (B / 4) + 16 * cc, v);
             tmem_wait_ld();
 #pragma unroll
-            for (int c = 0; c < 32; ++c) {
+            for (int c = 0; c < 16; ++c) {
               v[c] = have ? __float_as_uint(__uint_as_float(v[c]) * inv) : 0u;
               finite(v[c]);
             }
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
-              st_shared16(buf + 128 * cc + 16 * c,
+            for (int c = 0; c < 4; ++c)
+              st_shared16(buf + 64 * cc + 16 * c,
                           make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]));
           }
         } else {
 #pragma unroll
-          for (int cc = 0; cc < D / 32; ++cc) {
-            CS_TMEM_LD32(oc + 32 * cc, v);
+          for (int cc = 0; cc < B / 64; ++cc) {
+            CS_TMEM_LD32(col + 32 * cc, v);
             tmem_wait_ld();
 #pragma unroll
             for (int c = 0; c < 16; ++c) {
@@ -706,25 +719,27 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
           }
         }
         __syncwarp();
+        // a partial's thread has two rounds, an output's one
+        const int64_t first = part ? (part2 * 2 + round) * B : part2 * B;
 #pragma unroll
-        for (int n0 = 0; n0 < L; n0 += 8) {
-          uint4 x[8];
-          uint64_t dst[8];
+        for (int n0 = 0; n0 < L; n0 += 4) {
+          uint4 x[4];
+          uint64_t dst[4];
 #pragma unroll
-          for (int n = 0; n < 8; ++n) {
+          for (int n = 0; n < 4; ++n) {
             const int row = (n0 + n) * (32 / L) + lane / L;
             dst[n] = __shfl_sync(~0u, to, row);
-            x[n] = ld_shared16(stage + row * (2 * D + 16) + 16 * (lane % L));
+            x[n] = ld_shared16(stage + row * W + 16 * (lane % L));
           }
 #pragma unroll
-          for (int n = 0; n < 8; ++n)
-            if (dst[n]) *reinterpret_cast<uint4*>(dst[n] + half * 2 * D + 16 * (lane % L)) = x[n];
+          for (int n = 0; n < 4; ++n)
+            if (dst[n]) *reinterpret_cast<uint4*>(dst[n] + first + 16 * (lane % L)) = x[n];
         }
         __syncwarp();
       }
     } else {
 #pragma unroll 1
-      for (int cc = 0; cc < D / 32; ++cc) {
+      for (int cc = part2 * (D / 64); cc < (part2 + 1) * (D / 32 / TPR); ++cc) {
         uint32_t v[32];
         CS_TMEM_LD32(oc + 32 * cc, v);
         tmem_wait_ld();
@@ -747,7 +762,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
                       reinterpret_cast<void*>(__shfl_sync(~0u, reinterpret_cast<uint64_t>(orow), src)),
                       part);
     }
-    if (row_ok && ok) {
+    if (row_ok && ok && part2 == 0) {
       if (it.part >= 0) a.part_lse[prow] = lse2;
       else if (a.lse) a.lse[token * a.hq + h] = lse2 * kLn2;
     }
