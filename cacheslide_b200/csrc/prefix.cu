@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <functional>
 #include <new>
 #include <type_traits>
 #include <vector>
@@ -188,14 +189,16 @@ std::vector<Unit> split_units(const Layout& l, int64_t keys) {
   return out;
 }
 
-// Every unit cut into equal runs of at most `most` key tiles, of a part's
-// tokens only those that see its keys.
-std::vector<PrefixItem> cut(const Layout& l, const std::vector<Unit>& units, int64_t most) {
+// Every unit from `whole` on cut into equal runs of at most `most` key tiles
+// (those before it stay whole), of a part's tokens only those that see its keys.
+std::vector<PrefixItem> cut(const Layout& l, const std::vector<Unit>& units, int64_t most,
+                            size_t whole) {
   std::vector<PrefixItem> out;
-  for (const Unit& u : units) {
+  for (size_t x = 0; x < units.size(); ++x) {
+    const Unit& u = units[x];
     const int64_t steps = u.steps(), na = Unit::tiles(u.a1 - u.a0);
     if (steps == 0) continue;
-    const int64_t parts = (steps + most - 1) / most;
+    const int64_t parts = x < whole ? 1 : (steps + most - 1) / most;
     for (int64_t p = 0; p < parts; ++p) {
       const int64_t s0 = steps * p / parts, s1 = steps * (p + 1) / parts;
       Unit v = u;
@@ -212,48 +215,80 @@ std::vector<PrefixItem> cut(const Layout& l, const std::vector<Unit>& units, int
                      (int32_t)v.b0, (int32_t)v.b1, -1, 0});
     }
   }
+  // long ones first, as the blocks are dealt out
+  std::stable_sort(out.begin(), out.end(), [](const PrefixItem& x, const PrefixItem& y) {
+    return x.steps() > y.steps();
+  });
   return out;
 }
 
-int64_t item_steps(const PrefixItem& i) {
-  return Unit::tiles(i.a1 - i.a0) + Unit::tiles(i.b1 - i.b0);
-}
-
-// Estimated time of a launch, in key tiles of one 128-row block: blocks are
-// dealt out in order over `slots`, each costs its tiles and `fixed` more, and
-// a partial result costs its way to memory and back.
-double estimate(const Layout& l, const std::vector<PrefixItem>& items, int slots, double step,
-                double fixed) {
-  double sum = 0, longest = 0, parts = 0;
-  for (const PrefixItem& i : items) {
-    const double c = item_steps(i) * step + fixed;
-    sum += c;
-    longest = std::max(longest, c);
-    parts += i.ntok;
+// What a block costs, in microseconds: a tile of prefix keys, and its start and
+// end.  A tile of own keys costs more: masks, and rows that lie apart.
+struct Cost {
+  int slots;
+  double step, fixed;
+  double of(const PrefixItem& i) const {
+    return step * (Unit::tiles(i.a1 - i.a0) + 1.3 * Unit::tiles(i.b1 - i.b0)) + fixed;
   }
-  const double blocks = (double)items.size() * l.kv_heads;
-  // full waves of equal blocks, or the dealt sum plus half a block's tail
-  const double mean = items.empty() ? 0 : sum / items.size();
-  const double waves = std::max(longest, std::min(std::ceil(blocks / slots) * mean,
-                                                  sum * l.kv_heads / slots + 0.5 * longest));
-  return waves + parts * l.q_heads * l.head_dim * 8.0 / 6.0e6;
+};
+
+// Estimated time of a launch: the blocks dealt out in order to the slot that
+// is free first (their sum and half the longest where they are many), joined
+// with the way of their records to the SMs by a soft maximum; then the partial
+// results to memory and back and the launch that joins them.
+double estimate(const Layout& l, const std::vector<PrefixItem>& items, const Cost& c) {
+  if (items.empty()) return 0;
+  double tiles = 0, sum = 0, end = 0;
+  std::vector<int32_t> cover(l.tokens + 1, 0);  // items that begin less those that end
+  for (const PrefixItem& i : items) {
+    tiles += i.steps();
+    sum += c.of(i);
+    ++cover[i.tok0];
+    --cover[i.tok0 + i.ntok];
+  }
+  double parts = 0;  // of the tokens in several items
+  for (int64_t t = 0, n = 0; t < l.tokens; ++t) {
+    n += cover[t];
+    if (n > 1) parts += n;
+  }
+  if ((int64_t)items.size() * l.kv_heads <= 4ll * c.slots) {
+    std::vector<double> busy(c.slots, 0.0);  // a heap, the first to be free in front
+    for (const PrefixItem& i : items)
+      for (int h = 0; h < l.kv_heads; ++h) {
+        std::pop_heap(busy.begin(), busy.end(), std::greater<double>());
+        busy.back() += c.of(i);
+        end = std::max(end, busy.back());
+        std::push_heap(busy.begin(), busy.end(), std::greater<double>());
+      }
+  } else {
+    end = sum * l.kv_heads / c.slots + 0.5 * c.of(items[0]);
+  }
+  const double bytes = tiles * l.kv_heads * kPrefixTile * 4.0 * l.head_dim;
+  end = std::cbrt(std::pow(end, 3) + std::pow(bytes / 6.0e6 + c.fixed, 3));
+  return end + (parts > 0 ? 4.0 + parts * l.q_heads * l.head_dim * 8.0 / 4.0e6 : 0.0);
 }
 
-// The cut of least estimated time: candidates are numbers of key tiles a part.
+// The cut of least estimated time: candidates are numbers of key tiles a part,
+// and with them numbers of units that stay whole (what full rounds of the
+// slots take; the rest, cut, fills the last one).
 template <typename Make>
-double best_cut(const Layout& l, int slots, double step, double fixed, Make units_for,
-                std::vector<PrefixItem>& best) {
+double best_cut(const Layout& l, const Cost& c, Make units_for, std::vector<PrefixItem>& best) {
   double least = -1;
   int64_t longest = 1;
-  for (int64_t most = 1; most <= 2 * longest; most += most < 16 ? 1 : most / 8) {
+  for (int64_t most = 1; most <= 2 * longest; most += most < 6 ? 1 : most / 4) {
     const std::vector<Unit> units = units_for(most);
     for (const Unit& u : units) longest = std::max(longest, u.steps());
-    std::vector<PrefixItem> items = cut(l, units, most);
-    if ((int64_t)items.size() * l.kv_heads > (int64_t)slots * 16 && most < longest) continue;
-    const double e = estimate(l, items, slots, step, fixed);
-    if (least < 0 || e < least) {
-      least = e;
-      best = std::move(items);
+    const size_t rounds = units.size() * l.kv_heads / c.slots;
+    for (size_t whole : {(size_t)0, rounds * c.slots / l.kv_heads}) {
+      if (whole > 0 && most >= longest) continue;
+      std::vector<PrefixItem> items = cut(l, units, most, whole);
+      if ((int64_t)items.size() * l.kv_heads > (int64_t)c.slots * 8 && most < longest) continue;
+      const double e = estimate(l, items, c);
+      if (least < 0 || e < least) {
+        least = e;
+        best = std::move(items);
+      }
+      if (rounds == 0) break;
     }
   }
   return least;
@@ -311,21 +346,18 @@ int make_plan(const cs_prefix_shape* s, cs_prefix_plan_info* info, int32_t* word
   if (tc && tokens > 0) {
     info->variant = 1;
     const int sms = num_sms();
-    // two 128-row blocks an SM, or one 256-row block whose step takes as long
-    // as two of theirs but reads its keys once for all its rows
-    const double e1 = best_cut(l, 2 * sms, 1.0, 2.5,
+    // two blocks of 128 rows an SM, which read their keys for each row tile,
+    // or one of 256 rows; both costs as measured with 32/8 heads of 128
+    const double e1 = best_cut(l, Cost{2 * sms, 1.75, 5.0},
                                [&](int64_t most) { return split_units(l, most * kPrefixTile); },
                                items);
     std::vector<PrefixItem> wide;
-    const double e2 = best_cut(l, sms, 0.9, 4.0,
+    const double e2 = best_cut(l, Cost{sms, 2.1, 6.0},
                                [&](int64_t) { return whole_units(l, 2 * kPrefixTile); }, wide);
     if (e2 >= 0 && (e1 < 0 || e2 < e1)) {
       info->variant = 2;
       items = std::move(wide);
     }
-    std::stable_sort(items.begin(), items.end(), [](const PrefixItem& x, const PrefixItem& y) {
-      return item_steps(x) > item_steps(y);
-    });
     // a token in one item alone gets its output from it, if that holds for
     // all of the item's tokens; the others are joined from partials
     std::vector<int32_t> in(tokens + 1, 0);

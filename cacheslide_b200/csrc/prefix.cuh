@@ -16,16 +16,20 @@
 
 namespace cs {
 
+constexpr int kPrefixTile = 128;  // query rows of a tile, and the plan's unit of keys
+
 struct PrefixItem {
   int32_t tok0, ntok;
   int32_t a0, a1;  // prefix keys
   int32_t b0, b1;  // own keys
   int32_t part;    // first place of its partial results; -1: writes the output
   int32_t pad;
+  int64_t steps() const {
+    return ((int64_t)a1 - a0 + kPrefixTile - 1) / kPrefixTile +
+           ((int64_t)b1 - b0 + kPrefixTile - 1) / kPrefixTile;
+  }
 };
 static_assert(sizeof(PrefixItem) == 32, "plan words");
-
-constexpr int kPrefixTile = 128;  // query rows and keys of a tile
 
 // the tensor-core kernel (prefix_sm100.cu); CS_ERR_UNSUPPORTED when the
 // pool's layout does not fit its loads
