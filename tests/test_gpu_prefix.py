@@ -341,3 +341,30 @@ def test_refusals(cuda):
                    dict(out=s["query"].float())):
         with pytest.raises(ValueError):
             plan(**{**good, **change})
+
+
+def test_both_blocks_and_the_row_kernel_are_reached(cuda):
+    """The plan picks 128-row blocks for decodes, 256-row blocks for prefills of
+    questions and single rows where the tensor cores do not apply."""
+    for name, variant in (("decode many", 1), ("wide batch", 2)):
+        s, lens = batch(cuda, 32, 8, 128, BF, *LAYOUTS[name])
+        assert plan_of(s, lens).info.variant == variant
+    s, lens = batch(cuda, 4, 2, 80, BF, *LAYOUTS["decode"])
+    assert plan_of(s, lens).info.variant == 0
+
+
+@pytest.mark.parametrize("name,variant", [("decode many", 1), ("wide ragged", 2)])
+def test_in_a_graph(cuda, name, variant):
+    s, lens = batch(cuda, 32, 8, 128, BF, *LAYOUTS[name])
+    plan = plan_of(s, lens)
+    args = s["query"], s["cache"], s["prefix_slots"], s["suffix_slots"]
+    want = plan(*args)
+    out = torch.empty_like(want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(3):  # each replayed launch beside the end of the one before
+            plan(*args, out=out)
+    s["query"].copy_(s["query"].roll(1, 0))
+    graph.replay()
+    assert torch.equal(out, plan(*args))
+    assert not torch.equal(out, want)
