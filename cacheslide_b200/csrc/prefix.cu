@@ -274,15 +274,18 @@ double estimate(const Layout& l, const std::vector<PrefixItem>& items, const Cos
 template <typename Make>
 double best_cut(const Layout& l, const Cost& c, Make units_for, std::vector<PrefixItem>& best) {
   double least = -1;
-  int64_t longest = 1;
-  for (int64_t most = 1; most <= 2 * longest; most += most < 6 ? 1 : most / 4) {
+  int64_t longest = 1, tiles = 0;
+  for (const Unit& u : units_for(1)) tiles += u.steps();
+  // from what gives at most eight blocks a slot
+  const int64_t from = std::max<int64_t>(1, tiles * l.kv_heads / (8ll * c.slots));
+  for (int64_t most = from; most <= std::max(from, 2 * longest);
+       most += most < 6 ? 1 : most / 4) {
     const std::vector<Unit> units = units_for(most);
     for (const Unit& u : units) longest = std::max(longest, u.steps());
     const size_t rounds = units.size() * l.kv_heads / c.slots;
     for (size_t whole : {(size_t)0, rounds * c.slots / l.kv_heads}) {
       if (whole > 0 && most >= longest) continue;
       std::vector<PrefixItem> items = cut(l, units, most, whole);
-      if ((int64_t)items.size() * l.kv_heads > (int64_t)c.slots * 8 && most < longest) continue;
       const double e = estimate(l, items, c);
       if (least < 0 || e < least) {
         least = e;

@@ -495,16 +495,21 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
         return base + tk * a.qt + (row - tk * a.G) * a.qh + 16 * c;
       };
       if (a.vec_q && !a.neg) {
+        // rows without a query are zeros: their scores then are zeros too, which
+        // is what P should hold for them, and multiplying zeros draws less of
+        // the power that decodes are held back by
 #pragma unroll 4
-        for (int row = (tid % Sh::kTile) / C; row < rows; row += Sh::kTile / C)
-          cp_async16(qs + sw128(row, c, kPrefixTile), from(row), true);
+        for (int row = (tid % Sh::kTile) / C; row < kPrefixTile; row += Sh::kTile / C)
+          cp_async16(qs + sw128(row, c, kPrefixTile), row < rows ? from(row) : a.q, row < rows);
         cp_async_wait_all();
       } else {
-        for (int row = (tid % Sh::kTile) / C; row < rows; row += Sh::kTile / C) {
+        for (int row = (tid % Sh::kTile) / C; row < kPrefixTile; row += Sh::kTile / C) {
           uint16_t e[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            e[k] = reinterpret_cast<const uint16_t*>(from(row))[k] ^ (a.neg ? 0x8000 : 0);
+            e[k] = row < rows ? reinterpret_cast<const uint16_t*>(from(row))[k] ^
+                                    (a.neg ? 0x8000 : 0)
+                              : 0;
           st_shared16(qs + sw128(row, c, kPrefixTile),
                       make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16,
                                  e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16));
@@ -522,6 +527,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     int exchanges = 0;  // of maxima with the row's other thread
     const uint32_t pair = mb + Sh::bMax + 8 * (4 * qt + (warp & 3));
     float* row_max = reinterpret_cast<float*>(smem + Sh::oMeta + Sh::oMax) + qt * 512;
+    const bool any_row = __any_sync(~0u, row_ok);
     auto wait_pv = [&](int t) {
       ok = warp_wait(at(Sh::bPV, qt, t), (t >> 1) & 1, abort);
       tc_fence_after();
@@ -540,6 +546,10 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       if (!ok) break;  // a wait expired
       if (!Sh::kDirect && tid % Sh::kTile == 0) mbar_arrive(mb + Sh::bKr + 8 * (t % Sh::KS));
       tc_fence_after();
+      if (!any_row) {  // no query in these 32 rows: their P is zero already
+        mbar_arrive(at(Sh::bP, qt, t));
+        continue;
+      }
       uint32_t v[VC];
       // both threads of a row leave this way together
       if (__all_sync(~0u, vhi <= vlo)) {  // nothing to see for these 32 rows
