@@ -257,36 +257,35 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     }
     return r;
   };
-  auto resolve = [&](int t, const Slots& in, Src& s) {
+  // rows of the pool's map, for two keys in one block (32-bit arithmetic: a map
+  // has fewer than 2^31 rows, and there is none for larger pools)
+  auto resolve = [&](const Slots& in, Src& s) {
+    const uint32_t s0 = (uint32_t)in.s[0];
+    s.run = a.tma != 0 && in.s[0] >= 0 && in.s[1] == in.s[0] + 1 && in.s[1] < a.pv.native_total;
+    const uint32_t b = s.run ? (a.bs_shift >= 0 ? s0 >> a.bs_shift : s0 / (uint32_t)a.pv.bs) : 0u;
+    const uint32_t o = s0 - b * (uint32_t)a.pv.bs;
+    s.run = s.run && o + 1 < (uint32_t)a.pv.bs;
+    s.row = (int)(b * (uint32_t)a.nrb + g * (uint32_t)a.nrh + o);
+  };
+  auto addresses = [&](int t, const Slots& in, Src& s) {
     const Step st = step_of(it, na, t);
-    const int64_t* sl = in.s;
-    s.run = a.tma != 0 && sl[0] >= 0 && sl[1] < a.pv.native_total;
-    s.row = 0;
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       s.at[m] = 0;
-      int64_t b = 0, o = 0;
-      if (a.pv.valid(sl[m])) {
-        if (sl[m] < a.pv.native_total) {
-          if (a.bs_shift >= 0) {
-            b = sl[m] >> a.bs_shift;
-            o = sl[m] - (b << a.bs_shift);
-          } else {
-            b = sl[m] / a.pv.bs;
-            o = sl[m] - b * a.pv.bs;
-          }
+      const int64_t sl = in.s[m];
+      if (a.pv.valid(sl)) {
+        if (sl < a.pv.native_total) {
+          const int64_t b = a.bs_shift >= 0 ? sl >> a.bs_shift : sl / a.pv.bs;
+          const int64_t o = sl - (a.bs_shift >= 0 ? b << a.bs_shift : b * a.pv.bs);
           s.at[m] = reinterpret_cast<uint64_t>(a.pv.cache) + b * a.pv.sb + g * a.pv.sh +
                     o * a.pv.so + (isv ? 2 * D : 0);
         } else {
           s.at[m] = reinterpret_cast<uint64_t>(isv ? a.pv.side_v : a.pv.side_k) +
-                    (sl[m] - a.pv.native_total) * a.pv.ssr + g * a.pv.ssh;
+                    (sl - a.pv.native_total) * a.pv.ssr + g * a.pv.ssh;
         }
       } else if (2 * lane + m < st.n) {
         slot_bad = true;
       }
-      if (m == 0) s.row = (int)(b * a.nrb + g * a.nrh + o * a.nro);
-      // consecutive slots of one block, and blocks whose offsets are rows
-      s.run = s.run && sl[m] == sl[0] + m && (m == 0 || o > 0) && a.nro == 1;
     }
   };
   if (tid == 0) {
@@ -329,7 +328,12 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     int issued = 0;
     auto produce = [&](int t, Slots& mine) {
       Src cur;
-      resolve(t, mine, cur);
+      resolve(mine, cur);
+      const int r16 = __shfl_sync(~0u, cur.row, lane & ~7);
+      const uint32_t sq = __ballot_sync(~0u, cur.run && cur.row == r16 + 2 * (lane & 7));
+      const bool in_run = ((sq >> (lane & ~7)) & 0xFFu) == 0xFFu;
+      const uint32_t leads = __ballot_sync(~0u, in_run) & 0x01010101u;
+      if (leads != 0x01010101u) addresses(t, mine, cur);
       mine = load_slots(t + 3);
       // the stage is free once every row tile is done with its last use
       if (t >= ST) {
@@ -348,10 +352,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       // the others row by row with cp.async, whole rows an instruction, the
       // addresses through shared memory.  (tile::gather4 is issued lane by
       // lane, about 100 clocks each: 6400 for a tile of scattered rows.)
-      const int r16 = __shfl_sync(~0u, cur.row, lane & ~7);
-      const uint32_t sq = __ballot_sync(~0u, cur.run && cur.row == r16 + 2 * (lane & 7));
-      const bool lead = (lane & 7) == 0 && ((sq >> lane) & 0xFFu) == 0xFFu;
-      const uint32_t leads = __ballot_sync(~0u, lead);
       const uint32_t tab_at = Sh::oRows + (isv ? kKeys * 8 : 0);
       if (leads != 0x01010101u)
         st_shared16(mb + tab_at + 16 * lane,
@@ -359,11 +359,10 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
                                (uint32_t)cur.at[1], (uint32_t)(cur.at[1] >> 32)));
       if (lane == 0) mbar_expect_tx(bar, __popc(leads) * 16 * D * 2);
       __syncwarp();
-      if (lead) {
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c)
-          tma_tile2d(dst + c * (kKeys * 128) + 2 * lane * 128, &a.tm, (isv ? D : 0) + 64 * c,
-                     cur.row, bar);
+      if (in_run && (lane & 7) < D / 64) {
+        const int c = lane & 7;  // 64 columns each
+        tma_tile2d(dst + c * (kKeys * 128) + 2 * (lane & ~7) * 128, &a.tm, (isv ? D : 0) + 64 * c,
+                   r16, bar);
       }
       if (leads != 0x01010101u) {
         constexpr int C = D / 8, RI = 32 / C;  // 16-byte pieces a row, rows an instruction
@@ -955,7 +954,8 @@ int prefix_attn_sm100(const cs_prefix_params& p, const cs_prefix_plan_info& info
   a.scale2 = fmaxf(fabsf((float)p.scale) * kLog2e, 1e-30f);
   a.scale = (float)p.scale;
   a.nrb = a.nrh = a.nro = 0;
-  a.tma = setup_maps(a, kv) ? 1 : 0;
+  // runs are found where a block's offsets are consecutive rows
+  a.tma = setup_maps(a, kv) && a.nro == 1 ? 1 : 0;
   const bool half = kv.dtype == CS_F16;
   if (kv.head_dim == 128)
     return half ? launch_all<__half, 128>(a, info, plan, stream)
