@@ -419,10 +419,14 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       const uint32_t sc = tm + Sh::cS + 128 * qt, oc = tm + Sh::cO + D * qt;
       bool ok = warp_wait(mb + Sh::bQ, 0, abort);
       uint32_t last = 0, lastph = 0;  // the newest group issued
+      // a key tile that has arrived (and, for rows copied by cp.async, may be
+      // read by the tensor unit); waited for ahead of what comes later
+      auto arrived = [&](uint32_t bar, int t, int stages) {
+        ok = ok && warp_wait(mb + bar + 8 * (t % stages), (t / stages) & 1, abort);
+        fence_async_smem();
+        return ok;
+      };
       auto scores = [&](int t) {
-        ok = warp_wait(mb + Sh::bK + 8 * (t % Sh::KS), (t / Sh::KS) & 1, abort);
-        if (!ok) return;
-        fence_async_smem();  // rows copied by cp.async
         tc_fence_after();
         const uint64_t dk = dk0 + (uint64_t)((t % Sh::KS) * (Sh::TB >> 4));
         const uint32_t s = sc + kKeys * (t & 1);
@@ -437,13 +441,12 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
         }
         __syncwarp();
       };
-      if (ok && steps > 0) scores(0);
-      if (ok && steps > 1) scores(1);
+      if (steps > 0 && arrived(Sh::bK, 0, Sh::KS)) scores(0);
+      if (steps > 1 && arrived(Sh::bK, 1, Sh::KS)) scores(1);
       for (int t = 0; ok && t < steps; ++t) {
         const uint32_t ph = (t >> 1) & 1;
+        if (!arrived(Sh::bV, t, Sh::VS)) break;
         if (!(ok = warp_wait(at(Sh::bP, qt, t), ph, abort))) break;
-        if (!(ok = warp_wait(mb + Sh::bV + 8 * (t % Sh::VS), (t / Sh::VS) & 1, abort))) break;
-        fence_async_smem();
         tc_fence_after();
         const uint64_t dv = dv0 + (uint64_t)((t % Sh::VS) * (Sh::TB >> 4));
         const uint32_t p = sc + kKeys * (t & 1);
@@ -460,9 +463,10 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
         // V tile the stage just read
         const bool refill = !Sh::kDirect && t + Sh::VS < steps;
         if (t + 2 < steps || refill) {
-          if (!(ok = warp_wait(last, ph, abort))) break;
+          if (t + 2 < steps && Sh::kDirect && !arrived(Sh::bK, t + 2, Sh::KS)) break;
+          if (!(ok = warp_wait(at(Sh::bPV, qt, t), ph, abort))) break;
           if (refill && leader) mbar_arrive(mb + Sh::bVr + 8 * (t % Sh::VS));
-          if (t + 2 < steps) scores(t + 2);
+          if (t + 2 < steps && (Sh::kDirect || arrived(Sh::bK, t + 2, Sh::KS))) scores(t + 2);
         }
       }
       if (last) {
