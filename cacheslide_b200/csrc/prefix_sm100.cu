@@ -308,7 +308,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
   if (warp == Sh::kSoft + 2) tmem_alloc(mb + Sh::oTmem, Sh::kCols);
   // everything above touches only this block and the plan, which no kernel
   // writes; from here on the preceding grids' results are read
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   Slots ahead[3];
   if (warp == Sh::kSoft || warp == Sh::kSoft + 1) {
@@ -782,6 +781,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     }
   }
 
+  // the joining grid starts while the last blocks write (told earlier, its
+  // blocks wait beside these and cost 8 decodes behind 65536 keys 5 us)
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && *abort) report(a.status, CS_ST_TIMEOUT);
@@ -791,21 +793,29 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
   }
 }
 
-// One warp per (join token, head): o = sum_c w_c o_c / sum_c w_c with
-// w_c = 2^(lse_c - max), the partials in the plan's order.
-template <typename T, int D>
+// WPR warps per (join token, head): o = sum_c w_c o_c / sum_c w_c with
+// w_c = 2^(lse_c - max), warp i taking partials i, i + WPR, ... of the plan's
+// order, the warps' sums added in order.  Four warps where tokens have more
+// than 16 partials: 8 decodes behind 65536 keys (36 a token) take 53 us with
+// four and 59 with one, 64 decodes behind 5120 (11 a token) 26.7 and 23.5.
+template <typename T, int D, int WPR>
 __global__ void __launch_bounds__(128) prefix_join_kernel(const PArgs a, const int4* join,
                                                           const int32_t* list, int n) {
   constexpr int E = D / 32;
+  using V = typename std::conditional<E == 4, float4, float2>::type;
+  __shared__ V part_sum[WPR][32];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x & 31;
-  const int64_t w = blockIdx.x * 4ll + (threadIdx.x >> 5);
-  if (w >= (int64_t)n * a.hq) return;
-  const int4 j = join[w / a.hq];
+  const int lane = threadIdx.x & 31, wi = (threadIdx.x >> 5) % WPR;
+  const int64_t w = blockIdx.x * (4ll / WPR) + (threadIdx.x >> 5) / WPR;
+  const bool live = w < (int64_t)n * a.hq;
+  const int4 j = live ? join[w / a.hq] : make_int4(0, 0, 0, 0);
   const int h = (int)(w % a.hq);
-  float top = -INFINITY;
-  for (int c = lane; c < j.z; c += 32)
+  int32_t first = lane < j.z ? list[j.y + lane] : 0;
+  // the plan may be read before the preceding grid is done, its results not
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const float l0 = lane < j.z ? a.part_lse[(int64_t)first * a.hq + h] : -INFINITY;
+  float top = l0;
+  for (int c = 32 + lane; c < j.z; c += 32)
     top = fmaxf(top, a.part_lse[(int64_t)list[j.y + c] * a.hq + h]);
   top = warp_max(top);
   float o[E], sum = 0.f;
@@ -813,36 +823,51 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const PArgs a, const i
   for (int e = 0; e < E; ++e) o[e] = 0.f;
   for (int c0 = 0; c0 < j.z; c0 += 32) {
     // a lane's partial of these 32: its place and weight (NaN stays NaN)
-    int64_t row = 0;
-    float f = 0.f;
-    if (c0 + lane < j.z) {
-      row = (int64_t)list[j.y + c0 + lane] * a.hq + h;
-      const float l = a.part_lse[row];
-      f = l == -INFINITY ? 0.f : ex2(l - top);
+    float l = l0;
+    if (c0 > 0) {
+      first = c0 + lane < j.z ? list[j.y + c0 + lane] : 0;
+      l = c0 + lane < j.z ? a.part_lse[(int64_t)first * a.hq + h] : -INFINITY;
     }
+    const float f = l == -INFINITY ? 0.f : ex2(l - top);
     sum += warp_sum(f);
-    const int n = j.z - c0 < 32 ? j.z - c0 : 32;
+    const int m = j.z - c0 < 32 ? j.z - c0 : 32;
 #pragma unroll 1
-    for (int c = 0; c < n; c += 8) {
-      float x[8][E], w[8];
+    for (int c = wi; c < m; c += 8 * WPR) {
+      V x[8];
+      float wk[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const int64_t rk = __shfl_sync(~0u, row, c + k);
-        w[k] = __shfl_sync(~0u, f, c + k);
-        if (c + k >= n || w[k] == 0.f) w[k] = 0.f;
-        else {
-#pragma unroll
-          for (int e = 0; e < E; ++e) x[k][e] = a.part_o[rk * D + lane * E + e];
-        }
+        const int q = c + k * WPR;
+        const int64_t place = __shfl_sync(~0u, first, q & 31);
+        const float fk = __shfl_sync(~0u, f, q & 31);
+        wk[k] = q < m ? fk : 0.f;
+        if (wk[k] != 0.f)
+          x[k] = reinterpret_cast<const V*>(a.part_o + (place * a.hq + h) * D)[lane];
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        if (w[k] != 0.f) {
+        if (wk[k] != 0.f) {
+          const float* v = reinterpret_cast<const float*>(&x[k]);
 #pragma unroll
-          for (int e = 0; e < E; ++e) o[e] = fmaf(w[k], x[k][e], o[e]);
+          for (int e = 0; e < E; ++e) o[e] = fmaf(wk[k], v[e], o[e]);
         }
     }
   }
+  if constexpr (WPR > 1) {
+    V mine;
+#pragma unroll
+    for (int e = 0; e < E; ++e) reinterpret_cast<float*>(&mine)[e] = o[e];
+    part_sum[wi][lane] = mine;
+    __syncthreads();
+    if (wi > 0) return;
+#pragma unroll
+    for (int k = 1; k < WPR; ++k) {
+      const V x = part_sum[k][lane];
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] += reinterpret_cast<const float*>(&x)[e];
+    }
+  }
+  if (!live) return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   T* out = reinterpret_cast<T*>(a.out + (int64_t)j.x * a.ot + (int64_t)h * a.oh) + lane * E;
 #pragma unroll
@@ -911,10 +936,14 @@ int launch_all(const PArgs& a, const cs_prefix_plan_info& info, const int32_t* p
     if (rc != CS_OK) return rc;
   }
   if (info.n_join > 0) {
-    const unsigned blocks = (unsigned)((info.n_join * a.hq + 3) / 4);
-    return launch_dependent(prefix_join_kernel<T, D>, blocks, 128, 0, stream, a,
-                            reinterpret_cast<const int4*>(plan + info.join_off),
-                            plan + info.list_off, (int)info.n_join);
+    const int4* join = reinterpret_cast<const int4*>(plan + info.join_off);
+    const int32_t* list = plan + info.list_off;
+    const int64_t rows = info.n_join * a.hq, entries = info.words - info.list_off;
+    if (entries > 16 * info.n_join)
+      return launch_dependent(prefix_join_kernel<T, D, 4>, (unsigned)rows, 128, 0, stream, a, join,
+                              list, (int)info.n_join);
+    return launch_dependent(prefix_join_kernel<T, D, 1>, (unsigned)((rows + 3) / 4), 128, 0,
+                            stream, a, join, list, (int)info.n_join);
   }
   return CS_OK;
 }
