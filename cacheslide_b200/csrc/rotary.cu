@@ -147,7 +147,8 @@ __global__ void __launch_bounds__(kRowWarps * 32)
 }
 
 // Append: rows of q (dense out), k (rotated into the record's K half) and v
-// (copied into its V half).
+// (copied into its V half).  These one-warp-a-row kernels serve the heads,
+// strides and pools that vectors do not fit (latency bound, about 0.8 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(kRowWarps * 32)
     append_rows_kernel(RotArgs a, PagedView pv, const int64_t* __restrict__ slots, Rows v) {
@@ -286,6 +287,12 @@ __global__ void __launch_bounds__(kRowWarps * 32)
 // keep a lane's share small (8 elements of a row): with 8 pairs a lane the
 // kernels held 98 (forward) and 118 (gradient) registers, a quarter of the
 // SM's warps, and 2.9 TB/s.
+//
+// Forward, 32768 tokens of 32/8 heads of 128, bf16: 123 us, 5.5 TB/s, held
+// back by the instructions of the norm (two thirds of the issue slots);
+// append of 65536 tokens of 64/8 heads without norms, fp16: 404 us, 6.7 TB/s,
+// HBM.  Two groups a task: 143 and 497 us; eight: 137 and 422 us; 1, 2 or 8
+// warps a block: 129, 123, 129 us.
 constexpr int kP = 4;        // pairs a lane
 constexpr int kGroups = 4;   // row groups a task
 constexpr int kVecWarps = 4;
@@ -572,19 +579,32 @@ __device__ __forceinline__ void store_pairs(const Pairs<P>& p, uint4& x, uint4& 
   x = pack16<T, P>(u);
   y = pack16<T, P>(v);
 }
-template <int P, bool INTER>
-__device__ __forceinline__ Lane lane_of16(const RotArgs& a, int l) {
-  Lane n;
-  n.p0 = l * P;
+// which elements a lane owns: vectors at e0 and e1; its pairs are pa on (the
+// first half of them) and pb on, each half turning or not.  Interleaved pairs
+// lie inside a vector, and a row's vectors go to its lanes in two rounds, so
+// that an instruction copies neighbouring vectors (adjacent vectors a lane
+// left half of every sector to a second copy: 240 us against 180).
+struct Lane16 {
+  int e0, e1, pa, pb;
+  bool ta, tb;
+};
+template <int P, int LPR, bool INTER>
+__device__ __forceinline__ Lane16 lane_of16(const RotArgs& a, int l) {
+  Lane16 n;
   const int half = a.rot >> 1;
-  n.turns = n.p0 < half;
-  if (n.turns) {
-    n.e0 = INTER ? 2 * n.p0 : n.p0;
-    n.e1 = INTER ? n.e0 + P : n.p0 + half;
+  if constexpr (INTER) {
+    n.e0 = l * P;
+    n.e1 = (l + LPR) * P;
+    n.pa = n.e0 / 2;
+    n.pb = n.e1 / 2;
   } else {
-    n.e0 = a.rot + (n.p0 - half);
-    n.e1 = n.e0 + ((a.dim - a.rot) >> 1);
+    n.pa = l * P;
+    n.pb = n.pa + P / 2;
+    n.e0 = n.pa < half ? n.pa : a.rot + (n.pa - half);
+    n.e1 = n.e0 + (n.pa < half ? half : (a.dim - a.rot) >> 1);
   }
+  n.ta = n.pa < half;
+  n.tb = n.pb < half;
   return n;
 }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
@@ -593,6 +613,10 @@ __device__ __forceinline__ float2 neg(float2 x) { return make_float2(-x.x, -x.y)
 // P floats of shared memory, 16-byte aligned
 template <int P>
 __device__ __forceinline__ void load_floats(const float* src, float* f) {
+  if constexpr (P == 2) {
+    const float2 v = *reinterpret_cast<const float2*>(src);
+    f[0] = v.x, f[1] = v.y;
+  }
 #pragma unroll
   for (int i = 0; i < P / 4; ++i) {
     const float4 v = reinterpret_cast<const float4*>(src)[i];
@@ -600,7 +624,7 @@ __device__ __forceinline__ void load_floats(const float* src, float* f) {
   }
 }
 template <int P, bool INTER>
-__device__ __forceinline__ void shared_weights(const float* w, const Lane& ln, Pairs<P>& p) {
+__device__ __forceinline__ void shared_weights(const float* w, const Lane16& ln, Pairs<P>& p) {
   float u[P], v[P];
   load_floats<P>(w + ln.e0, u);
   load_floats<P>(w + ln.e1, v);
@@ -626,13 +650,12 @@ struct Place {
 // grad_weight_kernel) blocks are added in order.  Angles come with the rows
 // of a token's first group, weights lie in shared memory.
 //
-// 32768 tokens of 32/8 heads of 128, bf16: 187 us, 5.4 TB/s.  Tried: plain loads of 4
-// pairs a lane, two row groups in flight, three blocks an SM (286 us); this
-// ring with 80 registers and three blocks (325 us: spills); the same ring for
-// the forward (119 us against 123 us with plain loads, but 167 us where pairs
-// are interleaved), so the forward stays with plain loads.
+// 32768 tokens of 32/8 heads of 128, bf16: 176 us, 5.7 TB/s (interleaved pairs
+// 180 us).  Tried: plain loads of 4 pairs a lane, two row groups in flight,
+// three blocks an SM (286 us); this ring with 80 registers and three blocks
+// (325 us: spills); rings of 4 and 6 groups (185 and 255 us).
 constexpr int kStreamWarps = 8;
-constexpr int kRing = 4;  // row groups a warp has in flight, one being read
+constexpr int kRing = 3;  // row groups a warp has in flight, one being read
 
 template <typename T, int LPR>
 struct Stream {
@@ -663,7 +686,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 2)
   const Rows& rw = isk ? a.k : a.q;
   const int first = isk ? nq : 0;
   const unsigned step = (isk ? gridDim.x - nq : nq) * kStreamWarps;
-  const Lane ln = lane_of16<P, INTER>(a, lane % LPR);
+  const Lane16 ln = lane_of16<P, LPR, INTER>(a, lane % LPR);
   const bool norm = rw.w != nullptr;
   const int half = a.rot >> 1;
   for (int e = threadIdx.x; e < D; e += blockDim.x)
@@ -684,14 +707,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 2)
   int64_t pos = in.task < total ? a.positions[in.t] : 0;
   bool fresh = true;  // `in` is at a task's first group
   int in_slot = 0, in_ang = 0;
-  // interleaved pairs: a lane's two vectors are neighbours, so each copy takes
-  // half of every 32-byte sector and the other half should hit L1
-  auto copy = [&](uint32_t dst, const T* src) {
-    if constexpr (INTER)
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-    else
-      cp_async16(dst, src, true);
-  };
+  auto copy = [&](uint32_t dst, const T* src) { cp_async16(dst, src, true); };
   auto issue = [&]() {
     if (in.task < total) {
       if (fresh) {
@@ -737,7 +753,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 2)
 
   int slot = 0, aslot = 0;
   while (at.task < total) {
-    const float* cs = ang + aslot * D + ln.p0;
+    const float* cs = ang + aslot * D;
     aslot = aslot == kRing - 1 ? 0 : aslot + 1;
     for (; at.u < at.end; ++at.u) {
       cp_async_wait<kRing - 2>();
@@ -749,17 +765,33 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 2)
       Pairs<P> g, n, w;
       load_pairs<T, P, INTER>(mine[64], mine[96], g);
       if (norm) load_pairs<T, P, INTER>(mine[0], mine[32], n);
-      if (ln.turns) {
-        float cv[P], sv[P];
-        load_floats<P>(cs, cv);
-        load_floats<P>(cs + D / 2, sv);
+      float cv[P], sv[P];
+      auto turn_back = [&](int i) {
+        const float2 c = make_float2(cv[2 * i], cv[2 * i + 1]);
+        const float2 s = make_float2(sv[2 * i], sv[2 * i + 1]);
+        const float2 t = __ffma2_rn(g.a[i], c, __fmul2_rn(g.b[i], s));
+        g.b[i] = __ffma2_rn(g.b[i], c, neg(__fmul2_rn(g.a[i], s)));
+        g.a[i] = t;
+      };
+      if constexpr (!INTER) {
+        if (ln.ta) {
+          load_floats<P>(cs + ln.pa, cv);
+          load_floats<P>(cs + D / 2 + ln.pa, sv);
 #pragma unroll
-        for (int i = 0; i < P / 2; ++i) {
-          const float2 c = make_float2(cv[2 * i], cv[2 * i + 1]);
-          const float2 s = make_float2(sv[2 * i], sv[2 * i + 1]);
-          const float2 t = __ffma2_rn(g.a[i], c, __fmul2_rn(g.b[i], s));
-          g.b[i] = __ffma2_rn(g.b[i], c, neg(__fmul2_rn(g.a[i], s)));
-          g.a[i] = t;
+          for (int i = 0; i < P / 2; ++i) turn_back(i);
+        }
+      } else {
+        if (ln.ta) {
+          load_floats<P / 2>(cs + ln.pa, cv);
+          load_floats<P / 2>(cs + D / 2 + ln.pa, sv);
+#pragma unroll
+          for (int i = 0; i < P / 4; ++i) turn_back(i);
+        }
+        if (ln.tb) {
+          load_floats<P / 2>(cs + ln.pb, cv + P / 2);
+          load_floats<P / 2>(cs + D / 2 + ln.pb, sv + P / 2);
+#pragma unroll
+          for (int i = P / 4; i < P / 2; ++i) turn_back(i);
         }
       }
       issue();  // into the slot read in the last round
