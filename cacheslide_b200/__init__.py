@@ -17,7 +17,8 @@ drop-in replacement:
 * ``rotary``    -- head norms with the position rotation (differentiable) and
   the rotated append into the paged pool, for rotary layers on that pool;
 * ``prefix``    -- ``SharedPrefixAttention``: those layers' attention over the
-  pool for a batch that shares a long prefix.
+  pool for a batch that shares a long prefix;
+* ``rotary_rag`` -- ``RotaryRagBatch``: the two together for a retrieval batch.
 
 All device arithmetic is in ``_lib/libcacheslide_sm100.so`` (C ABI declared in
 ``include/cacheslide_b200.h``); build it with ``python -m cacheslide_b200.build``.
