@@ -295,6 +295,18 @@ def stream_of(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def launch(name: str, device: torch.device, *args) -> None:
+    """Call an entry point whose last argument is the stream, on ``device``'s
+    current stream and with ``device`` current, and check its status."""
+    fn = getattr(load(), name)
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, stream_of(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, stream_of(device))
+    check(rc, name)
+
+
 def require_cuda(*tensors: torch.Tensor) -> torch.device:
     device = None
     for t in tensors:

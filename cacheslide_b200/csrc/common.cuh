@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/cacheslide_b200.h"
 
 #define CS_HOST_CHECK(cond)        \
@@ -200,6 +202,24 @@ __device__ __forceinline__ int batch_item(const int64_t* start, int count, int64
     else hi = mid - 1;
   }
   return lo;
+}
+
+// Allows the kernel Kernel more than 48 KB of dynamic shared memory, once per
+// device (the attribute belongs to a device's context).
+template <auto Kernel>
+inline bool allow_smem(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return true;
+  if (cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
+      cudaSuccess) {
+    (void)cudaGetLastError();
+    return false;
+  }
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
 }
 
 inline int num_sms() {

@@ -4,7 +4,6 @@
 #include <cmath>
 #include <cstring>
 #include <functional>
-#include <new>
 #include <type_traits>
 #include <vector>
 
@@ -421,8 +420,8 @@ extern "C" int cs_prefix_plan(const cs_prefix_shape* s, cs_prefix_plan_info* inf
   if (s->head_dim > kMaxDim) return CS_ERR_UNSUPPORTED;
   try {
     return make_plan(s, info, words, capacity);
-  } catch (const std::bad_alloc&) {
-    return CS_ERR_UNSUPPORTED;
+  } catch (...) {  // no memory: nothing may leave a C entry but a status
+    return CS_ERR_TOO_LARGE;
   }
 }
 

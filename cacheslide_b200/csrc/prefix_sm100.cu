@@ -927,11 +927,8 @@ int launch_dependent(K kernel, unsigned blocks, int threads, uint32_t smem, cuda
 
 template <typename T, int D, int NT>
 int launch_main(const PArgs& a, int64_t blocks, cudaStream_t stream) {
-  auto kernel = prefix_sm100_kernel<T, D, NT>;
-  static const bool ready =
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           Shape<D, NT>::kSmem) == cudaSuccess;
-  if (!ready) return CS_ERR_CUDA;
+  constexpr auto kernel = prefix_sm100_kernel<T, D, NT>;
+  if (!allow_smem<kernel>(Shape<D, NT>::kSmem)) return CS_ERR_CUDA;
   return launch_dependent(kernel, (unsigned)blocks, Shape<D, NT>::kThreads, Shape<D, NT>::kSmem,
                           stream, a);
 }

@@ -766,9 +766,9 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 2)
       load_pairs<T, P, INTER>(mine[64], mine[96], g);
       if (norm) load_pairs<T, P, INTER>(mine[0], mine[32], n);
       float cv[P], sv[P];
-      auto turn_back = [&](int i) {
-        const float2 c = make_float2(cv[2 * i], cv[2 * i + 1]);
-        const float2 s = make_float2(sv[2 * i], sv[2 * i + 1]);
+      auto turn_back = [&](int i, const float* cp, const float* sp) {
+        const float2 c = make_float2(cp[2 * i], cp[2 * i + 1]);
+        const float2 s = make_float2(sp[2 * i], sp[2 * i + 1]);
         const float2 t = __ffma2_rn(g.a[i], c, __fmul2_rn(g.b[i], s));
         g.b[i] = __ffma2_rn(g.b[i], c, neg(__fmul2_rn(g.a[i], s)));
         g.a[i] = t;
@@ -778,20 +778,20 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 2)
           load_floats<P>(cs + ln.pa, cv);
           load_floats<P>(cs + D / 2 + ln.pa, sv);
 #pragma unroll
-          for (int i = 0; i < P / 2; ++i) turn_back(i);
+          for (int i = 0; i < P / 2; ++i) turn_back(i, cv, sv);
         }
       } else {
         if (ln.ta) {
           load_floats<P / 2>(cs + ln.pa, cv);
           load_floats<P / 2>(cs + D / 2 + ln.pa, sv);
 #pragma unroll
-          for (int i = 0; i < P / 4; ++i) turn_back(i);
+          for (int i = 0; i < P / 4; ++i) turn_back(i, cv, sv);
         }
         if (ln.tb) {
           load_floats<P / 2>(cs + ln.pb, cv + P / 2);
           load_floats<P / 2>(cs + D / 2 + ln.pb, sv + P / 2);
 #pragma unroll
-          for (int i = P / 4; i < P / 2; ++i) turn_back(i);
+          for (int i = P / 4; i < P / 2; ++i) turn_back(i, cv, sv);
         }
       }
       issue();  // into the slot read in the last round
@@ -1065,23 +1065,26 @@ extern "C" int cs_qk_norm_rope_grad(const cs_rotary_params* p, const void* q_dy,
   int nq, n, rc;
   if (lanes) {
     const Shares s = shares(a, lanes);
+    bool ready = true;
     nq = s.nq, n = s.n;
     rc = n == 0 ? CS_OK : by_type(p->dtype, [&](auto* ty) {
       using T = std::remove_pointer_t<decltype(ty)>;
       by_lanes(lanes, [&](auto l) {
         auto go = [&](auto inter) {
           constexpr int L = decltype(l)::value;
-          auto kernel = norm_rope_grad_kernel<T, L, decltype(inter)::value>;
+          constexpr auto kernel = norm_rope_grad_kernel<T, L, decltype(inter)::value>;
           constexpr int kBytes = Stream<T, L>::kUnits * 16;
-          static const cudaError_t set =
-              cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
-          (void)set;  // a failure shows at the launch
+          if (!allow_smem<kernel>(kBytes)) {
+            ready = false;
+            return;
+          }
           kernel<<<s.n, kStreamWarps * 32, kBytes, as_stream(stream)>>>(a, s.nq, s.parts, part);
         };
         if (a.interleaved) go(std::true_type());
         else go(std::false_type());
       });
     });
+    if (!ready) return CS_ERR_CUDA;
   } else {
     const int hq = p->q_heads, heads = hq + p->k_heads;
     auto share = [&](int h) {

@@ -135,6 +135,6 @@ class SharedPrefixAttention:
         workspace = None
         if self.info.workspace:
             workspace = torch.empty(self.info.workspace, dtype=torch.uint8, device=device)
-        N.check(N.load().cs_prefix_attn(p, self.info, self.words.data_ptr(), N.ptr(workspace),
-                                        N.stream_of(device)), "cs_prefix_attn")
+        N.launch("cs_prefix_attn", device, p, self.info, self.words.data_ptr(),
+                 N.ptr(workspace))
         return (out, lse) if return_lse else out

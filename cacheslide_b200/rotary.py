@@ -122,7 +122,7 @@ def _forward(query, key, positions, cos, sin, q_weight, k_weight, eps, interleav
     k_out = torch.empty(key.shape, dtype=key.dtype, device=key.device)
     p = _params(query, key, positions, cos, sin, q_weight, k_weight, eps, interleaved, q_out,
                 k_out, status)
-    N.check(N.load().cs_qk_norm_rope(p, N.stream_of(key.device)), "cs_qk_norm_rope")
+    N.launch("cs_qk_norm_rope", key.device, p)
     return q_out, k_out
 
 
@@ -146,12 +146,10 @@ class _NormRope(torch.autograd.Function):
                     status)
         dqw = None if q_weight is None else torch.empty_like(q_weight)
         dkw = None if k_weight is None else torch.empty_like(k_weight)
-        lib = N.load()
-        workspace = torch.empty(lib.cs_qk_norm_rope_grad_workspace(p), dtype=torch.uint8,
+        workspace = torch.empty(N.load().cs_qk_norm_rope_grad_workspace(p), dtype=torch.uint8,
                                 device=key.device)
-        N.check(lib.cs_qk_norm_rope_grad(
-            p, q_dy.data_ptr(), k_dy.data_ptr(), N.ptr(dqw), N.ptr(dkw), workspace.data_ptr(),
-            N.stream_of(key.device)), "cs_qk_norm_rope_grad")
+        N.launch("cs_qk_norm_rope_grad", key.device, p, q_dy.data_ptr(), k_dy.data_ptr(),
+                 N.ptr(dqw), N.ptr(dkw), workspace.data_ptr())
         return dq, dk, None, None, None, dqw, dkw, None, None, None
 
 
@@ -228,7 +226,6 @@ def append_rotated(kv: Tensor | NativePagedKV | N.PagedKV, slots: Tensor, key: T
     if view.dtype != p.dtype or view.kv_heads != p.k_heads or view.head_dim != p.head_dim:
         raise ValueError("K/V must match the pool's dtype, KV heads and head dim")
     st = value.stride()
-    N.check(N.load().cs_kv_append_rotated(p, view, slots.data_ptr(), value.data_ptr(), st[0],
-                                          st[1], N.stream_of(key.device)),
-            "cs_kv_append_rotated")
+    N.launch("cs_kv_append_rotated", key.device, p, view, slots.data_ptr(), value.data_ptr(),
+             st[0], st[1])
     return out
