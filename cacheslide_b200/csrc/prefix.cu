@@ -214,10 +214,6 @@ std::vector<PrefixItem> cut(const Layout& l, const std::vector<Unit>& units, int
                      (int32_t)v.b0, (int32_t)v.b1, -1, 0});
     }
   }
-  // long ones first, as the blocks are dealt out
-  std::stable_sort(out.begin(), out.end(), [](const PrefixItem& x, const PrefixItem& y) {
-    return x.steps() > y.steps();
-  });
   return out;
 }
 
@@ -235,44 +231,72 @@ struct Cost {
 // is free first (their sum and half the longest where they are many), joined
 // with the way of their records to the SMs by a soft maximum; then the partial
 // results to memory and back and the launch that joins them.
-double estimate(const Layout& l, const std::vector<PrefixItem>& items, const Cost& c) {
-  if (items.empty()) return 0;
-  double tiles = 0, sum = 0, end = 0;
-  std::vector<int32_t> cover(l.tokens + 1, 0);  // items that begin less those that end
-  for (const PrefixItem& i : items) {
-    tiles += i.steps();
-    sum += c.of(i);
-    ++cover[i.tok0];
-    --cover[i.tok0 + i.ntok];
+class Estimate {
+ public:
+  Estimate(const Layout& l, const std::vector<PrefixItem>& items, const Cost& c)
+      : heads_(l.kv_heads), c_(c) {
+    if (items.empty()) return;
+    double tiles = 0, sum = 0, longest = 0;
+    const PrefixItem* first = &items[0];  // of those with the most key tiles
+    std::vector<int32_t> cover(l.tokens + 1, 0);  // items that begin less those that end
+    for (const PrefixItem& i : items) {
+      tiles += i.steps();
+      sum += c.of(i);
+      longest = std::max(longest, c.of(i));
+      if (i.steps() > first->steps()) first = &i;
+      ++cover[i.tok0];
+      --cover[i.tok0 + i.ntok];
+    }
+    double parts = 0;  // of the tokens in several items
+    for (int64_t t = 0, n = 0; t < l.tokens; ++t) {
+      n += cover[t];
+      if (n > 1) parts += n;
+    }
+    const double bytes = tiles * l.kv_heads * kPrefixTile * 4.0 * l.head_dim;
+    read_ = std::pow(bytes / 6.0e6 + c.fixed, 3);
+    joined_ = parts > 0 ? 4.0 + parts * l.q_heads * l.head_dim * 8.0 / 4.0e6 : 0.0;
+    const double even = sum * heads_ / c.slots;
+    many_ = (int64_t)items.size() * heads_ > 4ll * c.slots;
+    bound = total(many_ ? even + 0.5 * c.of(*first) : std::max(longest, even));
   }
-  double parts = 0;  // of the tokens in several items
-  for (int64_t t = 0, n = 0; t < l.tokens; ++t) {
-    n += cover[t];
-    if (n > 1) parts += n;
-  }
-  if ((int64_t)items.size() * l.kv_heads <= 4ll * c.slots) {
-    std::vector<double> busy(c.slots, 0.0);  // a heap, the first to be free in front
+  // of the items as the blocks are dealt out, long ones first
+  double of(const std::vector<PrefixItem>& items) const {
+    if (items.empty() || many_) return bound;
+    double end = 0;
+    std::vector<double> busy(c_.slots, 0.0);  // a heap, the first to be free in front
     for (const PrefixItem& i : items)
-      for (int h = 0; h < l.kv_heads; ++h) {
+      for (int h = 0; h < heads_; ++h) {
         std::pop_heap(busy.begin(), busy.end(), std::greater<double>());
-        busy.back() += c.of(i);
+        busy.back() += c_.of(i);
         end = std::max(end, busy.back());
         std::push_heap(busy.begin(), busy.end(), std::greater<double>());
       }
-  } else {
-    end = sum * l.kv_heads / c.slots + 0.5 * c.of(items[0]);
+    return total(end);
   }
-  const double bytes = tiles * l.kv_heads * kPrefixTile * 4.0 * l.head_dim;
-  end = std::cbrt(std::pow(end, 3) + std::pow(bytes / 6.0e6 + c.fixed, 3));
-  return end + (parts > 0 ? 4.0 + parts * l.q_heads * l.head_dim * 8.0 / 4.0e6 : 0.0);
-}
+  double bound = 0;  // what it is not below
 
-// The cut of least estimated time: candidates are numbers of key tiles a part,
-// and with them numbers of units that stay whole (what full rounds of the
-// slots take; the rest, cut, fills the last one).
+ private:
+  double total(double end) const { return std::cbrt(end * end * end + read_) + joined_; }
+  int heads_;
+  Cost c_;
+  double read_ = 0, joined_ = 0;
+  bool many_ = false;
+};
+
+// The cut of least estimated time, if that is below `least` (or that is
+// negative): candidates are numbers of key tiles a part, and with them numbers
+// of units that stay whole (what full rounds of the slots take; the rest, cut,
+// fills the last one).  They are tried by their bounds, the lowest first, until
+// no other can be better.
 template <typename Make>
-double best_cut(const Layout& l, const Cost& c, Make units_for, std::vector<PrefixItem>& best) {
-  double least = -1;
+double best_cut(const Layout& l, const Cost& c, Make units_for, double least,
+                std::vector<PrefixItem>& best) {
+  struct Candidate {
+    double bound;
+    int64_t most;
+    size_t whole;
+  };
+  std::vector<Candidate> candidates;
   int64_t longest = 1, tiles = 0;
   for (const Unit& u : units_for(1)) tiles += u.steps();
   // from what gives at most eight blocks a slot
@@ -284,13 +308,23 @@ double best_cut(const Layout& l, const Cost& c, Make units_for, std::vector<Pref
     const size_t rounds = units.size() * l.kv_heads / c.slots;
     for (size_t whole : {(size_t)0, rounds * c.slots / l.kv_heads}) {
       if (whole > 0 && most >= longest) continue;
-      std::vector<PrefixItem> items = cut(l, units, most, whole);
-      const double e = estimate(l, items, c);
-      if (least < 0 || e < least) {
-        least = e;
-        best = std::move(items);
-      }
+      const Estimate e(l, cut(l, units, most, whole), c);
+      if (least < 0 || e.bound < least) candidates.push_back({e.bound, most, whole});
       if (rounds == 0) break;
+    }
+  }
+  std::stable_sort(candidates.begin(), candidates.end(),
+                   [](const Candidate& x, const Candidate& y) { return x.bound < y.bound; });
+  for (const Candidate& x : candidates) {
+    if (least >= 0 && x.bound >= least) break;
+    std::vector<PrefixItem> items = cut(l, units_for(x.most), x.most, x.whole);
+    std::stable_sort(items.begin(), items.end(), [](const PrefixItem& a, const PrefixItem& b) {
+      return a.steps() > b.steps();
+    });
+    const double e = Estimate(l, items, c).of(items);
+    if (least < 0 || e < least) {
+      least = e;
+      best = std::move(items);
     }
   }
   return least;
@@ -350,13 +384,12 @@ int make_plan(const cs_prefix_shape* s, cs_prefix_plan_info* info, int32_t* word
     const int sms = num_sms();
     // two blocks of 128 rows an SM, which read their keys for each row tile,
     // or one of 256 rows; both costs as measured with 32/8 heads of 128
-    const double e1 = best_cut(l, Cost{2 * sms, 1.75, 5.0},
-                               [&](int64_t most) { return split_units(l, most * kPrefixTile); },
-                               items);
+    const double narrow = best_cut(
+        l, Cost{2 * sms, 1.75, 5.0},
+        [&](int64_t most) { return split_units(l, most * kPrefixTile); }, -1, items);
     std::vector<PrefixItem> wide;
-    const double e2 = best_cut(l, Cost{sms, 2.1, 6.0},
-                               [&](int64_t) { return whole_units(l, 2 * kPrefixTile); }, wide);
-    if (e2 >= 0 && (e1 < 0 || e2 < e1)) {
+    if (best_cut(l, Cost{sms, 2.1, 6.0},
+                 [&](int64_t) { return whole_units(l, 2 * kPrefixTile); }, narrow, wide) < narrow) {
       info->variant = 2;
       items = std::move(wide);
     }
