@@ -86,6 +86,7 @@ class SharedPrefixAttention:
             capacity = self.info.words
         N.check(rc, "cs_prefix_plan")
         self.words = words[:self.info.words].to(self.device)
+        self._stream = N.stream_of(self.device) if self.device.type == "cuda" else None
 
     def __call__(self, query: Tensor, kv: Tensor | NativePagedKV | N.PagedKV,
                  prefix_slots: Tensor, suffix_slots: Tensor, *, scale: float | None = None,
@@ -132,6 +133,8 @@ class SharedPrefixAttention:
             query.data_ptr(), qs[0], qs[1], view, prefix_slots.data_ptr(),
             suffix_slots.data_ptr(), self.q_heads, scale, out.data_ptr(), os[0], os[1],
             N.ptr(lse), None if status is None else status.ptr)
+        if N.stream_of(device) != self._stream:  # the plan may be dropped before the call has run
+            self.words.record_stream(torch.cuda.current_stream(device))
         workspace = None
         if self.info.workspace:
             workspace = torch.empty(self.info.workspace, dtype=torch.uint8, device=device)

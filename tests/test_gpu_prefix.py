@@ -316,6 +316,23 @@ def test_same_bits_again_and_on_another_stream(cuda, name):
     assert torch.equal(got, want) and torch.equal(again, want)
 
 
+def test_plan_dropped_before_its_call_has_run(cuda):
+    """The plan's memory is not handed out while a call on another stream
+    than the plan's own still waits for its turn."""
+    s, lens = batch(cuda, 8, 2, 128, BF, [40] * 5, [50] * 5, [300])
+    plan = plan_of(s, lens)
+    words, place = plan.words.numel(), plan.words.data_ptr()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)
+        plan(s["query"], s["cache"], s["prefix_slots"], s["suffix_slots"])
+    del plan
+    assert torch.empty(words, dtype=torch.int32, device=cuda).data_ptr() != place
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+
+
 def test_no_tokens(cuda):
     s, lens = batch(cuda, 8, 2, 128, BF, [0, 0], [5, 0], [20])
     got, lse = run(s, lens)
