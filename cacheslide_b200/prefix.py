@@ -123,7 +123,7 @@ class SharedPrefixAttention:
         elif not math.isfinite(scale):
             raise ValueError("scale must be finite")
         if out is None:
-            out = torch.empty(shape, dtype=self.dtype, device=device)
+            out = torch.empty_like(query, memory_format=torch.contiguous_format)
         elif out.shape != shape or out.dtype is not self.dtype or out.get_device() != index \
                 or out.stride(2) != 1:
             raise ValueError("out must match query, with a contiguous last dimension")

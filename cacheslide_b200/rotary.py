@@ -26,6 +26,7 @@ from . import _native as N
 from .paged import NativePagedKV
 
 MAX_HEAD_DIM = 512
+_ROWS = torch.contiguous_format  # outputs are contiguous whatever the inputs' strides
 _TYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
@@ -118,8 +119,8 @@ def _params(query: Tensor | None, key: Tensor, positions: Tensor, cos: Tensor, s
 
 
 def _forward(query, key, positions, cos, sin, q_weight, k_weight, eps, interleaved, status):
-    q_out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    k_out = torch.empty(key.shape, dtype=key.dtype, device=key.device)
+    q_out = torch.empty_like(query, memory_format=_ROWS)
+    k_out = torch.empty_like(key, memory_format=_ROWS)
     p = _params(query, key, positions, cos, sin, q_weight, k_weight, eps, interleaved, q_out,
                 k_out, status)
     N.launch("cs_qk_norm_rope", key.device, p)
@@ -215,7 +216,7 @@ def append_rotated(kv: Tensor | NativePagedKV | N.PagedKV, slots: Tensor, key: T
     if query is not None:
         query = _rows("query", query)
         if out is None:
-            out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+            out = torch.empty_like(query, memory_format=_ROWS)
         elif (out.shape != query.shape or out.dtype is not query.dtype
               or out.get_device() != device or out.stride(2) != 1):
             raise ValueError("out must match query, with a contiguous last dimension")
