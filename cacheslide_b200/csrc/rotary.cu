@@ -323,6 +323,45 @@ __device__ __forceinline__ typename Vec4<T>::type pack(const float* f) {
     return make_uint2(Pack2<T>::pack(f[0], f[1]), Pack2<T>::pack(f[2], f[3]));
 }
 
+// A lane's P pairs, two at a time for the packed float32 instructions: a[i]
+// holds the first elements of pairs 2i and 2i + 1, b[i] the second.
+template <int P>
+struct Pairs {
+  float2 a[P / 2], b[P / 2];
+};
+
+// two vectors' elements <-> pairs
+template <int P, bool INTER>
+__device__ __forceinline__ void to_pairs(const float* u, const float* v, Pairs<P>& p) {
+#pragma unroll
+  for (int i = 0; i < P / 2; ++i) {
+    if constexpr (INTER) {
+      const float* x = i < P / 4 ? u + 4 * i : v + 4 * i - P;
+      p.a[i] = make_float2(x[0], x[2]);
+      p.b[i] = make_float2(x[1], x[3]);
+    } else {
+      p.a[i] = make_float2(u[2 * i], u[2 * i + 1]);
+      p.b[i] = make_float2(v[2 * i], v[2 * i + 1]);
+    }
+  }
+}
+template <int P, bool INTER>
+__device__ __forceinline__ void from_pairs(const Pairs<P>& p, float* u, float* v) {
+#pragma unroll
+  for (int i = 0; i < P / 2; ++i) {
+    if constexpr (INTER) {
+      float* x = i < P / 4 ? u + 4 * i : v + 4 * i - P;
+      x[0] = p.a[i].x, x[2] = p.a[i].y;
+      x[1] = p.b[i].x, x[3] = p.b[i].y;
+    } else {
+      u[2 * i] = p.a[i].x, u[2 * i + 1] = p.a[i].y;
+      v[2 * i] = p.b[i].x, v[2 * i + 1] = p.b[i].y;
+    }
+  }
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 neg(float2 x) { return make_float2(-x.x, -x.y); }
+
 // 4 weights from element e of a head on, as float32
 __device__ __forceinline__ void weights_at(const void* w, int dtype, int e, float* f) {
   if (dtype == CS_F32) {
@@ -365,19 +404,6 @@ __device__ __forceinline__ void angles(const RotArgs& a, int64_t pos, int p0, fl
   } else {
 #pragma unroll
     for (int i = 0; i < kP; ++i) c[i] = s[i] = __int_as_float(0x7fc00000);
-  }
-}
-
-// (x0, x1): a lane's two vectors, turned by the angle of (c, s)
-template <bool INTER>
-__device__ __forceinline__ void turn(float* x0, float* x1, const float* c, const float* s) {
-#pragma unroll
-  for (int i = 0; i < kP; ++i) {
-    float& u = INTER ? (i < 2 ? x0[2 * i] : x1[2 * i - 4]) : x0[i];
-    float& v = INTER ? (i < 2 ? x0[2 * i + 1] : x1[2 * i - 3]) : x1[i];
-    const float a = u, b = v;
-    u = turned0(a, b, c[i], s[i]);
-    v = turned1(a, b, c[i], s[i]);
   }
 }
 
@@ -459,29 +485,45 @@ __global__ void __launch_bounds__(kVecWarps * 32)
     }
   }
   if (!APPEND || kind < 2) {
-    float c[kP], s[kP], w0[kP], w1[kP];
+    float c[kP], s[kP];
     if (ln.turns) angles(a, pos, ln.p0, c, s);
+    Pairs<kP> w;
     if (rw.w) {
+      float w0[kP], w1[kP];
       weights_at(rw.w, a.wdtype, ln.e0, w0);
       weights_at(rw.w, a.wdtype, ln.e1, w1);
+      to_pairs<kP, INTER>(w0, w1, w);
     }
 #pragma unroll
     for (int u = 0; u < kGroups; ++u) {
       float f0[kP], f1[kP];
       unpack<T>(x0[u], f0);
       unpack<T>(x1[u], f1);
+      Pairs<kP> n;
+      to_pairs<kP, INTER>(f0, f1, n);
       if (rw.w) {
-        float ss = 0.f;
+        float2 ss = both(0.f);
 #pragma unroll
-        for (int i = 0; i < kP; ++i) ss += f0[i] * f0[i] + f1[i] * f1[i];
-        const float r = rsqrtf(row_sum<LPR>(ss) * a.inv_dim + a.eps);
+        for (int i = 0; i < kP / 2; ++i)
+          ss = __ffma2_rn(n.a[i], n.a[i], __ffma2_rn(n.b[i], n.b[i], ss));
+        const float2 r = both(rsqrtf(row_sum<LPR>(ss.x + ss.y) * a.inv_dim + a.eps));
 #pragma unroll
-        for (int i = 0; i < kP; ++i) {
-          f0[i] *= r * w0[i];
-          f1[i] *= r * w1[i];
+        for (int i = 0; i < kP / 2; ++i) {
+          n.a[i] = __fmul2_rn(n.a[i], __fmul2_rn(r, w.a[i]));
+          n.b[i] = __fmul2_rn(n.b[i], __fmul2_rn(r, w.b[i]));
         }
       }
-      if (ln.turns) turn<INTER>(f0, f1, c, s);
+      if (ln.turns) {
+#pragma unroll
+        for (int i = 0; i < kP / 2; ++i) {
+          const float2 ci = make_float2(c[2 * i], c[2 * i + 1]);
+          const float2 si = make_float2(s[2 * i], s[2 * i + 1]);
+          const float2 t = __ffma2_rn(n.a[i], ci, neg(__fmul2_rn(n.b[i], si)));
+          n.b[i] = __ffma2_rn(n.b[i], ci, __fmul2_rn(n.a[i], si));
+          n.a[i] = t;
+        }
+      }
+      from_pairs<kP, INTER>(n, f0, f1);
       x0[u] = pack<T>(f0);
       x1[u] = pack<T>(f1);
     }
@@ -502,13 +544,6 @@ __global__ void __launch_bounds__(kVecWarps * 32)
 // cp.async, every lane its own vectors (so no barrier): bytes in flight cost
 // no registers, and a lane's longer share halves the instructions a row.
 template <typename T> constexpr int kPairs = 16 / (int)sizeof(T);
-
-// A lane's P pairs, two at a time for the packed float32 instructions: a[i]
-// holds the first elements of pairs 2i and 2i + 1, b[i] the second.
-template <int P>
-struct Pairs {
-  float2 a[P / 2], b[P / 2];
-};
 
 template <typename T, int P>
 __device__ __forceinline__ void unpack16(const uint4& v, float* f) {
@@ -535,35 +570,6 @@ __device__ __forceinline__ uint4 pack16(const float* f) {
     else w[i] = Pack2<T>::pack(f[2 * i], f[2 * i + 1]);
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
-}
-// two vectors' elements <-> pairs
-template <int P, bool INTER>
-__device__ __forceinline__ void to_pairs(const float* u, const float* v, Pairs<P>& p) {
-#pragma unroll
-  for (int i = 0; i < P / 2; ++i) {
-    if constexpr (INTER) {
-      const float* x = i < P / 4 ? u + 4 * i : v + 4 * i - P;
-      p.a[i] = make_float2(x[0], x[2]);
-      p.b[i] = make_float2(x[1], x[3]);
-    } else {
-      p.a[i] = make_float2(u[2 * i], u[2 * i + 1]);
-      p.b[i] = make_float2(v[2 * i], v[2 * i + 1]);
-    }
-  }
-}
-template <int P, bool INTER>
-__device__ __forceinline__ void from_pairs(const Pairs<P>& p, float* u, float* v) {
-#pragma unroll
-  for (int i = 0; i < P / 2; ++i) {
-    if constexpr (INTER) {
-      float* x = i < P / 4 ? u + 4 * i : v + 4 * i - P;
-      x[0] = p.a[i].x, x[2] = p.a[i].y;
-      x[1] = p.b[i].x, x[3] = p.b[i].y;
-    } else {
-      u[2 * i] = p.a[i].x, u[2 * i + 1] = p.a[i].y;
-      v[2 * i] = p.b[i].x, v[2 * i + 1] = p.b[i].y;
-    }
-  }
 }
 template <typename T, int P, bool INTER>
 __device__ __forceinline__ void load_pairs(const uint4& x, const uint4& y, Pairs<P>& p) {
@@ -607,8 +613,6 @@ __device__ __forceinline__ Lane16 lane_of16(const RotArgs& a, int l) {
   n.tb = n.pb < half;
   return n;
 }
-__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
-__device__ __forceinline__ float2 neg(float2 x) { return make_float2(-x.x, -x.y); }
 
 // P floats of shared memory, 16-byte aligned
 template <int P>
