@@ -288,14 +288,17 @@ __global__ void __launch_bounds__(kRowWarps * 32)
 // kernels held 98 (forward) and 118 (gradient) registers, a quarter of the
 // SM's warps, and 2.9 TB/s.
 //
-// Forward, 32768 tokens of 32/8 heads of 128, bf16: 123 us, 5.5 TB/s, held
-// back by the instructions of the norm (two thirds of the issue slots);
-// append of 65536 tokens of 64/8 heads without norms, fp16: 404 us, 6.7 TB/s,
-// HBM.  Two groups a task: 143 and 497 us; eight: 137 and 422 us; 1, 2 or 8
-// warps a block: 129, 123, 129 us.
+// Forward, 32768 tokens of 32/8 heads of 128, bf16: 115 us, 5.8 TB/s (113 with
+// the row sums' shuffles left out: the rest is HBM and the warps' starts);
+// append of 65536 tokens of 64/8 heads without norms, fp16: 401 us, 6.8 TB/s,
+// HBM.  Two groups a task: 143 and 497 us; eight: 144 and 412 us; two warps a
+// block: 117 and 400 us; eight: 122 and 434 us.  Registers for nine blocks an SM
+// are 3 us better than the 60 that the compiler takes, for ten 15 us worse;
+// in float32 (103 us for 16384 tokens) nine are 2 us worse.
 constexpr int kP = 4;        // pairs a lane
 constexpr int kGroups = 4;   // row groups a task
 constexpr int kVecWarps = 4;
+template <typename T> constexpr int kVecBlocks = sizeof(T) == 2 ? 9 : 1;
 
 template <typename T> struct Vec4 { using type = uint2; };
 template <> struct Vec4<float> { using type = uint4; };
@@ -429,7 +432,7 @@ __host__ __device__ inline int tasks_of(int heads, int lanes) {
 
 // Forward and append: tasks of q, then k, then (append) v of each token.
 template <typename T, int LPR, bool INTER, bool APPEND>
-__global__ void __launch_bounds__(kVecWarps * 32)
+__global__ void __launch_bounds__(kVecWarps * 32, kVecBlocks<T>)
     norm_rope_vec_kernel(const __grid_constant__ RotArgs a, const __grid_constant__ AppendArgs ap,
                          unsigned tasks) {
   using V = typename Vec4<T>::type;
