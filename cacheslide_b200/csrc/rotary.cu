@@ -25,6 +25,11 @@ namespace {
 constexpr int kMaxDim = 512;
 constexpr int kMaxPairs = kMaxDim / 2 / 32;  // pairs a lane of a warp-per-row kernel
 constexpr int kStreamBlocks = 296;           // 148 SMs x 2: the fixed partition of the gradient
+// A token's angles, in row groups of the streamed gradient.  With none, the
+// blocks of the kind with fewer heads ended last; 32/8 heads of 128, 64/4 of
+// 128, 32/8 of 64 took 178, 367, 214 us at 0; 165, 283, 184 at 0.5; 162, 270,
+// 172 at 1; 168, 273, 178 at 1.5.
+constexpr double kAngleCost = 1.0;
 constexpr int kRowWarps = 8;
 
 struct Rows {
@@ -657,10 +662,10 @@ struct Place {
 // grad_weight_kernel) blocks are added in order.  Angles come with the rows
 // of a token's first group, weights lie in shared memory.
 //
-// 32768 tokens of 32/8 heads of 128, bf16: 176 us, 5.7 TB/s (interleaved pairs
-// 180 us).  Tried: plain loads of 4 pairs a lane, two row groups in flight,
-// three blocks an SM (286 us); this ring with 80 registers and three blocks
-// (325 us: spills); rings of 4 and 6 groups (185 and 255 us).
+// 32768 tokens of 32/8 heads of 128, bf16: 162 us, 6.2 TB/s (interleaved pairs
+// as fast); float32, half the tokens: 177 us.  Tried: plain loads of 4 pairs a
+// lane, two row groups in flight, three blocks an SM (286 us); this ring with
+// 80 registers and three blocks (325 us: spills); a ring of 4 groups (166 us).
 constexpr int kStreamWarps = 8;
 constexpr int kRing = 3;  // row groups a warp has in flight, one being read
 
@@ -984,26 +989,27 @@ void by_lanes(int lanes, F f) {
   }
 }
 
-// The streamed kernel's blocks: in proportion to the kinds' heads, no more
-// than the rows fill; where the tokens alone do not fill them, a token's row
-// groups go to several warps.
+// The streamed kernel's blocks: in proportion to the kinds' row groups a token,
+// with what a token's angles cost, no more than the rows fill; where the
+// tokens alone do not fill them, a token's row groups go to several warps.
 struct Shares {
   int nq, n, parts;
 };
 Shares shares(const RotArgs& a, int lanes) {
-  const int hq = a.q.heads, hk = a.k.heads, heads = hq + hk;
-  const int groups = std::max(1, (std::max(hq, hk) * lanes + 31) / 32);
+  auto groups = [&](int h) { return (h * lanes + 31) / 32; };
+  const int gq = groups(a.q.heads), gk = groups(a.k.heads);
   const int64_t fill = (int64_t)kStreamBlocks * kStreamWarps;
   Shares s;
-  s.parts = (int)std::max<int64_t>(1, std::min<int64_t>(groups, fill / a.tokens));
+  s.parts = (int)std::max<int64_t>(1, std::min<int64_t>(std::max(gq, gk), fill / a.tokens));
   const int64_t want = (a.tokens * s.parts + kStreamWarps - 1) / kStreamWarps;
-  auto blocks = [&](int h) {
-    if (h == 0) return 0;
-    const int64_t most = std::max<int64_t>(1, (int64_t)kStreamBlocks * h / heads);
-    return (int)std::min(most, want);
+  auto cost = [&](int g) { return g + kAngleCost * std::min(g, s.parts); };
+  auto blocks = [&](int g) {
+    if (g == 0) return 0;
+    const double share = kStreamBlocks * cost(g) / (cost(gq) + cost(gk));
+    return (int)std::min<int64_t>(std::max<int64_t>(1, (int64_t)share), want);
   };
-  s.nq = blocks(hq);
-  s.n = s.nq + blocks(hk);
+  s.nq = blocks(gq);
+  s.n = s.nq + blocks(gk);
   return s;
 }
 
