@@ -71,14 +71,11 @@ __device__ __forceinline__ void pair_elems(const RotArgs& a, int p, int& i, int&
   }
 }
 
+// of a pair that turns (p < rot / 2)
 __device__ __forceinline__ void angle(const RotArgs& a, int64_t pos, int p, float& c, float& s) {
-  c = 1.f;
-  s = 0.f;
-  if (p < (a.rot >> 1)) {
-    const bool ok = pos >= 0 && pos < a.table_rows;
-    c = ok ? a.cos[pos * a.table_stride + p] : __int_as_float(0x7fc00000);
-    s = ok ? a.sin[pos * a.table_stride + p] : __int_as_float(0x7fc00000);
-  }
+  const bool ok = pos >= 0 && pos < a.table_rows;
+  c = ok ? a.cos[pos * a.table_stride + p] : __int_as_float(0x7fc00000);
+  s = ok ? a.sin[pos * a.table_stride + p] : __int_as_float(0x7fc00000);
 }
 
 // one pair turned; the products' order is fixed, so that every kernel here
@@ -116,16 +113,22 @@ __device__ __forceinline__ void norm_turn_row(const RotArgs& a, const T* x, At a
     const int p = lane + 32 * m;
     if (p < pairs) {
       int i, j;
-      float c, s;
       pair_elems(a, p, i, j);
-      angle(a, pos, p, c, s);
       float p0 = u[m], p1 = v[m];
       if (w) {
         p0 *= r * load_weight(w, a.wdtype, i);
         p1 *= r * load_weight(w, a.wdtype, j);
       }
-      *at(i) = Elem<T>::from_f(turned0(p0, p1, c, s));
-      *at(j) = Elem<T>::from_f(turned1(p0, p1, c, s));
+      // elements past rot are not turned by a zero angle: 0 x inf is NaN
+      if (p < (a.rot >> 1)) {
+        float c, s;
+        angle(a, pos, p, c, s);
+        const float t = turned0(p0, p1, c, s);
+        p1 = turned1(p0, p1, c, s);
+        p0 = t;
+      }
+      *at(i) = Elem<T>::from_f(p0);
+      *at(j) = Elem<T>::from_f(p1);
     }
   }
 }
@@ -226,12 +229,16 @@ __global__ void __launch_bounds__(kRowWarps * 32)
       n0[m] = n1[m] = g0[m] = g1[m] = 0.f;
       if (p < pairs) {
         int i, j;
-        float c, s;
         pair_elems(a, p, i, j);
-        angle(a, pos, p, c, s);
-        const float y0 = Elem<T>::to_f(dy[i]), y1 = Elem<T>::to_f(dy[j]);
-        g0[m] = turned0(y0, y1, c, -s);
-        g1[m] = turned1(y0, y1, c, -s);
+        g0[m] = Elem<T>::to_f(dy[i]);
+        g1[m] = Elem<T>::to_f(dy[j]);
+        if (p < (a.rot >> 1)) {
+          float c, s;
+          angle(a, pos, p, c, s);
+          const float t = turned0(g0[m], g1[m], c, -s);
+          g1[m] = turned1(g0[m], g1[m], c, -s);
+          g0[m] = t;
+        }
         if (rw.w) {
           n0[m] = Elem<T>::to_f(x[i]);
           n1[m] = Elem<T>::to_f(x[j]);
