@@ -100,7 +100,8 @@ class SharedPrefixAttention:
         -inf for a row that sees no key, whose output is zero).
 
         A slot outside the pool reads as a zero key and value and sets
-        ``ST_SLOT_RANGE`` in ``status``."""
+        ``ST_SLOT_RANGE`` in ``status``.  A serving operator: it has no
+        derivative of either mode, and its outputs are constants to autograd."""
         shape, device = self.shape, self.device
         index = device.index
         if query.shape != shape or query.dtype is not self.dtype or query.get_device() != index:

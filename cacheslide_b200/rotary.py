@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _native as N
 from .paged import NativePagedKV
@@ -165,10 +166,16 @@ def qk_norm_rope(query: Tensor, key: Tensor, positions: Tensor, cos: Tensor, sin
     ``cos`` / ``sin`` come from ``rotary_tables``; twice their width is the
     rotated part of the head, the rest passes through.  ``interleaved`` pairs
     elements (2i, 2i + 1) instead of (i, i + rotary_dim / 2).  Gradients flow
-    to query, key and the weights.  A position outside the tables makes its
-    rows NaN and sets ``ST_POS_RANGE`` in ``status`` (read it after the
-    stream has drained)."""
+    to query, key and the weights (cos and sin are constants); there is no
+    forward-mode derivative, and a tensor that carries a tangent is refused.
+    A position outside the tables makes its rows NaN and sets ``ST_POS_RANGE``
+    in ``status`` (read it after the stream has drained)."""
     query, key = _rows("query", query), _rows("key", key)
+    # (a level of dual numbers is rarely open, and this test of it is free)
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None
+            for t in (query, key, cos, sin, q_weight, k_weight)):
+        raise ValueError("qk_norm_rope has no forward-mode derivative")
     if torch.is_grad_enabled() and any(
             t is not None and t.requires_grad for t in (query, key, q_weight, k_weight)):
         return _NormRope.apply(query, key, positions, cos, sin, q_weight, k_weight, eps,
@@ -203,7 +210,8 @@ def append_rotated(kv: Tensor | NativePagedKV | N.PagedKV, slots: Tensor, key: T
     position outside the tables, is skipped and sets ``ST_SLOT_RANGE`` /
     ``ST_POS_RANGE`` in ``status``.  Distinct tokens need distinct slots.  The
     slot map's guards are the caller's: this writes where it is told, as a
-    model runner's cache write does."""
+    model runner's cache write does.  A serving operator: it has no derivative
+    of either mode, and what it returns is a constant to autograd."""
     key, value = _rows("key", key), _rows("value", value)
     device = key.get_device()
     if value.shape != key.shape or value.dtype is not key.dtype or value.get_device() != device:
