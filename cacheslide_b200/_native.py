@@ -46,6 +46,7 @@ _f64 = ctypes.c_double
 
 
 class PagedKV(ctypes.Structure):
+    device = None  # index of the cache's device, where paged_view made the view
     _fields_ = [
         ("cache", _p),
         ("num_blocks", _i64), ("kv_heads", _i64), ("block_size", _i64), ("head_dim", _i64),
@@ -339,6 +340,21 @@ class Status:
         return int(self.word.item())
 
 
+def status_ptr(status: Status | None, device: int) -> int | None:
+    """The status word's address for a launch on the device of that index."""
+    if status is None:
+        return None
+    if status.word.get_device() != device:
+        raise ValueError("the status must be on the same CUDA device as the tensors")
+    return status.ptr
+
+
+def require_pool_on(kv: PagedKV, device: int) -> None:
+    """Raise if the pool behind a view is known to lie on another device."""
+    if kv.device is not None and kv.device != device:
+        raise ValueError("the pool must be on the same CUDA device as the tensors")
+
+
 def paged_view(
     cache: torch.Tensor,
     side_k: torch.Tensor | None = None,
@@ -352,6 +368,7 @@ def paged_view(
     blocks, heads, block_size, width = cache.shape
     kv = PagedKV(cache.data_ptr(), blocks, heads, block_size, width // 2, *cache.stride(),
                  None, None, 0, 0, 0, 0, DTYPES[cache.dtype])
+    kv.device = cache.get_device()
     if side_k is not None and side_v is not None:
         if side_k.stride() != side_v.stride() or side_k.shape != side_v.shape:
             raise ValueError("sidecar K and V must share shape and strides")

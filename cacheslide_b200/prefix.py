@@ -116,6 +116,8 @@ class SharedPrefixAttention:
             query = query.contiguous()
             qs = query.stride()
         view = pool_view(kv)
+        N.require_pool_on(view, index)
+        status_ptr = N.status_ptr(status, index)
         if view.dtype != N.DTYPES[self.dtype] or view.kv_heads != self.kv_heads \
                 or view.head_dim != self.head_dim:
             raise ValueError("the pool's dtype, KV heads and head dim must be the plan's")
@@ -133,7 +135,7 @@ class SharedPrefixAttention:
         p = N.PrefixParams(
             query.data_ptr(), qs[0], qs[1], view, prefix_slots.data_ptr(),
             suffix_slots.data_ptr(), self.q_heads, scale, out.data_ptr(), os[0], os[1],
-            N.ptr(lse), None if status is None else status.ptr)
+            N.ptr(lse), status_ptr)
         if N.stream_of(device) != self._stream:  # the plan may be dropped before the call has run
             self.words.record_stream(torch.cuda.current_stream(device))
         workspace = None

@@ -103,6 +103,7 @@ def _params(query: Tensor | None, key: Tensor, positions: Tensor, cos: Tensor, s
             raise ValueError("all tensors must be on the same CUDA device")
         st = query.stride()
         q = (query.data_ptr(), st[0], st[1], q_heads)
+    status_ptr = N.status_ptr(status, device)
     if device < 0:
         N.require_cuda(key)
     qo = ko = (None, 0, 0)
@@ -116,7 +117,7 @@ def _params(query: Tensor | None, key: Tensor, positions: Tensor, cos: Tensor, s
     return N.RotaryParams(
         cos.data_ptr(), sin.data_ptr(), rows, strides[0], positions.data_ptr(), tokens, dim,
         2 * half, 1 if interleaved else 0, N.DTYPES[dtype], weight_dtype, eps, *q, qw, *qo,
-        key.data_ptr(), st[0], st[1], k_heads, kw, *ko, None if status is None else status.ptr)
+        key.data_ptr(), st[0], st[1], k_heads, kw, *ko, status_ptr)
 
 
 def _forward(query, key, positions, cos, sin, q_weight, k_weight, eps, interleaved, status):
@@ -221,6 +222,7 @@ def append_rotated(kv: Tensor | NativePagedKV | N.PagedKV, slots: Tensor, key: T
             or slots.get_device() != device or tokens > 1 and slots.stride(0) != 1):
         raise ValueError("slots must be a contiguous int64 [token] vector")
     view = pool_view(kv)
+    N.require_pool_on(view, device)
     if query is not None:
         query = _rows("query", query)
         if out is None:
