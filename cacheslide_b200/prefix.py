@@ -45,7 +45,9 @@ class SharedPrefixAttention:
     request may have fewer own keys than queries (the first queries then see
     only the prefix).  The requests form consecutive groups of
     ``group_sizes``, group ``g`` sharing ``prefix_lens[g]`` keys; by default
-    one group holds them all."""
+    one group holds them all.  The lengths stay on the plan under these names:
+    a call compares only their sums with its tensors, so a caller that keeps
+    plans compares the lengths."""
 
     def __init__(self, q_heads: int, kv_heads: int, head_dim: int, dtype: torch.dtype,
                  device: torch.device | str, *, query_lens: Sequence[int],
@@ -65,6 +67,8 @@ class SharedPrefixAttention:
         sizes, members = _lens("group_sizes", group_sizes)
         if members != len(query_lens):
             raise ValueError("group_sizes must add up to the requests")
+        self.query_lens, self.suffix_lens = tuple(query_lens), tuple(suffix_lens)
+        self.prefix_lens, self.group_sizes = tuple(prefix_lens), tuple(group_sizes)
         self.q_heads, self.kv_heads, self.head_dim = q_heads, kv_heads, head_dim
         self.shape = torch.Size((self.tokens, q_heads, head_dim))
         self.dtype, self.device = dtype, torch.device(device)

@@ -13,7 +13,7 @@ three calls run as a model runner would make them:
   (``append_rotated`` and ``prefix.SharedPrefixAttention``).
 
 A step's plan depends on the lengths alone: build it once (``plan``) and pass
-it to every layer.  The prefill of the document itself is ordinary causal
+it to every layer; a plan of other lengths is refused.  The prefill of the document itself is ordinary causal
 attention over ``rotary.qk_norm_rope``'s output.
 """
 
@@ -78,11 +78,16 @@ class RotaryRagBatch:
         self._append(self.prefix_slots, key, value,
                      torch.arange(key.shape[0], device=self.pool.device))
 
-    def plan(self, query_lens: Sequence[int]) -> SharedPrefixAttention:
-        """The attention of a step in which request b brings query_lens[b] tokens."""
+    def _own(self, query_lens: Sequence[int]) -> list[int]:
+        """Each request's own keys after a step."""
         own = [have + new for have, new in zip(self.lengths, query_lens, strict=True)]
         if max(own) > self.max_own:
             raise ValueError("a request's own keys pass its blocks")
+        return own
+
+    def plan(self, query_lens: Sequence[int]) -> SharedPrefixAttention:
+        """The attention of a step in which request b brings query_lens[b] tokens."""
+        own = self._own(query_lens)
         return SharedPrefixAttention(
             self.q_heads, self.pool.shape[1], self.pool.shape[3] // 2, self.pool.dtype,
             self.pool.device, query_lens=query_lens, suffix_lens=own,
@@ -92,8 +97,20 @@ class RotaryRagBatch:
              plan: SharedPrefixAttention | None = None) -> Tensor:
         """One layer of a step: ``query`` [token, q_head, dim] and ``key`` /
         ``value`` [token, kv_head, dim] of the new tokens, requests in order.
-        Returns the attention's output [token, q_head, dim]."""
-        plan = self.plan(query_lens) if plan is None else plan
+        Returns the attention's output [token, q_head, dim].  Everything that
+        the attention would refuse is refused before the keys are written."""
+        if plan is None:
+            plan = self.plan(query_lens)
+        else:
+            pool = self.pool
+            mine = (tuple(query_lens), tuple(self._own(query_lens)),
+                    (self.prefix_slots.numel(),), (self.requests,), self.q_heads, pool.shape[1],
+                    pool.shape[3] // 2, pool.dtype, pool.device)
+            if mine != (plan.query_lens, plan.suffix_lens, plan.prefix_lens, plan.group_sizes,
+                        plan.q_heads, plan.kv_heads, plan.head_dim, plan.dtype, plan.device):
+                raise ValueError("the plan is of other lengths, heads or pool than this step")
+        if query.shape != plan.shape or query.dtype is not plan.dtype:
+            raise ValueError(f"query must be {plan.dtype} {tuple(plan.shape)}")
         first = self.prefix_slots.numel()
         device = self.pool.device
         spans = [(b, have, have + new)

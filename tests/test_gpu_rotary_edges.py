@@ -1,6 +1,6 @@
 """Rotary operators where they are easily wrong: infinities in the part of a
 head that is not rotated, in the kernels for heads and strides that vectors do
-not fit.
+not fit; plans of other lengths.
 
 Elements past ``rotary_dim`` pass through (times the norm's factor and weight):
 one of them that is infinite touches no other element of its row, except
@@ -12,6 +12,7 @@ import pytest
 import torch
 
 from cacheslide_b200 import rotary
+from cacheslide_b200.rotary_rag import RotaryRagBatch
 
 pytestmark = pytest.mark.gpu
 
@@ -106,3 +107,19 @@ def test_append_of_an_infinity_past_the_rotated_part(cuda, tokens, dim, rot, int
         k[n + 1, 1, e] = want[slot // 16, 1, slot % 16, e] = -INF
     got_q = rotary.append_rotated(cache, slots, k, v, query=q, **args)
     assert torch.equal(got_q, want_q) and torch.equal(cache, want)
+
+
+def test_a_batch_refuses_a_plan_of_other_lengths_and_writes_nothing(cuda):
+    rand = lambda *s: torch.randn(*s, device=cuda).to(BF)  # noqa: E731
+    pool = torch.zeros(30, 2, 16, 256, dtype=BF, device=cuda)
+    batch = RotaryRagBatch(pool, 8, 200, 2, 64)
+    batch.write_prefix(rand(200, 2, 128), rand(200, 2, 128))
+    args = rand(4, 8, 128), rand(4, 2, 128), rand(4, 2, 128)
+    before, other = pool.clone(), batch.plan([1, 3])  # the same sums
+    with pytest.raises(ValueError, match="plan"):
+        batch.step(*args, [3, 1], other)
+    assert torch.equal(pool, before) and batch.lengths == [0, 0]
+    got = batch.step(*args, [3, 1], batch.plan([3, 1]))
+    batch.lengths = [0, 0]
+    assert torch.equal(batch.step(*args, [3, 1]), got)
+    batch.check()
