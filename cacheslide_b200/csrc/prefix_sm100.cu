@@ -188,10 +188,12 @@ struct Src {
 };
 
 // One row of an item by one warp, over the keys that it sees (the CUDA-core
-// form of prefix.cu): the way out for rows whose sums are not finite.
-template <typename T, int D>
+// form of prefix.cu): the way out for rows whose sums are not finite.  Of TPR
+// threads a row, each warp writes the columns that are its own: the warp of
+// the others may be storing them meanwhile.
+template <typename T, int D, int TPR>
 __device__ __noinline__ void row_again(const PArgs& a, const PrefixItem& it, int g, int tok, int h,
-                                       int lane, void* out, bool part) {
+                                       int lane, int part2, void* out, bool part) {
   constexpr int E = D / 32;
   const int4 tk = a.tokens[it.tok0 + tok];
   const T* q = reinterpret_cast<const T*>(a.q + (int64_t)(it.tok0 + tok) * a.qt + (int64_t)h * a.qh);
@@ -224,6 +226,7 @@ __device__ __noinline__ void row_again(const PArgs& a, const PrefixItem& it, int
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = acc[e] * keep + p * v[e];
   }
+  if (lane / (32 / TPR) != part2) return;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const float x = sum == 0.f ? 0.f : acc[e] / sum;
@@ -687,8 +690,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     if (part) orow = reinterpret_cast<char*>(a.part_o + prow * D);
     const bool have = ok && steps > 0 && lsum != 0.f;
     // An infinite or NaN value of a key that this row does not see reaches its
-    // sums as 0 x inf = NaN, so a row that is not finite is computed again
-    // below, from the keys it sees alone.
+    // sums as 0 x inf = NaN, so a row (a thread's columns of it) that is not
+    // finite is computed again below, from the keys it sees alone.
     float worst = 0.f;
     auto finite = [&](uint32_t x) { worst = max_nan(worst, fabsf(__uint_as_float(x))); };
     if (part || a.vec_out) {
@@ -780,9 +783,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       const int src = __ffs(again) - 1;
       const int rr = r - lane + src;
       const int tt = qt * a.R + rr / a.G, hh = g * a.G + rr % a.G;
-      row_again<T, D>(a, it, g, tt, hh, lane,
-                      reinterpret_cast<void*>(__shfl_sync(~0u, reinterpret_cast<uint64_t>(orow), src)),
-                      part);
+      row_again<T, D, TPR>(
+          a, it, g, tt, hh, lane, part2,
+          reinterpret_cast<void*>(__shfl_sync(~0u, reinterpret_cast<uint64_t>(orow), src)), part);
     }
     if (row_ok && ok && part2 == 0) {
       if (it.part >= 0) a.part_lse[prow] = lse2;
