@@ -45,6 +45,7 @@ namespace {
 constexpr int kKeys = 64;  // keys of a step: one K and V tile, scores, softmax, P V
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kKinds = 3;  // of values that are not finite: NaN, +inf, -inf
 
 struct PArgs {
   CUtensorMap tm;  // the pool's rows in boxes of 64 x 16
@@ -68,7 +69,6 @@ struct PArgs {
   int vec_q, vec_out; // 16-byte loads / stores fit
   int neg;            // the scale is negative: the queries are negated
   float scale2;       // |scale| * log2 e
-  float scale;
 };
 
 template <typename T> constexpr int umma_format() { return std::is_same<T, __half>::value ? 0 : 1; }
@@ -105,10 +105,12 @@ struct Shape {
                             bVr = bKr + 8 * KS, bS = bVr + 8 * VS, bP = bS + 16 * NT,
                             bPV = bP + 16 * NT, bMax = bPV + 16 * NT, oTmem = bMax + 32 * NT,
                             oAbort = oTmem + 4,
-                            oRows = (oAbort + 4 + 15) / 16 * 16,
-                            oMax = oRows + 2 * kKeys * 8,
-                            kMeta = oMax + NT * 2 * 2 * 128 * 4;
-  static_assert(oMeta % 1024 == 0 && oRows % 16 == 0 && oTmem % 4 == 0,
+                            oAgain = oAbort + 4, bClean = oAgain + 8, oFound = bClean + 8,
+                            oRows = (oFound + 8 + 15) / 16 * 16,
+                            oMax = oRows + 2 * kKeys * 8, oBad = oMax + NT * 2 * 2 * 128 * 4,
+                            kMeta = oBad + 2 * kKinds * kKeys * (D / 8);
+  static_assert(oMeta % 1024 == 0 && oRows % 16 == 0 && oTmem % 4 == 0 && bClean % 8 == 0 &&
+                    oBad % 16 == 0,
                 "alignment of the shared-memory places");
   static constexpr uint32_t kSmem = oMeta + kMeta + 1024;  // the base is rounded up to 1024
   static constexpr uint32_t kCols = 256 * NT;
@@ -187,52 +189,21 @@ struct Src {
   bool run;        // the two lie in consecutive rows of the pool's map
 };
 
-// One row of an item by one warp, over the keys that it sees (the CUDA-core
-// form of prefix.cu): the way out for rows whose sums are not finite.  Of TPR
-// threads a row, each warp writes the columns that are its own: the warp of
-// the others may be storing them meanwhile.
-template <typename T, int D, int TPR>
-__device__ __noinline__ void row_again(const PArgs& a, const PrefixItem& it, int g, int tok, int h,
-                                       int lane, int part2, void* out, bool part) {
-  constexpr int E = D / 32;
-  const int4 tk = a.tokens[it.tok0 + tok];
-  const T* q = reinterpret_cast<const T*>(a.q + (int64_t)(it.tok0 + tok) * a.qt + (int64_t)h * a.qh);
-  float qr[E], acc[E], mx = -INFINITY, sum = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    qr[e] = Elem<T>::to_f(q[lane * E + e]) * a.scale;
-    acc[e] = 0.f;
-  }
-  const int lo = tk.z > it.b0 ? tk.z : it.b0, hi = tk.w < it.b1 ? tk.w : it.b1;
-  const int np = it.a1 - it.a0, n = np + (hi > lo ? hi - lo : 0);
-  for (int j = 0; j < n; ++j) {
-    const int64_t s = j < np ? a.prefix_slots[it.a0 + j] : a.suffix_slots[lo + (j - np)];
-    const bool have = a.pv.valid(s);
-    float dot = 0.f, v[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      v[e] = 0.f;
-      if (have) {
-        dot += qr[e] * Elem<T>::to_f(*reinterpret_cast<const T*>(a.pv.addr(s, g, lane * E + e)));
-        v[e] = Elem<T>::to_f(*reinterpret_cast<const T*>(a.pv.addr(s, g, D + lane * E + e)));
-      }
-    }
-    dot = warp_sum(dot);
-    if (dot == -INFINITY) continue;
-    const float top = fmaxf(mx, dot);
-    const float keep = mx == -INFINITY ? 0.f : expf(mx - top), p = expf(dot - top);
-    mx = top;
-    sum = sum * keep + p;
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = acc[e] * keep + p * v[e];
-  }
-  if (lane / (32 / TPR) != part2) return;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const float x = sum == 0.f ? 0.f : acc[e] / sum;
-    if (part) static_cast<float*>(out)[lane * E + e] = x;
-    else static_cast<T*>(out)[lane * E + e] = Elem<T>::from_f(x);
-  }
+// bits of the elements of a 16-bit pair that are not finite (0, 1), and the pair
+// without them
+template <typename T>
+__device__ __forceinline__ uint32_t take_out(uint32_t& x) {
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  const bool lo = (x & e) == e, hi = (x & (e << 16)) == (e << 16);
+  if (lo) x &= 0xffff0000u;
+  if (hi) x &= 0x0000ffffu;
+  return (lo ? 1u : 0u) | (hi ? 2u : 0u);
+}
+// of those, the NaN ones (mantissa not 0), given the pair as it was
+template <typename T>
+__device__ __forceinline__ uint32_t nan_bits(uint32_t x, uint32_t bad) {
+  constexpr uint32_t m = std::is_same<T, __half>::value ? 0x03ffu : 0x007fu;
+  return bad & ((x & m ? 1u : 0u) | (x & (m << 16) ? 2u : 0u));
 }
 
 template <typename T, int D, int NT>
@@ -245,6 +216,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
   char* smem = smem_raw + (sbase - raw);
   const uint32_t mb = sbase + Sh::oMeta;
   volatile int* abort = reinterpret_cast<volatile int*>(smem + Sh::oMeta + Sh::oAbort);
+  volatile int* again = reinterpret_cast<volatile int*>(smem + Sh::oMeta + Sh::oAgain);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = blockIdx.x % a.hkv;
   const PrefixItem it = a.items[blockIdx.x / a.hkv];
@@ -301,7 +273,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       }
     }
   };
-  if (tid == 0) {
+  auto init_barriers = [&] {
     mbar_init(mb + Sh::bQ, Sh::kTile * tiles);
     for (int s = 0; s < Sh::KS; ++s) mbar_init(mb + Sh::bK + 8 * s, 32);
     for (int s = 0; s < Sh::VS; ++s) mbar_init(mb + Sh::bV + 8 * s, 32);
@@ -313,8 +285,12 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       mbar_init(mb + Sh::bPV + 8 * s, 1);
     }
     for (int s = 0; s < 4 * NT; ++s) mbar_init(mb + Sh::bMax + 8 * s, 2);
-    *abort = 0;
     mbar_init_fence();
+  };
+  if (tid == 0) {
+    init_barriers();
+    *abort = 0;
+    *again = 0;
     if (a.tma)
       asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&a.tm)) : "memory");
   }
@@ -334,9 +310,23 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
   // step t uses score buffer t & 1 of its row tile
   auto at = [&](uint32_t bar, int qt, int t) { return mb + bar + 8 * (2 * qt + (t & 1)); };
 
+  bool bad_row = false;  // (softmax) this thread's columns of its row came out not finite
+
+  // One pass of the block over its keys.  The careful one follows where a value
+  // that is not finite got into a row's sums: it takes such values out of the V
+  // tiles and writes again the columns that were not finite.  With one such
+  // value in a prefix of 5120 keys, 64 questions of 64 tokens take 1.0 ms and 64
+  // decodes 57 us, against 0.34 ms and 30 us (a block's rows walked one by one,
+  // key after key, took 1.5 s and 42 ms).
+  auto pass = [&](auto careful) {
+  constexpr bool kCareful = decltype(careful)::value;
   if (warp == Sh::kSoft || warp == Sh::kSoft + 1) {
     // ============================================== producers: K, then V warp
     const int ST = isv ? Sh::VS : Sh::KS;
+    if constexpr (kCareful) {
+#pragma unroll
+      for (int k = 0; k < 3; ++k) ahead[k] = load_slots(k);
+    }
     int issued = 0;
     auto produce = [&](int t, Slots& mine) {
       Src cur;
@@ -539,14 +529,62 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     const uint32_t oc = tmem + lane_base + Sh::cO + D * qt;
     float mref = -INFINITY, lsum = 0.f;  // log2 domain; P = 2^(x - mref + up)
     bool ok = true;
-    int exchanges = 0;  // of maxima with the row's other thread
-    const uint32_t pair = mb + Sh::bMax + 8 * (4 * qt + (warp & 3));
-    float* row_max = reinterpret_cast<float*>(smem + Sh::oMeta + Sh::oMax) + qt * 512;
+    [[maybe_unused]] int exchanges = 0;  // of maxima with the row's other thread
+    [[maybe_unused]] const uint32_t pair = mb + Sh::bMax + 8 * (4 * qt + (warp & 3));
+    [[maybe_unused]] float* row_max =
+        reinterpret_cast<float*>(smem + Sh::oMeta + Sh::oMax) + qt * 512;
     const bool any_row = __any_sync(~0u, row_ok);
+    // (careful) which columns of the row keys that it sees make not finite: a
+    // bit a column, NaN, +inf and -inf
+    uint32_t poison[kCareful ? kKinds : 1][D / 32];
+    if constexpr (kCareful) {
+#pragma unroll
+      for (int k = 0; k < kKinds; ++k) {
+#pragma unroll
+        for (int w = 0; w < D / 32; ++w) poison[k][w] = 0u;
+      }
+    }
     auto wait_pv = [&](int t) {
       ok = warp_wait(at(Sh::bPV, qt, t), (t >> 1) & 1, abort);
       tc_fence_after();
       return ok;
+    };
+
+    // (careful) takes the values that are not finite out of step t's V tile,
+    // all softmax threads an equal share of its 16-byte pieces, and notes which
+    // they were: a byte of column bits a piece and kind, for two steps in turn
+    const int softs = Sh::kTile * tiles;
+    volatile int* found = reinterpret_cast<volatile int*>(smem + Sh::oMeta + Sh::oFound);
+    auto clean = [&](int t) {
+      if (!warp_wait(mb + Sh::bV + 8 * (t % Sh::VS), (t / Sh::VS) & 1, abort)) return false;
+      constexpr int C = D / 8;
+      const uint32_t tile = sbase + Sh::oV + (t % Sh::VS) * Sh::TB;
+      uint8_t* notes = reinterpret_cast<uint8_t*>(smem + Sh::oMeta + Sh::oBad) +
+                       (t & 1) * kKinds * kKeys * C;
+      for (int i = tid; i < kKeys * C; i += softs) {
+        const uint32_t at = tile + sw128(i / C, i % C, kKeys);
+        const uint4 was = ld_shared16(at);
+        const uint32_t x[4] = {was.x, was.y, was.z, was.w};
+        uint32_t y[4], bad = 0u, nan = 0u, minus = 0u;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          y[k] = x[k];
+          const uint32_t b = take_out<T>(y[k]);
+          bad |= b << (2 * k);
+          nan |= nan_bits<T>(x[k], b) << (2 * k);
+          minus |= ((x[k] >> 15 & 1u) | (x[k] >> 30 & 2u)) << (2 * k);
+        }
+        notes[i] = (uint8_t)nan;
+        notes[kKeys * C + i] = (uint8_t)(bad & ~nan & ~minus);
+        notes[2 * kKeys * C + i] = (uint8_t)(bad & ~nan & minus);
+        if (bad) {
+          st_shared16(at, make_uint4(y[0], y[1], y[2], y[3]));
+          found[t & 1] = t + 1;
+        }
+      }
+      fence_async_smem();
+      mbar_arrive(mb + Sh::bClean);
+      return warp_wait(mb + Sh::bClean, t & 1, abort);
     };
 
     for (int t = 0; t < steps; ++t) {
@@ -561,6 +599,10 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       if (!ok) break;  // a wait expired
       if (!Sh::kDirect && tid % Sh::kTile == 0) mbar_arrive(mb + Sh::bKr + 8 * (t % Sh::KS));
       tc_fence_after();
+      if constexpr (kCareful) {
+        ok = clean(t);
+        if (!ok) break;
+      }
       if (!any_row) {  // no query in these 32 rows: their P is zero already
         mbar_arrive(at(Sh::bP, qt, t));
         continue;
@@ -587,6 +629,35 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
 #pragma unroll
           for (int c = 0; c < 32; ++c)
             v[32 * cc + c] = (bits >> c) & 1u ? v[32 * cc + c] : 0xff800000u;  // -inf
+        }
+      }
+      if constexpr (kCareful) {
+        if (found[t & 1] == t + 1) {
+          // keys that the row sees, but for scores of -inf, which weigh nothing
+          uint32_t seen[VC / 32];
+#pragma unroll
+          for (int cc = 0; cc < VC / 32; ++cc) {
+            seen[cc] = 0u;
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              seen[cc] |= v[32 * cc + c] != 0xff800000u ? 1u << c : 0u;
+          }
+          const uint32_t* notes = reinterpret_cast<const uint32_t*>(smem + Sh::oMeta + Sh::oBad) +
+                                  (t & 1) * kKinds * kKeys * (D / 32);
+#pragma unroll
+          for (int cc = 0; cc < VC / 32; ++cc) {
+#pragma unroll 1
+            for (int c = 0; c < 32; ++c) {
+              if (!(seen[cc] >> c & 1u)) continue;
+#pragma unroll
+              for (int k = 0; k < kKinds; ++k) {
+#pragma unroll
+                for (int w = 0; w < D / 32; ++w)
+                  poison[k][w] |=
+                      notes[(k * kKeys + 32 * (part2 + cc) + c) * (D / 32) + w];
+              }
+            }
+          }
         }
       }
       float top;
@@ -679,6 +750,33 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       if (lane == 0) mbar_arrive(pair);
       ok = ok && warp_wait(pair, exchanges & 1, abort);
       lsum += sum[(1 - part2) * 128 + r];
+      if constexpr (kCareful) {
+        // each thread looked at half the step's keys: both halves' findings,
+        // through the place of the queries (read by no product any more)
+        ++exchanges;
+        constexpr int kWords = kKinds * (D / 32);
+        static_assert(2 * kWords * 4 <= 2 * D + 16, "within the row's place of the staging below");
+        uint32_t* row = reinterpret_cast<uint32_t*>(smem + Sh::oQ + qt * Sh::QB + r * (2 * D + 16));
+        uint32_t *mine = row + part2 * kWords, *theirs = row + (1 - part2) * kWords;
+#pragma unroll
+        for (int k = 0; k < kKinds; ++k) {
+#pragma unroll
+          for (int w = 0; w < D / 32; ++w) mine[k * (D / 32) + w] = poison[k][w];
+        }
+        for (int turn = 0; turn < 2; ++turn) {  // written, then read
+          __syncwarp();
+          if (lane == 0) mbar_arrive(pair);
+          ok = ok && warp_wait(pair, exchanges & 1, abort);
+          ++exchanges;
+          if (turn == 0) {
+#pragma unroll
+            for (int k = 0; k < kKinds; ++k) {
+#pragma unroll
+              for (int w = 0; w < D / 32; ++w) poison[k][w] |= theirs[k * (D / 32) + w];
+            }
+          }
+        }
+      }
     }
     const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
     const float lse2 = lsum == 0.f ? -INFINITY
@@ -690,10 +788,37 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
     if (part) orow = reinterpret_cast<char*>(a.part_o + prow * D);
     const bool have = ok && steps > 0 && lsum != 0.f;
     // An infinite or NaN value of a key that this row does not see reaches its
-    // sums as 0 x inf = NaN, so a row (a thread's columns of it) that is not
-    // finite is computed again below, from the keys it sees alone.
+    // sums as 0 x inf = NaN.  So where a row (a thread's columns of it) is not
+    // finite, the block passes over its keys once more, with such values taken
+    // out of the V tiles, and the columns that they belong to are set for the
+    // rows that see them.  (A NaN sum of weights makes the row NaN as it is.)
     float worst = 0.f;
-    auto finite = [&](uint32_t x) { worst = max_nan(worst, fabsf(__uint_as_float(x))); };
+    uint32_t set_to[kKinds][D / 32 / TPR];  // of this thread's columns
+    if constexpr (kCareful) {
+#pragma unroll
+      for (int k = 0; k < kKinds; ++k) {
+#pragma unroll
+        for (int w = 0; w < D / 32 / TPR; ++w) {
+          const uint32_t low = poison[k][w], high = poison[k][w + D / 32 - D / 32 / TPR];
+          set_to[k][w] = part2 == 0 ? low : high;
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < D / 32 / TPR; ++w) set_to[0][w] |= set_to[1][w] & set_to[2][w];
+    }
+    // element c of this thread's columns as it is written
+    auto final = [&](float x, int c) {
+      if constexpr (kCareful) {
+        const int w = c / 32, b = c % 32;
+        if (set_to[2][w] >> b & 1u) x = -INFINITY;
+        if (set_to[1][w] >> b & 1u) x = INFINITY;
+        if (set_to[0][w] >> b & 1u) x = __int_as_float(0x7fffffff);
+      } else {
+        worst = max_nan(worst, fabsf(x));
+      }
+      return x;
+    };
+    const bool write = ok && (kCareful ? bad_row : row_ok);
     if (part || a.vec_out) {
       // each thread stages its row (32-bit partials in two halves) where the
       // queries were, and the warp writes whole rows: stores straight from the
@@ -704,8 +829,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
       constexpr int W = 2 * D + 16;
       const uint32_t stage = sbase + Sh::oQ + qt * Sh::QB + (r - lane) * W + part2 * B;
       const uint32_t buf = stage + lane * W;
-      const uint64_t to = row_ok && ok ? reinterpret_cast<uint64_t>(orow) : 0;
-#pragma unroll 1
+      const uint64_t to = write ? reinterpret_cast<uint64_t>(orow) : 0;
+#pragma unroll(kCareful ? 2 : 1)
       for (int round = 0; round < (part ? 2 : 1); ++round) {
         uint32_t v[32];
         const uint32_t col = oc + part2 * (D / 2);
@@ -715,10 +840,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
             CS_TMEM_LD16(col + round * (B / 4) + 16 * cc, v);
             tmem_wait_ld();
 #pragma unroll
-            for (int c = 0; c < 16; ++c) {
-              v[c] = have ? __float_as_uint(__uint_as_float(v[c]) * inv) : 0u;
-              finite(v[c]);
-            }
+            for (int c = 0; c < 16; ++c)
+              v[c] = __float_as_uint(final(have ? __uint_as_float(v[c]) * inv : 0.f,
+                                           round * (B / 4) + 16 * cc + c));
 #pragma unroll
             for (int c = 0; c < 4; ++c)
               st_shared16(buf + 64 * cc + 16 * c,
@@ -733,9 +857,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
             for (int c = 0; c < 16; ++c) {
               const float x = have ? __uint_as_float(v[2 * c]) * inv : 0.f;
               const float y = have ? __uint_as_float(v[2 * c + 1]) * inv : 0.f;
-              finite(__float_as_uint(x));
-              finite(__float_as_uint(y));
-              v[c] = Pack2<T>::pack(x, y);
+              v[c] = Pack2<T>::pack(final(x, 32 * cc + 2 * c), final(y, 32 * cc + 2 * c + 1));
             }
 #pragma unroll
             for (int c = 0; c < 4; ++c)
@@ -763,42 +885,52 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, NT == 1 ? 2 : 1)
         __syncwarp();
       }
     } else {
-#pragma unroll 1
-      for (int cc = part2 * (D / 64); cc < (part2 + 1) * (D / 32 / TPR); ++cc) {
+#pragma unroll(kCareful ? D / 32 / TPR : 1)
+      for (int cc = 0; cc < D / 32 / TPR; ++cc) {
         uint32_t v[32];
-        CS_TMEM_LD32(oc + 32 * cc, v);
+        const int col = part2 * (D / 2) + 32 * cc;
+        CS_TMEM_LD32(oc + col, v);
         tmem_wait_ld();
-        if (!row_ok || !ok) continue;
+        if (!write) continue;
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          const float x = have ? __uint_as_float(v[c]) * inv : 0.f;
-          finite(__float_as_uint(x));
-          reinterpret_cast<T*>(orow)[32 * cc + c] = Elem<T>::from_f(x);
-        }
+        for (int c = 0; c < 32; ++c)
+          reinterpret_cast<T*>(orow)[col + c] = Elem<T>::from_f(
+              final(have ? __uint_as_float(v[c]) * inv : 0.f, 32 * cc + c));
       }
     }
-    __syncwarp();
-    for (uint32_t again = __ballot_sync(~0u, row_ok && have && !(worst < INFINITY)); again;
-         again &= again - 1) {
-      const int src = __ffs(again) - 1;
-      const int rr = r - lane + src;
-      const int tt = qt * a.R + rr / a.G, hh = g * a.G + rr % a.G;
-      row_again<T, D, TPR>(
-          a, it, g, tt, hh, lane, part2,
-          reinterpret_cast<void*>(__shfl_sync(~0u, reinterpret_cast<uint64_t>(orow), src)), part);
+    if constexpr (!kCareful) {
+      bad_row = write && have && lsum == lsum && !(worst < INFINITY);
+      if (bad_row) *again = 1;
     }
-    if (row_ok && ok && part2 == 0) {
+    if (!kCareful && write && part2 == 0) {
       if (it.part >= 0) a.part_lse[prow] = lse2;
       else if (a.lse) a.lse[token * a.hq + h] = lse2 * kLn2;
     }
     }
   }
+  };
+  pass(std::false_type());
 
   // the joining grid starts while the last blocks write (told earlier, its
   // blocks wait beside these and cost 8 decodes behind 65536 keys 5 us)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   tc_fence_before();
   __syncthreads();
+  if (*again && !*abort) {  // nothing of the first pass is in flight
+    tc_fence_after();
+    if (tid == 0) {
+      for (uint32_t b = Sh::bQ; b < Sh::oTmem; b += 8) mbar_inval(mb + b);
+      init_barriers();
+      mbar_init(mb + Sh::bClean, Sh::kTile * tiles);
+      mbar_init_fence();
+      volatile int* found = reinterpret_cast<volatile int*>(smem + Sh::oMeta + Sh::oFound);
+      found[0] = found[1] = 0;
+    }
+    __syncthreads();
+    pass(std::true_type());
+    tc_fence_before();
+    __syncthreads();
+  }
   if (tid == 0 && *abort) report(a.status, CS_ST_TIMEOUT);
   if (warp == Sh::kSoft + 2) {
     tc_fence_after();
@@ -995,7 +1127,6 @@ int prefix_attn_sm100(const cs_prefix_params& p, const cs_prefix_plan_info& info
   a.neg = p.scale < 0.0;
   // masked scores are -inf before they are scaled, so the factor is never 0
   a.scale2 = fmaxf(fabsf((float)p.scale) * kLog2e, 1e-30f);
-  a.scale = (float)p.scale;
   a.nrb = a.nrh = a.nro = 0;
   // runs are found where a block's offsets are consecutive rows
   a.tma = setup_maps(a, kv) && a.nro == 1 ? 1 : 0;

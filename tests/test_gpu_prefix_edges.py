@@ -6,8 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_gpu_prefix import BF, HF, LAYOUTS, batch, bounds, plan_of
-from oracle import prefix as oprefix
+from test_gpu_prefix import BF, HF, LAYOUTS, batch, plan_of
 
 pytestmark = pytest.mark.gpu
 
@@ -26,35 +25,103 @@ def last_own_slots(s, lens):
     return out
 
 
-@pytest.mark.parametrize("name", ["wide batch", "wide ragged", "drafts"])
+def put(s, slots, values, d):
+    """values[k][column] written to the V half of slot k's records, every head."""
+    for slot, row in zip(slots, values):
+        for c, x in row.items():
+            s["cache"][slot // 16, :, slot % 16, d + c] = x
+
+
+NAMES = ["decode", "drafts", "groups", "questions", "wide batch", "wide ragged"]
+
+
+@pytest.mark.parametrize("name", NAMES)
 @pytest.mark.parametrize("hq,hk,d,dtype", HEADS)
-@pytest.mark.parametrize("column", ["first", "last"])
-def test_a_hidden_value_in_one_half_leaves_the_other_half_alone(cuda, name, hq, hk, d, dtype,
-                                                                column):
-    """Rows that do not see the key keep, in the columns of the half of the head
-    without it, the bits that they have without the infinity; the columns of
-    its half are computed again (within the tolerance); equal calls give equal
-    bits."""
+@pytest.mark.parametrize("columns", ["first half", "last half", "all"])
+def test_a_hidden_value_leaves_no_trace(cuda, name, hq, hk, d, dtype, columns):
+    """Rows that do not see the key have the bits that they have without the
+    infinity, also in repeated calls, and in the row that sees it the other
+    columns are finite."""
     s, lens = batch(cuda, hq, hk, d, dtype, *LAYOUTS[name])
     plan = plan_of(s, lens)
     args = s["query"], s["cache"], s["prefix_slots"], s["suffix_slots"]
-    clean = plan(*args)
-    c = 3 if column == "first" else d - 2
-    other = slice(d // 2, d) if column == "first" else slice(0, d // 2)
     sees = torch.zeros(s["query"].shape[0], dtype=torch.bool, device=cuda)
-    for i, (token, slot) in enumerate(last_own_slots(s, lens)):
-        s["cache"][slot // 16, :, slot % 16, d + c] = (NAN, INF, -INF)[i % 3]
-        sees[token] = True
-    got = plan(*args)
-    for _ in range(5):
-        assert torch.equal(plan(*args)[~sees], got[~sees])
-    if plan.info.variant == 2:
-        assert torch.equal(got[~sees][..., other], clean[~sees][..., other])
-    tol = bounds(dtype, d, lens, *oprefix.attention(
-        s["query"], s["cache"].nan_to_num(0, 0, 0), s["prefix_slots"], s["suffix_slots"], **lens))[0]
-    off = (got.double() - clean.double()).abs()[~sees]
-    assert (off <= 2 * tol[~sees]).all()
-    # those that see it: that column alone is not finite
-    assert not torch.isfinite(got[sees][..., c]).any()
-    rest = torch.arange(d, device=cuda) != c
-    assert torch.isfinite(got[sees][..., rest]).all()
+    cols = dict([("first half", [3]), ("last half", [d - 2]), ("all", range(d))])[columns]
+    last = last_own_slots(s, lens)
+    put(s, [slot for _, slot in last], [dict.fromkeys(cols, 0.0)] * len(last), d)
+    clean, clean_lse = plan(*args, return_lse=True)
+    put(s, [slot for _, slot in last],
+        [dict.fromkeys(cols, (NAN, INF, -INF)[i % 3]) for i in range(len(last))], d)
+    sees[[token for token, _ in last]] = True
+    for _ in range(4):
+        got, lse = plan(*args, return_lse=True)
+        assert torch.equal(got[~sees], clean[~sees]) and torch.equal(lse, clean_lse)
+    hit = torch.zeros(d, dtype=torch.bool, device=cuda)
+    hit[list(cols)] = True
+    for i, (token, _) in enumerate(last):
+        if i % 3 == 0:
+            assert torch.isnan(got[token][:, hit]).all()
+        else:
+            assert (got[token][:, hit] == (INF, -INF)[i % 3 - 1]).all()
+        assert torch.equal(got[token][:, ~hit], clean[token][:, ~hit])
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("hq,hk,d,dtype", HEADS)
+def test_values_in_the_prefix_reach_their_columns_alone(cuda, name, hq, hk, d, dtype):
+    """NaN, infinities of one sign and of both: what a sum of positive weights
+    times such values is, and the bits without them in every other column."""
+    s, lens = batch(cuda, hq, hk, d, dtype, *LAYOUTS[name])
+    plan = plan_of(s, lens)
+    args = s["query"], s["cache"], s["prefix_slots"], s["suffix_slots"]
+    where = [int(s["prefix_slots"][i]) for i in (0, 66, 100)]
+    values = [{0: NAN, 5: INF, 6: -INF, 7: INF}, {7: -INF, d - 1: NAN, d // 2: INF},
+              {0: INF, 5: INF, d // 2 + 1: -INF}]
+    put(s, where, [dict.fromkeys(row, 0.0) for row in values], d)
+    clean, clean_lse = plan(*args, return_lse=True)
+    put(s, where, values, d)
+    want = clean.clone()
+    sees = torch.zeros(s["query"].shape[0], dtype=torch.bool, device=cuda)
+    sees[:sum(lens["query_lens"][:(lens["group_sizes"] or [len(lens["query_lens"])])[0]])] = True
+    for c, x in ((0, NAN), (5, INF), (6, -INF), (7, NAN), (d - 1, NAN), (d // 2, INF),
+                 (d // 2 + 1, -INF)):
+        want[sees, :, c] = x
+    got, lse = plan(*args, return_lse=True)
+    torch.testing.assert_close(got, want, rtol=0, atol=0, equal_nan=True)
+    assert torch.equal(lse, clean_lse)
+
+
+@pytest.mark.parametrize("name", ["decode", "wide batch"])
+@pytest.mark.parametrize("hq,hk,d,dtype", HEADS)
+def test_values_of_keys_that_weigh_nothing(cuda, name, hq, hk, d, dtype):
+    """A score of -inf weighs nothing, whatever its value holds."""
+    s, lens = batch(cuda, hq, hk, d, dtype, *LAYOUTS[name])
+    plan = plan_of(s, lens)
+    args = s["query"], s["cache"], s["prefix_slots"], s["suffix_slots"]
+    s["query"][..., 0] = 1.0
+    first = s["prefix_slots"][30:130]
+    s["cache"][first // 16, :, first % 16, 0] = -INF
+    s["cache"][first // 16, :, first % 16, d:] = 0.0
+    clean = plan(*args)
+    s["cache"][first // 16, :, first % 16, d:] = NAN
+    assert torch.equal(plan(*args), clean)
+
+
+@pytest.mark.parametrize("name", ["decode", "questions", "wide ragged"])
+def test_values_in_strided_outputs_and_odd_queries(cuda, name):
+    """The same where outputs are not stored in vectors."""
+    s, lens = batch(cuda, 8, 2, 128, BF, *LAYOUTS[name])
+    plan = plan_of(s, lens)
+    tokens = s["query"].shape[0]
+    slot = int(s["prefix_slots"][70])
+    put(s, [slot], [{2: 0.0, 100: 0.0}], 128)
+    args = s["query"], s["cache"], s["prefix_slots"], s["suffix_slots"]
+    want = plan(*args)
+    put(s, [slot], [{2: NAN, 100: INF}], 128)
+    want[..., 2], want[..., 100] = NAN, INF
+    out = torch.zeros(tokens, 8, 129, dtype=BF, device=cuda)
+    odd = torch.zeros(tokens, 8 * 128 + 1, dtype=BF, device=cuda)[:, 1:].unflatten(1, (8, 128))
+    odd.copy_(s["query"])
+    got = plan(odd, *args[1:], out=out[..., 1:])
+    torch.testing.assert_close(got, want, rtol=0, atol=0, equal_nan=True)
+    assert not out[..., 0].any()
