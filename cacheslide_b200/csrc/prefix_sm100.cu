@@ -967,13 +967,15 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const PArgs a, const i
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
   for (int c0 = 0; c0 < j.z; c0 += 32) {
-    // a lane's partial of these 32: its place and weight (NaN stays NaN)
+    // a lane's partial of these 32: its place and weight (NaN stays NaN; one
+    // below 2^-126 of the largest is that, not 0, so that what is not finite
+    // in it is not lost)
     float l = l0;
     if (c0 > 0) {
       first = c0 + lane < j.z ? list[j.y + c0 + lane] : 0;
       l = c0 + lane < j.z ? a.part_lse[(int64_t)first * a.hq + h] : -INFINITY;
     }
-    const float f = l == -INFINITY ? 0.f : ex2(l - top);
+    const float f = l == -INFINITY ? 0.f : max_nan(ex2(l - top), 0x1p-126f);
     sum += warp_sum(f);
     const int m = j.z - c0 < 32 ? j.z - c0 : 32;
 #pragma unroll 1

@@ -125,3 +125,23 @@ def test_values_in_strided_outputs_and_odd_queries(cuda, name):
     got = plan(odd, *args[1:], out=out[..., 1:])
     torch.testing.assert_close(got, want, rtol=0, atol=0, equal_nan=True)
     assert not out[..., 0].any()
+
+
+@pytest.mark.parametrize("hq,hk,d,dtype", HEADS + [(4, 2, 80, BF), (4, 2, 64, torch.float32)])
+@pytest.mark.parametrize("value", [NAN, INF])
+def test_a_part_of_little_weight_keeps_what_is_not_finite(cuda, hq, hk, d, dtype, value):
+    """Scores far below the row's largest (here by some 2000) still weigh more
+    than nothing: a NaN or infinite value among them makes its column not
+    finite, wherever the plan cuts the keys."""
+    s, lens = batch(cuda, hq, hk, d, dtype, [1] * 3, [40] * 3, [4000])
+    plan = plan_of(s, lens)
+    s["query"][..., 0] = 160.0
+    slots = s["prefix_slots"]
+    s["cache"][..., 0] = 0.0
+    s["cache"][slots[:1000] // 16, :, slots[:1000] % 16, 0] = 160.0
+    far = int(slots[3000])
+    put(s, [far], [{9: value}], d)
+    got = plan(s["query"], s["cache"], s["prefix_slots"], s["suffix_slots"])
+    assert not torch.isfinite(got[..., 9]).any()
+    rest = torch.arange(d, device=cuda) != 9
+    assert torch.isfinite(got[..., rest]).all()
