@@ -333,18 +333,21 @@ double best_cut(const Layout& l, const Cost& c, Make units_for, double least,
 int make_plan(const cs_prefix_shape* s, cs_prefix_plan_info* info, int32_t* words,
               int64_t capacity) {
   int64_t tokens = 0, n_suffix = 0, n_prefix = 0, members = 0;
+  // each length is bounded before it is added, so that no sum wraps
   for (int b = 0; b < s->requests; ++b) {
     CS_HOST_CHECK(s->query_lens[b] >= 0 && s->suffix_lens[b] >= 0);
+    if (s->query_lens[b] > INT32_MAX || s->suffix_lens[b] > INT32_MAX) return CS_ERR_UNSUPPORTED;
     tokens += s->query_lens[b];
     n_suffix += s->suffix_lens[b];
     if (tokens > INT32_MAX / 8 || n_suffix > INT32_MAX / 2) return CS_ERR_UNSUPPORTED;
   }
   for (int g = 0; g < s->groups; ++g) {
     CS_HOST_CHECK(s->group_sizes[g] >= 0 && s->prefix_lens[g] >= 0);
+    CS_HOST_CHECK(s->group_sizes[g] <= s->requests - members);
     members += s->group_sizes[g];
+    if (s->prefix_lens[g] > INT32_MAX) return CS_ERR_UNSUPPORTED;
     n_prefix += s->prefix_lens[g];
     if (n_prefix > INT32_MAX / 2) return CS_ERR_UNSUPPORTED;
-    CS_HOST_CHECK(members <= s->requests);
   }
   CS_HOST_CHECK(members == s->requests);
   std::memset(info, 0, sizeof(*info));
