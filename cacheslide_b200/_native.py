@@ -171,6 +171,7 @@ class PrefixPlanInfo(ctypes.Structure):
         ("words", _i64), ("workspace", _i64), ("tokens", _i64), ("n_prefix", _i64),
         ("n_suffix", _i64), ("item_off", _i64), ("n_items", _i64), ("join_off", _i64),
         ("n_join", _i64), ("list_off", _i64), ("part_tokens", _i64), ("variant", _i32),
+        ("group", _i32),
     ]
 
 

@@ -330,6 +330,11 @@ double best_cut(const Layout& l, const Cost& c, Make units_for, double least,
   return least;
 }
 
+// partial results: an output row and its sum, float32
+int64_t part_bytes(int64_t part_tokens, int64_t q_heads, int64_t head_dim) {
+  return part_tokens * q_heads * (head_dim + 1) * (int64_t)sizeof(float);
+}
+
 int make_plan(const cs_prefix_shape* s, cs_prefix_plan_info* info, int32_t* words,
               int64_t capacity) {
   int64_t tokens = 0, n_suffix = 0, n_prefix = 0, members = 0;
@@ -351,6 +356,7 @@ int make_plan(const cs_prefix_shape* s, cs_prefix_plan_info* info, int32_t* word
   }
   CS_HOST_CHECK(members == s->requests);
   std::memset(info, 0, sizeof(*info));
+  info->group = s->q_heads / s->kv_heads;
   info->tokens = tokens;
   info->n_prefix = n_prefix;
   info->n_suffix = n_suffix;
@@ -432,7 +438,7 @@ int make_plan(const cs_prefix_shape* s, cs_prefix_plan_info* info, int32_t* word
   info->join_off = info->item_off + iw;
   info->list_off = info->join_off + (int64_t)join.size();
   info->words = info->list_off + (int64_t)list.size();
-  info->workspace = info->part_tokens * s->q_heads * (s->head_dim + 1) * (int64_t)sizeof(float);
+  info->workspace = part_bytes(info->part_tokens, s->q_heads, s->head_dim);
   if (words == nullptr || capacity < info->words) return CS_ERR_TOO_LARGE;
   std::copy(rows.begin(), rows.end(), words);
   if (iw) std::memcpy(words + info->item_off, items.data(), iw * 4);
@@ -470,6 +476,12 @@ extern "C" int cs_prefix_attn(const cs_prefix_params* p, const cs_prefix_plan_in
   CS_HOST_CHECK(p->q_heads > 0 && p->q_heads % kv.kv_heads == 0);
   if (kv.dtype != CS_F32 && kv.dtype != CS_F16 && kv.dtype != CS_BF16) return CS_ERR_UNSUPPORTED;
   if (kv.head_dim > kMaxDim) return CS_ERR_UNSUPPORTED;
+  // a plan's row tiles, partials and workspace belong to its heads and type
+  CS_HOST_CHECK(info->group == p->q_heads / kv.kv_heads);
+  if (info->variant > 0)
+    CS_HOST_CHECK((kv.dtype == CS_F16 || kv.dtype == CS_BF16) &&
+                  (kv.head_dim == 64 || kv.head_dim == 128) &&
+                  info->workspace == part_bytes(info->part_tokens, p->q_heads, kv.head_dim));
   if (info->tokens == 0) return CS_OK;
   CS_HOST_CHECK(p->q && p->out && plan && (info->workspace == 0 || workspace));
   CS_HOST_CHECK((info->n_prefix == 0 || p->prefix_slots) &&

@@ -733,6 +733,7 @@ typedef struct {
   int64_t part_tokens;
   int32_t variant;        /* 0: CUDA cores; 1, 2: tensor cores, 128 or 256
                              query rows a block                           */
+  int32_t group;          /* query heads a KV head                        */
 } cs_prefix_plan_info;
 
 CS_API int cs_prefix_plan(const cs_prefix_shape* shape, cs_prefix_plan_info* info,
@@ -756,7 +757,8 @@ typedef struct {
  * The attention itself.  `plan` is the device copy of the plan's words and
  * `workspace` holds info->workspace bytes that nothing else uses meanwhile
  * (its content does not matter).  A slot outside the pool sets
- * CS_ST_SLOT_RANGE and its key is read as zeros.
+ * CS_ST_SLOT_RANGE and its key is read as zeros.  CS_ERR_INVALID when the
+ * heads or the type are not those that `info` was planned for.
  */
 CS_API int cs_prefix_attn(const cs_prefix_params* p, const cs_prefix_plan_info* info,
                           const int32_t* plan, void* workspace, void* stream);

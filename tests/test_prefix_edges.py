@@ -1,15 +1,13 @@
 """The C entries of the attention behind shared prefixes without a GPU: lengths
-that no plan holds, plans of other heads, scales that float32 does not hold."""
+that no plan holds, plans of other heads."""
 
 from __future__ import annotations
 
 import ctypes
 
 import pytest
-import torch
 
 from cacheslide_b200 import _native as N
-from cacheslide_b200.prefix import SharedPrefixAttention
 
 HUGE = (1 << 63) - 1
 
@@ -37,3 +35,30 @@ def test_lengths_whose_sums_pass_64_bits(lens):
 @pytest.mark.parametrize("sizes", [[HUGE, HUGE, 4], [2, HUGE], [1 << 32, 2], [-1, 3]])
 def test_group_sizes_that_only_add_up_modulo_64_bits(sizes):
     assert c_plan([5] * len(sizes), sizes, [1, 1], [3, 3])[0] == N.CS_ERR_INVALID
+
+
+def c_call(info, heads=(32, 8, 128), dtype=N.CS_BF16, workspace=16, scale=0.1):
+    """cs_prefix_attn up to its checks: no argument is a place in memory."""
+    kv = N.PagedKV(cache=16, num_blocks=4, kv_heads=heads[1], block_size=16, head_dim=heads[2],
+                   stride_block=heads[1] * 32 * heads[2], stride_head=32 * heads[2],
+                   stride_offset=2 * heads[2], stride_elem=1, dtype=dtype)
+    p = N.PrefixParams(q=16, paged=kv, prefix_slots=16, suffix_slots=16, q_heads=heads[0],
+                       scale=scale, out=16)
+    return N.load().cs_prefix_attn(ctypes.byref(p), ctypes.byref(info), 16, workspace, None)
+
+
+@pytest.mark.parametrize("heads,dtype", [
+    ((64, 8, 128), N.CS_BF16), ((64, 16, 128), N.CS_BF16), ((32, 4, 128), N.CS_BF16),
+    ((32, 8, 64), N.CS_BF16), ((32, 8, 80), N.CS_BF16), ((32, 8, 128), N.CS_F32),
+])
+def test_a_call_refuses_a_plan_of_other_heads(heads, dtype):
+    rc, info = c_plan([3000], [4], [1] * 4, [30] * 4)
+    assert rc == N.CS_OK and info.variant > 0 and info.workspace > 0
+    assert c_call(info, heads, dtype) == N.CS_ERR_INVALID
+    assert c_call(info, workspace=None) == N.CS_ERR_INVALID
+
+
+def test_a_call_refuses_a_row_plan_of_other_groups():
+    rc, info = c_plan([3000], [4], [1] * 4, [30] * 4, dtype=N.CS_F32)
+    assert rc == N.CS_OK and info.variant == 0
+    assert c_call(info, (32, 4, 128), N.CS_F32) == N.CS_ERR_INVALID
