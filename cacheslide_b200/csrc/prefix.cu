@@ -474,6 +474,7 @@ extern "C" int cs_prefix_attn(const cs_prefix_params* p, const cs_prefix_plan_in
   const cs_paged_kv& kv = p->paged;
   CS_HOST_CHECK(kv.cache != nullptr && kv.block_size > 0 && kv.kv_heads > 0 && kv.head_dim > 0);
   CS_HOST_CHECK(p->q_heads > 0 && p->q_heads % kv.kv_heads == 0);
+  CS_HOST_CHECK(std::isfinite((float)p->scale));  // as the kernels use it
   if (kv.dtype != CS_F32 && kv.dtype != CS_F16 && kv.dtype != CS_BF16) return CS_ERR_UNSUPPORTED;
   if (kv.head_dim > kMaxDim) return CS_ERR_UNSUPPORTED;
   // a plan's row tiles, partials and workspace belong to its heads and type

@@ -758,7 +758,8 @@ typedef struct {
  * `workspace` holds info->workspace bytes that nothing else uses meanwhile
  * (its content does not matter).  A slot outside the pool sets
  * CS_ST_SLOT_RANGE and its key is read as zeros.  CS_ERR_INVALID when the
- * heads or the type are not those that `info` was planned for.
+ * heads or the type are not those that `info` was planned for, or the scale is
+ * not finite as a float.
  */
 CS_API int cs_prefix_attn(const cs_prefix_params* p, const cs_prefix_plan_info* info,
                           const int32_t* plan, void* workspace, void* stream);

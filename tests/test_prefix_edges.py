@@ -1,5 +1,5 @@
 """The C entries of the attention behind shared prefixes without a GPU: lengths
-that no plan holds, plans of other heads."""
+that no plan holds, plans of other heads, scales that float32 does not hold."""
 
 from __future__ import annotations
 
@@ -62,3 +62,9 @@ def test_a_call_refuses_a_row_plan_of_other_groups():
     rc, info = c_plan([3000], [4], [1] * 4, [30] * 4, dtype=N.CS_F32)
     assert rc == N.CS_OK and info.variant == 0
     assert c_call(info, (32, 4, 128), N.CS_F32) == N.CS_ERR_INVALID
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 1e39, -1e300])
+def test_a_call_refuses_scales_that_are_not_finite_floats(scale):
+    _, info = c_plan([3000], [4], [1] * 4, [30] * 4)
+    assert c_call(info, scale=scale) == N.CS_ERR_INVALID
