@@ -123,3 +123,26 @@ def test_a_batch_refuses_a_plan_of_other_lengths_and_writes_nothing(cuda):
     batch.lengths = [0, 0]
     assert torch.equal(batch.step(*args, [3, 1]), got)
     batch.check()
+
+
+@pytest.mark.parametrize("dim,dtype", [(128, BF), (80, HF)])
+def test_append_in_a_graph(cuda, dim, dtype):
+    """The append as it is captured in a decode step, replayed with new tokens."""
+    args = args_of(cuda, 9, dim, dim // 2, False)
+    q, k = rows(cuda, 9, 4, dim, dtype, 0, 1), rows(cuda, 9, 2, dim, dtype, 0, 2)
+    v, w = rows(cuda, 9, 2, dim, dtype, 0, 3), torch.ones(dim, dtype=dtype, device=cuda)
+    slots = torch.arange(9, device=cuda)
+    cache = torch.zeros(4, 2, 16, 2 * dim, dtype=dtype, device=cuda)
+    call = lambda pool: rotary.append_rotated(  # noqa: E731
+        pool, slots, k, v, query=q, q_weight=w, k_weight=w, **args)
+    call(cache)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call(cache)
+    for x in (q, k, v):
+        x.copy_(x.roll(1, 0))
+    slots.copy_(torch.randperm(64, device=cuda)[:9])
+    cache.zero_()
+    graph.replay()
+    other = torch.zeros_like(cache)
+    assert torch.equal(out, call(other)) and torch.equal(cache, other) and other.any()
