@@ -145,3 +145,39 @@ def test_a_part_of_little_weight_keeps_what_is_not_finite(cuda, hq, hk, d, dtype
     assert not torch.isfinite(got[..., 9]).any()
     rest = torch.arange(d, device=cuda) != 9
     assert torch.isfinite(got[..., rest]).all()
+
+
+@pytest.mark.parametrize("name,block,scattered", [("drafts", 16, 1.0), ("wide ragged", 5, 0.0),
+                                                  ("wide ragged", 16, 0.2), ("decode", 1, 0.0)])
+@pytest.mark.parametrize("scale", [None, -0.1])
+def test_values_in_relocated_slots_and_in_a_graph(cuda, name, block, scattered, scale):
+    """Keys copied row by row, negative scales, and calls that follow each
+    other closely."""
+    s, lens = batch(cuda, 8, 2, 128, BF, *LAYOUTS[name], block=block, scattered=scattered)
+    plan = plan_of(s, lens)
+    hidden = [slot for _, slot in last_own_slots(s, lens)]
+    seen = int(s["prefix_slots"][77])
+    sees = torch.zeros(s["query"].shape[0], dtype=torch.bool, device=cuda)
+    sees[[token for token, _ in last_own_slots(s, lens)]] = True
+
+    def fill(value):
+        for slot in hidden:
+            s["cache"][slot // block, :, slot % block, 128 + 40] = value
+        s["cache"][seen // block, :, seen % block, 128 + 90] = value
+
+    args = s["query"], s["cache"], s["prefix_slots"], s["suffix_slots"]
+    fill(0.0)
+    want = plan(*args, scale=scale)
+    want[..., 90] = NAN
+    want[sees, :, 40] = NAN
+    fill(NAN)
+    got = plan(*args, scale=scale)
+    torch.testing.assert_close(got, want, rtol=0, atol=0, equal_nan=True)
+    outs = [torch.empty_like(got) for _ in range(3)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for out in outs:
+            plan(*args, scale=scale, out=out)
+    graph.replay()
+    for out in outs:
+        torch.testing.assert_close(out, want, rtol=0, atol=0, equal_nan=True)
