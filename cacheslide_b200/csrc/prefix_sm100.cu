@@ -8,7 +8,9 @@
 //   S = Q K^T (tcgen05, TMEM),  P = 2^(S c - m),  O += P V (P from TMEM)
 // with the running maximum m and sum of each row in float32 registers; P is
 // rounded to the inputs' type, as the tensor unit takes it, and the sum is
-// taken before that.  Every row sees the whole prefix range; of the own keys
+// taken before that: outputs lie 2.3e-3 (bf16) and 2.9e-4 (fp16) from float64,
+// 1.7e-3 and 2.1e-4 of which their own rounding is; the rest of P as a second
+// 16-bit operand would be another product as large as P V.  Every row sees the whole prefix range; of the own keys
 // it sees [lo, hi) of its token, which covers the causal limit, requests of
 // other lengths in the same tile and padding alike.
 //
@@ -20,14 +22,16 @@
 // sidecar, range ends, which are filled with zeros, and pools no tensor map
 // describes).
 //
-// Measured with 32/8 heads of 128, bf16 (64/8 and fp16 where said):
-//   64 questions of 64 tokens behind 5120 keys: 318 us, 1.09 PFLOP/s; bound by
-//     the softmax warps: 64 keys of two row tiles take 1950 clocks, of which
-//     the exponentials, at 8 clocks a warp instruction, take 1024;
+// Measured with 32/8 heads of 128, bf16 (64/8 and fp16 where said), twelve
+// calls in a row:
+//   64 questions of 64 tokens behind 5120 keys: 336 us, 1.03 PFLOP/s (368 us,
+//     0.94 PFLOP/s, sustained, under the power limit); bound by the softmax
+//     warps: 64 keys of two row tiles take 1950 clocks, of which the
+//     exponentials, at 8 clocks a warp instruction, take 1024;
 //   8 decodes behind 65536 keys (64/8): 54 us, 5.0 TB/s;
-//   32 sessions of 4 drafts, own keys up to 16K (fp16): 212 us, 5.2 TB/s (242
+//   32 sessions of 4 drafts, own keys up to 16K (fp16): 216 us, 5.1 TB/s (245
 //     us sustained: the power limit takes the clock to 1.55 GHz);
-//   64 decodes behind 5120 keys: 23.5 us, of which 9 are the block's eight
+//   64 decodes behind 5120 keys: 24 us, of which 9 are the block's eight
 //     steps of 1500 clocks and 5 the join: latency.
 #include <cuda.h>
 #include <math.h>

@@ -302,11 +302,16 @@ __global__ void __launch_bounds__(kRowWarps * 32)
 //
 // Forward, 32768 tokens of 32/8 heads of 128, bf16: 115 us, 5.8 TB/s (113 with
 // the row sums' shuffles left out: the rest is HBM and the warps' starts);
-// append of 65536 tokens of 64/8 heads without norms, fp16: 401 us, 6.8 TB/s,
-// HBM.  Two groups a task: 143 and 497 us; eight: 144 and 412 us; two warps a
-// block: 117 and 400 us; eight: 122 and 434 us.  Registers for nine blocks an SM
-// are 3 us better than the 60 that the compiler takes, for ten 15 us worse;
-// in float32 (103 us for 16384 tokens) nine are 2 us worse.
+// append of 65536 tokens of 64/8 heads without norms, fp16: 400 us, 6.8 TB/s, in
+// a short run, 428 us, 6.35 TB/s, sustained (a plain copy: 6.46): HBM.  Two
+// groups a task: 143 and 497 us; eight: 144 and 412 us; two warps a block: 117
+// and 400 us; eight: 122 and 434 us.  Registers for nine blocks an SM against
+// the 60 that the compiler takes (32768 tokens of 32/8 heads of 128): forward
+// 114 to 117 us in bf16, 118 to 129 interleaved, 113 to 118 in fp16; append 139
+// to 146, 139 to 148, 133 to 141; the 56 registers that this leaves cost most
+// bf16 forms 4 to 24 bytes of spills, which these times include.  For ten
+// blocks the forward was 15 us worse; in float32 (103 us for 16384 tokens)
+// nine are 2 us worse.
 constexpr int kP = 4;        // pairs a lane
 constexpr int kGroups = 4;   // row groups a task
 constexpr int kVecWarps = 4;

@@ -169,8 +169,9 @@ def qk_norm_rope(query: Tensor, key: Tensor, positions: Tensor, cos: Tensor, sin
     elements (2i, 2i + 1) instead of (i, i + rotary_dim / 2).  Gradients flow
     to query, key and the weights (cos and sin are constants); there is no
     forward-mode derivative, and a tensor that carries a tangent is refused.
-    A position outside the tables makes its rows NaN and sets ``ST_POS_RANGE``
-    in ``status`` (read it after the stream has drained)."""
+    A position outside the tables makes the rotated elements of its rows NaN
+    and sets ``ST_POS_RANGE`` in ``status`` (read it after the stream has
+    drained)."""
     query, key = _rows("query", query), _rows("key", key)
     # (a level of dual numbers is rarely open, and this test of it is free)
     if getattr(forward_ad, "_current_level", 0) >= 0 and any(
@@ -209,7 +210,9 @@ def append_rotated(kv: Tensor | NativePagedKV | N.PagedKV, slots: Tensor, key: T
     Norms, rotation and tables as in ``qk_norm_rope``.  Slot -1 marks padding
     and is not written; any other slot outside the pool (and sidecar), or a
     position outside the tables, is skipped and sets ``ST_SLOT_RANGE`` /
-    ``ST_POS_RANGE`` in ``status``.  Distinct tokens need distinct slots.  The
+    ``ST_POS_RANGE`` in ``status`` (a query there has NaN in its rotated
+    elements).  Distinct tokens need distinct slots: equal ones leave a mix of
+    their rows.  The
     slot map's guards are the caller's: this writes where it is told, as a
     model runner's cache write does.  A serving operator: it has no derivative
     of either mode, and what it returns is a constant to autograd."""

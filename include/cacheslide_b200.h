@@ -690,8 +690,8 @@ CS_API int cs_qk_norm_rope_grad(const cs_rotary_params* p, const void* q_dy,
  * with the queries of the same tokens normed and rotated into p->q_out in the
  * same launch (q_heads = 0: none).  p->k_out is not used.  Slot -1 is padding
  * (not written); any other slot outside the arena, or a position outside the
- * table, is skipped and sets its status bit.  Of equal slots in one call any
- * one row is kept.
+ * table, is skipped and sets its status bit.  Slots of one call are distinct:
+ * equal ones leave a mix of their rows.
  */
 CS_API int cs_kv_append_rotated(const cs_rotary_params* p, const cs_paged_kv* kv,
                                 const int64_t* slots, const void* v,
