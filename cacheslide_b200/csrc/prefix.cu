@@ -393,7 +393,7 @@ int make_plan(const cs_prefix_shape* s, cs_prefix_plan_info* info, int32_t* word
     const int sms = num_sms();
     // two blocks of 128 rows an SM, which read their keys for each row tile,
     // or one of 256 rows; both costs as measured with 32/8 heads of 128 (of 64 a
-    // step costs less, which only the byte terms below know)
+    // step costs less, which only the byte terms know)
     const double narrow = best_cut(
         l, Cost{2 * sms, 1.75, 5.0},
         [&](int64_t most) { return split_units(l, most * kPrefixTile); }, -1, items);

@@ -36,6 +36,17 @@ def _lens(name: str, values: Sequence[int]) -> tuple[ctypes.Array, int]:
     return (ctypes.c_int64 * max(1, len(values)))(*values), sum(values)
 
 
+def _overlap(a: Tensor, b: Tensor) -> bool:
+    """Whether the spans of memory from first to last element meet."""
+    def span(t: Tensor) -> tuple[int, int]:
+        first = t.data_ptr()
+        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+        return first, first + (last + 1) * t.element_size()
+
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
 class SharedPrefixAttention:
     """The attention of one batch layout; call it once per layer.
 
@@ -99,7 +110,8 @@ class SharedPrefixAttention:
         """``query`` [token, q_head, dim] of all requests in order;
         ``prefix_slots`` / ``suffix_slots`` (int64) the pool slots of the
         groups' prefixes and the requests' own keys, concatenated.  ``scale``
-        defaults to ``dim ** -0.5``.  Returns [token, q_head, dim] (and, with
+        defaults to ``dim ** -0.5``.  ``out`` may overlap ``query`` (which is then
+        copied first).  Returns [token, q_head, dim] (and, with
         ``return_lse``, the float32 log of each row's softmax denominator,
         -inf for a row that sees no key, whose output is zero).
 
@@ -134,6 +146,9 @@ class SharedPrefixAttention:
         elif out.shape != shape or out.dtype is not self.dtype or out.get_device() != index \
                 or out.stride(2) != 1:
             raise ValueError("out must match query, with a contiguous last dimension")
+        elif _overlap(out, query):  # blocks read queries after others have written
+            query = query.clone(memory_format=torch.contiguous_format)
+            qs = query.stride()
         os = out.stride()
         lse = torch.empty(shape[:2], dtype=torch.float32, device=device) if return_lse else None
         p = N.PrefixParams(

@@ -205,7 +205,7 @@ def append_rotated(kv: Tensor | NativePagedKV | N.PagedKV, slots: Tensor, key: T
     """Write new tokens to the paged pool: the record of ``slots[t]`` (int64)
     becomes the normed, rotated ``key[t]`` and ``value[t]``; with ``query``,
     its normed, rotated rows are returned (into ``out`` when given, which may
-    be ``query`` itself).
+    be ``query`` itself and else overlaps no input).
 
     Norms, rotation and tables as in ``qk_norm_rope``.  Slot -1 marks padding
     and is not written; any other slot outside the pool (and sidecar), or a

@@ -747,7 +747,8 @@ typedef struct {
   const int64_t* suffix_slots; /* [n_suffix] of all requests              */
   int32_t q_heads;
   double scale;
-  void* out;      /* [tokens, q_heads, head_dim], dtype of the pool       */
+  void* out;      /* [tokens, q_heads, head_dim], dtype of the pool;
+                     overlaps no input                                    */
   int64_t o_stride_tok, o_stride_head;
   float* lse;     /* [tokens, q_heads] natural logarithm, or NULL         */
   int32_t* status;

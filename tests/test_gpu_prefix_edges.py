@@ -181,3 +181,22 @@ def test_values_in_relocated_slots_and_in_a_graph(cuda, name, block, scattered, 
     graph.replay()
     for out in outs:
         torch.testing.assert_close(out, want, rtol=0, atol=0, equal_nan=True)
+
+
+@pytest.mark.parametrize("name", ["decode", "questions", "wide batch"])
+@pytest.mark.parametrize("hq,hk,d,dtype", HEADS + [(4, 2, 80, BF)])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_output_over_the_queries(cuda, name, hq, hk, d, dtype, shift):
+    """``out`` may be the queries' own memory, or overlap it, whatever the
+    values hold."""
+    s, lens = batch(cuda, hq, hk, d, dtype, *LAYOUTS[name])
+    plan = plan_of(s, lens)
+    for _, slot in last_own_slots(s, lens):
+        s["cache"][slot // 16, :, slot % 16, d + 3] = NAN
+    rest = s["cache"], s["prefix_slots"], s["suffix_slots"]
+    want = plan(s["query"], *rest)
+    tokens = s["query"].shape[0]
+    both = torch.zeros(tokens + shift, hq, d, dtype=dtype, device=cuda)
+    query, out = both[:tokens].copy_(s["query"]), both[shift:]
+    assert plan(query, *rest, out=out).data_ptr() == out.data_ptr()
+    torch.testing.assert_close(out, want, rtol=0, atol=0, equal_nan=True)
