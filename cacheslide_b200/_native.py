@@ -28,6 +28,7 @@ ST_PATH_INCR = 1 << 6
 ST_PATH_GAP = 1 << 7
 ST_TIMEOUT = 1 << 8
 ST_INPUT_NONFINITE = 1 << 9
+ST_CAPACITY = 1 << 10
 
 POS_CONTEXTUAL, POS_FIXED, POS_TABLE, POS_CHUNK = 0, 1, 2, 3
 LAUNCH_OVERLAP_PREV = 1
@@ -185,7 +186,42 @@ class PrefixParams(ctypes.Structure):
     ]
 
 
+class StepMapsParams(ctypes.Structure):
+    """cs_step_maps_params: block tables and slot maps of a step."""
+    _fields_ = [
+        ("lengths", _p), ("new_tokens", _p), ("requests", _i32), ("block_size", _i32),
+        ("num_blocks", _i64), ("tables", _p), ("table_stride", _i64), ("table_width", _i32),
+        ("position_offset", _i32), ("free_blocks", _p), ("free_count", _p), ("free_left", _p),
+        ("tokens", _i64), ("keys", _i64), ("starts", _p), ("positions", _p), ("slots", _p),
+        ("key_starts", _p), ("key_slots", _p), ("status", _p),
+    ]
+
+
+class KV4Pool(ctypes.Structure):
+    """cs_kv4_pool: a paged pool held in 4 bits."""
+    _fields_ = [
+        ("storage", _p), ("num_blocks", _i64), ("kv_heads", _i32), ("block_size", _i32),
+        ("head_dim", _i32), ("group", _i32), ("dtype", _i32),
+    ]
+
+
+class KV4AttnParams(ctypes.Structure):
+    """cs_kv4_attn_params: attention over a pool held in 4 bits."""
+    _fields_ = [
+        ("q", _p), ("q_stride_tok", _i64), ("q_stride_head", _i64), ("tokens", _i64),
+        ("q_heads", _i32), ("requests", _i32), ("pool", KV4Pool), ("tables", _p),
+        ("table_stride", _i64), ("table_width", _i32), ("zero_rest", _i32), ("lengths", _p),
+        ("starts", _p), ("scale", _f64), ("out", _p), ("o_stride_tok", _i64),
+        ("o_stride_head", _i64), ("lse", _p), ("status", _p),
+    ]
+
+
 _SIGNATURES = {
+    "cs_step_maps": [ctypes.POINTER(StepMapsParams), _p],
+    "cs_kv4_append": [ctypes.POINTER(KV4Pool), _p, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p],
+    "cs_kv4_gather": [ctypes.POINTER(KV4Pool), _p, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p],
+    "cs_kv4_attn_workspace": [ctypes.POINTER(KV4AttnParams)],
+    "cs_kv4_attn": [ctypes.POINTER(KV4AttnParams), _p, _p],
     "cs_prefix_plan": [ctypes.POINTER(PrefixShape), ctypes.POINTER(PrefixPlanInfo), _p, _i64],
     "cs_prefix_attn": [ctypes.POINTER(PrefixParams), ctypes.POINTER(PrefixPlanInfo), _p, _p, _p],
     "cs_qk_norm_rope": [ctypes.POINTER(RotaryParams), _p],
@@ -244,6 +280,7 @@ _SIGNATURES = {
 _RESTYPES = {"cs_build_info": ctypes.c_char_p, "cs_abi_version": _i32,
              "cs_cope_attn_decode_workspace": _i64,
              "cs_qk_norm_rope_grad_workspace": _i64,
+             "cs_kv4_attn_workspace": _i64,
              "cs_cope_attn_decode_batch_workspace": _i64}
 
 EXPORTED = tuple(_SIGNATURES)

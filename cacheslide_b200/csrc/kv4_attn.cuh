@@ -1,0 +1,130 @@
+// What the two attention kernels of the 4-bit pool share: their dependent
+// launch, how a row's result is written, and the join of partial results.
+#pragma once
+
+#include "kv4.cuh"
+#include "sm100.cuh"
+
+namespace cs {
+
+// the kernel for few query rows a KV head (kv4_decode.cu) and the one for many
+// (kv4_sm100.cu), for `workers` blocks
+int kv4_decode_blocks(int rows);  // an SM's, with so many rows a block
+int kv4_decode(const Attn4& a, const cs_kv4_pool& pool, int rows, int workers,
+               cudaStream_t stream);
+// workers and query rows a block for a call: the workspace's shape
+struct Plan4 {
+  int workers, rows;
+  bool wide;
+};
+Plan4 plan4(const cs_kv4_attn_params& p);
+
+// A launch that may start beside the end of the grid before it on the stream;
+// the kernel waits for that grid (griddepcontrol.wait) before it reads or
+// writes global memory.
+template <typename K, typename... A>
+int launch_dependent(K kernel, int blocks, int threads, int smem, cudaStream_t stream, A... args) {
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3(blocks);
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = stream;
+  c.attrs = at;
+  c.numAttrs = 1;
+  if (cudaLaunchKernelEx(&c, kernel, args...) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return CS_ERR_CUDA;
+  }
+  return CS_OK;
+}
+
+constexpr float kLn2 = 0.6931471805599453f;
+
+// four neighbouring elements from `c` on of row `row` of a (request, KV head)
+template <typename T>
+__device__ __forceinline__ void write4(const Attn4& a, int start, int row, int h, int c, float4 y) {
+  const int tok = row / a.G;
+  char* to = a.out + (int64_t)(start + tok) * a.ot +
+             (int64_t)(h * a.G + (row - tok * a.G)) * a.oh + 2 * c;
+  const uint32_t lo = Pack2<T>::pack(y.x, y.y), hi = Pack2<T>::pack(y.z, y.w);
+  if (a.vec_out) {
+    *reinterpret_cast<uint2*>(to) = make_uint2(lo, hi);
+  } else {
+    uint16_t* e = reinterpret_cast<uint16_t*>(to);
+    e[0] = (uint16_t)lo, e[1] = (uint16_t)(lo >> 16);
+    e[2] = (uint16_t)hi, e[3] = (uint16_t)(hi >> 16);
+  }
+}
+__device__ __forceinline__ void write_lse(const Attn4& a, int start, int row, int h, float lse2) {
+  if (a.lse == nullptr) return;
+  const int tok = row / a.G;
+  a.lse[(int64_t)(start + tok) * a.hq + h * a.G + (row - tok * a.G)] = lse2 * kLn2;
+}
+
+// rows outside every request, when they are to be zeros
+template <typename T, int D>
+__device__ __forceinline__ void zero_rest(const Attn4& a) {
+  if (!a.zero_rest || a.starts == nullptr) return;
+  const int64_t first = a.starts[0], end = a.starts[a.requests];
+  const int64_t n = a.tokens * a.hq * (D / 4);
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t token = i / (a.hq * (D / 4));
+    if (token >= first && token < end) continue;
+    const int at = (int)(i - token * (a.hq * (D / 4)));
+    const int head = at / (D / 4), c = 4 * (at % (D / 4));
+    uint16_t* to = reinterpret_cast<uint16_t*>(a.out + token * a.ot + head * a.oh) + c;
+    to[0] = to[1] = to[2] = to[3] = 0;
+    if (a.lse && c == 0) a.lse[token * a.hq + head] = -INFINITY;
+  }
+}
+
+// o = sum_c w_c o_c / sum_c w_c with w_c = 2^(lse_c - max) over the blocks that
+// shared a row tile, in their order; a block a tile that was cut, a warp a row.
+template <typename T, int D, int RT>
+__global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ Attn4 a) {
+  constexpr int E = D / 32;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 j = a.joins[blockIdx.x];
+  if (j.x < 0) return;
+  const int lane = threadIdx.x & 31, first = blockIdx.x, parts = j.w - first + 1;
+  const Request4 r = request4(a, j.x);
+  const int row0 = j.y * RT, rows = min(RT, r.n * a.G - row0), h = j.z >> 1;
+  auto place = [&](int i) { return i == 0 ? 2ll * first + (j.z & 1) : 2ll * (first + i); };
+  for (int row = threadIdx.x >> 5; row < rows; row += 4) {
+    float top = -INFINITY, sum = 0.f, o[E];
+    for (int i = lane; i < parts; i += 32)
+      top = fmaxf(top, a.part_lse[place(i) * RT + row]);
+    top = warp_max(top);
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) {
+      const float l = a.part_lse[place(i) * RT + row];
+      // one below 2^-126 of the largest is that, not 0: what is not finite stays
+      const float w = l == -INFINITY ? 0.f : (l != l ? l : fmaxf(ex2(l - top), 0x1p-126f));
+      const float* p = a.part_o + (place(i) * RT + row) * D + lane * E;
+      sum += w;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = w == 0.f ? o[e] : fmaf(w, p[e], o[e]);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int tok = (row0 + row) / a.G, head = h * a.G + (row0 + row - tok * a.G);
+    T* out = reinterpret_cast<T*>(a.out + (int64_t)(r.start + tok) * a.ot + (int64_t)head * a.oh);
+#pragma unroll
+    for (int e = 0; e < E; ++e) out[lane * E + e] = Elem<T>::from_f(o[e] * inv);
+    if (lane == 0)
+      write_lse(a, r.start, row0 + row, h, sum == 0.f ? -INFINITY : top + log2f(sum));
+  }
+}
+
+template <typename T, int D, int RT>
+int launch_join(const Attn4& a, int workers, cudaStream_t stream) {
+  return launch_dependent(kv4_join_kernel<T, D, RT>, workers, 128, 0, stream, a);
+}
+
+}  // namespace cs

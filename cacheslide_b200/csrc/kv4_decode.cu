@@ -1,0 +1,556 @@
+// Attention over the 4-bit pool for few query rows a KV head (decodes, drafted
+// tokens), and the join of its partial results.
+//
+// Per unit of 16 keys a warp forms
+//   S^T = K Q^T  (16 keys x 8 rows),  P = 2^(S c - m),  O^T += V^T P^T
+// on mma.sync.  The codes go into the products as they are: a 4-bit code in the
+// low bits of a 16-bit number is that number of the smallest fp16 subnormals,
+// exactly (and 16 times that, four bits up), so a word of eight codes becomes
+// four operand registers with a shift and four ANDs, with no bias to take off
+// and no rounding.  Scale and lowest value of a group enter in float32,
+//   q.k = scale (q.c) + low sum(q),   p v = (p scale) c + p low,
+// where p scale is rounded to fp16 for the product (what that rounding takes is
+// added back in float32 times 8, the codes' middle, so that it acts on the
+// value and not on the code).  Queries are fp16 too, each row scaled by a power
+// of two so that its largest element lies in [2^13, 2^14): 16-bit inputs of
+// either type keep every bit down to 2^-27 of that.
+//
+// Bound by HBM (136 to 160 bytes a key and head): the products are far too
+// small for tcgen05, whose operands would have to be written to shared memory
+// in 16 bits first, four times the bytes that come in -- at full bandwidth 87
+// bytes a clock and SM written and as many read again, of 128.  Here the codes
+// go from a ring of raw units (one bulk copy each) to registers.
+#include <math.h>
+
+#include <type_traits>
+
+#include "kv4.cuh"
+#include "kv4_attn.cuh"
+#include "sm100.cuh"
+
+namespace cs {
+namespace {
+
+constexpr int kWarps = 4, kThreads = 32 * kWarps;
+constexpr int kStep = kUnit * kWarps;  // keys of a block's step, a unit a warp
+constexpr int kLeast = 4;              // steps a block takes at least
+constexpr float kLazy = 8.f;  // O is rescaled when a maximum grew by more than 2^8
+constexpr float kUp = 6.f;    // the largest weight is 2^6: fp16 reaches 2^-20 of it unrounded
+
+template <int D, int NG, int NT>
+struct Ring {
+  static constexpr int RT = 8 * NT;  // query rows of a block
+  static constexpr int kStages = 4;
+  static constexpr int kBlocks = NT == 1 ? 4 : 3;  // an SM's
+  static constexpr int oBars = kWarps * kStages * Unit4<D, NG>::kBytes;
+  static constexpr int oSums = oBars + kWarps * kStages * 8;
+  static constexpr int oMax = oSums + (kThreads + 1 + kWarps) * 8 + 8;
+  static constexpr int oOut = (oMax + 2 * kWarps * RT * 4 + 15) / 16 * 16;
+  static constexpr int kBytes = oOut + kWarps * RT * D * 4;
+};
+
+// D += A B, 16 x 8 x 16 in fp16 with float32 sums
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                      uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes,
+                                          uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void arrive_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 2^e for e in [-126, 127]
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
+
+template <int N> struct Words;
+template <> struct Words<4> {
+  static __device__ __forceinline__ void load(uint32_t (&w)[4], const char* p) {
+    const uint4 x = *reinterpret_cast<const uint4*>(p);
+    w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+  }
+};
+template <> struct Words<2> {
+  static __device__ __forceinline__ void load(uint32_t (&w)[2], const char* p) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    w[0] = x.x, w[1] = x.y;
+  }
+};
+template <> struct Words<1> {
+  static __device__ __forceinline__ void load(uint32_t (&w)[1], const char* p) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+};
+
+constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
+
+template <typename T, int D, int NG, int NT>
+__global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
+    kv4_decode_kernel(const __grid_constant__ Attn4 a) {
+  using U = Unit4<D, NG>;
+  using R = Ring<D, NG, NT>;
+  using Share = Share4<R::RT, kStep>;
+  constexpr int W = U::W, RT = R::RT, S = R::kStages, WG = W / NG;  // words a group
+  extern __shared__ __align__(128) char smem[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, t = lane & 3;
+  char* ring = smem + warp * S * U::kBytes;
+  const uint32_t ring_at = smem_u32(ring), bars = smem_u32(smem + R::oBars) + warp * S * 8;
+  float* maxima = reinterpret_cast<float*>(smem + R::oMax);       // [warp][row]
+  float* sums = maxima + kWarps * RT;                             // [warp][row]
+  float* outs = reinterpret_cast<float*>(smem + R::oOut);         // [warp][row][dim]
+  if (lane == 0) {
+    for (int s = 0; s < S; ++s) mbar_init(bars + 8 * s, 1);
+    mbar_init_fence();
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  Share work;
+  work.template find<kThreads>(a, blockIdx.x, gridDim.x, kLeast,
+                               reinterpret_cast<int64_t*>(smem + R::oSums));
+  zero_rest<T, D>(a);
+  int issued = 0, taken = 0;  // units of this warp's ring
+  bool late = false, bad_block = false;
+  int which = 0;  // of this block's partial results
+  int4 join = make_int4(-1, 0, 0, 0);
+
+  while (work.todo > 0) {
+    const Request4 r = work.r;
+    const int all_steps = Share::steps(r, a.G, work.tile);
+    const int s0 = work.step;
+    const int s1 = (int)min((int64_t)all_steps, s0 + work.todo);
+    const int row0 = work.tile * RT, rows = r.n * a.G;
+    const int h = work.head;
+    // ------------------------------------------------------------ keys ahead
+    // this warp's units are s0 * kWarps + warp, then kWarps further; beyond the
+    // tile's last key none is fetched
+    const int seen = max(0, r.len - r.n + Share::last_token(r, a.G, work.tile) + 1);
+    const int unit0 = s0 * kWarps + warp;
+    const int last_unit = min(s1 * kWarps, (seen + kUnit - 1) / kUnit);
+    const int count = unit0 < last_unit ? (last_unit - unit0 + kWarps - 1) / kWarps : 0;
+    const int32_t* table = a.tables + work.request * a.table_stride;
+    int ids = 0, ids_at = 0;  // blocks of units ids_at .. ids_at + 31 of this warp
+    auto load_ids = [&](int from) {
+      const int u = unit0 + kWarps * (from + lane);
+      ids_at = from;
+      ids = from + lane < count ? table[u / a.pool.units] : 0;
+    };
+    int sent = 0;
+    auto send = [&] {  // the whole warp
+      if (sent - ids_at == 32) load_ids(sent);
+      const int id = __shfl_sync(~0u, ids, sent - ids_at);
+      const int u = unit0 + kWarps * sent, st = issued % S;
+      const uint32_t bar = bars + 8 * st, dst = ring_at + st * U::kBytes;
+      if (id >= 0 && id < a.pool.num_blocks) {
+        if (lane == 0) {
+          arrive_expect(bar, U::kBytes);
+          bulk_copy(dst, a.pool.unit(id, h, u % a.pool.units), U::kBytes, bar);
+        }
+      } else {  // zero codes, scales and lows: zero keys and values
+        bad_block = true;
+        for (int i = lane; i < U::kBytes / 16; i += 32)
+          *reinterpret_cast<uint4*>(ring + st * U::kBytes + 16 * i) = make_uint4(0, 0, 0, 0);
+        fence_async_smem();  // before a later copy into this place
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+      }
+      ++issued;
+      ++sent;
+    };
+    load_ids(0);
+    for (int i = 0; i < S && i < count; ++i) send();
+
+    // --------------------------------------------------------------- queries
+    uint32_t qf[NT][2 * W][2];      // operand fragments: word w, then its upper half
+    float qs[NT][NG][2];            // scale log2e sum(q) of rows 2t, 2t + 1
+    float qm[NT][2];                // scale log2e over the row's power of two
+    int limit[NT][2];               // the newest key these rows see
+    int low_limit = INT32_MAX;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = row0 + 8 * nt + g;
+      const bool ok = row < rows;
+      const int tok = ok ? row / a.G : 0;
+      const char* p = a.q + (int64_t)(r.start + tok) * a.qt +
+                      (int64_t)(h * a.G + (ok ? row - tok * a.G : 0)) * a.qh;
+      float f[W][8];
+      float top = 0.f, sum[NG];
+#pragma unroll
+      for (int k = 0; k < NG; ++k) sum[k] = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        uint32_t x[4];
+        const char* e = p + 2 * (32 * w + 8 * t);
+        if (!ok) {
+          x[0] = x[1] = x[2] = x[3] = 0u;
+        } else if (a.vec_q) {
+          Words<4>::load(x, e);
+        } else {
+          const uint16_t* u = reinterpret_cast<const uint16_t*>(e);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = u[2 * i] | (uint32_t)u[2 * i + 1] << 16;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 y = pair_of<T>(x[i]);
+          f[w][2 * i] = y.x, f[w][2 * i + 1] = y.y;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          top = fmaxf(top, fabsf(f[w][i]));
+          sum[w / WG] += f[w][i];
+        }
+      }
+      top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+#pragma unroll
+      for (int k = 0; k < NG; ++k) {
+        sum[k] += __shfl_xor_sync(~0u, sum[k], 1);
+        sum[k] += __shfl_xor_sync(~0u, sum[k], 2);
+      }
+      const int e = min(100, max(-100, (int)(__float_as_uint(top) >> 23) - 127));
+      const float up = pow2(13 - e);
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {  // elements 2k, 2k + 4 and (sixteenths) 2k + 1, 2k + 5
+          qf[nt][2 * w + k][0] = Pack2<__half>::pack(f[w][2 * k] * up, f[w][2 * k + 4] * up);
+          qf[nt][2 * w + k][1] = Pack2<__half>::pack(f[w][2 * k + 1] * (up * 0.0625f),
+                                                     f[w][2 * k + 5] * (up * 0.0625f));
+        }
+      }
+      // the codes are 2^-24 of theirs, the queries up of theirs
+      const float back = pow2(11 + e) * a.scale2;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int from = 4 * (2 * t + k), m = row0 + 8 * nt + 2 * t + k;
+        qm[nt][k] = __shfl_sync(~0u, back, from);
+#pragma unroll
+        for (int w = 0; w < NG; ++w)
+          qs[nt][w][k] = __shfl_sync(~0u, sum[w], from) * a.scale2;
+        limit[nt][k] = m < rows ? r.len - r.n + m / a.G : INT32_MAX;  // no row: of no matter
+        low_limit = min(low_limit, limit[nt][k]);
+      }
+    }
+    low_limit = __reduce_min_sync(~0u, low_limit);
+
+    // ------------------------------------------------------------------ keys
+    float o[NT][2 * W][4];
+    float mref[NT][2], lsum[NT][2], lows[NT][NG][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < 2 * W; ++i) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[nt][i][k] = 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        mref[nt][k] = -INFINITY, lsum[nt][k] = 0.f;
+#pragma unroll
+        for (int w = 0; w < NG; ++w) lows[nt][w][k] = 0.f;
+      }
+    }
+    for (int i = 0; i < count; ++i) {
+      const int st = taken % S;
+      if (!late && !mbar_try(bars + 8 * st, (taken / S) & 1)) {
+        const long long begin = clock64();
+        while (!mbar_try(bars + 8 * st, (taken / S) & 1))
+          if (clock64() - begin > kWaitCycles) {
+            late = true;
+            break;
+          }
+      }
+      late = __any_sync(~0u, late);
+      const char* unit = ring + st * U::kBytes;
+      ++taken;
+      float x[NT][4];  // (key g, rows 2t and 2t + 1), (key g + 8, the same)
+      {
+        uint32_t ka[W], kb[W];
+        Words<W>::load(ka, unit + g * U::kRow + 4 * W * t);
+        Words<W>::load(kb, unit + (g + 8) * U::kRow + 4 * W * t);
+        uint32_t pa[NG], pb[NG];
+        Words<NG>::load(pa, unit + U::oKp + 4 * NG * g);
+        Words<NG>::load(pb, unit + U::oKp + 4 * NG * (g + 8));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) x[nt][k] = 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < NG; ++k) {
+          float acc[NT][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[nt][c] = 0.f;
+          }
+#pragma unroll
+          for (int w = k * WG; w < (k + 1) * WG; ++w) {
+            const uint32_t ya = ka[w] >> 8, yb = kb[w] >> 8;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma16(acc[nt], ka[w] & kLow, kb[w] & kLow, ka[w] & kHigh, kb[w] & kHigh,
+                    qf[nt][2 * w][0], qf[nt][2 * w][1]);
+              mma16(acc[nt], ya & kLow, yb & kLow, ya & kHigh, yb & kHigh, qf[nt][2 * w + 1][0],
+                    qf[nt][2 * w + 1][1]);
+            }
+          }
+          const float2 fa = pair_of<T>(pa[k]), fb = pair_of<T>(pb[k]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const float2 f = c < 2 ? fa : fb;
+              x[nt][c] = fmaf(f.y, qs[nt][k][c & 1],
+                              fmaf(f.x * qm[nt][c & 1], acc[nt][c], x[nt][c]));
+            }
+          }
+        }
+      }
+      const int key0 = kUnit * (unit0 + kWarps * i) + g;
+      uint32_t shown = ~0u;  // bit 4 nt + c: the row sees the key
+      if (key0 - g + kUnit - 1 > low_limit) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (key0 + (c < 2 ? 0 : 8) > limit[nt][c & 1]) {
+              x[nt][c] = -INFINITY;
+              shown &= ~(1u << (4 * nt + c));
+            }
+        }
+      }
+      uint32_t va[NG], vb[NG];
+      Words<NG>::load(va, unit + U::oVp + 4 * NG * g);
+      Words<NG>::load(vb, unit + U::oVp + 4 * NG * (g + 8));
+      float2 fa[NG], fb[NG];
+      float sa = 0.f, sb = 0.f;
+#pragma unroll
+      for (int k = 0; k < NG; ++k) {
+        fa[k] = pair_of<T>(va[k]), fb[k] = pair_of<T>(vb[k]);
+        sa = fmaxf(sa, fa[k].x), sb = fmaxf(sb, fb[k].x);
+      }
+      // log2 of the largest scale: p scale is what has to fit fp16
+      const float la = fminf(fmaxf(lg2(sa), -100.f), 100.f);
+      const float lb = fminf(fmaxf(lg2(sb), -100.f), 100.f);
+      bool grow = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          grow |= x[nt][c] + (c < 2 ? la : lb) > mref[nt][c & 1] + kLazy;
+      }
+      if (__any_sync(~0u, grow)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float m = fmaxf(x[nt][k] + la, x[nt][k + 2] + lb);
+            m = fmaxf(m, __shfl_xor_sync(~0u, m, 4));
+            m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
+            m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
+            m = fmaxf(m, mref[nt][k]);
+            const float f = m == mref[nt][k] ? 1.f : ex2(mref[nt][k] - m);
+            mref[nt][k] = m;
+            lsum[nt][k] *= f;
+#pragma unroll
+            for (int w = 0; w < NG; ++w) lows[nt][w][k] *= f;
+#pragma unroll
+            for (int w = 0; w < 2 * W; ++w) o[nt][w][k] *= f, o[nt][w][k + 2] *= f;
+          }
+        }
+      }
+      // ------------------------------------------------------------- weights
+      uint32_t pf[NT][NG][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float p[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float m = mref[nt][c & 1];
+          p[c] = ex2(x[nt][c] - ((m == -INFINITY ? 0.f : m) - kUp));
+          lsum[nt][c & 1] += p[c];
+        }
+#pragma unroll
+        for (int k = 0; k < NG; ++k) {
+          float w[4], low[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const float2 f = c < 2 ? fa[k] : fb[k];
+            w[c] = p[c] * f.x;
+            low[c] = p[c] * fmaf(8.f, f.x, f.y);
+            // a scale that is not finite reaches no row that does not see its key
+            if (!(shown >> (4 * nt + c) & 1u)) w[c] = low[c] = 0.f;
+          }
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t y = Pack2<__half>::pack(w[2 * half], w[2 * half + 1]);
+            const float2 z = pair_of<__half>(y);
+            lows[nt][k][0] += fmaf(-8.f, z.x, low[2 * half]);
+            lows[nt][k][1] += fmaf(-8.f, z.y, low[2 * half + 1]);
+            pf[nt][k][half] = transposed(y);
+          }
+        }
+      }
+      // -------------------------------------------------------------- values
+      {
+        uint32_t v[4][(W + 1) / 2];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          Words<W / 2>::load(v[k], unit + U::oV + (2 * t + (k & 1) + 4 * (k & 2)) * U::kRow +
+                                       2 * W * g);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const uint32_t sel = w & 1 ? 0x7632u : 0x5410u;
+          const uint32_t xa = __byte_perm(v[0][w / 2], v[1][w / 2], sel);
+          const uint32_t xb = __byte_perm(v[2][w / 2], v[3][w / 2], sel);
+          const uint32_t ya = xa >> 8, yb = xb >> 8;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma16(o[nt][2 * w], xa & kLow, xa & kHigh, xb & kLow, xb & kHigh, pf[nt][w / WG][0],
+                  pf[nt][w / WG][1]);
+            mma16(o[nt][2 * w + 1], ya & kLow, ya & kHigh, yb & kLow, yb & kHigh,
+                  pf[nt][w / WG][0], pf[nt][w / WG][1]);
+          }
+        }
+      }
+      __syncwarp();  // the unit has been read
+      if (sent < count) send();
+    }
+
+    // --------------------------------------------------- the warps' results
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int s = 4; s < 32; s <<= 1) {
+          lsum[nt][k] += __shfl_xor_sync(~0u, lsum[nt][k], s);
+#pragma unroll
+          for (int w = 0; w < NG; ++w) lows[nt][w][k] += __shfl_xor_sync(~0u, lows[nt][w][k], s);
+        }
+        if (g == 0) {
+          maxima[warp * RT + 8 * nt + 2 * t + k] = mref[nt][k];
+          sums[warp * RT + 8 * nt + 2 * t + k] = lsum[nt][k];
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int row = 8 * nt + 2 * t + k;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, maxima[w * RT + row]);
+        const float f = mref[nt][k] == top ? 1.f : ex2(mref[nt][k] - top);
+        float* to = outs + (warp * RT + row) * D + 4 * g;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const float z = lows[nt][w / WG][k];
+          float4 y;
+          y.x = fmaf(o[nt][2 * w][k], 0x1p24f, z) * f;
+          y.y = fmaf(o[nt][2 * w][k + 2], 0x1p20f, z) * f;
+          y.z = fmaf(o[nt][2 * w + 1][k], 0x1p24f, z) * f;
+          y.w = fmaf(o[nt][2 * w + 1][k + 2], 0x1p20f, z) * f;
+          *reinterpret_cast<float4*>(to + 32 * w) = y;
+        }
+      }
+    }
+    __syncthreads();
+    const bool whole = s0 == 0 && s1 == all_steps;
+    const int64_t part = 2ll * blockIdx.x + which;
+    for (int i = tid; i < RT * (D / 4); i += kThreads) {
+      const int row = i / (D / 4), c = 4 * (i % (D / 4));
+      if (row0 + row >= rows) break;
+      float top = -INFINITY, l = 0.f;
+      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, maxima[w * RT + row]);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float m = maxima[w * RT + row];
+        l += sums[w * RT + row] * (m == top ? 1.f : ex2(m - top));
+        const float4 z = *reinterpret_cast<const float4*>(outs + (w * RT + row) * D + c);
+        y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float lse2 = l == 0.f ? -INFINITY
+                                  : (top == -INFINITY ? 0.f : top) - kUp + log2f(l);
+      y.x *= inv, y.y *= inv, y.z *= inv, y.w *= inv;
+      if (whole) {
+        write4<T>(a, r.start, row0 + row, h, c, y);
+        if (c == 0) write_lse(a, r.start, row0 + row, h, lse2);
+      } else {
+        *reinterpret_cast<float4*>(a.part_o + (part * RT + row) * D + c) = y;
+        if (c == 0) a.part_lse[part * RT + row] = lse2;
+      }
+    }
+    if (!whole) {
+      if (s0 == 0)  // the first of the tile's blocks has them joined
+        join = make_int4(work.request, work.tile, 2 * h + which,
+                         blockIdx.x + (int)((all_steps - s1 + work.per - 1) / work.per));
+      which = 1;
+    }
+    __syncthreads();  // the results have been read
+    work.todo -= s1 - s0;
+    if (work.todo > 0) work.next(a);
+  }
+  if (tid == 0) a.joins[blockIdx.x] = join;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (bad_block && lane == 0) report(a.status, CS_ST_SLOT_RANGE);
+  if (late) {  // copies of this block are to have landed before it ends
+    for (int s = taken - S < 0 ? 0 : taken - S; s < taken; ++s) {
+      const long long begin = clock64();
+      while (!mbar_try(bars + 8 * (s % S), (s / S) & 1) && clock64() - begin < kWaitCycles) {
+      }
+    }
+    if (lane == 0) report(a.status, CS_ST_TIMEOUT);
+  }
+}
+
+template <typename T, int D, int NG, int NT>
+int launch_decode(const Attn4& a, int workers, cudaStream_t stream) {
+  constexpr auto kernel = kv4_decode_kernel<T, D, NG, NT>;
+  constexpr int kBytes = Ring<D, NG, NT>::kBytes;
+  if (!allow_smem<kernel>(kBytes)) return CS_ERR_CUDA;
+  if (const int rc = launch_dependent(kernel, workers, kThreads, kBytes, stream, a)) return rc;
+  return launch_join<T, D, 8 * NT>(a, workers, stream);
+}
+
+}  // namespace
+
+int kv4_decode_blocks(int rows) { return rows <= 8 ? 4 : 3; }
+
+int kv4_decode(const Attn4& a, const cs_kv4_pool& pool, int rows, int workers,
+               cudaStream_t stream) {
+  return by_pool4(pool, [&](auto* t, auto d, auto g) -> int {
+    using T = std::remove_pointer_t<decltype(t)>;
+    constexpr int D = decltype(d)::value, NG = decltype(g)::value;
+    return rows <= 8 ? launch_decode<T, D, NG, 1>(a, workers, stream)
+                     : launch_decode<T, D, NG, 2>(a, workers, stream);
+  });
+}
+
+}  // namespace cs

@@ -100,7 +100,12 @@ class SharedPrefixAttention:
                 break
             capacity = self.info.words
         N.check(rc, "cs_prefix_plan")
-        self.words = words[:self.info.words].to(self.device)
+        # behind the plan's words, in the same copy: query_lens, then suffix_lens, for
+        # what makes the step's slots on the device
+        lens = torch.tensor([*query_lens, *suffix_lens], dtype=torch.int32)
+        both = torch.cat((words[:self.info.words], lens)).to(self.device)
+        self.words = both[:self.info.words]
+        self.device_lens = both[self.info.words:].view(2, len(self.query_lens))
         self._stream = N.stream_of(self.device) if self.device.type == "cuda" else None
 
     def __call__(self, query: Tensor, kv: Tensor | NativePagedKV | N.PagedKV,

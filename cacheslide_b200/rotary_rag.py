@@ -27,6 +27,7 @@ from torch import Tensor
 from . import _native as N
 from .prefix import SharedPrefixAttention
 from .rotary import append_rotated, rotary_tables
+from .tables import step_maps
 
 
 class RotaryRagBatch:
@@ -57,6 +58,7 @@ class RotaryRagBatch:
         self.pool, self.q_heads, self.requests, self.max_own = pool, q_heads, requests, max_own
         self.prefix_slots = slots[:prefix_length].contiguous()
         self.own_slots = slots[per_prefix * block:].view(requests, -1)
+        self.own_table = table[per_prefix:].view(requests, -1).int()
         self.lengths = [0] * requests
         self.cos, self.sin = rotary_tables(prefix_length + max_own,
                                            width // 2 if rotary_dim is None else rotary_dim,
@@ -65,18 +67,33 @@ class RotaryRagBatch:
         self.interleaved = interleaved
         self.status = N.Status(pool.device)
 
-    def _append(self, slots: Tensor, key: Tensor, value: Tensor, positions: Tensor,
-                query: Tensor | None = None) -> Tensor | None:
-        return append_rotated(self.pool, slots, key, value, positions, self.cos, self.sin,
-                              query=query, q_weight=self.q_weight if query is not None else None,
-                              k_weight=self.k_weight, eps=self.eps,
-                              interleaved=self.interleaved, status=self.status)
+    def _append(self, key: Tensor, value: Tensor, query: Tensor | None = None,
+                plan: SharedPrefixAttention | None = None) -> tuple[Tensor | None, Tensor | None]:
+        """The prefix's keys and values into its slots or, with a plan, a step's
+        new ones into their requests': the slots and positions of the new tokens
+        and the slots of every own key come from the plan's lengths on the
+        device.  Returns the turned queries and the own keys' slots."""
+        own = q_weight = None
+        if plan is None:
+            slots = self.prefix_slots
+            positions = torch.arange(key.shape[0], device=self.pool.device)
+        else:
+            blocks, _, block, _ = self.pool.shape
+            new_lens, own_lens = plan.device_lens
+            maps = step_maps(own_lens, new_lens, self.own_table, block, blocks,
+                             tokens=plan.tokens, keys=plan.suffix_keys,
+                             offset=self.prefix_slots.numel(), status=self.status)
+            slots, positions, q_weight = maps.slots, maps.positions, self.q_weight
+            own = slots[:0] if maps.key_slots is None else maps.key_slots
+        turned = append_rotated(self.pool, slots, key, value, positions, self.cos, self.sin,
+                                query=query, q_weight=q_weight, k_weight=self.k_weight,
+                                eps=self.eps, interleaved=self.interleaved, status=self.status)
+        return turned, own
 
     def write_prefix(self, key: Tensor, value: Tensor) -> None:
         """The prefix's keys (as projected, neither normed nor rotated) and
         values, [prefix, kv_head, dim]."""
-        self._append(self.prefix_slots, key, value,
-                     torch.arange(key.shape[0], device=self.pool.device))
+        self._append(key, value)
 
     def _own(self, query_lens: Sequence[int]) -> list[int]:
         """Each request's own keys after a step."""
@@ -111,17 +128,9 @@ class RotaryRagBatch:
                 raise ValueError("the plan is of other lengths, heads or pool than this step")
         if query.shape != plan.shape or query.dtype is not plan.dtype:
             raise ValueError(f"query must be {plan.dtype} {tuple(plan.shape)}")
-        first = self.prefix_slots.numel()
-        device = self.pool.device
-        spans = [(b, have, have + new)
-                 for b, (have, new) in enumerate(zip(self.lengths, query_lens, strict=True))]
-        new = torch.cat([self.own_slots[b, lo:hi] for b, lo, hi in spans])
-        own = torch.cat([self.own_slots[b, :hi] for b, _, hi in spans])
-        positions = torch.cat([torch.arange(first + lo, first + hi, device=device)
-                               for _, lo, hi in spans])
-        turned = self._append(new, key, value, positions, query)
+        turned, own = self._append(key, value, query, plan)
         out = plan(turned, self.pool, self.prefix_slots, own, status=self.status)
-        self.lengths = [hi for _, _, hi in spans]
+        self.lengths = list(plan.suffix_lens)
         return out
 
     def check(self) -> None:

@@ -55,6 +55,7 @@ typedef enum { CS_F32 = 0, CS_F16 = 1, CS_BF16 = 2, CS_F64 = 3 } cs_dtype;
 #define CS_ST_PATH_GAP (1 << 7)       /* strict path: drop > coordinate gap    */
 #define CS_ST_TIMEOUT (1 << 8)        /* a bounded device wait expired         */
 #define CS_ST_INPUT_NONFINITE (1 << 9)/* non-finite query/key/value element    */
+#define CS_ST_CAPACITY (1 << 10)      /* a step needs more places than there are    */
 
 /* ------------------------------------------------------- paged KV arena */
 /*
@@ -764,6 +765,138 @@ typedef struct {
  */
 CS_API int cs_prefix_attn(const cs_prefix_params* p, const cs_prefix_plan_info* info,
                           const int32_t* plan, void* workspace, void* stream);
+
+/* --------------------------------- block tables and slot maps of a step */
+/*
+ * A step's slots from the requests' lengths on the device.  Request b holds
+ * lengths[b] tokens after the step, the newest new_tokens[b] of which the step
+ * brings; position p lies in slot tables[b][p / block_size] * block_size +
+ * p % block_size.  Row i of request b's new tokens is row starts[b] + i,
+ * starts[b] = sum_{a<b} new_tokens[a]; its position is lengths[b] -
+ * new_tokens[b] + i (+ position_offset in `positions`).
+ *
+ * With `free_blocks` the blocks that a request needs beyond those of its first
+ * lengths - new_tokens positions come from the top of that stack, requests in
+ * order, and are written into `tables`; *free_left is what remains of
+ * *free_count.  Without it the tables are complete.
+ *
+ * All or nothing: a negative length, more new tokens than tokens, a row of the
+ * tables too short, more rows than `tokens`, more keys than `keys`, or too few
+ * free blocks sets CS_ST_CAPACITY; then every slot is -1, every position and
+ * start 0, the tables stay and *free_left = *free_count.  A block id outside
+ * [0, num_blocks) gives slot -1 and sets CS_ST_SLOT_RANGE.  Rows past the last
+ * request's have slot -1 and position 0, key slots past the last key -1.
+ * One launch; calls with equal inputs write equal outputs.
+ */
+typedef struct {
+  const int32_t* lengths;    /* [requests] */
+  const int32_t* new_tokens; /* [requests] */
+  int32_t requests, block_size;
+  int64_t num_blocks;
+  int32_t* tables;           /* [requests][table_width], table_stride apart */
+  int64_t table_stride;
+  int32_t table_width;
+  int32_t position_offset;
+  const int32_t* free_blocks; /* or NULL */
+  const int32_t* free_count;  /* [1] */
+  int32_t* free_left;         /* [1], not free_count */
+  int64_t tokens, keys;       /* places in the arrays below */
+  int32_t* starts;            /* [requests + 1] */
+  int64_t* positions;         /* [tokens] */
+  int64_t* slots;             /* [tokens] */
+  int64_t* key_starts;        /* [requests + 1], or NULL */
+  int64_t* key_slots;         /* [keys]: slots of every request's positions 0 .. length - 1 */
+  int32_t* status;
+} cs_step_maps_params;
+
+CS_API int cs_step_maps(const cs_step_maps_params* p, void* stream);
+
+/* ----------------------------------------------- paged cache in 4 bits */
+/*
+ * A pool of records in 4 bits, bytes [num_blocks][kv_heads][block_size / 16]
+ * [unit], contiguous and 16-byte aligned.  A group of `group` elements of one
+ * token's head stands for the values low + scale * code, code in 0 .. 15, with
+ *   low = min x,  scale = (max x - min x) / 15 in float32, rounded to `dtype`
+ *   (to the next lower number where low + 15 scale would overflow it),
+ *   code = (x - low) / scale, to the nearest, ties to even, at most 15
+ *   (0 where scale is 0);
+ * a group with an infinity or a NaN has low = scale = NaN.  A unit is 16
+ * tokens of a head: their key codes, head_dim / 2 bytes a token; their value
+ * codes; the (scale, low) pairs of their keys' groups [16][head_dim / group],
+ * then of their values': 16 head_dim + 128 head_dim / group bytes.  With
+ * W = head_dim / 32, bits 4 i .. 4 i + 3 of 32-bit word t W + w of a token's key
+ * codes hold element 32 w + 8 t + i; of 16-bit half-word g W + w of its value
+ * codes, element 32 w + 4 g + i.  head_dim 64 or 128, group 32, 64 or 128 and
+ * at most head_dim, block_size a multiple of 16, dtype float16 or bfloat16.
+ */
+typedef struct {
+  void* storage;
+  int64_t num_blocks;
+  int32_t kv_heads, block_size, head_dim, group;
+  int32_t dtype; /* of the rows that go in and come out, and of the pairs */
+} cs_kv4_pool;
+
+/*
+ * The record of slots[t] becomes k[t], v[t] in 4 bits ([n, kv_heads, head_dim],
+ * strides in elements, 1 in a row).  Slot -1 is padding (not written); any
+ * other slot outside the pool is skipped and sets CS_ST_SLOT_RANGE.  Slots of
+ * one call are distinct: equal ones leave a mix of their rows.
+ */
+CS_API int cs_kv4_append(const cs_kv4_pool* pool, const int64_t* slots, int64_t n, const void* k,
+                         int64_t k_stride_tok, int64_t k_stride_head, const void* v,
+                         int64_t v_stride_tok, int64_t v_stride_head, int32_t* status,
+                         void* stream);
+
+/*
+ * The values that the records of slots[t] stand for, rounded to `dtype`.  A row
+ * of slot -1 is zeros; of any other slot outside the pool too, which sets
+ * CS_ST_SLOT_RANGE.
+ */
+CS_API int cs_kv4_gather(const cs_kv4_pool* pool, const int64_t* slots, int64_t n, void* k,
+                         int64_t k_stride_tok, int64_t k_stride_head, void* v,
+                         int64_t v_stride_tok, int64_t v_stride_head, int32_t* status,
+                         void* stream);
+
+/*
+ * Attention over such a pool.  Request b's keys are positions 0 .. lengths[b]
+ * - 1 through its row of `tables`; its query rows are starts[b] .. starts[b +
+ * 1] - 1 (row b alone without `starts`), the newest of its positions: row i of
+ * n sees keys 0 .. lengths[b] - n + i.
+ *   o = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q.k_j - max),
+ *   lse = max + log(sum_j p_j);  o = 0 and lse = -inf where nothing is seen.
+ * lengths, starts and tables are read on the device: a captured call follows
+ * them.  Lengths past the tables' width end there and set CS_ST_CAPACITY, as
+ * do starts that are negative, fall or pass `tokens` (their rows are left out).
+ * A block id outside the pool sets CS_ST_SLOT_RANGE and its keys
+ * and values are zeros.  Rows before starts[0] or from starts[requests] on are
+ * left as they were, or zeroed (lse -inf) with `zero_rest`.
+ */
+typedef struct {
+  const void* q; /* [tokens, q_heads, head_dim], dtype of the pool */
+  int64_t q_stride_tok, q_stride_head;
+  int64_t tokens;
+  int32_t q_heads, requests;
+  cs_kv4_pool pool;
+  const int32_t* tables;
+  int64_t table_stride;
+  int32_t table_width;
+  int32_t zero_rest;
+  const int32_t* lengths; /* [requests] */
+  const int32_t* starts;  /* [requests + 1], or NULL: tokens == requests */
+  double scale;
+  void* out; /* [tokens, q_heads, head_dim]; overlaps no input */
+  int64_t o_stride_tok, o_stride_head;
+  float* lse; /* [tokens, q_heads], or NULL */
+  int32_t* status;
+} cs_kv4_attn_params;
+
+/*
+ * `workspace` holds cs_kv4_attn_workspace(p) bytes, 16-byte aligned, that
+ * nothing else uses meanwhile; its content does not matter and its size does
+ * not depend on the lengths.
+ */
+CS_API int64_t cs_kv4_attn_workspace(const cs_kv4_attn_params* p);
+CS_API int cs_kv4_attn(const cs_kv4_attn_params* p, void* workspace, void* stream);
 
 /* library identification: compile-time arch string and ABI version */
 CS_API const char* cs_build_info(void);

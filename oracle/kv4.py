@@ -1,0 +1,179 @@
+"""Float64 restatement of the 4-bit pool: records, attention, slot maps.
+
+    low = min x,  scale = (max x - min x) / 15,  code = (x - low) / scale, nearest
+    value = low + scale code
+    o = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q.k_j - max)
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+UNIT = 16
+
+
+def params(x: torch.Tensor, group: int):
+    """Scale and lowest value of each group of 16-bit x, in its type."""
+    y = x.float().unflatten(-1, (-1, group))
+    low, high = y.amin(-1), y.amax(-1)
+    # the quotient in float32 (its exact range in float64), then 16 bits
+    scale = ((high.double() - low.double()) / 15).float().to(x.dtype)
+    top = {torch.float16: 65520.0, torch.bfloat16: 3.3961775292304957e38}[x.dtype]
+    over = low.double() + 15 * scale.double() >= top
+    down = (scale.view(torch.int16) - 1).view(x.dtype)
+    scale = torch.where(over, down, scale)
+    bad = ~torch.isfinite(y).all(-1)
+    nan = torch.full_like(scale, math.nan)
+    return torch.where(bad, nan, scale), torch.where(bad, nan, low.to(x.dtype))
+
+
+def codes(x: torch.Tensor, scale: torch.Tensor, low: torch.Tensor, group: int) -> torch.Tensor:
+    y = x.double().unflatten(-1, (-1, group))
+    s, z = scale.double()[..., None], low.double()[..., None]
+    c = torch.where(s > 0, (y - z) / torch.where(s > 0, s, 1.0), 0.0).round().clamp(0, 15)
+    return c.flatten(-2).to(torch.uint8)
+
+
+def values(c: torch.Tensor, scale: torch.Tensor, low: torch.Tensor, group: int) -> torch.Tensor:
+    y = c.double().unflatten(-1, (-1, group))
+    return (y * scale.double()[..., None] + low.double()[..., None]).flatten(-2)
+
+
+def order(dim: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """The nibble of a row's codes that holds element e, of keys and of values."""
+    e, w = torch.arange(dim), dim // 32
+    return ((e % 32 // 8 * w + e // 32) * 8 + e % 8, (e % 32 // 4 * w + e // 32) * 4 + e % 4)
+
+
+def record(k, v, group):
+    """Codes and pairs of one token's heads as rows of bytes: key codes, value
+    codes, key pairs, value pairs (each [..., bytes])."""
+    out = []
+    for x, at in zip((k, v), order(k.shape[-1])):
+        s, z = params(x, group)
+        c = codes(x, s, z, group)
+        n = torch.empty_like(c)
+        n[..., at] = c
+        out += [n[..., 0::2] | n[..., 1::2] << 4,
+                torch.stack((s, z), -1).flatten(-2).contiguous().view(torch.uint8)]
+    return out[0], out[2], out[1], out[3]
+
+
+def write(storage, slots, k, v, group):
+    """The records of the slots in `storage` [block, head, units, unit bytes]."""
+    d = k.shape[-1]
+    row, pair = d // 2, 4 * (d // group)
+    bs = storage.shape[2] * UNIT
+    parts = record(k, v, group)
+    for t, slot in enumerate(slots.tolist()):
+        if not 0 <= slot < storage.shape[0] * bs:
+            continue
+        unit = storage[slot // bs, :, slot % bs // UNIT]
+        r, base = slot % UNIT, 0
+        for x, size in zip(parts, (row, row, pair, pair)):
+            unit[:, base + r * size: base + (r + 1) * size] = x[t]
+            base += UNIT * size
+
+
+def read(storage, slots, dim, group, dtype):
+    """float64 keys and values, and float64 scales of the values' elements."""
+    row, pair = dim // 2, 4 * (dim // group)
+    bs = storage.shape[2] * UNIT
+    unit = storage[slots // bs, :, slots % bs // UNIT]  # [n, heads, bytes]
+    r = (slots % UNIT)[:, None, None]
+    out, base = [], 0
+    for size in (row, row, pair, pair):
+        at = base + r * size + torch.arange(size)
+        out.append(unit.gather(2, at.expand(-1, unit.shape[1], -1)))
+        base += UNIT * size
+    res = []
+    for raw, pairs, at in ((out[0], out[2], order(dim)[0]), (out[1], out[3], order(dim)[1])):
+        n = torch.stack((raw & 15, raw >> 4), -1).flatten(-2)[..., at]
+        p = pairs.contiguous().view(dtype).unflatten(-1, (-1, 2)).double()
+        res += [values(n, p[..., 0], p[..., 1], group), p[..., 0].repeat_interleave(group, -1)]
+    return res
+
+
+def attention(q, storage, table, length, n, group, scale, wide):
+    """One request: out [n, hq, d] and lse [n, hq] in float64, and how far a
+    kernel may be from them before its output is rounded.
+
+    Score error: float32 sums of products of codes (15 s + |low| bounds what is
+    added up) and, of the kernel for many rows, keys rounded to fp16.  Weights
+    are rounded to fp16 (half a step, 2^-11) against the codes' middle (8 s) or,
+    of the kernel for many rows, against the value, which is rounded too;
+    weights below fp16's normal numbers (2^-20 of a unit's largest at least) by
+    2^-25 of 2^6."""
+    hk, d = storage.shape[1], q.shape[-1]
+    bs = storage.shape[2] * UNIT
+    at = torch.arange(max(0, length))
+    slots = table[at // bs].long() * bs + at % bs
+    k, ks, v, vs = read(storage, slots, d, group, q.dtype)
+    g = q.shape[1] // hk
+    x = q.double().view(n, hk, g, d)
+    z = torch.einsum("nhgd,khd->nhgk", x, k) * scale
+    size = torch.einsum("nhgd,khd->nhgk", x.abs(), k.abs() + 16 * ks) * abs(scale)
+    dz = size * (2.0 ** -21 + (2.0 ** -11 if wide else 0.0)) + 2.0 ** -21 * (1 + z.abs())
+    seen = at <= (length - n + torch.arange(n))[:, None]
+    seen = seen[:, None, None]
+    z = torch.where(seen, z, -math.inf)
+    if length <= 0:
+        return (torch.zeros(n, hk * g, d, dtype=torch.float64),
+                torch.full((n, hk * g), -math.inf, dtype=torch.float64),
+                torch.zeros(n, hk * g, d, dtype=torch.float64))
+    top = z.amax(-1, keepdim=True)
+    top = torch.where(top == -math.inf, 0.0, top)
+    p = torch.where(seen, (z - top).exp(), 0.0)
+    total = p.sum(-1, keepdim=True)
+    some = total != 0  # (true of NaN)
+    w = torch.where(some, p / torch.where(some, total, 1.0), 0.0)
+
+    def mix(weights, rows):  # a key that is not seen has no part, not even NaN
+        rows = rows[None, :, :, None, :].expand(n, -1, -1, 1, -1)
+        y = weights.permute(0, 3, 1, 2)[..., None] * rows
+        return torch.where(seen.permute(0, 3, 1, 2)[..., None], y, 0.0).sum(1)
+
+    o = mix(w, v)
+    middle = v.abs() if wide else 8 * vs
+    err = mix(w * dz.nan_to_num(), v.abs()) * 2 + 2.0 ** -11 * mix(w, middle) * (2 if wide else 1)
+    err = err + 2.0 ** -24 * vs.nan_to_num().amax() * 16
+    lse = torch.where(some, top + torch.where(some, total, 1.0).log(), -math.inf)[..., 0]
+    return o.reshape(n, hk * g, d), lse.reshape(n, hk * g), err.reshape(n, hk * g, d)
+
+
+def step_maps(lengths, new, tables, block, blocks, tokens, keys=0, offset=0, free=None,
+              free_count=0):
+    """Lists, token by token; the tables are changed in place.  None: refused."""
+    tables = [list(t) for t in tables]
+    width = len(tables[0]) if tables else 0
+    if any(n < 0 or a < n or -(-a // block) > width for a, n in zip(lengths, new)) or \
+            sum(new) > tokens or keys and sum(lengths) > keys:
+        return None
+    left = free_count
+    if free is not None:
+        for b, (a, n) in enumerate(zip(lengths, new)):
+            for j in range(-(-(a - n) // block), -(-a // block)):
+                if left == 0:
+                    return None
+                left -= 1
+                tables[b][j] = free[left]
+
+    def slot(b, p):
+        at = tables[b][p // block]
+        return at * block + p % block if 0 <= at < blocks else -1
+
+    starts, key_starts, positions, slots, key_slots = [0], [0], [], [], []
+    for b, (a, n) in enumerate(zip(lengths, new)):
+        starts.append(starts[-1] + n)
+        key_starts.append(key_starts[-1] + a)
+        positions += [offset + p for p in range(a - n, a)]
+        slots += [slot(b, p) for p in range(a - n, a)]
+        if keys:
+            key_slots += [slot(b, p) for p in range(a)]
+    positions += [0] * (tokens - len(positions))
+    slots += [-1] * (tokens - len(slots))
+    key_slots += [-1] * (keys - len(key_slots))
+    return dict(tables=tables, starts=starts, key_starts=key_starts, positions=positions,
+                slots=slots, key_slots=key_slots, left=left)
