@@ -264,9 +264,14 @@ Plan4 plan4(const cs_kv4_attn_params& p) {
   const int64_t g = p.q_heads / p.pool.kv_heads;
   // query rows of a KV head an average request has
   const int64_t rows = p.requests > 0 ? p.tokens * g / p.requests : 0;
-  plan.wide = false;
-  plan.rows = rows <= 8 ? 8 : 16;
-  plan.workers = num_sms() * kv4_decode_blocks(plan.rows);
+  plan.wide = rows > 16;
+  if (plan.wide) {
+    plan.rows = rows > 128 ? 256 : 128;
+    plan.workers = num_sms() * (plan.rows == 256 ? 1 : 2);
+  } else {
+    plan.rows = rows <= 8 ? 8 : 16;
+    plan.workers = num_sms() * kv4_decode_blocks(plan.rows);
+  }
   return plan;
 }
 
@@ -330,6 +335,8 @@ extern "C" int cs_kv4_attn(const cs_kv4_attn_params* p, void* workspace, void* s
   a.vec_q = aligned(p->q, a.qt, a.qh, 16);
   a.vec_out = aligned(p->out, a.ot, a.oh, 8);
   a.zero_rest = p->zero_rest;
-  a.scale2 = (float)p->scale * 1.4426950408889634f;
-  return kv4_decode(a, p->pool, plan.rows, plan.workers, as_stream(stream));
+  a.flip = p->scale < 0.0 ? 0x80008000u : 0u;
+  a.scale2 = fabsf((float)p->scale) * 1.4426950408889634f;
+  return (plan.wide ? kv4_wide : kv4_decode)(a, p->pool, plan.rows, plan.workers,
+                                             as_stream(stream));
 }

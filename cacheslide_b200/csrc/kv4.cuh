@@ -126,7 +126,8 @@ struct Attn4 {
   int requests, hq, G;
   int vec_q, vec_out;  // 16-byte loads, 8-byte stores fit
   int zero_rest;
-  float scale2;  // scale * log2 e
+  uint32_t flip;  // the scale is negative: the queries' signs
+  float scale2;   // |scale| * log2 e
 };
 
 struct Request4 {

@@ -12,6 +12,7 @@ namespace cs {
 int kv4_decode_blocks(int rows);  // an SM's, with so many rows a block
 int kv4_decode(const Attn4& a, const cs_kv4_pool& pool, int rows, int workers,
                cudaStream_t stream);
+int kv4_wide(const Attn4& a, const cs_kv4_pool& pool, int rows, int workers, cudaStream_t stream);
 // workers and query rows a block for a call: the workspace's shape
 struct Plan4 {
   int workers, rows;
@@ -23,12 +24,12 @@ Plan4 plan4(const cs_kv4_attn_params& p);
 // the kernel waits for that grid (griddepcontrol.wait) before it reads or
 // writes global memory.
 template <typename K, typename... A>
-int launch_dependent(K kernel, int blocks, int threads, int smem, cudaStream_t stream, A... args) {
+int launch_dependent(K kernel, dim3 blocks, int threads, int smem, cudaStream_t stream, A... args) {
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t c = {};
-  c.gridDim = dim3(blocks);
+  c.gridDim = blocks;
   c.blockDim = dim3(threads);
   c.dynamicSmemBytes = smem;
   c.stream = stream;
@@ -41,6 +42,7 @@ int launch_dependent(K kernel, int blocks, int threads, int smem, cudaStream_t s
   return CS_OK;
 }
 
+constexpr int kJoinRows = 16;
 constexpr float kLn2 = 0.6931471805599453f;
 
 // four neighbouring elements from `c` on of row `row` of a (request, KV head)
@@ -83,7 +85,8 @@ __device__ __forceinline__ void zero_rest(const Attn4& a) {
 }
 
 // o = sum_c w_c o_c / sum_c w_c with w_c = 2^(lse_c - max) over the blocks that
-// shared a row tile, in their order; a block a tile that was cut, a warp a row.
+// shared a row tile, in their order; a block 16 rows of a tile that was cut, a
+// warp a row.
 template <typename T, int D, int RT>
 __global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ Attn4 a) {
   constexpr int E = D / 32;
@@ -93,9 +96,10 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ A
   if (j.x < 0) return;
   const int lane = threadIdx.x & 31, first = blockIdx.x, parts = j.w - first + 1;
   const Request4 r = request4(a, j.x);
-  const int row0 = j.y * RT, rows = min(RT, r.n * a.G - row0), h = j.z >> 1;
+  const int row0 = j.y * RT, h = j.z >> 1;
+  const int rows = min(min(RT, r.n * a.G - row0), (int)blockIdx.y * kJoinRows + kJoinRows);
   auto place = [&](int i) { return i == 0 ? 2ll * first + (j.z & 1) : 2ll * (first + i); };
-  for (int row = threadIdx.x >> 5; row < rows; row += 4) {
+  for (int row = blockIdx.y * kJoinRows + (threadIdx.x >> 5); row < rows; row += 4) {
     float top = -INFINITY, sum = 0.f, o[E];
     for (int i = lane; i < parts; i += 32)
       top = fmaxf(top, a.part_lse[place(i) * RT + row]);
@@ -124,7 +128,8 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ A
 
 template <typename T, int D, int RT>
 int launch_join(const Attn4& a, int workers, cudaStream_t stream) {
-  return launch_dependent(kv4_join_kernel<T, D, RT>, workers, 128, 0, stream, a);
+  return launch_dependent(kv4_join_kernel<T, D, RT>,
+                          dim3(workers, (RT + kJoinRows - 1) / kJoinRows), 128, 0, stream, a);
 }
 
 }  // namespace cs

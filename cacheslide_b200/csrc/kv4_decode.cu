@@ -32,17 +32,21 @@ namespace cs {
 namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
-constexpr int kStep = kUnit * kWarps;  // keys of a block's step, a unit a warp
 constexpr int kLeast = 4;              // steps a block takes at least
-constexpr float kLazy = 8.f;  // O is rescaled when a maximum grew by more than 2^8
-constexpr float kUp = 6.f;    // the largest weight is 2^6: fp16 reaches 2^-20 of it unrounded
+constexpr float kUp = 6.f;  // a new largest p scale is 2^6: fp16's normal numbers reach 2^-20 of it
+constexpr float kTooLarge = 0x1p14f;  // it may grow to 2^14 before O is rescaled
+constexpr float kLowest = -3e38f;     // below every score, and finite
 
 template <int D, int NG, int NT>
 struct Ring {
   static constexpr int RT = 8 * NT;  // query rows of a block
-  static constexpr int kStages = 4;
+  // units a warp takes at once: two have twice the independent work and one
+  // wait, copy and vote between them
+  static constexpr int E = NT == 1 ? 2 : 1;
+  static constexpr int kStep = kUnit * kWarps * E;  // keys of a block's step
+  static constexpr int kStages = 4 / E;             // of E units
   static constexpr int kBlocks = NT == 1 ? 4 : 3;  // an SM's
-  static constexpr int oBars = kWarps * kStages * Unit4<D, NG>::kBytes;
+  static constexpr int oBars = kWarps * kStages * E * Unit4<D, NG>::kBytes;
   static constexpr int oSums = oBars + kWarps * kStages * 8;
   static constexpr int oMax = oSums + (kThreads + 1 + kWarps) * 8 + 8;
   static constexpr int oOut = (oMax + 2 * kWarps * RT * 4 + 15) / 16 * 16;
@@ -57,6 +61,15 @@ __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, u
       "{%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// D = A B
+__device__ __forceinline__ void mma16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                            uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   uint32_t y;
@@ -80,6 +93,7 @@ __device__ __forceinline__ float lg2(float x) {
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 // 2^e for e in [-126, 127]
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
 
@@ -109,18 +123,19 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
     kv4_decode_kernel(const __grid_constant__ Attn4 a) {
   using U = Unit4<D, NG>;
   using R = Ring<D, NG, NT>;
-  using Share = Share4<R::RT, kStep>;
-  constexpr int W = U::W, RT = R::RT, S = R::kStages, WG = W / NG;  // words a group
+  using Share = Share4<R::RT, R::kStep>;
+  constexpr int W = U::W, RT = R::RT, S = R::kStages, E = R::E, WG = W / NG;  // words a group
+  constexpr int kStage = E * U::kBytes;
   extern __shared__ __align__(128) char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
-  char* ring = smem + warp * S * U::kBytes;
-  const uint32_t ring_at = smem_u32(ring), bars = smem_u32(smem + R::oBars) + warp * S * 8;
+  char* ring = smem + warp * S * kStage;
+  const uint32_t bars = smem_u32(smem + R::oBars) + warp * S * 8;
   float* maxima = reinterpret_cast<float*>(smem + R::oMax);       // [warp][row]
   float* sums = maxima + kWarps * RT;                             // [warp][row]
   float* outs = reinterpret_cast<float*>(smem + R::oOut);         // [warp][row][dim]
   if (lane == 0) {
-    for (int s = 0; s < S; ++s) mbar_init(bars + 8 * s, 1);
+    for (int s = 0; s < S; ++s) mbar_init(bars + 8 * s, E);
     mbar_init_fence();
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -141,48 +156,57 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
     const int row0 = work.tile * RT, rows = r.n * a.G;
     const int h = work.head;
     // ------------------------------------------------------------ keys ahead
-    // this warp's units are s0 * kWarps + warp, then kWarps further; beyond the
-    // tile's last key none is fetched
+    // this warp's pass i takes units unit_of(i, 0 .. E - 1); beyond the tile's
+    // last key none is fetched
     const int seen = max(0, r.len - r.n + Share::last_token(r, a.G, work.tile) + 1);
-    const int unit0 = s0 * kWarps + warp;
-    const int last_unit = min(s1 * kWarps, (seen + kUnit - 1) / kUnit);
-    const int count = unit0 < last_unit ? (last_unit - unit0 + kWarps - 1) / kWarps : 0;
+    const int units = (seen + kUnit - 1) / kUnit;
+    auto unit_of = [&](int i, int e) { return ((s0 + i) * kWarps + warp) * E + e; };
+    int count = s1 - s0;  // passes
+    if (count > 0 && unit_of(count - 1, 0) >= units) --count;
     const int32_t* table = a.tables + work.request * a.table_stride;
-    int ids = 0, ids_at = 0;  // blocks of units ids_at .. ids_at + 31 of this warp
-    auto load_ids = [&](int from) {
-      const int u = unit0 + kWarps * (from + lane);
-      ids_at = from;
-      ids = from + lane < count ? table[u / a.pool.units] : 0;
+    // this lane's unit of passes batch .. batch + 32 / E - 1: -1 none, 0 no block
+    int64_t from = -1;
+    int batch = 0, sent = 0;
+    auto find_units = [&] {
+      batch = sent;
+      const int u = unit_of(sent + lane / E, lane % E), j = u / a.pool.units;
+      from = -1;
+      if (u < units) {
+        const int id = table[j];
+        from = id >= 0 && id < a.pool.num_blocks
+                   ? reinterpret_cast<int64_t>(a.pool.unit(id, h, u - j * a.pool.units))
+                   : 0;
+        bad_block |= from == 0;
+      }
     };
-    int sent = 0;
     auto send = [&] {  // the whole warp
-      if (sent - ids_at == 32) load_ids(sent);
-      const int id = __shfl_sync(~0u, ids, sent - ids_at);
-      const int u = unit0 + kWarps * sent, st = issued % S;
-      const uint32_t bar = bars + 8 * st, dst = ring_at + st * U::kBytes;
-      if (id >= 0 && id < a.pool.num_blocks) {
-        if (lane == 0) {
+      if (sent - batch == 32 / E) find_units();
+      if (lane / E == sent - batch) {
+        const int st = issued % S;
+        const uint32_t bar = bars + 8 * st;
+        char* to = ring + st * kStage + (lane % E) * U::kBytes;
+        if (from > 0) {
           arrive_expect(bar, U::kBytes);
-          bulk_copy(dst, a.pool.unit(id, h, u % a.pool.units), U::kBytes, bar);
+          bulk_copy(smem_u32(to), reinterpret_cast<const void*>(from), U::kBytes, bar);
+        } else {
+          if (from == 0) {  // zero codes, scales and lows: zero keys and values
+            for (int i = 0; i < U::kBytes / 16; ++i)
+              *reinterpret_cast<uint4*>(to + 16 * i) = make_uint4(0, 0, 0, 0);
+            fence_async_smem();  // before a later copy into this place
+          }
+          mbar_arrive(bar);
         }
-      } else {  // zero codes, scales and lows: zero keys and values
-        bad_block = true;
-        for (int i = lane; i < U::kBytes / 16; i += 32)
-          *reinterpret_cast<uint4*>(ring + st * U::kBytes + 16 * i) = make_uint4(0, 0, 0, 0);
-        fence_async_smem();  // before a later copy into this place
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar);
       }
       ++issued;
       ++sent;
     };
-    load_ids(0);
+    find_units();
     for (int i = 0; i < S && i < count; ++i) send();
 
     // --------------------------------------------------------------- queries
     uint32_t qf[NT][2 * W][2];      // operand fragments: word w, then its upper half
-    float qs[NT][NG][2];            // scale log2e sum(q) of rows 2t, 2t + 1
-    float qm[NT][2];                // scale log2e over the row's power of two
+    float2 qs[NT][NG];              // sum(q) of rows 2t, 2t + 1, as the products have it
+    float2 qm[NT];                  // from there to log2 of the weights
     int limit[NT][2];               // the newest key these rows see
     int low_limit = INT32_MAX;
 #pragma unroll
@@ -211,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float2 y = pair_of<T>(x[i]);
+          const float2 y = pair_of<T>(x[i] ^ a.flip);
           f[w][2 * i] = y.x, f[w][2 * i + 1] = y.y;
         }
 #pragma unroll
@@ -238,15 +262,18 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
                                                      f[w][2 * k + 5] * (up * 0.0625f));
         }
       }
-      // the codes are 2^-24 of theirs, the queries up of theirs
-      const float back = pow2(11 + e) * a.scale2;
+      // the codes are 2^-24 of theirs, the queries `up` of theirs; masked scores
+      // are -inf before they are scaled, so the factor is never 0
+      const float back = fmaxf(pow2(11 + e) * a.scale2, 1e-30f);
+#pragma unroll
+      for (int w = 0; w < NG; ++w) sum[w] *= pow2(-11 - e);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const int from = 4 * (2 * t + k), m = row0 + 8 * nt + 2 * t + k;
-        qm[nt][k] = __shfl_sync(~0u, back, from);
+        const int from_lane = 4 * (2 * t + k), m = row0 + 8 * nt + 2 * t + k;
+        (k ? qm[nt].y : qm[nt].x) = __shfl_sync(~0u, back, from_lane);
 #pragma unroll
         for (int w = 0; w < NG; ++w)
-          qs[nt][w][k] = __shfl_sync(~0u, sum[w], from) * a.scale2;
+          (k ? qs[nt][w].y : qs[nt][w].x) = __shfl_sync(~0u, sum[w], from_lane);
         limit[nt][k] = m < rows ? r.len - r.n + m / a.G : INT32_MAX;  // no row: of no matter
         low_limit = min(low_limit, limit[nt][k]);
       }
@@ -255,7 +282,8 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
 
     // ------------------------------------------------------------------ keys
     float o[NT][2 * W][4];
-    float mref[NT][2], lsum[NT][2], lows[NT][NG][2];
+    // log2 of the largest p scale so far, less kUp; and float32 sums of two rows
+    float2 ref[NT], lsum[NT], lows[NT][NG];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -263,28 +291,25 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[nt][i][k] = 0.f;
       }
+      ref[nt] = make_float2(kLowest, kLowest);
+      lsum[nt] = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        mref[nt][k] = -INFINITY, lsum[nt][k] = 0.f;
-#pragma unroll
-        for (int w = 0; w < NG; ++w) lows[nt][w][k] = 0.f;
-      }
+      for (int w = 0; w < NG; ++w) lows[nt][w] = make_float2(0.f, 0.f);
     }
     for (int i = 0; i < count; ++i) {
       const int st = taken % S;
-      if (!late && !mbar_try(bars + 8 * st, (taken / S) & 1)) {
+      if (!mbar_try(bars + 8 * st, (taken / S) & 1) && !late) {
         const long long begin = clock64();
-        while (!mbar_try(bars + 8 * st, (taken / S) & 1))
-          if (clock64() - begin > kWaitCycles) {
-            late = true;
-            break;
-          }
+        while (!late && !mbar_try(bars + 8 * st, (taken / S) & 1))
+          late = clock64() - begin > kWaitCycles;
       }
-      late = __any_sync(~0u, late);
-      const char* unit = ring + st * U::kBytes;
+      __syncwarp();
+      const char* stage = ring + st * kStage;
       ++taken;
-      float x[NT][4];  // (key g, rows 2t and 2t + 1), (key g + 8, the same)
-      {
+      float2 x[E][NT][2];  // rows 2t and 2t + 1 at key g, and at key g + 8
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const char* unit = stage + e * U::kBytes;
         uint32_t ka[W], kb[W];
         Words<W>::load(ka, unit + g * U::kRow + 4 * W * t);
         Words<W>::load(kb, unit + (g + 8) * U::kRow + 4 * W * t);
@@ -292,133 +317,173 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
         Words<NG>::load(pa, unit + U::oKp + 4 * NG * g);
         Words<NG>::load(pb, unit + U::oKp + 4 * NG * (g + 8));
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) x[nt][k] = 0.f;
-        }
-#pragma unroll
         for (int k = 0; k < NG; ++k) {
+          const float2 fa = pair_of<T>(pa[k]), fb = pair_of<T>(pb[k]);
           float acc[NT][4];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) acc[nt][c] = 0.f;
-          }
 #pragma unroll
           for (int w = k * WG; w < (k + 1) * WG; ++w) {
             const uint32_t ya = ka[w] >> 8, yb = kb[w] >> 8;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              mma16(acc[nt], ka[w] & kLow, kb[w] & kLow, ka[w] & kHigh, kb[w] & kHigh,
-                    qf[nt][2 * w][0], qf[nt][2 * w][1]);
+              if (w == k * WG)
+                mma16_first(acc[nt], ka[w] & kLow, kb[w] & kLow, ka[w] & kHigh, kb[w] & kHigh,
+                            qf[nt][2 * w][0], qf[nt][2 * w][1]);
+              else
+                mma16(acc[nt], ka[w] & kLow, kb[w] & kLow, ka[w] & kHigh, kb[w] & kHigh,
+                      qf[nt][2 * w][0], qf[nt][2 * w][1]);
               mma16(acc[nt], ya & kLow, yb & kLow, ya & kHigh, yb & kHigh, qf[nt][2 * w + 1][0],
                     qf[nt][2 * w + 1][1]);
             }
           }
-          const float2 fa = pair_of<T>(pa[k]), fb = pair_of<T>(pb[k]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const float2 sa = make_float2(acc[nt][0], acc[nt][1]),
+                         sb = make_float2(acc[nt][2], acc[nt][3]);
+            const float2 la = __fmul2_rn(both(fa.y), qs[nt][k]),
+                         lb = __fmul2_rn(both(fb.y), qs[nt][k]);
+            x[e][nt][0] = __ffma2_rn(both(fa.x), sa, k ? __fadd2_rn(x[e][nt][0], la) : la);
+            x[e][nt][1] = __ffma2_rn(both(fb.x), sb, k ? __fadd2_rn(x[e][nt][1], lb) : lb);
+          }
+        }
+      }
+      const int key0 = kUnit * unit_of(i, 0);
+      uint32_t shown = ~0u;  // bit 4 (NT e + nt) + c: the row sees the key
+      const bool some_hidden = key0 + E * kUnit - 1 > low_limit;
+      if (some_hidden) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              const float2 f = c < 2 ? fa : fb;
-              x[nt][c] = fmaf(f.y, qs[nt][k][c & 1],
-                              fmaf(f.x * qm[nt][c & 1], acc[nt][c], x[nt][c]));
+              if (key0 + kUnit * e + g + 8 * (c / 2) <= limit[nt][c & 1]) continue;
+              (c & 1 ? x[e][nt][c / 2].y : x[e][nt][c / 2].x) = -INFINITY;
+              shown &= ~(1u << (4 * (NT * e + nt) + c));
             }
-          }
-        }
-      }
-      const int key0 = kUnit * (unit0 + kWarps * i) + g;
-      uint32_t shown = ~0u;  // bit 4 nt + c: the row sees the key
-      if (key0 - g + kUnit - 1 > low_limit) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (key0 + (c < 2 ? 0 : 8) > limit[nt][c & 1]) {
-              x[nt][c] = -INFINITY;
-              shown &= ~(1u << (4 * nt + c));
-            }
-        }
-      }
-      uint32_t va[NG], vb[NG];
-      Words<NG>::load(va, unit + U::oVp + 4 * NG * g);
-      Words<NG>::load(vb, unit + U::oVp + 4 * NG * (g + 8));
-      float2 fa[NG], fb[NG];
-      float sa = 0.f, sb = 0.f;
-#pragma unroll
-      for (int k = 0; k < NG; ++k) {
-        fa[k] = pair_of<T>(va[k]), fb[k] = pair_of<T>(vb[k]);
-        sa = fmaxf(sa, fa[k].x), sb = fmaxf(sb, fb[k].x);
-      }
-      // log2 of the largest scale: p scale is what has to fit fp16
-      const float la = fminf(fmaxf(lg2(sa), -100.f), 100.f);
-      const float lb = fminf(fmaxf(lg2(sb), -100.f), 100.f);
-      bool grow = false;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          grow |= x[nt][c] + (c < 2 ? la : lb) > mref[nt][c & 1] + kLazy;
-      }
-      if (__any_sync(~0u, grow)) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            float m = fmaxf(x[nt][k] + la, x[nt][k + 2] + lb);
-            m = fmaxf(m, __shfl_xor_sync(~0u, m, 4));
-            m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
-            m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
-            m = fmaxf(m, mref[nt][k]);
-            const float f = m == mref[nt][k] ? 1.f : ex2(mref[nt][k] - m);
-            mref[nt][k] = m;
-            lsum[nt][k] *= f;
-#pragma unroll
-            for (int w = 0; w < NG; ++w) lows[nt][w][k] *= f;
-#pragma unroll
-            for (int w = 0; w < 2 * W; ++w) o[nt][w][k] *= f, o[nt][w][k + 2] *= f;
           }
         }
       }
       // ------------------------------------------------------------- weights
-      uint32_t pf[NT][NG][2];
+      // p scale has to fit fp16 (and p float32): where it would not, the
+      // reference moves up and what was summed goes down
+      float2 f[E][2][NG];  // (scale, 8 scale + low, the middle of a group's values)
+      float2 p[E][NT][2];
+      float most[E][2], top = 0.f;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float p[4];
+      for (int e = 0; e < E; ++e) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const float m = mref[nt][c & 1];
-          p[c] = ex2(x[nt][c] - ((m == -INFINITY ? 0.f : m) - kUp));
-          lsum[nt][c & 1] += p[c];
-        }
+        for (int c = 0; c < 2; ++c) {
+          uint32_t v[NG];
+          Words<NG>::load(v, stage + e * U::kBytes + U::oVp + 4 * NG * (g + 8 * c));
+          most[e][c] = 0.f;
 #pragma unroll
-        for (int k = 0; k < NG; ++k) {
-          float w[4], low[4];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const float2 f = c < 2 ? fa[k] : fb[k];
-            w[c] = p[c] * f.x;
-            low[c] = p[c] * fmaf(8.f, f.x, f.y);
-            // a scale that is not finite reaches no row that does not see its key
-            if (!(shown >> (4 * nt + c) & 1u)) w[c] = low[c] = 0.f;
-          }
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint32_t y = Pack2<__half>::pack(w[2 * half], w[2 * half + 1]);
-            const float2 z = pair_of<__half>(y);
-            lows[nt][k][0] += fmaf(-8.f, z.x, low[2 * half]);
-            lows[nt][k][1] += fmaf(-8.f, z.y, low[2 * half + 1]);
-            pf[nt][k][half] = transposed(y);
+          for (int k = 0; k < NG; ++k) {
+            const float2 y = pair_of<T>(v[k]);
+            f[e][c][k] = make_float2(y.x, fmaf(8.f, y.x, y.y));
+            most[e][c] = fmaxf(most[e][c], y.x);
           }
         }
       }
+      auto weights = [&] {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const float2 y = __ffma2_rn(x[e][nt][c], qm[nt], make_float2(-ref[nt].x, -ref[nt].y));
+              p[e][nt][c] = make_float2(ex2(y.x), ex2(y.y));
+            }
+          }
+        }
+      };
+      weights();
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float y = fmaxf(p[e][0][c].x, p[e][0][c].y);
+#pragma unroll
+          for (int nt = 1; nt < NT; ++nt) y = fmaxf(y, fmaxf(p[e][nt][c].x, p[e][nt][c].y));
+          top = fmaxf(top, y * fmaxf(most[e][c], kTooLarge * 0x1p-110f));
+        }
+      }
+      if (__any_sync(~0u, top > kTooLarge)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float ma = -INFINITY, mb = -INFINITY;
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const float l = fminf(fmaxf(lg2(most[e][c]), -100.f), 100.f) - kUp;
+              ma = fmaxf(ma, fmaf(x[e][nt][c].x, qm[nt].x, l));
+              mb = fmaxf(mb, fmaf(x[e][nt][c].y, qm[nt].y, l));
+            }
+          }
+          auto raise = [&](float& old, float m) {
+            m = fmaxf(m, __shfl_xor_sync(~0u, m, 4));
+            m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
+            m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
+            m = fmaxf(m, old);
+            const float f = m == old ? 1.f : ex2(old - m);
+            old = m;
+            return f;
+          };
+          const float2 down = make_float2(raise(ref[nt].x, ma), raise(ref[nt].y, mb));
+          lsum[nt] = __fmul2_rn(lsum[nt], down);
+#pragma unroll
+          for (int w = 0; w < NG; ++w) lows[nt][w] = __fmul2_rn(lows[nt][w], down);
+#pragma unroll
+          for (int w = 0; w < 2 * W; ++w) {
+            o[nt][w][0] *= down.x, o[nt][w][1] *= down.y;
+            o[nt][w][2] *= down.x, o[nt][w][3] *= down.y;
+          }
+        }
+        weights();
+      }
+      uint32_t pf[E][NT][NG][2];
+      auto weigh = [&](auto hidden) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            lsum[nt] = __fadd2_rn(lsum[nt], __fadd2_rn(p[e][nt][0], p[e][nt][1]));
+#pragma unroll
+            for (int k = 0; k < NG; ++k) {
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                const float2 s = f[e][c][k];
+                float2 w = __fmul2_rn(p[e][nt][c], both(s.x));
+                if constexpr (decltype(hidden)::value) {
+                  // a scale that is not finite reaches no row that does not see its key
+                  const int bit = 4 * (NT * e + nt) + 2 * c;
+                  const bool sx = shown >> bit & 1u, sy = shown >> (bit + 1) & 1u;
+                  w = make_float2(sx ? w.x : 0.f, sy ? w.y : 0.f);
+                  const float2 low = __fmul2_rn(p[e][nt][c], both(s.y));
+                  lows[nt][k] = __fadd2_rn(lows[nt][k],
+                                           make_float2(sx ? low.x : 0.f, sy ? low.y : 0.f));
+                } else {
+                  lows[nt][k] = __ffma2_rn(p[e][nt][c], both(s.y), lows[nt][k]);
+                }
+                const uint32_t y = Pack2<__half>::pack(w.x, w.y);
+                lows[nt][k] = __ffma2_rn(pair_of<__half>(y), both(-8.f), lows[nt][k]);
+                pf[e][nt][k][c] = transposed(y);
+              }
+            }
+          }
+        }
+      };
+      if (some_hidden) weigh(std::true_type());
+      else weigh(std::false_type());
       // -------------------------------------------------------------- values
-      {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
         uint32_t v[4][(W + 1) / 2];
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          Words<W / 2>::load(v[k], unit + U::oV + (2 * t + (k & 1) + 4 * (k & 2)) * U::kRow +
-                                       2 * W * g);
+          Words<W / 2>::load(v[k], stage + e * U::kBytes + U::oV +
+                                       (2 * t + (k & 1) + 4 * (k & 2)) * U::kRow + 2 * W * g);
 #pragma unroll
         for (int w = 0; w < W; ++w) {
           const uint32_t sel = w & 1 ? 0x7632u : 0x5410u;
@@ -427,14 +492,13 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
           const uint32_t ya = xa >> 8, yb = xb >> 8;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            mma16(o[nt][2 * w], xa & kLow, xa & kHigh, xb & kLow, xb & kHigh, pf[nt][w / WG][0],
-                  pf[nt][w / WG][1]);
-            mma16(o[nt][2 * w + 1], ya & kLow, ya & kHigh, yb & kLow, yb & kHigh,
-                  pf[nt][w / WG][0], pf[nt][w / WG][1]);
+            const uint32_t *b = pf[e][nt][w / WG];
+            mma16(o[nt][2 * w], xa & kLow, xa & kHigh, xb & kLow, xb & kHigh, b[0], b[1]);
+            mma16(o[nt][2 * w + 1], ya & kLow, ya & kHigh, yb & kLow, yb & kHigh, b[0], b[1]);
           }
         }
       }
-      __syncwarp();  // the unit has been read
+      __syncwarp();  // the units have been read
       if (sent < count) send();
     }
 
@@ -442,17 +506,18 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
+      for (int s = 4; s < 32; s <<= 1) {
+        auto add = [&](float2& y) {
+          y = __fadd2_rn(y, make_float2(__shfl_xor_sync(~0u, y.x, s),
+                                        __shfl_xor_sync(~0u, y.y, s)));
+        };
+        add(lsum[nt]);
 #pragma unroll
-        for (int s = 4; s < 32; s <<= 1) {
-          lsum[nt][k] += __shfl_xor_sync(~0u, lsum[nt][k], s);
-#pragma unroll
-          for (int w = 0; w < NG; ++w) lows[nt][w][k] += __shfl_xor_sync(~0u, lows[nt][w][k], s);
-        }
-        if (g == 0) {
-          maxima[warp * RT + 8 * nt + 2 * t + k] = mref[nt][k];
-          sums[warp * RT + 8 * nt + 2 * t + k] = lsum[nt][k];
-        }
+        for (int w = 0; w < NG; ++w) add(lows[nt][w]);
+      }
+      if (g == 0) {
+        *reinterpret_cast<float2*>(maxima + warp * RT + 8 * nt + 2 * t) = ref[nt];
+        *reinterpret_cast<float2*>(sums + warp * RT + 8 * nt + 2 * t) = lsum[nt];
       }
     }
     __syncthreads();
@@ -461,14 +526,15 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const int row = 8 * nt + 2 * t + k;
-        float top = -INFINITY;
+        float top = kLowest;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) top = fmaxf(top, maxima[w * RT + row]);
-        const float f = mref[nt][k] == top ? 1.f : ex2(mref[nt][k] - top);
+        const float mine = k ? ref[nt].y : ref[nt].x;
+        const float f = mine == top ? 1.f : ex2(mine - top);
         float* to = outs + (warp * RT + row) * D + 4 * g;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-          const float z = lows[nt][w / WG][k];
+          const float z = k ? lows[nt][w / WG].y : lows[nt][w / WG].x;
           float4 y;
           y.x = fmaf(o[nt][2 * w][k], 0x1p24f, z) * f;
           y.y = fmaf(o[nt][2 * w][k + 2], 0x1p20f, z) * f;
@@ -484,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
     for (int i = tid; i < RT * (D / 4); i += kThreads) {
       const int row = i / (D / 4), c = 4 * (i % (D / 4));
       if (row0 + row >= rows) break;
-      float top = -INFINITY, l = 0.f;
+      float top = kLowest, l = 0.f;
       float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) top = fmaxf(top, maxima[w * RT + row]);
@@ -496,8 +562,7 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
         y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
       }
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      const float lse2 = l == 0.f ? -INFINITY
-                                  : (top == -INFINITY ? 0.f : top) - kUp + log2f(l);
+      const float lse2 = l == 0.f ? -INFINITY : top + log2f(l);
       y.x *= inv, y.y *= inv, y.z *= inv, y.w *= inv;
       if (whole) {
         write4<T>(a, r.start, row0 + row, h, c, y);
@@ -519,7 +584,7 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
   }
   if (tid == 0) a.joins[blockIdx.x] = join;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (bad_block && lane == 0) report(a.status, CS_ST_SLOT_RANGE);
+  if (bad_block) report(a.status, CS_ST_SLOT_RANGE);
   if (late) {  // copies of this block are to have landed before it ends
     for (int s = taken - S < 0 ? 0 : taken - S; s < taken; ++s) {
       const long long begin = clock64();
@@ -535,7 +600,7 @@ int launch_decode(const Attn4& a, int workers, cudaStream_t stream) {
   constexpr auto kernel = kv4_decode_kernel<T, D, NG, NT>;
   constexpr int kBytes = Ring<D, NG, NT>::kBytes;
   if (!allow_smem<kernel>(kBytes)) return CS_ERR_CUDA;
-  if (const int rc = launch_dependent(kernel, workers, kThreads, kBytes, stream, a)) return rc;
+  if (const int rc = launch_dependent(kernel, dim3(workers), kThreads, kBytes, stream, a)) return rc;
   return launch_join<T, D, 8 * NT>(a, workers, stream);
 }
 

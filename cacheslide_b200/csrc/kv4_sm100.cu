@@ -1,0 +1,695 @@
+// Tensor-core attention over the 4-bit pool for many query rows a KV head
+// (questions, prompt chunks): tcgen05, TMEM.
+//
+// One block takes a range of the steps of all row tiles (Share4): up to NT
+// tiles of 128 query rows of a (request, KV head) and the keys that they see,
+// 64 a step.  Per step
+//   S = Q K^T (tcgen05, TMEM),  P = 2^(S c - m),  O += P V (P from TMEM)
+// with the running maximum m and sum of each row in float32 registers.
+//
+// Two warps turn the step's key codes into the operand tile and two the value
+// codes: a word of eight codes, fetched a step ahead, becomes four pairs of
+// fp16 numbers with five bit operations (1024 + code has the code in its low
+// bits), four subtractions and four multiply-adds with scale and lowest value;
+// that is shared by all rows of the block, up to 256.  Operands are fp16
+// whatever the pool's type: queries are scaled by a power of two a row, keys
+// and values by one a step (of what the step's scales and lowest values can
+// reach), so bfloat16 pools of any size of numbers keep fp16's 11 bits, where
+// bfloat16 operands would keep 8.  P carries the values' power of two, the
+// rows' sums do not.
+//
+// Pairs lie in the tiles as the codes come, elements (0, 4), (1, 5), (2, 6), (3,
+// 7) of eight: the queries are written in the same order, and the output's
+// columns are put back as they are written.
+#include <math.h>
+
+#include <type_traits>
+
+#include "kv4.cuh"
+#include "kv4_attn.cuh"
+#include "sm100.cuh"
+
+namespace cs {
+namespace {
+
+constexpr int kKeys = 64;         // keys of a step
+constexpr int kTileRows = 128;
+constexpr int kLeastSteps = 4;    // steps a block takes at least
+constexpr float kLazy = 8.f;      // O is rescaled when the maximum grew by more than 2^8
+constexpr float kUp = 7.f;        // P is stored up by 2^7: fp16's normal numbers reach 2^-21
+constexpr int kInfo = 4;          // steps whose scales are kept
+
+template <int D, int NT>
+struct Shape4 {
+  // threads a row in the softmax, as in the wide blocks of the shared-prefix kernel
+  static constexpr int TPR = NT;
+  static constexpr int kTile = kTileRows * TPR;  // softmax threads of a row tile
+  static constexpr int kSoft = 4 * NT * TPR;     // softmax warps, then 2 K, 2 V, NT MMA warps
+  static constexpr int kThreads = 32 * (kSoft + 4 + NT);
+  static constexpr uint32_t TB = kKeys * D * 2;  // a K or V tile, two of each
+  // a query tile's place also takes its output rows, 2 D bytes each and 16 more
+  static constexpr uint32_t QB = kTileRows * D * 2 + kTileRows * 16;
+  static constexpr uint32_t oQ = 0, oK = NT * QB, oV = oK + 2 * TB, oMeta = oV + 2 * TB;
+  // barriers: queries; a stage's K and V; a score buffer's S, P and PV of a row
+  // tile; a row's maxima
+  static constexpr uint32_t bQ = 0, bK = 8, bV = bK + 16, bS = bV + 16, bP = bS + 16 * NT,
+                            bPV = bP + 16 * NT, bMax = bPV + 16 * NT, oTmem = bMax + 32 * NT,
+                            oAbort = oTmem + 4, oFlag = oAbort + 4, oScale = oFlag + 4 * kInfo,
+                            oPower = oScale + 4 * kInfo, oReach = oPower + 4 * kInfo,
+                            oBad = oReach + 32, oRow = oBad + kInfo * kKeys,
+                            oMax = oRow + NT * kTileRows * 4,
+                            oSums = (oMax + NT * 2 * 2 * 128 * 4 + 7) / 8 * 8,
+                            kMeta = oSums + (128 + 1 + 4) * 8;
+  static_assert(oMeta % 1024 == 0 && oTmem % 4 == 0 && oRow % 4 == 0, "alignment");
+  static constexpr uint32_t kSmem = oMeta + kMeta + 1024;  // the base is rounded up to 1024
+  static constexpr uint32_t kCols = 256 * NT;
+  // two score buffers of 64 columns at 128 i for row tile i, O at cO + D i
+  static constexpr uint32_t cS = 0, cO = 128 * NT;
+};
+
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
+__device__ __forceinline__ void pair_sync(bool v) {  // the two warps of a producer
+  if (v) asm volatile("bar.sync 2, 64;" ::: "memory");
+  else asm volatile("bar.sync 1, 64;" ::: "memory");
+}
+__device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
+__device__ __forceinline__ uint32_t as_u32(__half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
+
+// eight codes as low + scale code, pairs (0, 4), (1, 5), (2, 6), (3, 7)
+__device__ __forceinline__ uint4 decode8(uint32_t w, __half2 scale, __half2 low) {
+  const uint32_t magic = 0x64006400u;  // 1024; codes in bits 0 .. 3, or 4 .. 7 (16 times them)
+  const __half2 k1024 = as_half2(magic), sixteenth = as_half2(0x2c002c00u),
+                k64 = as_half2(0xd400d400u);  // -64
+  const uint32_t y = w >> 8;
+  const __half2 a = __hsub2(as_half2((w & 0x000f000fu) | magic), k1024);
+  const __half2 b = __hfma2(as_half2((w & 0x00f000f0u) | magic), sixteenth, k64);
+  const __half2 c = __hsub2(as_half2((y & 0x000f000fu) | magic), k1024);
+  const __half2 d = __hfma2(as_half2((y & 0x00f000f0u) | magic), sixteenth, k64);
+  return make_uint4(as_u32(__hfma2(a, scale, low)), as_u32(__hfma2(b, scale, low)),
+                    as_u32(__hfma2(c, scale, low)), as_u32(__hfma2(d, scale, low)));
+}
+// where element d of eight lies in that order
+__host__ __device__ constexpr int place8(int d) { return 2 * (d & 3) + (d >> 2 & 1); }
+
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t (&w)[N], const char* p) {
+  if constexpr (N == 4) {
+    const uint4 x = *reinterpret_cast<const uint4*>(p);
+    w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+  } else if constexpr (N == 2) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    w[0] = x.x, w[1] = x.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+}
+
+template <typename T, int D, int NG, int NT>
+__global__ void __launch_bounds__(Shape4<D, NT>::kThreads, NT == 1 ? 2 : 1)
+    kv4_sm100_kernel(const __grid_constant__ Attn4 a) {
+  using Sh = Shape4<D, NT>;
+  using U = Unit4<D, NG>;
+  constexpr int RT = kTileRows * NT, W = U::W, WG = W / NG;
+  using Share = Share4<RT, kKeys>;
+  extern __shared__ char smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t sbase = (raw + 1023u) & ~1023u;
+  char* smem = smem_raw + (sbase - raw);
+  const uint32_t mb = sbase + Sh::oMeta;
+  char* meta = smem + Sh::oMeta;
+  volatile int* abort = reinterpret_cast<volatile int*>(meta + Sh::oAbort);
+  volatile int* flag = reinterpret_cast<volatile int*>(meta + Sh::oFlag);  // step + 1: bad values
+  volatile float* key_scale = reinterpret_cast<volatile float*>(meta + Sh::oScale);  // 2^E of keys
+  volatile float* val_power = reinterpret_cast<volatile float*>(meta + Sh::oPower);  // E of values
+  uint8_t* bad = reinterpret_cast<uint8_t*>(meta + Sh::oBad);  // [step % kInfo][key]: groups
+  float* row_scale = reinterpret_cast<float*>(meta + Sh::oRow);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (warp == Sh::kSoft + 4) tmem_alloc(mb + Sh::oTmem, Sh::kCols);
+  if (tid == 0) *abort = 0;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  Share work;
+  work.template find<128>(a, blockIdx.x, gridDim.x, kLeastSteps,
+                          reinterpret_cast<int64_t*>(meta + Sh::oSums));
+  zero_rest<T, D>(a);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(meta + Sh::oTmem);
+  bool bad_block = false, first = true;
+  int which = 0;  // of this block's partial results
+  int4 join = make_int4(-1, 0, 0, 0);
+
+  while (work.todo > 0) {
+    const Request4 rq = work.r;
+    const int all_steps = Share::steps(rq, a.G, work.tile);
+    const int s0 = work.step;
+    const int s1 = (int)min((int64_t)all_steps, s0 + work.todo);
+    const int row0 = work.tile * RT, rows = min(RT, rq.n * a.G - row0), g = work.head;
+    const int tiles = rows > kTileRows ? 2 : 1;
+    const int seen = max(0, rq.len - rq.n + Share::last_token(rq, a.G, work.tile) + 1);
+    const int steps = min(s1, (seen + kKeys - 1) / kKeys) - s0;  // with keys to see
+    const bool whole = s0 == 0 && s1 == all_steps;
+    const int64_t part = 2ll * blockIdx.x + which;
+    if (tid == 0) {
+      if (!first)
+        for (uint32_t b = Sh::bQ; b < Sh::oTmem; b += 8) mbar_inval(mb + b);
+      mbar_init(mb + Sh::bQ, Sh::kTile * tiles);
+      for (int s = 0; s < 2; ++s) {
+        mbar_init(mb + Sh::bK + 8 * s, 64);
+        mbar_init(mb + Sh::bV + 8 * s, 64);
+      }
+      for (int s = 0; s < 2 * NT; ++s) {
+        mbar_init(mb + Sh::bS + 8 * s, 1);
+        mbar_init(mb + Sh::bP + 8 * s, Sh::kTile);
+        mbar_init(mb + Sh::bPV + 8 * s, 1);
+      }
+      for (int s = 0; s < 4 * NT; ++s) mbar_init(mb + Sh::bMax + 8 * s, 2);
+      mbar_init_fence();
+      for (int s = 0; s < kInfo; ++s) flag[s] = 0;
+    }
+    first = false;
+    __syncthreads();
+    // step t uses score buffer t & 1 of its row tile
+    auto at = [&](uint32_t bar, int qt, int t) { return mb + bar + 8 * (2 * qt + (t & 1)); };
+
+    if (warp >= Sh::kSoft && warp < Sh::kSoft + 4) {
+      // =========================================== producers: K, then V pair
+      const bool isv = warp >= Sh::kSoft + 2;
+      const int i = (tid - 32 * Sh::kSoft) & 63;
+      // this thread's part of 16 keys' rows: token r, W words from word W c on
+      const int r = (i & 7) + 8 * (i >> 5), c = (i >> 3) & 3;
+      const int32_t* table = a.tables + work.request * a.table_stride;
+      const int units = (seen + kUnit - 1) / kUnit;
+      int64_t from = -1;  // this lane's unit of eight steps: -1 none, 0 no block
+      uint32_t code[4][W], pair[4][NG];
+      auto fetch = [&](int t) {
+        if (t >= steps) return;
+        if (t % 8 == 0) {
+          const int u = (s0 + t) * (kKeys / kUnit) + lane, j = u / a.pool.units;
+          from = -1;
+          if (u < units) {
+            const int id = table[j];
+            from = id >= 0 && id < a.pool.num_blocks
+                       ? reinterpret_cast<int64_t>(a.pool.unit(id, g, u - j * a.pool.units))
+                       : 0;
+            bad_block |= from == 0;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int64_t unit = __shfl_sync(~0u, from, (t % 8) * 4 + j);
+          const int key = (s0 + t) * kKeys + j * kUnit + r;
+          if (unit > 0 && key < seen) {
+            const char* p = reinterpret_cast<const char*>(unit);
+            load_words(code[j], p + (isv ? U::oV : 0) + r * U::kRow + 4 * W * c);
+            load_words(pair[j], p + (isv ? U::oVp : U::oKp) + 4 * NG * r);
+          } else {  // zeros: P is zero there too
+#pragma unroll
+            for (int w = 0; w < W; ++w) code[j][w] = 0u;
+#pragma unroll
+            for (int k = 0; k < NG; ++k) pair[j][k] = 0u;
+          }
+        }
+      };
+      fetch(0);
+      for (int t = 0; t < steps; ++t) {
+        // ------------------------------- the step's power of two, bad values
+        float2 f[4][NG];
+        float reach = 0.f;
+        uint32_t wrong = 0u;  // bit NG j + k
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int k = 0; k < NG; ++k) {
+            f[j][k] = pair_of<T>(pair[j][k]);
+            const float m = fmaxf(fabsf(f[j][k].y), fabsf(fmaf(15.f, f[j][k].x, f[j][k].y)));
+            if (m < INFINITY && f[j][k].x == f[j][k].x) {
+              reach = fmaxf(reach, m);
+            } else {
+              wrong |= 1u << (NG * j + k);
+              // a bad value becomes 0 here and marks the rows that see it
+              if (isv) f[j][k] = make_float2(0.f, 0.f);
+            }
+          }
+        }
+        int e = 0;
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+          const uint32_t m = __reduce_max_sync(~0u, __float_as_uint(reach));
+          volatile uint32_t* both = reinterpret_cast<volatile uint32_t*>(meta + Sh::oReach) +
+                                    (isv ? 4 : 0) + 2 * (t & 1);
+          if (lane == 0) both[warp & 1] = m;
+          pair_sync(isv);
+          const uint32_t all = max(both[0], both[1]);
+          e = all == 0u ? 0 : min(114, max(-80, (int)(all >> 23) - 127 - 13));
+        }
+        const float down = pow2(-e);
+        // --------------------------------------------------- a free stage
+        if (t >= 2) {
+          bool ok = true;
+          for (int qt = 0; qt < tiles; ++qt)
+            ok = ok && warp_wait(at(isv ? Sh::bPV : Sh::bS, qt, t), (t / 2 - 1) & 1, abort);
+          if (!ok) break;
+        }
+        if (i == 0) {
+          if (isv) val_power[t % kInfo] = (float)e;
+          else key_scale[t % kInfo] = pow2(e);
+        }
+        const uint32_t tile = sbase + (isv ? Sh::oV : Sh::oK) + (t & 1) * Sh::TB;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          __half2 scale[NG], low[NG];
+#pragma unroll
+          for (int k = 0; k < NG; ++k) {
+            scale[k] = __float2half2_rn(f[j][k].x * down);
+            low[k] = __float2half2_rn(f[j][k].y * down);
+          }
+#pragma unroll
+          for (int w = 0; w < W; ++w) {
+            const uint32_t x = isv ? __byte_perm(code[j][w / 2], code[j][W / 2 + w / 2],
+                                                 w & 1 ? 0x7632u : 0x5410u)
+                                   : code[j][w];
+            st_shared16(tile + sw128(j * kUnit + r, 4 * w + c, kKeys),
+                        decode8(x, scale[w / WG], low[w / WG]));
+          }
+          if (isv && c == 0)
+            bad[(t % kInfo) * kKeys + j * kUnit + r] = (uint8_t)(wrong >> (NG * j) & ((1u << NG) - 1u));
+        }
+        if (isv && wrong) flag[t % kInfo] = t + 1;
+        fetch(t + 1);
+        fence_async_smem();
+        mbar_arrive(mb + (isv ? Sh::bV : Sh::bK) + 8 * (t & 1));
+      }
+
+    } else if (warp >= Sh::kSoft + 4) {
+      // ================================================== MMA, one warp a tile
+      const int qt = __shfl_sync(~0u, warp, 0) - (Sh::kSoft + 4);
+      if (qt < tiles) {
+        const bool leader = elect_one();
+        const uint32_t id_s = umma_idesc(128, kKeys, 0, 0, 0);
+        const uint32_t id_o = umma_idesc(128, D, 0, 0, 1);  // V is MN-major
+        const uint64_t dq = umma_desc(sbase + Sh::oQ + qt * Sh::QB, 16, 1024);
+        const uint64_t dk0 = umma_desc(sbase + Sh::oK, 16, 1024);
+        const uint64_t dv0 = umma_desc(sbase + Sh::oV, kKeys * 128, 1024);
+        const uint32_t tm = __shfl_sync(~0u, tmem, 0);
+        const uint32_t sc = tm + Sh::cS + 128 * qt, oc = tm + Sh::cO + D * qt;
+        bool ok = warp_wait(mb + Sh::bQ, 0, abort);
+        uint32_t last = 0, lastph = 0;  // the newest group issued
+        auto arrived = [&](uint32_t bar, int t) {
+          ok = ok && warp_wait(mb + bar + 8 * (t & 1), (t / 2) & 1, abort);
+          return ok;
+        };
+        auto scores = [&](int t) {
+          tc_fence_after();
+          const uint64_t dk = dk0 + (uint64_t)((t & 1) * (Sh::TB >> 4));
+          const uint32_t s = sc + kKeys * (t & 1);
+          last = at(Sh::bS, qt, t);
+          lastph = (t >> 1) & 1;
+          if (leader) {
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk)  // offsets in 16-byte units
+              tc_mma(s, dq + (kk >> 2) * 1024 + (kk & 3) * 2,
+                     dk + (kk >> 2) * (kKeys * 8) + (kk & 3) * 2, id_s, kk ? 1u : 0u);
+            tc_commit(last);
+          }
+          __syncwarp();
+        };
+        if (steps > 0 && arrived(Sh::bK, 0)) scores(0);
+        if (steps > 1 && arrived(Sh::bK, 1)) scores(1);
+        for (int t = 0; ok && t < steps; ++t) {
+          const uint32_t ph = (t >> 1) & 1;
+          if (!arrived(Sh::bV, t)) break;
+          if (!(ok = warp_wait(at(Sh::bP, qt, t), ph, abort))) break;
+          tc_fence_after();
+          const uint64_t dv = dv0 + (uint64_t)((t & 1) * (Sh::TB >> 4));
+          const uint32_t p = sc + kKeys * (t & 1);
+          last = at(Sh::bPV, qt, t);
+          lastph = ph;
+          if (leader) {
+#pragma unroll
+            for (int kk = 0; kk < kKeys / 16; ++kk)
+              tc_mma_ts(oc, p + kk * 8, dv + kk * 128, id_o, (t | kk) ? 1u : 0u);
+            tc_commit(last);
+          }
+          __syncwarp();
+          // the next scores but one take the buffer that P lies in
+          if (t + 2 < steps) {
+            if (!arrived(Sh::bK, t + 2)) break;
+            if (!(ok = warp_wait(at(Sh::bPV, qt, t), ph, abort))) break;
+            scores(t + 2);
+          }
+        }
+        if (last) {
+          const long long t0 = clock64();
+          while (!mbar_try(last, lastph) && clock64() - t0 < kWaitCycles) {
+          }
+        }
+      }
+      __syncwarp();
+
+    } else if (warp / (4 * Sh::TPR) < tiles) {
+      // =============================================================== softmax
+      constexpr int TPR = Sh::TPR, VC = kKeys / TPR;  // scores of a step a thread holds
+      const int qt = warp / (4 * TPR), part2 = (warp >> 2) % TPR;
+      const int r = (warp & 3) * 32 + lane;  // TMEM lane
+      const int row = qt * kTileRows + r;    // of the block's
+      const bool row_ok = row < rows;
+      {
+        // queries into the swizzled operand layout, a power of two a row
+        constexpr int C = D / 8;
+        const int c = tid % C;
+        const uint32_t qs = sbase + Sh::oQ + qt * Sh::QB;
+        for (int m = (tid % Sh::kTile) / C; m < kTileRows; m += Sh::kTile / C) {
+          const int rr = row0 + qt * kTileRows + m;
+          const bool ok = qt * kTileRows + m < rows;
+          const int tk = ok ? rr / a.G : 0;
+          const char* p = a.q + (int64_t)(rq.start + tk) * a.qt +
+                          (int64_t)(g * a.G + (ok ? rr - tk * a.G : 0)) * a.qh + 16 * c;
+          uint32_t x[4] = {0u, 0u, 0u, 0u};
+          if (ok && a.vec_q) {
+            load_words(x, p);
+          } else if (ok) {
+            const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = u[2 * k] | (uint32_t)u[2 * k + 1] << 16;
+          }
+          float f[8], top = 0.f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 y = pair_of<T>(x[k] ^ a.flip);
+            f[2 * k] = y.x, f[2 * k + 1] = y.y;
+            top = fmaxf(top, fmaxf(fabsf(y.x), fabsf(y.y)));
+          }
+#pragma unroll
+          for (int o = 1; o < C; o <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+          const int e = min(100, max(-100, (int)(__float_as_uint(top) >> 23) - 127 - 13));
+          const float up = pow2(-e);
+          if (c == 0) row_scale[qt * kTileRows + m] = pow2(e);
+          uint32_t y[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) y[k] = Pack2<__half>::pack(f[k] * up, f[k + 4] * up);
+          st_shared16(qs + sw128(m, c, kTileRows), make_uint4(y[0], y[1], y[2], y[3]));
+        }
+        fence_async_smem();
+        mbar_arrive(mb + Sh::bQ);
+      }
+      bool ok = warp_wait(mb + Sh::bQ, 0, abort);
+      const float row_factor = row_scale[qt * kTileRows + r] * a.scale2;
+      // the newest key this row sees; no row: of no matter
+      const int limit = row_ok ? rq.len - rq.n + (row0 + row) / a.G : INT32_MAX;
+      const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+      const uint32_t sc0 = tmem + lane_base + Sh::cS + 128 * qt;
+      const uint32_t oc = tmem + lane_base + Sh::cO + D * qt;
+      float mref = -INFINITY, lsum = 0.f;  // log2 domain; P = 2^(x + E - mref + up)
+      uint32_t poison = 0u;  // groups of values that are not finite and that the row sees
+      [[maybe_unused]] int exchanges = 0;  // of maxima with the row's other thread
+      [[maybe_unused]] const uint32_t pair = mb + Sh::bMax + 8 * (4 * qt + (warp & 3));
+      [[maybe_unused]] float* row_max = reinterpret_cast<float*>(meta + Sh::oMax) + qt * 512;
+      const bool any_row = __any_sync(~0u, row_ok);
+      auto wait_pv = [&](int t) {
+        ok = warp_wait(at(Sh::bPV, qt, t), (t >> 1) & 1, abort);
+        tc_fence_after();
+        return ok;
+      };
+
+      for (int t = 0; ok && t < steps; ++t) {
+        const int base = (s0 + t) * kKeys;
+        const int vhi = limit - base >= kKeys ? kKeys : limit - base + 1;  // keys seen
+        const uint32_t sc = sc0 + kKeys * (t & 1);
+        // the values' power and bad groups come with the values (whose barrier
+        // cannot move on before this step's P is there)
+        ok = warp_wait(at(Sh::bS, qt, t), (t >> 1) & 1, abort) &&
+             warp_wait(mb + Sh::bV + 8 * (t & 1), (t >> 1) & 1, abort);
+        if (!ok) break;  // a wait expired
+        tc_fence_after();
+        uint32_t v[VC];
+        // both threads of a row leave this way together
+        if (!any_row || __all_sync(~0u, vhi <= 0)) {  // nothing to see for these 32 rows
+#pragma unroll
+          for (int c = 0; c < 16; ++c) v[c] = 0u;
+#pragma unroll
+          for (int cc = 0; cc < VC / 32; ++cc) CS_TMEM_ST16(sc + 16 * (part2 + cc), v);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(at(Sh::bP, qt, t));
+          continue;
+        }
+        CS_TMEM_LD32(sc + 32 * part2, v);
+        if constexpr (TPR == 1) CS_TMEM_LD32(sc + 32, (v + 32));
+        const float power = val_power[t % kInfo];
+        const float factor = fmaxf(row_factor * key_scale[t % kInfo], 1e-30f);
+        tmem_wait_ld();
+        if (!__all_sync(~0u, vhi >= kKeys)) {
+#pragma unroll
+          for (int cc = 0; cc < VC / 32; ++cc) {
+            const uint32_t bits = col_bits(0, vhi, 32 * (part2 + cc));
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              v[32 * cc + c] = (bits >> c) & 1u ? v[32 * cc + c] : 0xff800000u;  // -inf
+          }
+        }
+        if (flag[t % kInfo] == t + 1) {
+          for (int c = 0; c < VC; ++c) {
+            const int key = 32 * part2 + c;
+            if (key < vhi) poison |= bad[(t % kInfo) * kKeys + key];
+          }
+        }
+        float top;
+        {
+          float m[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            m[k] = max_nan(__uint_as_float(v[k]), __uint_as_float(v[k + 4]));
+#pragma unroll
+          for (int c = 8; c < VC; c += 8) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              m[k] = max3_nan(m[k], __uint_as_float(v[c + k]), __uint_as_float(v[c + k + 4]));
+          }
+          top = max_nan(max3_nan(m[0], m[1], m[2]), m[3]);
+        }
+        // the row's maximum from both its threads; past this barrier both have
+        // read their scores, so P may take their columns
+        if constexpr (TPR == 2) {
+          float* mx = row_max + (exchanges & 1) * 256;
+          mx[part2 * 128 + r] = top;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(pair);
+          ok = warp_wait(pair, exchanges & 1, abort);
+          if (!ok) break;
+          ++exchanges;
+          top = max_nan(top, mx[(1 - part2) * 128 + r]);
+        }
+        if (!(top < INFINITY)) {  // a NaN or +inf score makes the row NaN
+          lsum = __int_as_float(0x7fffffff);
+          top = -INFINITY;
+        }
+        const float top2 = top == -INFINITY ? -INFINITY : fmaf(top, factor, power);
+        const bool grow = top2 > mref + kLazy || mref == -INFINITY;
+        const bool rescale = grow && mref > -INFINITY && top2 > mref;
+        if (__any_sync(~0u, rescale)) {  // t > 0: a row has a finite maximum
+          if (!wait_pv(t - 1)) break;
+          const float f = rescale ? ex2(mref - top2) : 1.f;
+          lsum *= f;
+          uint32_t o[16];
+#pragma unroll 1
+          for (int cc = 0; cc < D / 16 / TPR; ++cc) {
+            const uint32_t col = oc + part2 * (D / 2) + 16 * cc;
+            CS_TMEM_LD16(col, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
+            CS_TMEM_ST16(col, o);
+          }
+          tmem_wait_st();
+        }
+        if (grow) mref = top2;
+        const float sub = (mref > -INFINITY ? mref : 0.f) - kUp - power;
+        const float2 scale = make_float2(factor, factor), off = make_float2(-sub, -sub);
+        float2 p0 = make_float2(0.f, 0.f), p1 = p0;
+#pragma unroll
+        for (int c = 0; c < VC; c += 2) {
+          const float2 x = __ffma2_rn(
+              make_float2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale, off);
+          v[c] = __float_as_uint(x.x);
+          v[c + 1] = __float_as_uint(x.y);
+        }
+#pragma unroll
+        for (int c = 0; c < VC; ++c) v[c] = __float_as_uint(ex2(__uint_as_float(v[c])));
+#pragma unroll
+        for (int c = 0; c < VC; c += 4) {
+          p0 = __fadd2_rn(p0, make_float2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])));
+          p1 = __fadd2_rn(p1, make_float2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])));
+        }
+#pragma unroll
+        for (int c = 0; c < VC / 2; ++c)
+          v[c] = Pack2<__half>::pack(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1]));
+#pragma unroll
+        for (int cc = 0; cc < VC / 32; ++cc) CS_TMEM_ST16(sc + 16 * (part2 + cc), (v + 16 * cc));
+        lsum = fmaf((p0.x + p0.y) + (p1.x + p1.y), ex2(-power), lsum);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(at(Sh::bP, qt, t));
+      }
+
+      // -------------------------------------------------------------- output
+      if (ok && steps > 0) wait_pv(steps - 1);
+      if constexpr (TPR == 2) {  // the row's sum and bad groups from both its threads
+#pragma unroll
+        for (int turn = 0; turn < 2; ++turn) {
+          float* both = row_max + (exchanges & 1) * 256;
+          both[part2 * 128 + r] = turn ? __uint_as_float(poison) : lsum;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(pair);
+          ok = ok && warp_wait(pair, exchanges & 1, abort);
+          ++exchanges;
+          const float other = both[(1 - part2) * 128 + r];
+          if (turn) poison |= __float_as_uint(other);
+          else lsum += other;
+        }
+      }
+      const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+      const float lse2 =
+          lsum == 0.f ? -INFINITY : (mref > -INFINITY ? mref : 0.f) - kUp + log2f(lsum);
+      const int tok = (row0 + row) / a.G, h = g * a.G + (row0 + row - tok * a.G);
+      const int64_t prow = part * RT + row;
+      char* orow = whole ? a.out + (int64_t)(rq.start + tok) * a.ot + (int64_t)h * a.oh
+                         : reinterpret_cast<char*>(a.part_o + prow * D);
+      const bool have = ok && steps > 0 && lsum != 0.f;
+      const bool write = ok && row_ok;
+      // element d of this thread's columns, which are loaded from column c0 on
+      auto final = [&](const uint32_t* v, int c0, int d) {
+        const float x = __uint_as_float(v[(d & ~7) + place8(d & 7)]);
+        const int group = (part2 * (D / 2) + c0 + d) / 32 / WG;
+        return poison >> group & 1u ? __int_as_float(0x7fffffff) : have ? x * inv : 0.f;
+      };
+      if (!whole || a.vec_out) {
+        // each thread stages its row where the queries were, and the warp
+        // writes whole rows: 32-bit partials in two halves
+        constexpr int B = 2 * D / TPR;  // bytes of a row a thread stages at once
+        constexpr int L = B / 16;       // lanes that write them
+        constexpr int WR = 2 * D + 16;
+        const uint32_t stage = sbase + Sh::oQ + qt * Sh::QB + (r - lane) * WR + part2 * B;
+        const uint32_t buf = stage + lane * WR;
+        const uint64_t to = write ? reinterpret_cast<uint64_t>(orow) : 0;
+#pragma unroll 1
+        for (int round = 0; round < (whole ? 1 : 2); ++round) {
+          uint32_t v[32];
+          const uint32_t col = oc + part2 * (D / 2);
+          if (!whole) {
+#pragma unroll
+            for (int cc = 0; cc < B / 64; ++cc) {
+              const int c0 = round * (B / 4) + 16 * cc;
+              CS_TMEM_LD16(col + c0, v);
+              tmem_wait_ld();
+#pragma unroll
+              for (int d = 0; d < 16; d += 4)
+                st_shared16(buf + 64 * cc + 4 * d,
+                            make_uint4(__float_as_uint(final(v, c0, d)),
+                                       __float_as_uint(final(v, c0, d + 1)),
+                                       __float_as_uint(final(v, c0, d + 2)),
+                                       __float_as_uint(final(v, c0, d + 3))));
+            }
+          } else {
+#pragma unroll
+            for (int cc = 0; cc < B / 64; ++cc) {
+              CS_TMEM_LD32(col + 32 * cc, v);
+              tmem_wait_ld();
+#pragma unroll
+              for (int d = 0; d < 32; d += 8) {
+                uint32_t y[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  y[k] = Pack2<T>::pack(final(v, 32 * cc, d + 2 * k), final(v, 32 * cc, d + 2 * k + 1));
+                st_shared16(buf + 64 * cc + 2 * d, make_uint4(y[0], y[1], y[2], y[3]));
+              }
+            }
+          }
+          __syncwarp();
+          // a partial's thread has two rounds, an output's one
+          const int64_t at0 = whole ? part2 * B : (part2 * 2 + round) * B;
+#pragma unroll
+          for (int n0 = 0; n0 < L; n0 += 4) {
+            uint4 x[4];
+            uint64_t dst[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              const int rw = (n0 + n) * (32 / L) + lane / L;
+              dst[n] = __shfl_sync(~0u, to, rw);
+              x[n] = ld_shared16(stage + rw * WR + 16 * (lane % L));
+            }
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              if (!dst[n]) continue;
+              uint2* y = reinterpret_cast<uint2*>(dst[n] + at0 + 16 * (lane % L));
+              y[0] = make_uint2(x[n].x, x[n].y);
+              y[1] = make_uint2(x[n].z, x[n].w);
+            }
+          }
+          __syncwarp();
+        }
+      } else {
+#pragma unroll 1
+        for (int cc = 0; cc < D / 32 / TPR; ++cc) {
+          uint32_t v[32];
+          const int col = part2 * (D / 2) + 32 * cc;
+          CS_TMEM_LD32(oc + col, v);
+          tmem_wait_ld();
+          if (!write) continue;
+#pragma unroll
+          for (int d = 0; d < 32; ++d)
+            reinterpret_cast<T*>(orow)[col + d] = Elem<T>::from_f(final(v, 32 * cc, d));
+        }
+      }
+      if (write && part2 == 0) {
+        if (whole) write_lse(a, rq.start, row0 + row, g, lse2);
+        else a.part_lse[prow] = lse2;
+      }
+    }
+
+    // nothing of this tile is in flight or in use behind this
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (!whole) {
+      if (s0 == 0)  // the first of the tile's blocks has them joined
+        join = make_int4(work.request, work.tile, 2 * g + which,
+                         blockIdx.x + (int)((all_steps - s1 + work.per - 1) / work.per));
+      which = 1;
+    }
+    if (*abort) break;
+    work.todo -= s1 - s0;
+    if (work.todo > 0) work.next(a);
+  }
+  if (tid == 0) a.joins[blockIdx.x] = join;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (bad_block) report(a.status, CS_ST_SLOT_RANGE);
+  if (tid == 0 && *abort) report(a.status, CS_ST_TIMEOUT);
+  if (warp == Sh::kSoft + 4) {
+    tc_fence_after();
+    tmem_dealloc(tmem, Sh::kCols);
+  }
+}
+
+template <typename T, int D, int NG, int NT>
+int launch_wide(const Attn4& a, int workers, cudaStream_t stream) {
+  using Sh = Shape4<D, NT>;
+  constexpr auto kernel = kv4_sm100_kernel<T, D, NG, NT>;
+  if (!allow_smem<kernel>(Sh::kSmem)) return CS_ERR_CUDA;
+  if (const int rc = launch_dependent(kernel, dim3(workers), Sh::kThreads, Sh::kSmem, stream, a))
+    return rc;
+  return launch_join<T, D, kTileRows * NT>(a, workers, stream);
+}
+
+}  // namespace
+
+int kv4_wide(const Attn4& a, const cs_kv4_pool& pool, int rows, int workers, cudaStream_t stream) {
+  return by_pool4(pool, [&](auto* t, auto d, auto g) -> int {
+    using T = std::remove_pointer_t<decltype(t)>;
+    constexpr int D = decltype(d)::value, NG = decltype(g)::value;
+    return rows > kTileRows ? launch_wide<T, D, NG, 2>(a, workers, stream)
+                            : launch_wide<T, D, NG, 1>(a, workers, stream);
+  });
+}
+
+}  // namespace cs

@@ -122,19 +122,6 @@ struct Shape {
   static constexpr uint32_t cS = 0, cO = 128 * NT;
 };
 
-// the larger of the two, NaN if either is
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float y;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-  return y;
-}
-
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
-  float y;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-  return y;
-}
-
 struct Step {
   int base, n, own;  // first key, keys, 1: own keys
 };
@@ -145,45 +132,6 @@ __device__ __forceinline__ Step step_of(const PrefixItem& it, int na, int t) {
   const int end = s.own ? it.b1 : it.a1;
   s.n = end - s.base < kKeys ? end - s.base : kKeys;
   return s;
-}
-
-// bits lo .. hi - 1 of the 32 columns from col0 on
-__device__ __forceinline__ uint32_t col_bits(int lo, int hi, int col0) {
-  lo = lo - col0 < 0 ? 0 : lo - col0;
-  hi = hi - col0 > 32 ? 32 : hi - col0;
-  if (hi <= lo) return 0u;
-  const uint32_t up = hi == 32 ? ~0u : (1u << hi) - 1u;
-  return up & ~((1u << lo) - 1u);
-}
-
-// the same lane of a whole warp every time
-__device__ __forceinline__ bool elect_one() {
-  uint32_t p;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "elect.sync _|p, 0xffffffff;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(p));
-  return p != 0;
-}
-// bounded wait of a whole warp; a phase that is over already costs one test
-// (the clock and the abort flag are read only when it is not)
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
-  if (__all_sync(~0u, mbar_try(bar, parity))) return true;
-  return __all_sync(~0u, mbar_wait(bar, parity, abort));
-}
-__device__ __forceinline__ void st_shared16(uint32_t dst, uint4 v) {
-  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z),
-               "r"(v.w)
-               : "memory");
-}
-__device__ __forceinline__ uint4 ld_shared16(uint32_t src) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(src)
-               : "memory");
-  return v;
 }
 
 // where the keys of one lane (2 consecutive keys of a tile) come from

@@ -150,7 +150,7 @@ def _batch(cuda, seed, new, lengths, hq, hk, dim, group, block, dtype, spare=2, 
 
 def _wide(new, heads):
     """Whether the kernel for many query rows a KV head takes such a batch."""
-    return False
+    return len(new) > 0 and sum(new) * heads // len(new) > 16
 
 
 def _check(got, lse, pool, table, q, starts, lengths, scale, wide, rows=None):
