@@ -153,6 +153,7 @@ template <int RT, int KT>
 struct Share4 {
   int request, tile, head, step;  // where the worker begins
   int64_t todo, per;              // steps it takes, and every one takes at most
+  int taken;                      // (the caller's) of them, from the present tile
   Request4 r;
 
   static __device__ __forceinline__ int tiles(const Request4& r, int G) {

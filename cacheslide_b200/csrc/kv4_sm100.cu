@@ -16,7 +16,9 @@
 // and values by one a step (of what the step's scales and lowest values can
 // reach), so bfloat16 pools of any size of numbers keep fp16's 11 bits, where
 // bfloat16 operands would keep 8.  P carries the values' power of two, the
-// rows' sums do not.
+// rows' sums do not.  Float16 outputs show the rounding of such keys (0.00047 to
+// 0.00054 off, 0.00021 of which is the output's own), so the keys of float16
+// pools are two operands, scale (code - zero) and what is left.
 //
 // Pairs lie in the tiles as the codes come, elements (0, 4), (1, 5), (2, 6), (3,
 // 7) of eight: the queries are written in the same order, and the output's
@@ -39,34 +41,75 @@ constexpr float kLazy = 8.f;      // O is rescaled when the maximum grew by more
 constexpr float kUp = 7.f;        // P is stored up by 2^7: fp16's normal numbers reach 2^-21
 constexpr int kInfo = 4;          // steps whose scales are kept
 
-template <int D, int NT>
+// TERMS 2: key tiles in two parts (float16 pools)
+template <int D, int NG, int NT, int TERMS>
 struct Shape4 {
   // threads a row in the softmax, as in the wide blocks of the shared-prefix kernel
   static constexpr int TPR = NT;
   static constexpr int kTile = kTileRows * TPR;  // softmax threads of a row tile
-  static constexpr int kSoft = 4 * NT * TPR;     // softmax warps, then 2 K, 2 V, NT MMA warps
-  static constexpr int kThreads = 32 * (kSoft + 4 + NT);
-  static constexpr uint32_t TB = kKeys * D * 2;  // a K or V tile, two of each
+  // the softmax warps, then a warpgroup of 2 K and 2 V warps, and one of the
+  // loader and NT MMA warps
+  static constexpr int kSoft = 4 * NT * TPR;
+  static constexpr int kThreads = 32 * (kSoft + 8);
+  // registers: the launch's share, then the softmax's, the producers', the rest's
+  static constexpr int kLaunchRegs = 80, kSoftRegs = NT == 1 ? 112 : 88,
+                       kMakeRegs = 72, kRestRegs = 56;
+  static_assert(kSoft * kSoftRegs + 4 * (kMakeRegs + kRestRegs) <= (kSoft + 8) * kLaunchRegs,
+                "more registers than the block is launched with");
+  static constexpr uint32_t TB = kKeys * D * 2;  // a V tile, or a part of a K tile
+  static constexpr uint32_t RB = (kKeys / kUnit) * Unit4<D, NG>::kBytes;  // a step's raw units
+  // stages of K and V tiles, and of raw units (two blocks of one row tile share an SM)
+  static constexpr int KS = NT == 1 && TERMS == 2 ? 1 : 2, VS = 2, RS = NT == 1 ? 1 : 3;
   // a query tile's place also takes its output rows, 2 D bytes each and 16 more
   static constexpr uint32_t QB = kTileRows * D * 2 + kTileRows * 16;
-  static constexpr uint32_t oQ = 0, oK = NT * QB, oV = oK + 2 * TB, oMeta = oV + 2 * TB;
+  static constexpr uint32_t oQ = 0, oK = NT * QB, oV = oK + KS * TERMS * TB, oR = oV + VS * TB,
+                            oMeta = oR + RS * RB;
   // barriers: queries; a stage's K and V; a score buffer's S, P and PV of a row
-  // tile; a row's maxima
+  // tile; a row's maxima; raw units there, and read
   static constexpr uint32_t bQ = 0, bK = 8, bV = bK + 16, bS = bV + 16, bP = bS + 16 * NT,
-                            bPV = bP + 16 * NT, bMax = bPV + 16 * NT, oTmem = bMax + 32 * NT,
+                            bPV = bP + 16 * NT, bMax = bPV + 16 * NT, bR = bMax + 32 * NT,
+                            bRead = bR + 8 * RS, oTmem = bRead + 8 * RS,
                             oAbort = oTmem + 4, oFlag = oAbort + 4, oScale = oFlag + 4 * kInfo,
                             oPower = oScale + 4 * kInfo, oReach = oPower + 4 * kInfo,
                             oBad = oReach + 32, oRow = oBad + kInfo * kKeys,
                             oMax = oRow + NT * kTileRows * 4,
-                            oSums = (oMax + NT * 2 * 2 * 128 * 4 + 7) / 8 * 8,
+                            oSeg = oMax + (TPR - 1) * NT * 2 * 2 * 128 * 4,
+                            oSums = (oSeg + 48 + 7) / 8 * 8,
                             kMeta = oSums + (128 + 1 + 4) * 8;
-  static_assert(oMeta % 1024 == 0 && oTmem % 4 == 0 && oRow % 4 == 0, "alignment");
+  static_assert(oR % 1024 == 0 && RB % 128 == 0 && oTmem % 4 == 0 && oRow % 4 == 0, "alignment");
   static constexpr uint32_t kSmem = oMeta + kMeta + 1024;  // the base is rounded up to 1024
+  static_assert(kSmem <= (NT == 1 ? 115712 : 232448), "shared memory");
   static constexpr uint32_t kCols = 256 * NT;
   // two score buffers of 64 columns at 128 i for row tile i, O at cO + D i
   static constexpr uint32_t cS = 0, cO = 128 * NT;
 };
 
+struct Segment {  // of a row tile's steps, for a block
+  int request, start;       // its first token's row
+  int g, row0, rows, tiles; // KV head, first row, rows and row tiles
+  int s0, steps;            // -1: no more
+  int seen, first_limit;    // keys its last token sees; the newest key of token 0
+  int part;                 // place of its partial results; -1: writes the output
+};
+
+template <int R> __device__ __forceinline__ void regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R));
+}
+template <int R> __device__ __forceinline__ void regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
+}
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes,
+                                          uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void arrive_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
 __device__ __forceinline__ void pair_sync(bool v) {  // the two warps of a producer
   if (v) asm volatile("bar.sync 2, 64;" ::: "memory");
@@ -91,6 +134,24 @@ __device__ __forceinline__ uint4 decode8(uint32_t w, __half2 scale, __half2 low)
 // where element d of eight lies in that order
 __host__ __device__ constexpr int place8(int d) { return 2 * (d & 3) + (d >> 2 & 1); }
 
+// the same in two parts: scale (code - zero), for a scale of 7 significant bits
+// exact, and low + more (code - zero); `zero` is 1024 + the code nearest to zero
+__device__ __forceinline__ void decode8(uint32_t w, __half2 scale, __half2 more, __half2 low,
+                                        __half2 zero, uint4& main, uint4& rest) {
+  const uint32_t magic = 0x64006400u;
+  const __half2 sixteenth = as_half2(0x2c002c00u), k960 = as_half2(0x63806380u);
+  const __half2 zero16 = __hsub2(k960, zero);  // -(64 + the code)
+  const uint32_t y = w >> 8;
+  const __half2 a = __hsub2(as_half2((w & 0x000f000fu) | magic), zero);
+  const __half2 b = __hfma2(as_half2((w & 0x00f000f0u) | magic), sixteenth, zero16);
+  const __half2 c = __hsub2(as_half2((y & 0x000f000fu) | magic), zero);
+  const __half2 d = __hfma2(as_half2((y & 0x00f000f0u) | magic), sixteenth, zero16);
+  main = make_uint4(as_u32(__hmul2(a, scale)), as_u32(__hmul2(b, scale)), as_u32(__hmul2(c, scale)),
+                    as_u32(__hmul2(d, scale)));
+  rest = make_uint4(as_u32(__hfma2(a, more, low)), as_u32(__hfma2(b, more, low)),
+                    as_u32(__hfma2(c, more, low)), as_u32(__hfma2(d, more, low)));
+}
+
 template <int N>
 __device__ __forceinline__ void load_words(uint32_t (&w)[N], const char* p) {
   if constexpr (N == 4) {
@@ -105,11 +166,13 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[N], const char* p) {
 }
 
 template <typename T, int D, int NG, int NT>
-__global__ void __launch_bounds__(Shape4<D, NT>::kThreads, NT == 1 ? 2 : 1)
+__global__ void __launch_bounds__(
+    Shape4<D, NG, NT, std::is_same<T, __half>::value ? 2 : 1>::kThreads, NT == 1 ? 2 : 1)
     kv4_sm100_kernel(const __grid_constant__ Attn4 a) {
-  using Sh = Shape4<D, NT>;
+  constexpr int TERMS = std::is_same<T, __half>::value ? 2 : 1;
+  using Sh = Shape4<D, NG, NT, TERMS>;
   using U = Unit4<D, NG>;
-  constexpr int RT = kTileRows * NT, W = U::W, WG = W / NG;
+  constexpr int RT = kTileRows * NT, W = U::W, WG = W / NG, KS = Sh::KS, RS = Sh::RS;
   using Share = Share4<RT, kKeys>;
   extern __shared__ char smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -125,7 +188,7 @@ __global__ void __launch_bounds__(Shape4<D, NT>::kThreads, NT == 1 ? 2 : 1)
   float* row_scale = reinterpret_cast<float*>(meta + Sh::oRow);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  if (warp == Sh::kSoft + 4) tmem_alloc(mb + Sh::oTmem, Sh::kCols);
+  if (warp == Sh::kSoft + 5) tmem_alloc(mb + Sh::oTmem, Sh::kCols);
   if (tid == 0) *abort = 0;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   Share work;
@@ -136,90 +199,60 @@ __global__ void __launch_bounds__(Shape4<D, NT>::kThreads, NT == 1 ? 2 : 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(meta + Sh::oTmem);
-  bool bad_block = false, first = true;
-  int which = 0;  // of this block's partial results
-  int4 join = make_int4(-1, 0, 0, 0);
 
-  while (work.todo > 0) {
-    const Request4 rq = work.r;
-    const int all_steps = Share::steps(rq, a.G, work.tile);
-    const int s0 = work.step;
-    const int s1 = (int)min((int64_t)all_steps, s0 + work.todo);
-    const int row0 = work.tile * RT, rows = min(RT, rq.n * a.G - row0), g = work.head;
-    const int tiles = rows > kTileRows ? 2 : 1;
-    const int seen = max(0, rq.len - rq.n + Share::last_token(rq, a.G, work.tile) + 1);
-    const int steps = min(s1, (seen + kKeys - 1) / kKeys) - s0;  // with keys to see
-    const bool whole = s0 == 0 && s1 == all_steps;
-    const int64_t part = 2ll * blockIdx.x + which;
-    if (tid == 0) {
-      if (!first)
-        for (uint32_t b = Sh::bQ; b < Sh::oTmem; b += 8) mbar_inval(mb + b);
-      mbar_init(mb + Sh::bQ, Sh::kTile * tiles);
-      for (int s = 0; s < 2; ++s) {
-        mbar_init(mb + Sh::bK + 8 * s, 64);
-        mbar_init(mb + Sh::bV + 8 * s, 64);
-      }
-      for (int s = 0; s < 2 * NT; ++s) {
-        mbar_init(mb + Sh::bS + 8 * s, 1);
-        mbar_init(mb + Sh::bP + 8 * s, Sh::kTile);
-        mbar_init(mb + Sh::bPV + 8 * s, 1);
-      }
-      for (int s = 0; s < 4 * NT; ++s) mbar_init(mb + Sh::bMax + 8 * s, 2);
-      mbar_init_fence();
-      for (int s = 0; s < kInfo; ++s) flag[s] = 0;
+  // step t uses score buffer t & 1 of its row tile
+  auto at = [&](uint32_t bar, int qt, int t) { return mb + bar + 8 * (2 * qt + (t & 1)); };
+  // Every role walks the block's segments, each between two barriers of the
+  // block; the loader says what is next (in shared memory: the other roles have
+  // no registers for the division of the work).
+  const Segment& seg = *reinterpret_cast<const Segment*>(meta + Sh::oSeg);
+  auto segments = [&](auto next, auto role) {
+    while (true) {
+      next();
+      __syncthreads();
+      if (seg.steps < 0 || *abort) break;
+      role();
+      // nothing of this tile is in flight or in use behind this
+      tc_fence_before();
+      __syncthreads();
+      tc_fence_after();
     }
-    first = false;
-    __syncthreads();
-    // step t uses score buffer t & 1 of its row tile
-    auto at = [&](uint32_t bar, int qt, int t) { return mb + bar + 8 * (2 * qt + (t & 1)); };
+  };
+  auto follow = [] {};
 
-    if (warp >= Sh::kSoft && warp < Sh::kSoft + 4) {
-      // =========================================== producers: K, then V pair
-      const bool isv = warp >= Sh::kSoft + 2;
-      const int i = (tid - 32 * Sh::kSoft) & 63;
-      // this thread's part of 16 keys' rows: token r, W words from word W c on
-      const int r = (i & 7) + 8 * (i >> 5), c = (i >> 3) & 3;
-      const int32_t* table = a.tables + work.request * a.table_stride;
-      const int units = (seen + kUnit - 1) / kUnit;
-      int64_t from = -1;  // this lane's unit of eight steps: -1 none, 0 no block
-      uint32_t code[4][W], pair[4][NG];
-      auto fetch = [&](int t) {
-        if (t >= steps) return;
-        if (t % 8 == 0) {
-          const int u = (s0 + t) * (kKeys / kUnit) + lane, j = u / a.pool.units;
-          from = -1;
-          if (u < units) {
-            const int id = table[j];
-            from = id >= 0 && id < a.pool.num_blocks
-                       ? reinterpret_cast<int64_t>(a.pool.unit(id, g, u - j * a.pool.units))
-                       : 0;
-            bad_block |= from == 0;
-          }
-        }
+  if (warp >= Sh::kSoft && warp < Sh::kSoft + 4) {
+    // ============================================= producers: K, then V pair
+    if constexpr (Sh::kMakeRegs > Sh::kLaunchRegs) regs_up<Sh::kMakeRegs>();
+    else regs_down<Sh::kMakeRegs>();
+    const bool isv = warp >= Sh::kSoft + 2;
+    const int i = (tid - 32 * Sh::kSoft) & 63;
+    // this thread's part of 16 keys' rows: token r, W words from word W c on
+    const int r = (i & 7) + 8 * (i >> 5), c = (i >> 3) & 3;
+    segments(follow, [&] {
+      const int steps = seg.steps, seen = seg.seen, first_key = seg.s0 * kKeys + r;
+      for (int t = 0; t < steps; ++t) {
+        uint32_t code[4][W], pair[4][NG];
+        if (!warp_wait(mb + Sh::bR + 8 * (t % RS), (t / RS) & 1, abort)) break;
+        const char* units = smem + Sh::oR + (t % RS) * Sh::RB;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int64_t unit = __shfl_sync(~0u, from, (t % 8) * 4 + j);
-          const int key = (s0 + t) * kKeys + j * kUnit + r;
-          if (unit > 0 && key < seen) {
-            const char* p = reinterpret_cast<const char*>(unit);
-            load_words(code[j], p + (isv ? U::oV : 0) + r * U::kRow + 4 * W * c);
-            load_words(pair[j], p + (isv ? U::oVp : U::oKp) + 4 * NG * r);
-          } else {  // zeros: P is zero there too
-#pragma unroll
-            for (int w = 0; w < W; ++w) code[j][w] = 0u;
-#pragma unroll
-            for (int k = 0; k < NG; ++k) pair[j][k] = 0u;
-          }
+          const char* p = units + j * U::kBytes;
+          load_words(code[j], p + (isv ? U::oV : 0) + r * U::kRow + 4 * W * c);
+          load_words(pair[j], p + (isv ? U::oVp : U::oKp) + 4 * NG * r);
         }
-      };
-      fetch(0);
-      for (int t = 0; t < steps; ++t) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(mb + Sh::bRead + 8 * (t % RS));
         // ------------------------------- the step's power of two, bad values
+        const int key0 = first_key + t * kKeys;
         float2 f[4][NG];
         float reach = 0.f;
         uint32_t wrong = 0u;  // bit NG j + k
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+          if (key0 + j * kUnit >= seen) {  // zeros: P is zero there too
+#pragma unroll
+            for (int k = 0; k < NG; ++k) pair[j][k] = 0u;
+          }
 #pragma unroll
           for (int k = 0; k < NG; ++k) {
             f[j][k] = pair_of<T>(pair[j][k]);
@@ -234,7 +267,7 @@ __global__ void __launch_bounds__(Shape4<D, NT>::kThreads, NT == 1 ? 2 : 1)
           }
         }
         int e = 0;
-        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        if constexpr (TERMS == 1) {
           const uint32_t m = __reduce_max_sync(~0u, __float_as_uint(reach));
           volatile uint32_t* both = reinterpret_cast<volatile uint32_t*>(meta + Sh::oReach) +
                                     (isv ? 4 : 0) + 2 * (t & 1);
@@ -245,46 +278,181 @@ __global__ void __launch_bounds__(Shape4<D, NT>::kThreads, NT == 1 ? 2 : 1)
         }
         const float down = pow2(-e);
         // --------------------------------------------------- a free stage
-        if (t >= 2) {
+        const int stages = isv ? Sh::VS : KS;
+        if (t >= stages) {
+          const int u = t - stages;
           bool ok = true;
-          for (int qt = 0; qt < tiles; ++qt)
-            ok = ok && warp_wait(at(isv ? Sh::bPV : Sh::bS, qt, t), (t / 2 - 1) & 1, abort);
+          for (int qt = 0; qt < seg.tiles; ++qt)
+            ok = ok && warp_wait(at(isv ? Sh::bPV : Sh::bS, qt, u), (u >> 1) & 1, abort);
           if (!ok) break;
         }
         if (i == 0) {
           if (isv) val_power[t % kInfo] = (float)e;
           else key_scale[t % kInfo] = pow2(e);
         }
-        const uint32_t tile = sbase + (isv ? Sh::oV : Sh::oK) + (t & 1) * Sh::TB;
+        if (isv) {
+          const uint32_t tile = sbase + Sh::oV + (t % Sh::VS) * Sh::TB;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          __half2 scale[NG], low[NG];
+          for (int j = 0; j < 4; ++j) {
 #pragma unroll
-          for (int k = 0; k < NG; ++k) {
-            scale[k] = __float2half2_rn(f[j][k].x * down);
-            low[k] = __float2half2_rn(f[j][k].y * down);
+            for (int w = 0; w < W; ++w) {
+              const uint32_t x = __byte_perm(code[j][w / 2], code[j][W / 2 + w / 2],
+                                             w & 1 ? 0x7632u : 0x5410u);
+              st_shared16(tile + sw128(j * kUnit + r, 4 * w + c, kKeys),
+                          decode8(x, __float2half2_rn(f[j][w / WG].x * down),
+                                  __float2half2_rn(f[j][w / WG].y * down)));
+            }
+            if (c == 0)
+              bad[(t % kInfo) * kKeys + j * kUnit + r] =
+                  (uint8_t)(wrong >> (NG * j) & ((1u << NG) - 1u));
           }
+          if (wrong) flag[t % kInfo] = t + 1;
+        } else {
+          const uint32_t tile = sbase + Sh::oK + (t % KS) * TERMS * Sh::TB;
 #pragma unroll
-          for (int w = 0; w < W; ++w) {
-            const uint32_t x = isv ? __byte_perm(code[j][w / 2], code[j][W / 2 + w / 2],
-                                                 w & 1 ? 0x7632u : 0x5410u)
-                                   : code[j][w];
-            st_shared16(tile + sw128(j * kUnit + r, 4 * w + c, kKeys),
-                        decode8(x, scale[w / WG], low[w / WG]));
+          for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+              const uint32_t to = tile + sw128(j * kUnit + r, 4 * w + c, kKeys);
+              const float2 y = f[j][w / WG];
+              if constexpr (TERMS == 1) {
+                st_shared16(to, decode8(code[j][w], __float2half2_rn(y.x * down),
+                                        __float2half2_rn(y.y * down)));
+              } else {
+                const uint32_t main = (pair[j][w / WG] + 8u) & 0xfff0u;  // 7 significant bits
+                const float zero = fminf(fmaxf(rintf(-y.y * rcp_approx(y.x)), 0.f), 15.f);
+                uint4 x, rest;
+                decode8(code[j][w], as_half2(main * 0x10001u),
+                        __float2half2_rn(y.x - pair_of<T>(main).x),
+                        __float2half2_rn(fmaf(zero, y.x, y.y)), __float2half2_rn(1024.f + zero), x,
+                        rest);
+                st_shared16(to, x);
+                st_shared16(to + Sh::TB, rest);
+              }
+            }
           }
-          if (isv && c == 0)
-            bad[(t % kInfo) * kKeys + j * kUnit + r] = (uint8_t)(wrong >> (NG * j) & ((1u << NG) - 1u));
         }
-        if (isv && wrong) flag[t % kInfo] = t + 1;
-        fetch(t + 1);
         fence_async_smem();
-        mbar_arrive(mb + (isv ? Sh::bV : Sh::bK) + 8 * (t & 1));
+        mbar_arrive(mb + (isv ? Sh::bV + 8 * (t % Sh::VS) : Sh::bK + 8 * (t % KS)));
       }
+    });
 
-    } else if (warp >= Sh::kSoft + 4) {
-      // ================================================== MMA, one warp a tile
-      const int qt = __shfl_sync(~0u, warp, 0) - (Sh::kSoft + 4);
-      if (qt < tiles) {
+  } else if (warp == Sh::kSoft + 4) {
+    // ============================================================ the loader
+    regs_down<Sh::kRestRegs>();
+    bool bad_block = false, first = true;
+    int which = 0;  // of this block's partial results
+    int4 join = make_int4(-1, 0, 0, 0);
+    auto next = [&] {
+      Segment& s = *reinterpret_cast<Segment*>(meta + Sh::oSeg);
+      if (!first && work.todo > 0) {
+        work.todo -= work.taken;
+        if (work.todo > 0) work.next(a);
+      }
+      if (work.todo <= 0) {
+        if (lane == 0) s.steps = -1;
+        return;
+      }
+      const int all_steps = Share::steps(work.r, a.G, work.tile);
+      const int s1 = (int)min((int64_t)all_steps, work.step + work.todo);
+      const bool whole = work.step == 0 && s1 == all_steps;
+      work.taken = s1 - work.step;
+      if (lane == 0) {
+        s.start = work.r.start;
+        s.request = work.request;
+        s.g = work.head;
+        s.s0 = work.step;
+        s.row0 = work.tile * RT;
+        s.rows = min(RT, work.r.n * a.G - s.row0);
+        s.tiles = s.rows > kTileRows ? 2 : 1;
+        s.first_limit = work.r.len - work.r.n;
+        s.seen = max(0, s.first_limit + Share::last_token(work.r, a.G, work.tile) + 1);
+        s.steps = max(0, min(s1, (s.seen + kKeys - 1) / kKeys) - work.step);
+        s.part = whole ? -1 : 2 * (int)blockIdx.x + which;
+        if (!first)
+          for (uint32_t b = Sh::bQ; b < Sh::oTmem; b += 8) mbar_inval(mb + b);
+        mbar_init(mb + Sh::bQ, Sh::kTile * s.tiles);
+        for (int k = 0; k < 2; ++k) {
+          mbar_init(mb + Sh::bK + 8 * k, 64);
+          mbar_init(mb + Sh::bV + 8 * k, 64);
+        }
+        for (int k = 0; k < 2 * NT; ++k) {
+          mbar_init(mb + Sh::bS + 8 * k, 1);
+          mbar_init(mb + Sh::bP + 8 * k, Sh::kTile);
+          mbar_init(mb + Sh::bPV + 8 * k, 1);
+        }
+        for (int k = 0; k < 4 * NT; ++k) mbar_init(mb + Sh::bMax + 8 * k, 2);
+        for (int k = 0; k < RS; ++k) {
+          mbar_init(mb + Sh::bR + 8 * k, kKeys / kUnit);
+          mbar_init(mb + Sh::bRead + 8 * k, 4);
+        }
+        mbar_init_fence();
+        for (int k = 0; k < kInfo; ++k) flag[k] = 0;
+      }
+      if (!whole) {
+        if (work.step == 0)  // the first of the tile's blocks has them joined
+          join = make_int4(work.request, work.tile, 2 * work.head + which,
+                           blockIdx.x + (int)((all_steps - s1 + work.per - 1) / work.per));
+        which = 1;
+      }
+      first = false;
+    };
+    segments(next, [&] {
+      const int32_t* table = a.tables + seg.request * a.table_stride;
+      const int units = (seg.seen + kUnit - 1) / kUnit, steps = seg.steps, s0 = seg.s0, g = seg.g;
+      int64_t from = -1;  // this lane's unit of eight steps: -1 none, 0 no block
+      int issued = 0;
+      for (int t = 0; t < steps; ++t) {
+        if (t % 8 == 0) {
+          const int u = (s0 + t) * (kKeys / kUnit) + lane, j = u / a.pool.units;
+          from = -1;
+          if (u < units) {
+            const int id = table[j];
+            from = id >= 0 && id < a.pool.num_blocks
+                       ? reinterpret_cast<int64_t>(a.pool.unit(id, g, u - j * a.pool.units))
+                       : 0;
+            bad_block |= from == 0;
+          }
+        }
+        if (t >= RS &&
+            !warp_wait(mb + Sh::bRead + 8 * (t % RS), (t / RS - 1) & 1, abort))
+          break;
+        if (lane / 4 == t % 8) {
+          const uint32_t bar = mb + Sh::bR + 8 * (t % RS);
+          const uint32_t to = Sh::oR + (t % RS) * Sh::RB + (lane % 4) * U::kBytes;
+          if (from > 0) {
+            arrive_expect(bar, U::kBytes);
+            bulk_copy(sbase + to, reinterpret_cast<const void*>(from), U::kBytes, bar);
+          } else {
+            if (from == 0) {  // zero codes, scales and lows: zero keys and values
+              for (int k = 0; k < U::kBytes / 16; ++k)
+                st_shared16(sbase + to + 16 * k, make_uint4(0, 0, 0, 0));
+              fence_async_smem();  // before a later copy into this place
+            }
+            mbar_arrive(bar);
+          }
+        }
+        __syncwarp();
+        issued = t + 1;
+      }
+      // nothing of this block's copies is in flight when it goes on
+      for (int t = issued - RS < 0 ? 0 : issued - RS; t < issued; ++t) {
+        const long long t0 = clock64();
+        while (!mbar_try(mb + Sh::bR + 8 * (t % RS), (t / RS) & 1) &&
+               clock64() - t0 < kWaitCycles) {
+        }
+      }
+      __syncwarp();
+    });
+    if (lane == 0) a.joins[blockIdx.x] = join;
+    if (bad_block) report(a.status, CS_ST_SLOT_RANGE);
+
+  } else if (warp > Sh::kSoft + 4) {
+    // ==================================================== MMA, one warp a tile
+    regs_down<Sh::kRestRegs>();
+    segments(follow, [&] {
+      const int qt = __shfl_sync(~0u, warp, 0) - (Sh::kSoft + 5), steps = seg.steps;
+      if (qt < seg.tiles) {
         const bool leader = elect_one();
         const uint32_t id_s = umma_idesc(128, kKeys, 0, 0, 0);
         const uint32_t id_o = umma_idesc(128, D, 0, 0, 1);  // V is MN-major
@@ -295,33 +463,37 @@ __global__ void __launch_bounds__(Shape4<D, NT>::kThreads, NT == 1 ? 2 : 1)
         const uint32_t sc = tm + Sh::cS + 128 * qt, oc = tm + Sh::cO + D * qt;
         bool ok = warp_wait(mb + Sh::bQ, 0, abort);
         uint32_t last = 0, lastph = 0;  // the newest group issued
-        auto arrived = [&](uint32_t bar, int t) {
-          ok = ok && warp_wait(mb + bar + 8 * (t & 1), (t / 2) & 1, abort);
+        auto arrived = [&](uint32_t bar, int t, int stages) {
+          ok = ok && warp_wait(mb + bar + 8 * (t % stages), (t / stages) & 1, abort);
           return ok;
         };
         auto scores = [&](int t) {
           tc_fence_after();
-          const uint64_t dk = dk0 + (uint64_t)((t & 1) * (Sh::TB >> 4));
-          const uint32_t s = sc + kKeys * (t & 1);
+          const uint64_t dk = dk0 + (uint64_t)((t % KS) * TERMS * (Sh::TB >> 4));
+          const uint32_t sb = sc + kKeys * (t & 1);
           last = at(Sh::bS, qt, t);
           lastph = (t >> 1) & 1;
           if (leader) {
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk)  // offsets in 16-byte units
-              tc_mma(s, dq + (kk >> 2) * 1024 + (kk & 3) * 2,
-                     dk + (kk >> 2) * (kKeys * 8) + (kk & 3) * 2, id_s, kk ? 1u : 0u);
+            for (int term = 0; term < TERMS; ++term) {
+#pragma unroll
+              for (int kk = 0; kk < D / 16; ++kk)  // offsets in 16-byte units
+                tc_mma(sb, dq + (kk >> 2) * 1024 + (kk & 3) * 2,
+                       dk + term * (Sh::TB >> 4) + (kk >> 2) * (kKeys * 8) + (kk & 3) * 2, id_s,
+                       term + kk ? 1u : 0u);
+            }
             tc_commit(last);
           }
           __syncwarp();
         };
-        if (steps > 0 && arrived(Sh::bK, 0)) scores(0);
-        if (steps > 1 && arrived(Sh::bK, 1)) scores(1);
+        if (steps > 0 && arrived(Sh::bK, 0, KS)) scores(0);
+        if (steps > 1 && arrived(Sh::bK, 1, KS)) scores(1);
         for (int t = 0; ok && t < steps; ++t) {
           const uint32_t ph = (t >> 1) & 1;
-          if (!arrived(Sh::bV, t)) break;
+          if (!arrived(Sh::bV, t, Sh::VS)) break;
           if (!(ok = warp_wait(at(Sh::bP, qt, t), ph, abort))) break;
           tc_fence_after();
-          const uint64_t dv = dv0 + (uint64_t)((t & 1) * (Sh::TB >> 4));
+          const uint64_t dv = dv0 + (uint64_t)((t % Sh::VS) * (Sh::TB >> 4));
           const uint32_t p = sc + kKeys * (t & 1);
           last = at(Sh::bPV, qt, t);
           lastph = ph;
@@ -334,7 +506,7 @@ __global__ void __launch_bounds__(Shape4<D, NT>::kThreads, NT == 1 ? 2 : 1)
           __syncwarp();
           // the next scores but one take the buffer that P lies in
           if (t + 2 < steps) {
-            if (!arrived(Sh::bK, t + 2)) break;
+            if (!arrived(Sh::bK, t + 2, KS)) break;
             if (!(ok = warp_wait(at(Sh::bPV, qt, t), ph, abort))) break;
             scores(t + 2);
           }
@@ -346,14 +518,19 @@ __global__ void __launch_bounds__(Shape4<D, NT>::kThreads, NT == 1 ? 2 : 1)
         }
       }
       __syncwarp();
+    });
 
-    } else if (warp / (4 * Sh::TPR) < tiles) {
-      // =============================================================== softmax
+  } else {
+    // ================================================================= softmax
+    regs_up<Sh::kSoftRegs>();
+    segments(follow, [&] {
+      if (warp / (4 * Sh::TPR) >= seg.tiles) return;
+      const int row0 = seg.row0, steps = seg.steps, s0 = seg.s0;
       constexpr int TPR = Sh::TPR, VC = kKeys / TPR;  // scores of a step a thread holds
       const int qt = warp / (4 * TPR), part2 = (warp >> 2) % TPR;
       const int r = (warp & 3) * 32 + lane;  // TMEM lane
       const int row = qt * kTileRows + r;    // of the block's
-      const bool row_ok = row < rows;
+      const bool row_ok = row < seg.rows;
       {
         // queries into the swizzled operand layout, a power of two a row
         constexpr int C = D / 8;
@@ -361,10 +538,10 @@ __global__ void __launch_bounds__(Shape4<D, NT>::kThreads, NT == 1 ? 2 : 1)
         const uint32_t qs = sbase + Sh::oQ + qt * Sh::QB;
         for (int m = (tid % Sh::kTile) / C; m < kTileRows; m += Sh::kTile / C) {
           const int rr = row0 + qt * kTileRows + m;
-          const bool ok = qt * kTileRows + m < rows;
+          const bool ok = qt * kTileRows + m < seg.rows;
           const int tk = ok ? rr / a.G : 0;
-          const char* p = a.q + (int64_t)(rq.start + tk) * a.qt +
-                          (int64_t)(g * a.G + (ok ? rr - tk * a.G : 0)) * a.qh + 16 * c;
+          const char* p = a.q + (int64_t)(seg.start + tk) * a.qt +
+                          (int64_t)(seg.g * a.G + (ok ? rr - tk * a.G : 0)) * a.qh + 16 * c;
           uint32_t x[4] = {0u, 0u, 0u, 0u};
           if (ok && a.vec_q) {
             load_words(x, p);
@@ -396,7 +573,7 @@ __global__ void __launch_bounds__(Shape4<D, NT>::kThreads, NT == 1 ? 2 : 1)
       bool ok = warp_wait(mb + Sh::bQ, 0, abort);
       const float row_factor = row_scale[qt * kTileRows + r] * a.scale2;
       // the newest key this row sees; no row: of no matter
-      const int limit = row_ok ? rq.len - rq.n + (row0 + row) / a.G : INT32_MAX;
+      const int limit = row_ok ? seg.first_limit + (row0 + row) / a.G : INT32_MAX;
       const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
       const uint32_t sc0 = tmem + lane_base + Sh::cS + 128 * qt;
       const uint32_t oc = tmem + lane_base + Sh::cO + D * qt;
@@ -551,9 +728,10 @@ __global__ void __launch_bounds__(Shape4<D, NT>::kThreads, NT == 1 ? 2 : 1)
       const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
       const float lse2 =
           lsum == 0.f ? -INFINITY : (mref > -INFINITY ? mref : 0.f) - kUp + log2f(lsum);
-      const int tok = (row0 + row) / a.G, h = g * a.G + (row0 + row - tok * a.G);
-      const int64_t prow = part * RT + row;
-      char* orow = whole ? a.out + (int64_t)(rq.start + tok) * a.ot + (int64_t)h * a.oh
+      const int tok = (row0 + row) / a.G, h = seg.g * a.G + (row0 + row - tok * a.G);
+      const bool whole = seg.part < 0;
+      const int64_t prow = (int64_t)seg.part * RT + row;
+      char* orow = whole ? a.out + (int64_t)(seg.start + tok) * a.ot + (int64_t)h * a.oh
                          : reinterpret_cast<char*>(a.part_o + prow * D);
       const bool have = ok && steps > 0 && lsum != 0.f;
       const bool write = ok && row_ok;
@@ -642,40 +820,37 @@ __global__ void __launch_bounds__(Shape4<D, NT>::kThreads, NT == 1 ? 2 : 1)
         }
       }
       if (write && part2 == 0) {
-        if (whole) write_lse(a, rq.start, row0 + row, g, lse2);
+        if (whole) write_lse(a, seg.start, row0 + row, seg.g, lse2);
         else a.part_lse[prow] = lse2;
       }
-    }
-
-    // nothing of this tile is in flight or in use behind this
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    if (!whole) {
-      if (s0 == 0)  // the first of the tile's blocks has them joined
-        join = make_int4(work.request, work.tile, 2 * g + which,
-                         blockIdx.x + (int)((all_steps - s1 + work.per - 1) / work.per));
-      which = 1;
-    }
-    if (*abort) break;
-    work.todo -= s1 - s0;
-    if (work.todo > 0) work.next(a);
+    });
   }
-  if (tid == 0) a.joins[blockIdx.x] = join;
+
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (bad_block) report(a.status, CS_ST_SLOT_RANGE);
   if (tid == 0 && *abort) report(a.status, CS_ST_TIMEOUT);
-  if (warp == Sh::kSoft + 4) {
+  if (warp == Sh::kSoft + 5) {
     tc_fence_after();
     tmem_dealloc(tmem, Sh::kCols);
   }
 }
 
+// The register split inside the kernel is made for a launch at this many a
+// thread: with another number a warpgroup could wait for registers for ever.
+template <auto Kernel>
+bool launched_with(int regs) {
+  static const int have = [] {
+    cudaFuncAttributes f{};
+    return cudaFuncGetAttributes(&f, Kernel) == cudaSuccess ? f.numRegs : -1;
+  }();
+  return have == regs;
+}
+
 template <typename T, int D, int NG, int NT>
 int launch_wide(const Attn4& a, int workers, cudaStream_t stream) {
-  using Sh = Shape4<D, NT>;
+  using Sh = Shape4<D, NG, NT, std::is_same<T, __half>::value ? 2 : 1>;
   constexpr auto kernel = kv4_sm100_kernel<T, D, NG, NT>;
-  if (!allow_smem<kernel>(Sh::kSmem)) return CS_ERR_CUDA;
+  if (!allow_smem<kernel>(Sh::kSmem) || !launched_with<kernel>(Sh::kLaunchRegs))
+    return CS_ERR_CUDA;
   if (const int rc = launch_dependent(kernel, dim3(workers), Sh::kThreads, Sh::kSmem, stream, a))
     return rc;
   return launch_join<T, D, kTileRows * NT>(a, workers, stream);
