@@ -157,10 +157,10 @@ struct Share4 {
   Request4 r;
 
   static __device__ __forceinline__ int tiles(const Request4& r, int G) {
-    return (int)(((int64_t)r.n * G + RT - 1) / RT);
+    return (r.n * G + RT - 1) / RT;  // (no row count passes 31 bits)
   }
   static __device__ __forceinline__ int last_token(const Request4& r, int G, int tile) {
-    const int i = (int)(((int64_t)tile * RT + RT - 1) / G);
+    const int i = (tile * RT + RT - 1) / G;
     return i < r.n ? i : r.n - 1;
   }
   static __device__ __forceinline__ int steps(const Request4& r, int G, int tile) {
@@ -175,65 +175,69 @@ struct Share4 {
   }
 
   // Every worker (block) sums up all requests for itself and takes an equal
-  // range of all steps, `least` of them at least.  `before`: THREADS + 1 +
-  // THREADS / 32 places of shared memory; the first THREADS threads sum, all
-  // threads of the block call.
+  // range of all steps, `least` of them at least; the thread whose requests hold
+  // the range's first step says where that is.  `Scratch` is shared memory; the
+  // first THREADS threads sum, all threads of the block call.
+  template <int THREADS>
+  struct Scratch {
+    int64_t warps[THREADS / 32];
+    Share4 found;
+  };
   template <int THREADS>
   __device__ __forceinline__ void find(const Attn4& a, int worker, int workers, int least,
-                                       int64_t* before) {
+                                       Scratch<THREADS>& s) {
     constexpr int kWarps = THREADS / 32;
-    int64_t* warps = before + THREADS + 1;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int share = (a.requests + THREADS - 1) / THREADS;
+    const int b0 = min(a.requests, tid * share), b1 = min(a.requests, b0 + share);
+    Request4 mine{0, 0, 0};
     int64_t own = 0, run = 0;
     if (tid < THREADS) {
-      const int b0 = min(a.requests, tid * share), b1 = min(a.requests, b0 + share);
-      for (int b = b0; b < b1; ++b) own += cost(a, request4(a, b));
+      for (int b = b0; b < b1; ++b) {
+        mine = request4(a, b);
+        own += cost(a, mine);
+      }
       run = own;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int64_t x = __shfl_up_sync(~0u, run, o);
         if (lane >= o) run += x;
       }
-      if (lane == 31) warps[warp] = run;
+      if (lane == 31) s.warps[warp] = run;
     }
     __syncthreads();
-    if (tid < THREADS) {
+    int64_t all = 0;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w)
-        if (w < warp) run += warps[w];
-      before[tid] = run - own;
-      if (tid == THREADS - 1) before[THREADS] = run;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w == warp) run += all;
+      all += s.warps[w];
     }
-    __syncthreads();
-    const int64_t all = before[THREADS];
     per = max((all + workers - 1) / workers, (int64_t)least);
     const int64_t from = worker * per;
     todo = max((int64_t)0, min(per, all - from));
-    request = tile = head = step = 0;
-    r = Request4{0, 0, 0};
-    if (todo == 0) return;
-    int lo = 0, hi = THREADS - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (before[mid] <= from) lo = mid;
-      else hi = mid - 1;
+    taken = 0;
+    if (todo > 0 && tid < THREADS && from >= run - own && from < run) {
+      int64_t at = run - own;
+      Share4 f;
+      for (f.request = b0;; ++f.request) {  // one of this thread's requests has it
+        f.r = share == 1 ? mine : request4(a, f.request);
+        const int64_t c = cost(a, f.r);
+        if (from < at + c) break;
+        at += c;
+      }
+      for (f.tile = 0;; ++f.tile) {
+        const int64_t c = (int64_t)steps(f.r, a.G, f.tile) * a.pool.hkv;
+        if (from < at + c) break;
+        at += c;
+      }
+      const int n = steps(f.r, a.G, f.tile), rest = (int)(from - at);
+      f.head = rest / n;
+      f.step = rest - f.head * n;
+      s.found = f;
     }
-    int64_t at = before[lo];
-    for (request = lo * share;; ++request) {  // from < all: one of the share's requests has it
-      r = request4(a, request);
-      const int64_t c = cost(a, r);
-      if (from < at + c) break;
-      at += c;
-    }
-    for (;; ++tile) {
-      const int64_t c = (int64_t)steps(r, a.G, tile) * a.pool.hkv;
-      if (from < at + c) break;
-      at += c;
-    }
-    const int s = steps(r, a.G, tile);
-    head = (int)((from - at) / s);
-    step = (int)((from - at) % s);
+    __syncthreads();
+    request = s.found.request, tile = s.found.tile, head = s.found.head, step = s.found.step;
+    r = s.found.r;
   }
 
   // to the first step of the next (head, tile, request) that has rows

@@ -5,6 +5,8 @@
 #include "kv4.cuh"
 #include "sm100.cuh"
 
+#include <type_traits>
+
 namespace cs {
 
 // the kernel for few query rows a KV head (kv4_decode.cu) and the one for many
@@ -42,7 +44,8 @@ int launch_dependent(K kernel, dim3 blocks, int threads, int smem, cudaStream_t 
   return CS_OK;
 }
 
-constexpr int kJoinRows = 16;
+// rows of a joining block: one a warp, four where a tile has many
+template <int RT> constexpr int kJoinRows = RT > 16 ? 16 : 4;
 constexpr float kLn2 = 0.6931471805599453f;
 
 // four neighbouring elements from `c` on of row `row` of a (request, KV head)
@@ -85,11 +88,12 @@ __device__ __forceinline__ void zero_rest(const Attn4& a) {
 }
 
 // o = sum_c w_c o_c / sum_c w_c with w_c = 2^(lse_c - max) over the blocks that
-// shared a row tile, in their order; a block 16 rows of a tile that was cut, a
-// warp a row.
+// shared a row tile, in their order; a block kJoinRows rows of a tile that was
+// cut, a warp a row, 32 weights at once and eight partial rows in flight.
 template <typename T, int D, int RT>
 __global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ Attn4 a) {
   constexpr int E = D / 32;
+  using V = typename std::conditional<E == 4, float4, float2>::type;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 j = a.joins[blockIdx.x];
@@ -97,24 +101,40 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ A
   const int lane = threadIdx.x & 31, first = blockIdx.x, parts = j.w - first + 1;
   const Request4 r = request4(a, j.x);
   const int row0 = j.y * RT, h = j.z >> 1;
-  const int rows = min(min(RT, r.n * a.G - row0), (int)blockIdx.y * kJoinRows + kJoinRows);
+  const int rows = min(min(RT, r.n * a.G - row0), (int)(blockIdx.y + 1) * kJoinRows<RT>);
   auto place = [&](int i) { return i == 0 ? 2ll * first + (j.z & 1) : 2ll * (first + i); };
-  for (int row = blockIdx.y * kJoinRows + (threadIdx.x >> 5); row < rows; row += 4) {
+  for (int row = blockIdx.y * kJoinRows<RT> + (threadIdx.x >> 5); row < rows; row += 4) {
     float top = -INFINITY, sum = 0.f, o[E];
     for (int i = lane; i < parts; i += 32)
       top = fmaxf(top, a.part_lse[place(i) * RT + row]);
     top = warp_max(top);
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < parts; ++i) {
-      const float l = a.part_lse[place(i) * RT + row];
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+      const float l = i0 + lane < parts ? a.part_lse[place(i0 + lane) * RT + row] : -INFINITY;
       // one below 2^-126 of the largest is that, not 0: what is not finite stays
-      const float w = l == -INFINITY ? 0.f : (l != l ? l : fmaxf(ex2(l - top), 0x1p-126f));
-      const float* p = a.part_o + (place(i) * RT + row) * D + lane * E;
-      sum += w;
+      const float f = l == -INFINITY ? 0.f : max_nan(ex2(l - top), 0x1p-126f);
+      sum += warp_sum(f);
+      const int m = min(32, parts - i0);
+#pragma unroll 1
+      for (int c = 0; c < m; c += 8) {
+        V x[8];
+        float w[8];
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = w == 0.f ? o[e] : fmaf(w, p[e], o[e]);
+        for (int k = 0; k < 8; ++k) {
+          w[k] = __shfl_sync(~0u, f, (c + k) & 31);
+          if (c + k >= m) w[k] = 0.f;
+          if (w[k] != 0.f)
+            x[k] = reinterpret_cast<const V*>(a.part_o + (place(i0 + c + k) * RT + row) * D)[lane];
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (w[k] == 0.f) continue;
+          const float* v = reinterpret_cast<const float*>(&x[k]);
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[e] = fmaf(w[k], v[e], o[e]);
+        }
+      }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const int tok = (row0 + row) / a.G, head = h * a.G + (row0 + row - tok * a.G);
@@ -129,7 +149,7 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ A
 template <typename T, int D, int RT>
 int launch_join(const Attn4& a, int workers, cudaStream_t stream) {
   return launch_dependent(kv4_join_kernel<T, D, RT>,
-                          dim3(workers, (RT + kJoinRows - 1) / kJoinRows), 128, 0, stream, a);
+                          dim3(workers, RT / kJoinRows<RT>), 128, 0, stream, a);
 }
 
 }  // namespace cs

@@ -32,7 +32,7 @@ namespace cs {
 namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
-constexpr int kLeast = 4;              // steps a block takes at least
+constexpr int kLeast = 1;              // steps a block takes at least
 constexpr float kUp = 6.f;  // a new largest p scale is 2^6: fp16's normal numbers reach 2^-20 of it
 constexpr float kTooLarge = 0x1p14f;  // it may grow to 2^14 before O is rescaled
 constexpr float kLowest = -3e38f;     // below every score, and finite
@@ -48,7 +48,7 @@ struct Ring {
   static constexpr int kBlocks = NT == 1 ? 4 : 3;  // an SM's
   static constexpr int oBars = kWarps * kStages * E * Unit4<D, NG>::kBytes;
   static constexpr int oSums = oBars + kWarps * kStages * 8;
-  static constexpr int oMax = oSums + (kThreads + 1 + kWarps) * 8 + 8;
+  static constexpr int oMax = oSums + 96;
   static constexpr int oOut = (oMax + 2 * kWarps * RT * 4 + 15) / 16 * 16;
   static constexpr int kBytes = oOut + kWarps * RT * D * 4;
 };
@@ -140,8 +140,10 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   Share work;
+  using Scratch = typename Share::template Scratch<kThreads>;
+  static_assert(sizeof(Scratch) <= R::oMax - R::oSums, "its place");
   work.template find<kThreads>(a, blockIdx.x, gridDim.x, kLeast,
-                               reinterpret_cast<int64_t*>(smem + R::oSums));
+                               *reinterpret_cast<Scratch*>(smem + R::oSums));
   zero_rest<T, D>(a);
   int issued = 0, taken = 0;  // units of this warp's ring
   bool late = false, bad_block = false;

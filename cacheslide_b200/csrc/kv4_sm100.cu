@@ -75,7 +75,7 @@ struct Shape4 {
                             oMax = oRow + NT * kTileRows * 4,
                             oSeg = oMax + (TPR - 1) * NT * 2 * 2 * 128 * 4,
                             oSums = (oSeg + 48 + 7) / 8 * 8,
-                            kMeta = oSums + (128 + 1 + 4) * 8;
+                            kMeta = oSums + 96;
   static_assert(oR % 1024 == 0 && RB % 128 == 0 && oTmem % 4 == 0 && oRow % 4 == 0, "alignment");
   static constexpr uint32_t kSmem = oMeta + kMeta + 1024;  // the base is rounded up to 1024
   static_assert(kSmem <= (NT == 1 ? 115712 : 232448), "shared memory");
@@ -192,8 +192,10 @@ __global__ void __launch_bounds__(
   if (tid == 0) *abort = 0;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   Share work;
+  using Scratch = typename Share::template Scratch<128>;
+  static_assert(sizeof(Scratch) <= Sh::kMeta - Sh::oSums, "its place");
   work.template find<128>(a, blockIdx.x, gridDim.x, kLeastSteps,
-                          reinterpret_cast<int64_t*>(meta + Sh::oSums));
+                          *reinterpret_cast<Scratch*>(meta + Sh::oSums));
   zero_rest<T, D>(a);
   tc_fence_before();
   __syncthreads();
