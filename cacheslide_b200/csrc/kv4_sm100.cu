@@ -39,7 +39,8 @@ constexpr int kTileRows = 128;
 constexpr int kLeastSteps = 4;    // steps a block takes at least
 constexpr float kLazy = 8.f;      // O is rescaled when the maximum grew by more than 2^8
 constexpr float kUp = 7.f;        // P is stored up by 2^7: fp16's normal numbers reach 2^-21
-constexpr int kInfo = 4;          // steps whose scales are kept
+constexpr int kInfo = 8;          // steps whose scales are kept
+constexpr int kSegments = 4;      // segments the loader may be ahead
 
 // TERMS 2: key tiles in two parts (float16 pools)
 template <int D, int NG, int NT, int TERMS>
@@ -64,17 +65,18 @@ struct Shape4 {
   static constexpr uint32_t QB = kTileRows * D * 2 + kTileRows * 16;
   static constexpr uint32_t oQ = 0, oK = NT * QB, oV = oK + KS * TERMS * TB, oR = oV + VS * TB,
                             oMeta = oR + RS * RB;
-  // barriers: queries; a stage's K and V; a score buffer's S, P and PV of a row
-  // tile; a row's maxima; raw units there, and read
-  static constexpr uint32_t bQ = 0, bK = 8, bV = bK + 16, bS = bV + 16, bP = bS + 16 * NT,
-                            bPV = bP + 16 * NT, bMax = bPV + 16 * NT, bR = bMax + 32 * NT,
-                            bRead = bR + 8 * RS, oTmem = bRead + 8 * RS,
+  // barriers: a row tile's queries, and their place free; a stage's K and V; a score buffer's S, P and
+  // PV of a row tile; a row's maxima; raw units there, and read; a segment said,
+  // and read
+  static constexpr uint32_t bQ = 0, bFree = bQ + 8 * NT, bK = bFree + 8 * NT, bV = bK + 16, bS = bV + 16,
+                            bP = bS + 16 * NT, bPV = bP + 16 * NT, bMax = bPV + 16 * NT,
+                            bR = bMax + 32 * NT, bRead = bR + 8 * RS, bSeg = bRead + 8 * RS,
+                            bSegRead = bSeg + 8 * kSegments, oTmem = bSegRead + 8 * kSegments,
                             oAbort = oTmem + 4, oFlag = oAbort + 4, oScale = oFlag + 4 * kInfo,
-                            oPower = oScale + 4 * kInfo, oReach = oPower + 4 * kInfo,
-                            oBad = oReach + 32, oRow = oBad + kInfo * kKeys,
+                            oPower = oScale + 8 * kInfo, oBad = oPower + 8 * kInfo, oRow = oBad + kInfo * kKeys,
                             oMax = oRow + NT * kTileRows * 4,
                             oSeg = oMax + (TPR - 1) * NT * 2 * 2 * 128 * 4,
-                            oSums = (oSeg + 48 + 7) / 8 * 8,
+                            oSums = (oSeg + 48 * kSegments + 7) / 8 * 8,
                             kMeta = oSums + 96;
   static_assert(oR % 1024 == 0 && RB % 128 == 0 && oTmem % 4 == 0 && oRow % 4 == 0, "alignment");
   static constexpr uint32_t kSmem = oMeta + kMeta + 1024;  // the base is rounded up to 1024
@@ -85,9 +87,9 @@ struct Shape4 {
 };
 
 struct Segment {  // of a row tile's steps, for a block
-  int request, start;       // its first token's row
+  int start;                // its first token's row
   int g, row0, rows, tiles; // KV head, first row, rows and row tiles
-  int s0, steps;            // -1: no more
+  int s0, steps;            // steps -1: no more segments
   int seen, first_limit;    // keys its last token sees; the newest key of token 0
   int part;                 // place of its partial results; -1: writes the output
 };
@@ -111,10 +113,6 @@ __device__ __forceinline__ void arrive_expect(uint32_t bar, uint32_t bytes) {
                : "memory");
 }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
-__device__ __forceinline__ void pair_sync(bool v) {  // the two warps of a producer
-  if (v) asm volatile("bar.sync 2, 64;" ::: "memory");
-  else asm volatile("bar.sync 1, 64;" ::: "memory");
-}
 __device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
 __device__ __forceinline__ uint32_t as_u32(__half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
 
@@ -182,14 +180,41 @@ __global__ void __launch_bounds__(
   char* meta = smem + Sh::oMeta;
   volatile int* abort = reinterpret_cast<volatile int*>(meta + Sh::oAbort);
   volatile int* flag = reinterpret_cast<volatile int*>(meta + Sh::oFlag);  // step + 1: bad values
-  volatile float* key_scale = reinterpret_cast<volatile float*>(meta + Sh::oScale);  // 2^E of keys
-  volatile float* val_power = reinterpret_cast<volatile float*>(meta + Sh::oPower);  // E of values
+  // 2^E of 32 keys, and E of 32 values: [step % kInfo][half]
+  volatile float* key_scale = reinterpret_cast<volatile float*>(meta + Sh::oScale);
+  volatile float* val_power = reinterpret_cast<volatile float*>(meta + Sh::oPower);
   uint8_t* bad = reinterpret_cast<uint8_t*>(meta + Sh::oBad);  // [step % kInfo][key]: groups
   float* row_scale = reinterpret_cast<float*>(meta + Sh::oRow);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (warp == Sh::kSoft + 5) tmem_alloc(mb + Sh::oTmem, Sh::kCols);
-  if (tid == 0) *abort = 0;
+  if (tid == 0) {
+    for (int k = 0; k < NT; ++k) {
+      mbar_init(mb + Sh::bQ + 8 * k, Sh::kTile);
+      mbar_init(mb + Sh::bFree + 8 * k, Sh::kTile / 32);
+    }
+    for (int k = 0; k < 2; ++k) {
+      mbar_init(mb + Sh::bK + 8 * k, 64);
+      mbar_init(mb + Sh::bV + 8 * k, 64);
+    }
+    for (int k = 0; k < 2 * NT; ++k) {
+      mbar_init(mb + Sh::bS + 8 * k, 1);
+      mbar_init(mb + Sh::bP + 8 * k, Sh::kTile);
+      mbar_init(mb + Sh::bPV + 8 * k, 1);
+    }
+    for (int k = 0; k < 4 * NT; ++k) mbar_init(mb + Sh::bMax + 8 * k, 2);
+    for (int k = 0; k < RS; ++k) {
+      mbar_init(mb + Sh::bR + 8 * k, kKeys / kUnit);
+      mbar_init(mb + Sh::bRead + 8 * k, 4);
+    }
+    for (int k = 0; k < kSegments; ++k) {
+      mbar_init(mb + Sh::bSeg + 8 * k, 1);
+      mbar_init(mb + Sh::bSegRead + 8 * k, Sh::kSoft + 4 + NT);
+    }
+    mbar_init_fence();
+    for (int k = 0; k < kInfo; ++k) flag[k] = -1;
+    *abort = 0;
+  }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   Share work;
   using Scratch = typename Share::template Scratch<128>;
@@ -202,48 +227,62 @@ __global__ void __launch_bounds__(
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(meta + Sh::oTmem);
 
-  // step t uses score buffer t & 1 of its row tile
-  auto at = [&](uint32_t bar, int qt, int t) { return mb + bar + 8 * (2 * qt + (t & 1)); };
-  // Every role walks the block's segments, each between two barriers of the
-  // block; the loader says what is next (in shared memory: the other roles have
-  // no registers for the division of the work).
-  const Segment& seg = *reinterpret_cast<const Segment*>(meta + Sh::oSeg);
-  auto segments = [&](auto next, auto role) {
-    while (true) {
-      next();
-      __syncthreads();
-      if (seg.steps < 0 || *abort) break;
-      role();
-      // nothing of this tile is in flight or in use behind this
-      tc_fence_before();
-      __syncthreads();
-      tc_fence_after();
+  // Steps are counted over the whole block, those of the second row tile (which
+  // not every segment has) apart; step n uses score buffer n & 1 of its row tile.
+  auto at = [&](uint32_t bar, int qt, int n) { return mb + bar + 8 * (2 * qt + (n & 1)); };
+  // The loader says what the block's segments are; every other role walks them
+  // for itself.  What keeps them apart are the barriers of the steps and the
+  // order within a role: the next segment's keys are on their way, and their
+  // first tiles made, while this one's rows are written.
+  const Segment* segs = reinterpret_cast<const Segment*>(meta + Sh::oSeg);
+  auto segments = [&](auto role) {
+    for (int n = 0;; ++n) {
+      const int k = n % kSegments;
+      if (!warp_wait(mb + Sh::bSeg + 8 * k, (n / kSegments) & 1, abort)) break;
+      if (segs[k].steps < 0) break;
+      if (!role(segs[k])) break;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(mb + Sh::bSegRead + 8 * k);
     }
   };
-  auto follow = [] {};
 
   if (warp >= Sh::kSoft && warp < Sh::kSoft + 4) {
     // ============================================= producers: K, then V pair
     if constexpr (Sh::kMakeRegs > Sh::kLaunchRegs) regs_up<Sh::kMakeRegs>();
     else regs_down<Sh::kMakeRegs>();
     const bool isv = warp >= Sh::kSoft + 2;
-    const int i = (tid - 32 * Sh::kSoft) & 63;
-    // this thread's part of 16 keys' rows: token r, W words from word W c on
-    const int r = (i & 7) + 8 * (i >> 5), c = (i >> 3) & 3;
-    segments(follow, [&] {
-      const int steps = seg.steps, seen = seg.seen, first_key = seg.s0 * kKeys + r;
-      for (int t = 0; t < steps; ++t) {
+    // a warp makes 32 keys' rows, with a power of two of their own; this thread's
+    // part of every eight is the W words from word W c on of row r
+    const int half = warp & 1, r = lane & 7, c = lane >> 3;
+    int n = 0, n1 = 0;           // steps, and those of the second row tile
+    int second[2] = {-1, -1};    // its step in the last two, if it had one
+    segments([&](const Segment& seg) {
+      const int steps = seg.steps, seen = seg.seen, first_key = seg.s0 * kKeys + 32 * half + r;
+      const bool two = seg.tiles == 2;
+      for (int t = 0; t < steps; ++t, ++n) {
         uint32_t code[4][W], pair[4][NG];
-        if (!warp_wait(mb + Sh::bR + 8 * (t % RS), (t / RS) & 1, abort)) break;
-        const char* units = smem + Sh::oR + (t % RS) * Sh::RB;
+        if (!warp_wait(mb + Sh::bR + 8 * (n % RS), (n / RS) & 1, abort)) return false;
+        const char* units = smem + Sh::oR + (n % RS) * Sh::RB;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const char* p = units + j * U::kBytes;
-          load_words(code[j], p + (isv ? U::oV : 0) + r * U::kRow + 4 * W * c);
-          load_words(pair[j], p + (isv ? U::oVp : U::oKp) + 4 * NG * r);
+          const char* p = units + (2 * half + j / 2) * U::kBytes;
+          const int token = 8 * (j & 1) + r;
+          load_words(code[j], p + (isv ? U::oV : 0) + token * U::kRow + 4 * W * c);
+          load_words(pair[j], p + (isv ? U::oVp : U::oKp) + 4 * NG * token);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(mb + Sh::bRead + 8 * (t % RS));
+        // The stage may be filled again once these loads have come back, which an
+        // arrival does not wait for by itself: it is made by a lane that a vote
+        // over the loaded words names (any of two will do).
+        uint32_t words = 0u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int w = 0; w < W; ++w) words |= code[j][w];
+#pragma unroll
+          for (int k = 0; k < NG; ++k) words |= pair[j][k];
+        }
+        if (lane == (__any_sync(~0u, words == 0x9e3779b9u) ? 1 : 0))
+          mbar_arrive(mb + Sh::bRead + 8 * (n % RS));
         // ------------------------------- the step's power of two, bad values
         const int key0 = first_key + t * kKeys;
         float2 f[4][NG];
@@ -251,7 +290,7 @@ __global__ void __launch_bounds__(
         uint32_t wrong = 0u;  // bit NG j + k
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (key0 + j * kUnit >= seen) {  // zeros: P is zero there too
+          if (key0 + 8 * j >= seen) {  // zeros: P is zero there too
 #pragma unroll
             for (int k = 0; k < NG; ++k) pair[j][k] = 0u;
           }
@@ -271,51 +310,47 @@ __global__ void __launch_bounds__(
         int e = 0;
         if constexpr (TERMS == 1) {
           const uint32_t m = __reduce_max_sync(~0u, __float_as_uint(reach));
-          volatile uint32_t* both = reinterpret_cast<volatile uint32_t*>(meta + Sh::oReach) +
-                                    (isv ? 4 : 0) + 2 * (t & 1);
-          if (lane == 0) both[warp & 1] = m;
-          pair_sync(isv);
-          const uint32_t all = max(both[0], both[1]);
-          e = all == 0u ? 0 : min(114, max(-80, (int)(all >> 23) - 127 - 13));
+          e = m == 0u ? 0 : min(114, max(-80, (int)(m >> 23) - 127 - 13));
         }
         const float down = pow2(-e);
         // --------------------------------------------------- a free stage
         const int stages = isv ? Sh::VS : KS;
-        if (t >= stages) {
-          const int u = t - stages;
-          bool ok = true;
-          for (int qt = 0; qt < seg.tiles; ++qt)
-            ok = ok && warp_wait(at(isv ? Sh::bPV : Sh::bS, qt, u), (u >> 1) & 1, abort);
-          if (!ok) break;
+        if (n >= stages) {
+          const int u = n - stages, u1 = second[u & 1];
+          const uint32_t bar = isv ? Sh::bPV : Sh::bS;
+          if (!warp_wait(at(bar, 0, u), (u >> 1) & 1, abort) ||
+              (u1 >= 0 && !warp_wait(at(bar, NT - 1, u1), (u1 >> 1) & 1, abort)))
+            return false;
         }
-        if (i == 0) {
-          if (isv) val_power[t % kInfo] = (float)e;
-          else key_scale[t % kInfo] = pow2(e);
+        second[n & 1] = two ? n1++ : -1;
+        if (lane == 0) {
+          if (isv) val_power[2 * (n % kInfo) + half] = (float)e;
+          else key_scale[2 * (n % kInfo) + half] = pow2(e);
         }
         if (isv) {
-          const uint32_t tile = sbase + Sh::oV + (t % Sh::VS) * Sh::TB;
+          const uint32_t tile = sbase + Sh::oV + (n % Sh::VS) * Sh::TB;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
 #pragma unroll
             for (int w = 0; w < W; ++w) {
               const uint32_t x = __byte_perm(code[j][w / 2], code[j][W / 2 + w / 2],
                                              w & 1 ? 0x7632u : 0x5410u);
-              st_shared16(tile + sw128(j * kUnit + r, 4 * w + c, kKeys),
+              st_shared16(tile + sw128(32 * half + 8 * j + r, 4 * w + c, kKeys),
                           decode8(x, __float2half2_rn(f[j][w / WG].x * down),
                                   __float2half2_rn(f[j][w / WG].y * down)));
             }
             if (c == 0)
-              bad[(t % kInfo) * kKeys + j * kUnit + r] =
+              bad[(n % kInfo) * kKeys + 32 * half + 8 * j + r] =
                   (uint8_t)(wrong >> (NG * j) & ((1u << NG) - 1u));
           }
-          if (wrong) flag[t % kInfo] = t + 1;
+          if (wrong) flag[n % kInfo] = n;
         } else {
-          const uint32_t tile = sbase + Sh::oK + (t % KS) * TERMS * Sh::TB;
+          const uint32_t tile = sbase + Sh::oK + (n % KS) * TERMS * Sh::TB;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
 #pragma unroll
             for (int w = 0; w < W; ++w) {
-              const uint32_t to = tile + sw128(j * kUnit + r, 4 * w + c, kKeys);
+              const uint32_t to = tile + sw128(32 * half + 8 * j + r, 4 * w + c, kKeys);
               const float2 y = f[j][w / WG];
               if constexpr (TERMS == 1) {
                 st_shared16(to, decode8(code[j][w], __float2half2_rn(y.x * down),
@@ -335,76 +370,61 @@ __global__ void __launch_bounds__(
           }
         }
         fence_async_smem();
-        mbar_arrive(mb + (isv ? Sh::bV + 8 * (t % Sh::VS) : Sh::bK + 8 * (t % KS)));
+        mbar_arrive(mb + (isv ? Sh::bV + 8 * (n % Sh::VS) : Sh::bK + 8 * (n % KS)));
       }
+      return true;
     });
 
   } else if (warp == Sh::kSoft + 4) {
     // ============================================================ the loader
     regs_down<Sh::kRestRegs>();
-    bool bad_block = false, first = true;
+    bool bad_block = false;
     int which = 0;  // of this block's partial results
     int4 join = make_int4(-1, 0, 0, 0);
-    auto next = [&] {
-      Segment& s = *reinterpret_cast<Segment*>(meta + Sh::oSeg);
-      if (!first && work.todo > 0) {
-        work.todo -= work.taken;
-        if (work.todo > 0) work.next(a);
-      }
+    int n = 0;  // steps
+    for (int k = 0;; ++k) {
+      Segment& s = reinterpret_cast<Segment*>(meta + Sh::oSeg)[k % kSegments];
+      const uint32_t said = mb + Sh::bSeg + 8 * (k % kSegments);
+      if (k >= kSegments && !warp_wait(mb + Sh::bSegRead + 8 * (k % kSegments),
+                                       (k / kSegments - 1) & 1, abort))
+        break;
       if (work.todo <= 0) {
-        if (lane == 0) s.steps = -1;
-        return;
+        if (lane == 0) {
+          s.steps = -1;
+          mbar_arrive(said);
+        }
+        break;
       }
       const int all_steps = Share::steps(work.r, a.G, work.tile);
-      const int s1 = (int)min((int64_t)all_steps, work.step + work.todo);
-      const bool whole = work.step == 0 && s1 == all_steps;
-      work.taken = s1 - work.step;
+      const int s0 = work.step, s1 = (int)min((int64_t)all_steps, s0 + work.todo), g = work.head;
+      const bool whole = s0 == 0 && s1 == all_steps;
+      const int first_limit = work.r.len - work.r.n;
+      const int seen = max(0, first_limit + Share::last_token(work.r, a.G, work.tile) + 1);
+      const int steps = max(0, min(s1, (seen + kKeys - 1) / kKeys) - s0);
       if (lane == 0) {
         s.start = work.r.start;
-        s.request = work.request;
-        s.g = work.head;
-        s.s0 = work.step;
+        s.g = g;
+        s.s0 = s0;
         s.row0 = work.tile * RT;
         s.rows = min(RT, work.r.n * a.G - s.row0);
         s.tiles = s.rows > kTileRows ? 2 : 1;
-        s.first_limit = work.r.len - work.r.n;
-        s.seen = max(0, s.first_limit + Share::last_token(work.r, a.G, work.tile) + 1);
-        s.steps = max(0, min(s1, (s.seen + kKeys - 1) / kKeys) - work.step);
+        s.first_limit = first_limit;
+        s.seen = seen;
+        s.steps = steps;
         s.part = whole ? -1 : 2 * (int)blockIdx.x + which;
-        if (!first)
-          for (uint32_t b = Sh::bQ; b < Sh::oTmem; b += 8) mbar_inval(mb + b);
-        mbar_init(mb + Sh::bQ, Sh::kTile * s.tiles);
-        for (int k = 0; k < 2; ++k) {
-          mbar_init(mb + Sh::bK + 8 * k, 64);
-          mbar_init(mb + Sh::bV + 8 * k, 64);
-        }
-        for (int k = 0; k < 2 * NT; ++k) {
-          mbar_init(mb + Sh::bS + 8 * k, 1);
-          mbar_init(mb + Sh::bP + 8 * k, Sh::kTile);
-          mbar_init(mb + Sh::bPV + 8 * k, 1);
-        }
-        for (int k = 0; k < 4 * NT; ++k) mbar_init(mb + Sh::bMax + 8 * k, 2);
-        for (int k = 0; k < RS; ++k) {
-          mbar_init(mb + Sh::bR + 8 * k, kKeys / kUnit);
-          mbar_init(mb + Sh::bRead + 8 * k, 4);
-        }
-        mbar_init_fence();
-        for (int k = 0; k < kInfo; ++k) flag[k] = 0;
+        mbar_arrive(said);
       }
       if (!whole) {
-        if (work.step == 0)  // the first of the tile's blocks has them joined
-          join = make_int4(work.request, work.tile, 2 * work.head + which,
+        if (s0 == 0)  // the first of the tile's blocks has them joined
+          join = make_int4(work.request, work.tile, 2 * g + which,
                            blockIdx.x + (int)((all_steps - s1 + work.per - 1) / work.per));
         which = 1;
       }
-      first = false;
-    };
-    segments(next, [&] {
-      const int32_t* table = a.tables + seg.request * a.table_stride;
-      const int units = (seg.seen + kUnit - 1) / kUnit, steps = seg.steps, s0 = seg.s0, g = seg.g;
+      const int32_t* table = a.tables + work.request * a.table_stride;
+      const int units = (seen + kUnit - 1) / kUnit;
       int64_t from = -1;  // this lane's unit of eight steps: -1 none, 0 no block
-      int issued = 0;
-      for (int t = 0; t < steps; ++t) {
+      bool ok = true;
+      for (int t = 0; ok && t < steps; ++t, ++n) {
         if (t % 8 == 0) {
           const int u = (s0 + t) * (kKeys / kUnit) + lane, j = u / a.pool.units;
           from = -1;
@@ -416,65 +436,74 @@ __global__ void __launch_bounds__(
             bad_block |= from == 0;
           }
         }
-        if (t >= RS &&
-            !warp_wait(mb + Sh::bRead + 8 * (t % RS), (t / RS - 1) & 1, abort))
-          break;
+        if (n >= RS) {
+          ok = warp_wait(mb + Sh::bRead + 8 * (n % RS), (n / RS - 1) & 1, abort);
+          if (!ok) break;
+        }
         if (lane / 4 == t % 8) {
-          const uint32_t bar = mb + Sh::bR + 8 * (t % RS);
-          const uint32_t to = Sh::oR + (t % RS) * Sh::RB + (lane % 4) * U::kBytes;
+          const uint32_t bar = mb + Sh::bR + 8 * (n % RS);
+          const uint32_t to = Sh::oR + (n % RS) * Sh::RB + (lane % 4) * U::kBytes;
           if (from > 0) {
             arrive_expect(bar, U::kBytes);
             bulk_copy(sbase + to, reinterpret_cast<const void*>(from), U::kBytes, bar);
           } else {
             if (from == 0) {  // zero codes, scales and lows: zero keys and values
-              for (int k = 0; k < U::kBytes / 16; ++k)
-                st_shared16(sbase + to + 16 * k, make_uint4(0, 0, 0, 0));
+              for (int m = 0; m < U::kBytes / 16; ++m)
+                st_shared16(sbase + to + 16 * m, make_uint4(0, 0, 0, 0));
               fence_async_smem();  // before a later copy into this place
             }
             mbar_arrive(bar);
           }
         }
         __syncwarp();
-        issued = t + 1;
       }
-      // nothing of this block's copies is in flight when it goes on
-      for (int t = issued - RS < 0 ? 0 : issued - RS; t < issued; ++t) {
-        const long long t0 = clock64();
-        while (!mbar_try(mb + Sh::bR + 8 * (t % RS), (t / RS) & 1) &&
-               clock64() - t0 < kWaitCycles) {
-        }
+      if (!ok) break;
+      work.todo -= s1 - s0;
+      if (work.todo > 0) work.next(a);
+    }
+    // nothing of this block's copies is in flight when it ends
+    for (int u = n - RS < 0 ? 0 : n - RS; u < n; ++u) {
+      const long long t0 = clock64();
+      while (!mbar_try(mb + Sh::bR + 8 * (u % RS), (u / RS) & 1) && clock64() - t0 < kWaitCycles) {
       }
-      __syncwarp();
-    });
+    }
     if (lane == 0) a.joins[blockIdx.x] = join;
     if (bad_block) report(a.status, CS_ST_SLOT_RANGE);
 
   } else if (warp > Sh::kSoft + 4) {
     // ==================================================== MMA, one warp a tile
     regs_down<Sh::kRestRegs>();
-    segments(follow, [&] {
-      const int qt = __shfl_sync(~0u, warp, 0) - (Sh::kSoft + 5), steps = seg.steps;
+    const int qt = __shfl_sync(~0u, warp, 0) - (Sh::kSoft + 5);
+    const bool leader = elect_one();
+    const uint32_t id_s = umma_idesc(128, kKeys, 0, 0, 0);
+    const uint32_t id_o = umma_idesc(128, D, 0, 0, 1);  // V is MN-major
+    const uint64_t dq = umma_desc(sbase + Sh::oQ + qt * Sh::QB, 16, 1024);
+    const uint64_t dk0 = umma_desc(sbase + Sh::oK, 16, 1024);
+    const uint64_t dv0 = umma_desc(sbase + Sh::oV, kKeys * 128, 1024);
+    const uint32_t tm = __shfl_sync(~0u, tmem, 0);
+    const uint32_t sc = tm + Sh::cS + 128 * qt, oc = tm + Sh::cO + D * qt;
+    int n = 0, m = 0, queries = 0;  // steps of the block and of the row tile; its segments
+    uint32_t last = 0, lastph = 0;  // the newest group issued
+    auto drained = [&] {
+      const long long t0 = clock64();
+      while (last && !mbar_try(last, lastph) && clock64() - t0 < kWaitCycles) {
+      }
+      last = 0;
+    };
+    if (qt < NT) segments([&](const Segment& seg) {
+      const int steps = seg.steps;
       if (qt < seg.tiles) {
-        const bool leader = elect_one();
-        const uint32_t id_s = umma_idesc(128, kKeys, 0, 0, 0);
-        const uint32_t id_o = umma_idesc(128, D, 0, 0, 1);  // V is MN-major
-        const uint64_t dq = umma_desc(sbase + Sh::oQ + qt * Sh::QB, 16, 1024);
-        const uint64_t dk0 = umma_desc(sbase + Sh::oK, 16, 1024);
-        const uint64_t dv0 = umma_desc(sbase + Sh::oV, kKeys * 128, 1024);
-        const uint32_t tm = __shfl_sync(~0u, tmem, 0);
-        const uint32_t sc = tm + Sh::cS + 128 * qt, oc = tm + Sh::cO + D * qt;
-        bool ok = warp_wait(mb + Sh::bQ, 0, abort);
-        uint32_t last = 0, lastph = 0;  // the newest group issued
-        auto arrived = [&](uint32_t bar, int t, int stages) {
-          ok = ok && warp_wait(mb + bar + 8 * (t % stages), (t / stages) & 1, abort);
-          return ok;
+        if (!warp_wait(mb + Sh::bQ + 8 * qt, queries++ & 1, abort)) return false;
+        auto arrived = [&](uint32_t bar, int u, int stages) {
+          return warp_wait(mb + bar + 8 * (u % stages), (u / stages) & 1, abort);
         };
         auto scores = [&](int t) {
+          if (!arrived(Sh::bK, n + t, KS)) return false;
           tc_fence_after();
-          const uint64_t dk = dk0 + (uint64_t)((t % KS) * TERMS * (Sh::TB >> 4));
-          const uint32_t sb = sc + kKeys * (t & 1);
-          last = at(Sh::bS, qt, t);
-          lastph = (t >> 1) & 1;
+          const uint64_t dk = dk0 + (uint64_t)(((n + t) % KS) * TERMS * (Sh::TB >> 4));
+          const uint32_t sb = sc + kKeys * ((m + t) & 1);
+          last = at(Sh::bS, qt, m + t);
+          lastph = ((m + t) >> 1) & 1;
           if (leader) {
 #pragma unroll
             for (int term = 0; term < TERMS; ++term) {
@@ -487,17 +516,18 @@ __global__ void __launch_bounds__(
             tc_commit(last);
           }
           __syncwarp();
+          return true;
         };
-        if (steps > 0 && arrived(Sh::bK, 0, KS)) scores(0);
-        if (steps > 1 && arrived(Sh::bK, 1, KS)) scores(1);
-        for (int t = 0; ok && t < steps; ++t) {
-          const uint32_t ph = (t >> 1) & 1;
-          if (!arrived(Sh::bV, t, Sh::VS)) break;
-          if (!(ok = warp_wait(at(Sh::bP, qt, t), ph, abort))) break;
+        for (int t = 0; t < 2 && t < steps; ++t)
+          if (!scores(t)) return false;
+        for (int t = 0; t < steps; ++t) {
+          const uint32_t ph = ((m + t) >> 1) & 1;
+          if (!arrived(Sh::bV, n + t, Sh::VS) || !warp_wait(at(Sh::bP, qt, m + t), ph, abort))
+            return false;
           tc_fence_after();
-          const uint64_t dv = dv0 + (uint64_t)((t % Sh::VS) * (Sh::TB >> 4));
-          const uint32_t p = sc + kKeys * (t & 1);
-          last = at(Sh::bPV, qt, t);
+          const uint64_t dv = dv0 + (uint64_t)(((n + t) % Sh::VS) * (Sh::TB >> 4));
+          const uint32_t p = sc + kKeys * ((m + t) & 1);
+          last = at(Sh::bPV, qt, m + t);
           lastph = ph;
           if (leader) {
 #pragma unroll
@@ -507,29 +537,35 @@ __global__ void __launch_bounds__(
           }
           __syncwarp();
           // the next scores but one take the buffer that P lies in
-          if (t + 2 < steps) {
-            if (!arrived(Sh::bK, t + 2, KS)) break;
-            if (!(ok = warp_wait(at(Sh::bPV, qt, t), ph, abort))) break;
-            scores(t + 2);
-          }
+          if (t + 2 < steps &&
+              (!warp_wait(at(Sh::bPV, qt, m + t), ph, abort) || !scores(t + 2)))
+            return false;
         }
-        if (last) {
-          const long long t0 = clock64();
-          while (!mbar_try(last, lastph) && clock64() - t0 < kWaitCycles) {
-          }
-        }
+        drained();  // (the next segment's scores take both buffers)
+        m += steps;
       }
-      __syncwarp();
+      n += steps;
+      return true;
     });
+    drained();
+    __syncwarp();
 
   } else {
     // ================================================================= softmax
     regs_up<Sh::kSoftRegs>();
-    segments(follow, [&] {
-      if (warp / (4 * Sh::TPR) >= seg.tiles) return;
+    int n = 0, m = 0, queries = 0;  // steps of the block and of the row tile; its segments
+    [[maybe_unused]] int exchanges = 0;  // of maxima with the row's other thread
+    segments([&](const Segment& seg) {
       const int row0 = seg.row0, steps = seg.steps, s0 = seg.s0;
       constexpr int TPR = Sh::TPR, VC = kKeys / TPR;  // scores of a step a thread holds
       const int qt = warp / (4 * TPR), part2 = (warp >> 2) % TPR;
+      if (qt >= seg.tiles) {
+        n += steps;
+        return true;
+      }
+      // all rows of the last segment are written: their places may take queries
+      if (queries > 0 && !warp_wait(mb + Sh::bFree + 8 * qt, (queries - 1) & 1, abort))
+        return false;
       const int r = (warp & 3) * 32 + lane;  // TMEM lane
       const int row = qt * kTileRows + r;    // of the block's
       const bool row_ok = row < seg.rows;
@@ -538,41 +574,50 @@ __global__ void __launch_bounds__(
         constexpr int C = D / 8;
         const int c = tid % C;
         const uint32_t qs = sbase + Sh::oQ + qt * Sh::QB;
-        for (int m = (tid % Sh::kTile) / C; m < kTileRows; m += Sh::kTile / C) {
-          const int rr = row0 + qt * kTileRows + m;
-          const bool ok = qt * kTileRows + m < seg.rows;
-          const int tk = ok ? rr / a.G : 0;
+        constexpr int kRows = kTileRows * C / Sh::kTile;  // a thread's, all fetched at once
+        uint32_t x[kRows][4];
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) {
+          const int q = qt * kTileRows + (tid % Sh::kTile) / C + k * (Sh::kTile / C);
+          const bool ok = q < seg.rows;
+          const int tk = ok ? (row0 + q) / a.G : 0;
           const char* p = a.q + (int64_t)(seg.start + tk) * a.qt +
-                          (int64_t)(seg.g * a.G + (ok ? rr - tk * a.G : 0)) * a.qh + 16 * c;
-          uint32_t x[4] = {0u, 0u, 0u, 0u};
+                          (int64_t)(seg.g * a.G + (ok ? row0 + q - tk * a.G : 0)) * a.qh + 16 * c;
           if (ok && a.vec_q) {
-            load_words(x, p);
+            load_words(x[k], p);
           } else if (ok) {
             const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[k] = u[2 * k] | (uint32_t)u[2 * k + 1] << 16;
+            for (int w = 0; w < 4; ++w) x[k][w] = u[2 * w] | (uint32_t)u[2 * w + 1] << 16;
+          } else {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) x[k][w] = 0u;
           }
+        }
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) {
+          const int q = (tid % Sh::kTile) / C + k * (Sh::kTile / C);
           float f[8], top = 0.f;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float2 y = pair_of<T>(x[k] ^ a.flip);
-            f[2 * k] = y.x, f[2 * k + 1] = y.y;
+          for (int w = 0; w < 4; ++w) {
+            const float2 y = pair_of<T>(x[k][w] ^ a.flip);
+            f[2 * w] = y.x, f[2 * w + 1] = y.y;
             top = fmaxf(top, fmaxf(fabsf(y.x), fabsf(y.y)));
           }
 #pragma unroll
           for (int o = 1; o < C; o <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
           const int e = min(100, max(-100, (int)(__float_as_uint(top) >> 23) - 127 - 13));
           const float up = pow2(-e);
-          if (c == 0) row_scale[qt * kTileRows + m] = pow2(e);
+          if (c == 0) row_scale[qt * kTileRows + q] = pow2(e);
           uint32_t y[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) y[k] = Pack2<__half>::pack(f[k] * up, f[k + 4] * up);
-          st_shared16(qs + sw128(m, c, kTileRows), make_uint4(y[0], y[1], y[2], y[3]));
+          for (int w = 0; w < 4; ++w) y[w] = Pack2<__half>::pack(f[w] * up, f[w + 4] * up);
+          st_shared16(qs + sw128(q, c, kTileRows), make_uint4(y[0], y[1], y[2], y[3]));
         }
         fence_async_smem();
-        mbar_arrive(mb + Sh::bQ);
+        mbar_arrive(mb + Sh::bQ + 8 * qt);
       }
-      bool ok = warp_wait(mb + Sh::bQ, 0, abort);
+      bool ok = warp_wait(mb + Sh::bQ + 8 * qt, queries++ & 1, abort);
       const float row_factor = row_scale[qt * kTileRows + r] * a.scale2;
       // the newest key this row sees; no row: of no matter
       const int limit = row_ok ? seg.first_limit + (row0 + row) / a.G : INT32_MAX;
@@ -581,12 +626,11 @@ __global__ void __launch_bounds__(
       const uint32_t oc = tmem + lane_base + Sh::cO + D * qt;
       float mref = -INFINITY, lsum = 0.f;  // log2 domain; P = 2^(x + E - mref + up)
       uint32_t poison = 0u;  // groups of values that are not finite and that the row sees
-      [[maybe_unused]] int exchanges = 0;  // of maxima with the row's other thread
       [[maybe_unused]] const uint32_t pair = mb + Sh::bMax + 8 * (4 * qt + (warp & 3));
       [[maybe_unused]] float* row_max = reinterpret_cast<float*>(meta + Sh::oMax) + qt * 512;
       const bool any_row = __any_sync(~0u, row_ok);
       auto wait_pv = [&](int t) {
-        ok = warp_wait(at(Sh::bPV, qt, t), (t >> 1) & 1, abort);
+        ok = warp_wait(at(Sh::bPV, qt, m + t), ((m + t) >> 1) & 1, abort);
         tc_fence_after();
         return ok;
       };
@@ -594,11 +638,12 @@ __global__ void __launch_bounds__(
       for (int t = 0; ok && t < steps; ++t) {
         const int base = (s0 + t) * kKeys;
         const int vhi = limit - base >= kKeys ? kKeys : limit - base + 1;  // keys seen
-        const uint32_t sc = sc0 + kKeys * (t & 1);
+        const uint32_t sc = sc0 + kKeys * ((m + t) & 1);
+        const int info = (n + t) % kInfo;
         // the values' power and bad groups come with the values (whose barrier
         // cannot move on before this step's P is there)
-        ok = warp_wait(at(Sh::bS, qt, t), (t >> 1) & 1, abort) &&
-             warp_wait(mb + Sh::bV + 8 * (t & 1), (t >> 1) & 1, abort);
+        ok = warp_wait(at(Sh::bS, qt, m + t), ((m + t) >> 1) & 1, abort) &&
+             warp_wait(mb + Sh::bV + 8 * ((n + t) % Sh::VS), ((n + t) / Sh::VS) & 1, abort);
         if (!ok) break;  // a wait expired
         tc_fence_after();
         uint32_t v[VC];
@@ -610,13 +655,18 @@ __global__ void __launch_bounds__(
           for (int cc = 0; cc < VC / 32; ++cc) CS_TMEM_ST16(sc + 16 * (part2 + cc), v);
           tmem_wait_st();
           tc_fence_before();
-          mbar_arrive(at(Sh::bP, qt, t));
+          mbar_arrive(at(Sh::bP, qt, m + t));
           continue;
         }
         CS_TMEM_LD32(sc + 32 * part2, v);
         if constexpr (TPR == 1) CS_TMEM_LD32(sc + 32, (v + 32));
-        const float power = val_power[t % kInfo];
-        const float factor = fmaxf(row_factor * key_scale[t % kInfo], 1e-30f);
+        // of this thread's 32 keys (one of two such sets, where it holds the row)
+        float power[VC / 32], factor[VC / 32];
+#pragma unroll
+        for (int cc = 0; cc < VC / 32; ++cc) {
+          power[cc] = val_power[2 * info + part2 + cc];
+          factor[cc] = fmaxf(row_factor * key_scale[2 * info + part2 + cc], 1e-30f);
+        }
         tmem_wait_ld();
         if (!__all_sync(~0u, vhi >= kKeys)) {
 #pragma unroll
@@ -627,25 +677,28 @@ __global__ void __launch_bounds__(
               v[32 * cc + c] = (bits >> c) & 1u ? v[32 * cc + c] : 0xff800000u;  // -inf
           }
         }
-        if (flag[t % kInfo] == t + 1) {
+        if (flag[info] == n + t) {
           for (int c = 0; c < VC; ++c) {
             const int key = 32 * part2 + c;
-            if (key < vhi) poison |= bad[(t % kInfo) * kKeys + key];
+            if (key < vhi) poison |= bad[info * kKeys + key];
           }
         }
-        float top;
-        {
-          float m[4];
+        float top = -INFINITY;  // of log2 of the weights, with the values' power
+#pragma unroll
+        for (int cc = 0; cc < VC / 32; ++cc) {
+          float m4[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            m[k] = max_nan(__uint_as_float(v[k]), __uint_as_float(v[k + 4]));
+            m4[k] = max_nan(__uint_as_float(v[32 * cc + k]), __uint_as_float(v[32 * cc + k + 4]));
 #pragma unroll
-          for (int c = 8; c < VC; c += 8) {
+          for (int c = 8; c < 32; c += 8) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              m[k] = max3_nan(m[k], __uint_as_float(v[c + k]), __uint_as_float(v[c + k + 4]));
+              m4[k] = max3_nan(m4[k], __uint_as_float(v[32 * cc + c + k]),
+                               __uint_as_float(v[32 * cc + c + k + 4]));
           }
-          top = max_nan(max3_nan(m[0], m[1], m[2]), m[3]);
+          top = max_nan(top, fmaf(max_nan(max3_nan(m4[0], m4[1], m4[2]), m4[3]), factor[cc],
+                                  power[cc]));
         }
         // the row's maximum from both its threads; past this barrier both have
         // read their scores, so P may take their columns
@@ -663,12 +716,11 @@ __global__ void __launch_bounds__(
           lsum = __int_as_float(0x7fffffff);
           top = -INFINITY;
         }
-        const float top2 = top == -INFINITY ? -INFINITY : fmaf(top, factor, power);
-        const bool grow = top2 > mref + kLazy || mref == -INFINITY;
-        const bool rescale = grow && mref > -INFINITY && top2 > mref;
+        const bool grow = top > mref + kLazy || mref == -INFINITY;
+        const bool rescale = grow && mref > -INFINITY && top > mref;
         if (__any_sync(~0u, rescale)) {  // t > 0: a row has a finite maximum
           if (!wait_pv(t - 1)) break;
-          const float f = rescale ? ex2(mref - top2) : 1.f;
+          const float f = rescale ? ex2(mref - top) : 1.f;
           lsum *= f;
           uint32_t o[16];
 #pragma unroll 1
@@ -682,12 +734,12 @@ __global__ void __launch_bounds__(
           }
           tmem_wait_st();
         }
-        if (grow) mref = top2;
-        const float sub = (mref > -INFINITY ? mref : 0.f) - kUp - power;
-        const float2 scale = make_float2(factor, factor), off = make_float2(-sub, -sub);
-        float2 p0 = make_float2(0.f, 0.f), p1 = p0;
+        if (grow) mref = top;
+        const float ref = (mref > -INFINITY ? mref : 0.f) - kUp;
 #pragma unroll
         for (int c = 0; c < VC; c += 2) {
+          const float2 scale = make_float2(factor[c / 32], factor[c / 32]),
+                       off = make_float2(power[c / 32] - ref, power[c / 32] - ref);
           const float2 x = __ffma2_rn(
               make_float2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale, off);
           v[c] = __float_as_uint(x.x);
@@ -696,19 +748,23 @@ __global__ void __launch_bounds__(
 #pragma unroll
         for (int c = 0; c < VC; ++c) v[c] = __float_as_uint(ex2(__uint_as_float(v[c])));
 #pragma unroll
-        for (int c = 0; c < VC; c += 4) {
-          p0 = __fadd2_rn(p0, make_float2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])));
-          p1 = __fadd2_rn(p1, make_float2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])));
+        for (int cc = 0; cc < VC / 32; ++cc) {
+          float2 p0 = make_float2(0.f, 0.f), p1 = p0;
+#pragma unroll
+          for (int c = 32 * cc; c < 32 * cc + 32; c += 4) {
+            p0 = __fadd2_rn(p0, make_float2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])));
+            p1 = __fadd2_rn(p1, make_float2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])));
+          }
+          lsum = fmaf((p0.x + p0.y) + (p1.x + p1.y), ex2(-power[cc]), lsum);
         }
 #pragma unroll
         for (int c = 0; c < VC / 2; ++c)
           v[c] = Pack2<__half>::pack(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1]));
 #pragma unroll
         for (int cc = 0; cc < VC / 32; ++cc) CS_TMEM_ST16(sc + 16 * (part2 + cc), (v + 16 * cc));
-        lsum = fmaf((p0.x + p0.y) + (p1.x + p1.y), ex2(-power), lsum);
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(at(Sh::bP, qt, t));
+        mbar_arrive(at(Sh::bP, qt, m + t));
       }
 
       // -------------------------------------------------------------- output
@@ -825,10 +881,18 @@ __global__ void __launch_bounds__(
         if (whole) write_lse(a, seg.start, row0 + row, seg.g, lse2);
         else a.part_lse[prow] = lse2;
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(mb + Sh::bFree + 8 * qt);
+      n += steps;
+      m += steps;
+      return ok;
     });
   }
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  tc_fence_before();
+  __syncthreads();
   if (tid == 0 && *abort) report(a.status, CS_ST_TIMEOUT);
   if (warp == Sh::kSoft + 5) {
     tc_fence_after();
