@@ -270,7 +270,7 @@ Plan4 plan4(const cs_kv4_attn_params& p) {
     plan.workers = num_sms() * (plan.rows == 256 ? 1 : 2);
   } else {
     plan.rows = rows <= 8 ? 8 : 16;
-    plan.workers = num_sms() * kv4_decode_blocks(plan.rows);
+    plan.workers = num_sms() * kv4_decode_blocks(plan.rows, p.pool.head_dim, p.pool.group);
   }
   return plan;
 }

@@ -11,7 +11,7 @@ namespace cs {
 
 // the kernel for few query rows a KV head (kv4_decode.cu) and the one for many
 // (kv4_sm100.cu), for `workers` blocks
-int kv4_decode_blocks(int rows);  // an SM's, with so many rows a block
+int kv4_decode_blocks(int rows, int dim, int group);  // an SM's, with so many rows a block
 int kv4_decode(const Attn4& a, const cs_kv4_pool& pool, int rows, int workers,
                cudaStream_t stream);
 int kv4_wide(const Attn4& a, const cs_kv4_pool& pool, int rows, int workers, cudaStream_t stream);

@@ -9,9 +9,10 @@
 // four operand registers with a shift and four ANDs, with no bias to take off
 // and no rounding.  Scale and lowest value of a group enter in float32,
 //   q.k = scale (q.c) + low sum(q),   p v = (p scale) c + p low,
-// where p scale is rounded to fp16 for the product (what that rounding takes is
-// added back in float32 times 8, the codes' middle, so that it acts on the
-// value and not on the code).  Queries are fp16 too, each row scaled by a power
+// where p scale is rounded to fp16 for the product.  (For float16 pools what that
+// rounding takes is added back in float32 times 8, the codes' middle: it then
+// acts on a value's distance from the middle and not on its code.  Bfloat16
+// outputs do not show the difference.)  Queries are fp16 too, each row scaled by a power
 // of two so that its largest element lies in [2^13, 2^14): 16-bit inputs of
 // either type keep every bit down to 2^-27 of that.
 //
@@ -37,6 +38,14 @@ constexpr float kUp = 6.f;  // a new largest p scale is 2^6: fp16's normal numbe
 constexpr float kTooLarge = 0x1p14f;  // it may grow to 2^14 before O is rescaled
 constexpr float kLowest = -3e38f;     // below every score, and finite
 
+// Blocks an SM holds, as the registers allow without spilling in the loop over
+// the keys: 32 decodes of up to 16K keys in four groups take 102 us with three
+// and 129 with four, in two groups 92 and 90; four drafts each (16 rows) in four
+// groups 183 with two and 251 with three, in two groups 159 and 161.
+constexpr int decode_blocks(int tiles, int dim, int groups) {
+  return tiles == 1 ? (dim == 128 && groups == 4 ? 3 : 4) : (dim == 128 ? 2 : 3);
+}
+
 template <int D, int NG, int NT>
 struct Ring {
   static constexpr int RT = 8 * NT;  // query rows of a block
@@ -45,12 +54,14 @@ struct Ring {
   static constexpr int E = NT == 1 ? 2 : 1;
   static constexpr int kStep = kUnit * kWarps * E;  // keys of a block's step
   static constexpr int kStages = 4 / E;             // of E units
-  static constexpr int kBlocks = NT == 1 ? 4 : 3;  // an SM's
+  static constexpr int kBlocks = decode_blocks(NT, D, NG);  // an SM's
   static constexpr int oBars = kWarps * kStages * E * Unit4<D, NG>::kBytes;
   static constexpr int oSums = oBars + kWarps * kStages * 8;
   static constexpr int oMax = oSums + 96;
   static constexpr int oOut = (oMax + 2 * kWarps * RT * 4 + 15) / 16 * 16;
-  static constexpr int kBytes = oOut + kWarps * RT * D * 4;
+  // the queries' operand registers, for 16 rows (those of 8 stay in registers)
+  static constexpr int oQuery = oOut + kWarps * RT * D * 4;
+  static constexpr int kBytes = oQuery + (NT > 1 ? NT * (D / 32) * 512 : 0);
 };
 
 // D += A B, 16 x 8 x 16 in fp16 with float32 sums
@@ -126,6 +137,7 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
   using Share = Share4<R::RT, R::kStep>;
   constexpr int W = U::W, RT = R::RT, S = R::kStages, E = R::E, WG = W / NG;  // words a group
   constexpr int kStage = E * U::kBytes;
+  constexpr bool kCentred = std::is_same<T, __half>::value;
   extern __shared__ __align__(128) char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
@@ -206,7 +218,8 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
     for (int i = 0; i < S && i < count; ++i) send();
 
     // --------------------------------------------------------------- queries
-    uint32_t qf[NT][2 * W][2];      // operand fragments: word w, then its upper half
+    uint4 qf[NT == 1 ? W : 1];      // operand registers: word w's lower half, then its upper
+    uint4* query = reinterpret_cast<uint4*>(smem + R::oQuery) + lane;  // [nt][w], 32 lanes each
     float2 qs[NT][NG];              // sum(q) of rows 2t, 2t + 1, as the products have it
     float2 qm[NT];                  // from there to log2 of the weights
     int limit[NT][2];               // the newest key these rows see
@@ -257,12 +270,14 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
       const float up = pow2(13 - e);
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {  // elements 2k, 2k + 4 and (sixteenths) 2k + 1, 2k + 5
-          qf[nt][2 * w + k][0] = Pack2<__half>::pack(f[w][2 * k] * up, f[w][2 * k + 4] * up);
-          qf[nt][2 * w + k][1] = Pack2<__half>::pack(f[w][2 * k + 1] * (up * 0.0625f),
-                                                     f[w][2 * k + 5] * (up * 0.0625f));
-        }
+        // elements 2k, 2k + 4 and (sixteenths) 2k + 1, 2k + 5
+        const float less = up * 0.0625f;
+        const uint4 y = make_uint4(Pack2<__half>::pack(f[w][0] * up, f[w][4] * up),
+                                   Pack2<__half>::pack(f[w][1] * less, f[w][5] * less),
+                                   Pack2<__half>::pack(f[w][2] * up, f[w][6] * up),
+                                   Pack2<__half>::pack(f[w][3] * less, f[w][7] * less));
+        if constexpr (NT == 1) qf[w] = y;
+        else if (warp == 0) query[32 * (W * nt + w)] = y;
       }
       // the codes are 2^-24 of theirs, the queries `up` of theirs; masked scores
       // are -inf before they are scaled, so the factor is never 0
@@ -281,6 +296,7 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
       }
     }
     low_limit = __reduce_min_sync(~0u, low_limit);
+    if constexpr (NT > 1) __syncthreads();
 
     // ------------------------------------------------------------------ keys
     float o[NT][2 * W][4];
@@ -327,14 +343,15 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
             const uint32_t ya = ka[w] >> 8, yb = kb[w] >> 8;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
+              uint4 q;
+              if constexpr (NT == 1) q = qf[w];
+              else q = query[32 * (W * nt + w)];
               if (w == k * WG)
-                mma16_first(acc[nt], ka[w] & kLow, kb[w] & kLow, ka[w] & kHigh, kb[w] & kHigh,
-                            qf[nt][2 * w][0], qf[nt][2 * w][1]);
+                mma16_first(acc[nt], ka[w] & kLow, kb[w] & kLow, ka[w] & kHigh, kb[w] & kHigh, q.x,
+                            q.y);
               else
-                mma16(acc[nt], ka[w] & kLow, kb[w] & kLow, ka[w] & kHigh, kb[w] & kHigh,
-                      qf[nt][2 * w][0], qf[nt][2 * w][1]);
-              mma16(acc[nt], ya & kLow, yb & kLow, ya & kHigh, yb & kHigh, qf[nt][2 * w + 1][0],
-                    qf[nt][2 * w + 1][1]);
+                mma16(acc[nt], ka[w] & kLow, kb[w] & kLow, ka[w] & kHigh, kb[w] & kHigh, q.x, q.y);
+              mma16(acc[nt], ya & kLow, yb & kLow, ya & kHigh, yb & kHigh, q.z, q.w);
             }
           }
 #pragma unroll
@@ -368,9 +385,9 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
       // ------------------------------------------------------------- weights
       // p scale has to fit fp16 (and p float32): where it would not, the
       // reference moves up and what was summed goes down
-      float2 f[E][2][NG];  // (scale, 8 scale + low, the middle of a group's values)
       float2 p[E][NT][2];
       float most[E][2], top = 0.f;
+      bool careful = false;  // a scale or low that is not finite, and a key hidden from a row
 #pragma unroll
       for (int e = 0; e < E; ++e) {
 #pragma unroll
@@ -379,10 +396,13 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
           Words<NG>::load(v, stage + e * U::kBytes + U::oVp + 4 * NG * (g + 8 * c));
           most[e][c] = 0.f;
 #pragma unroll
-          for (int k = 0; k < NG; ++k) {
-            const float2 y = pair_of<T>(v[k]);
-            f[e][c][k] = make_float2(y.x, fmaf(8.f, y.x, y.y));
-            most[e][c] = fmaxf(most[e][c], y.x);
+          for (int k = 0; k < NG; ++k) most[e][c] = fmaxf(most[e][c], pair_of<T>(v[k]).x);
+          if (some_hidden) {
+#pragma unroll
+            for (int k = 0; k < NG; ++k) {
+              const float2 y = pair_of<T>(v[k]);
+              careful |= !(fabsf(y.x) + fabsf(y.y) < INFINITY);
+            }
           }
         }
       }
@@ -444,18 +464,31 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
         }
         weights();
       }
-      uint32_t pf[E][NT][NG][2];
-      auto weigh = [&](auto hidden) {
+      auto finish = [&](auto hidden) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
+          const char* unit = stage + e * U::kBytes;
+          uint32_t v[4][(W + 1) / 2], va[NG], vb[NG];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
+          for (int k = 0; k < 4; ++k)
+            Words<W / 2>::load(v[k], unit + U::oV + (2 * t + (k & 1) + 4 * (k & 2)) * U::kRow +
+                                         2 * W * g);
+          Words<NG>::load(va, unit + U::oVp + 4 * NG * g);
+          Words<NG>::load(vb, unit + U::oVp + 4 * NG * (g + 8));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
             lsum[nt] = __fadd2_rn(lsum[nt], __fadd2_rn(p[e][nt][0], p[e][nt][1]));
 #pragma unroll
-            for (int k = 0; k < NG; ++k) {
+          for (int k = 0; k < NG; ++k) {
+            uint32_t pf[NT][2];
 #pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                const float2 s = f[e][c][k];
+            for (int c = 0; c < 2; ++c) {
+              float2 s = pair_of<T>(c ? vb[k] : va[k]);
+              // the middle of the group's values, where the weights' rounding is
+              // to act on the values' distance from it
+              if (kCentred) s.y = fmaf(8.f, s.x, s.y);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
                 float2 w = __fmul2_rn(p[e][nt][c], both(s.x));
                 if constexpr (decltype(hidden)::value) {
                   // a scale that is not finite reaches no row that does not see its key
@@ -469,37 +502,29 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
                   lows[nt][k] = __ffma2_rn(p[e][nt][c], both(s.y), lows[nt][k]);
                 }
                 const uint32_t y = Pack2<__half>::pack(w.x, w.y);
-                lows[nt][k] = __ffma2_rn(pair_of<__half>(y), both(-8.f), lows[nt][k]);
-                pf[e][nt][k][c] = transposed(y);
+                if (kCentred) lows[nt][k] = __ffma2_rn(pair_of<__half>(y), both(-8.f), lows[nt][k]);
+                pf[nt][c] = transposed(y);
+              }
+            }
+#pragma unroll
+            for (int w = k * WG; w < (k + 1) * WG; ++w) {
+              const uint32_t sel = w & 1 ? 0x7632u : 0x5410u;
+              const uint32_t xa = __byte_perm(v[0][w / 2], v[1][w / 2], sel);
+              const uint32_t xb = __byte_perm(v[2][w / 2], v[3][w / 2], sel);
+              const uint32_t ya = xa >> 8, yb = xb >> 8;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma16(o[nt][2 * w], xa & kLow, xa & kHigh, xb & kLow, xb & kHigh, pf[nt][0],
+                      pf[nt][1]);
+                mma16(o[nt][2 * w + 1], ya & kLow, ya & kHigh, yb & kLow, yb & kHigh, pf[nt][0],
+                      pf[nt][1]);
               }
             }
           }
         }
       };
-      if (some_hidden) weigh(std::true_type());
-      else weigh(std::false_type());
-      // -------------------------------------------------------------- values
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        uint32_t v[4][(W + 1) / 2];
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          Words<W / 2>::load(v[k], stage + e * U::kBytes + U::oV +
-                                       (2 * t + (k & 1) + 4 * (k & 2)) * U::kRow + 2 * W * g);
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-          const uint32_t sel = w & 1 ? 0x7632u : 0x5410u;
-          const uint32_t xa = __byte_perm(v[0][w / 2], v[1][w / 2], sel);
-          const uint32_t xb = __byte_perm(v[2][w / 2], v[3][w / 2], sel);
-          const uint32_t ya = xa >> 8, yb = xb >> 8;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const uint32_t *b = pf[e][nt][w / WG];
-            mma16(o[nt][2 * w], xa & kLow, xa & kHigh, xb & kLow, xb & kHigh, b[0], b[1]);
-            mma16(o[nt][2 * w + 1], ya & kLow, ya & kHigh, yb & kLow, yb & kHigh, b[0], b[1]);
-          }
-        }
-      }
+      if (__any_sync(~0u, careful)) finish(std::true_type());
+      else finish(std::false_type());
       __syncwarp();  // the units have been read
       if (sent < count) send();
     }
@@ -608,7 +633,9 @@ int launch_decode(const Attn4& a, int workers, cudaStream_t stream) {
 
 }  // namespace
 
-int kv4_decode_blocks(int rows) { return rows <= 8 ? 4 : 3; }
+int kv4_decode_blocks(int rows, int dim, int group) {
+  return decode_blocks(rows <= 8 ? 1 : 2, dim, dim / group);
+}
 
 int kv4_decode(const Attn4& a, const cs_kv4_pool& pool, int rows, int workers,
                cudaStream_t stream) {

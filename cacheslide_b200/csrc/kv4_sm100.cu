@@ -72,7 +72,7 @@ struct Shape4 {
                             bP = bS + 16 * NT, bPV = bP + 16 * NT, bMax = bPV + 16 * NT,
                             bR = bMax + 32 * NT, bRead = bR + 8 * RS, bSeg = bRead + 8 * RS,
                             bSegRead = bSeg + 8 * kSegments, oTmem = bSegRead + 8 * kSegments,
-                            oAbort = oTmem + 4, oFlag = oAbort + 4, oScale = oFlag + 4 * kInfo,
+                            oAbort = oTmem + 4, oWalked = oAbort + 4, oFlag = oWalked + 4, oScale = oFlag + 4 * kInfo,
                             oPower = oScale + 8 * kInfo, oBad = oPower + 8 * kInfo, oRow = oBad + kInfo * kKeys,
                             oMax = oRow + NT * kTileRows * 4,
                             oSeg = oMax + (TPR - 1) * NT * 2 * 2 * 128 * 4,
@@ -179,6 +179,7 @@ __global__ void __launch_bounds__(
   const uint32_t mb = sbase + Sh::oMeta;
   char* meta = smem + Sh::oMeta;
   volatile int* abort = reinterpret_cast<volatile int*>(meta + Sh::oAbort);
+  volatile int* walked = reinterpret_cast<volatile int*>(meta + Sh::oWalked);
   volatile int* flag = reinterpret_cast<volatile int*>(meta + Sh::oFlag);  // step + 1: bad values
   // 2^E of 32 keys, and E of 32 values: [step % kInfo][half]
   volatile float* key_scale = reinterpret_cast<volatile float*>(meta + Sh::oScale);
@@ -214,6 +215,7 @@ __global__ void __launch_bounds__(
     mbar_init_fence();
     for (int k = 0; k < kInfo; ++k) flag[k] = -1;
     *abort = 0;
+    *walked = 0;
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   Share work;
@@ -244,6 +246,23 @@ __global__ void __launch_bounds__(
       __syncwarp();
       if (lane == 0) mbar_arrive(mb + Sh::bSegRead + 8 * k);
     }
+  };
+
+  // A role of the second row tile that has left out segments must not look at a
+  // step's K and V barriers before the steps in between are over (a parity tells
+  // no phase from the last but one): the first tile's MMA warp, which walks every
+  // step, says how many have their tiles.
+  auto caught_up = [&](int qt, int n) {
+    if (NT == 1 || qt == 0 || *walked >= n) return true;
+    const long long t0 = clock64();
+    while (*walked < n) {
+      if (*abort) return false;
+      if (clock64() - t0 > kWaitCycles) {
+        *abort = 1;
+        return false;
+      }
+    }
+    return true;
   };
 
   if (warp >= Sh::kSoft && warp < Sh::kSoft + 4) {
@@ -493,7 +512,9 @@ __global__ void __launch_bounds__(
     if (qt < NT) segments([&](const Segment& seg) {
       const int steps = seg.steps;
       if (qt < seg.tiles) {
-        if (!warp_wait(mb + Sh::bQ + 8 * qt, queries++ & 1, abort)) return false;
+        if (!warp_wait(mb + Sh::bQ + 8 * qt, queries++ & 1, abort) ||
+            !__all_sync(~0u, caught_up(qt, n)))
+          return false;
         auto arrived = [&](uint32_t bar, int u, int stages) {
           return warp_wait(mb + bar + 8 * (u % stages), (u / stages) & 1, abort);
         };
@@ -524,6 +545,7 @@ __global__ void __launch_bounds__(
           const uint32_t ph = ((m + t) >> 1) & 1;
           if (!arrived(Sh::bV, n + t, Sh::VS) || !warp_wait(at(Sh::bP, qt, m + t), ph, abort))
             return false;
+          if (qt == 0 && lane == 0) *walked = n + t + 1;
           tc_fence_after();
           const uint64_t dv = dv0 + (uint64_t)(((n + t) % Sh::VS) * (Sh::TB >> 4));
           const uint32_t p = sc + kKeys * ((m + t) & 1);
@@ -564,7 +586,8 @@ __global__ void __launch_bounds__(
         return true;
       }
       // all rows of the last segment are written: their places may take queries
-      if (queries > 0 && !warp_wait(mb + Sh::bFree + 8 * qt, (queries - 1) & 1, abort))
+      if ((queries > 0 && !warp_wait(mb + Sh::bFree + 8 * qt, (queries - 1) & 1, abort)) ||
+          !__all_sync(~0u, caught_up(qt, n)))
         return false;
       const int r = (warp & 3) * 32 + lane;  // TMEM lane
       const int row = qt * kTileRows + r;    // of the block's

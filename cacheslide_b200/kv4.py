@@ -105,20 +105,22 @@ def append(pool: PagedKV4, slots: Tensor, key: Tensor, value: Tensor, *,
     distinct slots.  A serving operator without a derivative."""
     device = _pool(pool)
     n = _slots(slots, pool)
-    rows = []
+    shape = (n, pool.kv_heads, pool.head_dim)
     for name, x in (("key", key), ("value", value)):
-        if x.shape != (n, pool.kv_heads, pool.head_dim) or x.dtype is not pool.dtype or \
-                x.get_device() != device:
+        if x.shape != shape or x.dtype is not pool.dtype or x.get_device() != device:
             raise ValueError(f"{name} must be {pool.dtype} [token, {pool.kv_heads}, "
                              f"{pool.head_dim}] on the pool's device")
-        x = x if x.stride(2) == 1 else x.contiguous()
-        rows += [x]
-    key, value = rows
+    ks, vs = key.stride(), value.stride()
+    if ks[2] != 1:
+        key = key.contiguous()
+        ks = key.stride()
+    if vs[2] != 1:
+        value = value.contiguous()
+        vs = value.stride()
     status_ptr = N.status_ptr(status, device)
     N.require_cuda(pool.storage)
-    N.launch("cs_kv4_append", pool.device, pool.view, slots.data_ptr(), n, key.data_ptr(),
-             key.stride(0), key.stride(1), value.data_ptr(), value.stride(0), value.stride(1),
-             status_ptr)
+    N.launch("cs_kv4_append", pool.device, pool.view, slots.data_ptr(), n, key.data_ptr(), ks[0],
+             ks[1], value.data_ptr(), vs[0], vs[1], status_ptr)
 
 
 def gather(pool: PagedKV4, slots: Tensor, *,
@@ -132,7 +134,7 @@ def gather(pool: PagedKV4, slots: Tensor, *,
     status_ptr = N.status_ptr(status, device)
     N.require_cuda(pool.storage)
     key, value = torch.empty(2, n, pool.kv_heads, pool.head_dim, dtype=pool.dtype,
-                             device=pool.device)
+                             device=pool.device).unbind(0)
     st = key.stride()
     N.launch("cs_kv4_gather", pool.device, pool.view, slots.data_ptr(), n, key.data_ptr(), st[0],
              st[1], value.data_ptr(), st[0], st[1], status_ptr)

@@ -97,15 +97,14 @@ def step_maps(lengths: Tensor, new: Tensor, tables: Tensor, block_size: int, num
     if device < 0:
         N.require_cuda(tables)
     on = tables.device
-    # the int64 arrays and the int32 ones each from one allocation
-    wide = torch.empty(2 * tokens + (keys + requests + 1 if keys else 0), dtype=torch.int64,
-                       device=on)
-    narrow = torch.empty(requests + 1 + (free is not None), dtype=torch.int32, device=on)
-    positions, slots = wide[:tokens], wide[tokens:2 * tokens]
-    key_slots = wide[2 * tokens:2 * tokens + keys] if keys else None
-    key_starts = wide[2 * tokens + keys:] if keys else None
-    starts = narrow[:requests + 1]
-    left = narrow[requests + 1:] if free is not None else None
+    positions, slots = torch.empty(2, tokens, dtype=torch.int64, device=on).unbind(0)
+    starts = torch.empty(requests + 1, dtype=torch.int32, device=on)
+    left = key_starts = key_slots = None
+    if free is not None:
+        left = torch.empty(1, dtype=torch.int32, device=on)
+    if keys:
+        key_slots = torch.empty(keys, dtype=torch.int64, device=on)
+        key_starts = torch.empty(requests + 1, dtype=torch.int64, device=on)
     p = N.StepMapsParams(
         p_lengths, p_new, requests, block_size, num_blocks, tables.data_ptr(), tables.stride(0),
         width, offset, p_free, p_count, N.ptr(left), tokens, keys, starts.data_ptr(),

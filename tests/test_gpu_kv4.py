@@ -237,6 +237,28 @@ def test_small_and_large_keys(cuda, scale_k, new):
          scale_k=scale_k)
 
 
+@pytest.mark.parametrize("dtype,dim,group", [(torch.float16, 64, 32), (torch.bfloat16, 128, 128)])
+@pytest.mark.parametrize("hq,hk,new", [(16, 4, [3, 150, 40, 66, 7, 149, 12, 64, 65, 90, 3, 128, 130]),
+                                       (8, 8, [129, 300, 5, 260, 128, 511, 1, 257, 256, 140]),
+                                       (8, 1, [5, 16, 30, 2, 17, 33, 9])])
+def test_row_tiles_of_all_sizes_over_and_over(cuda, dtype, dim, group, hq, hk, new):
+    """Blocks that go from tiles of one row half to tiles of two and back: the
+    results are right, and the same in every call."""
+    lengths = [n + 53 * (b * b % 29) for b, n in enumerate(new)]
+    pool, table, q, starts = _batch(cuda, 4, new, lengths, hq, hk, dim, group, 16, dtype)
+    args = (q.to(cuda), pool, table.to(cuda),
+            torch.tensor(lengths, dtype=torch.int32, device=cuda), starts.to(cuda))
+    status = N.Status(cuda)
+    got, lse = kv4.attention(*args, return_lse=True, status=status)
+    _check(got, lse, pool, table, q, starts, lengths, dim ** -0.5, _wide(new, hq // hk))
+    busy = torch.empty(1 << 26, dtype=torch.uint8, device=cuda)
+    for i in range(60):
+        if i % 3 == 0:
+            busy.fill_(i)  # another state of the caches, other times of arrival
+        assert torch.equal(kv4.attention(*args, status=status), got), i
+    assert status.read() == 0
+
+
 def test_more_requests_than_threads(cuda):
     _run(cuda, [1] * 700, [1 + 37 * b % 120 for b in range(700)], 2, 1, 64, 32, 16,
          torch.bfloat16, one=True)
