@@ -103,8 +103,8 @@ def attention(q, storage, table, length, n, group, scale, wide):
     Score error: float32 sums of products of codes (15 s + |low| bounds what is
     added up) and, of the kernel for many rows, keys rounded to fp16.  Weights
     are rounded to fp16 (half a step, 2^-11): that acts on the codes' distance
-    from their middle (8 s; of bfloat16 pools on the codes, 15 s) or, of the
-    kernel for many rows, on the value, which is rounded too;
+    from their middle (8 s at most) or, of the kernel for many rows, on the
+    value, which is rounded too;
     weights below fp16's normal numbers (2^-20 of a unit's largest at least) by
     2^-25 of 2^6."""
     hk, d = storage.shape[1], q.shape[-1]
@@ -137,7 +137,7 @@ def attention(q, storage, table, length, n, group, scale, wide):
         return torch.where(seen.permute(0, 3, 1, 2)[..., None], y, 0.0).sum(1)
 
     o = mix(w, v)
-    middle = v.abs() if wide else (8 if q.dtype is torch.float16 else 15) * vs
+    middle = v.abs() if wide else 8 * vs
     err = mix(w * dz.nan_to_num(), v.abs()) * 2 + 2.0 ** -11 * mix(w, middle) * (2 if wide else 1)
     err = err + 2.0 ** -24 * vs.nan_to_num().amax() * 16
     lse = torch.where(some, top + torch.where(some, total, 1.0).log(), -math.inf)[..., 0]

@@ -171,7 +171,8 @@ def _check(got, lse, pool, table, q, starts, lengths, scale, wide, rows=None):
         some = l != -math.inf
         assert torch.equal(lse[lo:hi] == -math.inf, ~some), b
         near = (lse[lo:hi] - l).abs() <= 2.0 ** (-9 if wide else -16) * (1 + l.abs())
-        assert (near | ~some | torch.isnan(l)).all(), b
+        off = (lse[lo:hi] - l).abs().masked_fill(~some | torch.isnan(l), 0)
+        assert (near | ~some | torch.isnan(l)).all(), (b, off.max(), off.argmax(), l.flatten()[off.argmax()])
 
 
 def _run(cuda, new, lengths, hq, hk, dim, group, block, dtype, seed=0, scale=None, one=False,
@@ -290,6 +291,36 @@ def test_records_that_are_not_finite_reach_the_rows_that_see_them(cuda, new):
         starts.to(cuda), return_lse=True, status=status)
     assert status.read() == 0 and torch.isnan(got).any() and not torch.isnan(got).all()
     _check(got, lse, pool, table, q, starts, lengths, 128 ** -0.5, _wide([new, new], 2))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new", [1, 4, 40])
+def test_whatever_lies_behind_the_last_token(cuda, dtype, new):
+    """Blocks full of large numbers, infinities and NaN behind the lengths, and
+    the same left in shared memory by a call before."""
+    lengths = [max(new, n) for n in (1, 9, 16, 65, 130, 260)]
+    pool, table, q, starts = _batch(cuda, 12, [new] * 6, lengths, 8, 2, 128, 64, 16, dtype)
+    args = (table.to(cuda), torch.tensor(lengths, dtype=torch.int32, device=cuda), starts.to(cuda))
+    want = kv4.attention(q.to(cuda), pool, *args)
+    big = torch.finfo(dtype).max
+    for value in (big, -big, math.nan, math.inf):
+        rows = torch.full((pool.num_blocks * 16, 2, 128), value, dtype=dtype, device=cuda)
+        rows[..., ::2] = 0
+        other = kv4.empty_pool(pool.num_blocks, 2, 16, 128, dtype, cuda, 64)
+        kv4.append(other, torch.arange(len(rows), device=cuda), rows, rows)
+        kv4.attention(q.to(cuda), other, *args)
+        for b, length in enumerate(lengths):
+            at = torch.arange(length)
+            slots = (table[b][at // 16].long() * 16 + at % 16).to(cuda)
+            # exact copies of the records
+            unit, r = slots // 16, slots % 16
+            for base, size in ((0, 64), (1024, 64), (2048, 8), (2176, 8)):
+                where = (base + r[:, None] * size + torch.arange(size, device=cuda))[:, None]
+                where = where.expand(-1, 2, -1)
+                src = pool.storage[unit][:, :, 0].gather(2, where)
+                for h in (0, 1):
+                    other.storage[unit[:, None], h, 0, where[:, h]] = src[:, h]
+        assert torch.equal(kv4.attention(q.to(cuda), other, *args), want), value
 
 
 @pytest.mark.parametrize("new", [1, 40])
