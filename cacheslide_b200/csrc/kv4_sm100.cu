@@ -16,9 +16,10 @@
 // and values by one a step (of what the step's scales and lowest values can
 // reach), so bfloat16 pools of any size of numbers keep fp16's 11 bits, where
 // bfloat16 operands would keep 8.  P carries the values' power of two, the
-// rows' sums do not.  Float16 outputs show the rounding of such keys (0.00047 to
-// 0.00054 off, 0.00021 of which is the output's own), so the keys of float16
-// pools are two operands, scale (code - zero) and what is left.
+// rows' sums do not.  Float16 outputs would show the rounding of such keys and
+// values (0.00047 to 0.00054 off with both, 0.00033 with the values', 0.00021 of
+// which is the output's own), so those of float16 pools are two operands each,
+// scale (code - zero) and what is left.
 //
 // Pairs lie in the tiles as the codes come, elements (0, 4), (1, 5), (2, 6), (3,
 // 7) of eight: the queries are written in the same order, and the output's
@@ -42,7 +43,7 @@ constexpr float kUp = 7.f;        // P is stored up by 2^7: fp16's normal number
 constexpr int kInfo = 8;          // steps whose scales are kept
 constexpr int kSegments = 4;      // segments the loader may be ahead
 
-// TERMS 2: key tiles in two parts (float16 pools)
+// TERMS 2: key and value tiles in two parts (float16 pools)
 template <int D, int NG, int NT, int TERMS>
 struct Shape4 {
   // threads a row in the softmax, as in the wide blocks of the shared-prefix kernel
@@ -57,13 +58,14 @@ struct Shape4 {
                        kMakeRegs = 72, kRestRegs = 56;
   static_assert(kSoft * kSoftRegs + 4 * (kMakeRegs + kRestRegs) <= (kSoft + 8) * kLaunchRegs,
                 "more registers than the block is launched with");
-  static constexpr uint32_t TB = kKeys * D * 2;  // a V tile, or a part of a K tile
+  static constexpr uint32_t TB = kKeys * D * 2;  // (a part of) a K or V tile
   static constexpr uint32_t RB = (kKeys / kUnit) * Unit4<D, NG>::kBytes;  // a step's raw units
   // stages of K and V tiles, and of raw units (two blocks of one row tile share an SM)
-  static constexpr int KS = NT == 1 && TERMS == 2 ? 1 : 2, VS = 2, RS = NT == 1 ? 1 : 3;
+  static constexpr int KS = NT == 1 && TERMS == 2 ? 1 : 2, VS = KS,
+                       RS = NT == 1 ? 1 : TERMS == 2 ? 2 : 3;
   // a query tile's place also takes its output rows, 2 D bytes each and 16 more
   static constexpr uint32_t QB = kTileRows * D * 2 + kTileRows * 16;
-  static constexpr uint32_t oQ = 0, oK = NT * QB, oV = oK + KS * TERMS * TB, oR = oV + VS * TB,
+  static constexpr uint32_t oQ = 0, oK = NT * QB, oV = oK + KS * TERMS * TB, oR = oV + VS * TERMS * TB,
                             oMeta = oR + RS * RB;
   // barriers: a row tile's queries, and their place free; a stage's K and V; a score buffer's S, P and
   // PV of a row tile; a row's maxima; raw units there, and read; a segment said,
@@ -248,7 +250,7 @@ __global__ void __launch_bounds__(
     }
   };
 
-  // A role of the second row tile that has left out segments must not look at a
+  // The second row tile's MMA warp, having left out segments, must not look at a
   // step's K and V barriers before the steps in between are over (a parity tells
   // no phase from the last but one): the first tile's MMA warp, which walks every
   // step, says how many have their tiles.
@@ -279,7 +281,7 @@ __global__ void __launch_bounds__(
       const int steps = seg.steps, seen = seg.seen, first_key = seg.s0 * kKeys + 32 * half + r;
       const bool two = seg.tiles == 2;
       for (int t = 0; t < steps; ++t, ++n) {
-        uint32_t code[4][W], pair[4][NG];
+        uint32_t code[4][W], pair[4][NG], values[4][NG];
         if (!warp_wait(mb + Sh::bR + 8 * (n % RS), (n / RS) & 1, abort)) return false;
         const char* units = smem + Sh::oR + (n % RS) * Sh::RB;
 #pragma unroll
@@ -288,6 +290,7 @@ __global__ void __launch_bounds__(
           const int token = 8 * (j & 1) + r;
           load_words(code[j], p + (isv ? U::oV : 0) + token * U::kRow + 4 * W * c);
           load_words(pair[j], p + (isv ? U::oVp : U::oKp) + 4 * NG * token);
+          if (!isv) load_words(values[j], p + U::oVp + 4 * NG * token);
         }
         // The stage may be filled again once these loads have come back, which an
         // arrival does not wait for by itself: it is made by a lane that a vote
@@ -298,38 +301,42 @@ __global__ void __launch_bounds__(
 #pragma unroll
           for (int w = 0; w < W; ++w) words |= code[j][w];
 #pragma unroll
-          for (int k = 0; k < NG; ++k) words |= pair[j][k];
+          for (int k = 0; k < NG; ++k) words |= isv ? pair[j][k] : pair[j][k] | values[j][k];
         }
         if (lane == (__any_sync(~0u, words == 0x9e3779b9u) ? 1 : 0))
           mbar_arrive(mb + Sh::bRead + 8 * (n % RS));
-        // ------------------------------- the step's power of two, bad values
+        // ------------------------------- the powers of two, bad values
+        // (the K warps look at the values' pairs too, and say with the key tile
+        // what the softmax has to know of them)
         const int key0 = first_key + t * kKeys;
-        float2 f[4][NG];
-        float reach = 0.f;
-        uint32_t wrong = 0u;  // bit NG j + k
+        auto reach_of = [&](uint32_t (&pairs)[4][NG], uint32_t& wrong) {
+          float reach = 0.f;
+          wrong = 0u;  // bit NG j + k
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (key0 + 8 * j >= seen) {  // zeros: P is zero there too
+          for (int j = 0; j < 4; ++j) {
 #pragma unroll
-            for (int k = 0; k < NG; ++k) pair[j][k] = 0u;
-          }
-#pragma unroll
-          for (int k = 0; k < NG; ++k) {
-            f[j][k] = pair_of<T>(pair[j][k]);
-            const float m = fmaxf(fabsf(f[j][k].y), fabsf(fmaf(15.f, f[j][k].x, f[j][k].y)));
-            if (m < INFINITY && f[j][k].x == f[j][k].x) {
-              reach = fmaxf(reach, m);
-            } else {
-              wrong |= 1u << (NG * j + k);
-              // a bad value becomes 0 here and marks the rows that see it
-              if (isv) f[j][k] = make_float2(0.f, 0.f);
+            for (int k = 0; k < NG; ++k) {
+              if (key0 + 8 * j >= seen) pairs[j][k] = 0u;  // zeros: P is zero there too
+              const float2 f = pair_of<T>(pairs[j][k]);
+              const float m = fmaxf(fabsf(f.y), fabsf(fmaf(15.f, f.x, f.y)));
+              if (m < INFINITY && f.x == f.x) reach = fmaxf(reach, m);
+              else wrong |= 1u << (NG * j + k);
             }
           }
-        }
-        int e = 0;
-        if constexpr (TERMS == 1) {
+          if constexpr (TERMS == 2) return 0;
           const uint32_t m = __reduce_max_sync(~0u, __float_as_uint(reach));
-          e = m == 0u ? 0 : min(114, max(-80, (int)(m >> 23) - 127 - 13));
+          return m == 0u ? 0 : min(114, max(-80, (int)(m >> 23) - 127 - 13));
+        };
+        uint32_t wrong, wrong_values = 0u;
+        const int e = reach_of(pair, wrong);
+        const int ev = isv ? 0 : reach_of(values, wrong_values);
+        if (isv && wrong) {  // a bad value becomes 0 and marks the rows that see it
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int k = 0; k < NG; ++k)
+              if (wrong >> (NG * j + k) & 1u) pair[j][k] = 0u;
+          }
         }
         const float down = pow2(-e);
         // --------------------------------------------------- a free stage
@@ -342,49 +349,43 @@ __global__ void __launch_bounds__(
             return false;
         }
         second[n & 1] = two ? n1++ : -1;
-        if (lane == 0) {
-          if (isv) val_power[2 * (n % kInfo) + half] = (float)e;
-          else key_scale[2 * (n % kInfo) + half] = pow2(e);
-        }
-        if (isv) {
-          const uint32_t tile = sbase + Sh::oV + (n % Sh::VS) * Sh::TB;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-              const uint32_t x = __byte_perm(code[j][w / 2], code[j][W / 2 + w / 2],
-                                             w & 1 ? 0x7632u : 0x5410u);
-              st_shared16(tile + sw128(32 * half + 8 * j + r, 4 * w + c, kKeys),
-                          decode8(x, __float2half2_rn(f[j][w / WG].x * down),
-                                  __float2half2_rn(f[j][w / WG].y * down)));
-            }
-            if (c == 0)
-              bad[(n % kInfo) * kKeys + 32 * half + 8 * j + r] =
-                  (uint8_t)(wrong >> (NG * j) & ((1u << NG) - 1u));
+        if (!isv) {
+          const int info = n % kInfo;
+          if (lane == 0) {
+            key_scale[2 * info + half] = pow2(e);
+            val_power[2 * info + half] = (float)ev;
           }
-          if (wrong) flag[n % kInfo] = n;
-        } else {
-          const uint32_t tile = sbase + Sh::oK + (n % KS) * TERMS * Sh::TB;
+          if (c == 0) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < 4; ++j)
+              bad[info * kKeys + 32 * half + 8 * j + r] =
+                  (uint8_t)(wrong_values >> (NG * j) & ((1u << NG) - 1u));
+          }
+          if (wrong_values) flag[info] = n;
+        }
+        const uint32_t tile =
+            sbase + (isv ? Sh::oV + (n % Sh::VS) * TERMS * Sh::TB : Sh::oK + (n % KS) * TERMS * Sh::TB);
 #pragma unroll
-            for (int w = 0; w < W; ++w) {
-              const uint32_t to = tile + sw128(32 * half + 8 * j + r, 4 * w + c, kKeys);
-              const float2 y = f[j][w / WG];
-              if constexpr (TERMS == 1) {
-                st_shared16(to, decode8(code[j][w], __float2half2_rn(y.x * down),
-                                        __float2half2_rn(y.y * down)));
-              } else {
-                const uint32_t main = (pair[j][w / WG] + 8u) & 0xfff0u;  // 7 significant bits
-                const float zero = fminf(fmaxf(rintf(-y.y * rcp_approx(y.x)), 0.f), 15.f);
-                uint4 x, rest;
-                decode8(code[j][w], as_half2(main * 0x10001u),
-                        __float2half2_rn(y.x - pair_of<T>(main).x),
-                        __float2half2_rn(fmaf(zero, y.x, y.y)), __float2half2_rn(1024.f + zero), x,
-                        rest);
-                st_shared16(to, x);
-                st_shared16(to + Sh::TB, rest);
-              }
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int w = 0; w < W; ++w) {
+            const uint32_t to = tile + sw128(32 * half + 8 * j + r, 4 * w + c, kKeys);
+            const uint32_t x = isv ? __byte_perm(code[j][w / 2], code[j][W / 2 + w / 2],
+                                                 w & 1 ? 0x7632u : 0x5410u)
+                                   : code[j][w];
+            const float2 y = pair_of<T>(pair[j][w / WG]);
+            if constexpr (TERMS == 1) {
+              st_shared16(to, decode8(x, __float2half2_rn(y.x * down),
+                                      __float2half2_rn(y.y * down)));
+            } else {
+              const uint32_t main = (pair[j][w / WG] + 8u) & 0xfff0u;  // 7 significant bits
+              const float zero = fminf(fmaxf(rintf(-y.y * rcp_approx(y.x)), 0.f), 15.f);
+              uint4 first, rest;
+              decode8(x, as_half2(main * 0x10001u), __float2half2_rn(y.x - pair_of<T>(main).x),
+                      __float2half2_rn(fmaf(zero, y.x, y.y)), __float2half2_rn(1024.f + zero),
+                      first, rest);
+              st_shared16(to, first);
+              st_shared16(to + Sh::TB, rest);
             }
           }
         }
@@ -547,14 +548,18 @@ __global__ void __launch_bounds__(
             return false;
           if (qt == 0 && lane == 0) *walked = n + t + 1;
           tc_fence_after();
-          const uint64_t dv = dv0 + (uint64_t)(((n + t) % Sh::VS) * (Sh::TB >> 4));
+          const uint64_t dv = dv0 + (uint64_t)(((n + t) % Sh::VS) * TERMS * (Sh::TB >> 4));
           const uint32_t p = sc + kKeys * ((m + t) & 1);
           last = at(Sh::bPV, qt, m + t);
           lastph = ph;
           if (leader) {
 #pragma unroll
-            for (int kk = 0; kk < kKeys / 16; ++kk)
-              tc_mma_ts(oc, p + kk * 8, dv + kk * 128, id_o, (t | kk) ? 1u : 0u);
+            for (int term = 0; term < TERMS; ++term) {
+#pragma unroll
+              for (int kk = 0; kk < kKeys / 16; ++kk)
+                tc_mma_ts(oc, p + kk * 8, dv + term * (Sh::TB >> 4) + kk * 128, id_o,
+                          (t | kk | term) ? 1u : 0u);
+            }
             tc_commit(last);
           }
           __syncwarp();
@@ -586,8 +591,7 @@ __global__ void __launch_bounds__(
         return true;
       }
       // all rows of the last segment are written: their places may take queries
-      if ((queries > 0 && !warp_wait(mb + Sh::bFree + 8 * qt, (queries - 1) & 1, abort)) ||
-          !__all_sync(~0u, caught_up(qt, n)))
+      if (queries > 0 && !warp_wait(mb + Sh::bFree + 8 * qt, (queries - 1) & 1, abort))
         return false;
       const int r = (warp & 3) * 32 + lane;  // TMEM lane
       const int row = qt * kTileRows + r;    // of the block's
@@ -663,10 +667,7 @@ __global__ void __launch_bounds__(
         const int vhi = limit - base >= kKeys ? kKeys : limit - base + 1;  // keys seen
         const uint32_t sc = sc0 + kKeys * ((m + t) & 1);
         const int info = (n + t) % kInfo;
-        // the values' power and bad groups come with the values (whose barrier
-        // cannot move on before this step's P is there)
-        ok = warp_wait(at(Sh::bS, qt, m + t), ((m + t) >> 1) & 1, abort) &&
-             warp_wait(mb + Sh::bV + 8 * ((n + t) % Sh::VS), ((n + t) / Sh::VS) & 1, abort);
+        ok = warp_wait(at(Sh::bS, qt, m + t), ((m + t) >> 1) & 1, abort);
         if (!ok) break;  // a wait expired
         tc_fence_after();
         uint32_t v[VC];
