@@ -9,9 +9,8 @@
 // word.  Both are bound by HBM: rows of D = 128 in groups of 64 move 512 + 144
 // bytes a (token, head).
 //
-// A code is decided exactly (as with the quotient in infinite precision): the
-// product with 1 / scale is within 3e-6 of it, and where that leaves a doubt
-// about the nearest number the remainder, which is exact, decides.
+// A code is decided as with the quotient in infinite precision: that is either
+// half way between two codes or 2^-16 of itself from there (scales have 11 bits).
 #include <math.h>
 
 #include <type_traits>
@@ -30,6 +29,20 @@ struct Rows4 {
   int64_t st, sh;  // byte strides of tokens and heads
 };
 
+// A block takes a head of 16 (D = 64: 32) neighbouring tokens, whose records are
+// mostly neighbours too: their stores then fill whole lines.  (Blocks of two
+// tokens' eight heads took 139 us for 65536 tokens of 8 heads of 128.)
+struct Row4 {
+  int64_t token;
+  int head;
+};
+template <int L>
+__device__ __forceinline__ Row4 row_of(int hkv) {
+  const unsigned group = blockIdx.x / (unsigned)hkv;
+  return Row4{(int64_t)group * (kRowThreads / L) + threadIdx.x / L,
+              (int)(blockIdx.x - group * (unsigned)hkv)};
+}
+
 template <typename T> __device__ __forceinline__ float overflow_of();  // rounds to infinity
 template <> __device__ __forceinline__ float overflow_of<__half>() { return 65520.f; }
 template <> __device__ __forceinline__ float overflow_of<__nv_bfloat16>() {
@@ -43,81 +56,112 @@ template <typename T> __device__ __forceinline__ float of_bits(uint32_t b) {
   return pair_of<T>(b & 0xffffu).x;
 }
 
+template <typename T> struct Pair16;
+template <> struct Pair16<__half> {
+  using type = __half2;
+};
+template <> struct Pair16<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+};
+template <typename T> using pair16 = typename Pair16<T>::type;
+template <typename T> __device__ __forceinline__ pair16<T> as_pair(uint32_t x) {
+  return *reinterpret_cast<pair16<T>*>(&x);
+}
+template <typename P> __device__ __forceinline__ uint32_t pair_bits(P x) {
+  return *reinterpret_cast<uint32_t*>(&x);
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
 // eight elements' codes (element i in bits 4 i ..) and their group's (scale, low)
 template <typename T, int LANES>
 __device__ __forceinline__ uint32_t encode(const uint32_t (&x)[4], uint32_t& pair) {
-  float v[8];
-  float lo = INFINITY, hi = -INFINITY;
-  bool nan = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = pair_of<T>(x[i]);
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
-    lo = fminf(lo, fminf(f.x, f.y));
-    hi = fmaxf(hi, fmaxf(f.x, f.y));
-    nan |= f.x != f.x || f.y != f.y;
+  // the extremes as a pair (least, -most), NaN if any element is
+  uint32_t least, most;
+  {
+    const auto a = __hmin2_nan(__hmin2_nan(as_pair<T>(x[0]), as_pair<T>(x[1])),
+                               __hmin2_nan(as_pair<T>(x[2]), as_pair<T>(x[3])));
+    const auto b = __hmax2_nan(__hmax2_nan(as_pair<T>(x[0]), as_pair<T>(x[1])),
+                               __hmax2_nan(as_pair<T>(x[2]), as_pair<T>(x[3])));
+    least = pair_bits(a), most = pair_bits(b) ^ 0x80008000u;
   }
-  if (nan) hi = INFINITY;  // as an infinity makes it: not finite
+  uint32_t ends = pair_bits(__hmin2_nan(as_pair<T>(__byte_perm(least, most, 0x5410u)),
+                                        as_pair<T>(__byte_perm(least, most, 0x7632u))));
 #pragma unroll
-  for (int o = 1; o < LANES; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(~0u, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, o));
-  }
+  for (int o = 1; o < LANES; o <<= 1)
+    ends = pair_bits(__hmin2_nan(as_pair<T>(ends), as_pair<T>(__shfl_xor_sync(~0u, ends, o))));
+  const float2 end = pair_of<T>(ends ^ 0x80000000u);
+  const float lo = end.x, hi = end.y;
   // a sixteenth of the range, which cannot overflow
-  const float range = hi * 0.0625f - lo * 0.0625f;
-  if (!(fabsf(range) < INFINITY)) {
+  const float range = fabsf(hi * 0.0625f - lo * 0.0625f);  // (no zero with a sign)
+  if (!(range < INFINITY)) {
     pair = 0x7fff7fffu;  // NaN in both types
     return 0u;
   }
-  uint32_t sb = bits_of<T>(__fdiv_rn(range, 0.9375f));
+  // range / 0.9375, rounded to nearest: the product with the rounded reciprocal,
+  // corrected once by its exact remainder (Markstein 1990)
+  constexpr float kRecip = 16.f / 15.f;
+  const float near = range * kRecip;
+  uint32_t sb = bits_of<T>(fmaf(fmaf(-0.9375f, near, range), kRecip, near));
   float s = of_bits<T>(sb);
   if (!(fmaf(15.f, s, lo) < overflow_of<T>())) s = of_bits<T>(--sb);
-  pair = sb | bits_of<T>(lo) << 16;
+  pair = sb | (lo == 0.f ? 0u : ends << 16);  // (a zero without a sign)
   if (sb == 0) return 0u;
   // both scaled by a power of two, so that 1 / s and the differences are finite
   const float up = s < 0x1p-60f ? 0x1p60f : 0x1p-4f;
-  const float su = s * up, lu = lo * up, inv = __fdiv_rn(1.f, su);
-  uint32_t word = 0u;
-  float doubt = 0.f;
+  const float su = s * up, lu = lo * up, inv = rcp_approx(su);
+  // Quotients, corrected once by their exact remainders: a quotient that lies
+  // half way between two codes then comes out exactly (and goes to the even one),
+  // and none other is as near to a half way as its error.  Four codes become one
+  // number of 16 bits.
+  constexpr float kWhole = 0x1.8p23f;
+  const bool over = (hi * up - lu) * inv > 15.4f;  // a scale of few bits: codes over 15
+  float2 c[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float f = fmaf(v[i], up, -lu) * inv;
-    const float c = fminf(f, 15.f) + 0x1.8p23f;  // to the nearest whole number
-    word |= (__float_as_uint(c) & 15u) << (4 * i);
-    doubt = fmaxf(doubt, fabsf(f - (c - 0x1.8p23f)));
+  for (int i = 0; i < 4; ++i) {
+    const float2 d = __ffma2_rn(pair_of<T>(x[i]), both(up), both(-lu));
+    const float2 f = __fmul2_rn(d, both(inv));
+    c[i] = __ffma2_rn(__ffma2_rn(f, both(-su), d), both(inv), f);
+    if (over) c[i] = make_float2(fminf(c[i].x, 15.f), fminf(c[i].y, 15.f));
+    c[i] = __fadd2_rn(__fadd2_rn(c[i], both(kWhole)), both(-kWhole));
   }
-  if (doubt > 0.49999f) {
-    word = 0u;
-#pragma unroll 1
-    for (int i = 0; i < 8; ++i) {
-      // v[i] by its register: the loop is not unrolled
-      float x1 = v[0];
+  const float low4 = fmaf(c[1].y, 4096.f, fmaf(c[1].x, 256.f, fmaf(c[0].y, 16.f, c[0].x)));
+  const float high4 = fmaf(c[3].y, 4096.f, fmaf(c[3].x, 256.f, fmaf(c[2].y, 16.f, c[2].x)));
+  return __byte_perm(__float_as_uint(low4 + kWhole), __float_as_uint(high4 + kWhole), 0x5410u);
+}
+
+// a pair of codes, in bits 0 .. 3 and 16 .. 19, as numbers (exact)
+template <typename T> __device__ __forceinline__ pair16<T> whole_pair(uint32_t x);
+template <> __device__ __forceinline__ __half2 whole_pair<__half>(uint32_t x) {
+  return __hsub2(as_pair<__half>(x | 0x64006400u), as_pair<__half>(0x64006400u));  // 1024
+}
+template <> __device__ __forceinline__ __nv_bfloat162 whole_pair<__nv_bfloat16>(uint32_t x) {
+  return __hsub2(as_pair<__nv_bfloat16>(x | 0x43004300u),
+                 as_pair<__nv_bfloat16>(0x43004300u));  // 128
+}
+
+// eight codes as low + scale code, rounded once
+template <typename T>
+__device__ __forceinline__ uint4 decode(uint32_t code, uint32_t pair) {
+  const pair16<T> scale = as_pair<T>(__byte_perm(pair, 0u, 0x1010u)),
+                  low = as_pair<T>(__byte_perm(pair, 0u, 0x3232u));
+  uint32_t y[4];  // elements (i, i + 4)
 #pragma unroll
-      for (int k = 1; k < 8; ++k) x1 = i == k ? v[k] : x1;
-      const float d = fmaf(x1, up, -lu);
-      int c = (int)rintf(fminf(d * inv, 15.f));
-      const float rest = fmaf(-(float)c, su, d), half = 0.5f * su;
-      if (rest > half || (rest == half && (c & 1))) ++c;
-      else if (rest < -half || (rest == -half && (c & 1))) --c;
-      word |= (uint32_t)min(c, 15) << (4 * i);
-    }
-  }
-  return word;
+  for (int i = 0; i < 4; ++i)
+    y[i] = pair_bits(__hfma2(whole_pair<T>(code >> (4 * i) & 0x000f000fu), scale, low));
+  return make_uint4(__byte_perm(y[0], y[1], 0x5410u), __byte_perm(y[2], y[3], 0x5410u),
+                    __byte_perm(y[0], y[1], 0x7632u), __byte_perm(y[2], y[3], 0x7632u));
 }
 
 template <typename T, int D, int NG>
 __global__ void __launch_bounds__(kRowThreads)
-    kv4_append_kernel(const Pool4 pool, const int64_t* slots, int64_t rows, const Rows4 k,
+    kv4_append_kernel(const Pool4 pool, const int64_t* slots, int64_t n, const Rows4 k,
                       const Rows4 v, int vec, int32_t* status) {
   using U = Unit4<D, NG>;
   constexpr int L = D / 8, LG = L / NG, W = U::W;  // lanes a row and a group
-  const int64_t at = ((int64_t)blockIdx.x * kRowThreads + threadIdx.x) / L;
-  const int lane = threadIdx.x % L;
-  const bool in = at < rows;
-  const int64_t row = in ? at : 0;
-  const int64_t token = row / pool.hkv;
-  const int head = (int)(row - token * pool.hkv);
+  const Row4 w4 = row_of<L>(pool.hkv);
+  const int64_t token = w4.token;
+  const int head = w4.head, lane = threadIdx.x % L;
+  const bool in = token < n;
   const int64_t slot = in ? slots[token] : -1;
   const bool live = pool.valid(slot);
   if (in && !live && slot != -1 && lane == 0 && head == 0) report(status, CS_ST_SLOT_RANGE);
@@ -161,15 +205,14 @@ __global__ void __launch_bounds__(kRowThreads)
 
 template <typename T, int D, int NG>
 __global__ void __launch_bounds__(kRowThreads)
-    kv4_gather_kernel(const Pool4 pool, const int64_t* slots, int64_t rows, const Rows4 k,
+    kv4_gather_kernel(const Pool4 pool, const int64_t* slots, int64_t n, const Rows4 k,
                       const Rows4 v, int vec, int32_t* status) {
   using U = Unit4<D, NG>;
   constexpr int L = D / 8, LG = L / NG, W = U::W;
-  const int64_t row = ((int64_t)blockIdx.x * kRowThreads + threadIdx.x) / L;
-  const int lane = threadIdx.x % L;
-  if (row >= rows) return;
-  const int64_t token = row / pool.hkv;
-  const int head = (int)(row - token * pool.hkv);
+  const Row4 w4 = row_of<L>(pool.hkv);
+  const int64_t token = w4.token;
+  const int head = w4.head, lane = threadIdx.x % L;
+  if (token >= n) return;
   const int64_t slot = slots[token];
   const bool live = pool.valid(slot);
   if (!live && slot != -1 && lane == 0 && head == 0) report(status, CS_ST_SLOT_RANGE);
@@ -188,19 +231,15 @@ __global__ void __launch_bounds__(kRowThreads)
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const Rows4& r = h ? v : k;
-    const float2 sl = pair_of<T>(pair[h]);
-    uint32_t y[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      y[i] = Pack2<T>::pack(fmaf((float)(code[h] >> (8 * i) & 15u), sl.x, sl.y),
-                            fmaf((float)(code[h] >> (8 * i + 4) & 15u), sl.x, sl.y));
+    const uint4 y = decode<T>(code[h], pair[h]);
     char* p = r.x + token * r.st + head * r.sh + lane * 16;
     if (vec) {
-      *reinterpret_cast<uint4*>(p) = make_uint4(y[0], y[1], y[2], y[3]);
+      *reinterpret_cast<uint4*>(p) = y;
     } else {
       uint16_t* e = reinterpret_cast<uint16_t*>(p);
+      const uint32_t z[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) e[2 * i] = (uint16_t)y[i], e[2 * i + 1] = (uint16_t)(y[i] >> 16);
+      for (int i = 0; i < 4; ++i) e[2 * i] = (uint16_t)z[i], e[2 * i + 1] = (uint16_t)(z[i] >> 16);
     }
   }
 }
@@ -218,8 +257,8 @@ int rows_call(bool append, const cs_kv4_pool* pool, const int64_t* slots, int64_
   CS_HOST_CHECK(slots != nullptr && k != nullptr && v != nullptr);
   const Rows4 kr{static_cast<char*>(const_cast<void*>(k)), 2 * kst, 2 * ksh};
   const Rows4 vr{static_cast<char*>(const_cast<void*>(v)), 2 * vst, 2 * vsh};
-  const int64_t rows = n * pool->kv_heads, per = kRowThreads / (pool->head_dim / 8);
-  const int64_t blocks = (rows + per - 1) / per;
+  const int64_t per = kRowThreads / (pool->head_dim / 8);
+  const int64_t blocks = (n + per - 1) / per * pool->kv_heads;
   if (blocks > INT32_MAX) return CS_ERR_TOO_LARGE;
   const Pool4 p = Pool4::make(*pool);
   const int vec = vec_rows(kr) && vec_rows(vr);
@@ -228,10 +267,10 @@ int rows_call(bool append, const cs_kv4_pool* pool, const int64_t* slots, int64_
     constexpr int D = decltype(d)::value, NG = decltype(g)::value;
     if (append)
       kv4_append_kernel<T, D, NG><<<(unsigned)blocks, kRowThreads, 0, as_stream(stream)>>>(
-          p, slots, rows, kr, vr, vec, status);
+          p, slots, n, kr, vr, vec, status);
     else
       kv4_gather_kernel<T, D, NG><<<(unsigned)blocks, kRowThreads, 0, as_stream(stream)>>>(
-          p, slots, rows, kr, vr, vec, status);
+          p, slots, n, kr, vr, vec, status);
     CS_LAUNCH_CHECK();
     return CS_OK;
   });

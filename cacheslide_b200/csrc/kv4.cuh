@@ -33,6 +33,7 @@ struct Pool4 {
   char* base;
   int64_t num_blocks;
   int hkv, bs, units, unit_bytes;
+  int shift;  // log2(bs), -1 when it is no power of two
 
   __host__ static Pool4 make(const cs_kv4_pool& p) {
     Pool4 v;
@@ -41,6 +42,9 @@ struct Pool4 {
     v.hkv = p.kv_heads;
     v.bs = p.block_size;
     v.units = p.block_size / kUnit;
+    v.shift = -1;
+    for (int s = 0; s < 31; ++s)
+      if (1 << s == p.block_size) v.shift = s;
     v.unit_bytes = kUnit * p.head_dim + 8 * kUnit * (p.head_dim / p.group);
     return v;
   }
@@ -52,7 +56,10 @@ struct Pool4 {
   }
   __device__ __forceinline__ Place4 place(int64_t slot) const {
     Place4 p;
-    if (slot < (1ll << 32)) {  // a 64-bit division is about 100 instructions
+    if (shift >= 0) {
+      p.block = slot >> shift;
+      p.row = (int)slot & (bs - 1);
+    } else if (slot < (1ll << 32)) {  // a 64-bit division is about 100 instructions
       const uint32_t b = (uint32_t)slot / (uint32_t)bs;
       p.block = b;
       p.row = (int)((uint32_t)slot - b * (uint32_t)bs);

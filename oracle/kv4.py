@@ -17,9 +17,9 @@ UNIT = 16
 def params(x: torch.Tensor, group: int):
     """Scale and lowest value of each group of 16-bit x, in its type."""
     y = x.float().unflatten(-1, (-1, group))
-    low, high = y.amin(-1), y.amax(-1)
+    low, high = y.amin(-1) + 0.0, y.amax(-1)  # (a zero without a sign)
     # the quotient in float32 (its exact range in float64), then 16 bits
-    scale = ((high.double() - low.double()) / 15).float().to(x.dtype)
+    scale = ((high.double() - low.double()) / 15).abs().float().to(x.dtype)
     top = {torch.float16: 65520.0, torch.bfloat16: 3.3961775292304957e38}[x.dtype]
     over = low.double() + 15 * scale.double() >= top
     down = (scale.view(torch.int16) - 1).view(x.dtype)

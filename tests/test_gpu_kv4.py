@@ -58,7 +58,7 @@ def test_records_bit_for_bit(cuda, dtype, dim, group, n, heads, block):
 def test_ties_constants_extremes_and_tiny_values(cuda, dtype):
     dim, group = 128, 32
     big, tiny = torch.finfo(dtype).max, torch.finfo(dtype).smallest_normal
-    x = torch.zeros(12, 1, dim)
+    x = torch.zeros(14, 1, dim)
     steps = torch.arange(31) * 0.5  # halves of a scale of 1: ties at every odd one
     x[0, 0, :31] = steps
     x[0, 0, 31] = 15
@@ -73,8 +73,10 @@ def test_ties_constants_extremes_and_tiny_values(cuda, dtype):
     x[9, 0, ::32] = big
     x[10, 0] = torch.linspace(0, 1, dim) ** 9
     x[11, 0] = -steps.repeat(5)[:dim] * 0.125
+    x[12, 0] = torch.where(torch.arange(dim) % 3 == 0, -0.0, 0.0)
+    x[13, 0] = torch.where(torch.arange(dim) % 3 == 0, -0.0, 1.0)
     x = x.to(dtype)
-    slots = torch.arange(12)
+    slots = torch.arange(14)
     pool = _pool(cuda, 1, 1, 16, dim, group, dtype)
     want = pool.storage.cpu()
     okv4.write(want, slots, x, x.flip(0), group)
