@@ -237,9 +237,9 @@ struct Share4 {
         if (from < at + c) break;
         at += c;
       }
-      const int n = steps(f.r, a.G, f.tile), rest = (int)(from - at);
-      f.head = rest / n;
-      f.step = rest - f.head * n;
+      const int n = steps(f.r, a.G, f.tile);
+      f.head = (int)((from - at) / n);
+      f.step = (int)(from - at - (int64_t)f.head * n);
       s.found = f;
     }
     __syncthreads();

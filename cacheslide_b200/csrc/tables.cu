@@ -13,7 +13,7 @@
 namespace cs {
 namespace {
 
-constexpr int kMapThreads = 256;
+constexpr int kMapThreads = 256, kKeysEach = 8;
 
 struct Sums {
   int64_t tok, key, need;
@@ -149,34 +149,38 @@ __global__ void __launch_bounds__(kMapThreads) step_maps_kernel(const cs_step_ma
     p.slots[i] = slot;
   }
   if (p.key_slots) {
-    // four keys a thread: one search, and mostly one block
-    for (int64_t i = 4 * first; i < p.keys; i += 4 * step) {
-      int64_t out[4];
+    // kKeysEach keys a thread: one search, and mostly one block
+    for (int64_t i = kKeysEach * first; i < p.keys; i += kKeysEach * step) {
+      int64_t out[kKeysEach], base = -1;  // base: slot of the block's first key
       Located l{0, 0, 0};
       Request q{0, 0, 0, 0};
-      int at_block = -1;
-      int64_t id = -1;
+      int block = 0, offset = 0;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < kKeysEach; ++k) {
         out[k] = -1;
         if (fail || i + k >= all.key) continue;
-        if (l.local >= q.len) {  // the first one, or the next request's
+        const bool search = l.local >= q.len;  // the first one, or the next request's
+        if (search) {
           l = locate(i + k, [](const Sums& s) { return s.key; },
                      [](const Request& r) { return (int64_t)r.len; });
           q = request_of(p, l.request);
-          at_block = -1;
+          block = l.local / p.block_size;
+          offset = l.local - block * p.block_size;
+        } else if (offset == p.block_size) {
+          ++block;
+          offset = 0;
         }
-        const int j = l.local / p.block_size;
-        if (j != at_block) id = block_id(l, q, at_block = j);
-        out[k] = slot_of(id, l.local - j * p.block_size);
+        if (search || offset == 0) base = slot_of(block_id(l, q, block), 0);
+        out[k] = base < 0 ? -1 : base + offset;
         ++l.local;
+        ++offset;
       }
-      if (i + 4 <= p.keys && reinterpret_cast<uintptr_t>(p.key_slots) % 16 == 0) {
+      if (i + kKeysEach <= p.keys && reinterpret_cast<uintptr_t>(p.key_slots) % 16 == 0) {
         longlong2* to = reinterpret_cast<longlong2*>(p.key_slots + i);
-        to[0] = make_longlong2(out[0], out[1]);
-        to[1] = make_longlong2(out[2], out[3]);
+#pragma unroll
+        for (int k = 0; k < kKeysEach / 2; ++k) to[k] = make_longlong2(out[2 * k], out[2 * k + 1]);
       } else {
-        for (int k = 0; k < 4 && i + k < p.keys; ++k) p.key_slots[i + k] = out[k];
+        for (int k = 0; k < kKeysEach && i + k < p.keys; ++k) p.key_slots[i + k] = out[k];
       }
     }
   }
@@ -205,7 +209,7 @@ extern "C" int cs_step_maps(const cs_step_maps_params* p, void* stream) {
   CS_HOST_CHECK(p->key_slots != nullptr || p->keys == 0);
   // blocks that fit the machine at once: each sums up every request (500 requests
   // with 2M keys in all take 41 us with one an SM)
-  const int64_t work = p->tokens + (p->key_slots ? (p->keys + 3) / 4 : 0);
+  const int64_t work = p->tokens + (p->key_slots ? (p->keys + kKeysEach - 1) / kKeysEach : 0);
   const int64_t blocks = (work + kMapThreads - 1) / kMapThreads;
   const int64_t most = 4ll * num_sms();
   step_maps_kernel<<<(unsigned)(blocks < 1 ? 1 : blocks > most ? most : blocks), kMapThreads, 0,
