@@ -18,7 +18,11 @@ drop-in replacement:
   the rotated append into the paged pool, for rotary layers on that pool;
 * ``prefix``    -- ``SharedPrefixAttention``: those layers' attention over the
   pool for a batch that shares a long prefix;
-* ``rotary_rag`` -- ``RotaryRagBatch``: the two together for a retrieval batch.
+* ``rotary_rag`` -- ``RotaryRagBatch``: the two together for a retrieval batch;
+* ``tables``    -- ``step_maps``: block tables and slot maps of a step from
+  lengths on the device;
+* ``kv4``       -- the paged pool in 4 bits: ``append``, ``gather`` and
+  ``attention`` over it.
 
 All device arithmetic is in ``_lib/libcacheslide_sm100.so`` (C ABI declared in
 ``include/cacheslide_b200.h``); build it with ``python -m cacheslide_b200.build``.
