@@ -301,16 +301,16 @@ namespace cs {
 Plan4 plan4(const cs_kv4_attn_params& p) {
   Plan4 plan;
   const int64_t g = p.q_heads / p.pool.kv_heads;
-  // query rows of a KV head an average request has
+  // Query rows of a KV head an average request has.  Up to 32 go to the kernel
+  // for few, in tiles of 16 that each read the keys: 16 requests behind 4096 keys
+  // take 83 us with 24 or 28 rows and 98 in the wide kernel; 116 with 48 rows and
+  // 101 there, 201 with 96 and 111.  (The wide kernel in blocks of 128 rows was no
+  // faster with any of these, and slower with less work.)
   const int64_t rows = p.requests > 0 ? p.tokens * g / p.requests : 0;
-  plan.wide = rows > 16;
-  if (plan.wide) {
-    plan.rows = rows > 128 ? 256 : 128;
-    plan.workers = num_sms() * (plan.rows == 256 ? 1 : 2);
-  } else {
-    plan.rows = rows <= 8 ? 8 : 16;
-    plan.workers = num_sms() * kv4_decode_blocks(plan.rows, p.pool.head_dim, p.pool.group);
-  }
+  plan.wide = rows > 32;
+  plan.rows = plan.wide ? kWideRows : rows <= 8 ? 8 : 16;
+  plan.workers = num_sms() * (plan.wide ? 1 : kv4_decode_blocks(plan.rows, p.pool.head_dim,
+                                                                p.pool.group));
   return plan;
 }
 
@@ -376,6 +376,6 @@ extern "C" int cs_kv4_attn(const cs_kv4_attn_params* p, void* workspace, void* s
   a.zero_rest = p->zero_rest;
   a.flip = p->scale < 0.0 ? 0x80008000u : 0u;
   a.scale2 = fabsf((float)p->scale) * 1.4426950408889634f;
-  return (plan.wide ? kv4_wide : kv4_decode)(a, p->pool, plan.rows, plan.workers,
-                                             as_stream(stream));
+  return plan.wide ? kv4_wide(a, p->pool, plan.workers, as_stream(stream))
+                   : kv4_decode(a, p->pool, plan.rows, plan.workers, as_stream(stream));
 }

@@ -14,7 +14,8 @@ namespace cs {
 int kv4_decode_blocks(int rows, int dim, int group);  // an SM's, with so many rows a block
 int kv4_decode(const Attn4& a, const cs_kv4_pool& pool, int rows, int workers,
                cudaStream_t stream);
-int kv4_wide(const Attn4& a, const cs_kv4_pool& pool, int rows, int workers, cudaStream_t stream);
+constexpr int kWideRows = 256;  // query rows a block of the wide kernel
+int kv4_wide(const Attn4& a, const cs_kv4_pool& pool, int workers, cudaStream_t stream);
 // workers and query rows a block for a call: the workspace's shape
 struct Plan4 {
   int workers, rows;

@@ -1,7 +1,7 @@
 // Tensor-core attention over the 4-bit pool for many query rows a KV head
 // (questions, prompt chunks): tcgen05, TMEM.
 //
-// One block takes a range of the steps of all row tiles (Share4): up to NT
+// One block takes a range of the steps of all row tiles (Share4): up to two
 // tiles of 128 query rows of a (request, KV head) and the keys that they see,
 // 64 a step.  Per step
 //   S = Q K^T (tcgen05, TMEM),  P = 2^(S c - m),  O += P V (P from TMEM)
@@ -36,7 +36,8 @@ namespace cs {
 namespace {
 
 constexpr int kKeys = 64;         // keys of a step
-constexpr int kTileRows = 128;
+constexpr int kTileRows = 128, NT = 2;  // query rows of a tile, row tiles of a block
+static_assert(kTileRows * NT == kWideRows, "the workspace's rows");
 constexpr int kLeastSteps = 4;    // steps a block takes at least
 constexpr float kLazy = 8.f;      // O is rescaled when the maximum grew by more than 2^8
 constexpr float kUp = 7.f;        // P is stored up by 2^7: fp16's normal numbers reach 2^-21
@@ -44,25 +45,24 @@ constexpr int kInfo = 8;          // steps whose scales are kept
 constexpr int kSegments = 4;      // segments the loader may be ahead
 
 // TERMS 2: key and value tiles in two parts (float16 pools)
-template <int D, int NG, int NT, int TERMS>
+template <int D, int NG, int TERMS>
 struct Shape4 {
-  // threads a row in the softmax, as in the wide blocks of the shared-prefix kernel
-  static constexpr int TPR = NT;
+  // threads a row in the softmax: two, as in the wide blocks of the shared-prefix
+  // kernel (chunks of 512 tokens over 4096: 403 us against 431 with one)
+  static constexpr int TPR = 2;
   static constexpr int kTile = kTileRows * TPR;  // softmax threads of a row tile
   // the softmax warps, then a warpgroup of 2 K and 2 V warps, and one of the
   // loader and NT MMA warps
   static constexpr int kSoft = 4 * NT * TPR;
   static constexpr int kThreads = 32 * (kSoft + 8);
   // registers: the launch's share, then the softmax's, the producers', the rest's
-  static constexpr int kLaunchRegs = 80, kSoftRegs = NT == 1 ? 112 : 88,
-                       kMakeRegs = 72, kRestRegs = 56;
+  static constexpr int kLaunchRegs = 80, kSoftRegs = 88, kMakeRegs = 72, kRestRegs = 56;
   static_assert(kSoft * kSoftRegs + 4 * (kMakeRegs + kRestRegs) <= (kSoft + 8) * kLaunchRegs,
                 "more registers than the block is launched with");
   static constexpr uint32_t TB = kKeys * D * 2;  // (a part of) a K or V tile
   static constexpr uint32_t RB = (kKeys / kUnit) * Unit4<D, NG>::kBytes;  // a step's raw units
-  // stages of K and V tiles, and of raw units (two blocks of one row tile share an SM)
-  static constexpr int KS = NT == 1 && TERMS == 2 ? 1 : 2, VS = KS,
-                       RS = NT == 1 ? 1 : TERMS == 2 ? 2 : 3;
+  // stages of K and V tiles, and of raw units
+  static constexpr int KS = 2, VS = 2, RS = TERMS == 2 ? 2 : 3;
   // a query tile's place also takes its output rows, 2 D bytes each and 16 more
   static constexpr uint32_t QB = kTileRows * D * 2 + kTileRows * 16;
   static constexpr uint32_t oQ = 0, oK = NT * QB, oV = oK + KS * TERMS * TB, oR = oV + VS * TERMS * TB,
@@ -77,12 +77,12 @@ struct Shape4 {
                             oAbort = oTmem + 4, oWalked = oAbort + 4, oFlag = oWalked + 4, oScale = oFlag + 4 * kInfo,
                             oPower = oScale + 8 * kInfo, oBad = oPower + 8 * kInfo, oRow = oBad + kInfo * kKeys,
                             oMax = oRow + NT * kTileRows * 4,
-                            oSeg = oMax + (TPR - 1) * NT * 2 * 2 * 128 * 4,
+                            oSeg = oMax + NT * 2 * 2 * 128 * 4,
                             oSums = (oSeg + 48 * kSegments + 7) / 8 * 8,
                             kMeta = oSums + 96;
   static_assert(oR % 1024 == 0 && RB % 128 == 0 && oTmem % 4 == 0 && oRow % 4 == 0, "alignment");
   static constexpr uint32_t kSmem = oMeta + kMeta + 1024;  // the base is rounded up to 1024
-  static_assert(kSmem <= (NT == 1 ? 115712 : 232448), "shared memory");
+  static_assert(kSmem <= 232448, "shared memory");
   static constexpr uint32_t kCols = 256 * NT;
   // two score buffers of 64 columns at 128 i for row tile i, O at cO + D i
   static constexpr uint32_t cS = 0, cO = 128 * NT;
@@ -165,14 +165,14 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[N], const char* p) {
   }
 }
 
-template <typename T, int D, int NG, int NT>
-__global__ void __launch_bounds__(
-    Shape4<D, NG, NT, std::is_same<T, __half>::value ? 2 : 1>::kThreads, NT == 1 ? 2 : 1)
+template <typename T, int D, int NG>
+__global__ void __launch_bounds__(Shape4<D, NG, std::is_same<T, __half>::value ? 2 : 1>::kThreads,
+                                  1)
     kv4_sm100_kernel(const __grid_constant__ Attn4 a) {
   constexpr int TERMS = std::is_same<T, __half>::value ? 2 : 1;
-  using Sh = Shape4<D, NG, NT, TERMS>;
+  using Sh = Shape4<D, NG, TERMS>;
   using U = Unit4<D, NG>;
-  constexpr int RT = kTileRows * NT, W = U::W, WG = W / NG, KS = Sh::KS, RS = Sh::RS;
+  constexpr int RT = kWideRows, W = U::W, WG = W / NG, KS = Sh::KS, RS = Sh::RS;
   using Share = Share4<RT, kKeys>;
   extern __shared__ char smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(
   // no phase from the last but one): the first tile's MMA warp, which walks every
   // step, says how many have their tiles.
   auto caught_up = [&](int qt, int n) {
-    if (NT == 1 || qt == 0 || *walked >= n) return true;
+    if (qt == 0 || *walked >= n) return true;
     const long long t0 = clock64();
     while (*walked < n) {
       if (*abort) return false;
@@ -269,8 +269,7 @@ __global__ void __launch_bounds__(
 
   if (warp >= Sh::kSoft && warp < Sh::kSoft + 4) {
     // ============================================= producers: K, then V pair
-    if constexpr (Sh::kMakeRegs > Sh::kLaunchRegs) regs_up<Sh::kMakeRegs>();
-    else regs_down<Sh::kMakeRegs>();
+    regs_down<Sh::kMakeRegs>();
     const bool isv = warp >= Sh::kSoft + 2;
     // a warp makes 32 keys' rows, with a power of two of their own; this thread's
     // part of every eight is the W words from word W c on of row r
@@ -345,7 +344,7 @@ __global__ void __launch_bounds__(
           const int u = n - stages, u1 = second[u & 1];
           const uint32_t bar = isv ? Sh::bPV : Sh::bS;
           if (!warp_wait(at(bar, 0, u), (u >> 1) & 1, abort) ||
-              (u1 >= 0 && !warp_wait(at(bar, NT - 1, u1), (u1 >> 1) & 1, abort)))
+              (u1 >= 0 && !warp_wait(at(bar, 1, u1), (u1 >> 1) & 1, abort)))
             return false;
         }
         second[n & 1] = two ? n1++ : -1;
@@ -581,10 +580,11 @@ __global__ void __launch_bounds__(
     // ================================================================= softmax
     regs_up<Sh::kSoftRegs>();
     int n = 0, m = 0, queries = 0;  // steps of the block and of the row tile; its segments
-    [[maybe_unused]] int exchanges = 0;  // of maxima with the row's other thread
+    int exchanges = 0;  // of maxima with the row's other thread
     segments([&](const Segment& seg) {
       const int row0 = seg.row0, steps = seg.steps, s0 = seg.s0;
       constexpr int TPR = Sh::TPR, VC = kKeys / TPR;  // scores of a step a thread holds
+      static_assert(VC == 32, "the keys of one power of two");
       const int qt = warp / (4 * TPR), part2 = (warp >> 2) % TPR;
       if (qt >= seg.tiles) {
         n += steps;
@@ -653,8 +653,8 @@ __global__ void __launch_bounds__(
       const uint32_t oc = tmem + lane_base + Sh::cO + D * qt;
       float mref = -INFINITY, lsum = 0.f;  // log2 domain; P = 2^(x + E - mref + up)
       uint32_t poison = 0u;  // groups of values that are not finite and that the row sees
-      [[maybe_unused]] const uint32_t pair = mb + Sh::bMax + 8 * (4 * qt + (warp & 3));
-      [[maybe_unused]] float* row_max = reinterpret_cast<float*>(meta + Sh::oMax) + qt * 512;
+      const uint32_t pair = mb + Sh::bMax + 8 * (4 * qt + (warp & 3));
+      float* row_max = reinterpret_cast<float*>(meta + Sh::oMax) + qt * 512;
       const bool any_row = __any_sync(~0u, row_ok);
       auto wait_pv = [&](int t) {
         ok = warp_wait(at(Sh::bPV, qt, m + t), ((m + t) >> 1) & 1, abort);
@@ -675,31 +675,20 @@ __global__ void __launch_bounds__(
         if (!any_row || __all_sync(~0u, vhi <= 0)) {  // nothing to see for these 32 rows
 #pragma unroll
           for (int c = 0; c < 16; ++c) v[c] = 0u;
-#pragma unroll
-          for (int cc = 0; cc < VC / 32; ++cc) CS_TMEM_ST16(sc + 16 * (part2 + cc), v);
+          CS_TMEM_ST16(sc + 16 * part2, v);
           tmem_wait_st();
           tc_fence_before();
           mbar_arrive(at(Sh::bP, qt, m + t));
           continue;
         }
         CS_TMEM_LD32(sc + 32 * part2, v);
-        if constexpr (TPR == 1) CS_TMEM_LD32(sc + 32, (v + 32));
-        // of this thread's 32 keys (one of two such sets, where it holds the row)
-        float power[VC / 32], factor[VC / 32];
-#pragma unroll
-        for (int cc = 0; cc < VC / 32; ++cc) {
-          power[cc] = val_power[2 * info + part2 + cc];
-          factor[cc] = fmaxf(row_factor * key_scale[2 * info + part2 + cc], 1e-30f);
-        }
+        const float power = val_power[2 * info + part2];
+        const float factor = fmaxf(row_factor * key_scale[2 * info + part2], 1e-30f);
         tmem_wait_ld();
         if (!__all_sync(~0u, vhi >= kKeys)) {
+          const uint32_t bits = col_bits(0, vhi, 32 * part2);
 #pragma unroll
-          for (int cc = 0; cc < VC / 32; ++cc) {
-            const uint32_t bits = col_bits(0, vhi, 32 * (part2 + cc));
-#pragma unroll
-            for (int c = 0; c < 32; ++c)
-              v[32 * cc + c] = (bits >> c) & 1u ? v[32 * cc + c] : 0xff800000u;  // -inf
-          }
+          for (int c = 0; c < 32; ++c) v[c] = (bits >> c) & 1u ? v[c] : 0xff800000u;  // -inf
         }
         if (flag[info] == n + t) {
           for (int c = 0; c < VC; ++c) {
@@ -707,35 +696,30 @@ __global__ void __launch_bounds__(
             if (key < vhi) poison |= bad[info * kKeys + key];
           }
         }
-        float top = -INFINITY;  // of log2 of the weights, with the values' power
-#pragma unroll
-        for (int cc = 0; cc < VC / 32; ++cc) {
+        float top;  // of log2 of the weights, with the values' power
+        {
           float m4[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            m4[k] = max_nan(__uint_as_float(v[32 * cc + k]), __uint_as_float(v[32 * cc + k + 4]));
+            m4[k] = max_nan(__uint_as_float(v[k]), __uint_as_float(v[k + 4]));
 #pragma unroll
           for (int c = 8; c < 32; c += 8) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              m4[k] = max3_nan(m4[k], __uint_as_float(v[32 * cc + c + k]),
-                               __uint_as_float(v[32 * cc + c + k + 4]));
+              m4[k] = max3_nan(m4[k], __uint_as_float(v[c + k]), __uint_as_float(v[c + k + 4]));
           }
-          top = max_nan(top, fmaf(max_nan(max3_nan(m4[0], m4[1], m4[2]), m4[3]), factor[cc],
-                                  power[cc]));
+          top = fmaf(max_nan(max3_nan(m4[0], m4[1], m4[2]), m4[3]), factor, power);
         }
         // the row's maximum from both its threads; past this barrier both have
         // read their scores, so P may take their columns
-        if constexpr (TPR == 2) {
-          float* mx = row_max + (exchanges & 1) * 256;
-          mx[part2 * 128 + r] = top;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(pair);
-          ok = warp_wait(pair, exchanges & 1, abort);
-          if (!ok) break;
-          ++exchanges;
-          top = max_nan(top, mx[(1 - part2) * 128 + r]);
-        }
+        float* mx = row_max + (exchanges & 1) * 256;
+        mx[part2 * 128 + r] = top;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(pair);
+        ok = warp_wait(pair, exchanges & 1, abort);
+        if (!ok) break;
+        ++exchanges;
+        top = max_nan(top, mx[(1 - part2) * 128 + r]);
         if (!(top < INFINITY)) {  // a NaN or +inf score makes the row NaN
           lsum = __int_as_float(0x7fffffff);
           top = -INFINITY;
@@ -759,11 +743,11 @@ __global__ void __launch_bounds__(
           tmem_wait_st();
         }
         if (grow) mref = top;
-        const float ref = (mref > -INFINITY ? mref : 0.f) - kUp;
+        const float less = power - ((mref > -INFINITY ? mref : 0.f) - kUp);
+        const float2 scale = make_float2(factor, factor), off = make_float2(less, less);
+        float2 p0 = make_float2(0.f, 0.f), p1 = p0;
 #pragma unroll
         for (int c = 0; c < VC; c += 2) {
-          const float2 scale = make_float2(factor[c / 32], factor[c / 32]),
-                       off = make_float2(power[c / 32] - ref, power[c / 32] - ref);
           const float2 x = __ffma2_rn(
               make_float2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale, off);
           v[c] = __float_as_uint(x.x);
@@ -772,20 +756,15 @@ __global__ void __launch_bounds__(
 #pragma unroll
         for (int c = 0; c < VC; ++c) v[c] = __float_as_uint(ex2(__uint_as_float(v[c])));
 #pragma unroll
-        for (int cc = 0; cc < VC / 32; ++cc) {
-          float2 p0 = make_float2(0.f, 0.f), p1 = p0;
-#pragma unroll
-          for (int c = 32 * cc; c < 32 * cc + 32; c += 4) {
-            p0 = __fadd2_rn(p0, make_float2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])));
-            p1 = __fadd2_rn(p1, make_float2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])));
-          }
-          lsum = fmaf((p0.x + p0.y) + (p1.x + p1.y), ex2(-power[cc]), lsum);
+        for (int c = 0; c < VC; c += 4) {
+          p0 = __fadd2_rn(p0, make_float2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])));
+          p1 = __fadd2_rn(p1, make_float2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])));
         }
+        lsum = fmaf((p0.x + p0.y) + (p1.x + p1.y), ex2(-power), lsum);
 #pragma unroll
         for (int c = 0; c < VC / 2; ++c)
           v[c] = Pack2<__half>::pack(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1]));
-#pragma unroll
-        for (int cc = 0; cc < VC / 32; ++cc) CS_TMEM_ST16(sc + 16 * (part2 + cc), (v + 16 * cc));
+        CS_TMEM_ST16(sc + 16 * part2, v);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(at(Sh::bP, qt, m + t));
@@ -793,19 +772,18 @@ __global__ void __launch_bounds__(
 
       // -------------------------------------------------------------- output
       if (ok && steps > 0) wait_pv(steps - 1);
-      if constexpr (TPR == 2) {  // the row's sum and bad groups from both its threads
+      // the row's sum and bad groups from both its threads
 #pragma unroll
-        for (int turn = 0; turn < 2; ++turn) {
-          float* both = row_max + (exchanges & 1) * 256;
-          both[part2 * 128 + r] = turn ? __uint_as_float(poison) : lsum;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(pair);
-          ok = ok && warp_wait(pair, exchanges & 1, abort);
-          ++exchanges;
-          const float other = both[(1 - part2) * 128 + r];
-          if (turn) poison |= __float_as_uint(other);
-          else lsum += other;
-        }
+      for (int turn = 0; turn < 2; ++turn) {
+        float* both = row_max + (exchanges & 1) * 256;
+        both[part2 * 128 + r] = turn ? __uint_as_float(poison) : lsum;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(pair);
+        ok = ok && warp_wait(pair, exchanges & 1, abort);
+        ++exchanges;
+        const float other = both[(1 - part2) * 128 + r];
+        if (turn) poison |= __float_as_uint(other);
+        else lsum += other;
       }
       const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
       const float lse2 =
@@ -935,25 +913,23 @@ bool launched_with(int regs) {
   return have == regs;
 }
 
-template <typename T, int D, int NG, int NT>
+template <typename T, int D, int NG>
 int launch_wide(const Attn4& a, int workers, cudaStream_t stream) {
-  using Sh = Shape4<D, NG, NT, std::is_same<T, __half>::value ? 2 : 1>;
-  constexpr auto kernel = kv4_sm100_kernel<T, D, NG, NT>;
+  using Sh = Shape4<D, NG, std::is_same<T, __half>::value ? 2 : 1>;
+  constexpr auto kernel = kv4_sm100_kernel<T, D, NG>;
   if (!allow_smem<kernel>(Sh::kSmem) || !launched_with<kernel>(Sh::kLaunchRegs))
     return CS_ERR_CUDA;
   if (const int rc = launch_dependent(kernel, dim3(workers), Sh::kThreads, Sh::kSmem, stream, a))
     return rc;
-  return launch_join<T, D, kTileRows * NT>(a, workers, stream);
+  return launch_join<T, D, kWideRows>(a, workers, stream);
 }
 
 }  // namespace
 
-int kv4_wide(const Attn4& a, const cs_kv4_pool& pool, int rows, int workers, cudaStream_t stream) {
+int kv4_wide(const Attn4& a, const cs_kv4_pool& pool, int workers, cudaStream_t stream) {
   return by_pool4(pool, [&](auto* t, auto d, auto g) -> int {
     using T = std::remove_pointer_t<decltype(t)>;
-    constexpr int D = decltype(d)::value, NG = decltype(g)::value;
-    return rows > kTileRows ? launch_wide<T, D, NG, 2>(a, workers, stream)
-                            : launch_wide<T, D, NG, 1>(a, workers, stream);
+    return launch_wide<T, decltype(d)::value, decltype(g)::value>(a, workers, stream);
   });
 }
 

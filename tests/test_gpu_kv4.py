@@ -152,7 +152,7 @@ def _batch(cuda, seed, new, lengths, hq, hk, dim, group, block, dtype, spare=2, 
 
 def _wide(new, heads):
     """Whether the kernel for many query rows a KV head takes such a batch."""
-    return len(new) > 0 and sum(new) * heads // len(new) > 16
+    return len(new) > 0 and sum(new) * heads // len(new) > 32
 
 
 def _check(got, lse, pool, table, q, starts, lengths, scale, wide, rows=None):
@@ -199,7 +199,7 @@ def test_decode(cuda, dtype, dim, group, hq, hk):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("new", [2, 3, 4, 7])
+@pytest.mark.parametrize("new", [2, 3, 4, 7, 9, 20])
 def test_drafts(cuda, dtype, new):
     _run(cuda, [new] * 6, [new, new + 1, 30, 64, 129, 700], 8, 2, 128, 64, 16, dtype)
 
