@@ -67,7 +67,8 @@ def step_maps(lengths: Tensor, new: Tensor, tables: Tensor, block_size: int, num
     the same inputs does the same again.  Without them the tables are complete.
 
     All or nothing: a negative length, ``new > lengths``, too narrow a table,
-    more rows than ``tokens`` (or keys than ``keys``) or too few free blocks
+    more rows than ``tokens`` (or keys than ``keys``), too few free blocks or a
+    ``free_count`` that is negative or past ``free``
     sets ``ST_CAPACITY`` in ``status``, and then every slot is -1, every
     position and start 0 and the tables are left alone.  A block outside the
     pool gives slot -1 and sets ``ST_SLOT_RANGE``.  Nothing waits on the host."""
@@ -91,7 +92,7 @@ def step_maps(lengths: Tensor, new: Tensor, tables: Tensor, block_size: int, num
     if free is not None:
         p_free = _vector("free", free, None, device)
         p_count = _vector("free_count", free_count, 1, device)
-        if free.shape[0] == 0:  # an empty tensor has no address
+        if free.shape[0] == 0:  # an empty tensor has no address, and is not read
             p_free = p_count
     status_ptr = N.status_ptr(status, device)
     if device < 0:
@@ -107,7 +108,7 @@ def step_maps(lengths: Tensor, new: Tensor, tables: Tensor, block_size: int, num
         key_starts = torch.empty(requests + 1, dtype=torch.int64, device=on)
     p = N.StepMapsParams(
         p_lengths, p_new, requests, block_size, num_blocks, tables.data_ptr(), tables.stride(0),
-        width, offset, p_free, p_count, N.ptr(left), tokens, keys, starts.data_ptr(),
+        width, offset, p_free, p_count, N.ptr(left), 0 if free is None else free.shape[0], tokens, keys, starts.data_ptr(),
         positions.data_ptr(), slots.data_ptr(), N.ptr(key_starts), N.ptr(key_slots), status_ptr)
     N.launch("cs_step_maps", on, p)
     return StepMaps(starts, positions, slots, key_starts, key_slots, left)

@@ -800,6 +800,7 @@ typedef struct {
   const int32_t* free_blocks; /* or NULL */
   const int32_t* free_count;  /* [1] */
   int32_t* free_left;         /* [1], not free_count */
+  int64_t free_size;          /* places of free_blocks; a count past it sets CS_ST_CAPACITY */
   int64_t tokens, keys;       /* places in the arrays below */
   int32_t* starts;            /* [requests + 1] */
   int64_t* positions;         /* [tokens] */

@@ -470,6 +470,28 @@ def test_streams_and_graphs(cuda):
         assert torch.equal(s["pool"].storage, eager["pool"].storage)
 
 
+def test_calls_at_once_on_several_streams(cuda):
+    """Few and many rows side by side over one pool: each call has its own
+    workspace."""
+    cases = []
+    for seed, new in ((1, [1] * 9), (2, [70, 3, 200]), (3, [4] * 5), (4, [90] * 4)):
+        lengths = [n + 300 * (b + 1) for b, n in enumerate(new)]
+        pool, table, q, starts = _batch(cuda, seed, new, lengths, 8, 2, 128, 64, 16,
+                                        torch.bfloat16)
+        args = (q.to(cuda), pool, table.to(cuda),
+                torch.tensor(lengths, dtype=torch.int32, device=cuda), starts.to(cuda))
+        cases.append((args, kv4.attention(*args), torch.cuda.Stream(cuda)))
+    torch.cuda.synchronize()
+    out = []
+    for i in range(10):
+        for args, _, stream in cases:
+            with torch.cuda.stream(stream):
+                out.append(kv4.attention(*args))
+    torch.cuda.synchronize()
+    for i, got in enumerate(out):
+        assert torch.equal(got, cases[i % 4][1]), i
+
+
 def test_refusals(cuda):
     pool, table, q, starts = _batch(cuda, 1, [2, 2], [20, 30], 4, 2, 128, 64, 16, torch.bfloat16)
     table, q, starts = table.to(cuda), q.to(cuda), starts.to(cuda)

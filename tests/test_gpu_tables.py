@@ -72,7 +72,8 @@ def test_slots_pass_32_bits(cuda):
     assert m.slots.tolist() == want == m.key_slots.tolist()
 
 
-@pytest.mark.parametrize("change", ["negative", "more new", "narrow", "rows", "keys", "free"])
+@pytest.mark.parametrize("change", ["negative", "more new", "narrow", "rows", "keys", "free",
+                                    "count past the stack", "negative count"])
 def test_all_or_nothing(cuda, change):
     lengths, new, tables, free, blocks = _batch(11, 40, 16, 9, 300)
     tokens, keys, count = sum(new), sum(lengths), len(free)
@@ -88,6 +89,12 @@ def test_all_or_nothing(cuda, change):
         tokens -= 1
     elif change == "keys":
         keys -= 1
+    elif change == "count past the stack":
+        count += 1
+    elif change == "negative count":
+        count = -1
+        new, lengths = [0] * 40, [16] * 40
+        keys = 640
     else:
         need = sum(-(-a // 16) - -(-(a - n) // 16) for a, n in zip(lengths, new))
         count = need - 1
