@@ -470,6 +470,29 @@ def test_streams_and_graphs(cuda):
         assert torch.equal(s["pool"].storage, eager["pool"].storage)
 
 
+@pytest.mark.parametrize("new", [1, 50])
+def test_byte_offsets_past_32_bits(cuda, new):
+    pool, table, q, starts = _batch(cuda, 13, [new] * 2, [400, 555], 4, 1, 128, 128, 16,
+                                    torch.bfloat16)
+    lengths = torch.tensor([400, 555], dtype=torch.int32, device=cuda)
+    args = (lengths, starts.to(cuda))
+    want = kv4.attention(q.to(cuda), pool, table.to(cuda), *args)
+    blocks = (1 << 32) // pool.storage[0].numel() + 200_000  # 4.7 GB
+    far = kv4.PagedKV4(torch.empty((blocks, *pool.storage.shape[1:]), dtype=torch.uint8,
+                                   device=cuda), 128, torch.bfloat16, 128)
+    shift = blocks - pool.num_blocks
+    slots = torch.arange(pool.num_blocks * 16, device=cuda)
+    k, v = kv4.gather(pool, slots)
+    far.storage[shift:] = pool.storage
+    for a, b in zip(kv4.gather(far, slots + 16 * shift), (k, v)):
+        assert torch.equal(a, b)
+    got = kv4.attention(q.to(cuda), far, (table + shift).to(cuda), *args)
+    assert torch.equal(got, want)
+    kv4.append(pool, slots, k, v)
+    kv4.append(far, slots + 16 * shift, k, v)
+    assert torch.equal(far.storage[shift:], pool.storage)
+
+
 def test_calls_at_once_on_several_streams(cuda):
     """Few and many rows side by side over one pool: each call has its own
     workspace."""
