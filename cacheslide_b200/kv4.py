@@ -118,7 +118,8 @@ def append(pool: PagedKV4, slots: Tensor, key: Tensor, value: Tensor, *,
         value = value.contiguous()
         vs = value.stride()
     status_ptr = N.status_ptr(status, device)
-    N.require_cuda(pool.storage)
+    if device < 0:
+        N.require_cuda(pool.storage)
     N.launch("cs_kv4_append", pool.device, pool.view, slots.data_ptr(), n, key.data_ptr(), ks[0],
              ks[1], value.data_ptr(), vs[0], vs[1], status_ptr)
 
@@ -132,7 +133,8 @@ def gather(pool: PagedKV4, slots: Tensor, *,
     device = _pool(pool)
     n = _slots(slots, pool)
     status_ptr = N.status_ptr(status, device)
-    N.require_cuda(pool.storage)
+    if device < 0:
+        N.require_cuda(pool.storage)
     key, value = torch.empty(2, n, pool.kv_heads, pool.head_dim, dtype=pool.dtype,
                              device=pool.device).unbind(0)
     st = key.stride()
@@ -209,7 +211,8 @@ def attention(query: Tensor, pool: PagedKV4, tables: Tensor, lengths: Tensor,
         raise ValueError("out must match query, with a contiguous last dimension")
     elif tokens and _overlap(out, query):  # blocks read queries after others have written
         query = query.clone(memory_format=torch.contiguous_format)
-    N.require_cuda(pool.storage)
+    if device < 0:
+        N.require_cuda(pool.storage)
     lse = None
     if return_lse:
         lse = torch.empty(shape[:2], dtype=torch.float32, device=pool.device)
