@@ -59,20 +59,6 @@ template <typename T> __device__ __forceinline__ float of_bits(uint32_t b) {
   return pair_of<T>(b & 0xffffu).x;
 }
 
-template <typename T> struct Pair16;
-template <> struct Pair16<__half> {
-  using type = __half2;
-};
-template <> struct Pair16<__nv_bfloat16> {
-  using type = __nv_bfloat162;
-};
-template <typename T> using pair16 = typename Pair16<T>::type;
-template <typename T> __device__ __forceinline__ pair16<T> as_pair(uint32_t x) {
-  return *reinterpret_cast<pair16<T>*>(&x);
-}
-template <typename P> __device__ __forceinline__ uint32_t pair_bits(P x) {
-  return *reinterpret_cast<uint32_t*>(&x);
-}
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
 // eight elements' codes (element i in bits 4 i ..) and their group's (scale, low)

@@ -113,6 +113,22 @@ template <> __device__ __forceinline__ float2 pair_of<__nv_bfloat16>(uint32_t x)
   return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
 }
 
+// ... and as such a pair
+template <typename T> struct Pair16;
+template <> struct Pair16<__half> {
+  using type = __half2;
+};
+template <> struct Pair16<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+};
+template <typename T> using pair16 = typename Pair16<T>::type;
+template <typename T> __device__ __forceinline__ pair16<T> as_pair(uint32_t x) {
+  return *reinterpret_cast<pair16<T>*>(&x);
+}
+template <typename P> __device__ __forceinline__ uint32_t pair_bits(P x) {
+  return *reinterpret_cast<uint32_t*>(&x);
+}
+
 // ------------------------------------------------------------- attention
 struct Attn4 {
   Pool4 pool;

@@ -104,6 +104,9 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ A
   const int row0 = j.y * RT, h = j.z >> 1;
   const int rows = min(min(RT, r.n * a.G - row0), (int)(blockIdx.y + 1) * kJoinRows<RT>);
   auto place = [&](int i) { return i == 0 ? 2ll * first + (j.z & 1) : 2ll * (first + i); };
+  // the weights are down by a power of two that keeps their sum below 1, and so
+  // that of the parts within float32
+  const float back = __int_as_float((127 + 32 - __clz(parts)) << 23), down = 1.f / back;
   for (int row = blockIdx.y * kJoinRows<RT> + (threadIdx.x >> 5); row < rows; row += 4) {
     float top = -INFINITY, sum = 0.f, o[E];
     for (int i = lane; i < parts; i += 32)
@@ -114,7 +117,7 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ A
     for (int i0 = 0; i0 < parts; i0 += 32) {
       const float l = i0 + lane < parts ? a.part_lse[place(i0 + lane) * RT + row] : -INFINITY;
       // one below 2^-126 of the largest is that, not 0: what is not finite stays
-      const float f = l == -INFINITY ? 0.f : max_nan(ex2(l - top), 0x1p-126f);
+      const float f = l == -INFINITY ? 0.f : down * max_nan(ex2(l - top), 0x1p-126f);
       sum += warp_sum(f);
       const int m = min(32, parts - i0);
 #pragma unroll 1
@@ -143,7 +146,7 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ A
 #pragma unroll
     for (int e = 0; e < E; ++e) out[lane * E + e] = Elem<T>::from_f(o[e] * inv);
     if (lane == 0)
-      write_lse(a, r.start, row0 + row, h, sum == 0.f ? -INFINITY : top + log2f(sum));
+      write_lse(a, r.start, row0 + row, h, sum == 0.f ? -INFINITY : top + log2f(sum * back));
   }
 }
 

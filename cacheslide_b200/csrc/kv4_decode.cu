@@ -42,6 +42,12 @@ constexpr int kLeast = 1;              // steps a block takes at least
 constexpr float kUp = 6.f;  // a new largest p scale is 2^6: fp16's normal numbers reach 2^-20 of it
 constexpr float kTooLarge = 0x1p14f;  // it may grow to 2^14 before O is rescaled
 constexpr float kLowest = -3e38f;     // below every score, and finite
+// What a key may add goes by its largest scale, 2^-40 of its largest lowest value
+// (constant groups have no scale: p low then stays below 2^54) and at least
+// 2^-80, so that the sums of p stay below 2^125 over 2^31 keys of zeros.  Above
+// 2^116 the reference stops rising: p scale is at most 2^16 there, and p at least
+// 2^-110 for a row's largest score, 2^-16 of which float32 still holds.
+constexpr float kLowCounts = 0x1p-40f, kLeastMost = 0x1p-80f, kMostLog = 116.f;
 
 // Blocks an SM holds, as the registers allow without spilling in the loop over
 // the keys: 32 decodes of up to 16K keys in four groups take 102 us with three
@@ -107,6 +113,12 @@ __device__ __forceinline__ void arrive_expect(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ float lg2(float x) {
   float y;
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// the largest that is a number
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
 // a pair of codes (of 16 times codes: 128) less 8, as numbers of 2^-24
@@ -407,9 +419,12 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
         for (int c = 0; c < 2; ++c) {
           uint32_t v[NG];
           Words<NG>::load(v, stage + e * U::kBytes + U::oVp + 4 * NG * (g + 8 * c));
-          most[e][c] = 0.f;
+          // |scale| and |low|, the largest of the groups' (NaN: the others')
+          pair16<T> ends = __habs2(as_pair<T>(v[0]));
 #pragma unroll
-          for (int k = 0; k < NG; ++k) most[e][c] = fmaxf(most[e][c], pair_of<T>(v[k]).x);
+          for (int k = 1; k < NG; ++k) ends = __hmax2(ends, __habs2(as_pair<T>(v[k])));
+          const float2 end = pair_of<T>(pair_bits(ends));
+          most[e][c] = max3(end.x, end.y * kLowCounts, kLeastMost);
           if (some_hidden) {
 #pragma unroll
             for (int k = 0; k < NG; ++k) {
@@ -440,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
           float y = fmaxf(p[e][0][c].x, p[e][0][c].y);
 #pragma unroll
           for (int nt = 1; nt < NT; ++nt) y = fmaxf(y, fmaxf(p[e][nt][c].x, p[e][nt][c].y));
-          top = fmaxf(top, y * fmaxf(most[e][c], kTooLarge * 0x1p-110f));
+          top = fmaxf(top, y * most[e][c]);
         }
       }
       if (__any_sync(~0u, top > kTooLarge)) {
@@ -451,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
           for (int e = 0; e < E; ++e) {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              const float l = fminf(fmaxf(lg2(most[e][c]), -100.f), 100.f) - kUp;
+              const float l = fminf(lg2(most[e][c]), kMostLog) - kUp;
               ma = fmaxf(ma, fmaf(x[e][nt][c].x, qm[nt].x, l));
               mb = fmaxf(mb, fmaf(x[e][nt][c].y, qm[nt].y, l));
             }
@@ -461,12 +476,16 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
             m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
             m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
             m = fmaxf(m, old);
-            const float f = m == old ? 1.f : ex2(old - m);
+            const float f = m == old ? 1.f : ex2(0.5f * (old - m));
             old = m;
             return f;
           };
-          const float2 down = make_float2(raise(ref[nt].x, ma), raise(ref[nt].y, mb));
-          lsum[nt] = __fmul2_rn(lsum[nt], down);
+          // The root, since the reference may rise by more than float32's range
+          // (zero values, then large ones); the sums of p, which were as much
+          // larger, keep theirs.
+          const float2 half = make_float2(raise(ref[nt].x, ma), raise(ref[nt].y, mb));
+          const float2 down = __fmul2_rn(half, half);
+          lsum[nt] = __fmul2_rn(__fmul2_rn(lsum[nt], half), half);
 #pragma unroll
           for (int w = 0; w < NG; ++w) lows[nt][w] = __fmul2_rn(lows[nt][w], down);
 #pragma unroll
@@ -595,7 +614,8 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float m = maxima[w * RT + row];
-        l += sums[w * RT + row] * (m == top ? 1.f : ex2(m - top));
+        const float half = m == top ? 1.f : ex2(0.5f * (m - top));
+        l += sums[w * RT + row] * half * half;
         const float4 z = *reinterpret_cast<const float4*>(outs + (w * RT + row) * D + c);
         y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
       }

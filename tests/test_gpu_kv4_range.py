@@ -1,0 +1,81 @@
+"""Attention over the 4-bit pool with values of all sizes that its records can
+hold: constants, the ends of the types, sizes far apart in one context."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from cacheslide_b200 import _native as N
+from cacheslide_b200 import kv4
+from test_gpu_kv4 import _check, _pool, _rows, _wide
+
+pytestmark = pytest.mark.gpu
+
+
+def _filled(cuda, seed, new, lengths, hq, hk, dim, group, dtype, values, keys=None):
+    """A pool in order, `values` [slot, head, dim] (or a number for all), random
+    keys (or `keys`), and queries."""
+    g = torch.Generator().manual_seed(seed)
+    per = [-(-n // 16) for n in lengths]
+    blocks, width = sum(per), max(per)
+    table, at = torch.full((len(new), width), -3, dtype=torch.int32), 0
+    for b, n in enumerate(per):
+        table[b, :n] = torch.arange(at, at + n)
+        at += n
+    pool = _pool(cuda, blocks, hk, 16, dim, group, dtype)
+    n = 16 * blocks
+    k = _rows(seed, n, hk, dim, dtype) if keys is None else keys
+    v = values if isinstance(values, torch.Tensor) else torch.full((n, hk, dim), values)
+    kv4.append(pool, torch.arange(n, device=cuda), k.to(cuda), v.to(dtype).to(cuda))
+    q = (0.5 * torch.randn(sum(new), hq, dim, generator=g)).to(dtype)
+    return pool, table, q, torch.tensor([0, *new]).cumsum(0).int()
+
+
+def _attend(cuda, pool, table, q, starts, lengths, scale=None):
+    status = N.Status(cuda)
+    got = kv4.attention(q.to(cuda), pool, table.to(cuda),
+                        torch.tensor(lengths, dtype=torch.int32, device=cuda), starts.to(cuda),
+                        scale=scale, return_lse=True, status=status)
+    assert status.read() == 0
+    return got
+
+
+CONSTANTS = [(torch.float16, 60000.0), (torch.float16, -1000.0), (torch.float16, 6e-8),
+             (torch.bfloat16, 1e7), (torch.bfloat16, 2.0 ** 22), (torch.bfloat16, -3e38),
+             (torch.bfloat16, 1e-38), (torch.bfloat16, 1.0), (torch.float16, 0.0)]
+
+
+@pytest.mark.parametrize("dtype,value", CONSTANTS)
+@pytest.mark.parametrize("dim,group", [(128, 32), (64, 64)])
+@pytest.mark.parametrize("new", [1, 3])
+def test_constant_values_come_back(cuda, dtype, value, dim, group, new):
+    """Every group of every value is one number, whose scale is 0: any weights
+    give that number, to float32's rounding (256 additions a thread at most, 2^-16
+    of it), which the output's rounding takes away."""
+    lengths = [max(new, n) for n in (1, 17, 1024, 8192, 30000)]
+    pool, table, q, starts = _filled(cuda, 3, [new] * 5, lengths, 8, 2, dim, group, dtype, value)
+    got, lse = _attend(cuda, pool, table, q, starts, lengths)
+    want = torch.tensor(value, dtype=dtype, device=cuda)
+    assert torch.equal(got, want.expand_as(got)) and torch.isfinite(lse).all()
+
+
+SPANS = [[0.0, 1e7], [0.0, 1e20], [1e7, 0.0], [1e-30, 1e20], [1e30, 1e-20, 1.0], [1e-35, 1e38],
+         [1e38, 1e-35], [1e38, 1e-6, 0.0, 1e-30], [1.0, 1e-12], [1e-20], [1e35], [1e37, 1e34]]
+
+
+@pytest.mark.parametrize("sizes", SPANS)
+@pytest.mark.parametrize("new", [1, 4])
+@pytest.mark.parametrize("few", [False, True])
+def test_sizes_far_apart_in_one_context(cuda, sizes, new, few):
+    """Runs of keys whose values differ by many powers of two, in either order:
+    each keeps its weight in the softmax denominator."""
+    dtype = torch.bfloat16
+    lengths = [3 * 256, 97, 64] if few else [40, 640, 4096]
+    lengths = [max(new, n) for n in lengths]
+    n = 16 * sum(-(-a // 16) for a in lengths)
+    size = torch.tensor(sizes, dtype=torch.float64)[torch.arange(n) // 32 % len(sizes)]
+    v = (_rows(8, n, 2, 128, torch.float32).double().clamp(-2.5, 2.5) * size[:, None, None])
+    pool, table, q, starts = _filled(cuda, 5, [new] * 3, lengths, 8, 2, 128, 64, dtype, v.float())
+    got, lse = _attend(cuda, pool, table, q, starts, lengths)
+    _check(got, lse, pool, table, q, starts, lengths, 128 ** -0.5, _wide([new] * 3, 4))
