@@ -328,7 +328,10 @@ __global__ void __launch_bounds__(Shape4<D, NG, std::is_same<T, __half>::value ?
               else wrong |= 1u << (NG * j + k);
             }
           }
-          if constexpr (TERMS == 2) return 0;
+          // scale (code - zero), scale rounded to 7 bits, reaches 1.08 of this at
+          // most, so two parts hold any number below 2^15; the keys (values) of a
+          // warp that have larger ones are halved
+          if constexpr (TERMS == 2) return __any_sync(~0u, reach >= 0x1p15f) ? 1 : 0;
           const uint32_t m = __reduce_max_sync(~0u, __float_as_uint(reach));
           return m == 0u ? 0 : min(114, max(-80, (int)(m >> 23) - 127 - 13));
         };
@@ -344,6 +347,16 @@ __global__ void __launch_bounds__(Shape4<D, NG, std::is_same<T, __half>::value ?
           }
         }
         const float down = pow2(-e);
+        if constexpr (TERMS == 2) {
+          if (e) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+#pragma unroll
+              for (int k = 0; k < NG; ++k)
+                pair[j][k] = as_u32(__hmul2(as_half2(pair[j][k]), __float2half2_rn(0.5f)));
+            }
+          }
+        }
         // --------------------------------------------------- a free stage
         const int stages = isv ? Sh::VS : KS;
         if (n >= stages) {

@@ -8,7 +8,7 @@ import torch
 
 from cacheslide_b200 import _native as N
 from cacheslide_b200 import kv4
-from test_gpu_kv4 import _check, _pool, _rows, _wide
+from test_gpu_kv4 import FORMS, _check, _pool, _rows, _wide
 
 pytestmark = pytest.mark.gpu
 
@@ -79,3 +79,26 @@ def test_sizes_far_apart_in_one_context(cuda, sizes, new, few):
     pool, table, q, starts = _filled(cuda, 5, [new] * 3, lengths, 8, 2, 128, 64, dtype, v.float())
     got, lse = _attend(cuda, pool, table, q, starts, lengths)
     _check(got, lse, pool, table, q, starts, lengths, 128 ** -0.5, _wide([new] * 3, 4))
+
+
+@pytest.mark.parametrize("dim,group", FORMS)
+@pytest.mark.parametrize("new", [1, 4, 60])
+@pytest.mark.parametrize("what", ["keys", "values"])
+def test_groups_at_the_end_of_float16(cuda, dim, group, new, what):
+    """-65504 .. 65504 and the like: whatever the operands are, they hold it."""
+    dtype, lengths = torch.float16, [max(new, n) for n in (20, 300, 77)]
+    n = 16 * sum(-(-a // 16) for a in lengths)
+    x = _rows(6, n, 2, dim, torch.float32)
+    ends = torch.tensor([65504.0, 62000.0, 61000.0, 65000.0])[torch.arange(n) % 4][:, None]
+    at = torch.arange(n) % 3 > 0
+    x[at, :, 5] = ends[at]
+    x[at, :, 30] = -ends[at]
+    x[at, :, 31] = 12345.0
+    values = x if what == "values" else _rows(7, n, 2, dim, torch.float32)
+    keys = x.half() if what == "keys" else None
+    pool, table, q, starts = _filled(cuda, 5, [new] * 3, lengths, 8, 2, dim, group, dtype, values,
+                                     keys)
+    scale = 1e-5 if what == "keys" else dim ** -0.5
+    got, lse = _attend(cuda, pool, table, q, starts, lengths, scale)
+    assert torch.isfinite(got).all() and torch.isfinite(lse).all()
+    _check(got, lse, pool, table, q, starts, lengths, scale, _wide([new] * 3, 4))
