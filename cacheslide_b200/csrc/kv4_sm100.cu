@@ -47,6 +47,9 @@ static_assert(kTileRows * NT == kWideRows, "the workspace's rows");
 constexpr int kLeastSteps = 4;    // steps a block takes at least
 constexpr float kLazy = 8.f;      // O is rescaled when the maximum grew by more than 2^8
 constexpr float kUp = 7.f;        // P is stored up by 2^7: fp16's normal numbers reach 2^-21
+// A thread's weights (which carry the values' power of two) that all lie below
+// 2^-100 of the reference are summed without that power, which may be as far down.
+constexpr float kFaint = 100.f;
 constexpr int kInfo = 8;          // steps whose scales are kept
 constexpr int kSegments = 4;      // segments the loader may be ahead
 
@@ -701,7 +704,7 @@ __global__ void __launch_bounds__(Shape4<D, NG, std::is_same<T, __half>::value ?
           continue;
         }
         CS_TMEM_LD32(sc + 32 * part2, v);
-        const float power = val_power[2 * info + part2];
+        float power = val_power[2 * info + part2];
         const float factor = fmaxf(row_factor * key_scale[2 * info + part2], 1e-30f);
         tmem_wait_ld();
         if (!__all_sync(~0u, vhi >= kKeys)) {
@@ -733,6 +736,7 @@ __global__ void __launch_bounds__(Shape4<D, NG, std::is_same<T, __half>::value ?
         // read their scores, so P may take their columns
         float* mx = row_max + (exchanges & 1) * 256;
         mx[part2 * 128 + r] = top;
+        const float own = top;
         __syncwarp();
         if (lane == 0) mbar_arrive(pair);
         ok = warp_wait(pair, exchanges & 1, abort);
@@ -745,21 +749,33 @@ __global__ void __launch_bounds__(Shape4<D, NG, std::is_same<T, __half>::value ?
         }
         const bool grow = top > mref + kLazy || mref == -INFINITY;
         const bool rescale = grow && mref > -INFINITY && top > mref;
-        if (__any_sync(~0u, rescale)) {  // t > 0: a row has a finite maximum
-          if (!wait_pv(t - 1)) break;
-          const float f = rescale ? ex2(mref - top) : 1.f;
-          lsum *= f;
-          uint32_t o[16];
+        // weights that leave float32 beside larger values' (own: not the masked -inf)
+        const bool faint = own < (grow ? top : mref) - kFaint && own > -INFINITY;
+        if (__any_sync(~0u, rescale || faint)) {
+          if (__any_sync(~0u, rescale)) {  // t > 0: a row has a finite maximum
+            if (!wait_pv(t - 1)) break;
+            // the root, since the reference may rise by more than float32's range;
+            // the sums of weights without the values' powers keep theirs
+            const float h = rescale ? ex2(0.5f * (mref - top)) : 1.f, f = h * h;
+            lsum = lsum * h * h;
+            uint32_t o[16];
 #pragma unroll 1
-          for (int cc = 0; cc < D / 16 / TPR; ++cc) {
-            const uint32_t col = oc + part2 * (D / 2) + 16 * cc;
-            CS_TMEM_LD16(col, o);
-            tmem_wait_ld();
+            for (int cc = 0; cc < D / 16 / TPR; ++cc) {
+              const uint32_t col = oc + part2 * (D / 2) + 16 * cc;
+              CS_TMEM_LD16(col, o);
+              tmem_wait_ld();
 #pragma unroll
-            for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
-            CS_TMEM_ST16(col, o);
+              for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
+              CS_TMEM_ST16(col, o);
+            }
+            tmem_wait_st();
           }
-          tmem_wait_st();
+          if (faint) {  // these weights count in the sum alone, and are zeros below
+            const float off = kUp - (grow ? top : mref);
+#pragma unroll
+            for (int c = 0; c < VC; ++c) lsum += ex2(fmaf(__uint_as_float(v[c]), factor, off));
+            power -= 126.f - kFaint + kUp;
+          }
         }
         if (grow) mref = top;
         const float less = power - ((mref > -INFINITY ? mref : 0.f) - kUp);

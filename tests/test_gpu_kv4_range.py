@@ -65,7 +65,7 @@ SPANS = [[0.0, 1e7], [0.0, 1e20], [1e7, 0.0], [1e-30, 1e20], [1e30, 1e-20, 1.0],
 
 
 @pytest.mark.parametrize("sizes", SPANS)
-@pytest.mark.parametrize("new", [1, 4])
+@pytest.mark.parametrize("new", [1, 4, 60])
 @pytest.mark.parametrize("few", [False, True])
 def test_sizes_far_apart_in_one_context(cuda, sizes, new, few):
     """Runs of keys whose values differ by many powers of two, in either order:
