@@ -49,13 +49,22 @@ int launch_dependent(K kernel, dim3 blocks, int threads, int smem, cudaStream_t 
 template <int RT> constexpr int kJoinRows = RT > 16 ? 16 : 4;
 constexpr float kLn2 = 0.6931471805599453f;
 
+// A mean of the type's numbers is none past its largest: what the weights'
+// rounding (2^-11 of it at most) carried there comes back.  Bfloat16's own half
+// step is wider than that.
+template <typename T> __device__ __forceinline__ float mean_of(float x) { return x; }
+template <> __device__ __forceinline__ float mean_of<__half>(float x) {
+  return fabsf(x) < 65600.f ? fminf(fmaxf(x, -65504.f), 65504.f) : x;
+}
+
 // four neighbouring elements from `c` on of row `row` of a (request, KV head)
 template <typename T>
 __device__ __forceinline__ void write4(const Attn4& a, int start, int row, int h, int c, float4 y) {
   const int tok = row / a.G;
   char* to = a.out + (int64_t)(start + tok) * a.ot +
              (int64_t)(h * a.G + (row - tok * a.G)) * a.oh + 2 * c;
-  const uint32_t lo = Pack2<T>::pack(y.x, y.y), hi = Pack2<T>::pack(y.z, y.w);
+  const uint32_t lo = Pack2<T>::pack(mean_of<T>(y.x), mean_of<T>(y.y)),
+                 hi = Pack2<T>::pack(mean_of<T>(y.z), mean_of<T>(y.w));
   if (a.vec_out) {
     *reinterpret_cast<uint2*>(to) = make_uint2(lo, hi);
   } else {
@@ -144,7 +153,7 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ A
     const int tok = (row0 + row) / a.G, head = h * a.G + (row0 + row - tok * a.G);
     T* out = reinterpret_cast<T*>(a.out + (int64_t)(r.start + tok) * a.ot + (int64_t)head * a.oh);
 #pragma unroll
-    for (int e = 0; e < E; ++e) out[lane * E + e] = Elem<T>::from_f(o[e] * inv);
+    for (int e = 0; e < E; ++e) out[lane * E + e] = Elem<T>::from_f(mean_of<T>(o[e] * inv));
     if (lane == 0)
       write_lse(a, r.start, row0 + row, h, sum == 0.f ? -INFINITY : top + log2f(sum * back));
   }

@@ -102,3 +102,35 @@ def test_groups_at_the_end_of_float16(cuda, dim, group, new, what):
     got, lse = _attend(cuda, pool, table, q, starts, lengths, scale)
     assert torch.isfinite(got).all() and torch.isfinite(lse).all()
     _check(got, lse, pool, table, q, starts, lengths, scale, _wide([new] * 3, 4))
+
+
+@pytest.mark.parametrize("value", [65504.0, -65504.0])
+@pytest.mark.parametrize("length", [130, 4000])
+@pytest.mark.parametrize("new", [1, 4, 60])
+@pytest.mark.parametrize("spread", [False, True])
+@pytest.mark.parametrize("odd", [False, True])
+def test_means_of_the_largest_number_stay_in_float16(cuda, value, length, new, spread, odd):
+    """A mean of numbers of a type is none that the type does not hold, however
+    the weights are rounded: all keys but the first 64 are equal, so that their
+    weights' roundings add up."""
+    lengths = [length + 5 * b for b in range(6)]
+    n = 16 * sum(-(-a // 16) for a in lengths)
+    keys, at = _rows(9, n, 2, 128, torch.float16), 0
+    for a in lengths:
+        keys[at:at + 64] = keys[at]
+        at += 16 * -(-a // 16)
+        keys[at - 16 * -(-a // 16) + 64:at] = keys[at - 1]
+    v = torch.full((n, 2, 128), value)
+    if spread:  # a scale of 8728 whose top is 65512, which rounds to the largest number
+        v[..., 1::2] = -65408.0 if value > 0 else 65408.0
+    pool, table, q, starts = _filled(cuda, 5, [new] * 6, lengths, 8, 2, 128, 64, torch.float16, v,
+                                     keys)
+    rows = torch.empty(*q.shape[:2], 133, dtype=q.dtype, device=cuda)[..., 1:129]
+    rows.copy_(q)
+    got = kv4.attention(rows, pool, table.to(cuda),
+                        torch.tensor(lengths, dtype=torch.int32, device=cuda), starts.to(cuda),
+                        out=rows if odd else None)
+    assert torch.isfinite(got).all()
+    _, held = kv4.gather(pool, torch.zeros(1, dtype=torch.int64, device=cuda))
+    # weights rounded to 2^-11 each act on 15 scales at most
+    assert ((got.float() - held[0, 0].float()).abs() <= 2.0 ** -11 * 2 * 65504 + 32).all()
