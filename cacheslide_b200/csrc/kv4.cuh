@@ -157,14 +157,16 @@ struct Request4 {
   int len, n, start;
 };
 
-__device__ __forceinline__ Request4 request4(const Attn4& a, int b) {
+// `floor`: the largest start before its own (0 at least), below which its rows
+// belong to another request
+__device__ __forceinline__ Request4 request4(const Attn4& a, int b, int floor) {
   Request4 r;
   r.len = a.lengths[b];
   r.start = a.starts ? a.starts[b] : b;
-  r.n = a.starts ? a.starts[b + 1] - r.start : 1;
-  const bool rows = r.start >= 0 && r.n >= 0 && (int64_t)r.start + r.n <= a.tokens;
+  const int end = a.starts ? a.starts[b + 1] : b + 1;
+  const bool rows = r.start >= floor && end >= r.start && end <= a.tokens;
   if (!rows || r.len > a.longest) report(a.status, CS_ST_CAPACITY);
-  if (!rows) r.n = 0;
+  r.n = rows ? end - r.start : 0;
   r.len = r.len < 0 ? 0 : r.len > a.longest ? (int)a.longest : r.len;
   return r;
 }
@@ -176,7 +178,6 @@ template <int RT, int KT>
 struct Share4 {
   int request, tile, head, step;  // where the worker begins
   int64_t todo, per;              // steps it takes, and every one takes at most
-  int taken;                      // (the caller's) of them, from the present tile
   Request4 r;
 
   static __device__ __forceinline__ int tiles(const Request4& r, int G) {
@@ -200,14 +201,17 @@ struct Share4 {
   // Every worker (block) sums up all requests for itself and takes an equal
   // range of all steps, `least` of them at least; the thread whose requests hold
   // the range's first step says where that is.  `Scratch` is shared memory; the
-  // first THREADS threads sum, all threads of the block call.
+  // first THREADS threads sum, all threads of the block call.  Returns whether the
+  // starts are in order; where they are not, the sums are made once more with each
+  // thread's largest start before its own.
   template <int THREADS>
   struct Scratch {
     int64_t warps[THREADS / 32];
+    int floors[THREADS / 32];
     Share4 found;
   };
   template <int THREADS>
-  __device__ __forceinline__ void find(const Attn4& a, int worker, int workers, int least,
+  __device__ __forceinline__ bool find(const Attn4& a, int worker, int workers, int least,
                                        Scratch<THREADS>& s) {
     constexpr int kWarps = THREADS / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -215,20 +219,46 @@ struct Share4 {
     const int b0 = min(a.requests, tid * share), b1 = min(a.requests, b0 + share);
     Request4 mine{0, 0, 0};
     int64_t own = 0, run = 0;
-    if (tid < THREADS) {
-      for (int b = b0; b < b1; ++b) {
-        mine = request4(a, b);
-        own += cost(a, mine);
-      }
-      run = own;
+    int floor = 0;  // before this thread's first request
+    bool ordered;
+    for (int pass = 0;; ++pass) {
+      bool falls = false;
+      if (tid < THREADS) {
+        own = 0;
+        int low = floor;
+        for (int b = b0; b < b1; ++b) {
+          mine = request4(a, b, low);
+          if (a.starts) {
+            falls |= a.starts[b + 1] < a.starts[b];
+            low = max(low, a.starts[b]);
+          }
+          own += cost(a, mine);
+        }
+        run = own;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(~0u, run, o);
-        if (lane >= o) run += x;
+        for (int o = 1; o < 32; o <<= 1) {
+          const int64_t x = __shfl_up_sync(~0u, run, o);
+          if (lane >= o) run += x;
+        }
+        if (lane == 31) s.warps[warp] = run;
       }
-      if (lane == 31) s.warps[warp] = run;
+      ordered = !__syncthreads_or(falls);
+      if (ordered || pass) break;
+      if (tid < THREADS) {
+        for (int b = b0; b < b1; ++b) floor = max(floor, a.starts[b]);
+#pragma unroll 1
+        for (int o = 1; o < 32; o <<= 1) {
+          const int x = __shfl_up_sync(~0u, floor, o);
+          if (lane >= o) floor = max(floor, x);
+        }
+        if (lane == 31) s.floors[warp] = floor;
+        floor = __shfl_up_sync(~0u, floor, 1);
+        if (lane == 0) floor = 0;
+      }
+      __syncthreads();
+      if (tid < THREADS)
+        for (int w = 0; w < warp; ++w) floor = max(floor, s.floors[w]);
     }
-    __syncthreads();
     int64_t all = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
@@ -238,15 +268,15 @@ struct Share4 {
     per = max((all + workers - 1) / workers, (int64_t)least);
     const int64_t from = worker * per;
     todo = max((int64_t)0, min(per, all - from));
-    taken = 0;
     if (todo > 0 && tid < THREADS && from >= run - own && from < run) {
       int64_t at = run - own;
       Share4 f;
       for (f.request = b0;; ++f.request) {  // one of this thread's requests has it
-        f.r = share == 1 ? mine : request4(a, f.request);
+        f.r = share == 1 ? mine : request4(a, f.request, floor);
         const int64_t c = cost(a, f.r);
         if (from < at + c) break;
         at += c;
+        if (a.starts) floor = max(floor, a.starts[f.request]);
       }
       for (f.tile = 0;; ++f.tile) {
         const int64_t c = (int64_t)steps(f.r, a.G, f.tile) * a.pool.hkv;
@@ -261,6 +291,7 @@ struct Share4 {
     __syncthreads();
     request = s.found.request, tile = s.found.tile, head = s.found.head, step = s.found.step;
     r = s.found.r;
+    return ordered;
   }
 
   // to the first step of the next (head, tile, request) that has rows
@@ -270,8 +301,10 @@ struct Share4 {
     head = 0;
     if (++tile < tiles(r, a.G)) return;
     tile = 0;
+    int floor = r.start + r.n;  // the largest start so far: its rows were in order
     do {
-      r = request4(a, ++request);  // there is one: the worker has steps to do
+      r = request4(a, ++request, floor);  // there is one: the worker has steps to do
+      floor = max(floor, r.start);
     } while (r.n == 0);
   }
 };

@@ -56,7 +56,6 @@ template <typename T> __device__ __forceinline__ float mean_of(float x) { return
 template <> __device__ __forceinline__ float mean_of<__half>(float x) {
   return fabsf(x) < 65600.f ? fminf(fmaxf(x, -65504.f), 65504.f) : x;
 }
-
 // four neighbouring elements from `c` on of row `row` of a (request, KV head)
 template <typename T>
 __device__ __forceinline__ void write4(const Attn4& a, int start, int row, int h, int c, float4 y) {
@@ -79,16 +78,29 @@ __device__ __forceinline__ void write_lse(const Attn4& a, int start, int row, in
   a.lse[(int64_t)(start + tok) * a.hq + h * a.G + (row - tok * a.G)] = lse2 * kLn2;
 }
 
-// rows outside every request, when they are to be zeros
+// rows outside every request, when they are to be zeros (`ordered`: the starts
+// are)
 template <typename T, int D>
-__device__ __forceinline__ void zero_rest(const Attn4& a) {
+__device__ __forceinline__ void zero_rest(const Attn4& a, bool ordered) {
   if (!a.zero_rest || a.starts == nullptr) return;
   const int64_t first = a.starts[0], end = a.starts[a.requests];
+  const bool plain = ordered && first >= 0 && end <= a.tokens;
+  if (plain && first == 0 && end == a.tokens) return;
+  // Requests that were left out leave rows in between.  A row belongs to the
+  // newest of the starts up to it that lies below none before.
+  auto owned = [&](int64_t row) {
+    for (int b = 0, floor = 0; b < a.requests; ++b) {
+      const int lo = a.starts[b], hi = a.starts[b + 1];
+      if (lo >= floor && lo <= row && row < hi && hi <= a.tokens) return true;
+      floor = max(floor, lo);
+    }
+    return false;
+  };
   const int64_t n = a.tokens * a.hq * (D / 4);
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n;
        i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t token = i / (a.hq * (D / 4));
-    if (token >= first && token < end) continue;
+    if (plain ? token >= first && token < end : owned(token)) continue;
     const int at = (int)(i - token * (a.hq * (D / 4)));
     const int head = at / (D / 4), c = 4 * (at % (D / 4));
     uint16_t* to = reinterpret_cast<uint16_t*>(a.out + token * a.ot + head * a.oh) + c;
@@ -109,7 +121,7 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ A
   const int4 j = a.joins[blockIdx.x];
   if (j.x < 0) return;
   const int lane = threadIdx.x & 31, first = blockIdx.x, parts = j.w - first + 1;
-  const Request4 r = request4(a, j.x);
+  const Request4 r = request4(a, j.x, 0);  // (its blocks have seen to its starts)
   const int row0 = j.y * RT, h = j.z >> 1;
   const int rows = min(min(RT, r.n * a.G - row0), (int)(blockIdx.y + 1) * kJoinRows<RT>);
   auto place = [&](int i) { return i == 0 ? 2ll * first + (j.z & 1) : 2ll * (first + i); };

@@ -177,9 +177,9 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
   Share work;
   using Scratch = typename Share::template Scratch<kThreads>;
   static_assert(sizeof(Scratch) <= R::oMax - R::oSums, "its place");
-  work.template find<kThreads>(a, blockIdx.x, gridDim.x, kLeast,
-                               *reinterpret_cast<Scratch*>(smem + R::oSums));
-  zero_rest<T, D>(a);
+  const bool ordered = work.template find<kThreads>(a, blockIdx.x, gridDim.x, kLeast,
+                                                    *reinterpret_cast<Scratch*>(smem + R::oSums));
+  zero_rest<T, D>(a, ordered);
   int issued = 0, taken = 0;  // units of this warp's ring
   bool late = false, bad_block = false;
   int which = 0;  // of this block's partial results

@@ -232,9 +232,9 @@ __global__ void __launch_bounds__(Shape4<D, NG, std::is_same<T, __half>::value ?
   Share work;
   using Scratch = typename Share::template Scratch<128>;
   static_assert(sizeof(Scratch) <= Sh::kMeta - Sh::oSums, "its place");
-  work.template find<128>(a, blockIdx.x, gridDim.x, kLeastSteps,
-                          *reinterpret_cast<Scratch*>(meta + Sh::oSums));
-  zero_rest<T, D>(a);
+  const bool ordered = work.template find<128>(a, blockIdx.x, gridDim.x, kLeastSteps,
+                                               *reinterpret_cast<Scratch*>(meta + Sh::oSums));
+  zero_rest<T, D>(a, ordered);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

@@ -174,8 +174,10 @@ def attention(query: Tensor, pool: PagedKV4, tables: Tensor, lengths: Tensor,
 
     A block outside the pool reads as zero keys and values and sets
     ``ST_SLOT_RANGE`` in ``status``; a length past the tables' width is cut
-    there, and starts that fall or leave the rows leave their request out;
-    both set ``ST_CAPACITY``.  A serving operator without a derivative."""
+    there, and a request is left out whose first row lies below an earlier one's
+    or whose rows fall or leave the query's; both set ``ST_CAPACITY``.  Rows of
+    a request that is left out belong to none.  A serving operator without a
+    derivative."""
     device = _pool(pool)
     if query.dim() != 3 or query.dtype is not pool.dtype or query.get_device() != device or \
             query.shape[2] != pool.head_dim or query.shape[1] < 1 or \

@@ -867,10 +867,11 @@ CS_API int cs_kv4_gather(const cs_kv4_pool* pool, const int64_t* slots, int64_t 
  *   lse = max + log(sum_j p_j);  o = 0 and lse = -inf where nothing is seen.
  * lengths, starts and tables are read on the device: a captured call follows
  * them.  Lengths past the tables' width end there and set CS_ST_CAPACITY, as
- * do starts that are negative, fall or pass `tokens` (their rows are left out).
+ * do starts[b] that are negative or below an earlier one and starts[b + 1] that
+ * are below starts[b] or pass `tokens`: request b is then left out.
  * A block id outside the pool sets CS_ST_SLOT_RANGE and its keys
- * and values are zeros.  Rows before starts[0] or from starts[requests] on are
- * left as they were, or zeroed (lse -inf) with `zero_rest`.
+ * and values are zeros.  Rows of no request, and of those left out, are left as
+ * they were, or zeroed (lse -inf) with `zero_rest`.
  */
 typedef struct {
   const void* q; /* [tokens, q_heads, head_dim], dtype of the pool */
