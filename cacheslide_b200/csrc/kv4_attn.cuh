@@ -56,6 +56,16 @@ template <typename T> __device__ __forceinline__ float mean_of(float x) { return
 template <> __device__ __forceinline__ float mean_of<__half>(float x) {
   return fabsf(x) < 65600.f ? fminf(fmaxf(x, -65504.f), 65504.f) : x;
 }
+// two of them as a pair of the type, none of which is an infinity of its own
+template <typename T> __device__ __forceinline__ uint32_t mean_pair(float x, float y) {
+  return Pack2<T>::pack(x, y);
+}
+template <> __device__ __forceinline__ uint32_t mean_pair<__half>(float x, float y) {
+  const uint32_t z = Pack2<__half>::pack(x, y);
+  return pair_bits(__hmin2_nan(__hmax2_nan(as_pair<__half>(z), as_pair<__half>(0xfbfffbffu)),
+                               as_pair<__half>(0x7bff7bffu)));
+}
+
 // four neighbouring elements from `c` on of row `row` of a (request, KV head)
 template <typename T>
 __device__ __forceinline__ void write4(const Attn4& a, int start, int row, int h, int c, float4 y) {

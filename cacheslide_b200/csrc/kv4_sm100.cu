@@ -873,8 +873,7 @@ __global__ void __launch_bounds__(Shape4<D, NG, std::is_same<T, __half>::value ?
                 uint32_t y[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                  y[k] = Pack2<T>::pack(mean_of<T>(final(v, 32 * cc, d + 2 * k)),
-                                        mean_of<T>(final(v, 32 * cc, d + 2 * k + 1)));
+                  y[k] = mean_pair<T>(final(v, 32 * cc, d + 2 * k), final(v, 32 * cc, d + 2 * k + 1));
                 st_shared16(buf + 64 * cc + 2 * d, make_uint4(y[0], y[1], y[2], y[3]));
               }
             }
