@@ -416,187 +416,190 @@ __global__ void __launch_bounds__(Shape4<D, NG, std::is_same<T, __half>::value ?
       return true;
     });
 
-  } else if (warp == Sh::kSoft + 4) {
-    // ============================================================ the loader
+  } else if (warp >= Sh::kSoft + 4) {
+    // a warpgroup's warps give up registers at one instruction, before their roles part
     regs_down<Sh::kRestRegs>();
-    bool bad_block = false;
-    int which = 0;  // of this block's partial results
-    int4 join = make_int4(-1, 0, 0, 0);
-    int n = 0;  // steps
-    for (int k = 0;; ++k) {
-      Segment& s = reinterpret_cast<Segment*>(meta + Sh::oSeg)[k % kSegments];
-      const uint32_t said = mb + Sh::bSeg + 8 * (k % kSegments);
-      if (k >= kSegments && !warp_wait(mb + Sh::bSegRead + 8 * (k % kSegments),
-                                       (k / kSegments - 1) & 1, abort))
-        break;
-      if (work.todo <= 0) {
+    if (warp == Sh::kSoft + 4) {
+      // ============================================================ the loader
+      bool bad_block = false;
+      int which = 0;  // of this block's partial results
+      int4 join = make_int4(-1, 0, 0, 0);
+      int n = 0;  // steps
+      for (int k = 0;; ++k) {
+        Segment& s = reinterpret_cast<Segment*>(meta + Sh::oSeg)[k % kSegments];
+        const uint32_t said = mb + Sh::bSeg + 8 * (k % kSegments);
+        if (k >= kSegments && !warp_wait(mb + Sh::bSegRead + 8 * (k % kSegments),
+                                         (k / kSegments - 1) & 1, abort))
+          break;
+        if (work.todo <= 0) {
+          if (lane == 0) {
+            s.steps = -1;
+            mbar_arrive(said);
+          }
+          break;
+        }
+        const int all_steps = Share::steps(work.r, a.G, work.tile);
+        const int s0 = work.step, s1 = (int)min((int64_t)all_steps, s0 + work.todo), g = work.head;
+        const bool whole = s0 == 0 && s1 == all_steps;
+        const int first_limit = work.r.len - work.r.n;
+        const int seen = max(0, first_limit + Share::last_token(work.r, a.G, work.tile) + 1);
+        const int steps = max(0, min(s1, (seen + kKeys - 1) / kKeys) - s0);
         if (lane == 0) {
-          s.steps = -1;
+          s.start = work.r.start;
+          s.g = g;
+          s.s0 = s0;
+          s.row0 = work.tile * RT;
+          s.rows = min(RT, work.r.n * a.G - s.row0);
+          s.tiles = s.rows > kTileRows ? 2 : 1;
+          s.first_limit = first_limit;
+          s.seen = seen;
+          s.steps = steps;
+          s.part = whole ? -1 : 2 * (int)blockIdx.x + which;
           mbar_arrive(said);
         }
-        break;
-      }
-      const int all_steps = Share::steps(work.r, a.G, work.tile);
-      const int s0 = work.step, s1 = (int)min((int64_t)all_steps, s0 + work.todo), g = work.head;
-      const bool whole = s0 == 0 && s1 == all_steps;
-      const int first_limit = work.r.len - work.r.n;
-      const int seen = max(0, first_limit + Share::last_token(work.r, a.G, work.tile) + 1);
-      const int steps = max(0, min(s1, (seen + kKeys - 1) / kKeys) - s0);
-      if (lane == 0) {
-        s.start = work.r.start;
-        s.g = g;
-        s.s0 = s0;
-        s.row0 = work.tile * RT;
-        s.rows = min(RT, work.r.n * a.G - s.row0);
-        s.tiles = s.rows > kTileRows ? 2 : 1;
-        s.first_limit = first_limit;
-        s.seen = seen;
-        s.steps = steps;
-        s.part = whole ? -1 : 2 * (int)blockIdx.x + which;
-        mbar_arrive(said);
-      }
-      if (!whole) {
-        if (s0 == 0)  // the first of the tile's blocks has them joined
-          join = make_int4(work.request, work.tile, 2 * g + which,
-                           blockIdx.x + (int)((all_steps - s1 + work.per - 1) / work.per));
-        which = 1;
-      }
-      const int32_t* table = a.tables + work.request * a.table_stride;
-      const int units = (seen + kUnit - 1) / kUnit;
-      int64_t from = -1;  // this lane's unit of eight steps: -1 none, 0 no block
-      bool ok = true;
-      for (int t = 0; ok && t < steps; ++t, ++n) {
-        if (t % 8 == 0) {
-          const int u = (s0 + t) * (kKeys / kUnit) + lane, j = u / a.pool.units;
-          from = -1;
-          if (u < units) {
-            const int id = table[j];
-            from = id >= 0 && id < a.pool.num_blocks
-                       ? reinterpret_cast<int64_t>(a.pool.unit(id, g, u - j * a.pool.units))
-                       : 0;
-            bad_block |= from == 0;
-          }
+        if (!whole) {
+          if (s0 == 0)  // the first of the tile's blocks has them joined
+            join = make_int4(work.request, work.tile, 2 * g + which,
+                             blockIdx.x + (int)((all_steps - s1 + work.per - 1) / work.per));
+          which = 1;
         }
-        if (n >= RS) {
-          ok = warp_wait(mb + Sh::bRead + 8 * (n % RS), (n / RS - 1) & 1, abort);
-          if (!ok) break;
-        }
-        if (lane / 4 == t % 8) {
-          const uint32_t bar = mb + Sh::bR + 8 * (n % RS);
-          const uint32_t to = Sh::oR + (n % RS) * Sh::RB + (lane % 4) * U::kBytes;
-          if (from > 0) {
-            arrive_expect(bar, U::kBytes);
-            bulk_copy(sbase + to, reinterpret_cast<const void*>(from), U::kBytes, bar);
-          } else {
-            if (from == 0) {  // zero codes, scales and lows: zero keys and values
-              for (int m = 0; m < U::kBytes / 16; ++m)
-                st_shared16(sbase + to + 16 * m, make_uint4(0, 0, 0, 0));
-              fence_async_smem();  // before a later copy into this place
+        const int32_t* table = a.tables + work.request * a.table_stride;
+        const int units = (seen + kUnit - 1) / kUnit;
+        int64_t from = -1;  // this lane's unit of eight steps: -1 none, 0 no block
+        bool ok = true;
+        for (int t = 0; ok && t < steps; ++t, ++n) {
+          if (t % 8 == 0) {
+            const int u = (s0 + t) * (kKeys / kUnit) + lane, j = u / a.pool.units;
+            from = -1;
+            if (u < units) {
+              const int id = table[j];
+              from = id >= 0 && id < a.pool.num_blocks
+                         ? reinterpret_cast<int64_t>(a.pool.unit(id, g, u - j * a.pool.units))
+                         : 0;
+              bad_block |= from == 0;
             }
-            mbar_arrive(bar);
           }
+          if (n >= RS) {
+            ok = warp_wait(mb + Sh::bRead + 8 * (n % RS), (n / RS - 1) & 1, abort);
+            if (!ok) break;
+          }
+          if (lane / 4 == t % 8) {
+            const uint32_t bar = mb + Sh::bR + 8 * (n % RS);
+            const uint32_t to = Sh::oR + (n % RS) * Sh::RB + (lane % 4) * U::kBytes;
+            if (from > 0) {
+              arrive_expect(bar, U::kBytes);
+              bulk_copy(sbase + to, reinterpret_cast<const void*>(from), U::kBytes, bar);
+            } else {
+              if (from == 0) {  // zero codes, scales and lows: zero keys and values
+                for (int m = 0; m < U::kBytes / 16; ++m)
+                  st_shared16(sbase + to + 16 * m, make_uint4(0, 0, 0, 0));
+                fence_async_smem();  // before a later copy into this place
+              }
+              mbar_arrive(bar);
+            }
+          }
+          __syncwarp();
         }
-        __syncwarp();
+        if (!ok) break;
+        work.todo -= s1 - s0;
+        if (work.todo > 0) work.next(a);
       }
-      if (!ok) break;
-      work.todo -= s1 - s0;
-      if (work.todo > 0) work.next(a);
-    }
-    // nothing of this block's copies is in flight when it ends
-    for (int u = n - RS < 0 ? 0 : n - RS; u < n; ++u) {
-      const long long t0 = clock64();
-      while (!mbar_try(mb + Sh::bR + 8 * (u % RS), (u / RS) & 1) && clock64() - t0 < kWaitCycles) {
+      // nothing of this block's copies is in flight when it ends
+      for (int u = n - RS < 0 ? 0 : n - RS; u < n; ++u) {
+        const long long t0 = clock64();
+        while (!mbar_try(mb + Sh::bR + 8 * (u % RS), (u / RS) & 1) &&
+               clock64() - t0 < kWaitCycles) {
+        }
       }
-    }
-    if (lane == 0) a.joins[blockIdx.x] = join;
-    if (bad_block) report(a.status, CS_ST_SLOT_RANGE);
+      if (lane == 0) a.joins[blockIdx.x] = join;
+      if (bad_block) report(a.status, CS_ST_SLOT_RANGE);
 
-  } else if (warp > Sh::kSoft + 4) {
-    // ==================================================== MMA, one warp a tile
-    regs_down<Sh::kRestRegs>();
-    const int qt = __shfl_sync(~0u, warp, 0) - (Sh::kSoft + 5);
-    const bool leader = elect_one();
-    const uint32_t id_s = umma_idesc(128, kKeys, 0, 0, 0);
-    const uint32_t id_o = umma_idesc(128, D, 0, 0, 1);  // V is MN-major
-    const uint64_t dq = umma_desc(sbase + Sh::oQ + qt * Sh::QB, 16, 1024);
-    const uint64_t dk0 = umma_desc(sbase + Sh::oK, 16, 1024);
-    const uint64_t dv0 = umma_desc(sbase + Sh::oV, kKeys * 128, 1024);
-    const uint32_t tm = __shfl_sync(~0u, tmem, 0);
-    const uint32_t sc = tm + Sh::cS + 128 * qt, oc = tm + Sh::cO + D * qt;
-    int n = 0, m = 0, queries = 0;  // steps of the block and of the row tile; its segments
-    uint32_t last = 0, lastph = 0;  // the newest group issued
-    auto drained = [&] {
-      const long long t0 = clock64();
-      while (last && !mbar_try(last, lastph) && clock64() - t0 < kWaitCycles) {
-      }
-      last = 0;
-    };
-    if (qt < NT) segments([&](const Segment& seg) {
-      const int steps = seg.steps;
-      if (qt < seg.tiles) {
-        if (!warp_wait(mb + Sh::bQ + 8 * qt, queries++ & 1, abort) ||
-            !__all_sync(~0u, caught_up(qt, n)))
-          return false;
-        auto arrived = [&](uint32_t bar, int u, int stages) {
-          return warp_wait(mb + bar + 8 * (u % stages), (u / stages) & 1, abort);
-        };
-        auto scores = [&](int t) {
-          if (!arrived(Sh::bK, n + t, KS)) return false;
-          tc_fence_after();
-          const uint64_t dk = dk0 + (uint64_t)(((n + t) % KS) * TERMS * (Sh::TB >> 4));
-          const uint32_t sb = sc + kKeys * ((m + t) & 1);
-          last = at(Sh::bS, qt, m + t);
-          lastph = ((m + t) >> 1) & 1;
-          if (leader) {
-#pragma unroll
-            for (int term = 0; term < TERMS; ++term) {
-#pragma unroll
-              for (int kk = 0; kk < D / 16; ++kk)  // offsets in 16-byte units
-                tc_mma(sb, dq + (kk >> 2) * 1024 + (kk & 3) * 2,
-                       dk + term * (Sh::TB >> 4) + (kk >> 2) * (kKeys * 8) + (kk & 3) * 2, id_s,
-                       term + kk ? 1u : 0u);
-            }
-            tc_commit(last);
-          }
-          __syncwarp();
-          return true;
-        };
-        for (int t = 0; t < 2 && t < steps; ++t)
-          if (!scores(t)) return false;
-        for (int t = 0; t < steps; ++t) {
-          const uint32_t ph = ((m + t) >> 1) & 1;
-          if (!arrived(Sh::bV, n + t, Sh::VS) || !warp_wait(at(Sh::bP, qt, m + t), ph, abort))
-            return false;
-          if (qt == 0 && lane == 0) *walked = n + t + 1;
-          tc_fence_after();
-          const uint64_t dv = dv0 + (uint64_t)(((n + t) % Sh::VS) * TERMS * (Sh::TB >> 4));
-          const uint32_t p = sc + kKeys * ((m + t) & 1);
-          last = at(Sh::bPV, qt, m + t);
-          lastph = ph;
-          if (leader) {
-#pragma unroll
-            for (int term = 0; term < TERMS; ++term) {
-#pragma unroll
-              for (int kk = 0; kk < kKeys / 16; ++kk)
-                tc_mma_ts(oc, p + kk * 8, dv + term * (Sh::TB >> 4) + kk * 128, id_o,
-                          (t | kk | term) ? 1u : 0u);
-            }
-            tc_commit(last);
-          }
-          __syncwarp();
-          // the next scores but one take the buffer that P lies in
-          if (t + 2 < steps &&
-              (!warp_wait(at(Sh::bPV, qt, m + t), ph, abort) || !scores(t + 2)))
-            return false;
+    } else {
+      // ==================================================== MMA, one warp a tile
+      const int qt = __shfl_sync(~0u, warp, 0) - (Sh::kSoft + 5);
+      const bool leader = elect_one();
+      const uint32_t id_s = umma_idesc(128, kKeys, 0, 0, 0);
+      const uint32_t id_o = umma_idesc(128, D, 0, 0, 1);  // V is MN-major
+      const uint64_t dq = umma_desc(sbase + Sh::oQ + qt * Sh::QB, 16, 1024);
+      const uint64_t dk0 = umma_desc(sbase + Sh::oK, 16, 1024);
+      const uint64_t dv0 = umma_desc(sbase + Sh::oV, kKeys * 128, 1024);
+      const uint32_t tm = __shfl_sync(~0u, tmem, 0);
+      const uint32_t sc = tm + Sh::cS + 128 * qt, oc = tm + Sh::cO + D * qt;
+      int n = 0, m = 0, queries = 0;  // steps of the block and of the row tile; its segments
+      uint32_t last = 0, lastph = 0;  // the newest group issued
+      auto drained = [&] {
+        const long long t0 = clock64();
+        while (last && !mbar_try(last, lastph) && clock64() - t0 < kWaitCycles) {
         }
-        drained();  // (the next segment's scores take both buffers)
-        m += steps;
-      }
-      n += steps;
-      return true;
-    });
-    drained();
-    __syncwarp();
+        last = 0;
+      };
+      if (qt < NT) segments([&](const Segment& seg) {
+        const int steps = seg.steps;
+        if (qt < seg.tiles) {
+          if (!warp_wait(mb + Sh::bQ + 8 * qt, queries++ & 1, abort) ||
+              !__all_sync(~0u, caught_up(qt, n)))
+            return false;
+          auto arrived = [&](uint32_t bar, int u, int stages) {
+            return warp_wait(mb + bar + 8 * (u % stages), (u / stages) & 1, abort);
+          };
+          auto scores = [&](int t) {
+            if (!arrived(Sh::bK, n + t, KS)) return false;
+            tc_fence_after();
+            const uint64_t dk = dk0 + (uint64_t)(((n + t) % KS) * TERMS * (Sh::TB >> 4));
+            const uint32_t sb = sc + kKeys * ((m + t) & 1);
+            last = at(Sh::bS, qt, m + t);
+            lastph = ((m + t) >> 1) & 1;
+            if (leader) {
+  #pragma unroll
+              for (int term = 0; term < TERMS; ++term) {
+  #pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk)  // offsets in 16-byte units
+                  tc_mma(sb, dq + (kk >> 2) * 1024 + (kk & 3) * 2,
+                         dk + term * (Sh::TB >> 4) + (kk >> 2) * (kKeys * 8) + (kk & 3) * 2, id_s,
+                         term + kk ? 1u : 0u);
+              }
+              tc_commit(last);
+            }
+            __syncwarp();
+            return true;
+          };
+          for (int t = 0; t < 2 && t < steps; ++t)
+            if (!scores(t)) return false;
+          for (int t = 0; t < steps; ++t) {
+            const uint32_t ph = ((m + t) >> 1) & 1;
+            if (!arrived(Sh::bV, n + t, Sh::VS) || !warp_wait(at(Sh::bP, qt, m + t), ph, abort))
+              return false;
+            if (qt == 0 && lane == 0) *walked = n + t + 1;
+            tc_fence_after();
+            const uint64_t dv = dv0 + (uint64_t)(((n + t) % Sh::VS) * TERMS * (Sh::TB >> 4));
+            const uint32_t p = sc + kKeys * ((m + t) & 1);
+            last = at(Sh::bPV, qt, m + t);
+            lastph = ph;
+            if (leader) {
+  #pragma unroll
+              for (int term = 0; term < TERMS; ++term) {
+  #pragma unroll
+                for (int kk = 0; kk < kKeys / 16; ++kk)
+                  tc_mma_ts(oc, p + kk * 8, dv + term * (Sh::TB >> 4) + kk * 128, id_o,
+                            (t | kk | term) ? 1u : 0u);
+              }
+              tc_commit(last);
+            }
+            __syncwarp();
+            // the next scores but one take the buffer that P lies in
+            if (t + 2 < steps &&
+                (!warp_wait(at(Sh::bPV, qt, m + t), ph, abort) || !scores(t + 2)))
+              return false;
+          }
+          drained();  // (the next segment's scores take both buffers)
+          m += steps;
+        }
+        n += steps;
+        return true;
+      });
+      drained();
+      __syncwarp();
+    }
 
   } else {
     // ================================================================= softmax
@@ -873,7 +876,8 @@ __global__ void __launch_bounds__(Shape4<D, NG, std::is_same<T, __half>::value ?
                 uint32_t y[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                  y[k] = mean_pair<T>(final(v, 32 * cc, d + 2 * k), final(v, 32 * cc, d + 2 * k + 1));
+                  y[k] = mean_pair<T>(final(v, 32 * cc, d + 2 * k),
+                                      final(v, 32 * cc, d + 2 * k + 1));
                 st_shared16(buf + 64 * cc + 2 * d, make_uint4(y[0], y[1], y[2], y[3]));
               }
             }
