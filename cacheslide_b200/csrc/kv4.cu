@@ -12,8 +12,11 @@
 // issue slots (139 with a second look at doubtful codes and two rows a warp), and
 // 74 us out.
 //
-// A code is decided as with the quotient in infinite precision: that is either
-// half way between two codes or 2^-16 of itself from there (scales have 11 bits).
+// A code is decided by the quotient, in infinite precision, of the float32
+// difference x - min x: that is either half way between two codes or 2^-16 of
+// itself from there (scales have 11 bits).  The difference of two numbers of the
+// type is mostly exact in float32; one that is not can lie on a half way that the
+// exact one misses (-832 and 2^-24 at a scale of 128: 6, not 7).
 #include <math.h>
 
 #include <type_traits>

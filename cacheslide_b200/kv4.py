@@ -98,8 +98,8 @@ def append(pool: PagedKV4, slots: Tensor, key: Tensor, value: Tensor, *,
     """The records of ``slots`` (int64 [token]) become ``key`` and ``value``
     [token, kv_head, dim] in 4 bits.
 
-    Each group's codes are the nearest of its sixteen values, ties to the even
-    code; a group that holds an infinity or a NaN stands for NaN throughout.
+    Each group's codes are the nearest of its sixteen values by their float32
+    difference to the lowest, ties to the even code; a group that holds an infinity or a NaN stands for NaN throughout.
     Slot -1 is padding and is not written; any other slot outside the pool is
     skipped and sets ``ST_SLOT_RANGE`` in ``status``.  Distinct tokens need
     distinct slots.  A serving operator without a derivative."""

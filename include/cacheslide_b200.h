@@ -819,8 +819,8 @@ CS_API int cs_step_maps(const cs_step_maps_params* p, void* stream);
  * token's head stands for the values low + scale * code, code in 0 .. 15, with
  *   low = min x,  scale = (max x - min x) / 15 in float32, rounded to `dtype`
  *   (to the next lower number where low + 15 scale would overflow it),
- *   code = (x - low) / scale, to the nearest, ties to even, at most 15
- *   (0 where scale is 0);
+ *   code = (x - low in float32) / scale, to the nearest, ties to even, at most
+ *   15 (0 where scale is 0);
  * a group with an infinity or a NaN has low = scale = NaN.  A unit is 16
  * tokens of a head: their key codes, head_dim / 2 bytes a token; their value
  * codes; the (scale, low) pairs of their keys' groups [16][head_dim / group],

@@ -1,6 +1,7 @@
 """Float64 restatement of the 4-bit pool: records, attention, slot maps.
 
-    low = min x,  scale = (max x - min x) / 15,  code = (x - low) / scale, nearest
+    low = min x,  scale = (max x - min x) / 15,  code = (x - low in float32) / scale,
+    nearest
     value = low + scale code
     o = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q.k_j - max)
 """
@@ -31,9 +32,9 @@ def params(x: torch.Tensor, group: int):
 
 
 def codes(x: torch.Tensor, scale: torch.Tensor, low: torch.Tensor, group: int) -> torch.Tensor:
-    y = x.double().unflatten(-1, (-1, group))
-    s, z = scale.double()[..., None], low.double()[..., None]
-    c = torch.where(s > 0, (y - z) / torch.where(s > 0, s, 1.0), 0.0).round().clamp(0, 15)
+    y = x.float().unflatten(-1, (-1, group)) - low.float()[..., None]
+    s = scale.double()[..., None]
+    c = torch.where(s > 0, y.double() / torch.where(s > 0, s, 1.0), 0.0).round().clamp(0, 15)
     return c.flatten(-2).to(torch.uint8)
 
 

@@ -8,6 +8,7 @@ import torch
 
 from cacheslide_b200 import _native as N
 from cacheslide_b200 import kv4
+from oracle import kv4 as okv4
 from test_gpu_kv4 import FORMS, _check, _pool, _rows, _wide
 
 pytestmark = pytest.mark.gpu
@@ -39,6 +40,25 @@ def _attend(cuda, pool, table, q, starts, lengths, scale=None):
                         scale=scale, return_lse=True, status=status)
     assert status.read() == 0
     return got
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_codes_by_differences_that_float32_rounds(cuda, dtype):
+    """Lowest values and elements far apart, at and beside the half ways."""
+    x = torch.zeros(60, 1, 64)
+    for i in range(60):
+        low = -832.0 * 2 ** (i % 5) if i % 2 else -13.0 * 2 ** (i % 7)
+        scale = -low * 2 / 13
+        x[i, 0, 0], x[i, 0, 1] = low, low + 15 * scale
+        x[i, 0, 2:34] = 2.0 ** -torch.arange(32) * (-1) ** (i // 3)
+        x[i, 0, 34:48] = low + scale * (torch.arange(14) + 0.5)
+    x = x.to(dtype)
+    slots = torch.arange(60)
+    pool = _pool(cuda, 4, 1, 16, 64, 64, dtype)
+    want = pool.storage.cpu()
+    okv4.write(want, slots, x, x.flip(0), 64)
+    kv4.append(pool, slots.to(cuda), x.to(cuda), x.flip(0).to(cuda))
+    assert torch.equal(pool.storage.cpu(), want)
 
 
 CONSTANTS = [(torch.float16, 60000.0), (torch.float16, -1000.0), (torch.float16, 6e-8),

@@ -1,5 +1,6 @@
-"""The bounds that the 4-bit attention is held to: the stated roundings, done in
-float64, stay inside, and mistakes do not."""
+"""The restatement of the 4-bit pool: the codes' float32 difference, and the bounds
+that the attention is held to (the stated roundings, done in float64, stay inside,
+and mistakes do not)."""
 
 from __future__ import annotations
 
@@ -99,3 +100,12 @@ def test_the_stated_roundings_are_inside_and_mistakes_are_not(dtype, dim, group,
         assert not o and not l
     for o, l, ratio in mistakes[3:]:
         assert ratio > 1.15
+
+
+def test_codes_go_by_the_difference_in_float32():
+    """2^-24 + 832 is 832 in float32, six and a half scales of 128."""
+    x = torch.zeros(1, 32, dtype=torch.float16)
+    x[0, 0], x[0, 1], x[0, 2], x[0, 3] = -832.0, 1088.0, 2.0 ** -24, 1.0
+    scale, low = okv4.params(x, 32)
+    assert scale.item() == 128 and low.item() == -832
+    assert okv4.codes(x, scale, low, 32)[0, :4].tolist() == [0, 15, 6, 7]
