@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from array import array
 from collections.abc import Sequence
 
 import torch
@@ -91,22 +92,28 @@ class SharedPrefixAttention:
             ctypes.addressof(suffixes))
         self.info = N.PrefixPlanInfo()
         lib = N.load()
+        # behind the plan's words, in the same copy to the device: query_lens, then
+        # suffix_lens, for what makes the step's slots there
+        lens = array("i", (*query_lens, *suffix_lens))
         capacity = 16 * self.tokens + 4096
         while True:
-            words = torch.empty(capacity, dtype=torch.int32)
+            words = torch.empty(capacity + len(lens), dtype=torch.int32)
             rc = lib.cs_prefix_plan(ctypes.byref(shape), ctypes.byref(self.info),
                                     words.data_ptr(), capacity)
             if rc != N.CS_ERR_TOO_LARGE or self.info.words <= capacity:
                 break
             capacity = self.info.words
         N.check(rc, "cs_prefix_plan")
-        # behind the plan's words, in the same copy: query_lens, then suffix_lens, for
-        # what makes the step's slots on the device
-        lens = torch.tensor([*query_lens, *suffix_lens], dtype=torch.int32)
-        both = torch.cat((words[:self.info.words], lens)).to(self.device)
-        self.words = both[:self.info.words]
-        self.device_lens = both[self.info.words:].view(2, len(self.query_lens))
+        ctypes.memmove(words.data_ptr() + 4 * self.info.words, lens.buffer_info()[0],
+                       4 * len(lens))
+        self._both = words[:self.info.words + len(lens)].to(self.device)
+        self.words = self._both[:self.info.words]
         self._stream = N.stream_of(self.device) if self.device.type == "cuda" else None
+
+    @property
+    def device_lens(self) -> Tensor:
+        """int32 [2, request] on the device: the query lengths, the suffix lengths."""
+        return self._both[self.info.words:].view(2, len(self.query_lens))
 
     def __call__(self, query: Tensor, kv: Tensor | NativePagedKV | N.PagedKV,
                  prefix_slots: Tensor, suffix_slots: Tensor, *, scale: float | None = None,
