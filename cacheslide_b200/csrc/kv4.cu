@@ -312,7 +312,7 @@ int check_attn4(const cs_kv4_attn_params* p) {
   CS_HOST_CHECK(p != nullptr && p->tokens >= 0 && p->tokens < INT32_MAX && p->requests >= 0);
   if (const int rc = check_pool4(p->pool)) return rc;
   CS_HOST_CHECK(p->q_heads > 0 && p->q_heads % p->pool.kv_heads == 0);
-  CS_HOST_CHECK(p->tokens * (p->q_heads / p->pool.kv_heads) < INT32_MAX);
+  CS_HOST_CHECK(p->tokens * (p->q_heads / p->pool.kv_heads) < INT32_MAX - kWideRows);
   CS_HOST_CHECK(p->starts != nullptr || p->tokens == p->requests);
   CS_HOST_CHECK(p->requests == 0 || (p->lengths && (p->tables || p->table_width == 0)));
   CS_HOST_CHECK(p->table_width >= 0 && (p->requests <= 1 || p->table_stride >= p->table_width));

@@ -181,7 +181,7 @@ struct Share4 {
   Request4 r;
 
   static __device__ __forceinline__ int tiles(const Request4& r, int G) {
-    return (r.n * G + RT - 1) / RT;  // (no row count passes 31 bits)
+    return (r.n * G + RT - 1) / RT;  // (31 bits hold any row count and a tile more)
   }
   static __device__ __forceinline__ int last_token(const Request4& r, int G, int tile) {
     const int i = (tile * RT + RT - 1) / G;
