@@ -643,7 +643,8 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
   if (tid == 0) a.joins[blockIdx.x] = join;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (bad_block) report(a.status, CS_ST_SLOT_RANGE);
-  if (late) {  // copies of this block are to have landed before it ends
+  // (any lane's wait: another may have seen the phase end just after)
+  if (__any_sync(~0u, late)) {  // copies of this block are to have landed before it ends
     for (int s = taken - S < 0 ? 0 : taken - S; s < taken; ++s) {
       const long long begin = clock64();
       while (!mbar_try(bars + 8 * (s % S), (s / S) & 1) && clock64() - begin < kWaitCycles) {
