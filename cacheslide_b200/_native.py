@@ -191,7 +191,8 @@ class StepMapsParams(ctypes.Structure):
     _fields_ = [
         ("lengths", _p), ("new_tokens", _p), ("requests", _i32), ("block_size", _i32),
         ("num_blocks", _i64), ("tables", _p), ("table_stride", _i64), ("table_width", _i32),
-        ("position_offset", _i32), ("free_blocks", _p), ("free_count", _p), ("free_left", _p), ("free_size", _i64),
+        ("position_offset", _i32), ("free_blocks", _p), ("free_count", _p), ("free_left", _p),
+        ("free_size", _i64),
         ("tokens", _i64), ("keys", _i64), ("starts", _p), ("positions", _p), ("slots", _p),
         ("key_starts", _p), ("key_slots", _p), ("status", _p),
     ]

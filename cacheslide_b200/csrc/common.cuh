@@ -222,6 +222,28 @@ inline bool allow_smem(int bytes) {
   return true;
 }
 
+// A launch that may start beside the end of the grid before it on the stream;
+// the kernel waits for that grid (griddepcontrol.wait) before it reads or
+// writes global memory.
+template <typename K, typename... A>
+int launch_dependent(K kernel, dim3 blocks, int threads, int smem, cudaStream_t stream, A... args) {
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t c = {};
+  c.gridDim = blocks;
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = stream;
+  c.attrs = at;
+  c.numAttrs = 1;
+  if (cudaLaunchKernelEx(&c, kernel, args...) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return CS_ERR_CUDA;
+  }
+  return CS_OK;
+}
+
 inline int num_sms() {
   static int n = 0;
   if (n == 0) {

@@ -1,5 +1,5 @@
-// What the two attention kernels of the 4-bit pool share: their dependent
-// launch, how a row's result is written, and the join of partial results.
+// What the two attention kernels of the 4-bit pool share: how a row's result is
+// written, and the join of partial results.
 #pragma once
 
 #include "kv4.cuh"
@@ -22,28 +22,6 @@ struct Plan4 {
   bool wide;
 };
 Plan4 plan4(const cs_kv4_attn_params& p);
-
-// A launch that may start beside the end of the grid before it on the stream;
-// the kernel waits for that grid (griddepcontrol.wait) before it reads or
-// writes global memory.
-template <typename K, typename... A>
-int launch_dependent(K kernel, dim3 blocks, int threads, int smem, cudaStream_t stream, A... args) {
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t c = {};
-  c.gridDim = blocks;
-  c.blockDim = dim3(threads);
-  c.dynamicSmemBytes = smem;
-  c.stream = stream;
-  c.attrs = at;
-  c.numAttrs = 1;
-  if (cudaLaunchKernelEx(&c, kernel, args...) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return CS_ERR_CUDA;
-  }
-  return CS_OK;
-}
 
 // rows of a joining block: one a warp, four where a tile has many
 template <int RT> constexpr int kJoinRows = RT > 16 ? 16 : 4;

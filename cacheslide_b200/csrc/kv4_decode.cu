@@ -98,18 +98,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes,
-                                          uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-          dst),
-      "l"(src), "r"(bytes), "r"(bar)
-      : "memory");
-}
-__device__ __forceinline__ void arrive_expect(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
-               : "memory");
-}
 __device__ __forceinline__ float lg2(float x) {
   float y;
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -129,9 +117,6 @@ __device__ __forceinline__ uint32_t less_middle(uint32_t x, uint32_t by) {
   return *reinterpret_cast<const uint32_t*>(&y);
 }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
-// 2^e for e in [-126, 127]
-__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
-
 template <int N> struct Words;
 template <> struct Words<4> {
   static __device__ __forceinline__ void load(uint32_t (&w)[4], const char* p) {
@@ -223,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
         const uint32_t bar = bars + 8 * st;
         char* to = ring + st * kStage + (lane % E) * U::kBytes;
         if (from > 0) {
-          arrive_expect(bar, U::kBytes);
+          mbar_arrive_expect(bar, U::kBytes);
           bulk_copy(smem_u32(to), reinterpret_cast<const void*>(from), U::kBytes, bar);
         } else {
           if (from == 0) {  // zero codes, scales and lows: zero keys and values
@@ -659,7 +644,8 @@ int launch_decode(const Attn4& a, int workers, cudaStream_t stream) {
   constexpr auto kernel = kv4_decode_kernel<T, D, NG, NT>;
   constexpr int kBytes = Ring<D, NG, NT>::kBytes;
   if (!allow_smem<kernel>(kBytes)) return CS_ERR_CUDA;
-  if (const int rc = launch_dependent(kernel, dim3(workers), kThreads, kBytes, stream, a)) return rc;
+  if (const int rc = launch_dependent(kernel, dim3(workers), kThreads, kBytes, stream, a))
+    return rc;
   return launch_join<T, D, 8 * NT>(a, workers, stream);
 }
 

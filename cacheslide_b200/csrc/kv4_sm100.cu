@@ -74,17 +74,18 @@ struct Shape4 {
   static constexpr int KS = 2, VS = 2, RS = TERMS == 2 ? 2 : 3;
   // a query tile's place also takes its output rows, 2 D bytes each and 16 more
   static constexpr uint32_t QB = kTileRows * D * 2 + kTileRows * 16;
-  static constexpr uint32_t oQ = 0, oK = NT * QB, oV = oK + KS * TERMS * TB, oR = oV + VS * TERMS * TB,
-                            oMeta = oR + RS * RB;
-  // barriers: a row tile's queries, and their place free; a stage's K and V; a score buffer's S, P and
-  // PV of a row tile; a row's maxima; raw units there, and read; a segment said,
-  // and read
-  static constexpr uint32_t bQ = 0, bFree = bQ + 8 * NT, bK = bFree + 8 * NT, bV = bK + 16, bS = bV + 16,
-                            bP = bS + 16 * NT, bPV = bP + 16 * NT, bMax = bPV + 16 * NT,
-                            bR = bMax + 32 * NT, bRead = bR + 8 * RS, bSeg = bRead + 8 * RS,
+  static constexpr uint32_t oQ = 0, oK = NT * QB, oV = oK + KS * TERMS * TB,
+                            oR = oV + VS * TERMS * TB, oMeta = oR + RS * RB;
+  // barriers: a row tile's queries, and their place free; a stage's K and V; a
+  // score buffer's S, P and PV of a row tile; a row's maxima; raw units there, and
+  // read; a segment said, and read
+  static constexpr uint32_t bQ = 0, bFree = bQ + 8 * NT, bK = bFree + 8 * NT, bV = bK + 16,
+                            bS = bV + 16, bP = bS + 16 * NT, bPV = bP + 16 * NT,
+                            bMax = bPV + 16 * NT, bR = bMax + 32 * NT, bRead = bR + 8 * RS, bSeg = bRead + 8 * RS,
                             bSegRead = bSeg + 8 * kSegments, oTmem = bSegRead + 8 * kSegments,
-                            oAbort = oTmem + 4, oWalked = oAbort + 4, oFlag = oWalked + 4, oScale = oFlag + 4 * kInfo,
-                            oPower = oScale + 8 * kInfo, oBad = oPower + 8 * kInfo, oRow = oBad + kInfo * kKeys,
+                            oAbort = oTmem + 4, oWalked = oAbort + 4, oFlag = oWalked + 4,
+                            oScale = oFlag + 4 * kInfo, oPower = oScale + 8 * kInfo,
+                            oBad = oPower + 8 * kInfo, oRow = oBad + kInfo * kKeys,
                             oMax = oRow + NT * kTileRows * 4,
                             oSeg = oMax + NT * 2 * 2 * 128 * 4,
                             oSums = (oSeg + 48 * kSegments + 7) / 8 * 8,
@@ -111,19 +112,6 @@ template <int R> __device__ __forceinline__ void regs_up() {
 template <int R> __device__ __forceinline__ void regs_down() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
 }
-__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes,
-                                          uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-          dst),
-      "l"(src), "r"(bytes), "r"(bar)
-      : "memory");
-}
-__device__ __forceinline__ void arrive_expect(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
-               : "memory");
-}
-__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
 __device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
 __device__ __forceinline__ uint32_t as_u32(__half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
 
@@ -385,7 +373,8 @@ __global__ void __launch_bounds__(Shape4<D, NG, std::is_same<T, __half>::value ?
           if (wrong_values) flag[info] = n;
         }
         const uint32_t tile =
-            sbase + (isv ? Sh::oV + (n % Sh::VS) * TERMS * Sh::TB : Sh::oK + (n % KS) * TERMS * Sh::TB);
+            sbase + (isv ? Sh::oV + (n % Sh::VS) * TERMS * Sh::TB
+                         : Sh::oK + (n % KS) * TERMS * Sh::TB);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
 #pragma unroll
@@ -487,7 +476,7 @@ __global__ void __launch_bounds__(Shape4<D, NG, std::is_same<T, __half>::value ?
             const uint32_t bar = mb + Sh::bR + 8 * (n % RS);
             const uint32_t to = Sh::oR + (n % RS) * Sh::RB + (lane % 4) * U::kBytes;
             if (from > 0) {
-              arrive_expect(bar, U::kBytes);
+              mbar_arrive_expect(bar, U::kBytes);
               bulk_copy(sbase + to, reinterpret_cast<const void*>(from), U::kBytes, bar);
             } else {
               if (from == 0) {  // zero codes, scales and lows: zero keys and values

@@ -991,35 +991,12 @@ bool setup_maps(PArgs& a, const cs_paged_kv& kv) {
   return true;
 }
 
-// A launch that may start beside the end of the grid before it on the stream;
-// the kernel waits for that grid (griddepcontrol.wait) before it reads or
-// writes global memory.
-template <typename K, typename... A>
-int launch_dependent(K kernel, unsigned blocks, int threads, uint32_t smem, cudaStream_t stream,
-                     A... args) {
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t c = {};
-  c.gridDim = dim3(blocks);
-  c.blockDim = dim3(threads);
-  c.dynamicSmemBytes = smem;
-  c.stream = stream;
-  c.attrs = at;
-  c.numAttrs = 1;
-  if (cudaLaunchKernelEx(&c, kernel, args...) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return CS_ERR_CUDA;
-  }
-  return CS_OK;
-}
-
 template <typename T, int D, int NT>
 int launch_main(const PArgs& a, int64_t blocks, cudaStream_t stream) {
   constexpr auto kernel = prefix_sm100_kernel<T, D, NT>;
   if (!allow_smem<kernel>(Shape<D, NT>::kSmem)) return CS_ERR_CUDA;
-  return launch_dependent(kernel, (unsigned)blocks, Shape<D, NT>::kThreads, Shape<D, NT>::kSmem,
-                          stream, a);
+  return launch_dependent(kernel, dim3((unsigned)blocks), Shape<D, NT>::kThreads,
+                          Shape<D, NT>::kSmem, stream, a);
 }
 
 template <typename T, int D>
@@ -1036,9 +1013,9 @@ int launch_all(const PArgs& a, const cs_prefix_plan_info& info, const int32_t* p
     const int32_t* list = plan + info.list_off;
     const int64_t rows = info.n_join * a.hq, entries = info.words - info.list_off;
     if (entries > 16 * info.n_join)
-      return launch_dependent(prefix_join_kernel<T, D, 4>, (unsigned)rows, 128, 0, stream, a, join,
-                              list, (int)info.n_join);
-    return launch_dependent(prefix_join_kernel<T, D, 1>, (unsigned)((rows + 3) / 4), 128, 0,
+      return launch_dependent(prefix_join_kernel<T, D, 4>, dim3((unsigned)rows), 128, 0, stream, a,
+                              join, list, (int)info.n_join);
+    return launch_dependent(prefix_join_kernel<T, D, 1>, dim3((unsigned)((rows + 3) / 4)), 128, 0,
                             stream, a, join, list, (int)info.n_join);
   }
   return CS_OK;

@@ -206,6 +206,8 @@ __device__ __forceinline__ uint32_t sw128(int row, int c16, int rows) {
   return (uint32_t)((c16 >> 3) * rows * 128 + row * 128 + (((c16 & 7) ^ (row & 7)) << 4));
 }
 
+// 2^e for e in [-126, 127]
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -253,6 +255,19 @@ __device__ __forceinline__ void tma_tile2d(uint32_t dst, const CUtensorMap* map,
 __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes)
                : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+// `bytes` (whole 16s, both ends 16-byte aligned) into shared memory
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes,
+                                          uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1], %2, [%3];" ::"r"(dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
 }
 // tile::gather4: rows r0..r3 of a 2-D tensor map, 64 elements from column x,
 // into 4 consecutive 128-byte rows at dst (the map's 128-byte swizzle applies)

@@ -99,10 +99,11 @@ def append(pool: PagedKV4, slots: Tensor, key: Tensor, value: Tensor, *,
     [token, kv_head, dim] in 4 bits.
 
     Each group's codes are the nearest of its sixteen values by their float32
-    difference to the lowest, ties to the even code; a group that holds an infinity or a NaN stands for NaN throughout.
-    Slot -1 is padding and is not written; any other slot outside the pool is
-    skipped and sets ``ST_SLOT_RANGE`` in ``status``.  Distinct tokens need
-    distinct slots.  A serving operator without a derivative."""
+    difference to the lowest, ties to the even code; a group that holds an
+    infinity or a NaN stands for NaN throughout.  Slot -1 is padding and is not
+    written; any other slot outside the pool is skipped and sets
+    ``ST_SLOT_RANGE`` in ``status``.  Distinct tokens need distinct slots.  A
+    serving operator without a derivative."""
     device = _pool(pool)
     n = _slots(slots, pool)
     shape = (n, pool.kv_heads, pool.head_dim)

@@ -108,7 +108,8 @@ def step_maps(lengths: Tensor, new: Tensor, tables: Tensor, block_size: int, num
         key_starts = torch.empty(requests + 1, dtype=torch.int64, device=on)
     p = N.StepMapsParams(
         p_lengths, p_new, requests, block_size, num_blocks, tables.data_ptr(), tables.stride(0),
-        width, offset, p_free, p_count, N.ptr(left), 0 if free is None else free.shape[0], tokens, keys, starts.data_ptr(),
-        positions.data_ptr(), slots.data_ptr(), N.ptr(key_starts), N.ptr(key_slots), status_ptr)
+        width, offset, p_free, p_count, N.ptr(left), 0 if free is None else free.shape[0], tokens,
+        keys, starts.data_ptr(), positions.data_ptr(), slots.data_ptr(), N.ptr(key_starts),
+        N.ptr(key_slots), status_ptr)
     N.launch("cs_step_maps", on, p)
     return StepMaps(starts, positions, slots, key_starts, key_slots, left)

@@ -196,7 +196,8 @@ def bounds(q, storage, table, length, n, group, scale, wide) -> Bounds:
     most, widest = w.nan_to_num().amax(-1)[..., None], v.nan_to_num(0, 0, 0).abs().amax()
     step = vs.nan_to_num(0, 0, 0).amax()
     err = 2 * mix(w * dz, v.abs())
-    lse_err = (w * dz).sum(-1).nan_to_num() + 2.0 ** -20 * (1 + lse.abs().nan_to_num(0, 0, 0) + power)
+    lse_err = (w * dz).sum(-1).nan_to_num()
+    lse_err = lse_err + 2.0 ** -20 * (1 + lse.abs().nan_to_num(0, 0, 0) + power)
     if wide:
         k2, v2 = operands(kc, ks, kz, q.dtype), operands(vc, vs, vz, q.dtype)
         _, w2, lse2 = soft(k2)

@@ -67,7 +67,8 @@ def test_cut_and_joined(cuda, dtype, new):
 
 @pytest.mark.parametrize("dtype", TYPES)
 def test_decodes_beside_a_chunk(cuda, dtype):
-    _tight(cuda, [1] * 20 + [300], [100 + 90 * b for b in range(20)] + [700], 8, 2, 128, 64, 16, dtype)
+    _tight(cuda, [1] * 20 + [300], [100 + 90 * b for b in range(20)] + [700], 8, 2, 128, 64, 16,
+           dtype)
 
 
 @pytest.mark.parametrize("new", [1, 60])

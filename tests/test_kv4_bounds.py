@@ -70,7 +70,8 @@ def _kernel(q, storage, table, length, group, scale, wide, *, shift=0, drop=None
         o = o * down[..., None] + here
     some = total != 0
     out = torch.where(some[..., None], o / torch.where(some, total, 1.0)[..., None], 0.0)
-    lse = torch.where(some, ref - (7 if wide else 6) + torch.where(some, total, 1.0).log2(), -math.inf)
+    total = torch.where(some, total, 1.0)
+    lse = torch.where(some, ref - (7 if wide else 6) + total.log2(), -math.inf)
     return out.reshape(n, hq, d).to(q.dtype), lse.reshape(n, hq) * math.log(2)
 
 
