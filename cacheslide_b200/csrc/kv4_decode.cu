@@ -274,7 +274,8 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
         sum[k] += __shfl_xor_sync(~0u, sum[k], 1);
         sum[k] += __shfl_xor_sync(~0u, sum[k], 2);
       }
-      const int e = min(100, max(-100, (int)(__float_as_uint(top) >> 23) - 127));
+      // (2^-124 and 2^124 below: queries of up to 2^116)
+      const int e = min(113, max(-100, (int)(__float_as_uint(top) >> 23) - 127));
       const float up = pow2(13 - e);
 #pragma unroll
       for (int w = 0; w < W; ++w) {

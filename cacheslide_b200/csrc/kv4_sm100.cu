@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(Shape4<D, NG, std::is_same<T, __half>::value ?
         // (the K warps look at the values' pairs too, and say with the key tile
         // what the softmax has to know of them)
         const int key0 = first_key + t * kKeys;
-        auto reach_of = [&](uint32_t (&pairs)[4][NG], uint32_t& wrong) {
+        auto reach_of = [&](uint32_t (&pairs)[4][NG], int least, uint32_t& wrong) {
           float reach = 0.f;
           wrong = 0u;  // bit NG j + k
 #pragma unroll
@@ -324,11 +324,13 @@ __global__ void __launch_bounds__(Shape4<D, NG, std::is_same<T, __half>::value ?
           // warp that have larger ones are halved
           if constexpr (TERMS == 2) return __any_sync(~0u, reach >= 0x1p15f) ? 1 : 0;
           const uint32_t m = __reduce_max_sync(~0u, __float_as_uint(reach));
-          return m == 0u ? 0 : min(114, max(-80, (int)(m >> 23) - 127 - 13));
+          return m == 0u ? 0 : min(114, max(least, (int)(m >> 23) - 127 - 13));
         };
         uint32_t wrong, wrong_values = 0u;
-        const int e = reach_of(pair, wrong);
-        const int ev = isv ? 0 : reach_of(values, wrong_values);
+        // (the rows' sums take the values' power off again: 2^80 times 2^15 of 2^31 keys)
+        constexpr int kLeastKeys = -114, kLeastValues = -80;
+        const int e = reach_of(pair, isv ? kLeastValues : kLeastKeys, wrong);
+        const int ev = isv ? 0 : reach_of(values, kLeastValues, wrong_values);
         if (isv && wrong) {  // a bad value becomes 0 and marks the rows that see it
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -647,7 +649,7 @@ __global__ void __launch_bounds__(Shape4<D, NG, std::is_same<T, __half>::value ?
           }
 #pragma unroll
           for (int o = 1; o < C; o <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-          const int e = min(100, max(-100, (int)(__float_as_uint(top) >> 23) - 127 - 13));
+          const int e = min(114, max(-100, (int)(__float_as_uint(top) >> 23) - 127 - 13));
           const float up = pow2(-e);
           if (c == 0) row_scale[qt * kTileRows + q] = pow2(e);
           uint32_t y[4];

@@ -154,3 +154,44 @@ def test_means_of_the_largest_number_stay_in_float16(cuda, value, length, new, s
     _, held = kv4.gather(pool, torch.zeros(1, dtype=torch.int64, device=cuda))
     # weights rounded to 2^-11 each act on 15 scales at most
     assert ((got.float() - held[0, 0].float()).abs() <= 2.0 ** -11 * 2 * 65504 + 32).all()
+
+
+@pytest.mark.parametrize("up", [-100, -60, 60, 100, 112])
+@pytest.mark.parametrize("new", [1, 4, 60])
+def test_queries_and_keys_of_opposite_sizes(cuda, up, new):
+    """Powers of two that the scores do not show."""
+    lengths = [max(new, n) for n in (40, 640, 97)]
+    n = 16 * sum(-(-a // 16) for a in lengths)
+    values = _rows(4, n, 2, 128, torch.bfloat16)
+    keys = _rows(5, n, 2, 128, torch.float32)
+    outs = []
+    for power in (0, up):
+        pool, table, q, starts = _filled(cuda, 5, [new] * 3, lengths, 8, 2, 128, 64, torch.bfloat16,
+                                         values, torch.ldexp(keys, torch.tensor(-power)).bfloat16())
+        q = torch.ldexp(q.float(), torch.tensor(power)).bfloat16()
+        got, lse = _attend(cuda, pool, table, q, starts, lengths)
+        _check(got, lse, pool, table, q, starts, lengths, 128 ** -0.5, _wide([new] * 3, 4))
+        outs.append(got)
+    # (numbers below fp16's normal ones may lose bits, 2^-27 of the largest at least)
+    assert (outs[0].float() - outs[1].float()).abs().max() <= 2.0 ** -7 * outs[0].abs().max()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("new", [1, 4, 60])
+def test_a_query_that_is_not_finite_reaches_its_own_row(cuda, bad, dtype, new):
+    lengths = [max(new, n) for n in (40, 640, 97)]
+    pool, table, q, starts = _filled(cuda, 5, [new] * 3, lengths, 8, 2, 128, 64, dtype,
+                                     _rows(4, 16 * 88, 2, 128, dtype)[:16 * sum(
+                                         -(-a // 16) for a in lengths)])
+    want, want_lse = _attend(cuda, pool, table, q, starts, lengths)
+    # newest tokens, which see keys of either sign: a score of +inf or NaN among theirs
+    at = [(new - 1, 3), (2 * new - 1, 7), (3 * new - 1, 0)]
+    for token, head in at:
+        q[token, head, 77] = bad
+    got, lse = _attend(cuda, pool, table, q, starts, lengths)
+    own = torch.zeros(q.shape[:2], dtype=torch.bool)
+    for token, head in at:
+        own[token, head] = True
+    assert torch.isnan(got[own]).all() and not torch.isfinite(lse[own]).any()
+    assert torch.equal(got[~own], want[~own]) and torch.equal(lse[~own], want_lse[~own])
