@@ -300,7 +300,8 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
 #pragma unroll
         for (int w = 0; w < NG; ++w)
           (k ? qs[nt][w].y : qs[nt][w].x) = __shfl_sync(~0u, sum[w], from_lane);
-        limit[nt][k] = m < rows ? r.len - r.n + m / a.G : INT32_MAX;  // no row: of no matter
+        // (no row: what lies behind the last key is not to move the others' reference)
+        limit[nt][k] = m < rows ? r.len - r.n + m / a.G : seen - 1;
         low_limit = min(low_limit, limit[nt][k]);
       }
     }
@@ -511,9 +512,8 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
                   const int bit = 4 * (NT * e + nt) + 2 * c;
                   const bool sx = shown >> bit & 1u, sy = shown >> (bit + 1) & 1u;
                   w = make_float2(sx ? w.x : 0.f, sy ? w.y : 0.f);
-                  const float2 low = __fmul2_rn(p[e][nt][c], both(s.y));
-                  lows[nt][k] = __fadd2_rn(lows[nt][k],
-                                           make_float2(sx ? low.x : 0.f, sy ? low.y : 0.f));
+                  const float2 low = make_float2(sx ? s.y : 0.f, sy ? s.y : 0.f);
+                  lows[nt][k] = __ffma2_rn(p[e][nt][c], low, lows[nt][k]);
                 } else {
                   lows[nt][k] = __ffma2_rn(p[e][nt][c], both(s.y), lows[nt][k]);
                 }
