@@ -22,7 +22,8 @@ def params(x: torch.Tensor, group: int):
     low, high = y.amin(-1) + 0.0, y.amax(-1)  # (a zero without a sign)
     # the quotient in float32 (its exact range in float64), then 16 bits
     scale = ((high.double() - low.double()) / 15).abs().float().to(x.dtype)
-    top = {torch.float16: 65520.0, torch.bfloat16: 3.3961775292304957e38}[x.dtype]
+    # half a step past the largest number, which rounds to infinity
+    top = torch.finfo(x.dtype).max + {torch.float16: 16.0, torch.bfloat16: 2.0 ** 119}[x.dtype]
     over = low.double() + 15 * scale.double() >= top
     down = (scale.view(torch.int16) - 1).view(x.dtype)
     scale = torch.where(over, down, scale)
@@ -32,8 +33,10 @@ def params(x: torch.Tensor, group: int):
 
 
 def codes(x: torch.Tensor, scale: torch.Tensor, low: torch.Tensor, group: int) -> torch.Tensor:
-    y = x.float().unflatten(-1, (-1, group)) - low.float()[..., None]
-    s = scale.double()[..., None]
+    # (a power of two keeps the difference below float32's largest number)
+    up = torch.where(scale.float() < 2.0 ** -60, 2.0 ** 60, 2.0 ** -4)[..., None]
+    y = x.float().unflatten(-1, (-1, group)) * up - low.float()[..., None] * up
+    s = scale.double()[..., None] * up
     c = torch.where(s > 0, y.double() / torch.where(s > 0, s, 1.0), 0.0).round().clamp(0, 15)
     return c.flatten(-2).to(torch.uint8)
 

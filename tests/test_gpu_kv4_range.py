@@ -61,6 +61,28 @@ def test_codes_by_differences_that_float32_rounds(cuda, dtype):
     assert torch.equal(pool.storage.cpu(), want)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim,group", FORMS)
+def test_records_of_any_bits(cuda, dtype, dim, group):
+    """Numbers of all patterns: within a few powers of two, to the types' ends, and
+    with infinities and NaN among them (a group of one is NaN, whichever)."""
+    g = torch.Generator().manual_seed(dim + group)
+    top = 0x7C00 if dtype == torch.float16 else 0x7F80
+    first = torch.randint(0, top, (400, 1, 1), generator=g)
+    size = 2 ** torch.randint(0, 15, (400, 1, 1), generator=g)
+    bits = first + torch.randint(0, 1 << 15, (400, 2, dim), generator=g) % size
+    bits = bits.clamp(max=top - 1) | torch.randint(0, 2, bits.shape, generator=g) << 15
+    bits[:40] = torch.randint(0, 1 << 16, (40, 2, dim), generator=g)
+    x = bits.to(torch.int32).to(torch.int16).view(dtype)
+    slots = torch.arange(400)
+    pool = _pool(cuda, 25, 2, 16, dim, group, dtype)
+    want = pool.storage.cpu()
+    okv4.write(want, slots, x, x.flip(0), group)
+    kv4.append(pool, slots.to(cuda), x.to(cuda), x.flip(0).to(cuda))
+    for a, b in zip(*(okv4.read(s, slots, dim, group, dtype) for s in (pool.storage.cpu(), want))):
+        assert ((a == b) | a.isnan() & b.isnan()).all()
+
+
 CONSTANTS = [(torch.float16, 60000.0), (torch.float16, -1000.0), (torch.float16, 6e-8),
              (torch.bfloat16, 1e7), (torch.bfloat16, 2.0 ** 22), (torch.bfloat16, -3e38),
              (torch.bfloat16, 1e-38), (torch.bfloat16, 1.0), (torch.float16, 0.0)]

@@ -110,3 +110,23 @@ def test_codes_go_by_the_difference_in_float32():
     scale, low = okv4.params(x, 32)
     assert scale.item() == 128 and low.item() == -832
     assert okv4.codes(x, scale, low, 32)[0, :4].tolist() == [0, 15, 6, 7]
+
+
+def test_codes_of_the_widest_groups():
+    """Differences past float32's largest number, and far below its smallest scale."""
+    big = torch.finfo(torch.bfloat16).max
+    for unit in (big, 1e-37):
+        x = (torch.linspace(-1, 1, 32) * unit).bfloat16()[None]
+        scale, low = okv4.params(x, 32)
+        got = okv4.codes(x, scale, low, 32)[0].double()
+        exact = (x[0].double() - low.double()) / scale.double()
+        assert ((got - exact).abs() <= 0.5 + (exact - 15).clamp(min=0)).all()
+
+
+def test_a_scale_whose_last_value_would_round_to_infinity():
+    """low + 15 scale exactly half a step past the largest number: the scale below."""
+    x = torch.zeros(1, 32, dtype=torch.bfloat16)
+    x[0, 0] = -6.911985578081563e37
+    x[0, 1] = torch.finfo(torch.bfloat16).max
+    scale, low = okv4.params(x, 32)
+    assert torch.isfinite((low.double() + 15 * scale.double()).to(torch.bfloat16)).all()
