@@ -44,10 +44,12 @@ constexpr float kTooLarge = 0x1p14f;  // it may grow to 2^14 before O is rescale
 constexpr float kLowest = -3e38f;     // below every score, and finite
 // What a key may add goes by its largest scale, 2^-40 of its largest lowest value
 // (constant groups have no scale: p low then stays below 2^54) and at least
-// 2^-80, so that the sums of p stay below 2^125 over 2^31 keys of zeros.  Above
-// 2^116 the reference stops rising: p scale is at most 2^16 there, and p at least
-// 2^-110 for a row's largest score, 2^-16 of which float32 still holds.
-constexpr float kLowCounts = 0x1p-40f, kLeastMost = 0x1p-80f, kMostLog = 116.f;
+// 2^-100; the sums of p, which are kept 2^-24 of theirs, then stay below 2^121 over
+// 2^31 keys of zeros.  Above 2^116 the reference stops rising: p scale is at most
+// 2^16 there, and p at least 2^-110 for a row's largest score, 2^-16 of which
+// float32 still holds.
+constexpr float kLowCounts = 0x1p-40f, kLeastMost = 0x1p-100f, kMostLog = 116.f;
+constexpr float kSumDown = 0x1p-24f;
 
 // Blocks an SM holds, as the registers allow without spilling in the loop over
 // the keys: 32 decodes of up to 16K keys in four groups take 102 us with three
@@ -496,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
           Words<NG>::load(vb, unit + U::oVp + 4 * NG * (g + 8));
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
-            lsum[nt] = __fadd2_rn(lsum[nt], __fadd2_rn(p[e][nt][0], p[e][nt][1]));
+            lsum[nt] = __ffma2_rn(__fadd2_rn(p[e][nt][0], p[e][nt][1]), both(kSumDown), lsum[nt]);
 #pragma unroll
           for (int k = 0; k < NG; ++k) {
             uint32_t pf[NT][2];
@@ -605,9 +607,12 @@ __global__ void __launch_bounds__(kThreads, Ring<D, NG, NT>::kBlocks)
         const float4 z = *reinterpret_cast<const float4*>(outs + (w * RT + row) * D + c);
         y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
       }
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      const float lse2 = l == 0.f ? -INFINITY : top + log2f(l);
-      y.x *= inv, y.y *= inv, y.z *= inv, y.w *= inv;
+      // (l from 2^-134 to 2^121: its reciprocal in float32's range)
+      const float up = l < 0x1p-60f ? 0x1p64f : 1.f, down = up * kSumDown;
+      const float inv = l == 0.f ? 0.f : 1.f / (l * up);
+      const float lse2 = l == 0.f ? -INFINITY : top + (log2f(l) + 24.f);
+      y.x = y.x * down * inv, y.y = y.y * down * inv;
+      y.z = y.z * down * inv, y.w = y.w * down * inv;
       if (whole) {
         write4<T>(a, r.start, row0 + row, h, c, y);
         if (c == 0) write_lse(a, r.start, row0 + row, h, lse2);
