@@ -47,6 +47,7 @@ static_assert(kTileRows * NT == kWideRows, "the workspace's rows");
 constexpr int kLeastSteps = 4;    // steps a block takes at least
 constexpr float kLazy = 8.f;      // O is rescaled when the maximum grew by more than 2^8
 constexpr float kUp = 7.f;        // P is stored up by 2^7: fp16's normal numbers reach 2^-21
+constexpr float kSumDown = 0x1p-24f;  // the sums of weights are kept this much smaller
 // A thread's weights (which carry the values' power of two) that all lie below
 // 2^-100 of the reference are summed without that power, which may be as far down.
 constexpr float kFaint = 100.f;
@@ -327,8 +328,9 @@ __global__ void __launch_bounds__(Shape4<D, NG, std::is_same<T, __half>::value ?
           return m == 0u ? 0 : min(114, max(least, (int)(m >> 23) - 127 - 13));
         };
         uint32_t wrong, wrong_values = 0u;
-        // (the rows' sums take the values' power off again: 2^80 times 2^15 of 2^31 keys)
-        constexpr int kLeastKeys = -114, kLeastValues = -80;
+        // (the rows' sums, which are 2^-24 of theirs, take the values' power off again:
+        // 2^104 times 2^15 of 2^31 keys)
+        constexpr int kLeastKeys = -114, kLeastValues = -104;
         const int e = reach_of(pair, isv ? kLeastValues : kLeastKeys, wrong);
         const int ev = isv ? 0 : reach_of(values, kLeastValues, wrong_values);
         if (isv && wrong) {  // a bad value becomes 0 and marks the rows that see it
@@ -767,7 +769,8 @@ __global__ void __launch_bounds__(Shape4<D, NG, std::is_same<T, __half>::value ?
           if (faint) {  // these weights count in the sum alone, and are zeros below
             const float off = kUp - (grow ? top : mref);
 #pragma unroll
-            for (int c = 0; c < VC; ++c) lsum += ex2(fmaf(__uint_as_float(v[c]), factor, off));
+            for (int c = 0; c < VC; ++c)
+              lsum = fmaf(ex2(fmaf(__uint_as_float(v[c]), factor, off)), kSumDown, lsum);
             power -= 126.f - kFaint + kUp;
           }
         }
@@ -789,7 +792,8 @@ __global__ void __launch_bounds__(Shape4<D, NG, std::is_same<T, __half>::value ?
           p0 = __fadd2_rn(p0, make_float2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])));
           p1 = __fadd2_rn(p1, make_float2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])));
         }
-        lsum = fmaf((p0.x + p0.y) + (p1.x + p1.y), ex2(-power), lsum);
+        // (in two steps: the power goes from -137 to 114)
+        lsum = fmaf(((p0.x + p0.y) + (p1.x + p1.y)) * 0x1p-12f, ex2(-12.f - power), lsum);
 #pragma unroll
         for (int c = 0; c < VC / 2; ++c)
           v[c] = Pack2<__half>::pack(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1]));
@@ -814,9 +818,11 @@ __global__ void __launch_bounds__(Shape4<D, NG, std::is_same<T, __half>::value ?
         if (turn) poison |= __float_as_uint(other);
         else lsum += other;
       }
-      const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
-      const float lse2 =
-          lsum == 0.f ? -INFINITY : (mref > -INFINITY ? mref : 0.f) - kUp + log2f(lsum);
+      // (the sum from 2^-131 to 2^126: its reciprocal in float32's range)
+      const float up = lsum < 0x1p-60f ? 0x1p64f : 1.f, down = up * kSumDown;
+      const float inv = lsum == 0.f ? 0.f : 1.f / (lsum * up);
+      const float lse2 = lsum == 0.f ? -INFINITY
+                                     : (mref > -INFINITY ? mref : 0.f) - kUp + (log2f(lsum) + 24.f);
       const int tok = (row0 + row) / a.G, h = seg.g * a.G + (row0 + row - tok * a.G);
       const bool whole = seg.part < 0;
       const int64_t prow = (int64_t)seg.part * RT + row;
@@ -828,7 +834,7 @@ __global__ void __launch_bounds__(Shape4<D, NG, std::is_same<T, __half>::value ?
       auto final = [&](const uint32_t* v, int c0, int d) {
         const float x = __uint_as_float(v[(d & ~7) + place8(d & 7)]);
         const int group = (part2 * (D / 2) + c0 + d) / 32 / WG;
-        return poison >> group & 1u ? __int_as_float(0x7fffffff) : have ? x * inv : 0.f;
+        return poison >> group & 1u ? __int_as_float(0x7fffffff) : have ? x * down * inv : 0.f;
       };
       if (!whole || a.vec_out) {
         // each thread stages its row where the queries were, and the warp

@@ -103,7 +103,8 @@ def test_constant_values_come_back(cuda, dtype, value, dim, group, new):
 
 
 SPANS = [[0.0, 1e7], [0.0, 1e20], [1e7, 0.0], [1e-30, 1e20], [1e30, 1e-20, 1.0], [1e-35, 1e38],
-         [1e38, 1e-35], [1e38, 1e-6, 0.0, 1e-30], [1.0, 1e-12], [1e-20], [1e35], [1e37, 1e34]]
+         [1e38, 1e-35], [1e38, 1e-6, 0.0, 1e-30], [1.0, 1e-12], [1e-20], [1e35], [1e37, 1e34], [1e-31],
+         [1e-34], [1e-33, 1.0]]
 
 
 @pytest.mark.parametrize("sizes", SPANS)
