@@ -295,9 +295,11 @@ Plan4 plan4(const cs_kv4_attn_params& p) {
   const int64_t g = p.q_heads / p.pool.kv_heads;
   // Query rows of a KV head an average request has.  Up to 32 go to the kernel
   // for few, in tiles of 16 that each read the keys: 16 requests behind 4096 keys
-  // take 83 us with 24 or 28 rows and 98 in the wide kernel; 116 with 48 rows and
-  // 101 there, 201 with 96 and 111.  (The wide kernel in blocks of 128 rows was no
-  // faster with any of these, and slower with less work.)
+  // take 82 us with 24 or 28 rows and 98 in the wide kernel; 117 with 48 rows and
+  // 100 there, 205 with 96 and 102.  (The wide kernel in blocks of 128 rows was no
+  // faster with any of these, and slower with less work.)  One kernel takes the
+  // whole batch: 63 decodes of up to 16K keys beside a chunk of 512 tokens take 756
+  // us in the wide one, in two calls 174 and 86.
   const int64_t rows = p.requests > 0 ? p.tokens * g / p.requests : 0;
   plan.wide = rows > 32;
   plan.rows = plan.wide ? kWideRows : rows <= 8 ? 8 : 16;

@@ -18,10 +18,11 @@
 // either type keep every bit down to 2^-27 of that.
 //
 // HBM (136 to 160 bytes a key and head) is the floor; what bounds it is the issue
-// of about 250 instructions a unit, half of them on the ALU, at 0.55 a clock with
+// of about 255 instructions a unit, half of them on the ALU, at 0.55 a clock with
 // four warps a scheduler.  8 decodes of 65K keys (64/8 heads, groups of 128) take
-// 134 us, 4.2 TB/s; 32 of up to 16K (32/8, groups of 64) 85 us, 3.6 TB/s; four
-// drafts each (16 rows, groups of 32) 170 us.  The products are far too small for
+// 135 us, 4.2 TB/s; 32 of up to 16K (32/8, groups of 64) 87 us, 3.5 TB/s (85 with a
+// reference by the scales alone, which constant values overflow); four drafts each
+// (16 rows, groups of 32) 171 us.  The products are far too small for
 // tcgen05, whose operands would have to be written to shared memory
 // in 16 bits first, four times the bytes that come in -- at full bandwidth 87
 // bytes a clock and SM written and as many read again, of 128.  Here the codes

@@ -12,20 +12,22 @@
 // fp16 numbers with five bit operations (1024 + code has the code in its low
 // bits), four subtractions and four multiply-adds with scale and lowest value;
 // that is shared by all rows of the block, up to 256.  Operands are fp16
-// whatever the pool's type: queries are scaled by a power of two a row, keys
-// and values by one a step (of what the step's scales and lowest values can
-// reach), so bfloat16 pools of any size of numbers keep fp16's 11 bits, where
-// bfloat16 operands would keep 8.  P carries the values' power of two, the
-// rows' sums do not.  Float16 outputs would show the rounding of such keys and
-// values (0.00047 to 0.00054 off with both, 0.00033 with the values', 0.00021 of
-// which is the output's own), so those of float16 pools are two operands each,
-// scale (code - zero) and what is left.
+// whatever the pool's type: queries are scaled by a power of two a row, bfloat16
+// keys and values by one for 32 of a step (of what their scales and lowest values
+// can reach), so they keep fp16's 11 bits, where bfloat16 operands would keep 8:
+// queries up to 2^127, keys from 2^-126 and values from 2^-118 on, and down to
+// 2^-27 of the largest of the 32 (whether a row sees that one or not; 2^-38 of it
+// is 0).  P carries the values' power of two, the rows' sums do not.  Float16
+// outputs would show the rounding of such keys and values (0.00047 to 0.00054 off
+// with both, 0.00033 with the values', 0.00021 of which is the output's own), so
+// those of float16 pools are two operands each, scale (code - zero) and what is
+// left.
 //
-// Bound by the softmax warps: 2750 clocks a step of 64 keys of two row tiles, of
+// Bound by the softmax warps: 2600 clocks a step of 64 keys of two row tiles, of
 // which the exponentials take 1024.  8 chunks of 512 tokens over 4096 keys (32/8
-// heads of 128, bfloat16) take 400 us, 640 TFLOP/s (430 us sustained, under the
+// heads of 128, bfloat16) take 393 us, 655 TFLOP/s (406 us sustained, under the
 // power limit; 583 with codes fetched from global memory by the warps that decode
-// them), 13 questions of 3 to 150 tokens 69 us.
+// them), 490 in float16, 13 questions of 3 to 150 tokens 70 us.
 //
 // Pairs lie in the tiles as the codes come, elements (0, 4), (1, 5), (2, 6), (3,
 // 7) of eight: the queries are written in the same order, and the output's
@@ -82,7 +84,8 @@ struct Shape4 {
   // read; a segment said, and read
   static constexpr uint32_t bQ = 0, bFree = bQ + 8 * NT, bK = bFree + 8 * NT, bV = bK + 16,
                             bS = bV + 16, bP = bS + 16 * NT, bPV = bP + 16 * NT,
-                            bMax = bPV + 16 * NT, bR = bMax + 32 * NT, bRead = bR + 8 * RS, bSeg = bRead + 8 * RS,
+                            bMax = bPV + 16 * NT, bR = bMax + 32 * NT, bRead = bR + 8 * RS,
+                            bSeg = bRead + 8 * RS,
                             bSegRead = bSeg + 8 * kSegments, oTmem = bSegRead + 8 * kSegments,
                             oAbort = oTmem + 4, oWalked = oAbort + 4, oFlag = oWalked + 4,
                             oScale = oFlag + 4 * kInfo, oPower = oScale + 8 * kInfo,
